@@ -272,6 +272,22 @@ MOSS_API int moss_rmsnorm_bwd(const void* dy, const void* x, int x_dtype, int64_
                      const void* weight, int w_dtype, const float* rstd, void* dx, moss_stream_t stream);
 
 /*
+ * Rotary positions: q [batch, tokens, q_heads, head_dim] and k [.., k_heads, ..] (strides in elements,
+ * dense last dimension) into dense q_out / k_out. The first rotary_dim values of each head are
+ * pairs, (2 i, 2 i + 1) if interleaved, else (i, i + rotary_dim / 2); pair i of a token becomes
+ * (a cos - b sin, a sin + b cos) with row `place` of cos / sin, f32 [table_rows, rotary_dim / 2]; the other
+ * values are copied. place is the token's index, or positions[batch * position_stride + token] (device
+ * int64; position_stride 0 or tokens): a place outside the table gives NaN. inverse != 0 turns
+ * back, which is also the gradient. f32 arithmetic, rounded once. Reference: the position
+ * embedding of training/model.py:269-314.
+ */
+MOSS_API int moss_rotary(const void* q, int64_t q_batch_stride, int64_t q_token_stride, int64_t q_head_stride,
+                int64_t q_heads, const void* k, int64_t k_batch_stride, int64_t k_token_stride, int64_t k_head_stride,
+                int64_t k_heads, int dtype, int64_t batch, int64_t tokens, int64_t head_dim, const float* cos,
+                const float* sin, int64_t table_rows, int64_t rotary_dim, const int64_t* positions,
+                int64_t position_stride, int interleaved, int inverse, void* q_out, void* k_out, moss_stream_t stream);
+
+/*
  * Dense gather of a strided (non-overlapping) view into a contiguous buffer, and the
  * inverse scatter. Used by the activation offload to turn the payload views of
  * _offload_view (training/activation_offload.py:32-61) into one copy-engine transfer and
