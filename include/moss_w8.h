@@ -272,6 +272,32 @@ MOSS_API int moss_rmsnorm_bwd(const void* dy, const void* x, int x_dtype, int64_
                      const void* weight, int w_dtype, const float* rstd, void* dx, moss_stream_t stream);
 
 /*
+ * Block-scaled fp8 (e4m3) frozen linear: the 8-bit floating-point sibling of the int8 linear
+ * (training/quantization.py:68-131). Weight codes [n, k] with a row pitch ld (a multiple of 16 bytes, 16-byte
+ * aligned) and one f32 scale per 128 x 128 block, [ceil(n / 128), ceil(k / 128)]. Activations and gradients are
+ * quantised inside the call: per row and 128 reduction indices one scale, the least power of two that brings
+ * the block within +-448, codes rounded to nearest even.
+ *   fwd: y[m, n] = q(x)[m, k] dec(W)^T + bias      dx: dx[m, k] = q(dy)[m, n] dec(W)
+ * Sums and scales in f32, one rounding to the output type. `workspace`: at least
+ * moss_fp8_linear_workspace_bytes(m, output columns, reduction size) bytes, 256-byte aligned, free for reuse
+ * once the stream has passed the call. A row with an infinity or NaN in a block gives NaN in that row.
+ */
+MOSS_API int moss_fp8_linear_workspace_bytes(int64_t m, int64_t n_out, int64_t k_red, size_t* bytes);
+MOSS_API int moss_fp8_linear_fwd(const void* x, int x_dtype, int64_t m, int64_t k, const uint8_t* codes, int64_t ld,
+                        const float* scale, int64_t n, const void* bias, int bias_dtype, void* y, int y_dtype,
+                        void* workspace, size_t workspace_bytes, int* status, moss_stream_t stream);
+MOSS_API int moss_fp8_linear_dx(const void* dy, int dy_dtype, int64_t m, int64_t n, const uint8_t* codes, int64_t ld,
+                       const float* scale, int64_t k, void* dx, int dx_dtype, void* workspace, size_t workspace_bytes,
+                       int* status, moss_stream_t stream);
+/* The row quantiser on its own: codes [m, ceil(k / 128) * 128] (zero past k), scale [ceil(k / 128)][row_pitch]. */
+MOSS_API int moss_fp8_quantize_rows(const void* x, int x_dtype, int64_t m, int64_t k, uint8_t* codes, float* scale,
+                           int64_t row_pitch, moss_stream_t stream);
+/* The weight quantiser: scale max|w| / 448 per block, codes [n, k] with pitch ld = k rounded up to 16.
+ * Non-finite weights set MOSS_STATUS_NONFINITE_WEIGHT in *status. */
+MOSS_API int moss_fp8_quantize_weight(const void* w, int w_dtype, int64_t n, int64_t k, uint8_t* codes, int64_t ld,
+                             float* scale, int* status, moss_stream_t stream);
+
+/*
  * Rotary positions: q [batch, tokens, q_heads, head_dim] and k [.., k_heads, ..] (strides in elements,
  * dense last dimension) into dense q_out / k_out. The first rotary_dim values of each head are
  * pairs, (2 i, 2 i + 1) if interleaved, else (i, i + rotary_dim / 2); pair i of a token becomes

@@ -68,6 +68,12 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "moss_segment_gate_bwd": (_i32, [_vp, _vp, _i32, _i64, _i64, _vp, _i32, _i64, _vp, _i64, _vp, _vp, _vp]),
     "moss_rmsnorm_fwd": (_i32, [_vp, _i32, _i64, _i64, _vp, _i32, _f32, _vp, _vp, _vp]),
     "moss_rmsnorm_bwd": (_i32, [_vp, _vp, _i32, _i64, _i64, _vp, _i32, _vp, _vp, _vp]),
+    "moss_fp8_linear_workspace_bytes": (_i32, [_i64, _i64, _i64, ctypes.POINTER(_sz)]),
+    "moss_fp8_linear_fwd": (
+        _i32, [_vp, _i32, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _i32, _vp, _i32, _vp, _sz, _vp, _vp]),
+    "moss_fp8_linear_dx": (_i32, [_vp, _i32, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _i32, _vp, _sz, _vp, _vp]),
+    "moss_fp8_quantize_rows": (_i32, [_vp, _i32, _i64, _i64, _vp, _vp, _i64, _vp]),
+    "moss_fp8_quantize_weight": (_i32, [_vp, _i32, _i64, _i64, _vp, _i64, _vp, _vp, _vp]),
     "moss_rotary": (
         _i32,
         [_vp, _i64, _i64, _i64, _i64, _vp, _i64, _i64, _i64, _i64, _i32, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _vp,

@@ -37,6 +37,15 @@ inline int check_cuda(cudaError_t e, const char* what) {
   return fail(MOSS_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
 }
 
+// Makes the current device's context current on this thread, as a kernel launch would. A thread
+// that has made no CUDA call yet (an autograd worker's first backward) has none, and the
+// driver's tensor-map encoder refuses to work without one.
+inline int bind_context() {
+  int device = 0;
+  const int rc = check_cuda(cudaGetDevice(&device), "cudaGetDevice");
+  return rc != MOSS_OK ? rc : check_cuda(cudaSetDevice(device), "cudaSetDevice");
+}
+
 inline int clear_ok() {
   last_error_slot().clear();
   return MOSS_OK;

@@ -1,0 +1,411 @@
+// Block-scaled fp8 GEMM with the rows (tokens) in the accumulator's lanes, for sm_100a.
+//
+// Two shapes of one kernel:
+//   * a CTA pair (cta_group::2) on 256 x 256 output tiles, for problems that fill the GPU with
+//     them: every operand byte in shared memory feeds twice the products of a 128 x 128 tile;
+//   * one CTA on 128 x 128 tiles, for those that do not.
+// Warp 0 streams 128-wide reduction blocks by TMA (both operands straight from their 8-bit
+// storage: no decode), warp 1 issues four 32-wide tcgen05.mma per block into one of two
+// TMEM buffers, and eight warps take each finished block out of TMEM, multiply it by its two
+// scales and add it into f32 registers while the tensor cores run the next block. The
+// grad-input reads the same [out, in] weight codes: there the tile is MN-major.
+//
+// What bounds it: a 256 x 256 x 128 block is 512 cycles of the pair's tensor cores. Taking its
+// 128 x 256 half out of each CTA's TMEM costs 4 x 64 packed multiply-adds a thread pair of
+// columns (f32x2) and the TMEM reads, about half of that, on the other pipes.
+#include <algorithm>
+#include <cstring>
+#include <mutex>
+
+#include "dequant.cuh"
+#include "fp8_args.cuh"
+
+namespace moss {
+namespace fp8 {
+namespace {
+
+constexpr int kHalf = 128;  // rows of A and columns (or half of the pair's columns) of W per CTA
+constexpr int kEpiWarp0 = 2;
+constexpr int kEpiWarps = 8;
+constexpr int kThreads = (kEpiWarp0 + kEpiWarps) * 32;
+constexpr int kStages = 6;
+constexpr uint32_t kTileBytes = kHalf * kBlock;      // 16 KB: 128 rows of 128 bytes
+constexpr uint32_t kStageBytes = 2 * kTileBytes;     // A rows and W columns
+constexpr uint32_t kDataBytes = kStages * kStageBytes;
+constexpr uint32_t kSmemBytes = kDataBytes + 1024 + 512;
+// The final wait for the peer outlasts every other bounded wait of the pair (each gives up within
+// kWaitBudgetCycles, the drain of the ring within kStages more).
+constexpr long long kExitBudgetCycles = (kStages + 4) * kWaitBudgetCycles;
+static_assert(kSmemBytes <= 227 * 1024, "rings exceed the shared memory a CTA may use");
+
+struct Barriers {
+  uint64_t full[kStages];   // leader: both CTAs' operands of a stage landed
+  uint64_t empty[kStages];  // local: stage free (MMA commit)
+  uint64_t acc_full[2];     // local: block product ready (MMA commit)
+  uint64_t acc_empty[2];    // leader: block product taken by every epilogue warp
+  uint64_t drain;           // leader: all MMAs retired
+  uint64_t exit_bar;        // local: peer finished
+  uint32_t tmem_base;
+  int abort_flag;
+};
+static_assert(sizeof(Barriers) <= 512, "barrier block too large");
+
+__device__ __forceinline__ void fma2(uint64_t& acc, uint32_t lo, uint32_t hi, uint64_t s) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(lo), "r"(hi));
+  asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc) : "l"(d), "l"(s));
+}
+
+// Bias and the rounded store of 32 consecutive outputs of one row.
+__device__ __forceinline__ void store32(const Args& args, float (&v)[32], int row, int col0, bool vec_ok) {
+  if (args.bias != nullptr) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      if (col0 + j < args.Nc) v[j] += load_as_float(args.bias, args.bias_kind, col0 + j);
+  }
+  const int64_t off = static_cast<int64_t>(row) * args.Nc + col0;
+  if (vec_ok && col0 + 32 <= args.Nc) {
+    uint32_t p0[8], p1[8];
+    if (args.out_kind == kBF16) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        p0[j] = gemm::pack2_kind<kBF16>(v[2 * j], v[2 * j + 1]);
+        p1[j] = gemm::pack2_kind<kBF16>(v[16 + 2 * j], v[16 + 2 * j + 1]);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        p0[j] = gemm::pack2_kind<kF16>(v[2 * j], v[2 * j + 1]);
+        p1[j] = gemm::pack2_kind<kF16>(v[16 + 2 * j], v[16 + 2 * j + 1]);
+      }
+    }
+    uint16_t* dst = static_cast<uint16_t*>(args.out) + off;
+    gemm::stg256(dst, p0);
+    gemm::stg256(dst + 16, p1);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      if (col0 + j < args.Nc) store_from_float(args.out, args.out_kind, off + j, v[j]);
+  }
+}
+
+template <bool kDX, int kCtas>
+__global__ void __launch_bounds__(kThreads, 1)
+    fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_w, const Args args) {
+  constexpr int kTileM = kHalf * kCtas;
+  constexpr int kTileN = kHalf * kCtas;
+  constexpr int kCols = kTileN / 2;  // accumulator columns of one epilogue thread
+  constexpr uint32_t kTmemCols = 2 * kTileN;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw_base = smem_u32(smem_raw);
+  const uint32_t base = (raw_base + 1023u) & ~1023u;
+  Barriers* bars = reinterpret_cast<Barriers*>(smem_raw + (base - raw_base) + kDataBytes);
+  auto bar = [&](uint64_t& b) { return smem_u32(&b); };
+  volatile int* abort_flag = &bars->abort_flag;
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const uint32_t rank = kCtas == 2 ? cluster_ctarank() : 0;
+  const bool leader = rank == 0;
+  const int first_unit = blockIdx.x / kCtas;
+  const int unit_step = gridDim.x / kCtas;
+  const int num_units = args.tiles_m * args.tiles_n * args.splits;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(bar(bars->full[s]), 1);
+      mbar_init(bar(bars->empty[s]), 1);
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(bar(bars->acc_full[s]), 1);
+      mbar_init(bar(bars->acc_empty[s]), kCtas * kEpiWarps);
+    }
+    mbar_init(bar(bars->drain), 1);
+    mbar_init(bar(bars->exit_bar), 1);
+    bars->abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    if constexpr (kCtas == 2) {
+      tmem_alloc_pair(smem_u32(&bars->tmem_base), kTmemCols);
+      tmem_relinquish_pair();
+    } else {
+      tmem_alloc(smem_u32(&bars->tmem_base), kTmemCols);
+      tmem_relinquish();
+    }
+  }
+  tc_fence_before();
+  if constexpr (kCtas == 2)  // both CTAs' barriers exist before any arrival from the peer
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  else
+    __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = bars->tmem_base;
+
+  if (warp == 0) {
+    // ---------------------------------------------------------------- producer (every CTA)
+    if (lane == 0) {
+      tma_prefetch_desc(&tm_a);
+      tma_prefetch_desc(&tm_w);
+    }
+    int stage = 0;
+    uint32_t phase = 0, used = 0, last_phase = 0;
+    bool ok = true;
+    for (int u = first_unit; u < num_units && ok; u += unit_step) {
+      const int tile = u / args.splits, split = u - tile * args.splits;
+      int m_blk, n_blk;
+      gemm::tile_coords(tile, args.tiles_m, args.tiles_n, m_blk, n_blk, args.group_m);
+      const int m0 = m_blk * kTileM + static_cast<int>(rank) * kHalf;
+      const int n0 = n_blk * kTileN + static_cast<int>(rank) * kHalf;
+      const int kb1 = min(args.kb, (split + 1) * args.kb_per_split);
+      for (int kb = split * args.kb_per_split; kb < kb1; ++kb) {
+        if (!mbar_wait_cluster(bar(bars->empty[stage]), phase ^ 1u, abort_flag, args.status,
+                               MOSS_STATUS_TIMEOUT_LOAD)) {
+          ok = false;
+          break;
+        }
+        if (lane == 0) {
+          const uint32_t a_dst = base + stage * kStageBytes;
+          const int wx = kDX ? n0 : kb * kBlock, wy = kDX ? kb * kBlock : n0;
+          if constexpr (kCtas == 2) {
+            // the leader's barrier counts both CTAs' bytes; the peer's copies signal it too
+            if (leader) mbar_arrive_expect_tx(bar(bars->full[stage]), kCtas * kStageBytes);
+            const uint32_t fb = mapa_shared(bar(bars->full[stage]), 0);
+            tma_load_2d_pair(a_dst, &tm_a, fb, kb * kBlock, m0);
+            tma_load_2d_pair(a_dst + kTileBytes, &tm_w, fb, wx, wy);
+          } else {
+            mbar_arrive_expect_tx(bar(bars->full[stage]), kStageBytes);
+            tma_load_2d(a_dst, &tm_a, bar(bars->full[stage]), kb * kBlock, m0);
+            tma_load_2d(a_dst + kTileBytes, &tm_w, bar(bars->full[stage]), wx, wy);
+          }
+          used |= 1u << stage;
+          last_phase = (last_phase & ~(1u << stage)) | (phase << stage);
+        }
+        __syncwarp();
+        if (++stage == kStages) { stage = 0; phase ^= 1u; }
+      }
+    }
+    // The copies land before the CTA may leave. The leader sees the peer's too, and the peer
+    // leaves only after the leader's exit arrival.
+    if (lane == 0 && leader) {
+      for (int s = 0; s < kStages; ++s) {
+        if (!((used >> s) & 1u)) continue;
+        const long long start = clock64();
+        while (!mbar_try_wait(bar(bars->full[s]), (last_phase >> s) & 1u)) {
+          if (clock64() - start > kWaitBudgetCycles) {
+            report_status(args.status, MOSS_STATUS_TIMEOUT_DRAIN);
+            break;
+          }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ---------------------------------------------------------------- MMA issuer (leader)
+    if (leader) {
+      constexpr uint32_t idesc = idesc_e4m3(false, kDX, kTileM, kTileN);
+      int stage = 0, it = 0;
+      uint32_t phase = 0;
+      bool ok = true, issued = false;
+      for (int u = first_unit; u < num_units && ok; u += unit_step) {
+        const int split = u % args.splits;
+        const int kb1 = min(args.kb, (split + 1) * args.kb_per_split);
+        for (int kb = split * args.kb_per_split; kb < kb1; ++kb, ++it) {
+          const int acc = it & 1;
+          if (!mbar_wait_cluster(bar(bars->acc_empty[acc]), ((it >> 1) & 1) ^ 1u, abort_flag, args.status,
+                                 MOSS_STATUS_TIMEOUT_MMA) ||
+              !mbar_wait_cluster(bar(bars->full[stage]), phase, abort_flag, args.status, MOSS_STATUS_TIMEOUT_MMA)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          if (lane == 0) {
+            const uint32_t a_tile = base + stage * kStageBytes;
+            const uint32_t d = tmem_base + static_cast<uint32_t>(acc * kTileN);
+#pragma unroll
+            for (int kk = 0; kk < kBlock / 32; ++kk) {
+              const uint64_t ad = step_desc(a_tile, kk, false);
+              const uint64_t wd = step_desc(a_tile + kTileBytes, kk, kDX);
+              if constexpr (kCtas == 2)
+                umma_f8_pair(d, ad, wd, idesc, kk > 0);
+              else
+                umma_f8(d, ad, wd, idesc, kk > 0);
+            }
+            if constexpr (kCtas == 2) {
+              umma_commit_pair_mc(bar(bars->empty[stage]), 0x3);
+              umma_commit_pair_mc(bar(bars->acc_full[acc]), 0x3);
+            } else {
+              umma_commit(bar(bars->empty[stage]));
+              umma_commit(bar(bars->acc_full[acc]));
+            }
+            issued = true;
+          }
+          __syncwarp();
+          if (++stage == kStages) { stage = 0; phase ^= 1u; }
+        }
+      }
+      if (lane == 0 && issued) {
+        if constexpr (kCtas == 2)
+          umma_commit_pair(bar(bars->drain));
+        else
+          umma_commit(bar(bars->drain));
+        const long long start = clock64();
+        while (!mbar_try_wait(bar(bars->drain), 0)) {
+          if (clock64() - start > kWaitBudgetCycles) {
+            report_status(args.status, MOSS_STATUS_TIMEOUT_DRAIN);
+            break;
+          }
+        }
+      }
+      __syncwarp();
+    }
+  } else {
+    // ---------------------------------------------------------------- epilogue (every CTA)
+    const int q = warp & 3;
+    const int half = (warp - kEpiWarp0) >> 2;
+    const uint32_t lane_addr = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(half * kCols);
+    const bool vec_ok = args.out_kind != kF32 && (args.Nc & 15) == 0 && (reinterpret_cast<uintptr_t>(args.out) & 31) == 0;
+    int it = 0;
+    bool ok = true;
+    for (int u = first_unit; u < num_units && ok; u += unit_step) {
+      const int tile = u / args.splits, split = u - tile * args.splits;
+      int m_blk, n_blk;
+      gemm::tile_coords(tile, args.tiles_m, args.tiles_n, m_blk, n_blk, args.group_m);
+      const int row = m_blk * kTileM + static_cast<int>(rank) * kHalf + q * 32 + lane;
+      const int col0 = n_blk * kTileN + half * kCols;
+      const float* row_scale = args.row_scale + min(row, args.M - 1);
+      const float* w_scale = args.w_scale + static_cast<int64_t>(min(col0 / kBlock, args.col_blocks - 1)) * args.ws_col;
+      const int kb0 = split * args.kb_per_split, kb1 = min(args.kb, kb0 + args.kb_per_split);
+      uint64_t sum[kCols / 2];
+#pragma unroll
+      for (int j = 0; j < kCols / 2; ++j) sum[j] = 0;
+      float next = __ldg(row_scale + kb0 * args.row_pitch) * __ldg(w_scale + static_cast<int64_t>(kb0) * args.ws_red);
+      for (int kb = kb0; kb < kb1; ++kb, ++it) {
+        const uint32_t s32 = __float_as_uint(next);
+        const uint64_t s = (static_cast<uint64_t>(s32) << 32) | s32;
+        if (kb + 1 < kb1)
+          next = __ldg(row_scale + (kb + 1) * args.row_pitch) * __ldg(w_scale + static_cast<int64_t>(kb + 1) * args.ws_red);
+        const int acc = it & 1;
+        if (!mbar_wait_cluster(bar(bars->acc_full[acc]), (it >> 1) & 1, abort_flag, args.status,
+                               MOSS_STATUS_TIMEOUT_EPILOGUE)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+#pragma unroll
+        for (int c = 0; c < kCols / 32; ++c) {
+          uint32_t r[32];
+          tmem_ld_32x32b_x32(lane_addr + static_cast<uint32_t>(acc * kTileN + c * 32), r);
+          tmem_wait_ld();
+          if (c == kCols / 32 - 1) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+              const uint32_t eb = bar(bars->acc_empty[acc]);
+              if (kCtas == 1 || leader)
+                mbar_arrive(eb);
+              else
+                mbar_arrive_cluster(mapa_shared(eb, 0));
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < 16; ++j) fma2(sum[c * 16 + j], r[2 * j], r[2 * j + 1], s);
+        }
+      }
+      if (!ok) break;
+      if (row >= args.M) continue;
+#pragma unroll
+      for (int c = 0; c < kCols / 32; ++c) {
+        const int col = col0 + c * 32;
+        if (col >= args.Nc) break;
+        float v[32];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          v[2 * j] = __uint_as_float(static_cast<uint32_t>(sum[c * 16 + j]));
+          v[2 * j + 1] = __uint_as_float(static_cast<uint32_t>(sum[c * 16 + j] >> 32));
+        }
+        if (args.splits > 1) {
+          float* dst = args.partial + (static_cast<int64_t>(split) * args.M + row) * args.Nc + col;
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            if (col + j < args.Nc) dst[j] = v[j];
+        } else {
+          store32(args, v, row, col, vec_ok);
+        }
+      }
+    }
+  }
+
+  // Leave together: the leader's MMAs read the peer's shared memory and write its TMEM, and the
+  // peer arrives on the leader's barriers, so neither CTA exits or frees TMEM first.
+  tc_fence_before();
+  __syncthreads();
+  if constexpr (kCtas == 2) {
+    if (threadIdx.x == 0) {
+      if (*abort_flag) st_shared_cluster_u32(mapa_shared(smem_u32(&bars->abort_flag), rank ^ 1u), 1u);
+      mbar_arrive_cluster(mapa_shared(bar(bars->exit_bar), rank ^ 1u));
+      const long long start = clock64();
+      while (!mbar_try_wait_cluster(bar(bars->exit_bar), 0)) {
+        if (clock64() - start > kExitBudgetCycles) {
+          report_status(args.status, MOSS_STATUS_TIMEOUT_DRAIN);
+          break;
+        }
+      }
+    }
+    __syncthreads();
+  }
+  if (warp == 1) {
+    tc_fence_after();
+    if constexpr (kCtas == 2)
+      tmem_dealloc_pair(tmem_base, kTmemCols);
+    else
+      tmem_dealloc(tmem_base, kTmemCols);
+  }
+}
+
+template <bool kDX, int kCtas>
+int launch_typed(const CUtensorMap& ta, const CUtensorMap& tw, const Args& a, cudaStream_t stream) {
+  auto kern = fp8_gemm_kernel<kDX, kCtas>;
+  static std::once_flag once;
+  static cudaError_t attr_err = cudaSuccess;
+  static int max_groups = 0;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = kCtas;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = kSmemBytes;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  std::call_once(once, [&] {
+    attr_err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+    if (attr_err != cudaSuccess) return;
+    max_groups = sm_count() / kCtas;
+    if (kCtas > 1) {
+      cfg.gridDim = dim3(kCtas * max_groups);
+      int clusters = 0;
+      if (cudaOccupancyMaxActiveClusters(&clusters, kern, &cfg) == cudaSuccess && clusters > 0)
+        max_groups = clusters;
+      else
+        cudaGetLastError();
+    }
+  });
+  MOSS_CUDA_TRY(attr_err);
+  const int64_t units = static_cast<int64_t>(a.tiles_m) * a.tiles_n * a.splits;
+  cfg.gridDim = dim3(static_cast<unsigned>(kCtas * std::max<int64_t>(1, std::min<int64_t>(units, max_groups))));
+  cfg.stream = stream;
+  return check_cuda(cudaLaunchKernelEx(&cfg, kern, ta, tw, a), "fp8_gemm_kernel");
+}
+
+}  // namespace
+
+int launch_gemm(bool dx, const Plan& plan, const CUtensorMap& ta, const CUtensorMap& tw, const Args& a,
+                cudaStream_t stream) {
+  if (plan.kind == Plan::kPair)
+    return dx ? launch_typed<true, 2>(ta, tw, a, stream) : launch_typed<false, 2>(ta, tw, a, stream);
+  return dx ? launch_typed<true, 1>(ta, tw, a, stream) : launch_typed<false, 1>(ta, tw, a, stream);
+}
+
+}  // namespace fp8
+}  // namespace moss

@@ -1,0 +1,216 @@
+// Block quantisers of the fp8 linear.
+//
+// Rows (activations, gradients): one scale for each row and 128 columns, the least power of two
+// 2^p with max|x| <= 448 * 2^p. Dividing by a power of two is exact, so a code is the one correct
+// rounding of x / 2^p (ties to even) whichever way the division is done, and a block keeps the
+// format's full relative precision: fp8 is a floating-point type, so only the range matters.
+// Weights: one f32 scale max|w| / 448 for each 128 x 128 block, as fp8 checkpoints store them.
+//
+// Both are bound by HBM: 2 bytes read and 1 written per value. A half-warp holds one row's 128
+// columns (16 bytes a lane), so the maximum is four shuffles away and the values are read once.
+#include <cuda_fp8.h>
+
+#include <algorithm>
+
+#include "fp8_args.cuh"
+
+namespace moss {
+namespace fp8 {
+
+constexpr int kThreads = 256;
+constexpr int kRowsPerCta = kThreads / 16;
+constexpr int kBatch = 4;  // column blocks per half-warp: independent loads in flight
+
+// 8 consecutive values of a row from column c0, zero past k.
+template <int kKind>
+__device__ __forceinline__ void load8(const void* x, int64_t row, int64_t k, int64_t c0, bool wide, float (&v)[8]) {
+  const int64_t at = row * k + c0;
+  if (wide && c0 + 8 <= k) {
+    if constexpr (kKind == kF32) {
+      const float4 a = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(x) + at));
+      const float4 b = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(x) + at) + 1);
+      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+      v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    } else {
+      const uint4 a = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(x) + at));
+      const uint32_t p[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (kKind == kBF16) {
+          v[2 * i] = __uint_as_float(p[i] << 16);
+          v[2 * i + 1] = __uint_as_float(p[i] & 0xffff0000u);
+        } else {
+          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&p[i]));
+          v[2 * i] = f.x;
+          v[2 * i + 1] = f.y;
+        }
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = c0 + i < k ? load_as_float(x, kKind, at + i) : 0.0f;
+  }
+}
+
+// fmaxf drops NaN; a block that holds one has to show it.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// Exponent p of the row scale: the least with amax <= 448 * 2^p = 1.75 * 2^(p + 8).
+__device__ __forceinline__ int scale_exponent(float amax) {
+  const uint32_t bits = __float_as_uint(amax);
+  return static_cast<int>(bits >> 23) - 127 - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
+}
+__device__ __forceinline__ float pow2(int p) { return __uint_as_float(static_cast<uint32_t>(p + 127) << 23); }
+
+__device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d) {
+  const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+  const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
+  return lo | (hi << 16);
+}
+
+template <int kKind>
+__global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const void* __restrict__ x, int64_t m, int64_t k, int kb,
+                                                                 bool wide, uint8_t* __restrict__ codes,
+                                                                 float* __restrict__ scale, int64_t row_pitch) {
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * kRowsPerCta + (threadIdx.x >> 4);
+  const int sub = threadIdx.x & 15;
+  const bool live = row < m;
+  const int first = static_cast<int>(blockIdx.y) * kBatch;
+  float v[kBatch][8];
+#pragma unroll
+  for (int i = 0; i < kBatch; ++i) {
+    if (live && first + i < kb) {
+      load8<kKind>(x, row, k, static_cast<int64_t>(first + i) * kBlock + sub * 8, wide, v[i]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[i][j] = 0.0f;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kBatch; ++i) {
+    float amax = kAmaxFloor;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) amax = max_nan(amax, fabsf(v[i][j]));
+#pragma unroll
+    for (int d = 8; d > 0; d >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, d));
+    if (!live || first + i >= kb) continue;
+    // a block with an infinity or a NaN has no scale: NaN, and so has every product with it
+    const bool finite = amax < __uint_as_float(0x7f800000u);
+    const int p = finite ? scale_exponent(amax) : 0;
+    const float inv = pow2(-p);
+    uint2 q;
+    q.x = codes4(v[i][0] * inv, v[i][1] * inv, v[i][2] * inv, v[i][3] * inv);
+    q.y = codes4(v[i][4] * inv, v[i][5] * inv, v[i][6] * inv, v[i][7] * inv);
+    *reinterpret_cast<uint2*>(codes + (row * kb + first + i) * kBlock + sub * 8) = q;
+    if (sub == 0) scale[(first + i) * row_pitch + row] = finite ? pow2(p) : __uint_as_float(0x7fffffffu);
+  }
+}
+
+int launch_quantize_rows(const void* x, int dtype, int64_t m, int64_t k, uint8_t* codes, float* scale,
+                         int64_t row_pitch, cudaStream_t stream) {
+  const int kb = static_cast<int>((k + kBlock - 1) / kBlock);
+  const int esize = dtype_size(dtype);
+  const bool wide = reinterpret_cast<uintptr_t>(x) % 16 == 0 && (k * esize) % 16 == 0;
+  const dim3 grid(static_cast<unsigned>((m + kRowsPerCta - 1) / kRowsPerCta), (kb + kBatch - 1) / kBatch);
+  if (dtype == kBF16)
+    quantize_rows_kernel<kBF16><<<grid, kThreads, 0, stream>>>(x, m, k, kb, wide, codes, scale, row_pitch);
+  else if (dtype == kF16)
+    quantize_rows_kernel<kF16><<<grid, kThreads, 0, stream>>>(x, m, k, kb, wide, codes, scale, row_pitch);
+  else
+    quantize_rows_kernel<kF32><<<grid, kThreads, 0, stream>>>(x, m, k, kb, wide, codes, scale, row_pitch);
+  return check_cuda(cudaGetLastError(), "quantize_rows_kernel");
+}
+
+// One CTA per 128 x 128 weight block: 16 rows at a time, 8 sweeps held in registers.
+template <int kKind>
+__global__ void __launch_bounds__(kThreads) quantize_weight_kernel(const void* __restrict__ w, int64_t n, int64_t k,
+                                                                   bool wide, uint8_t* __restrict__ codes, int64_t ld,
+                                                                   float* __restrict__ scale, int* status) {
+  constexpr int kSweeps = kBlock / kRowsPerCta;
+  __shared__ float warp_max[kThreads / 32];
+  const int64_t row0 = static_cast<int64_t>(blockIdx.y) * kBlock + (threadIdx.x >> 4);
+  const int64_t c0 = static_cast<int64_t>(blockIdx.x) * kBlock + (threadIdx.x & 15) * 8;
+  float v[kSweeps][8];
+  float amax = kAmaxFloor;
+#pragma unroll
+  for (int i = 0; i < kSweeps; ++i) {
+    const int64_t row = row0 + i * kRowsPerCta;
+    if (row < n) {
+      load8<kKind>(w, row, k, c0, wide, v[i]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[i][j] = 0.0f;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) amax = max_nan(amax, fabsf(v[i][j]));
+  }
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, d));
+  if ((threadIdx.x & 31) == 0) warp_max[threadIdx.x >> 5] = amax;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kThreads / 32; ++i) amax = max_nan(amax, warp_max[i]);
+  const float s = __fdiv_rn(amax, 448.0f);
+  if (threadIdx.x == 0) {
+    scale[static_cast<int64_t>(blockIdx.y) * gridDim.x + blockIdx.x] = s;
+    if (!(amax < __uint_as_float(0x7f800000u))) report_status(status, MOSS_STATUS_NONFINITE_WEIGHT);
+  }
+#pragma unroll
+  for (int i = 0; i < kSweeps; ++i) {
+    const int64_t row = row0 + i * kRowsPerCta;
+    if (row >= n) continue;
+    uint32_t q[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      q[h] = codes4(__fdiv_rn(v[i][4 * h], s), __fdiv_rn(v[i][4 * h + 1], s), __fdiv_rn(v[i][4 * h + 2], s),
+                    __fdiv_rn(v[i][4 * h + 3], s));
+    // rows of codes are a multiple of 16 bytes long: whole words up to that, zero past k
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      if (c0 + 4 * h < ld) *reinterpret_cast<uint32_t*>(codes + row * ld + c0 + 4 * h) = q[h];
+  }
+}
+
+}  // namespace fp8
+}  // namespace moss
+
+using namespace moss;
+
+extern "C" int moss_fp8_quantize_rows(const void* x, int x_dtype, int64_t m, int64_t k, uint8_t* codes, float* scale,
+                                      int64_t row_pitch, moss_stream_t stream) {
+  if (!is_float_kind(x_dtype)) return fail(MOSS_ERR_UNSUPPORTED, "unsupported dtype code %d", x_dtype);
+  if (m < 0 || k < 0 || m > INT32_MAX || k > (1 << 22)) return fail(MOSS_ERR_INVALID_ARGUMENT, "bad quantiser shape");
+  if (row_pitch < m) return fail(MOSS_ERR_INVALID_ARGUMENT, "row_pitch is less than the row count");
+  if (m == 0 || k == 0) return clear_ok();
+  if (x == nullptr || codes == nullptr || scale == nullptr) return fail(MOSS_ERR_INVALID_ARGUMENT, "null pointer");
+  if (reinterpret_cast<uintptr_t>(codes) % 16 != 0) return fail(MOSS_ERR_INVALID_ARGUMENT, "codes must be 16-byte aligned");
+  const int rc = fp8::launch_quantize_rows(x, x_dtype, m, k, codes, scale, row_pitch, reinterpret_cast<cudaStream_t>(stream));
+  return rc == MOSS_OK ? clear_ok() : rc;
+}
+
+extern "C" int moss_fp8_quantize_weight(const void* w, int w_dtype, int64_t n, int64_t k, uint8_t* codes, int64_t ld,
+                                        float* scale, int* status, moss_stream_t stream) {
+  if (!is_float_kind(w_dtype)) return fail(MOSS_ERR_UNSUPPORTED, "unsupported dtype code %d", w_dtype);
+  if (n < 0 || k < 0 || n > (1 << 22) || k > INT32_MAX - 256) return fail(MOSS_ERR_INVALID_ARGUMENT, "bad quantiser shape");
+  if (ld % 16 != 0 || ld < k || ld >= k + 16)
+    return fail(MOSS_ERR_INVALID_ARGUMENT, "the code pitch must be k rounded up to a multiple of 16");
+  if (n == 0 || k == 0) return clear_ok();
+  if (w == nullptr || codes == nullptr || scale == nullptr) return fail(MOSS_ERR_INVALID_ARGUMENT, "null pointer");
+  if (reinterpret_cast<uintptr_t>(codes) % 16 != 0) return fail(MOSS_ERR_INVALID_ARGUMENT, "codes must be 16-byte aligned");
+  const bool wide = reinterpret_cast<uintptr_t>(w) % 16 == 0 && (k * dtype_size(w_dtype)) % 16 == 0;
+  const dim3 grid(static_cast<unsigned>((k + fp8::kBlock - 1) / fp8::kBlock),
+                  static_cast<unsigned>((n + fp8::kBlock - 1) / fp8::kBlock));
+  const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  if (w_dtype == MOSS_DTYPE_BF16)
+    fp8::quantize_weight_kernel<kBF16><<<grid, fp8::kThreads, 0, s>>>(w, n, k, wide, codes, ld, scale, status);
+  else if (w_dtype == MOSS_DTYPE_F16)
+    fp8::quantize_weight_kernel<kF16><<<grid, fp8::kThreads, 0, s>>>(w, n, k, wide, codes, ld, scale, status);
+  else
+    fp8::quantize_weight_kernel<kF32><<<grid, fp8::kThreads, 0, s>>>(w, n, k, wide, codes, ld, scale, status);
+  MOSS_CUDA_TRY(cudaGetLastError());
+  return clear_ok();
+}
