@@ -298,6 +298,20 @@ MOSS_API int moss_fp8_quantize_weight(const void* w, int w_dtype, int64_t n, int
                              float* scale, int* status, moss_stream_t stream);
 
 /*
+ * Orthogonalised update of `batch` dense matrices g [batch, rows, cols]: X = g / max(|g|, eps) (Frobenius norm
+ * of each matrix), then `steps` of A = X X^T, X <- a X + (b A + c A A) X on the shorter side, with
+ * coefficients (host) a, b, c of each step one after another; out (bf16, same shape) is the last X. The
+ * reference trains with AdamW and Adafactor (training/optimizers.py); this is the matrix step of an
+ * orthogonalising optimiser for its fully trained projections. Refused (MOSS_ERR_INVALID_ARGUMENT): more than
+ * 16 steps, or coefficients that can carry a singular value of [0, 1] past 32. `workspace`: at least
+ * moss_orthogonalize_workspace_bytes(batch, rows, cols) bytes, 256-byte aligned.
+ */
+MOSS_API int moss_orthogonalize_workspace_bytes(int64_t batch, int64_t rows, int64_t cols, size_t* bytes);
+MOSS_API int moss_orthogonalize(const void* g, int g_dtype, int64_t batch, int64_t rows, int64_t cols, int steps,
+                       const float* coefficients, float eps, void* out, void* workspace, size_t workspace_bytes,
+                       int* status, moss_stream_t stream);
+
+/*
  * Rotary positions: q [batch, tokens, q_heads, head_dim] and k [.., k_heads, ..] (strides in elements,
  * dense last dimension) into dense q_out / k_out. The first rotary_dim values of each head are
  * pairs, (2 i, 2 i + 1) if interleaved, else (i, i + rotary_dim / 2); pair i of a token becomes

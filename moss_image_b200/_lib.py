@@ -74,6 +74,9 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "moss_fp8_linear_dx": (_i32, [_vp, _i32, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _i32, _vp, _sz, _vp, _vp]),
     "moss_fp8_quantize_rows": (_i32, [_vp, _i32, _i64, _i64, _vp, _vp, _i64, _vp]),
     "moss_fp8_quantize_weight": (_i32, [_vp, _i32, _i64, _i64, _vp, _i64, _vp, _vp, _vp]),
+    "moss_orthogonalize_workspace_bytes": (_i32, [_i64, _i64, _i64, ctypes.POINTER(_sz)]),
+    "moss_orthogonalize": (
+        _i32, [_vp, _i32, _i64, _i64, _i64, _i32, ctypes.POINTER(_f32), _f32, _vp, _vp, _sz, _vp, _vp]),
     "moss_rotary": (
         _i32,
         [_vp, _i64, _i64, _i64, _i64, _vp, _i64, _i64, _i64, _i64, _i32, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _vp,

@@ -1,0 +1,496 @@
+// The products of a Newton-Schulz step on the tensor cores (tcgen05.mma.kind::f16, f32 sums).
+//
+// Two shapes of one kernel: a CTA pair on 256 x 256 tiles where those fill the GPU, one CTA on
+// 128 x 128 tiles where they do not. Warp 0 streams 128-wide reduction steps by TMA (one box of
+// 32 KB per operand), warp 1 issues the MMAs into one of two TMEM accumulators, warps 2-5 drain the
+// other. A and B are symmetric: only tiles on and above the diagonal are computed, and written
+// twice; both orders of a diagonal tile's products sum alike, so A and B stay symmetric bit for
+// bit, and the update may read B by rows. X is read by columns there (MN-major), from the same
+// storage.
+//
+// Bound by the tensor cores at the sides the update is worth its time for: 2 r^2 c products for
+// X', half of that for A, and r^3 for B, against 4 r c + 2 r^2 values moved.
+#include <algorithm>
+#include <cstring>
+#include <mutex>
+
+#include "dequant.cuh"
+#include "ns_args.cuh"
+
+namespace moss {
+namespace ns {
+namespace {
+
+constexpr int kHalf = 128;
+constexpr int kStep = 128;  // reduction indices per stage: two 64-wide boxes
+constexpr int kStages = 3;
+constexpr int kEpiWarp0 = 2;
+constexpr int kThreads = 6 * 32;
+constexpr uint32_t kTileBytes = kHalf * kStep * 2;  // 32 KB
+constexpr uint32_t kStageBytes = 2 * kTileBytes;
+constexpr uint32_t kDataBytes = kStages * kStageBytes;
+constexpr uint32_t kSmemBytes = kDataBytes + 1024 + 512;
+constexpr long long kExitBudgetCycles = (kStages + 4) * kWaitBudgetCycles;
+static_assert(kSmemBytes <= 227 * 1024, "rings exceed the shared memory a CTA may use");
+
+struct Barriers {
+  uint64_t full[kStages];   // leader: both CTAs' operands landed
+  uint64_t empty[kStages];  // local
+  uint64_t acc_full[2];     // local
+  uint64_t acc_empty[2];    // leader
+  uint64_t drain;
+  uint64_t exit_bar;
+  uint32_t tmem_base;
+  int abort_flag;
+};
+static_assert(sizeof(Barriers) <= 512, "barrier block too large");
+
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int c2) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(c2)
+      : "memory");
+}
+__device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1,
+                                                 int c2) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(c2)
+      : "memory");
+}
+
+// Tile t of a symmetric product: column n holds the n + 1 tiles (0..n, n).
+__device__ __forceinline__ void upper_tile(int t, int& m, int& n) {
+  n = static_cast<int>((sqrtf(8.0f * static_cast<float>(t) + 1.0f) - 1.0f) * 0.5f);
+  while (n * (n + 1) / 2 > t) --n;
+  while ((n + 1) * (n + 2) / 2 <= t) ++n;
+  m = t - n * (n + 1) / 2;
+}
+
+template <Mode kMode>
+__device__ __forceinline__ void locate(const Args& a, int u, int& b, int& m, int& n) {
+  b = u / a.tiles;
+  const int t = u - b * a.tiles;
+  if constexpr (kMode == kUpdate) {
+    gemm::tile_coords(t, a.tiles_m, a.tiles_n, m, n);
+  } else {
+    upper_tile(t, m, n);
+  }
+}
+
+__device__ __forceinline__ void load32(const __half* p, float (&v)[32]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint4 w = __ldg(reinterpret_cast<const uint4*>(p) + i);
+    const uint32_t h[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[j]));
+      v[8 * i + 2 * j] = f.x;
+      v[8 * i + 2 * j + 1] = f.y;
+    }
+  }
+}
+__device__ __forceinline__ void store32(__half* p, const float (&v)[32]) {
+  uint32_t w0[8], w1[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    w0[j] = gemm::pack2_kind<kF16>(v[2 * j], v[2 * j + 1]);
+    w1[j] = gemm::pack2_kind<kF16>(v[16 + 2 * j], v[16 + 2 * j + 1]);
+  }
+  gemm::stg256(p, w0);
+  gemm::stg256(p + 16, w1);
+}
+
+// 32 consecutive accumulators of one row through the mode's epilogue. i, j: row and first column.
+template <Mode kMode>
+__device__ __forceinline__ void finish32(const Args& a, int b, int i, int j, bool mirror, float (&v)[32]) {
+  if constexpr (kMode == kUpdate) {
+    const int64_t at = (static_cast<int64_t>(b) * a.rp + i) * a.cp + j;
+    float x[32];
+    load32(a.add_hi + at, x);
+    if (a.add_lo != nullptr) {
+      float lo[32];
+      load32(a.add_lo + at, lo);
+#pragma unroll
+      for (int e = 0; e < 32; ++e) x[e] += lo[e];
+    }
+#pragma unroll
+    for (int e = 0; e < 32; ++e) v[e] = fmaf(a.beta, x[e], a.alpha * v[e]);
+    if (a.result != nullptr) {
+      if (i >= a.r) return;
+      __nv_bfloat16* out = a.result + static_cast<int64_t>(b) * a.r * a.c;
+      if (a.tall) {  // lanes hold consecutive rows: 64 contiguous bytes per column
+#pragma unroll
+        for (int e = 0; e < 32; ++e)
+          if (j + e < a.c) out[static_cast<int64_t>(j + e) * a.r + i] = __float2bfloat16_rn(v[e]);
+      } else {
+        __nv_bfloat16* row = out + static_cast<int64_t>(i) * a.c + j;
+        if (j + 32 <= a.c && (reinterpret_cast<uintptr_t>(row) & 31) == 0) {
+          uint32_t w0[8], w1[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            w0[e] = gemm::pack2_kind<kBF16>(v[2 * e], v[2 * e + 1]);
+            w1[e] = gemm::pack2_kind<kBF16>(v[16 + 2 * e], v[16 + 2 * e + 1]);
+          }
+          gemm::stg256(row, w0);
+          gemm::stg256(row + 16, w1);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            if (j + e < a.c) row[e] = __float2bfloat16_rn(v[e]);
+        }
+      }
+      return;
+    }
+    store32(a.out_hi + at, v);
+    if (a.out_lo != nullptr) {
+#pragma unroll
+      for (int e = 0; e < 32; ++e) v[e] -= __half2float(__float2half_rn(v[e]));
+      store32(a.out_lo + at, v);
+    }
+  } else {
+    const int64_t base = static_cast<int64_t>(b) * a.rp * a.rp;
+    const int64_t at = base + static_cast<int64_t>(i) * a.rp + j;
+    if constexpr (kMode == kSquare) {
+      float x[32];
+      load32(a.add_hi + at, x);
+#pragma unroll
+      for (int e = 0; e < 32; ++e) v[e] = fmaf(a.beta, x[e], a.alpha * v[e]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 32; ++e) v[e] *= a.alpha;
+    }
+    store32(a.out_hi + at, v);
+    if (mirror) {
+#pragma unroll
+      for (int e = 0; e < 32; ++e) a.out_hi[base + static_cast<int64_t>(j + e) * a.rp + i] = __float2half_rn(v[e]);
+    }
+  }
+}
+
+template <Mode kMode, int kCtas>
+__global__ void __launch_bounds__(kThreads, 1)
+    ns_gemm_kernel(const __grid_constant__ CUtensorMap tm_left, const __grid_constant__ CUtensorMap tm_right,
+                   const Args args) {
+  constexpr bool kColumns = kMode == kUpdate;  // the right operand is read by columns (MN-major)
+  constexpr int kTile = kHalf * kCtas;
+  constexpr uint32_t kTmemCols = 2 * kTile;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw_base = smem_u32(smem_raw);
+  const uint32_t base = (raw_base + 1023u) & ~1023u;
+  Barriers* bars = reinterpret_cast<Barriers*>(smem_raw + (base - raw_base) + kDataBytes);
+  auto bar = [&](uint64_t& b) { return smem_u32(&b); };
+  volatile int* abort_flag = &bars->abort_flag;
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const uint32_t rank = kCtas == 2 ? cluster_ctarank() : 0;
+  const bool leader = rank == 0;
+  const int first_unit = blockIdx.x / kCtas;
+  const int unit_step = gridDim.x / kCtas;
+  const int num_units = args.tiles * args.batch;
+  const int steps = (kMode == kGram ? args.cp : args.rp) / kStep;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(bar(bars->full[s]), 1);
+      mbar_init(bar(bars->empty[s]), 1);
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(bar(bars->acc_full[s]), 1);
+      mbar_init(bar(bars->acc_empty[s]), kCtas * 4);
+    }
+    mbar_init(bar(bars->drain), 1);
+    mbar_init(bar(bars->exit_bar), 1);
+    bars->abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    if constexpr (kCtas == 2) {
+      tmem_alloc_pair(smem_u32(&bars->tmem_base), kTmemCols);
+      tmem_relinquish_pair();
+    } else {
+      tmem_alloc(smem_u32(&bars->tmem_base), kTmemCols);
+      tmem_relinquish();
+    }
+  }
+  tc_fence_before();
+  if constexpr (kCtas == 2)
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  else
+    __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = bars->tmem_base;
+
+  if (warp == 0) {
+    // ---------------------------------------------------------------- producer (every CTA)
+    if (lane == 0) {
+      tma_prefetch_desc(&tm_left);
+      tma_prefetch_desc(&tm_right);
+    }
+    int stage = 0;
+    uint32_t phase = 0, used = 0, last_phase = 0;
+    bool ok = true;
+    for (int u = first_unit; u < num_units && ok; u += unit_step) {
+      int b, m, n;
+      locate<kMode>(args, u, b, m, n);
+      const int m0 = b * args.rp + m * kTile + static_cast<int>(rank) * kHalf;  // row of the left operand
+      const int n0 = n * kTile + static_cast<int>(rank) * kHalf;                // this CTA's columns
+      for (int s = 0; s < steps; ++s) {
+        if (!mbar_wait_cluster(bar(bars->empty[stage]), phase ^ 1u, abort_flag, args.status,
+                               MOSS_STATUS_TIMEOUT_LOAD)) {
+          ok = false;
+          break;
+        }
+        if (lane == 0) {
+          const uint32_t dst = base + stage * kStageBytes;
+          const int ry = kColumns ? b * args.rp + s * kStep : b * args.rp + n0;
+          const int rz = kColumns ? n0 / 64 : s * 2;
+          if constexpr (kCtas == 2) {
+            if (leader) mbar_arrive_expect_tx(bar(bars->full[stage]), kCtas * kStageBytes);
+            const uint32_t fb = mapa_shared(bar(bars->full[stage]), 0);
+            tma_load_3d_pair(dst, &tm_left, fb, 0, m0, s * 2);
+            tma_load_3d_pair(dst + kTileBytes, &tm_right, fb, 0, ry, rz);
+          } else {
+            mbar_arrive_expect_tx(bar(bars->full[stage]), kStageBytes);
+            tma_load_3d(dst, &tm_left, bar(bars->full[stage]), 0, m0, s * 2);
+            tma_load_3d(dst + kTileBytes, &tm_right, bar(bars->full[stage]), 0, ry, rz);
+          }
+          used |= 1u << stage;
+          last_phase = (last_phase & ~(1u << stage)) | (phase << stage);
+        }
+        __syncwarp();
+        if (++stage == kStages) { stage = 0; phase ^= 1u; }
+      }
+    }
+    if (lane == 0 && leader) {  // the copies land before the CTA may leave (the peer waits for the leader)
+      for (int s = 0; s < kStages; ++s) {
+        if (!((used >> s) & 1u)) continue;
+        const long long start = clock64();
+        while (!mbar_try_wait(bar(bars->full[s]), (last_phase >> s) & 1u)) {
+          if (clock64() - start > kWaitBudgetCycles) {
+            report_status(args.status, MOSS_STATUS_TIMEOUT_DRAIN);
+            break;
+          }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ---------------------------------------------------------------- MMA issuer (leader)
+    if (leader) {
+      constexpr uint32_t idesc = umma_idesc_f16(0u, kColumns, kTile, kTile);
+      int stage = 0, it = 0;
+      uint32_t phase = 0;
+      bool ok = true, issued = false;
+      for (int u = first_unit; u < num_units && ok; u += unit_step, ++it) {
+        const int acc = it & 1;
+        if (!mbar_wait_cluster(bar(bars->acc_empty[acc]), ((it >> 1) & 1) ^ 1u, abort_flag, args.status,
+                               MOSS_STATUS_TIMEOUT_MMA))
+          break;
+        tc_fence_after();
+        const uint32_t d = tmem_base + static_cast<uint32_t>(acc * kTile);
+        for (int s = 0; s < steps; ++s) {
+          if (!mbar_wait_cluster(bar(bars->full[stage]), phase, abort_flag, args.status, MOSS_STATUS_TIMEOUT_MMA)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          if (lane == 0) {
+            const uint32_t left = base + stage * kStageBytes, right = left + kTileBytes;
+#pragma unroll
+            for (int kk = 0; kk < kStep / 16; ++kk) {
+              // K-major: [2 boxes][128 rows][64 values]; by columns: [2 boxes of 64 columns][128 rows]
+              const uint64_t ld = umma_desc_sw128(left + (kk >> 2) * (kTileBytes / 2) + (kk & 3) * 32, 16, 1024);
+              const uint64_t rd = kColumns
+                                      ? umma_desc_sw128(right + kk * 2048, kTileBytes / 2, 1024)
+                                      : umma_desc_sw128(right + (kk >> 2) * (kTileBytes / 2) + (kk & 3) * 32, 16, 1024);
+              if constexpr (kCtas == 2)
+                umma_f16_pair(d, ld, rd, idesc, (s > 0 || kk > 0) ? 1u : 0u);
+              else
+                umma_f16(d, ld, rd, idesc, (s > 0 || kk > 0) ? 1u : 0u);
+            }
+            if constexpr (kCtas == 2)
+              umma_commit_pair_mc(bar(bars->empty[stage]), 0x3);
+            else
+              umma_commit(bar(bars->empty[stage]));
+            issued = true;
+          }
+          __syncwarp();
+          if (++stage == kStages) { stage = 0; phase ^= 1u; }
+        }
+        if (!ok) break;
+        if (lane == 0) {
+          if constexpr (kCtas == 2)
+            umma_commit_pair_mc(bar(bars->acc_full[acc]), 0x3);
+          else
+            umma_commit(bar(bars->acc_full[acc]));
+        }
+        __syncwarp();
+      }
+      if (lane == 0 && issued) {
+        if constexpr (kCtas == 2)
+          umma_commit_pair(bar(bars->drain));
+        else
+          umma_commit(bar(bars->drain));
+        const long long start = clock64();
+        while (!mbar_try_wait(bar(bars->drain), 0)) {
+          if (clock64() - start > kWaitBudgetCycles) {
+            report_status(args.status, MOSS_STATUS_TIMEOUT_DRAIN);
+            break;
+          }
+        }
+      }
+      __syncwarp();
+    }
+  } else {
+    // ---------------------------------------------------------------- epilogue (every CTA)
+    const int q = warp & 3;
+    int it = 0;
+    for (int u = first_unit; u < num_units; u += unit_step, ++it) {
+      const int acc = it & 1;
+      if (!mbar_wait_cluster(bar(bars->acc_full[acc]), (it >> 1) & 1, abort_flag, args.status,
+                             MOSS_STATUS_TIMEOUT_EPILOGUE))
+        break;
+      tc_fence_after();
+      int b, m, n;
+      locate<kMode>(args, u, b, m, n);
+      const int i = m * kTile + static_cast<int>(rank) * kHalf + q * 32 + lane;
+      const int cols = kMode == kUpdate ? args.cp : args.rp;
+#pragma unroll 1
+      for (int c = 0; c < kTile / 32; ++c) {
+        uint32_t r[32];
+        tmem_ld_32x32b_x32(tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(acc * kTile + c * 32),
+                           r);
+        tmem_wait_ld();
+        if (c == kTile / 32 - 1) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) {
+            const uint32_t eb = bar(bars->acc_empty[acc]);
+            if (kCtas == 1 || leader)
+              mbar_arrive(eb);
+            else
+              mbar_arrive_cluster(mapa_shared(eb, 0));
+          }
+        }
+        const int j = n * kTile + c * 32;
+        if (i >= args.rp || j >= cols) continue;  // past this matrix: the next one's rows, or nothing
+        float v[32];
+#pragma unroll
+        for (int e = 0; e < 32; ++e) v[e] = __uint_as_float(r[e]);
+        finish32<kMode>(args, b, i, j, m != n, v);
+      }
+    }
+  }
+
+  // Leave together (the pair reads and signals each other's shared memory and TMEM).
+  tc_fence_before();
+  __syncthreads();
+  if constexpr (kCtas == 2) {
+    if (threadIdx.x == 0) {
+      if (*abort_flag) st_shared_cluster_u32(mapa_shared(smem_u32(&bars->abort_flag), rank ^ 1u), 1u);
+      mbar_arrive_cluster(mapa_shared(bar(bars->exit_bar), rank ^ 1u));
+      const long long start = clock64();
+      while (!mbar_try_wait_cluster(bar(bars->exit_bar), 0)) {
+        if (clock64() - start > kExitBudgetCycles) {
+          report_status(args.status, MOSS_STATUS_TIMEOUT_DRAIN);
+          break;
+        }
+      }
+    }
+    __syncthreads();
+  }
+  if (warp == 1) {
+    tc_fence_after();
+    if constexpr (kCtas == 2)
+      tmem_dealloc_pair(tmem_base, kTmemCols);
+    else
+      tmem_dealloc(tmem_base, kTmemCols);
+  }
+}
+
+template <Mode kMode, int kCtas>
+int launch_typed(const CUtensorMap& tl, const CUtensorMap& tr, Args a, cudaStream_t stream) {
+  auto kern = ns_gemm_kernel<kMode, kCtas>;
+  static std::once_flag once;
+  static cudaError_t attr_err = cudaSuccess;
+  static int max_groups = 0;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = kCtas;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = kSmemBytes;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  std::call_once(once, [&] {
+    attr_err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+    if (attr_err != cudaSuccess) return;
+    max_groups = sm_count() / kCtas;
+    if (kCtas > 1) {
+      cfg.gridDim = dim3(kCtas * max_groups);
+      int clusters = 0;
+      if (cudaOccupancyMaxActiveClusters(&clusters, kern, &cfg) == cudaSuccess && clusters > 0)
+        max_groups = clusters;
+      else
+        cudaGetLastError();
+    }
+  });
+  MOSS_CUDA_TRY(attr_err);
+  const int side = kHalf * kCtas;
+  a.tiles_m = (a.rp + side - 1) / side;
+  a.tiles_n = kMode == kUpdate ? (a.cp + side - 1) / side : a.tiles_m;
+  a.tiles = kMode == kUpdate ? a.tiles_m * a.tiles_n : a.tiles_m * (a.tiles_m + 1) / 2;
+  const int64_t units = static_cast<int64_t>(a.tiles) * a.batch;
+  if (units > INT32_MAX) return fail(MOSS_ERR_INVALID_ARGUMENT, "too many matrices to orthogonalize in one call");
+  cfg.gridDim = dim3(static_cast<unsigned>(kCtas * std::min<int64_t>(units, max_groups)));
+  cfg.stream = stream;
+  return check_cuda(cudaLaunchKernelEx(&cfg, kern, tl, tr, a), "ns_gemm_kernel");
+}
+
+// Pair tiles where their rounds over the GPU take no longer than those of 128 x 128 tiles. A pair
+// tile's stage lasts twice as long for four times the products; a single tile reads twice the
+// shared memory for each (the factor 1.3).
+bool use_pair(Mode mode, const Args& a) {
+  const int sms = sm_count();
+  auto tiles = [&](int side) {
+    const int64_t tm = (a.rp + side - 1) / side, tn = (a.cp + side - 1) / side;
+    return (mode == kUpdate ? tm * tn : tm * (tm + 1) / 2) * a.batch;
+  };
+  const int64_t pairs = std::max(1, sms / 2);
+  const int64_t pair_cost = (tiles(256) + pairs - 1) / pairs * 20;
+  const int64_t single_cost = (tiles(128) + sms - 1) / sms * 13;
+  return pair_cost <= single_cost;
+}
+
+}  // namespace
+
+int launch_gemm(Mode mode, const __half* left, const __half* right, const Args& a, cudaStream_t stream) {
+  // [batch * rp][cols] viewed as {64, rows, cols / 64}: a box is 128 rows of two 64-wide columns
+  auto map = [&](CUtensorMap* m, const __half* p, int cols) {
+    memset(m, 0, sizeof(*m));
+    const uint64_t dims[3] = {64, static_cast<uint64_t>(a.batch) * a.rp, static_cast<uint64_t>(cols / 64)};
+    const uint64_t strides[2] = {static_cast<uint64_t>(cols) * 2, 128};
+    const uint32_t box[3] = {64, 128, 2};
+    return gemm::make_map_nd(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, p, 3, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+  };
+  CUtensorMap tl, tr;
+  if (!map(&tl, left, mode == kGram ? a.cp : a.rp) || !map(&tr, right, mode == kSquare ? a.rp : a.cp))
+    return fail(MOSS_ERR_CUDA, "the driver refused a tensor map of the orthogonalised update");
+  const bool pair = use_pair(mode, a);
+  switch (mode) {
+    case kGram:
+      return pair ? launch_typed<kGram, 2>(tl, tr, a, stream) : launch_typed<kGram, 1>(tl, tr, a, stream);
+    case kSquare:
+      return pair ? launch_typed<kSquare, 2>(tl, tr, a, stream) : launch_typed<kSquare, 1>(tl, tr, a, stream);
+    default:
+      return pair ? launch_typed<kUpdate, 2>(tl, tr, a, stream) : launch_typed<kUpdate, 1>(tl, tr, a, stream);
+  }
+}
+
+}  // namespace ns
+}  // namespace moss

@@ -1,0 +1,143 @@
+"""Orthogonalised updates of trained matrices on the tensor cores (``moss_orthogonalize``).
+
+For the projections that are trained in full (``full_qkvo`` models) and for adapter factors: the
+optimiser replaces a matrix's momentum by the nearest matrix with equal singular values, found by
+a few steps of an odd polynomial (Newton-Schulz; the Muon optimiser of Jordan et al., 2024),
+
+    X = G / max(|G|, eps);   A = X X^T,  X <- a X + (b A + c A A) X   (each step)
+
+:func:`orthogonalize` is that map for one matrix or a batch of them, :class:`Muon` the optimiser
+around it. CUDA tensors only: there is no CPU path.
+
+The result is bfloat16 whatever the input's type: it is a direction, and its own rounding is the
+largest error in it. The iteration runs on float16 operands with float32 sums (float32 throughout
+when the shorter side is at most 64), which keeps the error against float64 within 1.5 times that
+rounding. An infinity or NaN in a matrix gives a NaN matrix; a zero matrix gives zeros.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+from functools import lru_cache
+from typing import Iterable, Sequence
+
+import torch
+
+from . import _lib
+from .quant_kernels import poll_device_status, status_buffer
+
+# Steep at zero: small singular values grow 3.4-fold a step, and all end within about 0.7 to 1.2.
+COEFFICIENTS = (3.4445, -4.7750, 2.0315)
+
+
+@lru_cache(maxsize=1024)
+def _workspace_bytes(batch: int, rows: int, cols: int) -> int:
+    size = ctypes.c_size_t()
+    _lib.check(_lib.library().moss_orthogonalize_workspace_bytes(batch, rows, cols, ctypes.byref(size)),
+               "moss_orthogonalize_workspace_bytes")
+    return size.value
+
+
+@lru_cache(maxsize=64)
+def _coefficient_array(coefficients: tuple, steps: int) -> ctypes.Array:
+    if coefficients and not isinstance(coefficients[0], tuple):
+        coefficients = (coefficients,) * steps
+    if len(coefficients) != steps or any(len(step) != 3 for step in coefficients):
+        raise ValueError("orthogonalize: coefficients must be (a, b, c), or one such triple for each step.")
+    return (ctypes.c_float * (3 * steps))(*(float(value) for step in coefficients for value in step))
+
+
+def orthogonalize(update: torch.Tensor, steps: int = 5,
+                  coefficients: Sequence[float] | Sequence[Sequence[float]] = COEFFICIENTS, eps: float = 1e-7, *,
+                  out: torch.Tensor | None = None) -> torch.Tensor:
+    """The orthogonalised update of ``[rows, cols]`` or each of ``[..., rows, cols]``, in bfloat16.
+
+    ``update``: float16, bfloat16 or float32 on CUDA. ``coefficients``: one ``(a, b, c)`` for all ``steps``
+    (1 to 16), or one for each. ``eps``: the least norm a matrix is divided by.
+    """
+    if not update.is_cuda:
+        raise RuntimeError("orthogonalize runs on CUDA tensors only (there is no CPU path).")
+    if update.ndim < 2 or update.dtype not in _lib.DTYPE_CODES:
+        raise ValueError("orthogonalize: the update must be a float16, bfloat16 or float32 [..., rows, cols] tensor.")
+    if not 1 <= steps <= 16:
+        raise ValueError("orthogonalize: steps must be between 1 and 16.")
+    if not (eps > 0.0 and math.isfinite(eps)):
+        raise ValueError("orthogonalize: eps must be positive and finite.")
+    values = _coefficient_array(tuple(tuple(c) if isinstance(c, (tuple, list)) else c for c in coefficients), steps)
+    device = update.device
+    status = status_buffer(device)
+    poll_device_status(device)
+    update = update.detach().contiguous()
+    if out is None:
+        out = torch.empty(update.shape, dtype=torch.bfloat16, device=device)
+    elif out.shape != update.shape or out.dtype != torch.bfloat16 or out.device != device or not out.is_contiguous():
+        raise ValueError("orthogonalize: the output buffer must be a contiguous bfloat16 tensor like the update.")
+    rows, cols = update.shape[-2:]
+    batch = 1
+    for length in update.shape[:-2]:
+        batch *= length
+    size = _workspace_bytes(batch, rows, cols)
+    workspace = torch.empty(size, dtype=torch.uint8, device=device) if size else None
+    _lib.check(_lib.library().moss_orthogonalize(
+        update.data_ptr(), _lib.DTYPE_CODES[update.dtype], batch, rows, cols, steps, values, float(eps), out.data_ptr(),
+        _lib.ptr(workspace), size, status.data_ptr(), _lib.stream_handle(device)), "moss_orthogonalize")
+    _lib.count_launch("orthogonalize")
+    return out
+
+
+class Muon(torch.optim.Optimizer):
+    """Momentum, orthogonalised, as the update of each trained matrix.
+
+    ``m <- momentum m + g``; the direction is ``orthogonalize(g + momentum m)`` (``nesterov``) or
+    ``orthogonalize(m)``; then ``w <- (1 - lr weight_decay) w - lr s direction`` with
+    ``s = 0.2 sqrt(max(rows, cols))``, which gives the update the root mean square that AdamW's usually
+    has, so that its learning rates carry over. Matrices only: norms, biases and embeddings
+    belong to another optimiser. Parameters of one shape and dtype are orthogonalised in one call.
+    """
+
+    def __init__(self, params: Iterable, lr: float = 1e-3, *, momentum: float = 0.95, nesterov: bool = True,
+                 weight_decay: float = 0.0, steps: int = 5, coefficients: Sequence[float] = COEFFICIENTS,
+                 eps: float = 1e-7) -> None:
+        if lr < 0.0 or weight_decay < 0.0 or not 0.0 <= momentum < 1.0:
+            raise ValueError("Muon: lr and weight_decay must not be negative, and momentum must be in [0, 1).")
+        super().__init__(params, dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay,
+                                      steps=steps, coefficients=tuple(coefficients), eps=eps))
+
+    def add_param_group(self, param_group: dict) -> None:
+        super().add_param_group(param_group)
+        if any(p.ndim != 2 for p in self.param_groups[-1]["params"]):
+            self.param_groups.pop()
+            raise ValueError("Muon updates matrices only (2 dimensions).")
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        for group in self.param_groups:
+            shapes: dict[tuple, list[torch.Tensor]] = {}
+            for p in group["params"]:
+                if p.grad is not None:
+                    shapes.setdefault((p.shape, p.dtype, p.device), []).append(p)
+            for (shape, _, _), params in shapes.items():
+                self._step_shape(group, shape, params)
+        return loss
+
+    def _step_shape(self, group: dict, shape: torch.Size, params: list[torch.Tensor]) -> None:
+        momentum, grads = group["momentum"], [p.grad for p in params]
+        buffers = []
+        for p in params:
+            state = self.state[p]
+            if "momentum_buffer" not in state:
+                state["momentum_buffer"] = torch.zeros_like(p)
+            buffers.append(state["momentum_buffer"])
+        torch._foreach_mul_(buffers, momentum)
+        torch._foreach_add_(buffers, grads)
+        updates = torch._foreach_add(grads, buffers, alpha=momentum) if group["nesterov"] else buffers
+        directions = orthogonalize(torch.stack(updates), group["steps"], group["coefficients"], group["eps"])
+        if group["weight_decay"]:
+            torch._foreach_mul_(params, 1.0 - group["lr"] * group["weight_decay"])
+        rate = group["lr"] * 0.2 * math.sqrt(max(shape))
+        torch._foreach_add_(params, list(directions.unbind(0)), alpha=-rate)

@@ -1,0 +1,163 @@
+"""The orthogonalised update on the GPU against the same iteration in float64."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from moss_image_b200.muon import COEFFICIENTS, Muon, orthogonalize
+
+pytestmark = pytest.mark.gpu
+
+# The result's rounding to bfloat16 alone is off by 1.66e-3 (relative 2-norm: the root mean square of
+# a uniform half-step error over a mantissa uniform in its logarithm). The iteration may add as
+# much again in square: 1.5 times the rounding in all.
+WITHIN = 1.5 * 1.66e-3
+
+
+def _exact(update, steps=5, coefficients=COEFFICIENTS, eps=1e-7):
+    x = update.double()
+    tall = x.shape[-2] > x.shape[-1]
+    x = x.mT if tall else x
+    x = x / torch.linalg.matrix_norm(x, keepdim=True).clamp_min(eps)
+    for step in range(steps):
+        a, b, c = coefficients if not isinstance(coefficients[0], tuple) else coefficients[step]
+        gram = x @ x.mT
+        x = a * x + (b * gram + c * gram @ gram) @ x
+    return x.mT if tall else x
+
+
+def _off(got, want):
+    return float((got.double() - want).norm() / want.norm())
+
+
+def _updates(kind, shape, device, seed=0):
+    gen = torch.Generator(device=device).manual_seed(seed)
+    *lead, m, n = shape
+    base = torch.randn(*shape, generator=gen, device=device)
+    if kind == "strong":  # a few directions 80 times stronger than all the others together
+        base = base + 30.0 * torch.randn(*lead, m, 8, generator=gen, device=device) @ torch.randn(*lead, 8, n, generator=gen,
+                                                                                                   device=device)
+    elif kind == "rows":
+        base = base * torch.exp(torch.randn(*lead, m, 1, generator=gen, device=device))
+    elif kind == "decay":
+        base = base * (torch.arange(m, device=device) + 1.0).reciprocal()[:, None]
+    return 1e-3 * base
+
+
+SHAPES = [(16, 16), (1, 40), (40, 1), (3, 5), (17, 300), (32, 3072), (3072, 32), (64, 64), (61, 517), (65, 65), (100, 300),
+          (300, 100), (128, 128), (129, 257), (521, 1000), (1000, 521), (384, 2048), (2304, 700)]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_one_matrix(cuda_device, shape, dtype):
+    update = _updates("plain", shape, cuda_device, seed=shape[0]).to(dtype)
+    got = orthogonalize(update)
+    assert got.dtype == torch.bfloat16 and got.shape == update.shape
+    # few values do not average: one rounding step of each is 2^-8 at most
+    assert _off(got, _exact(update)) < (WITHIN if update.numel() >= 4096 else 2.0 ** -8 + 1e-4)
+
+
+@pytest.mark.parametrize("kind", ["strong", "rows", "decay"])
+@pytest.mark.parametrize("shape", [(32, 1024), (256, 256), (640, 1500), (1500, 640), (1024, 1024)])
+def test_uneven_spectra_keep_their_precision(cuda_device, shape, kind):
+    update = _updates(kind, shape, cuda_device, seed=3)
+    assert _off(orthogonalize(update), _exact(update)) < WITHIN
+
+
+@pytest.mark.parametrize("shape", [(5, 24, 200), (3, 200, 24), (3, 130, 150), (2, 2, 300, 200), (7, 512, 512), (2, 1100, 1300)])
+def test_batches_are_their_matrices_one_by_one(cuda_device, shape):
+    update = _updates("rows", shape, cuda_device, seed=4)
+    got, want = orthogonalize(update), _exact(update)
+    for one, exact in zip(got.flatten(0, -3), want.flatten(0, -3)):
+        assert _off(one, exact) < WITHIN
+    assert torch.equal(got, orthogonalize(update))
+
+
+@pytest.mark.parametrize("shape", [(24, 100), (200, 300)])
+def test_steps_coefficients_and_out(cuda_device, shape):
+    update = _updates("plain", shape, cuda_device, seed=5)
+    cubic = (1.5, -0.5, 0.0)
+    each = ((3.4445, -4.7750, 2.0315), (2.5, -2.0, 0.5), (1.875, -1.25, 0.375))
+    for steps, coefficients in ((1, COEFFICIENTS), (2, cubic), (12, cubic), (3, each)):
+        assert _off(orthogonalize(update, steps, coefficients), _exact(update, steps, coefficients)) < 2.0 ** -8
+    out = torch.empty(shape, dtype=torch.bfloat16, device=cuda_device)
+    assert orthogonalize(update, out=out) is out and torch.equal(out, orthogonalize(update))
+    # 12 cubic steps converge for singular values that started above 1 / 1.5^11
+    converged = orthogonalize(update, 16, cubic).double()
+    square = converged @ converged.mT
+    assert float((square - torch.eye(shape[0], device=cuda_device)).abs().max()) < 0.02
+
+
+@pytest.mark.parametrize("shape", [(2, 20, 60), (2, 150, 210)])
+def test_zero_tiny_large_and_nonfinite_matrices(cuda_device, shape):
+    update = _updates("plain", shape, cuda_device, seed=6)
+    clean = orthogonalize(update)
+    update[1] = 0.0
+    got = orthogonalize(update)
+    assert torch.equal(got[0], clean[0]) and not got[1].any()
+    update[1] = update[0] * 1e-9  # below eps: scaled by 1 / eps, as the definition says
+    assert _off(orthogonalize(update)[1], _exact(update)[1]) < 2.0 ** -8
+    update[1] = update[0] * 1e12
+    assert _off(orthogonalize(update)[1], _exact(update)[1]) < 2.0 ** -8
+    for value in (float("nan"), float("inf")):
+        update[1] = update[0]
+        update[1, 3, 7] = value
+        got = orthogonalize(update)
+        assert torch.equal(got[0], clean[0]) and got[1].isnan().all()
+
+
+def test_strides_streams_and_empty(cuda_device):
+    update = _updates("plain", (200, 150), cuda_device, seed=7)
+    got = orthogonalize(update)
+    assert torch.equal(orthogonalize(update.t().contiguous().t()), got)
+    odd = torch.empty(200 * 150 + 1, device=cuda_device)[1:].view(200, 150).copy_(update)
+    assert torch.equal(orthogonalize(odd), got)
+    stream = torch.cuda.Stream(cuda_device)
+    stream.wait_stream(torch.cuda.current_stream(cuda_device))
+    with torch.cuda.stream(stream):
+        other = orthogonalize(update)
+    stream.synchronize()
+    assert torch.equal(other, got)
+    assert orthogonalize(update[:0]).shape == (0, 150) and orthogonalize(update[None, :, :0]).shape == (1, 200, 0)
+    assert orthogonalize(update.expand(0, 200, 150)).shape == (0, 200, 150)
+
+
+def test_optimizer_step_matches_its_formula(cuda_device):
+    gen = torch.Generator(device=cuda_device).manual_seed(8)
+    shapes = [(96, 160), (160, 96), (96, 160), (24, 300)]
+    params = [torch.nn.Parameter(torch.randn(*s, generator=gen, device=cuda_device)) for s in shapes]
+    mine = [p.detach().double() for p in params]
+    buffers = [torch.zeros_like(p) for p in mine]
+    optimizer = Muon(params, lr=0.02, momentum=0.9, weight_decay=0.1)
+    for _ in range(3):
+        for p, w, m in zip(params, mine, buffers):
+            p.grad = torch.randn(p.shape, generator=gen, device=cuda_device)
+            m.mul_(0.9).add_(p.grad.double())
+            direction = _exact(p.grad.double() + 0.9 * m)
+            w.mul_(1 - 0.02 * 0.1).sub_(0.02 * 0.2 * max(p.shape) ** 0.5 * direction)
+        optimizer.step()
+    for p, w in zip(params, mine):
+        # three updates, each off by at most WITHIN of its norm 0.004 sqrt(max) sqrt(min) 1.2, and f32 weights
+        room = 3 * WITHIN * 0.004 * (p.shape[0] * p.shape[1]) ** 0.5 * 1.2 + 1e-6 * float(w.norm())
+        assert float((p.detach().double() - w).norm()) < room
+
+
+def test_refusals(cuda_device):
+    update = torch.zeros(8, 8, device=cuda_device)
+    for arguments in (dict(steps=0), dict(steps=17), dict(eps=0.0), dict(eps=float("inf")), dict(coefficients=(1.0, 2.0)),
+                      dict(coefficients=((1.0, 0.0, 0.0),) * 2), dict(coefficients=(40.0, 0.0, 0.0)),
+                      dict(coefficients=(float("nan"), 0.0, 0.0)), dict(out=update)):
+        with pytest.raises(ValueError):
+            orthogonalize(update, **arguments)
+    with pytest.raises(ValueError):
+        orthogonalize(update[0])
+    with pytest.raises(ValueError):
+        orthogonalize(update.long())
+    with pytest.raises(RuntimeError, match="CUDA"):
+        orthogonalize(update.cpu())
+    with pytest.raises(ValueError):
+        Muon([torch.nn.Parameter(torch.zeros(4, device=cuda_device))])
+    with pytest.raises(ValueError):
+        Muon([torch.nn.Parameter(update)], momentum=1.0)
