@@ -228,6 +228,19 @@ __host__ __device__ constexpr uint32_t umma_idesc_f16_ab(uint32_t fmt, bool a_mn
   return umma_idesc_f16(fmt, b_mn_major, m, n) | ((a_mn_major ? 1u : 0u) << 15);
 }
 
+// True in one lane of a converged warp. Unlike a test of the lane index, the compiler knows that
+// one lane is left, and keeps the operands of tcgen05.mma in uniform registers: the issue of an MMA
+// then costs a few cycles instead of about 200 (fp8_gemm.cu, ns_gemm.cu).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t one;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(one));
+  return one != 0;
+}
+
 // ---------------------------------------------------------------- clusters and 2-SM (cta_group::2)
 __device__ __forceinline__ uint32_t cluster_ctarank() {
   uint32_t r;

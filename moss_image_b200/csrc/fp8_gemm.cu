@@ -25,9 +25,13 @@ namespace fp8 {
 namespace {
 
 constexpr int kHalf = 128;  // rows of A and columns (or half of the pair's columns) of W per CTA
-constexpr int kEpiWarp0 = 2;
+constexpr int kEpiWarp0 = 4;
 constexpr int kEpiWarps = 8;
 constexpr int kThreads = (kEpiWarp0 + kEpiWarps) * 32;
+// Registers of the pair kernel's warpgroups: 384 threads start with 168 each; the first warpgroup
+// (producer and issuer) gives its share to the two that hold 128 sums and two loads in flight a thread.
+constexpr int kIssueRegs = 40, kEpiRegs = 232;
+static_assert(kIssueRegs + 2 * kEpiRegs <= 3 * 168, "a larger split would wait forever");
 constexpr int kStages = 6;
 constexpr uint32_t kTileBytes = kHalf * kBlock;      // 16 KB: 128 rows of 128 bytes
 constexpr uint32_t kStageBytes = 2 * kTileBytes;     // A rows and W columns
@@ -50,18 +54,44 @@ struct Barriers {
 };
 static_assert(sizeof(Barriers) <= 512, "barrier block too large");
 
-__device__ __forceinline__ void fma2(uint64_t& acc, uint32_t lo, uint32_t hi, uint64_t s) {
-  uint64_t d;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(lo), "r"(hi));
-  asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc) : "l"(d), "l"(s));
+// tcgen05.wait::ld that also orders the use of the loaded registers behind it.
+__device__ __forceinline__ void tmem_wait_ld_of(uint32_t (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                 "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]),
+                 "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]),
+                 "+r"(r[30]), "+r"(r[31])
+               :
+               : "memory");
 }
 
 // Bias and the rounded store of 32 consecutive outputs of one row.
 __device__ __forceinline__ void store32(const Args& args, float (&v)[32], int row, int col0, bool vec_ok) {
   if (args.bias != nullptr) {
+    const uint16_t* b16 = static_cast<const uint16_t*>(args.bias) + col0;
+    if (args.bias_kind != kF32 && col0 + 32 <= args.Nc && (reinterpret_cast<uintptr_t>(b16) & 15) == 0) {
 #pragma unroll
-    for (int j = 0; j < 32; ++j)
-      if (col0 + j < args.Nc) v[j] += load_as_float(args.bias, args.bias_kind, col0 + j);
+      for (int i = 0; i < 4; ++i) {
+        const uint4 u = __ldg(reinterpret_cast<const uint4*>(b16) + i);
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          if (args.bias_kind == kBF16) {
+            v[8 * i + 2 * k] += __uint_as_float(w[k] << 16);
+            v[8 * i + 2 * k + 1] += __uint_as_float(w[k] & 0xFFFF0000u);
+          } else {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[k]));
+            v[8 * i + 2 * k] += f.x;
+            v[8 * i + 2 * k + 1] += f.y;
+          }
+        }
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 32; ++j)
+        if (col0 + j < args.Nc) v[j] += load_as_float(args.bias, args.bias_kind, col0 + j);
+    }
   }
   const int64_t off = static_cast<int64_t>(row) * args.Nc + col0;
   if (vec_ok && col0 + 32 <= args.Nc) {
@@ -142,6 +172,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_after();
   const uint32_t tmem_base = bars->tmem_base;
 
+  if (warp < kEpiWarp0) {
+  if constexpr (kCtas == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegs));
   if (warp == 0) {
     // ---------------------------------------------------------------- producer (every CTA)
     if (lane == 0) {
@@ -203,42 +235,45 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ---------------------------------------------------------------- MMA issuer (leader)
     if (leader) {
       constexpr uint32_t idesc = idesc_e4m3(false, kDX, kTileM, kTileN);
+      // descriptors of the first stage; every other differs by multiples of 16 bytes in the address field
+      const uint64_t a_desc0 = step_desc(base, 0, false), w_desc0 = step_desc(base + kTileBytes, 0, kDX);
       int stage = 0, it = 0;
       uint32_t phase = 0;
       bool ok = true, issued = false;
       for (int u = first_unit; u < num_units && ok; u += unit_step) {
         const int split = u % args.splits;
         const int kb1 = min(args.kb, (split + 1) * args.kb_per_split);
-        for (int kb = split * args.kb_per_split; kb < kb1; ++kb, ++it) {
-          const int acc = it & 1;
-          if (!mbar_wait_cluster(bar(bars->acc_empty[acc]), ((it >> 1) & 1) ^ 1u, abort_flag, args.status,
-                                 MOSS_STATUS_TIMEOUT_MMA) ||
-              !mbar_wait_cluster(bar(bars->full[stage]), phase, abort_flag, args.status, MOSS_STATUS_TIMEOUT_MMA)) {
+        for (int kb = split * args.kb_per_split; kb < kb1 && ok; ++kb, ++it) {
+          const int buf = it & 1;
+          // operands first: they are there long before the accumulator, whose wait is the critical one
+          if (!mbar_wait_cluster(bar(bars->full[stage]), phase, abort_flag, args.status, MOSS_STATUS_TIMEOUT_MMA) ||
+              !mbar_wait_cluster(bar(bars->acc_empty[buf]), ((it >> 1) & 1) ^ 1u, abort_flag, args.status,
+                                 MOSS_STATUS_TIMEOUT_MMA)) {
             ok = false;
             break;
           }
           tc_fence_after();
-          if (lane == 0) {
-            const uint32_t a_tile = base + stage * kStageBytes;
-            const uint32_t d = tmem_base + static_cast<uint32_t>(acc * kTileN);
+          if (elect_one()) {
+            const uint64_t at_stage = static_cast<uint64_t>(stage) * (kStageBytes >> 4);
+            const uint32_t d = tmem_base + static_cast<uint32_t>(buf * kTileN);
 #pragma unroll
             for (int kk = 0; kk < kBlock / 32; ++kk) {
-              const uint64_t ad = step_desc(a_tile, kk, false);
-              const uint64_t wd = step_desc(a_tile + kTileBytes, kk, kDX);
+              const uint64_t ad = a_desc0 + at_stage + kk * (32 >> 4);
+              const uint64_t wd = w_desc0 + at_stage + kk * ((kDX ? 4096 : 32) >> 4);
               if constexpr (kCtas == 2)
                 umma_f8_pair(d, ad, wd, idesc, kk > 0);
               else
                 umma_f8(d, ad, wd, idesc, kk > 0);
             }
             if constexpr (kCtas == 2) {
+              umma_commit_pair_mc(bar(bars->acc_full[buf]), 0x3);
               umma_commit_pair_mc(bar(bars->empty[stage]), 0x3);
-              umma_commit_pair_mc(bar(bars->acc_full[acc]), 0x3);
             } else {
+              umma_commit(bar(bars->acc_full[buf]));
               umma_commit(bar(bars->empty[stage]));
-              umma_commit(bar(bars->acc_full[acc]));
             }
-            issued = true;
           }
+          issued = true;
           __syncwarp();
           if (++stage == kStages) { stage = 0; phase ^= 1u; }
         }
@@ -258,11 +293,15 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       __syncwarp();
     }
+  }
   } else {
     // ---------------------------------------------------------------- epilogue (every CTA)
+    if constexpr (kCtas == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kEpiRegs));
     const int q = warp & 3;
     const int half = (warp - kEpiWarp0) >> 2;
     const uint32_t lane_addr = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(half * kCols);
+    // acc_empty[0] of the leader, as this CTA sees it; acc_empty[1] is 8 bytes further
+    const uint32_t release = kCtas == 2 ? mapa_shared(bar(bars->acc_empty[0]), 0) : bar(bars->acc_empty[0]);
     const bool vec_ok = args.out_kind != kF32 && (args.Nc & 15) == 0 && (reinterpret_cast<uintptr_t>(args.out) & 31) == 0;
     int it = 0;
     bool ok = true;
@@ -271,45 +310,65 @@ __global__ void __launch_bounds__(kThreads, 1)
       int m_blk, n_blk;
       gemm::tile_coords(tile, args.tiles_m, args.tiles_n, m_blk, n_blk, args.group_m);
       const int row = m_blk * kTileM + static_cast<int>(rank) * kHalf + q * 32 + lane;
-      const int col0 = n_blk * kTileN + half * kCols;
-      const float* row_scale = args.row_scale + min(row, args.M - 1);
-      const float* w_scale = args.w_scale + static_cast<int64_t>(min(col0 / kBlock, args.col_blocks - 1)) * args.ws_col;
+      const int col0 = n_blk * kTileN + half * kCols;  // this thread's columns: all in one weight block
       const int kb0 = split * args.kb_per_split, kb1 = min(args.kb, kb0 + args.kb_per_split);
-      uint64_t sum[kCols / 2];
+      float sum[kCols];
 #pragma unroll
-      for (int j = 0; j < kCols / 2; ++j) sum[j] = 0;
-      float next = __ldg(row_scale + kb0 * args.row_pitch) * __ldg(w_scale + static_cast<int64_t>(kb0) * args.ws_red);
-      for (int kb = kb0; kb < kb1; ++kb, ++it) {
-        const uint32_t s32 = __float_as_uint(next);
-        const uint64_t s = (static_cast<uint64_t>(s32) << 32) | s32;
-        if (kb + 1 < kb1)
-          next = __ldg(row_scale + (kb + 1) * args.row_pitch) * __ldg(w_scale + static_cast<int64_t>(kb + 1) * args.ws_red);
-        const int acc = it & 1;
-        if (!mbar_wait_cluster(bar(bars->acc_full[acc]), (it >> 1) & 1, abort_flag, args.status,
-                               MOSS_STATUS_TIMEOUT_EPILOGUE)) {
-          ok = false;
-          break;
+      for (int j = 0; j < kCols; ++j) sum[j] = 0.0f;
+      // The scales come from L2, two blocks ahead, in two slots that take turns (the loop body exists once
+      // for each): a copy from slot to slot would wait for the load.
+      const float* row_scale = args.row_scale + kb0 * args.row_pitch + min(row, args.M - 1);
+      const float* w_scale = args.w_scale + static_cast<int64_t>(kb0) * args.ws_red +
+                             static_cast<int64_t>(min(col0 / kBlock, args.col_blocks - 1)) * args.ws_col;
+      int left = kb1 - kb0;  // blocks whose scales are still to be fetched
+      float sr[2], sw[2];
+      auto fetch = [&](int slot) {
+        if (left > 0) {
+          sr[slot] = __ldg(row_scale);
+          sw[slot] = __ldg(w_scale);
+          row_scale += args.row_pitch;
+          w_scale += args.ws_red;
+          --left;
         }
+      };
+      auto add_block = [&](int slot) {
+        const int buf = it & 1;
+        if (!mbar_wait_cluster(bar(bars->acc_full[buf]), (it >> 1) & 1, abort_flag, args.status,
+                               MOSS_STATUS_TIMEOUT_EPILOGUE))
+          return false;
+        ++it;
         tc_fence_after();
+        // the next 32 columns are on their way out of TMEM while these are added
+        uint32_t r[2][32];
+        const uint32_t buf_addr = lane_addr + static_cast<uint32_t>(buf * kTileN);
+        tmem_ld_32x32b_x32(buf_addr, r[0]);
+        const float s = sr[slot] * sw[slot];
+        fetch(slot);
 #pragma unroll
         for (int c = 0; c < kCols / 32; ++c) {
-          uint32_t r[32];
-          tmem_ld_32x32b_x32(lane_addr + static_cast<uint32_t>(acc * kTileN + c * 32), r);
-          tmem_wait_ld();
-          if (c == kCols / 32 - 1) {
+          tmem_wait_ld_of(r[c & 1]);
+          if (c + 1 < kCols / 32) {
+            tmem_ld_32x32b_x32(buf_addr + (c + 1) * 32, r[(c + 1) & 1]);
+          } else {
             tc_fence_before();
             __syncwarp();
             if (lane == 0) {
-              const uint32_t eb = bar(bars->acc_empty[acc]);
-              if (kCtas == 1 || leader)
-                mbar_arrive(eb);
+              if constexpr (kCtas == 2)
+                mbar_arrive_cluster(release + buf * 8);
               else
-                mbar_arrive_cluster(mapa_shared(eb, 0));
+                mbar_arrive(release + buf * 8);
             }
           }
 #pragma unroll
-          for (int j = 0; j < 16; ++j) fma2(sum[c * 16 + j], r[2 * j], r[2 * j + 1], s);
+          for (int j = 0; j < 32; ++j) sum[c * 32 + j] = fmaf(__uint_as_float(r[c & 1][j]), s, sum[c * 32 + j]);
         }
+        return true;
+      };
+      fetch(0);
+      fetch(1);
+      for (int kb = kb0; kb < kb1 && ok; kb += 2) {
+        ok = add_block(0);
+        if (ok && kb + 1 < kb1) ok = add_block(1);
       }
       if (!ok) break;
       if (row >= args.M) continue;
@@ -319,10 +378,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (col >= args.Nc) break;
         float v[32];
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          v[2 * j] = __uint_as_float(static_cast<uint32_t>(sum[c * 16 + j]));
-          v[2 * j + 1] = __uint_as_float(static_cast<uint32_t>(sum[c * 16 + j] >> 32));
-        }
+        for (int j = 0; j < 32; ++j) v[j] = sum[c * 32 + j];
         if (args.splits > 1) {
           float* dst = args.partial + (static_cast<int64_t>(split) * args.M + row) * args.Nc + col;
 #pragma unroll
