@@ -29,7 +29,9 @@ struct Args {
   int bias_kind;
   void* out;                // [M, Nc] dense
   int out_kind;
-  float* partial;           // [splits][M][Nc] when splits > 1
+  int tma_out;              // the output has a tensor map: 16-bit, rows and base on 16-byte boundaries
+  // splits > 1: f32 partials, [split][M][Nc] (few rows) or [split][tile][128 columns][128 rows]
+  float* partial;
   int splits, kb_per_split;
   int tiles_m, tiles_n, group_m;
   StatusSink status;
@@ -50,8 +52,8 @@ int sm_count();
 int launch_quantize_rows(const void* x, int dtype, int64_t m, int64_t k, uint8_t* codes, float* scale,
                          int64_t row_pitch, cudaStream_t stream);
 
-int launch_gemm(bool dx, const Plan& plan, const CUtensorMap& ta, const CUtensorMap& tw, const Args& a,
-                cudaStream_t stream);
+int launch_gemm(bool dx, const Plan& plan, const CUtensorMap& ta, const CUtensorMap& tw, const CUtensorMap& to,
+                const Args& a, cudaStream_t stream);
 int launch_rows(bool dx, const Plan& plan, const CUtensorMap& ta, const CUtensorMap& tw, const Args& a,
                 cudaStream_t stream);
 

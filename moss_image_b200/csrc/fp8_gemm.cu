@@ -32,10 +32,12 @@ constexpr int kThreads = (kEpiWarp0 + kEpiWarps) * 32;
 // (producer and issuer) gives its share to the two that hold 128 sums and two loads in flight a thread.
 constexpr int kIssueRegs = 40, kEpiRegs = 232;
 static_assert(kIssueRegs + 2 * kEpiRegs <= 3 * 168, "a larger split would wait forever");
-constexpr int kStages = 6;
+constexpr int kStages = 4;
 constexpr uint32_t kTileBytes = kHalf * kBlock;      // 16 KB: 128 rows of 128 bytes
 constexpr uint32_t kStageBytes = 2 * kTileBytes;     // A rows and W columns
-constexpr uint32_t kDataBytes = kStages * kStageBytes;
+constexpr uint32_t kOutBytes = 32 * 64 * 2;          // one store box: 32 rows of 64 16-bit outputs
+constexpr uint32_t kRingBytes = kStages * kStageBytes;
+constexpr uint32_t kDataBytes = kRingBytes + kEpiWarps * 2 * kOutBytes;
 constexpr uint32_t kSmemBytes = kDataBytes + 1024 + 512;
 // The final wait for the peer outlasts every other bounded wait of the pair (each gives up within
 // kWaitBudgetCycles, the drain of the ring within kStages more).
@@ -66,62 +68,51 @@ __device__ __forceinline__ void tmem_wait_ld_of(uint32_t (&r)[32]) {
                : "memory");
 }
 
-// Bias and the rounded store of 32 consecutive outputs of one row.
-__device__ __forceinline__ void store32(const Args& args, float (&v)[32], int row, int col0, bool vec_ok) {
-  if (args.bias != nullptr) {
-    const uint16_t* b16 = static_cast<const uint16_t*>(args.bias) + col0;
-    if (args.bias_kind != kF32 && col0 + 32 <= args.Nc && (reinterpret_cast<uintptr_t>(b16) & 15) == 0) {
+// Bias of 32 consecutive outputs of one row.
+__device__ __forceinline__ void add_bias32(const Args& args, float (&v)[32], int col0) {
+  const uint16_t* b16 = static_cast<const uint16_t*>(args.bias) + col0;
+  if (args.bias_kind != kF32 && col0 + 32 <= args.Nc && (reinterpret_cast<uintptr_t>(b16) & 15) == 0) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint4 u = __ldg(reinterpret_cast<const uint4*>(b16) + i);
-        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+    for (int i = 0; i < 4; ++i) {
+      const uint4 u = __ldg(reinterpret_cast<const uint4*>(b16) + i);
+      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          if (args.bias_kind == kBF16) {
-            v[8 * i + 2 * k] += __uint_as_float(w[k] << 16);
-            v[8 * i + 2 * k + 1] += __uint_as_float(w[k] & 0xFFFF0000u);
-          } else {
-            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[k]));
-            v[8 * i + 2 * k] += f.x;
-            v[8 * i + 2 * k + 1] += f.y;
-          }
+      for (int k = 0; k < 4; ++k) {
+        if (args.bias_kind == kBF16) {
+          v[8 * i + 2 * k] += __uint_as_float(w[k] << 16);
+          v[8 * i + 2 * k + 1] += __uint_as_float(w[k] & 0xFFFF0000u);
+        } else {
+          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[k]));
+          v[8 * i + 2 * k] += f.x;
+          v[8 * i + 2 * k + 1] += f.y;
         }
       }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 32; ++j)
-        if (col0 + j < args.Nc) v[j] += load_as_float(args.bias, args.bias_kind, col0 + j);
     }
-  }
-  const int64_t off = static_cast<int64_t>(row) * args.Nc + col0;
-  if (vec_ok && col0 + 32 <= args.Nc) {
-    uint32_t p0[8], p1[8];
-    if (args.out_kind == kBF16) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        p0[j] = gemm::pack2_kind<kBF16>(v[2 * j], v[2 * j + 1]);
-        p1[j] = gemm::pack2_kind<kBF16>(v[16 + 2 * j], v[16 + 2 * j + 1]);
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        p0[j] = gemm::pack2_kind<kF16>(v[2 * j], v[2 * j + 1]);
-        p1[j] = gemm::pack2_kind<kF16>(v[16 + 2 * j], v[16 + 2 * j + 1]);
-      }
-    }
-    uint16_t* dst = static_cast<uint16_t*>(args.out) + off;
-    gemm::stg256(dst, p0);
-    gemm::stg256(dst + 16, p1);
   } else {
 #pragma unroll
     for (int j = 0; j < 32; ++j)
-      if (col0 + j < args.Nc) store_from_float(args.out, args.out_kind, off + j, v[j]);
+      if (col0 + j < args.Nc) v[j] += load_as_float(args.bias, args.bias_kind, col0 + j);
+  }
+}
+
+// 32 outputs of row `lane`, rounded, as chunks 4 h .. 4 h + 3 of a store box (128-byte swizzle).
+template <int kKind>
+__device__ __forceinline__ void stage32(uint32_t box, int lane, int h, const float (&v)[32]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    uint4 w;
+    w.x = gemm::pack2_kind<kKind>(v[8 * i], v[8 * i + 1]);
+    w.y = gemm::pack2_kind<kKind>(v[8 * i + 2], v[8 * i + 3]);
+    w.z = gemm::pack2_kind<kKind>(v[8 * i + 4], v[8 * i + 5]);
+    w.w = gemm::pack2_kind<kKind>(v[8 * i + 6], v[8 * i + 7]);
+    gemm::sts128(box + lane * 128 + (((4 * h + i) ^ (lane & 7)) << 4), w);
   }
 }
 
 template <bool kDX, int kCtas>
 __global__ void __launch_bounds__(kThreads, 1)
-    fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_w, const Args args) {
+    fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_w,
+                    const __grid_constant__ CUtensorMap tm_out, const Args args) {
   constexpr int kTileM = kHalf * kCtas;
   constexpr int kTileN = kHalf * kCtas;
   constexpr int kCols = kTileN / 2;  // accumulator columns of one epilogue thread
@@ -302,7 +293,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t lane_addr = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(half * kCols);
     // acc_empty[0] of the leader, as this CTA sees it; acc_empty[1] is 8 bytes further
     const uint32_t release = kCtas == 2 ? mapa_shared(bar(bars->acc_empty[0]), 0) : bar(bars->acc_empty[0]);
-    const bool vec_ok = args.out_kind != kF32 && (args.Nc & 15) == 0 && (reinterpret_cast<uintptr_t>(args.out) & 31) == 0;
+    const uint32_t boxes = base + kRingBytes + (warp - kEpiWarp0) * 2 * kOutBytes;
     int it = 0;
     bool ok = true;
     for (int u = first_unit; u < num_units && ok; u += unit_step) {
@@ -371,24 +362,52 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (ok && kb + 1 < kb1) ok = add_block(1);
       }
       if (!ok) break;
-      if (row >= args.M) continue;
+      const bool staged = args.tma_out != 0 && args.splits == 1;
+      if (staged) {  // the boxes' last stores have been read
+        if (lane == 0) bulk_wait_read();
+        __syncwarp();
+      }
 #pragma unroll
       for (int c = 0; c < kCols / 32; ++c) {
         const int col = col0 + c * 32;
-        if (col >= args.Nc) break;
         float v[32];
 #pragma unroll
         for (int j = 0; j < 32; ++j) v[j] = sum[c * 32 + j];
         if (args.splits > 1) {
-          float* dst = args.partial + (static_cast<int64_t>(split) * args.M + row) * args.Nc + col;
+          // by columns: a warp's 32 rows are contiguous
+          float* dst = args.partial + ((static_cast<int64_t>(split) * args.tiles_m * args.tiles_n + tile) * kTileN +
+                                       half * kCols + c * 32) * kTileM + q * 32 + lane;
+#pragma unroll
+          for (int j = 0; j < 32; ++j) dst[j * kTileM] = v[j];
+          continue;
+        }
+        if (args.bias != nullptr) add_bias32(args, v, col);
+        if (staged) {
+          const uint32_t box = boxes + (c >> 1) * kOutBytes;
+          if (args.out_kind == kBF16)
+            stage32<kBF16>(box, lane, c & 1, v);
+          else
+            stage32<kF16>(box, lane, c & 1, v);
+        } else if (row < args.M) {
 #pragma unroll
           for (int j = 0; j < 32; ++j)
-            if (col + j < args.Nc) dst[j] = v[j];
-        } else {
-          store32(args, v, row, col, vec_ok);
+            if (col + j < args.Nc)
+              store_from_float(args.out, args.out_kind, static_cast<int64_t>(row) * args.Nc + col + j, v[j]);
+        }
+      }
+      if (staged) {
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          const int row0 = row - lane;
+#pragma unroll
+          for (int p = 0; p < kCols / 64; ++p)
+            if (row0 < args.M && col0 + p * 64 < args.Nc) tma_store_2d(&tm_out, boxes + p * kOutBytes, col0 + p * 64, row0);
+          bulk_commit();
         }
       }
     }
+    if (lane == 0) bulk_wait();
   }
 
   // Leave together: the leader's MMAs read the peer's shared memory and write its TMEM, and the
@@ -419,7 +438,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 template <bool kDX, int kCtas>
-int launch_typed(const CUtensorMap& ta, const CUtensorMap& tw, const Args& a, cudaStream_t stream) {
+int launch_typed(const CUtensorMap& ta, const CUtensorMap& tw, const CUtensorMap& to, const Args& a, cudaStream_t stream) {
   auto kern = fp8_gemm_kernel<kDX, kCtas>;
   static std::once_flag once;
   static cudaError_t attr_err = cudaSuccess;
@@ -451,16 +470,16 @@ int launch_typed(const CUtensorMap& ta, const CUtensorMap& tw, const Args& a, cu
   const int64_t units = static_cast<int64_t>(a.tiles_m) * a.tiles_n * a.splits;
   cfg.gridDim = dim3(static_cast<unsigned>(kCtas * std::max<int64_t>(1, std::min<int64_t>(units, max_groups))));
   cfg.stream = stream;
-  return check_cuda(cudaLaunchKernelEx(&cfg, kern, ta, tw, a), "fp8_gemm_kernel");
+  return check_cuda(cudaLaunchKernelEx(&cfg, kern, ta, tw, to, a), "fp8_gemm_kernel");
 }
 
 }  // namespace
 
-int launch_gemm(bool dx, const Plan& plan, const CUtensorMap& ta, const CUtensorMap& tw, const Args& a,
-                cudaStream_t stream) {
+int launch_gemm(bool dx, const Plan& plan, const CUtensorMap& ta, const CUtensorMap& tw, const CUtensorMap& to,
+                const Args& a, cudaStream_t stream) {
   if (plan.kind == Plan::kPair)
-    return dx ? launch_typed<true, 2>(ta, tw, a, stream) : launch_typed<false, 2>(ta, tw, a, stream);
-  return dx ? launch_typed<true, 1>(ta, tw, a, stream) : launch_typed<false, 1>(ta, tw, a, stream);
+    return dx ? launch_typed<true, 2>(ta, tw, to, a, stream) : launch_typed<false, 2>(ta, tw, to, a, stream);
+  return dx ? launch_typed<true, 1>(ta, tw, to, a, stream) : launch_typed<false, 1>(ta, tw, to, a, stream);
 }
 
 }  // namespace fp8

@@ -61,7 +61,13 @@ static Layout layout_of(int64_t m, int64_t nc, int64_t kr, const Plan& p) {
   l.codes = 0;
   l.scale = up(static_cast<size_t>(m) * kb * kBlock);
   l.partial = l.scale + up(static_cast<size_t>(kb) * l.row_pitch * 4);
-  l.total = l.partial + (p.splits > 1 ? up(static_cast<size_t>(p.splits) * m * nc * 4) : 0);
+  if (p.splits > 1) {
+    const size_t values = p.kind == Plan::kRows ? static_cast<size_t>(m) * nc
+                                                : static_cast<size_t>(p.tiles_m) * p.tiles_n * 128 * 128;
+    l.total = l.partial + up(values * p.splits * 4);
+  } else {
+    l.total = l.partial;
+  }
   return l;
 }
 
@@ -73,6 +79,37 @@ __global__ void __launch_bounds__(256) join_splits_kernel(const float* __restric
     for (int s = 0; s < splits; ++s) v += __ldg(partial + s * total + i);
     if (bias != nullptr) v += load_as_float(bias, bias_kind, i % nc);
     store_from_float(out, out_kind, i, v);
+  }
+}
+
+// The same for partials by tiles, [split][tile][128 columns][128 rows]: 32 x 32 outputs a CTA, turned
+// through shared memory so that both sides are read and written in rows of 32.
+__global__ void __launch_bounds__(256) join_tiles_kernel(const float* __restrict__ partial, int splits, int m, int nc,
+                                                         int tiles_m, int tiles_n, int group_m, const void* bias,
+                                                         int bias_kind, void* out, int out_kind) {
+  __shared__ float turned[32][33];
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  int m_blk, n_blk;
+  gemm::tile_coords(blockIdx.x, tiles_m, tiles_n, m_blk, n_blk, group_m);
+  const int r0 = static_cast<int>(blockIdx.y) / 4 * 32, c0 = static_cast<int>(blockIdx.y) % 4 * 32;
+  if (m_blk * 128 + r0 >= m || n_blk * 128 + c0 >= nc) return;
+  const int64_t step = static_cast<int64_t>(tiles_m) * tiles_n * 128 * 128;
+  const float* src = partial + (static_cast<int64_t>(blockIdx.x) * 128 + c0) * 128 + r0 + lane;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int c = w + 8 * i;
+    float v = 0.0f;
+    for (int s = 0; s < splits; ++s) v += __ldg(src + s * step + c * 128);
+    turned[c][lane] = v;
+  }
+  __syncthreads();
+  const int col = n_blk * 128 + c0 + lane;
+  if (col >= nc) return;
+  const float b = bias != nullptr ? load_as_float(bias, bias_kind, col) : 0.0f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int row = m_blk * 128 + r0 + w + 8 * i;
+    if (row < m) store_from_float(out, out_kind, static_cast<int64_t>(row) * nc + col, turned[lane][w + 8 * i] + b);
   }
 }
 
@@ -141,7 +178,8 @@ static int run(bool dx, const void* x, int x_dtype, int64_t m, int64_t n, int64_
 
   rc = bind_context();
   if (rc != MOSS_OK) return rc;
-  CUtensorMap ta, tw;
+  CUtensorMap ta, tw, to;
+  memset(&to, 0, sizeof(to));
   memset(&ta, 0, sizeof(ta));
   memset(&tw, 0, sizeof(tw));
   const uint32_t rows_box = plan.kind == Plan::kRows ? plan.tn : 128;
@@ -149,11 +187,18 @@ static int run(bool dx, const void* x, int x_dtype, int64_t m, int64_t n, int64_
                       static_cast<uint64_t>(a.kb) * kBlock, kBlock, rows_box, CU_TENSOR_MAP_SWIZZLE_128B) ||
       !gemm::make_map(&tw, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, codes, k, n, ld, kBlock, 128, CU_TENSOR_MAP_SWIZZLE_128B))
     return fail(MOSS_ERR_CUDA, "the driver refused a tensor map of the fp8 linear");
+  if (plan.kind != Plan::kRows && out_dtype != kF32)
+    a.tma_out = gemm::make_map(&to, out_dtype == kBF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                               2, out, nc, m, static_cast<uint64_t>(nc) * 2, 64, 32, CU_TENSOR_MAP_SWIZZLE_128B);
   rc = launch_quantize_rows(x, x_dtype, m, kr, ws + l.codes, reinterpret_cast<float*>(ws + l.scale), l.row_pitch, stream);
   if (rc != MOSS_OK) return rc;
-  rc = plan.kind == Plan::kRows ? launch_rows(dx, plan, ta, tw, a, stream) : launch_gemm(dx, plan, ta, tw, a, stream);
+  rc = plan.kind == Plan::kRows ? launch_rows(dx, plan, ta, tw, a, stream) : launch_gemm(dx, plan, ta, tw, to, a, stream);
   if (rc != MOSS_OK) return rc;
-  if (plan.splits > 1) {
+  if (plan.splits > 1 && plan.kind != Plan::kRows) {
+    join_tiles_kernel<<<dim3(static_cast<unsigned>(plan.tiles_m * plan.tiles_n), 16), 256, 0, stream>>>(
+        a.partial, plan.splits, a.M, a.Nc, plan.tiles_m, plan.tiles_n, a.group_m, bias, bias_dtype, out, out_dtype);
+    MOSS_CUDA_TRY(cudaGetLastError());
+  } else if (plan.splits > 1) {
     const unsigned grid = static_cast<unsigned>(std::min<int64_t>(ceil_div(m * nc, 256), 8LL * sm_count()));
     join_splits_kernel<<<grid, 256, 0, stream>>>(a.partial, plan.splits, m * nc, a.Nc, bias, bias_dtype, out, out_dtype);
     MOSS_CUDA_TRY(cudaGetLastError());
