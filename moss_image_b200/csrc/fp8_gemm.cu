@@ -35,10 +35,11 @@ static_assert(kIssueRegs + 2 * kEpiRegs <= 3 * 168, "a larger split would wait f
 constexpr int kStages = 4;
 constexpr uint32_t kTileBytes = kHalf * kBlock;      // 16 KB: 128 rows of 128 bytes
 constexpr uint32_t kStageBytes = 2 * kTileBytes;     // A rows and W columns
-constexpr uint32_t kOutBytes = 32 * 64 * 2;          // one store box: 32 rows of 64 16-bit outputs
+constexpr uint32_t kBoxBytes = kHalf * 64 * 2;       // one store box: 128 rows of 64 16-bit outputs
 constexpr uint32_t kRingBytes = kStages * kStageBytes;
-constexpr uint32_t kDataBytes = kRingBytes + kEpiWarps * 2 * kOutBytes;
-constexpr uint32_t kSmemBytes = kDataBytes + 1024 + 512;
+constexpr uint32_t kDataBytes = kRingBytes + 4 * kBoxBytes;
+constexpr uint32_t kBiasBytes = 2 * kHalf * 4;       // f32 bias of each epilogue warpgroup's columns
+constexpr uint32_t kSmemBytes = kDataBytes + kBiasBytes + 1024 + 512;
 // The final wait for the peer outlasts every other bounded wait of the pair (each gives up within
 // kWaitBudgetCycles, the drain of the ring within kStages more).
 constexpr long long kExitBudgetCycles = (kStages + 4) * kWaitBudgetCycles;
@@ -49,6 +50,8 @@ struct Barriers {
   uint64_t empty[kStages];  // local: stage free (MMA commit)
   uint64_t acc_full[2];     // local: block product ready (MMA commit)
   uint64_t acc_empty[2];    // leader: block product taken by every epilogue warp
+  uint64_t out_free[2];     // local, by warpgroup: its store boxes are free and its bias is there
+  uint64_t out_full[2];     // local: its outputs are staged
   uint64_t drain;           // leader: all MMAs retired
   uint64_t exit_bar;        // local: peer finished
   uint32_t tmem_base;
@@ -68,36 +71,9 @@ __device__ __forceinline__ void tmem_wait_ld_of(uint32_t (&r)[32]) {
                : "memory");
 }
 
-// Bias of 32 consecutive outputs of one row.
-__device__ __forceinline__ void add_bias32(const Args& args, float (&v)[32], int col0) {
-  const uint16_t* b16 = static_cast<const uint16_t*>(args.bias) + col0;
-  if (args.bias_kind != kF32 && col0 + 32 <= args.Nc && (reinterpret_cast<uintptr_t>(b16) & 15) == 0) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint4 u = __ldg(reinterpret_cast<const uint4*>(b16) + i);
-      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        if (args.bias_kind == kBF16) {
-          v[8 * i + 2 * k] += __uint_as_float(w[k] << 16);
-          v[8 * i + 2 * k + 1] += __uint_as_float(w[k] & 0xFFFF0000u);
-        } else {
-          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[k]));
-          v[8 * i + 2 * k] += f.x;
-          v[8 * i + 2 * k + 1] += f.y;
-        }
-      }
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 32; ++j)
-      if (col0 + j < args.Nc) v[j] += load_as_float(args.bias, args.bias_kind, col0 + j);
-  }
-}
-
-// 32 outputs of row `lane`, rounded, as chunks 4 h .. 4 h + 3 of a store box (128-byte swizzle).
+// 32 outputs of one row, rounded, as chunks 4 h .. 4 h + 3 of a store box (128-byte swizzle).
 template <int kKind>
-__device__ __forceinline__ void stage32(uint32_t box, int lane, int h, const float (&v)[32]) {
+__device__ __forceinline__ void stage32(uint32_t box, int row, int h, const float (&v)[32]) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     uint4 w;
@@ -105,7 +81,7 @@ __device__ __forceinline__ void stage32(uint32_t box, int lane, int h, const flo
     w.y = gemm::pack2_kind<kKind>(v[8 * i + 2], v[8 * i + 3]);
     w.z = gemm::pack2_kind<kKind>(v[8 * i + 4], v[8 * i + 5]);
     w.w = gemm::pack2_kind<kKind>(v[8 * i + 6], v[8 * i + 7]);
-    gemm::sts128(box + lane * 128 + (((4 * h + i) ^ (lane & 7)) << 4), w);
+    gemm::sts128(box + row * 128 + (((4 * h + i) ^ (row & 7)) << 4), w);
   }
 }
 
@@ -120,7 +96,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_base = smem_u32(smem_raw);
   const uint32_t base = (raw_base + 1023u) & ~1023u;
-  Barriers* bars = reinterpret_cast<Barriers*>(smem_raw + (base - raw_base) + kDataBytes);
+  float* const bias_smem = reinterpret_cast<float*>(smem_raw + (base - raw_base) + kDataBytes);
+  Barriers* bars = reinterpret_cast<Barriers*>(smem_raw + (base - raw_base) + kDataBytes + kBiasBytes);
   auto bar = [&](uint64_t& b) { return smem_u32(&b); };
   volatile int* abort_flag = &bars->abort_flag;
 
@@ -131,6 +108,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int first_unit = blockIdx.x / kCtas;
   const int unit_step = gridDim.x / kCtas;
   const int num_units = args.tiles_m * args.tiles_n * args.splits;
+  // outputs that are rounded here: staged in shared memory, whichever way they leave it
+  const bool staged = args.out_kind != kF32 && args.splits == 1;
+  const gemm::TileWalk walk(args.tiles_m, args.tiles_n, args.group_m);
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
@@ -140,6 +120,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int s = 0; s < 2; ++s) {
       mbar_init(bar(bars->acc_full[s]), 1);
       mbar_init(bar(bars->acc_empty[s]), kCtas * kEpiWarps);
+    }
+    for (int h = 0; h < 2; ++h) {
+      mbar_init(bar(bars->out_free[h]), 1);
+      mbar_init(bar(bars->out_full[h]), 4);
     }
     mbar_init(bar(bars->drain), 1);
     mbar_init(bar(bars->exit_bar), 1);
@@ -175,9 +159,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t phase = 0, used = 0, last_phase = 0;
     bool ok = true;
     for (int u = first_unit; u < num_units && ok; u += unit_step) {
-      const int tile = u / args.splits, split = u - tile * args.splits;
+      const int tile = args.splits == 1 ? u : u / args.splits, split = u - tile * args.splits;
       int m_blk, n_blk;
-      gemm::tile_coords(tile, args.tiles_m, args.tiles_n, m_blk, n_blk, args.group_m);
+      walk.at(tile, m_blk, n_blk);
       const int m0 = m_blk * kTileM + static_cast<int>(rank) * kHalf;
       const int n0 = n_blk * kTileN + static_cast<int>(rank) * kHalf;
       const int kb1 = min(args.kb, (split + 1) * args.kb_per_split);
@@ -232,7 +216,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint32_t phase = 0;
       bool ok = true, issued = false;
       for (int u = first_unit; u < num_units && ok; u += unit_step) {
-        const int split = u % args.splits;
+        const int split = args.splits == 1 ? 0 : u % args.splits;
         const int kb1 = min(args.kb, (split + 1) * args.kb_per_split);
         for (int kb = split * args.kb_per_split; kb < kb1 && ok; ++kb, ++it) {
           const int buf = it & 1;
@@ -284,6 +268,33 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       __syncwarp();
     }
+  } else if (staged) {
+    // ---------------------------------------------------------------- store warps (every CTA)
+    // Warp 2 + h serves epilogue warpgroup h: it brings the bias, and issues the stores, whose queue
+    // would hold an epilogue warp up for a thousand cycles a tile.
+    const int h = warp - 2;
+    int it = 0;
+    for (int u = first_unit; u < num_units; u += unit_step, ++it) {
+      int m_blk, n_blk;
+      walk.at(u, m_blk, n_blk);
+      const int row0 = m_blk * kTileM + static_cast<int>(rank) * kHalf;
+      const int col0 = n_blk * kTileN + h * kCols;
+      for (int j = lane; j < kCols; j += 32)
+        bias_smem[h * kHalf + j] =
+            args.bias != nullptr && col0 + j < args.Nc ? load_as_float(args.bias, args.bias_kind, col0 + j) : 0.0f;
+      if (lane == 0) bulk_wait_read();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(bars->out_free[h]));
+      if (!mbar_wait(bar(bars->out_full[h]), it & 1, abort_flag, args.status, MOSS_STATUS_TIMEOUT_EPILOGUE)) break;
+      if (args.tma_out != 0 && lane == 0) {
+        const uint32_t boxes = base + kRingBytes + h * 2 * kBoxBytes;
+#pragma unroll
+        for (int p = 0; p < kCols / 64; ++p)
+          if (row0 < args.M && col0 + p * 64 < args.Nc) tma_store_2d(&tm_out, boxes + p * kBoxBytes, col0 + p * 64, row0);
+        bulk_commit();
+      }
+    }
+    if (lane == 0) bulk_wait();
   }
   } else {
     // ---------------------------------------------------------------- epilogue (every CTA)
@@ -293,13 +304,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t lane_addr = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(half * kCols);
     // acc_empty[0] of the leader, as this CTA sees it; acc_empty[1] is 8 bytes further
     const uint32_t release = kCtas == 2 ? mapa_shared(bar(bars->acc_empty[0]), 0) : bar(bars->acc_empty[0]);
-    const uint32_t boxes = base + kRingBytes + (warp - kEpiWarp0) * 2 * kOutBytes;
-    int it = 0;
+    const uint32_t boxes = base + kRingBytes + half * 2 * kBoxBytes;
+    int it = 0, tiles_done = 0;
     bool ok = true;
     for (int u = first_unit; u < num_units && ok; u += unit_step) {
-      const int tile = u / args.splits, split = u - tile * args.splits;
+      const int tile = args.splits == 1 ? u : u / args.splits, split = u - tile * args.splits;
       int m_blk, n_blk;
-      gemm::tile_coords(tile, args.tiles_m, args.tiles_n, m_blk, n_blk, args.group_m);
+      walk.at(tile, m_blk, n_blk);
       const int row = m_blk * kTileM + static_cast<int>(rank) * kHalf + q * 32 + lane;
       const int col0 = n_blk * kTileN + half * kCols;  // this thread's columns: all in one weight block
       const int kb0 = split * args.kb_per_split, kb1 = min(args.kb, kb0 + args.kb_per_split);
@@ -362,52 +373,64 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (ok && kb + 1 < kb1) ok = add_block(1);
       }
       if (!ok) break;
-      const bool staged = args.tma_out != 0 && args.splits == 1;
-      if (staged) {  // the boxes' last stores have been read
-        if (lane == 0) bulk_wait_read();
-        __syncwarp();
-      }
+      if (staged && !mbar_wait(bar(bars->out_free[half]), tiles_done & 1, abort_flag, args.status,
+                               MOSS_STATUS_TIMEOUT_EPILOGUE))
+        break;
+      ++tiles_done;
 #pragma unroll
       for (int c = 0; c < kCols / 32; ++c) {
         const int col = col0 + c * 32;
         float v[32];
 #pragma unroll
         for (int j = 0; j < 32; ++j) v[j] = sum[c * 32 + j];
-        if (args.splits > 1) {
+        if (staged) {
+#pragma unroll
+          for (int j = 0; j < 32; j += 4) {
+            const float4 b = *reinterpret_cast<const float4*>(bias_smem + half * kHalf + c * 32 + j);
+            v[j] += b.x;
+            v[j + 1] += b.y;
+            v[j + 2] += b.z;
+            v[j + 3] += b.w;
+          }
+          const uint32_t box = boxes + (c >> 1) * kBoxBytes;
+          if (args.out_kind == kBF16)
+            stage32<kBF16>(box, q * 32 + lane, c & 1, v);
+          else
+            stage32<kF16>(box, q * 32 + lane, c & 1, v);
+        } else if (args.splits > 1) {
           // by columns: a warp's 32 rows are contiguous
           float* dst = args.partial + ((static_cast<int64_t>(split) * args.tiles_m * args.tiles_n + tile) * kTileN +
                                        half * kCols + c * 32) * kTileM + q * 32 + lane;
 #pragma unroll
           for (int j = 0; j < 32; ++j) dst[j * kTileM] = v[j];
-          continue;
-        }
-        if (args.bias != nullptr) add_bias32(args, v, col);
-        if (staged) {
-          const uint32_t box = boxes + (c >> 1) * kOutBytes;
-          if (args.out_kind == kBF16)
-            stage32<kBF16>(box, lane, c & 1, v);
-          else
-            stage32<kF16>(box, lane, c & 1, v);
         } else if (row < args.M) {
 #pragma unroll
-          for (int j = 0; j < 32; ++j)
-            if (col + j < args.Nc)
-              store_from_float(args.out, args.out_kind, static_cast<int64_t>(row) * args.Nc + col + j, v[j]);
+          for (int j = 0; j < 32; ++j) {
+            if (col + j >= args.Nc) break;
+            if (args.bias != nullptr) v[j] += load_as_float(args.bias, args.bias_kind, col + j);
+            static_cast<float*>(args.out)[static_cast<int64_t>(row) * args.Nc + col + j] = v[j];
+          }
         }
       }
-      if (staged) {
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) {
-          const int row0 = row - lane;
+      if (staged && args.tma_out != 0) fence_proxy_async_smem();
+      __syncwarp();
+      if (staged && args.tma_out == 0) {
+        // rows that TMA cannot address (an odd width): the warp writes its own, 64 columns at a time
+        const uint16_t* rows16 = reinterpret_cast<const uint16_t*>(smem_raw + (boxes - raw_base)) + q * 32 * 64;
+        const int row0 = row - lane;
+        for (int i = 0; i < 32 && row0 + i < args.M; ++i) {
+          uint16_t* dst = static_cast<uint16_t*>(args.out) + static_cast<int64_t>(row0 + i) * args.Nc + col0;
 #pragma unroll
-          for (int p = 0; p < kCols / 64; ++p)
-            if (row0 < args.M && col0 + p * 64 < args.Nc) tma_store_2d(&tm_out, boxes + p * kOutBytes, col0 + p * 64, row0);
-          bulk_commit();
+          for (int e = 0; e < kCols / 32; ++e) {
+            const int j = e * 32 + lane, k = j & 63;
+            const uint16_t v16 = rows16[(j >> 6) * (kBoxBytes / 2) + i * 64 + (((k >> 3) ^ (i & 7)) << 3) + (k & 7)];
+            if (col0 + j < args.Nc) dst[j] = v16;
+          }
         }
+        __syncwarp();
       }
+      if (staged && lane == 0) mbar_arrive(bar(bars->out_full[half]));
     }
-    if (lane == 0) bulk_wait();
   }
 
   // Leave together: the leader's MMAs read the peer's shared memory and write its TMEM, and the

@@ -189,7 +189,7 @@ static int run(bool dx, const void* x, int x_dtype, int64_t m, int64_t n, int64_
     return fail(MOSS_ERR_CUDA, "the driver refused a tensor map of the fp8 linear");
   if (plan.kind != Plan::kRows && out_dtype != kF32)
     a.tma_out = gemm::make_map(&to, out_dtype == kBF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
-                               2, out, nc, m, static_cast<uint64_t>(nc) * 2, 64, 32, CU_TENSOR_MAP_SWIZZLE_128B);
+                               2, out, nc, m, static_cast<uint64_t>(nc) * 2, 64, 128, CU_TENSOR_MAP_SWIZZLE_128B);
   rc = launch_quantize_rows(x, x_dtype, m, kr, ws + l.codes, reinterpret_cast<float*>(ws + l.scale), l.row_pitch, stream);
   if (rc != MOSS_OK) return rc;
   rc = plan.kind == Plan::kRows ? launch_rows(dx, plan, ta, tw, a, stream) : launch_gemm(dx, plan, ta, tw, to, a, stream);

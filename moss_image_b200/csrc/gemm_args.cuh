@@ -124,6 +124,34 @@ __device__ __forceinline__ void tile_coords(int t, int tiles_m, int tiles_n, int
   n_blk = r / gsm;
 }
 
+// The same walk without integer division in its calls (about 600 cycles a tile on the path of an
+// epilogue warp): quotients by an f32 reciprocal, put right by one either way.
+struct TileWalk {
+  int tiles_m, group_m, per_group;
+  float inv_group, inv_m, inv_last;
+  __device__ __forceinline__ TileWalk(int tiles_m_, int tiles_n, int group_m_)
+      : tiles_m(tiles_m_), group_m(group_m_), per_group(group_m_ * tiles_n) {
+    const int last = tiles_m % group_m;
+    inv_group = 1.0f / static_cast<float>(per_group);
+    inv_m = 1.0f / static_cast<float>(group_m);
+    inv_last = 1.0f / static_cast<float>(last > 0 ? last : group_m);
+  }
+  static __device__ __forceinline__ int quotient(int a, int b, float inv) {
+    int q = static_cast<int>(static_cast<float>(a) * inv);
+    if (q * b > a) --q;
+    if ((q + 1) * b <= a) ++q;
+    return q;
+  }
+  __device__ __forceinline__ void at(int t, int& m_blk, int& n_blk) const {
+    const int group = quotient(t, per_group, inv_group);
+    const int first_m = group * group_m;
+    const int gsm = min(tiles_m - first_m, group_m);
+    const int r = t - group * per_group;
+    n_blk = quotient(r, gsm, gsm == group_m ? inv_m : inv_last);
+    m_blk = first_m + r - n_blk * gsm;
+  }
+};
+
 // CTA-pair (cta_group::2) launcher, defined in w8a16_gemm_2sm.cu. Builds its own tensor maps;
 // returns MOSS_ERR_UNSUPPORTED (without launching) when the shapes do not fit it.
 int launch_pair(bool dx, int v_kind, bool fast, const Args& a, cudaStream_t stream);
