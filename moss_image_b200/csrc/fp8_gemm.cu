@@ -81,7 +81,9 @@ __device__ __forceinline__ void stage32(uint32_t box, int row, int h, const floa
     w.y = gemm::pack2_kind<kKind>(v[8 * i + 2], v[8 * i + 3]);
     w.z = gemm::pack2_kind<kKind>(v[8 * i + 4], v[8 * i + 5]);
     w.w = gemm::pack2_kind<kKind>(v[8 * i + 6], v[8 * i + 7]);
-    gemm::sts128(box + row * 128 + (((4 * h + i) ^ (row & 7)) << 4), w);
+    // no memory clobber: the next group's bias may be read meanwhile (a proxy fence or a warp barrier follows)
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(box + row * 128 + (((4 * h + i) ^ (row & 7)) << 4)),
+                 "r"(w.x), "r"(w.y), "r"(w.z), "r"(w.w));
   }
 }
 
@@ -384,6 +386,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int j = 0; j < 32; ++j) v[j] = sum[c * 32 + j];
         if (staged) {
+          if (args.bias != nullptr)
 #pragma unroll
           for (int j = 0; j < 32; j += 4) {
             const float4 b = *reinterpret_cast<const float4*>(bias_smem + half * kHalf + c * 32 + j);
