@@ -342,6 +342,14 @@ __device__ __forceinline__ void umma_commit_pair(uint32_t bar) {
   asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
 
+// ---------------------------------------------------------------- programmatic dependent launch
+// Kernels of one call that are launched with launch_dependent (errors.cuh): pdl_trigger lets the next
+// one start its prologue, pdl_wait holds it back until everything before it is done and visible.
+// Both are no-ops in an ordinary launch. A kernel launched that way calls pdl_wait before its
+// first access to global memory, whatever path it takes, so completion stays transitive.
+__device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // ---------------------------------------------------------------- misc
 __device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) {
   uint32_t d;

@@ -46,6 +46,23 @@ inline int bind_context() {
   return rc != MOSS_OK ? rc : check_cuda(cudaSetDevice(device), "cudaSetDevice");
 }
 
+// Launches a kernel that may start while the one before it in the stream ends (it calls pdl_wait).
+template <typename... Params, typename... Args>
+inline int launch_dependent(const char* what, void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem,
+                            cudaStream_t stream, const Args&... args) {
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return check_cuda(cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...), what);
+}
+
 inline int clear_ok() {
   last_error_slot().clear();
   return MOSS_OK;

@@ -223,6 +223,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = bars->tmem_base;
+  pdl_trigger();
+  pdl_wait();
 
   if (warp == 0) {
     // ---------------------------------------------------------------- producer (every CTA)
@@ -281,6 +283,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ---------------------------------------------------------------- MMA issuer (leader)
     if (leader) {
       constexpr uint32_t idesc = umma_idesc_f16(0u, kColumns, kTile, kTile);
+      // descriptors of the first stage; every other differs by multiples of 16 bytes in the address field.
+      // K-major: [2 boxes][128 rows][64 values]; by columns: [2 boxes of 64 columns][128 rows]
+      const uint64_t left0 = umma_desc_sw128(base, 16, 1024);
+      const uint64_t right0 = umma_desc_sw128(base + kTileBytes, kColumns ? kTileBytes / 2 : 16, 1024);
       int stage = 0, it = 0;
       uint32_t phase = 0;
       bool ok = true, issued = false;
@@ -297,15 +303,13 @@ __global__ void __launch_bounds__(kThreads, 1)
             break;
           }
           tc_fence_after();
-          if (lane == 0) {
-            const uint32_t left = base + stage * kStageBytes, right = left + kTileBytes;
+          if (elect_one()) {
+            const uint64_t at_stage = static_cast<uint64_t>(stage) * (kStageBytes >> 4);
 #pragma unroll
             for (int kk = 0; kk < kStep / 16; ++kk) {
-              // K-major: [2 boxes][128 rows][64 values]; by columns: [2 boxes of 64 columns][128 rows]
-              const uint64_t ld = umma_desc_sw128(left + (kk >> 2) * (kTileBytes / 2) + (kk & 3) * 32, 16, 1024);
-              const uint64_t rd = kColumns
-                                      ? umma_desc_sw128(right + kk * 2048, kTileBytes / 2, 1024)
-                                      : umma_desc_sw128(right + (kk >> 2) * (kTileBytes / 2) + (kk & 3) * 32, 16, 1024);
+              const uint32_t rows = ((kk >> 2) * (kTileBytes / 2) + (kk & 3) * 32) >> 4;
+              const uint64_t ld = left0 + at_stage + rows;
+              const uint64_t rd = right0 + at_stage + (kColumns ? (kk * 2048) >> 4 : rows);
               if constexpr (kCtas == 2)
                 umma_f16_pair(d, ld, rd, idesc, (s > 0 || kk > 0) ? 1u : 0u);
               else
@@ -315,13 +319,13 @@ __global__ void __launch_bounds__(kThreads, 1)
               umma_commit_pair_mc(bar(bars->empty[stage]), 0x3);
             else
               umma_commit(bar(bars->empty[stage]));
-            issued = true;
           }
+          issued = true;
           __syncwarp();
           if (++stage == kStages) { stage = 0; phase ^= 1u; }
         }
         if (!ok) break;
-        if (lane == 0) {
+        if (elect_one()) {
           if constexpr (kCtas == 2)
             umma_commit_pair_mc(bar(bars->acc_full[acc]), 0x3);
           else
@@ -417,11 +421,13 @@ int launch_typed(const CUtensorMap& tl, const CUtensorMap& tr, Args a, cudaStrea
   static std::once_flag once;
   static cudaError_t attr_err = cudaSuccess;
   static int max_groups = 0;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = kCtas;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = kSmemBytes;
@@ -449,6 +455,7 @@ int launch_typed(const CUtensorMap& tl, const CUtensorMap& tr, Args a, cudaStrea
   if (units > INT32_MAX) return fail(MOSS_ERR_INVALID_ARGUMENT, "too many matrices to orthogonalize in one call");
   cfg.gridDim = dim3(static_cast<unsigned>(kCtas * std::min<int64_t>(units, max_groups)));
   cfg.stream = stream;
+  cfg.numAttrs = 2;  // the kernel before it in the stream is one of this call
   return check_cuda(cudaLaunchKernelEx(&cfg, kern, tl, tr, a), "ns_gemm_kernel");
 }
 

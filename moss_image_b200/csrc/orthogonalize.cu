@@ -29,17 +29,53 @@ int sm_count() {
 }
 
 constexpr int kThreads = 256;
-constexpr int kNormParts = 64;
+constexpr int kNormParts = 512;       // at most, per matrix
+constexpr int kPartValues = 16384;    // values per part where there are fewer
+
+// 8 consecutive values, by 16-byte loads where `wide` says that every matrix allows them.
+template <int kKind>
+__device__ __forceinline__ void load8(const void* g, int64_t at, int count, bool wide, float (&v)[8]) {
+  if (wide) {
+    if constexpr (kKind == kF32) {
+      const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(g) + at);
+      const float4 a = __ldg(p), b = __ldg(p + 1);
+      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+      v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    } else {
+      const uint4 a = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(g) + at));
+      const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (kKind == kBF16) {
+          v[2 * i] = __uint_as_float(w[i] << 16);
+          v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        } else {
+          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+          v[2 * i] = f.x;
+          v[2 * i + 1] = f.y;
+        }
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = i < count ? load_as_float(g, kKind, at + i) : 0.0f;
+  }
+}
 
 // Sums of squares over equal ranges of a matrix, in f64 (neither overflow nor a loss in long sums).
-__global__ void __launch_bounds__(kThreads) sum_squares_kernel(const void* __restrict__ g, int dtype, int64_t size,
+template <int kKind>
+__global__ void __launch_bounds__(kThreads) sum_squares_kernel(const void* __restrict__ g, int64_t size, bool wide,
                                                                double* __restrict__ parts) {
   const int64_t base = static_cast<int64_t>(blockIdx.y) * size;
-  const int64_t first = size * blockIdx.x / gridDim.x, last = size * (blockIdx.x + 1) / gridDim.x;
+  const int64_t chunks = (size + 7) / 8;
+  const int64_t first = chunks * blockIdx.x / gridDim.x, last = chunks * (blockIdx.x + 1) / gridDim.x;
   double sum = 0.0;
+#pragma unroll 4
   for (int64_t i = first + threadIdx.x; i < last; i += kThreads) {
-    const double v = load_as_float(g, dtype, base + i);
-    sum += v * v;
+    float v[8];
+    load8<kKind>(g, base + i * 8, static_cast<int>(min(static_cast<int64_t>(8), size - i * 8)), wide, v);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) sum += static_cast<double>(v[j]) * v[j];
   }
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
@@ -50,38 +86,117 @@ __global__ void __launch_bounds__(kThreads) sum_squares_kernel(const void* __res
     for (int w = 1; w < kThreads / 32; ++w) sum += warps[w];
     parts[static_cast<int64_t>(blockIdx.y) * gridDim.x + blockIdx.x] = sum;
   }
+  pdl_trigger();
 }
 
-// hi + lo = G * unit / max(|G|, eps), padded with zeros to [rp][cp]; 32 x 32 tiles through shared memory
-// when G is tall (so that both sides are read and written by rows).
-__global__ void __launch_bounds__(kThreads) normalize_kernel(const void* __restrict__ g, int dtype, int r, int c, int rp,
-                                                             int cp, int tall, const double* __restrict__ parts,
-                                                             int num_parts, float eps, float unit, __half* __restrict__ hi,
-                                                             __half* __restrict__ lo) {
-  __shared__ float tile[32][33];
-  const int64_t b = blockIdx.z;
+// unit / max(|G|, eps) from the parts, the same in every warp.
+__device__ __forceinline__ float scale_of(const double* parts, int num_parts, float eps, float unit) {
   double sum = 0.0;
-  for (int p = 0; p < num_parts; ++p) sum += parts[b * num_parts + p];
+  for (int p = threadIdx.x & 31; p < num_parts; p += 32) sum += parts[p];
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
   const float norm = static_cast<float>(sqrt(sum));
-  const float scale = unit / (norm < eps ? eps : norm);  // NaN stays NaN
-  const int i0 = blockIdx.y * 32, j0 = blockIdx.x * 32;
-  const int64_t base = b * r * c;
-  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  for (int k = w; k < 32; k += kThreads / 32) {
-    const int i = tall ? i0 + lane : i0 + k, j = tall ? j0 + k : j0 + lane;
-    float v = 0.0f;
-    if (i < r && j < c)
-      v = load_as_float(g, dtype, base + (tall ? static_cast<int64_t>(j) * r + i : static_cast<int64_t>(i) * c + j));
-    tile[tall ? lane : k][tall ? k : lane] = v * scale;
+  return unit / (norm < eps ? eps : norm);  // NaN stays NaN
+}
+
+__device__ __forceinline__ void split8(const float (&v)[8], float scale, uint4& hi, uint4& lo) {
+  uint32_t h[4], l[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float a = v[2 * i] * scale, b = v[2 * i + 1] * scale;
+    const __half2 p = __floats2half2_rn(a, b);
+    const float2 back = __half22float2(p);
+    const __half2 q = __floats2half2_rn(a - back.x, b - back.y);
+    h[i] = *reinterpret_cast<const uint32_t*>(&p);
+    l[i] = *reinterpret_cast<const uint32_t*>(&q);
+  }
+  hi = make_uint4(h[0], h[1], h[2], h[3]);
+  lo = make_uint4(l[0], l[1], l[2], l[3]);
+}
+
+// hi + lo = G * unit / max(|G|, eps), padded with zeros to [rp][cp]. A CTA: kNormRows rows of 512 columns.
+constexpr int kNormRows = 16;
+template <int kKind>
+__global__ void __launch_bounds__(kThreads) normalize_kernel(const void* __restrict__ g, int r, int c, int rp, int cp,
+                                                             bool wide, const double* __restrict__ parts, int num_parts,
+                                                             float eps, float unit, __half* __restrict__ hi,
+                                                             __half* __restrict__ lo) {
+  pdl_wait();
+  const int64_t b = blockIdx.z;
+  const float scale = scale_of(parts + b * num_parts, num_parts, eps, unit);
+  const int j = blockIdx.x * 512 + (threadIdx.x & 63) * 8;
+  const int i0 = blockIdx.y * kNormRows + (threadIdx.x >> 6);
+  pdl_trigger();
+  if (j >= cp) return;
+  float v[kNormRows / 4][8];
+#pragma unroll
+  for (int k = 0; k < kNormRows / 4; ++k) {
+    const int i = i0 + 4 * k;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[k][e] = 0.0f;
+    if (i < r && j < c) load8<kKind>(g, (b * r + i) * c + j, c - j, wide, v[k]);
+  }
+#pragma unroll
+  for (int k = 0; k < kNormRows / 4; ++k) {
+    uint4 h, l;
+    split8(v[k], scale, h, l);
+    const int64_t at = (b * rp + i0 + 4 * k) * cp + j;
+    *reinterpret_cast<uint4*>(hi + at) = h;
+    *reinterpret_cast<uint4*>(lo + at) = l;
+  }
+}
+
+// The same for a tall G [c][r]: 64 x 64 tiles turned through shared memory, so that both sides move whole rows.
+template <int kKind>
+__global__ void __launch_bounds__(kThreads) normalize_tall_kernel(const void* __restrict__ g, int r, int c, int rp, int cp,
+                                                                  bool wide, const double* __restrict__ parts,
+                                                                  int num_parts, float eps, float unit,
+                                                                  __half* __restrict__ hi, __half* __restrict__ lo) {
+  __shared__ float tile[64][65];
+  pdl_wait();
+  const int64_t b = blockIdx.z;
+  const float scale = scale_of(parts + b * num_parts, num_parts, eps, unit);
+  pdl_trigger();
+  const int i0 = blockIdx.y * 64, j0 = blockIdx.x * 64;
+  const int e = (threadIdx.x & 7) * 8, w = threadIdx.x >> 3;
+#pragma unroll
+  for (int k = w; k < 64; k += kThreads / 8) {  // rows of G
+    float v[8];
+#pragma unroll
+    for (int q = 0; q < 8; ++q) v[q] = 0.0f;
+    if (j0 + k < c && i0 + e < r) load8<kKind>(g, (b * c + j0 + k) * r + i0 + e, r - i0 - e, wide, v);
+#pragma unroll
+    for (int q = 0; q < 8; ++q) tile[e + q][k] = v[q];
   }
   __syncthreads();
-  for (int k = w; k < 32; k += kThreads / 32) {
-    const float v = tile[k][lane];
-    const __half h = __float2half_rn(v);
-    const int64_t at = (b * rp + i0 + k) * cp + j0 + lane;
-    hi[at] = h;
-    lo[at] = __float2half_rn(v - __half2float(h));
+#pragma unroll
+  for (int k = w; k < 64; k += kThreads / 8) {
+    float v[8];
+#pragma unroll
+    for (int q = 0; q < 8; ++q) v[q] = tile[k][e + q];
+    uint4 h, l;
+    split8(v, scale, h, l);
+    const int64_t at = (b * rp + i0 + k) * cp + j0 + e;
+    *reinterpret_cast<uint4*>(hi + at) = h;
+    *reinterpret_cast<uint4*>(lo + at) = l;
   }
+}
+
+// Norms and the padded, scaled operands.
+template <int kKind>
+static int launch_normalize(const void* g, int64_t batch, int r, int c, int rp, int cp, bool tall, float eps, float unit,
+                            double* parts, int num_parts, __half* hi, __half* lo, cudaStream_t stream) {
+  const int64_t size = static_cast<int64_t>(r) * c;
+  const bool aligned = reinterpret_cast<uintptr_t>(g) % 16 == 0;
+  const unsigned z = static_cast<unsigned>(batch);
+  sum_squares_kernel<kKind><<<dim3(num_parts, z), kThreads, 0, stream>>>(g, size, aligned && size % 8 == 0, parts);
+  MOSS_CUDA_TRY(cudaGetLastError());
+  const bool wide = aligned && (tall ? r : c) % 8 == 0;
+  if (tall)
+    return launch_dependent("normalize_tall_kernel", normalize_tall_kernel<kKind>, dim3(cp / 64, rp / 64, z), dim3(kThreads),
+                            0, stream, g, r, c, rp, cp, wide, parts, num_parts, eps, unit, hi, lo);
+  return launch_dependent("normalize_kernel", normalize_kernel<kKind>, dim3((cp + 511) / 512, rp / kNormRows, z),
+                          dim3(kThreads), 0, stream, g, r, c, rp, cp, wide, parts, num_parts, eps, unit, hi, lo);
 }
 
 struct Layout {
@@ -212,16 +327,19 @@ static int run(const void* g, int dtype, int64_t batch, int64_t rows, int64_t co
   const float gain = std::exp2(std::floor(14.0 - std::log2(most)));
   double* parts = reinterpret_cast<double*>(ws + l.parts);
   const int64_t size = rows * cols;
-  const int num_parts = static_cast<int>(std::min<int64_t>(kNormParts, (size + 4095) / 4096));
-  sum_squares_kernel<<<dim3(num_parts, static_cast<unsigned>(batch)), kThreads, 0, stream>>>(g, dtype, size, parts);
-  MOSS_CUDA_TRY(cudaGetLastError());
+  const int num_parts = static_cast<int>(std::max<int64_t>(
+      1, std::min<int64_t>({(size + kPartValues - 1) / kPartValues, kNormParts, 8LL * sm_count() / batch + 1})));
   __half* x[2] = {reinterpret_cast<__half*>(ws + l.x[0]), reinterpret_cast<__half*>(ws + l.x[1])};
   __half* low[2] = {reinterpret_cast<__half*>(ws + l.low[0]), reinterpret_cast<__half*>(ws + l.low[1])};
   __half* ga = reinterpret_cast<__half*>(ws + l.a);
   __half* gb = reinterpret_cast<__half*>(ws + l.b);
-  normalize_kernel<<<dim3(l.cp / 32, l.rp / 32, static_cast<unsigned>(batch)), kThreads, 0, stream>>>(
-      g, dtype, l.r, l.c, l.rp, l.cp, l.tall, parts, num_parts, eps, unit, x[0], low[0]);
-  MOSS_CUDA_TRY(cudaGetLastError());
+  if (dtype == kBF16)
+    rc = launch_normalize<kBF16>(g, batch, l.r, l.c, l.rp, l.cp, l.tall, eps, unit, parts, num_parts, x[0], low[0], stream);
+  else if (dtype == kF16)
+    rc = launch_normalize<kF16>(g, batch, l.r, l.c, l.rp, l.cp, l.tall, eps, unit, parts, num_parts, x[0], low[0], stream);
+  else
+    rc = launch_normalize<kF32>(g, batch, l.r, l.c, l.rp, l.cp, l.tall, eps, unit, parts, num_parts, x[0], low[0], stream);
+  if (rc != MOSS_OK) return rc;
   const int with_low = std::max(1, steps - 2);  // steps whose a X term reads lo
   for (int i = 0; i < steps; ++i) {
     const float* k = coefficients + 3 * i;
