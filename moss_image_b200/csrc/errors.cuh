@@ -4,6 +4,7 @@
 
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstdarg>
 #include <cstdio>
 #include <string>
@@ -35,6 +36,23 @@ inline int fail(int code, const char* fmt, ...) {
 inline int check_cuda(cudaError_t e, const char* what) {
   if (e == cudaSuccess) return MOSS_OK;
   return fail(MOSS_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
+}
+
+// SMs of the current device (148, a B200's, where there is none), asked for once per device.
+inline int device_sm_count() {
+  static std::atomic<int> known[64];
+  int device = 0, n = 0;
+  if (cudaGetDevice(&device) != cudaSuccess || device < 0) {
+    cudaGetLastError();
+    return 148;
+  }
+  if (device < 64 && (n = known[device].load(std::memory_order_relaxed)) > 0) return n;
+  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess || n <= 0) {
+    cudaGetLastError();
+    return 148;
+  }
+  if (device < 64) known[device].store(n, std::memory_order_relaxed);
+  return n;
 }
 
 // Makes the current device's context current on this thread, as a kernel launch would. A thread

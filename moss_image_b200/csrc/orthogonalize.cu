@@ -21,12 +21,7 @@
 namespace moss {
 namespace ns {
 
-int sm_count() {
-  int dev = 0, n = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return 148;
-  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) return 148;
-  return n;
-}
+int sm_count() { return device_sm_count(); }
 
 constexpr int kThreads = 256;
 constexpr int kNormParts = 512;       // at most, per matrix

@@ -18,6 +18,7 @@ CUDA tensors only: there is no CPU path and no fallback.
 from __future__ import annotations
 
 import ctypes
+import math
 from functools import lru_cache
 
 import torch
@@ -102,21 +103,24 @@ def _workspace_bytes(m: int, n_out: int, k_red: int) -> int:
     return size.value
 
 
-def _check(tokens: torch.Tensor, weight: torch.Tensor, scale: torch.Tensor, width: int, what: str) -> None:
-    if not tokens.is_cuda:
+def _check(tokens: torch.Tensor, weight: torch.Tensor, scale: torch.Tensor, side: int, what: str) -> None:
+    """``side``: the weight dimension that the input's last one has to match."""
+    device = tokens.device
+    if device.type != "cuda":
         raise RuntimeError(f"{what} runs on CUDA tensors only (there is no CPU path).")
     if tokens.dtype not in _FLOATS:
         raise ValueError(f"{what}: the input must be float16, bfloat16 or float32.")
-    if weight.device != tokens.device or scale.device != tokens.device:
+    if weight.device != device or scale.device != device:
         raise ValueError(f"{what}: the weight and its scales must be on the input's device.")
     if weight.dtype != torch.float8_e4m3fn or weight.ndim != 2 or scale.dtype != torch.float32:
         raise ValueError(f"{what}: the weight must be float8_e4m3fn [out, in] with float32 scales.")
     n, k = weight.shape
-    if tuple(scale.shape) != (_blocks(n), _blocks(k)) or not scale.is_contiguous():
+    if scale.shape != (_blocks(n), _blocks(k)) or not scale.is_contiguous():
         raise ValueError(f"{what}: the scales must be a contiguous [ceil(out / 128), ceil(in / 128)] tensor.")
-    if tokens.ndim < 1 or tokens.shape[-1] != width:
-        raise ValueError(f"{what}: the input's last dimension must be {width}.")
-    if weight.numel() and (weight.stride(1) != 1 or weight.stride(0) % 16 or weight.stride(0) < k or weight.data_ptr() % 16):
+    if tokens.ndim < 1 or tokens.shape[-1] != (n, k)[side]:
+        raise ValueError(f"{what}: the input's last dimension must be {(n, k)[side]}.")
+    pitch, step = weight.stride()
+    if n and k and (step != 1 or pitch % 16 or pitch < k or weight.data_ptr() % 16):
         raise ValueError(f"{what}: the weight's rows must be 16-byte aligned (lay_out_fp8_codes).")
 
 
@@ -132,10 +136,7 @@ def _output(tokens: torch.Tensor, width: int, dtype: torch.dtype, out: torch.Ten
 
 
 def _rows(tokens: torch.Tensor) -> int:
-    rows = 1
-    for size in tokens.shape[:-1]:
-        rows *= size
-    return rows
+    return tokens.shape[0] if tokens.ndim == 2 else math.prod(tokens.shape[:-1])
 
 
 def fp8_linear_forward(tokens: torch.Tensor, weight: torch.Tensor, scale: torch.Tensor,
@@ -143,7 +144,7 @@ def fp8_linear_forward(tokens: torch.Tensor, weight: torch.Tensor, scale: torch.
                        out: torch.Tensor | None = None) -> torch.Tensor:
     """``Y = q(X) dec(W)^T (+ bias)`` for ``[..., in]`` tokens; ``output_dtype`` defaults to the tokens' own."""
     what = "fp8_linear_forward"
-    _check(tokens, weight, scale, weight.shape[-1], what)
+    _check(tokens, weight, scale, 1, what)
     n, k = weight.shape
     if bias is not None and (bias.device != tokens.device or tuple(bias.shape) != (n,) or bias.dtype not in _FLOATS
                              or not bias.is_contiguous()):
@@ -169,7 +170,7 @@ def fp8_linear_backward(gradient: torch.Tensor, weight: torch.Tensor, scale: tor
                         output_dtype: torch.dtype | None = None, *, out: torch.Tensor | None = None) -> torch.Tensor:
     """``dX = q(dY) dec(W)`` for ``[..., out]`` gradients, from the same ``[out, in]`` codes."""
     what = "fp8_linear_backward"
-    _check(gradient, weight, scale, weight.shape[0], what)
+    _check(gradient, weight, scale, 0, what)
     n, k = weight.shape
     device = gradient.device
     status = status_buffer(device)

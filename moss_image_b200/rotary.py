@@ -94,8 +94,8 @@ def _launch(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor, sin: torch.Tens
             interleaved: bool, inverse: bool) -> tuple[torch.Tensor, torch.Tensor]:
     q4, k4 = _heads_view("q", q), _heads_view("k", k)
     batch, tokens, q_heads, head_dim = q4.shape
-    q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
     qs, ks = q4.stride(), k4.stride()
     rc = _lib.library().moss_rotary(
         q4.data_ptr(), qs[0], qs[1], qs[2], q_heads, k4.data_ptr(), ks[0], ks[1], ks[2], k4.shape[2],
