@@ -37,6 +37,7 @@ struct Small {
   int dtype;
   int64_t batch;
   int r, c, tall, steps;
+  int wide, out_wide;  // 4-value reads of G's rows, 4- or 8-value (tall) writes of the result's are aligned and whole
   float coefficients[3 * kMaxSteps];
   float eps;
   __nv_bfloat16* out;
@@ -45,7 +46,7 @@ struct Small {
   float* q;        // [batch][side * side], transposed
 };
 int small_side(int r);
-int small_chunks(int64_t batch, int c, int sms);
+int small_chunks(int64_t batch, int r, int c, int sms);
 int launch_small(const Small& s, cudaStream_t stream);
 
 int sm_count();

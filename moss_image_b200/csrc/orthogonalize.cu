@@ -214,7 +214,7 @@ static Layout layout_of(int64_t batch, int64_t rows, int64_t cols) {
   };
   if (l.small) {
     l.side = small_side(l.r);
-    l.chunks = small_chunks(batch, l.c, sm_count());
+    l.chunks = small_chunks(batch, l.r, l.c, sm_count());
     const size_t square = static_cast<size_t>(l.side) * l.side * 4 * batch;
     l.partial = take(square * l.chunks);
     l.q = take(square);
@@ -305,6 +305,9 @@ static int run(const void* g, int dtype, int64_t batch, int64_t rows, int64_t co
     s.c = l.c;
     s.tall = l.tall;
     s.steps = steps;
+    const int64_t inner = l.tall ? l.r : l.c;
+    s.wide = inner % 4 == 0 && reinterpret_cast<uintptr_t>(g) % 16 == 0;
+    s.out_wide = inner % (l.tall ? 8 : 4) == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0;
     std::memcpy(s.coefficients, coefficients, sizeof(float) * 3 * steps);
     s.eps = eps;
     s.out = out;
