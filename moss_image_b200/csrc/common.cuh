@@ -345,8 +345,9 @@ __device__ __forceinline__ void umma_commit_pair(uint32_t bar) {
 // ---------------------------------------------------------------- programmatic dependent launch
 // Kernels of one call that are launched with launch_dependent (errors.cuh): pdl_trigger lets the next
 // one start its prologue, pdl_wait holds it back until everything before it is done and visible.
-// Both are no-ops in an ordinary launch. A kernel launched that way calls pdl_wait before its
-// first access to global memory, whatever path it takes, so completion stays transitive.
+// Both are no-ops in an ordinary launch. Every kernel launched that way calls pdl_wait, whatever
+// path it takes, so that completion stays transitive; before it, it reads nothing that the
+// call's earlier kernels write and writes nothing at all.
 __device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
