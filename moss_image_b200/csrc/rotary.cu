@@ -11,6 +11,7 @@
 // so the f32 table costs L1 traffic once per kHeads heads and DRAM traffic once per token.
 #include <algorithm>
 #include <cstdint>
+#include <type_traits>
 
 #include "common.cuh"
 #include "errors.cuh"
@@ -20,6 +21,23 @@ namespace rotary {
 
 constexpr int kThreads = 256;
 constexpr int kHeads = 4;  // heads per thread: independent 16-byte loads in flight
+
+// n / d for 0 <= n < 2^31 by a multiplication (Granlund and Montgomery, 1994).
+struct Divisor {
+  uint32_t d, mul;
+  int shift;
+};
+static Divisor divisor(int d) {
+  Divisor v;
+  v.d = static_cast<uint32_t>(d);
+  v.shift = 0;
+  while ((1ll << v.shift) < d) ++v.shift;
+  v.mul = static_cast<uint32_t>(((1ull << 32) * ((1ull << v.shift) - v.d)) / v.d + 1);
+  return v;
+}
+__device__ __forceinline__ int quotient(int n, const Divisor& v) {
+  return static_cast<int>((__umulhi(static_cast<uint32_t>(n), v.mul) + static_cast<uint32_t>(n)) >> v.shift);
+}
 
 struct Part {  // the queries or the keys
   const void* in;
@@ -39,32 +57,55 @@ struct Args {
   int head_dim, half;
   int chunks, turned;  // work items of one head: all, and those that hold pairs
   int items;           // work items of one token
+  Divisor by_chunks, by_items, by_tokens;
   int rows_per_block;
   int inverse;
-};
-
-template <typename T>
-struct Wide;
-template <>
-struct Wide<__nv_bfloat16> {
-  static __device__ __forceinline__ float get(__nv_bfloat16 v) { return __bfloat162float(v); }
-  static __device__ __forceinline__ __nv_bfloat16 put(float v) { return __float2bfloat16_rn(v); }
-};
-template <>
-struct Wide<__half> {
-  static __device__ __forceinline__ float get(__half v) { return __half2float(v); }
-  static __device__ __forceinline__ __half put(float v) { return __float2half_rn(v); }
-};
-template <>
-struct Wide<float> {
-  static __device__ __forceinline__ float get(float v) { return v; }
-  static __device__ __forceinline__ float put(float v) { return v; }
 };
 
 template <typename T, int N>
 struct alignas(sizeof(T) * N) Vec {
   T v[N];
 };
+
+// To and from f32, pairs by packed conversions (one by one they are a third of the kernel's time).
+template <typename T, int N>
+__device__ __forceinline__ void widen(const Vec<T, N>& x, float (&f)[N]) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) f[i] = x.v[i];
+  } else if constexpr (N == 1) {
+    f[0] = static_cast<float>(x.v[0]);
+  } else {
+    using P = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) {
+      const P p = reinterpret_cast<const P*>(x.v)[i];
+      f[2 * i] = __low2float(p);
+      f[2 * i + 1] = __high2float(p);
+    }
+  }
+}
+template <typename T, int N>
+__device__ __forceinline__ void narrow(const float (&f)[N], Vec<T, N>& x) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) x.v[i] = f[i];
+  } else if constexpr (N == 1) {
+    if constexpr (std::is_same<T, __half>::value)
+      x.v[0] = __float2half_rn(f[0]);
+    else
+      x.v[0] = __float2bfloat16_rn(f[0]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) {
+      if constexpr (std::is_same<T, __half>::value)
+        reinterpret_cast<__half2*>(x.v)[i] = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+      else
+        reinterpret_cast<__nv_bfloat162*>(x.v)[i] = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+    }
+  }
+}
+
 
 // kVec values per access; a chunk of pairs covers kVec values (interleaved) or kVec values of
 // each half (half layout).
@@ -76,12 +117,12 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const Args args) {
   const int row0 = static_cast<int>(blockIdx.x) * args.rows_per_block;
   const int rows_here = min(args.rows_per_block, args.rows - row0);
   for (int it = threadIdx.x; it < rows_here * args.items; it += kThreads) {
-    const int r = it / args.items;
+    const int r = quotient(it, args.by_items);
     const int w = it - r * args.items;
     const int row = row0 + r;
-    const int b = row / args.tokens;
+    const int b = quotient(row, args.by_tokens);
     const int s = row - b * args.tokens;
-    const int g = w / args.chunks;
+    const int g = quotient(w, args.by_chunks);
     const int c = w - g * args.chunks;
     const bool keys = g >= args.part[0].groups;
     const Part& p = args.part[keys ? 1 : 0];
@@ -128,21 +169,26 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const Args args) {
     for (int j = 0; j < kHeads; ++j) {
       if (j >= n) continue;
       T* dst = out + j * args.head_dim;
+      float x[kVec], y[kVec];
+      widen(lo[j], x);
       if constexpr (kInterleaved && !kSplitPair) {
 #pragma unroll
         for (int i = 0; i < kAngles; ++i) {
-          const float x = Wide<T>::get(lo[j].v[2 * i]), y = Wide<T>::get(lo[j].v[2 * i + 1]);
-          lo[j].v[2 * i] = Wide<T>::put(x * co.v[i] - y * si.v[i]);
-          lo[j].v[2 * i + 1] = Wide<T>::put(x * si.v[i] + y * co.v[i]);
+          y[2 * i] = x[2 * i] * co.v[i] - x[2 * i + 1] * si.v[i];
+          y[2 * i + 1] = x[2 * i] * si.v[i] + x[2 * i + 1] * co.v[i];
         }
+        narrow(y, lo[j]);
         *reinterpret_cast<Vec<T, kVec>*>(dst + first) = lo[j];
       } else {
+        widen(hi[j], y);
 #pragma unroll
         for (int i = 0; i < kAngles; ++i) {
-          const float x = Wide<T>::get(lo[j].v[i]), y = Wide<T>::get(hi[j].v[i]);
-          lo[j].v[i] = Wide<T>::put(x * co.v[i] - y * si.v[i]);
-          hi[j].v[i] = Wide<T>::put(x * si.v[i] + y * co.v[i]);
+          const float a = x[i], b2 = y[i];
+          x[i] = a * co.v[i] - b2 * si.v[i];
+          y[i] = a * si.v[i] + b2 * co.v[i];
         }
+        narrow(x, lo[j]);
+        narrow(y, hi[j]);
         *reinterpret_cast<Vec<T, kVec>*>(dst + first) = lo[j];
         *reinterpret_cast<Vec<T, kVec>*>(dst + second) = hi[j];
       }
@@ -155,6 +201,9 @@ static int launch(Args a, bool interleaved, int rotary_dim, cudaStream_t stream)
   a.turned = interleaved ? (kVec == 1 ? a.half : rotary_dim / kVec) : a.half / kVec;
   a.chunks = a.turned + (a.head_dim - rotary_dim) / kVec;
   a.items = (a.part[0].groups + a.part[1].groups) * a.chunks;
+  a.by_chunks = divisor(a.chunks);
+  a.by_items = divisor(a.items);
+  a.by_tokens = divisor(a.tokens);
   // about four work items per thread and block, fewer when that would leave SMs without a block
   const int64_t want = std::max<int64_t>(1, 4 * kThreads / a.items);
   a.rows_per_block = static_cast<int>(std::min<int64_t>(want, std::max<int64_t>(1, a.rows / 592)));
