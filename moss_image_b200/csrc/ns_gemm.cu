@@ -2,7 +2,7 @@
 //
 // Two shapes of one kernel: a CTA pair on 256 x 256 tiles where those fill the GPU, one CTA on
 // 128 x 128 tiles where they do not. Warp 0 streams 128-wide reduction steps by TMA (one box of
-// 32 KB per operand), warp 1 issues the MMAs into one of two TMEM accumulators, warps 2-5 drain the
+// 32 KB per operand), warp 1 issues the MMAs into one of two TMEM accumulators, warps 2-9 drain the
 // other. A and B are symmetric: only tiles on and above the diagonal are computed, and written
 // twice; both orders of a diagonal tile's products sum alike, so A and B stay symmetric bit for
 // bit, and the update may read B by rows. X is read by columns there (MN-major), from the same
@@ -25,7 +25,8 @@ constexpr int kHalf = 128;
 constexpr int kStep = 128;  // reduction indices per stage: two 64-wide boxes
 constexpr int kStages = 3;
 constexpr int kEpiWarp0 = 2;
-constexpr int kThreads = 6 * 32;
+constexpr int kEpiWarps = 8;  // two per quarter of the lanes, each with half of the columns
+constexpr int kThreads = (kEpiWarp0 + kEpiWarps) * 32;
 constexpr uint32_t kTileBytes = kHalf * kStep * 2;  // 32 KB
 constexpr uint32_t kStageBytes = 2 * kTileBytes;
 constexpr uint32_t kDataBytes = kStages * kStageBytes;
@@ -80,11 +81,28 @@ __device__ __forceinline__ void locate(const Args& a, int u, int& b, int& m, int
   }
 }
 
-__device__ __forceinline__ void load32(const __half* p, float (&v)[32]) {
+// 32 consecutive values of the operand that is added to a tile's row, as they are stored. They do not depend
+// on the products, so they are on their way before the accumulator is done (one at a time after it, they
+// took half of a small tile's life).
+struct Added {
+  uint4 hi[4], lo[4];
+};
+template <Mode kMode>
+__device__ __forceinline__ void fetch32(const Args& a, int b, int i, int j, Added& x) {
+  const int cols = kMode == kUpdate ? a.cp : a.rp;
+  if (kMode == kGram || i >= a.rp || j >= cols) return;
+  const int64_t at = (static_cast<int64_t>(b) * a.rp + i) * cols + j;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) x.hi[e] = __ldg(reinterpret_cast<const uint4*>(a.add_hi + at) + e);
+  if (kMode == kUpdate && a.add_lo != nullptr) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x.lo[e] = __ldg(reinterpret_cast<const uint4*>(a.add_lo + at) + e);
+  }
+}
+__device__ __forceinline__ void widen32(const uint4 (&w)[4], float (&v)[32]) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const uint4 w = __ldg(reinterpret_cast<const uint4*>(p) + i);
-    const uint32_t h[4] = {w.x, w.y, w.z, w.w};
+    const uint32_t h[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[j]));
@@ -106,14 +124,15 @@ __device__ __forceinline__ void store32(__half* p, const float (&v)[32]) {
 
 // 32 consecutive accumulators of one row through the mode's epilogue. i, j: row and first column.
 template <Mode kMode>
-__device__ __forceinline__ void finish32(const Args& a, int b, int i, int j, bool mirror, float (&v)[32]) {
+__device__ __forceinline__ void finish32(const Args& a, int b, int i, int j, bool mirror, const Added& added,
+                                         float (&v)[32]) {
   if constexpr (kMode == kUpdate) {
     const int64_t at = (static_cast<int64_t>(b) * a.rp + i) * a.cp + j;
     float x[32];
-    load32(a.add_hi + at, x);
+    widen32(added.hi, x);
     if (a.add_lo != nullptr) {
       float lo[32];
-      load32(a.add_lo + at, lo);
+      widen32(added.lo, lo);
 #pragma unroll
       for (int e = 0; e < 32; ++e) x[e] += lo[e];
     }
@@ -156,7 +175,7 @@ __device__ __forceinline__ void finish32(const Args& a, int b, int i, int j, boo
     const int64_t at = base + static_cast<int64_t>(i) * a.rp + j;
     if constexpr (kMode == kSquare) {
       float x[32];
-      load32(a.add_hi + at, x);
+      widen32(added.hi, x);
 #pragma unroll
       for (int e = 0; e < 32; ++e) v[e] = fmaf(a.beta, x[e], a.alpha * v[e]);
     } else {
@@ -200,7 +219,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int s = 0; s < 2; ++s) {
       mbar_init(bar(bars->acc_full[s]), 1);
-      mbar_init(bar(bars->acc_empty[s]), kCtas * 4);
+      mbar_init(bar(bars->acc_empty[s]), kCtas * kEpiWarps);
     }
     mbar_init(bar(bars->drain), 1);
     mbar_init(bar(bars->exit_bar), 1);
@@ -350,25 +369,31 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else {
     // ---------------------------------------------------------------- epilogue (every CTA)
+    constexpr int kGroups = kTile / 2 / 32;  // groups of 32 columns of one warp
     const int q = warp & 3;
+    const int half = (warp - kEpiWarp0) >> 2;
+    const uint32_t lane_addr = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(half * (kTile / 2));
+    const int cols = kMode == kUpdate ? args.cp : args.rp;
     int it = 0;
     for (int u = first_unit; u < num_units; u += unit_step, ++it) {
+      int b, m, n;
+      locate<kMode>(args, u, b, m, n);
+      const int i = m * kTile + static_cast<int>(rank) * kHalf + q * 32 + lane;
+      const int j0 = n * kTile + half * (kTile / 2);
+      Added added[2];
+      fetch32<kMode>(args, b, i, j0, added[0]);
+      fetch32<kMode>(args, b, i, j0 + 32, added[1]);
       const int acc = it & 1;
       if (!mbar_wait_cluster(bar(bars->acc_full[acc]), (it >> 1) & 1, abort_flag, args.status,
                              MOSS_STATUS_TIMEOUT_EPILOGUE))
         break;
       tc_fence_after();
-      int b, m, n;
-      locate<kMode>(args, u, b, m, n);
-      const int i = m * kTile + static_cast<int>(rank) * kHalf + q * 32 + lane;
-      const int cols = kMode == kUpdate ? args.cp : args.rp;
-#pragma unroll 1
-      for (int c = 0; c < kTile / 32; ++c) {
+#pragma unroll
+      for (int c = 0; c < kGroups; ++c) {
         uint32_t r[32];
-        tmem_ld_32x32b_x32(tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(acc * kTile + c * 32),
-                           r);
+        tmem_ld_32x32b_x32(lane_addr + static_cast<uint32_t>(acc * kTile + c * 32), r);
         tmem_wait_ld();
-        if (c == kTile / 32 - 1) {
+        if (c == kGroups - 1) {
           tc_fence_before();
           __syncwarp();
           if (lane == 0) {
@@ -379,12 +404,14 @@ __global__ void __launch_bounds__(kThreads, 1)
               mbar_arrive_cluster(mapa_shared(eb, 0));
           }
         }
-        const int j = n * kTile + c * 32;
-        if (i >= args.rp || j >= cols) continue;  // past this matrix: the next one's rows, or nothing
-        float v[32];
+        const int j = j0 + c * 32;
+        if (i < args.rp && j < cols) {  // otherwise past this matrix: the next one's rows, or nothing
+          float v[32];
 #pragma unroll
-        for (int e = 0; e < 32; ++e) v[e] = __uint_as_float(r[e]);
-        finish32<kMode>(args, b, i, j, m != n, v);
+          for (int e = 0; e < 32; ++e) v[e] = __uint_as_float(r[e]);
+          finish32<kMode>(args, b, i, j, m != n, added[c & 1], v);
+        }
+        if (c + 2 < kGroups) fetch32<kMode>(args, b, i, j + 64, added[c & 1]);
       }
     }
   }
