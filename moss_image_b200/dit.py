@@ -15,7 +15,9 @@ swapped or streamed with :func:`~moss_image_b200.memory.place_model`, and
 :meth:`SyntheticDiT.forward_packed` runs a heterogeneous batch as one packed stream.
 Per-sample modulation and gates are applied by the native segment kernels on CUDA
 (:mod:`moss_image_b200.packed`). Attention uses torch's scaled-dot-product attention (library
-code; the jagged, variable-length form for packed streams).
+code; the jagged, variable-length form for packed streams). Queries and keys may be turned by
+their positions (a table from :func:`~moss_image_b200.rotary.rotary_table`), and the frozen linears
+may be held in block-scaled fp8 instead of int8.
 """
 
 from __future__ import annotations
@@ -28,6 +30,7 @@ from torch.nn import functional as F
 from torch.utils.checkpoint import checkpoint
 
 from .activation_offload import KEEP_RESIDENT, activation_cpu_offload
+from .fp8 import quantize_frozen_linears_fp8
 from .lora import LoRALinear
 from .memory import offloaded_block
 from .norms import rms_norm
@@ -43,6 +46,7 @@ from .packed import (
     varlen_attention,
 )
 from .quantization import quantize_frozen_linears
+from .rotary import apply_rotary
 
 
 class RMSNorm(nn.Module):
@@ -78,9 +82,11 @@ class SyntheticBlock(nn.Module):
         self.mlp_down = nn.Linear(mlp_dim, dim, bias=True)
         self.adaln = nn.Linear(dim, 6 * dim, bias=True)
 
-    def forward(self, tokens: torch.Tensor, cond: torch.Tensor, cu_seqlens: torch.Tensor | None = None) -> torch.Tensor:
+    def forward(self, tokens: torch.Tensor, cond: torch.Tensor, cu_seqlens: torch.Tensor | None = None,
+                cos: torch.Tensor | None = None, sin: torch.Tensor | None = None) -> torch.Tensor:
         """tokens: [B, T, dim] with cond [B, dim] (timestep embedding per sample), or a packed
-        [1, total, dim] stream with cu_seqlens (int64 [S + 1]) and cond [S, dim].
+        [1, total, dim] stream with cu_seqlens (int64 [S + 1]) and cond [S, dim]. With ``cos`` and
+        ``sin`` (float32 [T, half], one row per token) q and k are turned by their positions.
 
         The conditioning follows training/model.py:288-312: ``norm(x) * (1 + scale) + shift``
         and ``x + branch * gate`` per sample, each op rounded in the activation dtype. On CUDA
@@ -111,6 +117,8 @@ class SyntheticBlock(nn.Module):
         q = self.q_norm(self.proj["q"](h).unflatten(-1, (self.heads, -1)))
         k = self.k_norm(self.proj["k"](h).unflatten(-1, (self.heads, -1)))
         v = self.proj["v"](h).unflatten(-1, (self.heads, -1))
+        if cos is not None:
+            q, k = apply_rotary(q, k, cos, sin)
         if cu_seqlens is None:
             attended = F.scaled_dot_product_attention(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2))
             attended = attended.transpose(1, 2).flatten(2)
@@ -149,10 +157,12 @@ class SyntheticDiT(nn.Module):
         self.gradient_checkpointing = gradient_checkpointing
         self.activation_offload = False
 
-    def forward(self, tokens: torch.Tensor, timestep: torch.Tensor, skip_layers: tuple[int, ...] = ()) -> torch.Tensor:
+    def forward(self, tokens: torch.Tensor, timestep: torch.Tensor, skip_layers: tuple[int, ...] = (),
+                rotary: tuple[torch.Tensor, torch.Tensor] | None = None) -> torch.Tensor:
+        """``rotary``: the (cos, sin) tables of the tokens' positions, shared by all blocks."""
         with activation_cpu_offload(self, self.activation_offload, tokens.device):
             cond = self.time_embedding(timestep).to(tokens.dtype)
-            tokens = self._run_layers(tokens, cond, frozenset(skip_layers))
+            tokens = self._run_layers(tokens, cond, frozenset(skip_layers), rotary=rotary)
             return self.final_norm(tokens)
 
     def forward_packed(self, samples: list[torch.Tensor], timestep: torch.Tensor) -> list[torch.Tensor]:
@@ -180,7 +190,8 @@ class SyntheticDiT(nn.Module):
             return list(self.final_norm(tokens)[0].split(lengths, 0))
 
     def _run_layers(self, tokens: torch.Tensor, cond: torch.Tensor, skipped: frozenset[int],
-                    cu_seqlens: torch.Tensor | None = None) -> torch.Tensor:
+                    cu_seqlens: torch.Tensor | None = None,
+                    rotary: tuple[torch.Tensor, torch.Tensor] | None = None) -> torch.Tensor:
         """Resident, synchronously swapped or streamed blocks, as ``place_model`` left them.
 
         Mirrors training/model.py:672-709: blocks at or past ``len(layers) - blocks_to_swap``
@@ -192,10 +203,14 @@ class SyntheticDiT(nn.Module):
         manager = getattr(self, "block_swap_manager", None)
         streamed = [index for index in range(boundary, len(self.layers)) if index not in skipped]
         position = {index: slot for slot, index in enumerate(streamed)}
+        for table in rotary or ():
+            setattr(table, KEEP_RESIDENT, True)  # the same table in every block
         for index, layer in enumerate(self.layers):
             if index in skipped:
                 continue
             inputs = (tokens, cond) if cu_seqlens is None else (tokens, cond, cu_seqlens)
+            if rotary is not None:
+                inputs = (tokens, cond, cu_seqlens, *rotary)
             if manager is not None and index >= boundary:
                 at = position[index]
                 tokens = manager.block(
@@ -240,7 +255,8 @@ def _inject_block(layer: SyntheticBlock, rank: int, alpha: float, targets: tuple
 
 def build_lora_model(depth: int, *, device: torch.device, dim: int = 3072, heads: int = 24, mlp_dim: int = 12288,
                      rank: int = 32, alpha: float | None = None, seed: int = 0,
-                     dtype: torch.dtype = torch.bfloat16, full_qkvo: bool = False) -> SyntheticDiT:
+                     dtype: torch.dtype = torch.bfloat16, full_qkvo: bool = False,
+                     frozen: str = "int8") -> SyntheticDiT:
     """Random-init stack (weights ~ N(0, 0.02)), int8 base, LoRA on q/k/v/o.
 
     Mirrors the trainer's order (training/train.py:577-589): build, cast, inject LoRA,
@@ -251,14 +267,18 @@ def build_lora_model(depth: int, *, device: torch.device, dim: int = 3072, heads
     ``dtype`` masters, no adapters) and every other linear is frozen int8: the hybrid that
     ``quantize_frozen_linears`` allows at module level (training/quantization.py:156-157;
     the reference trainer itself only pairs int8 bases with LoRA, training/train.py:543-545).
+    ``frozen="fp8"`` holds the frozen linears as block-scaled fp8 (:mod:`moss_image_b200.fp8`).
     """
+    if frozen not in ("int8", "fp8"):
+        raise ValueError("frozen linears are held as int8 or fp8.")
+    quantize = quantize_frozen_linears if frozen == "int8" else quantize_frozen_linears_fp8
     torch.manual_seed(seed)
     alpha = float(rank if alpha is None else alpha)
     model = SyntheticDiT(depth=0, dim=dim, heads=heads, mlp_dim=mlp_dim)
     model.time_embedding.to(device=device, dtype=dtype)
     model.final_norm.to(device=device, dtype=dtype)
     model.requires_grad_(False)
-    quantize_frozen_linears(model.time_embedding)
+    quantize(model.time_embedding)
     layers = []
     for _ in range(depth):
         block = SyntheticBlock(dim, heads, mlp_dim).to(device=device)
@@ -275,7 +295,7 @@ def build_lora_model(depth: int, *, device: torch.device, dim: int = 3072, heads
                 block.proj[name].requires_grad_(True)
         else:
             _inject_block(block, rank, alpha, ("q", "k", "v", "o"), 0.01)
-        quantize_frozen_linears(block)
+        quantize(block)
         layers.append(block)
     model.layers = nn.ModuleList(layers)
     return model
@@ -299,11 +319,11 @@ def packed_flow_matching_loss(model: SyntheticDiT, latents: list[torch.Tensor], 
 
 
 def flow_matching_loss(model: SyntheticDiT, latents: torch.Tensor, text: torch.Tensor, t: torch.Tensor,
-                       noise: torch.Tensor) -> torch.Tensor:
+                       noise: torch.Tensor, rotary: tuple[torch.Tensor, torch.Tensor] | None = None) -> torch.Tensor:
     """Rectified-flow velocity loss on the image tokens (text tokens are conditioning)."""
     sigma = t.view(-1, 1, 1).to(latents.dtype)
     noisy = (1 - sigma) * latents + sigma * noise
     tokens = torch.cat((noisy, text), dim=1)
-    pred = model(tokens, t)[:, : latents.shape[1]]
+    pred = model(tokens, t, rotary=rotary)[:, : latents.shape[1]]
     target = noise - latents
     return F.mse_loss(pred.float(), target.float())

@@ -375,12 +375,13 @@ class AsyncBlockStreamer:
         count = len(inputs)
         names = tuple(self._blocks[index].trainable)
         # aliases give the gradient hook tensors that belong to this invocation alone
-        input_aliases = tuple(tensor.view_as(tensor) if tensor.requires_grad else tensor for tensor in inputs)
+        input_aliases = tuple(tensor.view_as(tensor) if tensor is not None and tensor.requires_grad else tensor
+                              for tensor in inputs)
         adapter_aliases = tuple(parameter.view_as(parameter) for parameter in self._blocks[index].trainable.values())
 
         def run(*arguments: torch.Tensor) -> torch.Tensor:
             adapters = dict(zip(names, arguments[count:]))
-            completion = tuple(tensor for tensor in arguments if tensor.requires_grad)
+            completion = tuple(tensor for tensor in arguments if tensor is not None and tensor.requires_grad)
             return self._run(index, arguments[:count], adapters, completion, forward_prefetch, backward_prefetch)
 
         return checkpoint(run, *input_aliases, *adapter_aliases, use_reentrant=False,

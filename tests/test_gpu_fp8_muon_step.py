@@ -1,0 +1,92 @@
+"""Rotary positions, fp8 frozen linears and the Muon optimiser together, as the example runs them."""
+
+from __future__ import annotations
+
+import importlib.util
+from pathlib import Path
+
+import pytest
+import torch
+
+from moss_image_b200.dit import SyntheticBlock, build_lora_model
+from moss_image_b200.fp8 import FrozenFp8Linear
+from moss_image_b200.lora import LoRALinear
+from moss_image_b200.memory import place_model
+from moss_image_b200.rotary import rotary_frequencies, rotary_table
+
+pytestmark = pytest.mark.gpu
+
+EXAMPLE = Path(__file__).resolve().parents[1] / "examples" / "fp8_muon_finetune.py"
+
+
+def _example():
+    spec = importlib.util.spec_from_file_location("fp8_muon_finetune", EXAMPLE)
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+    return module
+
+
+def test_the_example_learns_its_batch(cuda_device):
+    losses = _example().finetune(depth=2, dim=256, heads=4, side=8, text_tokens=16, batch=2, steps=12, lr=4e-3,
+                                 device=cuda_device)
+    # small steps along descent directions lower the loss of the batch they were taken on
+    assert all(loss == loss for loss in losses)
+    assert sum(losses[-3:]) < sum(losses[:3])
+
+
+def test_lora_over_fp8_with_positions_offload_and_checkpointing(cuda_device):
+    """The same gradients with and without saved-activation offload, and a position that matters."""
+    model = build_lora_model(2, device=cuda_device, dim=256, heads=4, mlp_dim=512, rank=8, seed=3, frozen="fp8").train()
+    assert isinstance(model.layers[0].proj["q"], LoRALinear) and isinstance(model.layers[0].proj["q"].base, FrozenFp8Linear)
+    for layer in model.layers:
+        for name in ("q", "k", "v", "o"):
+            torch.nn.init.normal_(layer.proj[name].lora_B, std=0.02)
+    tokens = torch.randn(2, 40, 256, device=cuda_device, dtype=torch.bfloat16)
+    t = torch.tensor([0.2, 0.7], device=cuda_device)
+    rotary = rotary_table(torch.arange(40, device=cuda_device), rotary_frequencies(64, device=cuda_device))
+    trained = [p for p in model.parameters() if p.requires_grad]
+    grads = []
+    for offload in (False, True):
+        model.activation_offload = offload
+        model(tokens, t, rotary=rotary).float().square().mean().backward()
+        grads.append([p.grad.clone() for p in trained])
+        for p in trained:
+            p.grad = None
+    assert all(torch.equal(a, b) and a.isfinite().all() for a, b in zip(*grads))
+    model.activation_offload = False
+    with torch.no_grad():
+        still = model(tokens, t, rotary=(torch.ones_like(rotary[0]), torch.zeros_like(rotary[1])))
+        plain = model(tokens, t)
+        turned = model(tokens, t, rotary=rotary)
+    assert torch.equal(still, plain) and not torch.equal(turned, plain)
+
+
+def test_streamed_fp8_blocks_with_positions(cuda_device):
+    """Blocks whose fp8 codes stream from pinned host memory give the resident model's gradients."""
+    resident, streamed = (build_lora_model(3, device=cuda_device, dim=128, heads=2, mlp_dim=256, rank=4, seed=5,
+                                           frozen="fp8").train() for _ in range(2))
+    for model in (resident, streamed):
+        gen = torch.Generator(device=cuda_device).manual_seed(6)
+        for layer in model.layers:
+            for name in ("q", "k", "v", "o"):
+                layer.proj[name].lora_B.data.normal_(0.0, 0.03, generator=gen)
+    place_model(resident, cuda_device, 0)
+    place_model(streamed, cuda_device, 2, block_swap_mode="async")
+    tokens = torch.randn(2, 24, 128, device=cuda_device, dtype=torch.bfloat16)
+    t = torch.tensor([0.3, 0.6], device=cuda_device)
+    rotary = rotary_table(torch.arange(24, device=cuda_device), rotary_frequencies(64, device=cuda_device))
+    outputs = [model(tokens, t, rotary=rotary) for model in (resident, streamed)]
+    assert torch.equal(*outputs)
+    for output in outputs:
+        output.float().square().mean().backward()
+    for a, b in zip(resident.parameters(), streamed.parameters()):
+        assert (a.grad is None) == (b.grad is None)
+        if a.grad is not None:
+            assert torch.equal(a.grad, b.grad.to(a.grad.device))
+    streamed.block_swap_manager.close()
+
+
+def test_frozen_format_is_checked(cuda_device):
+    with pytest.raises(ValueError, match="int8 or fp8"):
+        build_lora_model(1, device=cuda_device, dim=64, heads=1, mlp_dim=64, frozen="fp4")
+    assert SyntheticBlock(64, 1, 128).heads == 1
