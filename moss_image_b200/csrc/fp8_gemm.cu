@@ -148,6 +148,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = bars->tmem_base;
+  pdl_trigger();
+  pdl_wait();
 
   if (warp < kEpiWarp0) {
   if constexpr (kCtas == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegs));
@@ -469,11 +471,13 @@ int launch_typed(const CUtensorMap& ta, const CUtensorMap& tw, const CUtensorMap
   static std::once_flag once;
   static cudaError_t attr_err = cudaSuccess;
   static int max_groups = 0;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = kCtas;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = kSmemBytes;
@@ -496,6 +500,7 @@ int launch_typed(const CUtensorMap& ta, const CUtensorMap& tw, const CUtensorMap
   const int64_t units = static_cast<int64_t>(a.tiles_m) * a.tiles_n * a.splits;
   cfg.gridDim = dim3(static_cast<unsigned>(kCtas * std::max<int64_t>(1, std::min<int64_t>(units, max_groups))));
   cfg.stream = stream;
+  cfg.numAttrs = 2;  // after this call's quantiser
   return check_cuda(cudaLaunchKernelEx(&cfg, kern, ta, tw, to, a), "fp8_gemm_kernel");
 }
 

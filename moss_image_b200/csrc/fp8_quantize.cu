@@ -157,6 +157,7 @@ template <int kKind, bool kWide>
 __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const void* __restrict__ x, int64_t m, int64_t k, int kb,
                                                                  uint8_t* __restrict__ codes, float* __restrict__ scale,
                                                                  int64_t row_pitch) {
+  pdl_trigger();
   // neighbouring CTAs walk along the rows: DRAM pages are read whole
   constexpr int kB = kBatch<kKind>;
   const int groups = (kb + kB - 1) / kB;

@@ -82,6 +82,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = bars->tmem_base;
+  pdl_trigger();
 
   if (warp == 0) {
     // ---------------------------------------------------------------- producer
@@ -89,15 +90,23 @@ __global__ void __launch_bounds__(kThreads, 2)
       tma_prefetch_desc(&tm_a);
       tma_prefetch_desc(&tm_w);
     }
+    // The weight does not depend on the quantiser that runs before: a ring of it is on its way meanwhile.
+    const int early = min(kStages, kb1 - kb0);
+    auto load_weight = [&](int stage, int kb) {
+      mbar_arrive_expect_tx(bar(bars->full[stage]), R::kStageBytes);
+      tma_load_2d(base + stage * R::kStageBytes, &tm_w, bar(bars->full[stage]), kDX ? f0 : kb * kBlock,
+                  kDX ? kb * kBlock : f0);
+    };
+    if (lane == 0)
+      for (int i = 0; i < early; ++i) load_weight(i, kb0 + i);
+    pdl_wait();
     int stage = 0;
     uint32_t phase = 0, used = 0, last_phase = 0;
     for (int kb = kb0; kb < kb1; ++kb) {
       if (!mbar_wait(bar(bars->empty[stage]), phase ^ 1u, abort_flag, args.status, MOSS_STATUS_TIMEOUT_LOAD)) break;
       if (lane == 0) {
-        const uint32_t dst = base + stage * R::kStageBytes;
-        mbar_arrive_expect_tx(bar(bars->full[stage]), R::kStageBytes);
-        tma_load_2d(dst, &tm_w, bar(bars->full[stage]), kDX ? f0 : kb * kBlock, kDX ? kb * kBlock : f0);
-        tma_load_2d(dst + kWBytes, &tm_a, bar(bars->full[stage]), kb * kBlock, m0);
+        if (kb - kb0 >= early) load_weight(stage, kb);
+        tma_load_2d(base + stage * R::kStageBytes + kWBytes, &tm_a, bar(bars->full[stage]), kb * kBlock, m0);
         used |= 1u << stage;
         last_phase = (last_phase & ~(1u << stage)) | (phase << stage);
       }
@@ -118,7 +127,9 @@ __global__ void __launch_bounds__(kThreads, 2)
     }
   } else if (warp == 1) {
     // ---------------------------------------------------------------- MMA issuer
+    pdl_wait();
     constexpr uint32_t idesc = idesc_e4m3(kDX, false, kFeatures, kTN);
+    const uint64_t w_desc0 = step_desc(base, 0, kDX), a_desc0 = step_desc(base + kWBytes, 0, false);
     int stage = 0;
     uint32_t phase = 0;
     bool issued = false;
@@ -129,16 +140,16 @@ __global__ void __launch_bounds__(kThreads, 2)
           !mbar_wait(bar(bars->full[stage]), phase, abort_flag, args.status, MOSS_STATUS_TIMEOUT_MMA))
         break;
       tc_fence_after();
-      if (lane == 0) {
-        const uint32_t w_tile = base + stage * R::kStageBytes;
+      if (elect_one()) {
+        const uint64_t at_stage = static_cast<uint64_t>(stage) * (R::kStageBytes >> 4);
         const uint32_t d = tmem_base + static_cast<uint32_t>(acc * kTN);
 #pragma unroll
         for (int kk = 0; kk < kBlock / 32; ++kk)
-          umma_f8(d, step_desc(w_tile, kk, kDX), step_desc(w_tile + kWBytes, kk, false), idesc, kk > 0);
-        umma_commit(bar(bars->empty[stage]));
+          umma_f8(d, w_desc0 + at_stage + kk * ((kDX ? 4096 : 32) >> 4), a_desc0 + at_stage + kk * (32 >> 4), idesc, kk > 0);
         umma_commit(bar(bars->acc_full[acc]));
-        issued = true;
+        umma_commit(bar(bars->empty[stage]));
       }
+      issued = true;
       __syncwarp();
       if (++stage == kStages) { stage = 0; phase ^= 1u; }
     }
@@ -155,6 +166,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     __syncwarp();
   } else {
     // ---------------------------------------------------------------- epilogue
+    pdl_wait();
     const int q = warp & 3;
     const int feature = f0 + q * 32 + lane;
     const uint32_t lane_addr = tmem_base + (static_cast<uint32_t>(q * 32) << 16);
@@ -227,8 +239,8 @@ int launch_typed(const CUtensorMap& ta, const CUtensorMap& tw, const Args& a, cu
     attr_err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Ring<kTN>::kSmemBytes);
   });
   MOSS_CUDA_TRY(attr_err);
-  kern<<<static_cast<unsigned>(a.tiles_m * a.tiles_n * a.splits), kThreads, Ring<kTN>::kSmemBytes, stream>>>(ta, tw, a);
-  return check_cuda(cudaGetLastError(), "fp8_rows_kernel");
+  return launch_dependent("fp8_rows_kernel", kern, dim3(static_cast<unsigned>(a.tiles_m * a.tiles_n * a.splits)),
+                          dim3(kThreads), Ring<kTN>::kSmemBytes, stream, ta, tw, a);
 }
 
 }  // namespace
