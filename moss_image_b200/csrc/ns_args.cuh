@@ -37,13 +37,14 @@ struct Small {
   int dtype;
   int64_t batch;
   int r, c, tall, steps;
-  int wide, out_wide;  // 4-value reads of G's rows, 4- or 8-value (tall) writes of the result's are aligned and whole
+  int wide, out_wide;  // 4-value reads of G's rows, 8-value writes of the result's are aligned and whole
   float coefficients[3 * kMaxSteps];
   float eps;
   __nv_bfloat16* out;
   int chunks;      // column ranges per matrix of the Gram kernel
   float* partial;  // [batch][chunks][side * side]
-  float* q;        // [batch][side * side], transposed
+  __half* q;       // [batch][hi, lo][side * side], scaled by a power of two
+  float* factors;  // [batch][2]: X's scale in the product with Q, and the product's own
 };
 int small_side(int r);
 int small_chunks(int64_t batch, int r, int c, int sms);

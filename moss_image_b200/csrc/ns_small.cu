@@ -3,8 +3,11 @@
 // With R = X X^T, a step X <- (a I + b R + c R R) X =: P X turns R into P R P, so the whole iteration
 // stays on the r x r square: Q <- P Q, R <- P R P, and the result is Q X. X is read twice (once
 // for R, whose trace is the squared Frobenius norm, once for Q X) however many steps there are,
-// instead of three times a step. All of it is f32: R's small eigenvalues, which grow by (a^2) a step,
-// need its precision, and Q X is rounded once.
+// instead of three times a step. R's small eigenvalues, which grow by a^2 a step, need f32's
+// precision: the iteration is f32, and the two products with X run on the tensor cores
+// (mma.sync m16n8k16) with each f32 operand as the sum of two float16 numbers, scaled by powers of two,
+// hi hi + hi lo + lo hi with f32 sums. What that leaves out is 2^-22 of a product. (tcgen05's 128-row
+// tiles would be three quarters empty here, and these kernels are bound by HBM and latency.)
 //
 // Three launches: partial R over column ranges, the iteration (one CTA per matrix), Q X.
 #include <algorithm>
@@ -17,12 +20,14 @@ namespace ns {
 namespace {
 
 constexpr int kThreads = 256;
-// Columns of X in shared memory at a time: 16 KB of f32 (Gram) or 32 KB (apply). Rows lie 16 bytes past a
-// multiple of 128 apart, so that 16-byte reads of neighbouring rows meet in different banks.
+// Columns of X in shared memory at a time: 8192 values, as two float16 tiles whose rows lie 16 bytes past a
+// multiple of 128 apart, so that the eight rows of an ldmatrix meet in different banks.
 template <int kSide>
-constexpr int kGramCols = 4096 / kSide;
+constexpr int kCols = 8192 / kSide;
 template <int kSide>
-constexpr int kApplyCols = 8192 / kSide;
+constexpr int kPitch = kCols<kSide> + 8;
+template <int kSide>
+constexpr int kTileHalves = kSide * kPitch<kSide>;  // of one of the two tiles
 
 template <int kKind>
 struct Raw4 {  // four neighbouring values of G as they are stored
@@ -70,11 +75,30 @@ __device__ __forceinline__ float4 to_float4(const Raw4<kKind>& r) {
   }
 }
 
-// kC columns of X from column c0 on their way to shared memory: fetch() starts the loads (zero past r and c),
-// put() writes xs[row][column]. Between the two the CTA works on the tile before.
-template <int kSide, int kC, int kKind>
+// fmaxf drops NaN; a tile that holds one has to show it.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float pow2(int p) { return __uint_as_float(static_cast<uint32_t>(p + 127) << 23); }
+// p with v in [2^(p + 10), 2^(p + 11)): v 2^-p is about 1024. Kept where 2^p and 2^-p are normal.
+__device__ __forceinline__ int scale_of(float v) {
+  return min(110, max(-110, static_cast<int>((__float_as_uint(v) >> 23) & 0xffu) - 127 - 10));
+}
+__device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
+  const __half2 h = __floats2half2_rn(a, b);
+  const float2 back = __half22float2(h);
+  const __half2 l = __floats2half2_rn(a - back.x, b - back.y);
+  hi = *reinterpret_cast<const uint32_t*>(&h);
+  lo = *reinterpret_cast<const uint32_t*>(&l);
+}
+
+// kCols columns of X from column c0 on their way to shared memory: fetch() starts the loads (zero past r and
+// c), put() writes xs[row][column] as hi + lo. Between the two the CTA works on the tile before.
+template <int kSide, int kKind>
 struct Tile {
-  static constexpr int kPitch = kC + 4;
+  static constexpr int kC = kCols<kSide>;
   static constexpr int kLoads = kSide * kC / 4 / kThreads;
   Raw4<kKind> raw[kLoads];
   __device__ __forceinline__ void fetch(const Small& s, int64_t b, int c0) {
@@ -91,92 +115,179 @@ struct Tile {
       }
     }
   }
-  __device__ __forceinline__ void put(bool tall, float* xs) const {
+  __device__ __forceinline__ float amax() const {
+    float m = 0.0f;
+#pragma unroll
+    for (int l = 0; l < kLoads; ++l) {
+      const float4 v = to_float4<kKind>(raw[l]);
+      m = max_nan(m, max_nan(max_nan(fabsf(v.x), fabsf(v.y)), max_nan(fabsf(v.z), fabsf(v.w))));
+    }
+    return m;
+  }
+  __device__ __forceinline__ void put(bool tall, float scale, __half* hi, __half* lo) const {
+    constexpr int kP = kPitch<kSide>;
 #pragma unroll
     for (int l = 0; l < kLoads; ++l) {
       const int i = threadIdx.x + l * kThreads;
       const float4 v = to_float4<kKind>(raw[l]);
+      uint2 h, q;
+      split2(v.x * scale, v.y * scale, h.x, q.x);
+      split2(v.z * scale, v.w * scale, h.y, q.y);
       if (!tall) {
-        *reinterpret_cast<float4*>(xs + i / (kC / 4) * kPitch + i % (kC / 4) * 4) = v;
+        const int at = i / (kC / 4) * kP + i % (kC / 4) * 4;
+        *reinterpret_cast<uint2*>(hi + at) = h;
+        *reinterpret_cast<uint2*>(lo + at) = q;
       } else {
-        float* to = xs + i / kC * 4 * kPitch + i % kC;
-        to[0] = v.x;
-        to[kPitch] = v.y;
-        to[2 * kPitch] = v.z;
-        to[3 * kPitch] = v.w;
+        const int at = i / kC * 4 * kP + i % kC;
+        const __half2 h0 = *reinterpret_cast<const __half2*>(&h.x), h1 = *reinterpret_cast<const __half2*>(&h.y);
+        const __half2 q0 = *reinterpret_cast<const __half2*>(&q.x), q1 = *reinterpret_cast<const __half2*>(&q.y);
+        hi[at] = __low2half(h0);
+        hi[at + kP] = __high2half(h0);
+        hi[at + 2 * kP] = __low2half(h1);
+        hi[at + 3 * kP] = __high2half(h1);
+        lo[at] = __low2half(q0);
+        lo[at + kP] = __high2half(q0);
+        lo[at + 2 * kP] = __low2half(q1);
+        lo[at + 3 * kP] = __high2half(q1);
       }
     }
   }
 };
 
-// Partial X X^T over this CTA's column range, upper half. With T = side / 8, piece (t, u), t <= u, is the
-// 8 x 8 products of rows t, t + T, .. with rows u, u + T, ..; a thread sums one piece over every kSlices-th
-// group of four columns. 64 multiply-adds for 16 values read is what keeps shared memory from
-// being the bound (4 x 4 pieces took 53 us for 144 x 32 x 3072).
+__device__ __forceinline__ void ldmatrix4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr));
+}
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr));
+}
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// Lane addresses within a 16 x 16 block of halves at (row, column) of a tile. A operand and, by .trans, a B
+// operand that lies [reduction][column]: rows by lane % 16, column halves by lane / 16.
+__device__ __forceinline__ uint32_t block_rows(uint32_t tile, int pitch, int row, int col, int lane) {
+  return tile + 2 * ((row + (lane & 15)) * pitch + col + (lane >> 4) * 8);
+}
+// A B operand that lies [column][reduction]: two 8-column tiles, each two 8-wide reduction halves.
+__device__ __forceinline__ uint32_t block_columns(uint32_t tile, int pitch, int row, int col, int lane) {
+  return tile + 2 * ((row + (lane >> 4) * 8 + (lane & 7)) * pitch + col + ((lane >> 3) & 1) * 8);
+}
+
+// Partial X X^T over this CTA's column range: hi hi^T + hi lo^T + (hi lo^T)^T. A warp holds one block of at
+// most 32 x 32 of both products, over every kSplits-th 16 columns. X is scaled by the largest value met so
+// far; when a tile brings a larger one, the sums are scaled down with it (powers of two, exact).
 template <int kSide, int kKind>
 __global__ void __launch_bounds__(kThreads, 2) small_gram_kernel(const Small s) {
-  constexpr int kT = kSide / 8;
-  constexpr int kPieces = kT * (kT + 1) / 2;
-  constexpr int kSlices = kThreads / kPieces;
-  constexpr int kC = kGramCols<kSide>;
-  using T = Tile<kSide, kC, kKind>;
-  constexpr int kP = T::kPitch;
-  __shared__ __align__(16) float xs[kSide * kP > kThreads * 9 ? kSide * kP : kThreads * 9];
+  constexpr int kC = kCols<kSide>, kP = kPitch<kSide>;
+  constexpr int kBlk = kSide < 32 ? kSide : 32;
+  constexpr int kBlocks = kSide / kBlk;  // per side
+  constexpr int kSplits = kThreads / 32 / (kBlocks * kBlocks);
+  constexpr int kMT = kBlk / 16, kNT = kBlk / 8;
+  __shared__ __align__(16) __half tiles[2 * kTileHalves<kSide>];
+  __shared__ float warp_max[kThreads / 32];
+  static_assert(sizeof(tiles) >= kSplits * kSide * (kSide + 1) * 4, "the joined sums fit the tiles");
   const int64_t b = blockIdx.y;
   const int ranges = (s.c + kC - 1) / kC;
   const int first = static_cast<int>(static_cast<int64_t>(blockIdx.x) * ranges / s.chunks);
   const int last = static_cast<int>(static_cast<int64_t>(blockIdx.x + 1) * ranges / s.chunks);
-  const int piece = threadIdx.x % kPieces, slice = threadIdx.x / kPieces;
-  int u = 0;
-  while ((u + 1) * (u + 2) / 2 <= piece) ++u;
-  const int t = piece - u * (u + 1) / 2;
-  float acc[8][8] = {};
-  T next;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int split = warp % kSplits, block = warp / kSplits;
+  const int i0 = block / kBlocks * kBlk, j0 = block % kBlocks * kBlk;
+  __half* hi = tiles;
+  __half* lo = tiles + kTileHalves<kSide>;
+  const uint32_t hi_addr = smem_u32(hi), lo_addr = smem_u32(lo);
+  float hh[kMT][kNT][4] = {}, hl[kMT][kNT][4] = {};
+  int p = -110;  // X is held times 2^-p
+  Tile<kSide, kKind> next;
   if (first < last) next.fetch(s, b, first * kC);
   for (int range = first; range < last; ++range) {
-    __syncthreads();
-    next.put(s.tall, xs);
+    float amax = next.amax();
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, d));
+    if (lane == 0) warp_max[warp] = amax;
+    __syncthreads();  // the maxima are there, and the tiles free
+#pragma unroll
+    for (int w = 0; w < kThreads / 32; ++w) amax = max_nan(amax, warp_max[w]);
+    const int q = scale_of(amax);
+    if (q > p) {
+      const float down = pow2(max(-126, 2 * (p - q)));
+#pragma unroll
+      for (int i = 0; i < kMT; ++i)
+#pragma unroll
+        for (int j = 0; j < kNT; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            hh[i][j][e] *= down;
+            hl[i][j][e] *= down;
+          }
+      p = q;
+    }
+    next.put(s.tall, pow2(-p), hi, lo);
     __syncthreads();
     if (range + 1 < last) next.fetch(s, b, (range + 1) * kC);
-    if (slice < kSlices) {
-      for (int k = slice * 4; k < kC; k += kSlices * 4) {
-        float4 x[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = *reinterpret_cast<const float4*>(xs + (t + kT * i) * kP + k);
+    for (int k = split * 16; k < kC; k += kSplits * 16) {
+      uint32_t a[kMT][4];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float4 y = *reinterpret_cast<const float4*>(xs + (u + kT * j) * kP + k);
+      for (int i = 0; i < kMT; ++i) ldmatrix4(block_rows(hi_addr, kP, i0 + i * 16, k, lane), a[i]);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            acc[i][j] = fmaf(x[i].x, y.x, acc[i][j]);
-            acc[i][j] = fmaf(x[i].y, y.y, acc[i][j]);
-            acc[i][j] = fmaf(x[i].z, y.z, acc[i][j]);
-            acc[i][j] = fmaf(x[i].w, y.w, acc[i][j]);
-          }
+      for (int j = 0; j < kNT / 2; ++j) {
+        uint32_t bh[4], bl[4];
+        ldmatrix4(block_columns(hi_addr, kP, j0 + j * 16, k, lane), bh);
+        ldmatrix4(block_columns(lo_addr, kP, j0 + j * 16, k, lane), bl);
+#pragma unroll
+        for (int i = 0; i < kMT; ++i) {
+          mma16816(hh[i][2 * j], a[i], bh[0], bh[1]);
+          mma16816(hh[i][2 * j + 1], a[i], bh[2], bh[3]);
+          mma16816(hl[i][2 * j], a[i], bl[0], bl[1]);
+          mma16816(hl[i][2 * j + 1], a[i], bl[2], bl[3]);
         }
       }
     }
   }
-  // the slices' sums, in slice order, eight values of each piece at a time
+  // The warps' sums, always in the same order: the first half of the splits each to a region of its own, the
+  // second half on top of them, then the regions.
+  constexpr int kRegions = kSplits / 2;
+  using Row = float[kSide + 1];
+  Row* regions = reinterpret_cast<Row*>(tiles);  // [region][hh, hl][kSide]
+  Row* sum = regions + split % kRegions * 2 * kSide;
+  Row* cross = sum + kSide;
+#pragma unroll
+  for (int turn = 0; turn < 2; ++turn) {
+    __syncthreads();
+    if (split / kRegions != turn) continue;
+#pragma unroll
+    for (int i = 0; i < kMT; ++i)
+#pragma unroll
+      for (int j = 0; j < kNT; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int row = i0 + i * 16 + (lane >> 2) + (e >> 1) * 8, col = j0 + j * 8 + (lane & 3) * 2 + (e & 1);
+          sum[row][col] = (turn > 0 ? sum[row][col] : 0.0f) + hh[i][j][e];
+          cross[row][col] = (turn > 0 ? cross[row][col] : 0.0f) + hl[i][j][e];
+        }
+  }
+  __syncthreads();
   float* out = s.partial + (b * s.chunks + blockIdx.x) * kSide * kSide;
+  const float up = pow2(p);
+  for (int e = threadIdx.x; e < kSide * kSide; e += kThreads) {
+    const int row = e / kSide, col = e % kSide;
+    float same = 0.0f, across = 0.0f;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    __syncthreads();
-    if (slice < kSlices) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) xs[(slice * kPieces + piece) * 9 + j] = acc[i][j];
+    for (int k = 0; k < kRegions; ++k) {
+      const Row* part = regions + k * 2 * kSide;
+      same += part[row][col];
+      across += part[kSide + row][col] + part[kSide + col][row];
     }
-    __syncthreads();
-    for (int e = threadIdx.x; e < kPieces * 8; e += kThreads) {
-      const int p = e >> 3, j = e & 7;
-      float v = 0.0f;
-      for (int k = 0; k < kSlices; ++k) v += xs[(k * kPieces + p) * 9 + j];
-      int pu = 0;
-      while ((pu + 1) * (pu + 2) / 2 <= p) ++pu;
-      const int row = p - pu * (pu + 1) / 2 + kT * i, col = pu + kT * j;
-      out[row * kSide + col] = v;
-      out[col * kSide + row] = v;
-    }
+    out[e] = (same + across) * up * up;
   }
   pdl_trigger();
 }
@@ -254,7 +365,7 @@ __global__ void __launch_bounds__(kIterateThreads<kSide>) small_iterate_kernel(c
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) Q[i0 + i][j0 + j] = i0 + i == j0 + j ? inv : 0.0f;
+      for (int j = 0; j < 4; ++j) Q[i0 + i][j0 + j] = i0 + i == j0 + j ? 1.0f : 0.0f;
   }
   for (int step = 0; step < s.steps; ++step) {
     const float ca = s.coefficients[3 * step], cb = s.coefficients[3 * step + 1], cc = s.coefficients[3 * step + 2];
@@ -287,96 +398,136 @@ __global__ void __launch_bounds__(kIterateThreads<kSide>) small_iterate_kernel(c
     }
   }
   __syncthreads();
-  float* q = s.q + b * kSide * kSide;  // Q^T
-  for (int e = threadIdx.x; e < kSide * kSide; e += kIterateThreads<kSide>) q[e] = Q[e % kSide][e / kSide];
+  // Q as hi + lo, times 2^-qp, and what the product has to be multiplied by. |x| <= |X|, so X is held times 2^-xp.
+  __shared__ float warp_max[kIterateThreads<kSide> / 32];
+  float amax = 0.0f;
+  for (int e = threadIdx.x; e < kSide * kSide; e += kIterateThreads<kSide>)
+    amax = max_nan(amax, fabsf(Q[e / kSide][e % kSide]));
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, d));
+  if ((threadIdx.x & 31) == 0) warp_max[threadIdx.x >> 5] = amax;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kIterateThreads<kSide> / 32; ++w) amax = max_nan(amax, warp_max[w]);
+  const int qp = scale_of(amax), xp = scale_of(norm);
+  const float down = pow2(-qp);
+  __half* hi = s.q + b * 2 * kSide * kSide;
+  __half* lo = hi + kSide * kSide;
+  for (int e = threadIdx.x * 2; e < kSide * kSide; e += kIterateThreads<kSide> * 2) {
+    uint32_t h, l;
+    split2(Q[e / kSide][e % kSide] * down, Q[e / kSide][e % kSide + 1] * down, h, l);
+    *reinterpret_cast<uint32_t*>(hi + e) = h;
+    *reinterpret_cast<uint32_t*>(lo + e) = l;
+  }
+  if (threadIdx.x == 0) {
+    // 1 / |X| is divided between the two powers of two: each of the three may be far from 1, their product is not
+    s.factors[2 * b] = pow2(-xp);
+    s.factors[2 * b + 1] = (inv * pow2(xp)) * pow2(qp);
+  }
 }
 
-// out = Q X over this CTA's column range. A warp takes 8 rows of 128 columns, 4 columns a lane: Q is read by
-// the whole warp at once, X once for 8 rows.
+// out = Q X over this CTA's column range: hi hi + hi lo + lo hi. A warp takes an eighth of a tile's columns, all rows.
 template <int kSide, int kKind>
 __global__ void __launch_bounds__(kThreads, 2) small_apply_kernel(const Small s) {
-  constexpr int kC = kApplyCols<kSide>;
-  using T = Tile<kSide, kC, kKind>;
-  constexpr int kP = T::kPitch;
-  extern __shared__ __align__(16) float xs[];
-  float* q = xs + kSide * kP;  // Q^T, dense
+  constexpr int kC = kCols<kSide>, kP = kPitch<kSide>, kQP = kSide + 8;
+  constexpr int kMT = kSide / 16, kNT = kC / 64;  // 16-row and 8-column tiles of a warp
+  extern __shared__ __align__(16) __half smem_halves[];
+  __half* hi = smem_halves;
+  __half* lo = hi + kTileHalves<kSide>;
+  __half* qh = lo + kTileHalves<kSide>;
+  __half* ql = qh + kSide * kQP;
+  __nv_bfloat16* staged = reinterpret_cast<__nv_bfloat16*>(smem_halves);  // over the tiles, once they are used
+  constexpr int kWidePitch = kC + 8, kTallPitch = kSide + 8;
+  static_assert(kC * kTallPitch <= 2 * kTileHalves<kSide>, "the turned outputs fit the tiles");
   const int64_t b = blockIdx.y;
   const int ranges = (s.c + kC - 1) / kC;
   const int first = static_cast<int>(static_cast<int64_t>(blockIdx.x) * ranges / gridDim.x);
   const int last = static_cast<int>(static_cast<int64_t>(blockIdx.x + 1) * ranges / gridDim.x);
-  T next;
+  Tile<kSide, kKind> next;
   if (first < last) next.fetch(s, b, first * kC);  // G is the caller's: no kernel of this call writes it
   pdl_wait();
-  for (int e = threadIdx.x; e < kSide * kSide; e += kThreads) q[e] = s.q[b * kSide * kSide + e];
+  for (int e = threadIdx.x * 8; e < 2 * kSide * kSide; e += kThreads * 8) {
+    const int part = e / (kSide * kSide), at = e % (kSide * kSide);
+    *reinterpret_cast<uint4*>((part ? ql : qh) + at / kSide * kQP + at % kSide) =
+        *reinterpret_cast<const uint4*>(s.q + b * 2 * kSide * kSide + e);
+  }
+  const float x_scale = s.factors[2 * b], factor = s.factors[2 * b + 1];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int i0 = warp % (kSide / 8) * 8, j0 = warp / (kSide / 8) * 128 + lane * 4;
-  for (int range = first; range < last; ++range) {
-  __syncthreads();
-  next.put(s.tall, xs);
-  __syncthreads();
-  if (range + 1 < last) next.fetch(s, b, (range + 1) * kC);
-  const int c0 = range * kC;
-  float acc[8][4] = {};
-#pragma unroll 8
-  for (int k = 0; k < kSide; ++k) {
-    const float4 x = *reinterpret_cast<const float4*>(xs + k * kP + j0);
-    const float4 lo = *reinterpret_cast<const float4*>(q + k * kSide + i0);
-    const float4 hi = *reinterpret_cast<const float4*>(q + k * kSide + i0 + 4);
-    const float w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      acc[i][0] = fmaf(w[i], x.x, acc[i][0]);
-      acc[i][1] = fmaf(w[i], x.y, acc[i][1]);
-      acc[i][2] = fmaf(w[i], x.z, acc[i][2]);
-      acc[i][3] = fmaf(w[i], x.w, acc[i][3]);
-    }
-  }
+  const uint32_t hi_addr = smem_u32(hi), lo_addr = smem_u32(lo), qh_addr = smem_u32(qh), ql_addr = smem_u32(ql);
   __nv_bfloat16* out = s.out + b * s.r * s.c;
-  const int col0 = c0 + j0;
-  if (!s.tall) {
-    const bool whole = s.out_wide && col0 + 4 <= s.c;
+  for (int range = first; range < last; ++range) {
+    __syncthreads();
+    next.put(s.tall, x_scale, hi, lo);
+    __syncthreads();
+    if (range + 1 < last) next.fetch(s, b, (range + 1) * kC);
+    const int c0 = range * kC;
+    float acc[kMT][kNT][4] = {};
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      if (i0 + i >= s.r) break;
-      __nv_bfloat16* dst = out + static_cast<int64_t>(i0 + i) * s.c + col0;
-      if (whole) {
-        const __nv_bfloat162 p0 = __floats2bfloat162_rn(acc[i][0], acc[i][1]);
-        const __nv_bfloat162 p1 = __floats2bfloat162_rn(acc[i][2], acc[i][3]);
-        *reinterpret_cast<uint2*>(dst) =
-            make_uint2(*reinterpret_cast<const uint32_t*>(&p0), *reinterpret_cast<const uint32_t*>(&p1));
-      } else {
+    for (int k = 0; k < kSide; k += 16) {
+      uint32_t ah[kMT][4], al[kMT][4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (col0 + j < s.c) dst[j] = __float2bfloat16_rn(acc[i][j]);
+      for (int i = 0; i < kMT; ++i) {
+        ldmatrix4(block_rows(qh_addr, kQP, i * 16, k, lane), ah[i]);
+        ldmatrix4(block_rows(ql_addr, kQP, i * 16, k, lane), al[i]);
       }
-    }
-  } else {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if (col0 + j >= s.c) break;
-      __nv_bfloat16* dst = out + static_cast<int64_t>(col0 + j) * s.r + i0;
-      if (s.out_wide && i0 + 8 <= s.r) {
-        uint32_t p[4];
+      for (int j = 0; j < kNT / 2; ++j) {
+        uint32_t bh[4], bl[4];
+        const int col = warp * kNT * 8 + j * 16;
+        ldmatrix4_trans(block_rows(hi_addr, kP, k, col, lane), bh);
+        ldmatrix4_trans(block_rows(lo_addr, kP, k, col, lane), bl);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const __nv_bfloat162 h = __floats2bfloat162_rn(acc[2 * i][j], acc[2 * i + 1][j]);
-          p[i] = *reinterpret_cast<const uint32_t*>(&h);
+        for (int i = 0; i < kMT; ++i) {
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            mma16816(acc[i][2 * j + t], al[i], bh[2 * t], bh[2 * t + 1]);
+            mma16816(acc[i][2 * j + t], ah[i], bl[2 * t], bl[2 * t + 1]);
+            mma16816(acc[i][2 * j + t], ah[i], bh[2 * t], bh[2 * t + 1]);
+          }
         }
-        *reinterpret_cast<uint4*>(dst) = make_uint4(p[0], p[1], p[2], p[3]);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (i0 + i < s.r) dst[i] = __float2bfloat16_rn(acc[i][j]);
       }
     }
-  }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kMT; ++i)
+#pragma unroll
+      for (int j = 0; j < kNT; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; e += 2) {
+          const int row = i * 16 + (lane >> 2) + (e >> 1) * 8, col = warp * kNT * 8 + j * 8 + (lane & 3) * 2;
+          const __nv_bfloat162 v = __floats2bfloat162_rn(acc[i][j][e] * factor, acc[i][j][e + 1] * factor);
+          if (!s.tall) {
+            *reinterpret_cast<__nv_bfloat162*>(staged + row * kWidePitch + col) = v;
+          } else {
+            staged[col * kTallPitch + row] = __low2bfloat16(v);
+            staged[(col + 1) * kTallPitch + row] = __high2bfloat16(v);
+          }
+        }
+    __syncthreads();
+    // whole rows of the result: of kC columns, or (tall) of r values
+    const int rows = s.tall ? min(kC, s.c - c0) : s.r, width = s.tall ? s.r : min(kC, s.c - c0);
+    const int64_t pitch = s.tall ? s.r : s.c;
+    __nv_bfloat16* to = out + (s.tall ? static_cast<int64_t>(c0) * s.r : c0);
+    const int from_pitch = s.tall ? kTallPitch : kWidePitch;
+    if (s.out_wide) {
+      const int per_row = width / 8;
+      for (int e = threadIdx.x; e < rows * per_row; e += kThreads) {
+        const int row = e / per_row, col = e % per_row * 8;
+        *reinterpret_cast<uint4*>(to + row * pitch + col) = *reinterpret_cast<const uint4*>(staged + row * from_pitch + col);
+      }
+    } else {
+      for (int e = threadIdx.x; e < rows * width; e += kThreads) {
+        const int row = e / width, col = e % width;
+        to[row * pitch + col] = staged[row * from_pitch + col];
+      }
+    }
   }
 }
 
 template <int kSide, int kKind>
 int launch_typed(const Small& s, cudaStream_t stream) {
   constexpr int kIterateBytes = 4 * kSide * (kSide + 4) * 4;
-  constexpr int kApplyBytes = kSide * Tile<kSide, kApplyCols<kSide>, kKind>::kPitch * 4 + kSide * kSide * 4;
+  constexpr int kApplyBytes = 2 * (2 * kTileHalves<kSide> + 2 * kSide * (kSide + 8));
   static std::once_flag once;
   static cudaError_t attr_err = cudaSuccess;
   std::call_once(once, [] {
@@ -391,7 +542,7 @@ int launch_typed(const Small& s, cudaStream_t stream) {
   const int rc = launch_dependent("small_iterate_kernel", small_iterate_kernel<kSide>, dim3(batch),
                                   dim3(kIterateThreads<kSide>), kIterateBytes, stream, s);
   if (rc != MOSS_OK) return rc;
-  const int tiles = (s.c + kApplyCols<kSide> - 1) / kApplyCols<kSide>;
+  const int tiles = (s.c + kCols<kSide> - 1) / kCols<kSide>;
   return launch_dependent("small_apply_kernel", small_apply_kernel<kSide, kKind>, dim3(std::min(tiles, s.chunks), batch),
                           dim3(kThreads), kApplyBytes, stream, s);
 }
@@ -406,11 +557,12 @@ int launch_side(const Small& s, cudaStream_t stream) {
 
 int small_side(int r) { return r <= 16 ? 16 : r <= 32 ? 32 : 64; }
 
-// Column ranges per matrix: enough CTAs for the GPU (two a multiprocessor), no more than there are tiles.
+// Column ranges per matrix: one round of the GPU (two CTAs a multiprocessor; two rounds took 25 us for the Gram
+// pass of 144 x 32 x 3072 instead of 20), no more than there are tiles.
 int small_chunks(int64_t batch, int r, int c, int sms) {
-  const int cols = 4096 / small_side(r);
+  const int cols = 8192 / small_side(r);
   const int64_t ranges = (c + cols - 1) / cols;
-  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(ranges, 4LL * sms / std::max<int64_t>(1, batch))));
+  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(ranges, 2LL * sms / std::max<int64_t>(1, batch))));
 }
 
 int launch_small(const Small& s, cudaStream_t stream) {

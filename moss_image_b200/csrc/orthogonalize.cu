@@ -197,7 +197,7 @@ static int launch_normalize(const void* g, int64_t batch, int r, int c, int rp, 
 struct Layout {
   int r, c, rp, cp, side, chunks;
   bool tall, small;
-  size_t x[2], low[2], a, b, parts, partial, q, total;
+  size_t x[2], low[2], a, b, parts, partial, q, factors, total;
 };
 
 static Layout layout_of(int64_t batch, int64_t rows, int64_t cols) {
@@ -218,6 +218,7 @@ static Layout layout_of(int64_t batch, int64_t rows, int64_t cols) {
     const size_t square = static_cast<size_t>(l.side) * l.side * 4 * batch;
     l.partial = take(square * l.chunks);
     l.q = take(square);
+    l.factors = take(static_cast<size_t>(batch) * 8);
   } else {
     l.rp = (l.r + 127) / 128 * 128;
     l.cp = (l.c + 127) / 128 * 128;
@@ -307,13 +308,14 @@ static int run(const void* g, int dtype, int64_t batch, int64_t rows, int64_t co
     s.steps = steps;
     const int64_t inner = l.tall ? l.r : l.c;
     s.wide = inner % 4 == 0 && reinterpret_cast<uintptr_t>(g) % 16 == 0;
-    s.out_wide = inner % (l.tall ? 8 : 4) == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0;
+    s.out_wide = inner % 8 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0;
     std::memcpy(s.coefficients, coefficients, sizeof(float) * 3 * steps);
     s.eps = eps;
     s.out = out;
     s.chunks = l.chunks;
     s.partial = reinterpret_cast<float*>(ws + l.partial);
-    s.q = reinterpret_cast<float*>(ws + l.q);
+    s.q = reinterpret_cast<__half*>(ws + l.q);
+    s.factors = reinterpret_cast<float*>(ws + l.factors);
     rc = launch_small(s, stream);
     return rc == MOSS_OK ? clear_ok() : rc;
   }
