@@ -105,20 +105,20 @@ def _workspace_bytes(m: int, n_out: int, k_red: int) -> int:
 
 def _check(tokens: torch.Tensor, weight: torch.Tensor, scale: torch.Tensor, side: int, what: str) -> None:
     """``side``: the weight dimension that the input's last one has to match."""
-    device = tokens.device
-    if device.type != "cuda":
+    if not tokens.is_cuda:
         raise RuntimeError(f"{what} runs on CUDA tensors only (there is no CPU path).")
     if tokens.dtype not in _FLOATS:
         raise ValueError(f"{what}: the input must be float16, bfloat16 or float32.")
-    if weight.device != device or scale.device != device:
+    device = tokens.get_device()
+    if weight.get_device() != device or scale.get_device() != device:
         raise ValueError(f"{what}: the weight and its scales must be on the input's device.")
     if weight.dtype != torch.float8_e4m3fn or weight.ndim != 2 or scale.dtype != torch.float32:
         raise ValueError(f"{what}: the weight must be float8_e4m3fn [out, in] with float32 scales.")
-    n, k = weight.shape
-    if scale.shape != (_blocks(n), _blocks(k)) or not scale.is_contiguous():
+    n, k = shape = weight.shape
+    if scale.shape != (-(-n // BLOCK), -(-k // BLOCK)) or not scale.is_contiguous():
         raise ValueError(f"{what}: the scales must be a contiguous [ceil(out / 128), ceil(in / 128)] tensor.")
-    if tokens.ndim < 1 or tokens.shape[-1] != (n, k)[side]:
-        raise ValueError(f"{what}: the input's last dimension must be {(n, k)[side]}.")
+    if tokens.ndim < 1 or tokens.shape[-1] != shape[side]:
+        raise ValueError(f"{what}: the input's last dimension must be {shape[side]}.")
     pitch, step = weight.stride()
     if n and k and (step != 1 or pitch % 16 or pitch < k or weight.data_ptr() % 16):
         raise ValueError(f"{what}: the weight's rows must be 16-byte aligned (lay_out_fp8_codes).")
@@ -129,7 +129,7 @@ def _output(tokens: torch.Tensor, width: int, dtype: torch.dtype, out: torch.Ten
     if dtype not in _FLOATS:
         raise ValueError(f"{what}: the output must be float16, bfloat16 or float32.")
     if out is None:
-        return torch.empty(shape, dtype=dtype, device=tokens.device)
+        return tokens.new_empty(shape) if dtype is tokens.dtype else tokens.new_empty(shape, dtype=dtype)
     if tuple(out.shape) != shape or out.dtype != dtype or out.device != tokens.device or not out.is_contiguous():
         raise ValueError(f"{what}: the output buffer has the wrong shape, dtype or device or is not contiguous.")
     return out

@@ -135,25 +135,26 @@ def apply_rotary(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor, sin: torch
     """
     if not q.is_cuda:
         raise RuntimeError("apply_rotary runs on CUDA tensors only (there is no CPU path).")
-    device = q.device
-    if k.device != device or cos.device != device or sin.device != device:
+    device = q.get_device()
+    if k.get_device() != device or cos.get_device() != device or sin.get_device() != device:
         raise ValueError("apply_rotary: q, k, cos and sin must be on one device.")
     if q.dtype != k.dtype or q.dtype not in _lib.DTYPE_CODES:
         raise ValueError("apply_rotary: q and k must have one dtype of float16, bfloat16 or float32.")
-    if q.ndim not in (3, 4) or q.ndim != k.ndim or q.shape[:-2] != k.shape[:-2] or q.shape[-1] != k.shape[-1]:
+    q_shape, k_shape = q.shape, k.shape
+    if q.ndim not in (3, 4) or q.ndim != k.ndim or q_shape[:-2] != k_shape[:-2] or q_shape[-1] != k_shape[-1]:
         raise ValueError("apply_rotary: q and k must agree in all dimensions but the heads.")
     if cos.dtype != torch.float32 or sin.dtype != torch.float32 or cos.ndim != 2 or cos.shape != sin.shape:
         raise ValueError("apply_rotary: cos and sin must be float32 [rows, rotary_dim / 2].")
-    if 2 * cos.shape[1] > q.shape[-1]:
+    if 2 * cos.shape[1] > q_shape[-1]:
         raise ValueError("apply_rotary: the table turns more values than a head has.")
-    tokens = q.shape[-3]
+    tokens = q_shape[-3]
     if positions is None:
         if cos.shape[0] < tokens:
             raise ValueError("apply_rotary: the table has fewer rows than there are tokens.")
     else:
-        if positions.device != device or positions.dtype != torch.int64:
+        if positions.get_device() != device or positions.dtype != torch.int64:
             raise ValueError("apply_rotary: positions must be int64 on the tensors' device.")
-        if tuple(positions.shape) not in ((tokens,), tuple(q.shape[:-2])):
+        if tuple(positions.shape) not in ((tokens,), tuple(q_shape[:-2])):
             raise ValueError("apply_rotary: positions must be [tokens] or [batch, tokens].")
         positions = positions.contiguous()
     cos, sin = cos.contiguous(), sin.contiguous()
