@@ -1,8 +1,8 @@
 // The products of a Newton-Schulz step on the tensor cores (tcgen05.mma.kind::f16, f32 sums).
 //
-// Two shapes of one kernel: a CTA pair on 256 x 256 tiles where those fill the GPU, one CTA on
-// 128 x 128 tiles where they do not. Warp 0 streams 128-wide reduction steps by TMA (one box of
-// 32 KB per operand), warp 1 issues the MMAs into one of two TMEM accumulators, warps 2-9 drain the
+// Three shapes of one kernel: a CTA pair on 256 x 256 tiles where those fill the GPU, one CTA on
+// 128 x 128 or 128 x 64 tiles where they do not. Warp 0 streams 128-wide reduction steps by TMA (one
+// box per operand), warp 1 issues the MMAs into one of two TMEM accumulators, warps 2-9 drain the
 // other. A and B are symmetric: only tiles on and above the diagonal are computed, and written
 // twice; both orders of a diagonal tile's products sum alike, so A and B stay symmetric bit for
 // bit, and the update may read B by rows. X is read by columns there (MN-major), from the same
@@ -23,20 +23,29 @@ namespace {
 
 constexpr int kHalf = 128;
 constexpr int kStep = 128;  // reduction indices per stage: two 64-wide boxes
-constexpr int kStages = 3;
 constexpr int kEpiWarp0 = 2;
 constexpr int kEpiWarps = 8;  // two per quarter of the lanes, each with half of the columns
 constexpr int kThreads = (kEpiWarp0 + kEpiWarps) * 32;
-constexpr uint32_t kTileBytes = kHalf * kStep * 2;  // 32 KB
-constexpr uint32_t kStageBytes = 2 * kTileBytes;
-constexpr uint32_t kDataBytes = kStages * kStageBytes;
-constexpr uint32_t kSmemBytes = kDataBytes + 1024 + 512;
-constexpr long long kExitBudgetCycles = (kStages + 4) * kWaitBudgetCycles;
-static_assert(kSmemBytes <= 227 * 1024, "rings exceed the shared memory a CTA may use");
+constexpr int kMaxStages = 4;
+constexpr uint32_t kLeftBytes = kHalf * kStep * 2;  // 32 KB
+
+// kN: columns of a tile (of the pair's, where there is one).
+template <int kCtas, int kN>
+struct Shape {
+  static constexpr int kTileM = kHalf * kCtas;
+  static constexpr int kRight = kN / kCtas;  // columns this CTA holds of the right operand
+  static constexpr uint32_t kRightBytes = kRight * kStep * 2;
+  static constexpr uint32_t kStageBytes = kLeftBytes + kRightBytes;
+  static constexpr int kStages = kRight == 64 ? 4 : 3;
+  static constexpr uint32_t kDataBytes = kStages * kStageBytes;
+  static constexpr uint32_t kSmemBytes = kDataBytes + 1024 + 512;
+  static_assert(kSmemBytes <= 227 * 1024, "rings exceed the shared memory a CTA may use");
+};
+constexpr long long kExitBudgetCycles = (kMaxStages + 4) * kWaitBudgetCycles;
 
 struct Barriers {
-  uint64_t full[kStages];   // leader: both CTAs' operands landed
-  uint64_t empty[kStages];  // local
+  uint64_t full[kMaxStages];   // leader: both CTAs' operands landed
+  uint64_t empty[kMaxStages];  // local
   uint64_t acc_full[2];     // local
   uint64_t acc_empty[2];    // leader
   uint64_t drain;
@@ -70,12 +79,16 @@ __device__ __forceinline__ void upper_tile(int t, int& m, int& n) {
   m = t - n * (n + 1) / 2;
 }
 
-template <Mode kMode>
+// Unit u: matrix b, row tile m, column tile n (of kN columns; a 128-row tile's diagonal block is two of 64).
+template <Mode kMode, int kN>
 __device__ __forceinline__ void locate(const Args& a, int u, int& b, int& m, int& n) {
   b = u / a.tiles;
   const int t = u - b * a.tiles;
   if constexpr (kMode == kUpdate) {
     gemm::tile_coords(t, a.tiles_m, a.tiles_n, m, n);
+  } else if constexpr (kN == 64) {
+    upper_tile(t >> 1, m, n);
+    n = 2 * n + (t & 1);
   } else {
     upper_tile(t, m, n);
   }
@@ -190,17 +203,19 @@ __device__ __forceinline__ void finish32(const Args& a, int b, int i, int j, boo
   }
 }
 
-template <Mode kMode, int kCtas>
+template <Mode kMode, int kCtas, int kN>
 __global__ void __launch_bounds__(kThreads, 1)
     ns_gemm_kernel(const __grid_constant__ CUtensorMap tm_left, const __grid_constant__ CUtensorMap tm_right,
                    const Args args) {
   constexpr bool kColumns = kMode == kUpdate;  // the right operand is read by columns (MN-major)
-  constexpr int kTile = kHalf * kCtas;
-  constexpr uint32_t kTmemCols = 2 * kTile;
+  using S = Shape<kCtas, kN>;
+  constexpr int kTileM = S::kTileM, kStages = S::kStages;
+  constexpr uint32_t kStageBytes = S::kStageBytes;
+  constexpr uint32_t kTmemCols = 2 * kN;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_base = smem_u32(smem_raw);
   const uint32_t base = (raw_base + 1023u) & ~1023u;
-  Barriers* bars = reinterpret_cast<Barriers*>(smem_raw + (base - raw_base) + kDataBytes);
+  Barriers* bars = reinterpret_cast<Barriers*>(smem_raw + (base - raw_base) + S::kDataBytes);
   auto bar = [&](uint64_t& b) { return smem_u32(&b); };
   volatile int* abort_flag = &bars->abort_flag;
   const int warp = threadIdx.x >> 5;
@@ -256,9 +271,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     bool ok = true;
     for (int u = first_unit; u < num_units && ok; u += unit_step) {
       int b, m, n;
-      locate<kMode>(args, u, b, m, n);
-      const int m0 = b * args.rp + m * kTile + static_cast<int>(rank) * kHalf;  // row of the left operand
-      const int n0 = n * kTile + static_cast<int>(rank) * kHalf;                // this CTA's columns
+      locate<kMode, kN>(args, u, b, m, n);
+      const int m0 = b * args.rp + m * kTileM + static_cast<int>(rank) * kHalf;  // row of the left operand
+      const int n0 = n * kN + static_cast<int>(rank) * S::kRight;                // this CTA's columns
       for (int s = 0; s < steps; ++s) {
         if (!mbar_wait_cluster(bar(bars->empty[stage]), phase ^ 1u, abort_flag, args.status,
                                MOSS_STATUS_TIMEOUT_LOAD)) {
@@ -273,11 +288,11 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (leader) mbar_arrive_expect_tx(bar(bars->full[stage]), kCtas * kStageBytes);
             const uint32_t fb = mapa_shared(bar(bars->full[stage]), 0);
             tma_load_3d_pair(dst, &tm_left, fb, 0, m0, s * 2);
-            tma_load_3d_pair(dst + kTileBytes, &tm_right, fb, 0, ry, rz);
+            tma_load_3d_pair(dst + kLeftBytes, &tm_right, fb, 0, ry, rz);
           } else {
             mbar_arrive_expect_tx(bar(bars->full[stage]), kStageBytes);
             tma_load_3d(dst, &tm_left, bar(bars->full[stage]), 0, m0, s * 2);
-            tma_load_3d(dst + kTileBytes, &tm_right, bar(bars->full[stage]), 0, ry, rz);
+            tma_load_3d(dst + kLeftBytes, &tm_right, bar(bars->full[stage]), 0, ry, rz);
           }
           used |= 1u << stage;
           last_phase = (last_phase & ~(1u << stage)) | (phase << stage);
@@ -301,11 +316,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else if (warp == 1) {
     // ---------------------------------------------------------------- MMA issuer (leader)
     if (leader) {
-      constexpr uint32_t idesc = umma_idesc_f16(0u, kColumns, kTile, kTile);
+      constexpr uint32_t idesc = umma_idesc_f16(0u, kColumns, kTileM, kN);
       // descriptors of the first stage; every other differs by multiples of 16 bytes in the address field.
-      // K-major: [2 boxes][128 rows][64 values]; by columns: [2 boxes of 64 columns][128 rows]
+      // K-major: [2 boxes][rows][64 values]; by columns: [boxes of 64 columns][128 rows]
       const uint64_t left0 = umma_desc_sw128(base, 16, 1024);
-      const uint64_t right0 = umma_desc_sw128(base + kTileBytes, kColumns ? kTileBytes / 2 : 16, 1024);
+      const uint64_t right0 = umma_desc_sw128(base + kLeftBytes, kColumns ? 16384 : 16, 1024);
       int stage = 0, it = 0;
       uint32_t phase = 0;
       bool ok = true, issued = false;
@@ -315,7 +330,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                                MOSS_STATUS_TIMEOUT_MMA))
           break;
         tc_fence_after();
-        const uint32_t d = tmem_base + static_cast<uint32_t>(acc * kTile);
+        const uint32_t d = tmem_base + static_cast<uint32_t>(acc * kN);
         for (int s = 0; s < steps; ++s) {
           if (!mbar_wait_cluster(bar(bars->full[stage]), phase, abort_flag, args.status, MOSS_STATUS_TIMEOUT_MMA)) {
             ok = false;
@@ -326,9 +341,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             const uint64_t at_stage = static_cast<uint64_t>(stage) * (kStageBytes >> 4);
 #pragma unroll
             for (int kk = 0; kk < kStep / 16; ++kk) {
-              const uint32_t rows = ((kk >> 2) * (kTileBytes / 2) + (kk & 3) * 32) >> 4;
-              const uint64_t ld = left0 + at_stage + rows;
-              const uint64_t rd = right0 + at_stage + (kColumns ? (kk * 2048) >> 4 : rows);
+              const uint64_t ld = left0 + at_stage + (((kk >> 2) * (kLeftBytes / 2) + (kk & 3) * 32) >> 4);
+              const uint64_t rd = right0 + at_stage +
+                                  ((kColumns ? kk * 2048 : (kk >> 2) * (S::kRightBytes / 2) + (kk & 3) * 32) >> 4);
               if constexpr (kCtas == 2)
                 umma_f16_pair(d, ld, rd, idesc, (s > 0 || kk > 0) ? 1u : 0u);
               else
@@ -369,20 +384,20 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else {
     // ---------------------------------------------------------------- epilogue (every CTA)
-    constexpr int kGroups = kTile / 2 / 32;  // groups of 32 columns of one warp
+    constexpr int kGroups = kN / 2 / 32;  // groups of 32 columns of one warp
     const int q = warp & 3;
     const int half = (warp - kEpiWarp0) >> 2;
-    const uint32_t lane_addr = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(half * (kTile / 2));
+    const uint32_t lane_addr = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(half * (kN / 2));
     const int cols = kMode == kUpdate ? args.cp : args.rp;
     int it = 0;
     for (int u = first_unit; u < num_units; u += unit_step, ++it) {
       int b, m, n;
-      locate<kMode>(args, u, b, m, n);
-      const int i = m * kTile + static_cast<int>(rank) * kHalf + q * 32 + lane;
-      const int j0 = n * kTile + half * (kTile / 2);
+      locate<kMode, kN>(args, u, b, m, n);
+      const int i = m * kTileM + static_cast<int>(rank) * kHalf + q * 32 + lane;
+      const int j0 = n * kN + half * (kN / 2);
       Added added[2];
       fetch32<kMode>(args, b, i, j0, added[0]);
-      fetch32<kMode>(args, b, i, j0 + 32, added[1]);
+      if constexpr (kGroups > 1) fetch32<kMode>(args, b, i, j0 + 32, added[1]);
       const int acc = it & 1;
       if (!mbar_wait_cluster(bar(bars->acc_full[acc]), (it >> 1) & 1, abort_flag, args.status,
                              MOSS_STATUS_TIMEOUT_EPILOGUE))
@@ -391,7 +406,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
       for (int c = 0; c < kGroups; ++c) {
         uint32_t r[32];
-        tmem_ld_32x32b_x32(lane_addr + static_cast<uint32_t>(acc * kTile + c * 32), r);
+        tmem_ld_32x32b_x32(lane_addr + static_cast<uint32_t>(acc * kN + c * 32), r);
         tmem_wait_ld();
         if (c == kGroups - 1) {
           tc_fence_before();
@@ -409,7 +424,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           float v[32];
 #pragma unroll
           for (int e = 0; e < 32; ++e) v[e] = __uint_as_float(r[e]);
-          finish32<kMode>(args, b, i, j, m != n, added[c & 1], v);
+          finish32<kMode>(args, b, i, j, kN == 64 ? m != n >> 1 : m != n, added[c & 1], v);
         }
         if (c + 2 < kGroups) fetch32<kMode>(args, b, i, j + 64, added[c & 1]);
       }
@@ -442,9 +457,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-template <Mode kMode, int kCtas>
+template <Mode kMode, int kCtas, int kN>
 int launch_typed(const CUtensorMap& tl, const CUtensorMap& tr, Args a, cudaStream_t stream) {
-  auto kern = ns_gemm_kernel<kMode, kCtas>;
+  constexpr uint32_t kSmemBytes = Shape<kCtas, kN>::kSmemBytes;
+  auto kern = ns_gemm_kernel<kMode, kCtas, kN>;
   static std::once_flag once;
   static cudaError_t attr_err = cudaSuccess;
   static int max_groups = 0;
@@ -474,10 +490,9 @@ int launch_typed(const CUtensorMap& tl, const CUtensorMap& tr, Args a, cudaStrea
     }
   });
   MOSS_CUDA_TRY(attr_err);
-  const int side = kHalf * kCtas;
-  a.tiles_m = (a.rp + side - 1) / side;
-  a.tiles_n = kMode == kUpdate ? (a.cp + side - 1) / side : a.tiles_m;
-  a.tiles = kMode == kUpdate ? a.tiles_m * a.tiles_n : a.tiles_m * (a.tiles_m + 1) / 2;
+  a.tiles_m = (a.rp + kHalf * kCtas - 1) / (kHalf * kCtas);
+  a.tiles_n = ((kMode == kUpdate ? a.cp : a.rp) + kN - 1) / kN;
+  a.tiles = kMode == kUpdate ? a.tiles_m * a.tiles_n : a.tiles_m * (a.tiles_m + 1) / 2 * (kN == 64 ? 2 : 1);
   const int64_t units = static_cast<int64_t>(a.tiles) * a.batch;
   if (units > INT32_MAX) return fail(MOSS_ERR_INVALID_ARGUMENT, "too many matrices to orthogonalize in one call");
   cfg.gridDim = dim3(static_cast<unsigned>(kCtas * std::min<int64_t>(units, max_groups)));
@@ -486,43 +501,55 @@ int launch_typed(const CUtensorMap& tl, const CUtensorMap& tr, Args a, cudaStrea
   return check_cuda(cudaLaunchKernelEx(&cfg, kern, tl, tr, a), "ns_gemm_kernel");
 }
 
-// Pair tiles where their rounds over the GPU take no longer than those of 128 x 128 tiles. A pair
-// tile's stage lasts twice as long for four times the products; a single tile reads twice the
-// shared memory for each (the factor 1.3).
-bool use_pair(Mode mode, const Args& a) {
-  const int sms = sm_count();
-  auto tiles = [&](int side) {
-    const int64_t tm = (a.rp + side - 1) / side, tn = (a.cp + side - 1) / side;
-    return (mode == kUpdate ? tm * tn : tm * (tm + 1) / 2) * a.batch;
+// The tile columns (256: a pair) whose rounds over the GPU take least. Relative cost of a round: a pair tile
+// has four times the products of a 128 x 128 one in twice its MMA time; single tiles are bound by what a
+// multiprocessor can read, 64 KB a step for 128 columns and 48 KB for 64 (700 and 530 cycles measured).
+int tile_columns(Mode mode, const Args& a) {
+  const int64_t sms = sm_count();
+  auto rounds = [&](int64_t tm, int64_t tn, int64_t slots) {
+    const int64_t tiles = mode == kUpdate ? tm * tn : tm * (tm + 1) / 2 * (tn / tm);
+    return (tiles * a.batch + slots - 1) / slots;
   };
-  const int64_t pairs = std::max(1, sms / 2);
-  const int64_t pair_cost = (tiles(256) + pairs - 1) / pairs * 20;
-  const int64_t single_cost = (tiles(128) + sms - 1) / sms * 13;
-  return pair_cost <= single_cost;
+  const int64_t cols = mode == kUpdate ? a.cp : a.rp;
+  const int64_t pair = rounds((a.rp + 255) / 256, (cols + 255) / 256, std::max<int64_t>(1, sms / 2)) * 20;
+  const int64_t wide = rounds(a.rp / 128, cols / 128, sms) * 13;
+  const int64_t narrow = rounds(a.rp / 128, cols / 64, sms) * 9;
+  if (pair <= wide && pair <= narrow) return 256;
+  return wide <= narrow ? 128 : 64;
+}
+
+template <Mode kMode>
+int launch_mode(int columns, const CUtensorMap& tl, const CUtensorMap& tr, const Args& a, cudaStream_t stream) {
+  if (columns == 256) return launch_typed<kMode, 2, 256>(tl, tr, a, stream);
+  if (columns == 128) return launch_typed<kMode, 1, 128>(tl, tr, a, stream);
+  return launch_typed<kMode, 1, 64>(tl, tr, a, stream);
 }
 
 }  // namespace
 
 int launch_gemm(Mode mode, const __half* left, const __half* right, const Args& a, cudaStream_t stream) {
-  // [batch * rp][cols] viewed as {64, rows, cols / 64}: a box is 128 rows of two 64-wide columns
-  auto map = [&](CUtensorMap* m, const __half* p, int cols) {
+  const int columns = tile_columns(mode, a);
+  const uint32_t held = columns == 64 ? 64 : 128;  // columns of the right operand in one CTA
+  // [batch * rp][cols] viewed as {64, rows, cols / 64}: a box is rows of 64-wide columns
+  auto map = [&](CUtensorMap* m, const __half* p, int cols, uint32_t rows, uint32_t wide) {
     memset(m, 0, sizeof(*m));
     const uint64_t dims[3] = {64, static_cast<uint64_t>(a.batch) * a.rp, static_cast<uint64_t>(cols / 64)};
     const uint64_t strides[2] = {static_cast<uint64_t>(cols) * 2, 128};
-    const uint32_t box[3] = {64, 128, 2};
+    const uint32_t box[3] = {64, rows, wide};
     return gemm::make_map_nd(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, p, 3, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
   };
   CUtensorMap tl, tr;
-  if (!map(&tl, left, mode == kGram ? a.cp : a.rp) || !map(&tr, right, mode == kSquare ? a.rp : a.cp))
+  const bool by_columns = mode == kUpdate;
+  if (!map(&tl, left, mode == kGram ? a.cp : a.rp, 128, 2) ||
+      !map(&tr, right, mode == kSquare ? a.rp : a.cp, by_columns ? 128 : held, by_columns ? held / 64 : 2))
     return fail(MOSS_ERR_CUDA, "the driver refused a tensor map of the orthogonalised update");
-  const bool pair = use_pair(mode, a);
   switch (mode) {
     case kGram:
-      return pair ? launch_typed<kGram, 2>(tl, tr, a, stream) : launch_typed<kGram, 1>(tl, tr, a, stream);
+      return launch_mode<kGram>(columns, tl, tr, a, stream);
     case kSquare:
-      return pair ? launch_typed<kSquare, 2>(tl, tr, a, stream) : launch_typed<kSquare, 1>(tl, tr, a, stream);
+      return launch_mode<kSquare>(columns, tl, tr, a, stream);
     default:
-      return pair ? launch_typed<kUpdate, 2>(tl, tr, a, stream) : launch_typed<kUpdate, 1>(tl, tr, a, stream);
+      return launch_mode<kUpdate>(columns, tl, tr, a, stream);
   }
 }
 
