@@ -21,6 +21,9 @@ constexpr float kAmaxFloor = 7.888609052210118e-31f;  // 2^-100
 
 struct Args {
   int M, Nc, kb;            // rows, output columns, reduction blocks
+  const void* x;            // the rows themselves, for the kernel that quantises them
+  int x_kind, x_wide;       // x_wide: 8 values at a time are aligned and whole
+  int64_t x_cols;
   const float* row_scale;   // [kb][row_pitch]
   int64_t row_pitch;
   const float* w_scale;     // element (block of the column, reduction block) at cb * ws_col + kb * ws_red
@@ -44,6 +47,7 @@ struct Plan {
   int tiles_m = 0, tiles_n = 0;
   int splits = 1, kb_per_split = 0;
 };
+constexpr int kRowsQuantised = 32;  // the few-row kernel quantises up to this many rows itself
 Plan make_plan(int64_t m, int64_t nc, int64_t kr, int sms);
 
 int sm_count();

@@ -56,8 +56,9 @@ static Layout layout_of(int64_t m, int64_t nc, int64_t kr, const Plan& p) {
   const int64_t kb = ceil_div(kr, kBlock);
   l.row_pitch = ceil_div(m, 128) * 128;
   l.codes = 0;
-  l.scale = up(static_cast<size_t>(m) * kb * kBlock);
-  l.partial = l.scale + up(static_cast<size_t>(kb) * l.row_pitch * 4);
+  const bool codes = m > kRowsQuantised;
+  l.scale = codes ? up(static_cast<size_t>(m) * kb * kBlock) : 0;
+  l.partial = l.scale + (codes ? up(static_cast<size_t>(kb) * l.row_pitch * 4) : 0);
   if (p.splits > 1) {
     const size_t values = p.kind == Plan::kRows ? static_cast<size_t>(m) * nc
                                                 : static_cast<size_t>(p.tiles_m) * p.tiles_n * 128 * 128;
@@ -146,7 +147,8 @@ static int run(bool dx, const void* x, int x_dtype, int64_t m, int64_t n, int64_
                 static_cast<long long>(ld), static_cast<long long>(k));
   const Plan plan = make_plan(m, nc, kr, sm_count());
   const Layout l = layout_of(m, nc, kr, plan);
-  if (workspace == nullptr || workspace_bytes < l.total || reinterpret_cast<uintptr_t>(workspace) % 256 != 0)
+  if (l.total > 0 &&
+      (workspace == nullptr || workspace_bytes < l.total || reinterpret_cast<uintptr_t>(workspace) % 256 != 0))
     return fail(MOSS_ERR_INVALID_ARGUMENT, "the fp8 linear needs %zu bytes of 256-byte aligned workspace", l.total);
   uint8_t* ws = static_cast<uint8_t*>(workspace);
 
@@ -154,6 +156,10 @@ static int run(bool dx, const void* x, int x_dtype, int64_t m, int64_t n, int64_
   a.M = static_cast<int>(m);
   a.Nc = static_cast<int>(nc);
   a.kb = static_cast<int>(ceil_div(kr, kBlock));
+  a.x = x;
+  a.x_kind = x_dtype;
+  a.x_cols = kr;
+  a.x_wide = kr % 8 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0;
   a.row_scale = reinterpret_cast<float*>(ws + l.scale);
   a.row_pitch = l.row_pitch;
   a.w_scale = scale;
@@ -182,15 +188,18 @@ static int run(bool dx, const void* x, int x_dtype, int64_t m, int64_t n, int64_
   memset(&ta, 0, sizeof(ta));
   memset(&tw, 0, sizeof(tw));
   const uint32_t rows_box = plan.kind == Plan::kRows ? plan.tn : 128;
-  if (!gemm::make_map(&ta, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, ws + l.codes, static_cast<uint64_t>(a.kb) * kBlock, m,
-                      static_cast<uint64_t>(a.kb) * kBlock, kBlock, rows_box, CU_TENSOR_MAP_SWIZZLE_128B) ||
+  const bool quantises = m <= kRowsQuantised;
+  if ((!quantises && !gemm::make_map(&ta, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, ws + l.codes, static_cast<uint64_t>(a.kb) * kBlock, m,
+                      static_cast<uint64_t>(a.kb) * kBlock, kBlock, rows_box, CU_TENSOR_MAP_SWIZZLE_128B)) ||
       !gemm::make_map(&tw, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, codes, k, n, ld, kBlock, 128, CU_TENSOR_MAP_SWIZZLE_128B))
     return fail(MOSS_ERR_CUDA, "the driver refused a tensor map of the fp8 linear");
   if (plan.kind != Plan::kRows && out_dtype != kF32)
     a.tma_out = gemm::make_map(&to, out_dtype == kBF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
                                2, out, nc, m, static_cast<uint64_t>(nc) * 2, 64, 128, CU_TENSOR_MAP_SWIZZLE_128B);
-  rc = launch_quantize_rows(x, x_dtype, m, kr, ws + l.codes, reinterpret_cast<float*>(ws + l.scale), l.row_pitch, stream);
-  if (rc != MOSS_OK) return rc;
+  if (!quantises) {
+    rc = launch_quantize_rows(x, x_dtype, m, kr, ws + l.codes, reinterpret_cast<float*>(ws + l.scale), l.row_pitch, stream);
+    if (rc != MOSS_OK) return rc;
+  }
   rc = plan.kind == Plan::kRows ? launch_rows(dx, plan, ta, tw, a, stream) : launch_gemm(dx, plan, ta, tw, to, a, stream);
   if (rc != MOSS_OK) return rc;
   if (plan.splits > 1 && plan.kind != Plan::kRows) {

@@ -8,11 +8,10 @@
 //
 // Both are bound by HBM: 2 bytes read and 1 written per value. A half-warp holds one row's 128
 // columns (16 bytes a lane), so the maximum is four shuffles away and the values are read once.
-#include <cuda_fp8.h>
-
 #include <algorithm>
 
 #include "fp8_args.cuh"
+#include "fp8_codes.cuh"
 
 namespace moss {
 namespace fp8 {
@@ -24,132 +23,13 @@ constexpr int kRowsPerCta = kThreads / 16;
 template <int kKind>
 constexpr int kBatch = kKind == kF32 ? 4 : 8;
 
-template <int kKind>
-struct Raw {  // 8 values
-  uint32_t w[kKind == kF32 ? 8 : 4];
-};
-
-// 8 consecutive values of a row from column c0, zero past k.
-template <int kKind>
-__device__ __forceinline__ void load8(const void* x, int64_t row, int64_t k, int64_t c0, bool wide, float (&v)[8]) {
-  const int64_t at = row * k + c0;
-  if (wide && c0 + 8 <= k) {
-    if constexpr (kKind == kF32) {
-      const float4 a = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(x) + at));
-      const float4 b = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(x) + at) + 1);
-      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-      v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-    } else {
-      const uint4 a = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(x) + at));
-      const uint32_t p[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if constexpr (kKind == kBF16) {
-          v[2 * i] = __uint_as_float(p[i] << 16);
-          v[2 * i + 1] = __uint_as_float(p[i] & 0xffff0000u);
-        } else {
-          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&p[i]));
-          v[2 * i] = f.x;
-          v[2 * i + 1] = f.y;
-        }
-      }
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = c0 + i < k ? load_as_float(x, kKind, at + i) : 0.0f;
-  }
-}
-
-// fmaxf drops NaN; a block that holds one has to show it.
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
-
-// Exponent p of the row scale: the least with amax <= 448 * 2^p = 1.75 * 2^(p + 8).
-__device__ __forceinline__ int scale_exponent(float amax) {
-  const uint32_t bits = __float_as_uint(amax);
-  return static_cast<int>(bits >> 23) - 127 - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
-}
-__device__ __forceinline__ float pow2(int p) { return __uint_as_float(static_cast<uint32_t>(p + 127) << 23); }
-
-__device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d) {
-  const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
-  const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
-  return lo | (hi << 16);
-}
-
-template <int kKind>
-__device__ __forceinline__ Raw<kKind> load_raw(const void* x, int64_t at) {
-  Raw<kKind> r;
-  const uint4* p = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(x) + at * (kKind == kF32 ? 4 : 2));
-#pragma unroll
-  for (int i = 0; i < static_cast<int>(sizeof(r)) / 16; ++i) {
-    const uint4 v = __ldg(p + i);
-    r.w[4 * i] = v.x;
-    r.w[4 * i + 1] = v.y;
-    r.w[4 * i + 2] = v.z;
-    r.w[4 * i + 3] = v.w;
-  }
-  return r;
-}
-template <int kKind>
-__device__ __forceinline__ float amax_of(const Raw<kKind>& r) {
-  if constexpr (kKind == kF32) {
-    float m = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) m = max_nan(m, fabsf(__uint_as_float(r.w[i])));
-    return m;
-  } else if constexpr (kKind == kBF16) {
-    __nv_bfloat162 m = __habs2(*reinterpret_cast<const __nv_bfloat162*>(&r.w[0]));
-#pragma unroll
-    for (int i = 1; i < 4; ++i) m = __hmax2_nan(m, __habs2(*reinterpret_cast<const __nv_bfloat162*>(&r.w[i])));
-    return max_nan(__low2float(m), __high2float(m));
-  } else {
-    __half2 m = __habs2(*reinterpret_cast<const __half2*>(&r.w[0]));
-#pragma unroll
-    for (int i = 1; i < 4; ++i) m = __hmax2_nan(m, __habs2(*reinterpret_cast<const __half2*>(&r.w[i])));
-    return max_nan(__low2float(m), __high2float(m));
-  }
-}
-template <int kKind>
-__device__ __forceinline__ void values_of(const Raw<kKind>& r, float (&v)[8]) {
-  if constexpr (kKind == kF32) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(r.w[i]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if constexpr (kKind == kBF16) {
-        v[2 * i] = __uint_as_float(r.w[i] << 16);
-        v[2 * i + 1] = __uint_as_float(r.w[i] & 0xffff0000u);
-      } else {
-        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&r.w[i]));
-        v[2 * i] = f.x;
-        v[2 * i + 1] = f.y;
-      }
-    }
-  }
-}
-
 // Codes and scale of the half-warp's 128 columns of one row, 8 a lane.
 __device__ __forceinline__ void emit_block(const float (&v)[8], float amax, int64_t row, int block, int kb, int sub,
                                            uint8_t* codes, float* scale, int64_t row_pitch) {
-  // a block with an infinity or a NaN has no scale: NaN, and so has every product with it
-  const bool finite = amax < __uint_as_float(0x7f800000u);
-  const int p = finite ? scale_exponent(amax) : 0;
-  const float inv = pow2(-p);
-  uint2 q;
-  q.x = codes4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
-  q.y = codes4(v[4] * inv, v[5] * inv, v[6] * inv, v[7] * inv);
+  float block_scale;
+  const uint2 q = block_codes(v, amax, block_scale);
   *reinterpret_cast<uint2*>(codes + (row * kb + block) * kBlock + sub * 8) = q;
-  if (sub == 0) scale[block * row_pitch + row] = finite ? pow2(p) : __uint_as_float(0x7fffffffu);
-}
-__device__ __forceinline__ float half_warp_max(float amax) {
-#pragma unroll
-  for (int d = 8; d > 0; d >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, d));
-  return amax;
+  if (sub == 0) scale[block * row_pitch + row] = block_scale;
 }
 
 // kWide: rows on 16-byte boundaries and whole 8-value chunks (k a multiple of 8).

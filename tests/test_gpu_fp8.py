@@ -225,3 +225,26 @@ def test_refusals(cuda_device):
         fp8.FrozenFp8Linear(nn.Linear(4, 4).to(cuda_device))
     with pytest.raises(ValueError):
         fp8.FrozenFp8Linear.from_codes(codes, scale[:0])
+
+
+@pytest.mark.parametrize("m", [15, 31, 32, 33, 63])
+@pytest.mark.parametrize("k,n", [(2048, 1536), (1031, 645)])
+def test_few_rows_on_either_side_of_the_kernels(cuda_device, m, k, n):
+    """Row counts around the few-row kernel's tiles, reductions long enough to be split and their gradients."""
+    x, codes, scale, bias, grad = _problem(m, k, n, torch.float32, cuda_device, seed=2)
+    weight = _decoded(codes, scale)
+    _check(fp8.fp8_linear_forward(x, codes, scale, bias), _quantized_rows(x), weight.t(), bias)
+    _check(fp8.fp8_linear_backward(grad, codes, scale), _quantized_rows(grad), weight)
+
+
+def test_calls_replay_from_a_graph(cuda_device):
+    problems = [_problem(m, 640, 520, torch.bfloat16, cuda_device, seed=4) for m in (3, 150, 2100)]
+    want = [fp8.fp8_linear_forward(x, codes, scale, bias) for x, codes, scale, bias, _ in problems]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = [fp8.fp8_linear_forward(x, codes, scale, bias) for x, codes, scale, bias, _ in problems]
+    for x, *_ in problems:
+        x.neg_()
+    graph.replay()
+    for (x, codes, scale, bias, _), y, before in zip(problems, got, want):
+        assert torch.equal(y, fp8.fp8_linear_forward(x, codes, scale, bias)) and not torch.equal(y, before)

@@ -161,3 +161,17 @@ def test_refusals(cuda_device):
         Muon([torch.nn.Parameter(torch.zeros(4, device=cuda_device))])
     with pytest.raises(ValueError):
         Muon([torch.nn.Parameter(update)], momentum=1.0)
+
+
+def test_calls_replay_from_a_graph(cuda_device):
+    updates = [_updates("rows", shape, cuda_device, seed=9) for shape in ((5, 20, 300), (200, 330))]
+    for update in updates:
+        orthogonalize(update)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = [orthogonalize(update) for update in updates]
+    for update in updates:
+        update.copy_(update.flip(-1))
+    graph.replay()
+    for update, direction in zip(updates, got):
+        assert torch.equal(direction, orthogonalize(update))
