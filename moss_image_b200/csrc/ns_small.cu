@@ -34,21 +34,27 @@ struct Raw4 {  // four neighbouring values of G as they are stored
   uint32_t w[kKind == kF32 ? 4 : 2];
 };
 template <int kKind>
+__device__ __forceinline__ Raw4<kKind> load_whole4(const void* g, int64_t at) {
+  Raw4<kKind> r;
+  if constexpr (kKind == kF32) {
+    const uint4 v = __ldg(reinterpret_cast<const uint4*>(static_cast<const float*>(g) + at));
+    r.w[0] = v.x;
+    r.w[1] = v.y;
+    r.w[2] = v.z;
+    r.w[3] = v.w;
+  } else {
+    const uint2 v = __ldg(reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(g) + at));
+    r.w[0] = v.x;
+    r.w[1] = v.y;
+  }
+  return r;
+}
+template <int kKind>
 __device__ __forceinline__ Raw4<kKind> load_raw4(const Small& s, int64_t at, int left) {
   Raw4<kKind> r{};
   if (left <= 0) return r;
   if (s.wide) {
-    if constexpr (kKind == kF32) {
-      const uint4 v = __ldg(reinterpret_cast<const uint4*>(static_cast<const float*>(s.g) + at));
-      r.w[0] = v.x;
-      r.w[1] = v.y;
-      r.w[2] = v.z;
-      r.w[3] = v.w;
-    } else {
-      const uint2 v = __ldg(reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(s.g) + at));
-      r.w[0] = v.x;
-      r.w[1] = v.y;
-    }
+    r = load_whole4<kKind>(s.g, at);
   } else {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -103,6 +109,23 @@ struct Tile {
   Raw4<kKind> raw[kLoads];
   __device__ __forceinline__ void fetch(const Small& s, int64_t b, int c0) {
     const int64_t base = b * s.r * s.c;
+    if (s.wide && s.r == kSide && c0 + kC <= s.c) {  // a whole tile: one address, constant steps
+      if (!s.tall) {
+        const int64_t at = base + static_cast<int64_t>(threadIdx.x / (kC / 4)) * s.c + c0 + threadIdx.x % (kC / 4) * 4;
+        const int64_t step = static_cast<int64_t>(kThreads / (kC / 4)) * s.c;
+#pragma unroll
+        for (int l = 0; l < kLoads; ++l) raw[l] = load_whole4<kKind>(s.g, at + l * step);
+      } else {
+        constexpr int kSweeps = kC > kThreads ? kC / kThreads : 1;  // of the CTA over a group of four rows
+        const int col = threadIdx.x % kC, row = threadIdx.x / kC * 4;
+        const int64_t at = base + static_cast<int64_t>(c0 + col) * kSide + row;
+#pragma unroll
+        for (int l = 0; l < kLoads; ++l)
+          raw[l] = load_whole4<kKind>(s.g, at + (l % kSweeps) * kThreads * kSide +
+                                               l / kSweeps * (kC < kThreads ? 4 * (kThreads / kC) : 4));
+      }
+      return;
+    }
 #pragma unroll
     for (int l = 0; l < kLoads; ++l) {
       const int i = threadIdx.x + l * kThreads;
