@@ -98,6 +98,15 @@ __device__ __forceinline__ void quantise_rows(const Args& args, uint32_t base, f
                                               int kb1, int warp, int lane) {
   using R = Ring<kTN>;
   const int half_warp = (warp - kQuantWarp0) * 2 + (lane >> 4), sub = lane & 15;
+  // All of this split's columns of the rows are asked for at once: block by block, each would wait for DRAM.
+  constexpr int kElem = kKind == kF32 ? 4 : 2, kLines = kBlock * kElem / 128;  // 128-byte lines per row and block
+  const int rows = min(kTN, args.M - m0);
+  for (int e = (warp - kQuantWarp0) * 32 + lane; e < (kb1 - kb0) * kLines * rows; e += kQuantWarps * 32) {
+    const int64_t col = (static_cast<int64_t>(kb0) * kLines + e / rows) * (128 / kElem);
+    if (col < args.x_cols)
+      asm volatile("prefetch.global.L2 [%0];" ::"l"(static_cast<const uint8_t*>(args.x) +
+                                                    ((m0 + e % rows) * args.x_cols + col) * kElem));
+  }
   RowBlocks<kKind, kTN> next;
   next.fetch(args, m0, kb0, half_warp, sub);
   int stage = 0;
@@ -264,6 +273,9 @@ __global__ void __launch_bounds__(Ring<kTN>::kThreads, 2)
     const int feature = f0 + q * 32 + lane;
     const uint32_t lane_addr = tmem_base + (static_cast<uint32_t>(q * 32) << 16);
     const float* w_scale = args.w_scale + static_cast<int64_t>(f0 / kBlock) * args.ws_col;
+    const float bias = args.splits == 1 && args.bias != nullptr && feature < args.Nc
+                           ? load_as_float(args.bias, args.bias_kind, feature)
+                           : 0.0f;
     float sum[kTN];
 #pragma unroll
     for (int j = 0; j < kTN; ++j) sum[j] = 0.0f;
@@ -302,8 +314,6 @@ __global__ void __launch_bounds__(Ring<kTN>::kThreads, 2)
       if (lane == 0) mbar_arrive(bar(bars->acc_empty[acc]));
     }
     if (ok && feature < args.Nc) {
-      const float bias =
-          args.splits == 1 && args.bias != nullptr ? load_as_float(args.bias, args.bias_kind, feature) : 0.0f;
 #pragma unroll
       for (int j = 0; j < kTN; ++j) {
         if (m0 + j >= args.M) break;
