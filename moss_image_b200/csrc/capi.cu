@@ -37,7 +37,7 @@ bool take_debug_stall() {
 }
 }  // namespace moss
 
-extern "C" int moss_version(void) { return 101; }
+extern "C" int moss_version(void) { return 102; }
 
 extern "C" const char* moss_last_error(void) { return moss::last_error_slot().c_str(); }
 

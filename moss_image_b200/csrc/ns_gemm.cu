@@ -9,7 +9,9 @@
 // storage.
 //
 // Bound by the tensor cores at the sides the update is worth its time for: 2 r^2 c products for
-// X', half of that for A, and r^3 for B, against 4 r c + 2 r^2 values moved.
+// X', half of that for A, and r^3 for B, against 4 r c + 2 r^2 values moved. 4 x 3072 x 3072: X' 162 us
+// (1.43 PFLOP/s), A and B 100 us each (4.2 rounds of pair tiles take the time of 5). Few tiles are bound by
+// latency, 5 us a product: 1.3 us from the launch to the first tile, the steps, the epilogue.
 #include <algorithm>
 #include <cstring>
 #include <mutex>

@@ -23,6 +23,7 @@ from functools import lru_cache
 
 import torch
 from torch import nn
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 from .quant_kernels import _poll_after_backward, autocast_compute_dtype, poll_device_status, status_buffer
@@ -198,6 +199,7 @@ class _Fp8Linear(torch.autograd.Function):
         return fp8_linear_forward(tokens, weight, scale, bias, output_dtype)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, gradient):
         weight, scale = ctx.saved_tensors
         _poll_after_backward(gradient.device)

@@ -110,16 +110,18 @@ def _launch(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor, sin: torch.Tens
 
 class _Rotary(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, cos, sin, positions, interleaved):
+    def forward(ctx, q, k, cos, sin, positions, interleaved, inverse):
         ctx.save_for_backward(cos, sin, positions)
-        ctx.interleaved = interleaved
-        return _launch(q, k, cos, sin, positions, interleaved, False)
+        ctx.interleaved, ctx.inverse = interleaved, inverse
+        return _launch(q, k, cos, sin, positions, interleaved, inverse)
 
     @staticmethod
     def backward(ctx, q_grad, k_grad):
         cos, sin, positions = ctx.saved_tensors
-        q_grad, k_grad = _launch(q_grad, k_grad, cos, sin, positions, ctx.interleaved, True)
-        return q_grad, k_grad, None, None, None, None
+        # a linear map: its gradient is the opposite turn, and so on for the gradient's
+        turn = _Rotary.apply if torch.is_grad_enabled() else _launch
+        q_grad, k_grad = turn(q_grad, k_grad, cos, sin, positions, ctx.interleaved, not ctx.inverse)
+        return q_grad, k_grad, None, None, None, None, None
 
 
 def apply_rotary(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, *, interleaved: bool = True,
@@ -159,5 +161,5 @@ def apply_rotary(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor, sin: torch
         positions = positions.contiguous()
     cos, sin = cos.contiguous(), sin.contiguous()
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad):
-        return _Rotary.apply(q, k, cos, sin, positions, interleaved)
+        return _Rotary.apply(q, k, cos, sin, positions, interleaved, False)
     return _launch(q, k, cos, sin, positions, interleaved, False)

@@ -248,3 +248,23 @@ def test_calls_replay_from_a_graph(cuda_device):
     graph.replay()
     for (x, codes, scale, bias, _), y, before in zip(problems, got, want):
         assert torch.equal(y, fp8.fp8_linear_forward(x, codes, scale, bias)) and not torch.equal(y, before)
+
+
+def test_offsets_past_32_bits(cuda_device):
+    m, k, n = 140_000, 128, 16_384  # 2.3e9 outputs
+    x, codes, scale, _, _ = _problem(3, k, n, torch.bfloat16, cuda_device, seed=6)
+    rows = torch.zeros(m, k, dtype=torch.bfloat16, device=cuda_device)
+    rows[-3:] = x
+    y = fp8.fp8_linear_forward(rows, codes, scale)
+    _check(y[-3:], _quantized_rows(x), _decoded(codes, scale).t())
+    assert not y[: m // 2].any()
+    back = fp8.fp8_linear_backward(y, codes, scale)  # reads past 2^31 values
+    _check(back[-3:], _quantized_rows(y[-3:]), _decoded(codes, scale))
+
+
+def test_a_second_gradient_is_refused(cuda_device):
+    x, codes, scale, _, grad = _problem(4, 128, 128, torch.float32, cuda_device)
+    x.requires_grad_()
+    first, = torch.autograd.grad(fp8.fp8_linear(x, codes, scale), x, grad.requires_grad_(), create_graph=True)
+    with pytest.raises(RuntimeError):
+        first.sum().backward()

@@ -175,3 +175,15 @@ def test_calls_replay_from_a_graph(cuda_device):
     graph.replay()
     for update, direction in zip(updates, got):
         assert torch.equal(direction, orthogonalize(update))
+
+
+def test_offsets_past_32_bits(cuda_device):
+    update = torch.zeros(33_000, 64, 1024, dtype=torch.bfloat16, device=cuda_device)  # 2.2e9 values
+    update[-1] = _updates("rows", (64, 1024), cuda_device, seed=10).bfloat16()
+    direction = orthogonalize(update)
+    assert _off(direction[-1], _exact(update[-1])) < WITHIN and not direction[-2].any()
+    del direction, update
+    wide = torch.zeros(1100, 512, 4096, dtype=torch.bfloat16, device=cuda_device)  # 2.3e9 values, iterated in float16
+    wide[-1] = _updates("rows", (512, 4096), cuda_device, seed=11).bfloat16()
+    direction = orthogonalize(wide)
+    assert _off(direction[-1], _exact(wide[-1])) < WITHIN and not direction[-2].any()

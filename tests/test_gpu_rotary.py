@@ -143,3 +143,26 @@ def test_refusals(cuda_device):
         with pytest.raises(ValueError):
             apply_rotary(arguments["q"], arguments["k"], arguments["cos"], arguments["sin"],
                          positions=arguments["positions"])
+
+
+def test_second_gradient(cuda_device):
+    """The turn is linear, so the gradient's own gradient is the turn again."""
+    gen = torch.Generator().manual_seed(8)
+    q = torch.randn(1, 6, 2, 16, generator=gen).to(cuda_device).requires_grad_()
+    cos, sin = _table(6, 8, cuda_device)
+    weight = torch.randn(1, 6, 2, 16, generator=gen).to(cuda_device).requires_grad_()
+    grad, = torch.autograd.grad(apply_rotary(q, q, cos, sin)[0], q, weight, create_graph=True)
+    direction = torch.randn(1, 6, 2, 16, generator=gen).to(cuda_device)
+    again, = torch.autograd.grad(grad, weight, direction)
+    _check(again, _turn(direction, cos, sin, True), direction)
+
+
+def test_offsets_past_32_bits(cuda_device):
+    tokens, heads, dim = 140_000, 64, 256  # 2.3e9 values
+    q = torch.zeros(1, tokens, heads, dim, dtype=torch.bfloat16, device=cuda_device)
+    tail = torch.randn(1, 3, heads, dim, generator=torch.Generator().manual_seed(9)).to(cuda_device, torch.bfloat16)
+    q[:, -3:] = tail
+    cos, sin = _table(tokens, dim // 2, cuda_device)
+    out, small = apply_rotary(q, q[:, :, :1], cos, sin, interleaved=False)
+    _check(out[:, -3:], _turn(tail, cos[-3:], sin[-3:], False), tail)
+    assert torch.equal(small[:, -3:], out[:, -3:, :1]) and not out[:, : tokens // 2].any()
