@@ -154,154 +154,154 @@ __global__ void __launch_bounds__(kThreads, 1)
   pdl_wait();
 
   if (warp < kEpiWarp0) {
-  if constexpr (kCtas == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegs));
-  if (warp == 0) {
-    // ---------------------------------------------------------------- producer (every CTA)
-    if (lane == 0) {
-      tma_prefetch_desc(&tm_a);
-      tma_prefetch_desc(&tm_w);
-    }
-    int stage = 0;
-    uint32_t phase = 0, used = 0, last_phase = 0;
-    bool ok = true;
-    for (int u = first_unit; u < num_units && ok; u += unit_step) {
-      const int tile = args.splits == 1 ? u : u / args.splits, split = u - tile * args.splits;
-      int m_blk, n_blk;
-      walk.at(tile, m_blk, n_blk);
-      const int m0 = m_blk * kTileM + static_cast<int>(rank) * kHalf;
-      const int n0 = n_blk * kTileN + static_cast<int>(rank) * kHalf;
-      const int kb1 = min(args.kb, (split + 1) * args.kb_per_split);
-      for (int kb = split * args.kb_per_split; kb < kb1; ++kb) {
-        if (!mbar_wait_cluster(bar(bars->empty[stage]), phase ^ 1u, abort_flag, args.status,
-                               MOSS_STATUS_TIMEOUT_LOAD)) {
-          ok = false;
-          break;
-        }
-        if (lane == 0) {
-          const uint32_t a_dst = base + stage * kStageBytes;
-          const int wx = kDX ? n0 : kb * kBlock, wy = kDX ? kb * kBlock : n0;
-          if constexpr (kCtas == 2) {
-            // the leader's barrier counts both CTAs' bytes; the peer's copies signal it too
-            if (leader) mbar_arrive_expect_tx(bar(bars->full[stage]), kCtas * kStageBytes);
-            const uint32_t fb = mapa_shared(bar(bars->full[stage]), 0);
-            tma_load_2d_pair(a_dst, &tm_a, fb, kb * kBlock, m0);
-            tma_load_2d_pair(a_dst + kTileBytes, &tm_w, fb, wx, wy);
-          } else {
-            mbar_arrive_expect_tx(bar(bars->full[stage]), kStageBytes);
-            tma_load_2d(a_dst, &tm_a, bar(bars->full[stage]), kb * kBlock, m0);
-            tma_load_2d(a_dst + kTileBytes, &tm_w, bar(bars->full[stage]), wx, wy);
-          }
-          used |= 1u << stage;
-          last_phase = (last_phase & ~(1u << stage)) | (phase << stage);
-        }
-        __syncwarp();
-        if (++stage == kStages) { stage = 0; phase ^= 1u; }
+    if constexpr (kCtas == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegs));
+    if (warp == 0) {
+      // ---------------------------------------------------------------- producer (every CTA)
+      if (lane == 0) {
+        tma_prefetch_desc(&tm_a);
+        tma_prefetch_desc(&tm_w);
       }
-    }
-    // The copies land before the CTA may leave. The leader sees the peer's too, and the peer
-    // leaves only after the leader's exit arrival.
-    if (lane == 0 && leader) {
-      for (int s = 0; s < kStages; ++s) {
-        if (!((used >> s) & 1u)) continue;
-        const long long start = clock64();
-        while (!mbar_try_wait(bar(bars->full[s]), (last_phase >> s) & 1u)) {
-          if (clock64() - start > kWaitBudgetCycles) {
-            report_status(args.status, MOSS_STATUS_TIMEOUT_DRAIN);
-            break;
-          }
-        }
-      }
-    }
-  } else if (warp == 1) {
-    // ---------------------------------------------------------------- MMA issuer (leader)
-    if (leader) {
-      constexpr uint32_t idesc = idesc_e4m3(false, kDX, kTileM, kTileN);
-      // descriptors of the first stage; every other differs by multiples of 16 bytes in the address field
-      const uint64_t a_desc0 = step_desc(base, 0, false), w_desc0 = step_desc(base + kTileBytes, 0, kDX);
-      int stage = 0, it = 0;
-      uint32_t phase = 0;
-      bool ok = true, issued = false;
+      int stage = 0;
+      uint32_t phase = 0, used = 0, last_phase = 0;
+      bool ok = true;
       for (int u = first_unit; u < num_units && ok; u += unit_step) {
-        const int split = args.splits == 1 ? 0 : u % args.splits;
+        const int tile = args.splits == 1 ? u : u / args.splits, split = u - tile * args.splits;
+        int m_blk, n_blk;
+        walk.at(tile, m_blk, n_blk);
+        const int m0 = m_blk * kTileM + static_cast<int>(rank) * kHalf;
+        const int n0 = n_blk * kTileN + static_cast<int>(rank) * kHalf;
         const int kb1 = min(args.kb, (split + 1) * args.kb_per_split);
-        for (int kb = split * args.kb_per_split; kb < kb1 && ok; ++kb, ++it) {
-          const int buf = it & 1;
-          // operands first: they are there long before the accumulator, whose wait is the critical one
-          if (!mbar_wait_cluster(bar(bars->full[stage]), phase, abort_flag, args.status, MOSS_STATUS_TIMEOUT_MMA) ||
-              !mbar_wait_cluster(bar(bars->acc_empty[buf]), ((it >> 1) & 1) ^ 1u, abort_flag, args.status,
-                                 MOSS_STATUS_TIMEOUT_MMA)) {
+        for (int kb = split * args.kb_per_split; kb < kb1; ++kb) {
+          if (!mbar_wait_cluster(bar(bars->empty[stage]), phase ^ 1u, abort_flag, args.status,
+                                 MOSS_STATUS_TIMEOUT_LOAD)) {
             ok = false;
             break;
           }
-          tc_fence_after();
-          if (elect_one()) {
-            const uint64_t at_stage = static_cast<uint64_t>(stage) * (kStageBytes >> 4);
-            const uint32_t d = tmem_base + static_cast<uint32_t>(buf * kTileN);
-#pragma unroll
-            for (int kk = 0; kk < kBlock / 32; ++kk) {
-              const uint64_t ad = a_desc0 + at_stage + kk * (32 >> 4);
-              const uint64_t wd = w_desc0 + at_stage + kk * ((kDX ? 4096 : 32) >> 4);
-              if constexpr (kCtas == 2)
-                umma_f8_pair(d, ad, wd, idesc, kk > 0);
-              else
-                umma_f8(d, ad, wd, idesc, kk > 0);
-            }
+          if (lane == 0) {
+            const uint32_t a_dst = base + stage * kStageBytes;
+            const int wx = kDX ? n0 : kb * kBlock, wy = kDX ? kb * kBlock : n0;
             if constexpr (kCtas == 2) {
-              umma_commit_pair_mc(bar(bars->acc_full[buf]), 0x3);
-              umma_commit_pair_mc(bar(bars->empty[stage]), 0x3);
+              // the leader's barrier counts both CTAs' bytes; the peer's copies signal it too
+              if (leader) mbar_arrive_expect_tx(bar(bars->full[stage]), kCtas * kStageBytes);
+              const uint32_t fb = mapa_shared(bar(bars->full[stage]), 0);
+              tma_load_2d_pair(a_dst, &tm_a, fb, kb * kBlock, m0);
+              tma_load_2d_pair(a_dst + kTileBytes, &tm_w, fb, wx, wy);
             } else {
-              umma_commit(bar(bars->acc_full[buf]));
-              umma_commit(bar(bars->empty[stage]));
+              mbar_arrive_expect_tx(bar(bars->full[stage]), kStageBytes);
+              tma_load_2d(a_dst, &tm_a, bar(bars->full[stage]), kb * kBlock, m0);
+              tma_load_2d(a_dst + kTileBytes, &tm_w, bar(bars->full[stage]), wx, wy);
             }
+            used |= 1u << stage;
+            last_phase = (last_phase & ~(1u << stage)) | (phase << stage);
           }
-          issued = true;
           __syncwarp();
           if (++stage == kStages) { stage = 0; phase ^= 1u; }
         }
       }
-      if (lane == 0 && issued) {
-        if constexpr (kCtas == 2)
-          umma_commit_pair(bar(bars->drain));
-        else
-          umma_commit(bar(bars->drain));
-        const long long start = clock64();
-        while (!mbar_try_wait(bar(bars->drain), 0)) {
-          if (clock64() - start > kWaitBudgetCycles) {
-            report_status(args.status, MOSS_STATUS_TIMEOUT_DRAIN);
-            break;
+      // The copies land before the CTA may leave. The leader sees the peer's too, and the peer
+      // leaves only after the leader's exit arrival.
+      if (lane == 0 && leader) {
+        for (int s = 0; s < kStages; ++s) {
+          if (!((used >> s) & 1u)) continue;
+          const long long start = clock64();
+          while (!mbar_try_wait(bar(bars->full[s]), (last_phase >> s) & 1u)) {
+            if (clock64() - start > kWaitBudgetCycles) {
+              report_status(args.status, MOSS_STATUS_TIMEOUT_DRAIN);
+              break;
+            }
           }
         }
       }
-      __syncwarp();
-    }
-  } else if (staged) {
-    // ---------------------------------------------------------------- store warps (every CTA)
-    // Warp 2 + h serves epilogue warpgroup h: it brings the bias, and issues the stores, whose queue
-    // would hold an epilogue warp up for a thousand cycles a tile.
-    const int h = warp - 2;
-    int it = 0;
-    for (int u = first_unit; u < num_units; u += unit_step, ++it) {
-      int m_blk, n_blk;
-      walk.at(u, m_blk, n_blk);
-      const int row0 = m_blk * kTileM + static_cast<int>(rank) * kHalf;
-      const int col0 = n_blk * kTileN + h * kCols;
-      for (int j = lane; j < kCols; j += 32)
-        bias_smem[h * kHalf + j] =
-            args.bias != nullptr && col0 + j < args.Nc ? load_as_float(args.bias, args.bias_kind, col0 + j) : 0.0f;
-      if (lane == 0) bulk_wait_read();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar(bars->out_free[h]));
-      if (!mbar_wait(bar(bars->out_full[h]), it & 1, abort_flag, args.status, MOSS_STATUS_TIMEOUT_EPILOGUE)) break;
-      if (args.tma_out != 0 && lane == 0) {
-        const uint32_t boxes = base + kRingBytes + h * 2 * kBoxBytes;
+    } else if (warp == 1) {
+      // ---------------------------------------------------------------- MMA issuer (leader)
+      if (leader) {
+        constexpr uint32_t idesc = idesc_e4m3(false, kDX, kTileM, kTileN);
+        // descriptors of the first stage; every other differs by multiples of 16 bytes in the address field
+        const uint64_t a_desc0 = step_desc(base, 0, false), w_desc0 = step_desc(base + kTileBytes, 0, kDX);
+        int stage = 0, it = 0;
+        uint32_t phase = 0;
+        bool ok = true, issued = false;
+        for (int u = first_unit; u < num_units && ok; u += unit_step) {
+          const int split = args.splits == 1 ? 0 : u % args.splits;
+          const int kb1 = min(args.kb, (split + 1) * args.kb_per_split);
+          for (int kb = split * args.kb_per_split; kb < kb1 && ok; ++kb, ++it) {
+            const int buf = it & 1;
+            // operands first: they are there long before the accumulator, whose wait is the critical one
+            if (!mbar_wait_cluster(bar(bars->full[stage]), phase, abort_flag, args.status, MOSS_STATUS_TIMEOUT_MMA) ||
+                !mbar_wait_cluster(bar(bars->acc_empty[buf]), ((it >> 1) & 1) ^ 1u, abort_flag, args.status,
+                                   MOSS_STATUS_TIMEOUT_MMA)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            if (elect_one()) {
+              const uint64_t at_stage = static_cast<uint64_t>(stage) * (kStageBytes >> 4);
+              const uint32_t d = tmem_base + static_cast<uint32_t>(buf * kTileN);
 #pragma unroll
-        for (int p = 0; p < kCols / 64; ++p)
-          if (row0 < args.M && col0 + p * 64 < args.Nc) tma_store_2d(&tm_out, boxes + p * kBoxBytes, col0 + p * 64, row0);
-        bulk_commit();
+              for (int kk = 0; kk < kBlock / 32; ++kk) {
+                const uint64_t ad = a_desc0 + at_stage + kk * (32 >> 4);
+                const uint64_t wd = w_desc0 + at_stage + kk * ((kDX ? 4096 : 32) >> 4);
+                if constexpr (kCtas == 2)
+                  umma_f8_pair(d, ad, wd, idesc, kk > 0);
+                else
+                  umma_f8(d, ad, wd, idesc, kk > 0);
+              }
+              if constexpr (kCtas == 2) {
+                umma_commit_pair_mc(bar(bars->acc_full[buf]), 0x3);
+                umma_commit_pair_mc(bar(bars->empty[stage]), 0x3);
+              } else {
+                umma_commit(bar(bars->acc_full[buf]));
+                umma_commit(bar(bars->empty[stage]));
+              }
+            }
+            issued = true;
+            __syncwarp();
+            if (++stage == kStages) { stage = 0; phase ^= 1u; }
+          }
+        }
+        if (lane == 0 && issued) {
+          if constexpr (kCtas == 2)
+            umma_commit_pair(bar(bars->drain));
+          else
+            umma_commit(bar(bars->drain));
+          const long long start = clock64();
+          while (!mbar_try_wait(bar(bars->drain), 0)) {
+            if (clock64() - start > kWaitBudgetCycles) {
+              report_status(args.status, MOSS_STATUS_TIMEOUT_DRAIN);
+              break;
+            }
+          }
+        }
+        __syncwarp();
       }
+    } else if (staged) {
+      // ---------------------------------------------------------------- store warps (every CTA)
+      // Warp 2 + h serves epilogue warpgroup h: it brings the bias, and issues the stores, whose queue
+      // would hold an epilogue warp up for a thousand cycles a tile.
+      const int h = warp - 2;
+      int it = 0;
+      for (int u = first_unit; u < num_units; u += unit_step, ++it) {
+        int m_blk, n_blk;
+        walk.at(u, m_blk, n_blk);
+        const int row0 = m_blk * kTileM + static_cast<int>(rank) * kHalf;
+        const int col0 = n_blk * kTileN + h * kCols;
+        for (int j = lane; j < kCols; j += 32)
+          bias_smem[h * kHalf + j] =
+              args.bias != nullptr && col0 + j < args.Nc ? load_as_float(args.bias, args.bias_kind, col0 + j) : 0.0f;
+        if (lane == 0) bulk_wait_read();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(bars->out_free[h]));
+        if (!mbar_wait(bar(bars->out_full[h]), it & 1, abort_flag, args.status, MOSS_STATUS_TIMEOUT_EPILOGUE)) break;
+        if (args.tma_out != 0 && lane == 0) {
+          const uint32_t boxes = base + kRingBytes + h * 2 * kBoxBytes;
+#pragma unroll
+          for (int p = 0; p < kCols / 64; ++p)
+            if (row0 < args.M && col0 + p * 64 < args.Nc) tma_store_2d(&tm_out, boxes + p * kBoxBytes, col0 + p * 64, row0);
+          bulk_commit();
+        }
+      }
+      if (lane == 0) bulk_wait();
     }
-    if (lane == 0) bulk_wait();
-  }
   } else {
     // ---------------------------------------------------------------- epilogue (every CTA)
     if constexpr (kCtas == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kEpiRegs));
