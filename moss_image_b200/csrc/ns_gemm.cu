@@ -100,30 +100,32 @@ __device__ __forceinline__ void locate(const Args& a, int u, int& b, int& m, int
 // on the products, so they are on their way before the accumulator is done (one at a time after it, they
 // took half of a small tile's life).
 struct Added {
-  uint4 hi[4], lo[4];
+  uint32_t hi[16], lo[16];
 };
+// 64 bytes in two whole sectors a lane: what lies in between belongs to other lanes' rows, and 16-byte loads would
+// ask L1 for every sector twice.
+__device__ __forceinline__ void load64(const __half* p, uint32_t (&w)[16]) {
+#pragma unroll
+  for (int h = 0; h < 16; h += 8)
+    asm volatile("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(w[h]), "=r"(w[h + 1]), "=r"(w[h + 2]), "=r"(w[h + 3]), "=r"(w[h + 4]), "=r"(w[h + 5]),
+                   "=r"(w[h + 6]), "=r"(w[h + 7])
+                 : "l"(p + 2 * h));
+}
 template <Mode kMode>
 __device__ __forceinline__ void fetch32(const Args& a, int b, int i, int j, Added& x) {
   const int cols = kMode == kUpdate ? a.cp : a.rp;
   if (kMode == kGram || i >= a.rp || j >= cols) return;
   const int64_t at = (static_cast<int64_t>(b) * a.rp + i) * cols + j;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) x.hi[e] = __ldg(reinterpret_cast<const uint4*>(a.add_hi + at) + e);
-  if (kMode == kUpdate && a.add_lo != nullptr) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) x.lo[e] = __ldg(reinterpret_cast<const uint4*>(a.add_lo + at) + e);
-  }
+  load64(a.add_hi + at, x.hi);
+  if (kMode == kUpdate && a.add_lo != nullptr) load64(a.add_lo + at, x.lo);
 }
-__device__ __forceinline__ void widen32(const uint4 (&w)[4], float (&v)[32]) {
+__device__ __forceinline__ void widen32(const uint32_t (&w)[16], float (&v)[32]) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t h[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[j]));
-      v[8 * i + 2 * j] = f.x;
-      v[8 * i + 2 * j + 1] = f.y;
-    }
+  for (int i = 0; i < 16; ++i) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+    v[2 * i] = f.x;
+    v[2 * i + 1] = f.y;
   }
 }
 __device__ __forceinline__ void store32(__half* p, const float (&v)[32]) {
@@ -135,6 +137,46 @@ __device__ __forceinline__ void store32(__half* p, const float (&v)[32]) {
   }
   gemm::stg256(p, w0);
   gemm::stg256(p + 16, w1);
+}
+
+// A warp's 32 x 32 block of the result, lane by lane a row, written by columns: rows of any alignment, 64 bytes of
+// one at a time (stores of each lane along its own row meet 32 sectors each: 149 x 176 x 2546 took 1890 us then,
+// 1310 now). Turned by shuffles: shared memory for it would be taken from the L1
+// cache, and the products that read and write much were 10% slower.
+__device__ __forceinline__ void store_turned(const Args& a, __nv_bfloat16* out, int i0, int j, const float (&v)[32]) {
+  const int lane = threadIdx.x & 31;
+  uint32_t w[16];
+#pragma unroll
+  for (int e = 0; e < 16; ++e) w[e] = gemm::pack2_kind<kBF16>(v[2 * e], v[2 * e + 1]);
+  // within each half of the warp: word k of lane l becomes word l of lane k
+#pragma unroll
+  for (int d = 8; d > 0; d >>= 1) {
+    const bool upper = (lane & d) != 0;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+      if (k & d) continue;
+      const uint32_t got = __shfl_xor_sync(0xffffffffu, upper ? w[k] : w[k + d], d);
+      if (upper)
+        w[k] = got;
+      else
+        w[k + d] = got;
+    }
+  }
+  const int first = i0 + (lane & 16), rows = min(16, a.r - first);
+  const int col = j + 2 * (lane & 15);
+  __nv_bfloat16* to = out + static_cast<int64_t>(first) * a.c + col;
+  const bool words = a.c % 2 == 0 && (reinterpret_cast<uintptr_t>(out) & 3) == 0;
+#pragma unroll
+  for (int k = 0; k < 16; ++k, to += a.c) {
+    if (k >= rows || col >= a.c) continue;
+    if (words) {
+      *reinterpret_cast<uint32_t*>(to) = w[k];
+    } else {
+      const __nv_bfloat162 pair = *reinterpret_cast<const __nv_bfloat162*>(&w[k]);
+      to[0] = __low2bfloat16(pair);
+      if (col + 1 < a.c) to[1] = __high2bfloat16(pair);
+    }
+  }
 }
 
 // 32 consecutive accumulators of one row through the mode's epilogue. i, j: row and first column.
@@ -154,15 +196,17 @@ __device__ __forceinline__ void finish32(const Args& a, int b, int i, int j, boo
 #pragma unroll
     for (int e = 0; e < 32; ++e) v[e] = fmaf(a.beta, x[e], a.alpha * v[e]);
     if (a.result != nullptr) {
-      if (i >= a.r) return;
       __nv_bfloat16* out = a.result + static_cast<int64_t>(b) * a.r * a.c;
       if (a.tall) {  // lanes hold consecutive rows: 64 contiguous bytes per column
+        if (i >= a.r) return;
 #pragma unroll
         for (int e = 0; e < 32; ++e)
           if (j + e < a.c) out[static_cast<int64_t>(j + e) * a.r + i] = __float2bfloat16_rn(v[e]);
       } else {
-        __nv_bfloat16* row = out + static_cast<int64_t>(i) * a.c + j;
-        if (j + 32 <= a.c && (reinterpret_cast<uintptr_t>(row) & 31) == 0) {
+        // one choice for the whole warp: a row's alignment is the matrix's where c is a multiple of 16
+        if (j + 32 <= a.c && a.c % 16 == 0 && (reinterpret_cast<uintptr_t>(out) & 31) == 0) {
+          if (i >= a.r) return;
+          __nv_bfloat16* row = out + static_cast<int64_t>(i) * a.c + j;
           uint32_t w0[8], w1[8];
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
@@ -172,9 +216,7 @@ __device__ __forceinline__ void finish32(const Args& a, int b, int i, int j, boo
           gemm::stg256(row, w0);
           gemm::stg256(row + 16, w1);
         } else {
-#pragma unroll
-          for (int e = 0; e < 32; ++e)
-            if (j + e < a.c) row[e] = __float2bfloat16_rn(v[e]);
+          store_turned(a, out, i - static_cast<int>(threadIdx.x & 31), j, v);
         }
       }
       return;

@@ -187,3 +187,14 @@ def test_offsets_past_32_bits(cuda_device):
     wide[-1] = _updates("rows", (512, 4096), cuda_device, seed=11).bfloat16()
     direction = orthogonalize(wide)
     assert _off(direction[-1], _exact(wide[-1])) < WITHIN and not direction[-2].any()
+
+
+@pytest.mark.parametrize("offset", [0, 1])
+@pytest.mark.parametrize("shape", [(2, 200, 1501), (2, 200, 1502), (2, 130, 1504), (1, 257, 1000), (2, 301, 290)])
+def test_results_of_any_width_and_alignment_stay_in_their_place(cuda_device, shape, offset):
+    update = _updates("rows", shape, cuda_device, seed=8)
+    room = torch.full((update.numel() + 64,), 7.0, dtype=torch.bfloat16, device=cuda_device)
+    out = room[16 + offset:16 + offset + update.numel()].view(shape)
+    assert orthogonalize(update, out=out) is out
+    assert torch.equal(out, orthogonalize(update)) and _off(out, _exact(update)) < WITHIN
+    assert (room[:16 + offset] == 7.0).all() and (room[16 + offset + update.numel():] == 7.0).all()
