@@ -268,3 +268,19 @@ def test_a_second_gradient_is_refused(cuda_device):
     first, = torch.autograd.grad(fp8.fp8_linear(x, codes, scale), x, grad.requires_grad_(), create_graph=True)
     with pytest.raises(RuntimeError):
         first.sum().backward()
+
+
+@pytest.mark.parametrize("offset", [0, 1])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("m,k,n", [(2500, 256, 2052), (2500, 256, 2049), (700, 300, 646), (130, 128, 36)])
+def test_tile_outputs_of_any_width_and_alignment_stay_in_their_place(cuda_device, dtype, m, k, n, offset):
+    x, codes, scale, bias, grad = _problem(m, k, n, dtype, cuda_device, seed=5)
+    weight = _decoded(codes, scale)
+    for rows, width, run, want in (
+            (x, n, lambda o: fp8.fp8_linear_forward(x, codes, scale, bias, out=o), (weight.t(), bias)),
+            (grad, k, lambda o: fp8.fp8_linear_backward(grad, codes, scale, out=o), (weight, None))):
+        room = torch.full((m * width + 64,), 7.0, dtype=dtype, device=cuda_device)
+        out = room[16 + offset:16 + offset + m * width].view(m, width)
+        assert run(out) is out
+        _check(out, _quantized_rows(rows), *want)
+        assert (room[:16 + offset] == 7.0).all() and (room[16 + offset + m * width:] == 7.0).all()
