@@ -81,13 +81,13 @@ inline EncodeTiledFn encode_fn() {
 inline bool make_map_nd(CUtensorMap* map, CUtensorMapDataType dt, int esize, const void* ptr, int rank,
                         const uint64_t* dims, const uint64_t* strides, const uint32_t* box, CUtensorMapSwizzle swz) {
   EncodeTiledFn fn = encode_fn();
-  if (fn == nullptr || rank < 2 || rank > 3) return false;
+  if (fn == nullptr || rank < 2 || rank > 4) return false;
   if ((reinterpret_cast<uintptr_t>(ptr) & 15) != 0) return false;
   if ((static_cast<uint64_t>(box[0]) * esize) % 16 != 0) return false;
-  cuuint64_t d[3];
-  cuuint64_t st[2];
-  cuuint32_t bx[3];
-  cuuint32_t es[3] = {1, 1, 1};
+  cuuint64_t d[4];
+  cuuint64_t st[3];
+  cuuint32_t bx[4];
+  cuuint32_t es[4] = {1, 1, 1, 1};
   for (int i = 0; i < rank; ++i) {
     if (dims[i] == 0 || box[i] == 0 || box[i] > 256) return false;
     d[i] = dims[i];

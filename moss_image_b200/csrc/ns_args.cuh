@@ -8,15 +8,15 @@
 namespace moss {
 namespace ns {
 
-// One product of a Newton-Schulz step over a batch of padded matrices. r <= c are the sides,
-// rp and cp their multiples of 128; X is [batch][rp][cp] f16 (hi + lo), A and B [batch][rp][rp] f16.
+// One product of a Newton-Schulz step over a batch of matrices. r <= c are the sides; X is [batch][r][cp] f16
+// (hi + lo), A and B [batch][r][sp] f16, with columns padded by zeros to cp, a multiple of 128, and sp, of 64.
 enum Mode {
   kGram,    // A = alpha X X^T                 (upper tiles, mirrored)
   kSquare,  // B = beta A + alpha A A          (upper tiles, mirrored)
   kUpdate,  // X' = beta X + alpha B X
 };
 struct Args {
-  int r, c, rp, cp, batch;
+  int r, c, sp, cp, batch;
   int tiles_m, tiles_n, tiles;  // per matrix (tiles: those computed)
   float alpha, beta;
   const __half* add_hi;  // kSquare: A; kUpdate: X

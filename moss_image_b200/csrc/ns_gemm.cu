@@ -57,19 +57,20 @@ struct Barriers {
 };
 static_assert(sizeof(Barriers) <= 512, "barrier block too large");
 
-__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int c2) {
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int c2,
+                                            int c3) {
   asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(c2)
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
       : "memory");
 }
-__device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1,
-                                                 int c2) {
+__device__ __forceinline__ void tma_load_4d_pair(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1,
+                                                 int c2, int c3) {
   asm volatile(
-      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(c2)
+      "cp.async.bulk.tensor.4d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
       : "memory");
 }
 
@@ -100,7 +101,7 @@ __device__ __forceinline__ void locate(const Args& a, int u, int& b, int& m, int
 // on the products, so they are on their way before the accumulator is done (one at a time after it, they
 // took half of a small tile's life).
 struct Added {
-  uint32_t hi[16], lo[16];
+  uint32_t hi[16], lo[16];  // unset in lanes past the last row, which store nothing
 };
 // 64 bytes in two whole sectors a lane: what lies in between belongs to other lanes' rows, and 16-byte loads would
 // ask L1 for every sector twice.
@@ -114,9 +115,9 @@ __device__ __forceinline__ void load64(const __half* p, uint32_t (&w)[16]) {
 }
 template <Mode kMode>
 __device__ __forceinline__ void fetch32(const Args& a, int b, int i, int j, Added& x) {
-  const int cols = kMode == kUpdate ? a.cp : a.rp;
-  if (kMode == kGram || i >= a.rp || j >= cols) return;
-  const int64_t at = (static_cast<int64_t>(b) * a.rp + i) * cols + j;
+  const int cols = kMode == kUpdate ? a.cp : a.sp;
+  if (kMode == kGram || i >= a.r || j >= cols) return;
+  const int64_t at = (static_cast<int64_t>(b) * a.r + i) * cols + j;
   load64(a.add_hi + at, x.hi);
   if (kMode == kUpdate && a.add_lo != nullptr) load64(a.add_lo + at, x.lo);
 }
@@ -140,8 +141,8 @@ __device__ __forceinline__ void store32(__half* p, const float (&v)[32]) {
 }
 
 // A warp's 32 x 32 block of the result, lane by lane a row, written by columns: rows of any alignment, 64 bytes of
-// one at a time (stores of each lane along its own row meet 32 sectors each: 149 x 176 x 2546 took 1890 us then,
-// 1310 now). Turned by shuffles: shared memory for it would be taken from the L1
+// one at a time (stores of each lane along its own row meet 32 sectors each: 149 x 176 x 2546 took 1890 us,
+// 1310 without). Turned by shuffles: shared memory for it would be taken from the L1
 // cache, and the products that read and write much were 10% slower.
 __device__ __forceinline__ void store_turned(const Args& a, __nv_bfloat16* out, int i0, int j, const float (&v)[32]) {
   const int lane = threadIdx.x & 31;
@@ -184,7 +185,7 @@ template <Mode kMode>
 __device__ __forceinline__ void finish32(const Args& a, int b, int i, int j, bool mirror, const Added& added,
                                          float (&v)[32]) {
   if constexpr (kMode == kUpdate) {
-    const int64_t at = (static_cast<int64_t>(b) * a.rp + i) * a.cp + j;
+    const int64_t at = (static_cast<int64_t>(b) * a.r + i) * a.cp + j;
     float x[32];
     widen32(added.hi, x);
     if (a.add_lo != nullptr) {
@@ -221,6 +222,7 @@ __device__ __forceinline__ void finish32(const Args& a, int b, int i, int j, boo
       }
       return;
     }
+    if (i >= a.r) return;
     store32(a.out_hi + at, v);
     if (a.out_lo != nullptr) {
 #pragma unroll
@@ -228,8 +230,8 @@ __device__ __forceinline__ void finish32(const Args& a, int b, int i, int j, boo
       store32(a.out_lo + at, v);
     }
   } else {
-    const int64_t base = static_cast<int64_t>(b) * a.rp * a.rp;
-    const int64_t at = base + static_cast<int64_t>(i) * a.rp + j;
+    const int64_t base = static_cast<int64_t>(b) * a.r * a.sp;
+    const int64_t at = base + static_cast<int64_t>(i) * a.sp + j;
     if constexpr (kMode == kSquare) {
       float x[32];
       widen32(added.hi, x);
@@ -241,8 +243,15 @@ __device__ __forceinline__ void finish32(const Args& a, int b, int i, int j, boo
     }
     store32(a.out_hi + at, v);
     if (mirror) {
+      const int64_t down = base + static_cast<int64_t>(j) * a.sp + i;
+      if (j + 32 <= a.r) {  // 32 conditions would cost small products 6%
 #pragma unroll
-      for (int e = 0; e < 32; ++e) a.out_hi[base + static_cast<int64_t>(j + e) * a.rp + i] = __float2half_rn(v[e]);
+        for (int e = 0; e < 32; ++e) a.out_hi[down + static_cast<int64_t>(e) * a.sp] = __float2half_rn(v[e]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 32; ++e)
+          if (j + e < a.r) a.out_hi[down + static_cast<int64_t>(e) * a.sp] = __float2half_rn(v[e]);
+      }
     }
   }
 }
@@ -269,7 +278,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int first_unit = blockIdx.x / kCtas;
   const int unit_step = gridDim.x / kCtas;
   const int num_units = args.tiles * args.batch;
-  const int steps = (kMode == kGram ? args.cp : args.rp) / kStep;
+  const int steps = ((kMode == kGram ? args.cp : args.sp) + kStep - 1) / kStep;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
@@ -316,8 +325,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int u = first_unit; u < num_units && ok; u += unit_step) {
       int b, m, n;
       locate<kMode, kN>(args, u, b, m, n);
-      const int m0 = b * args.rp + m * kTileM + static_cast<int>(rank) * kHalf;  // row of the left operand
-      const int n0 = n * kN + static_cast<int>(rank) * S::kRight;                // this CTA's columns
+      const int m0 = m * kTileM + static_cast<int>(rank) * kHalf;  // row of the left operand
+      const int n0 = n * kN + static_cast<int>(rank) * S::kRight;  // this CTA's columns
       for (int s = 0; s < steps; ++s) {
         if (!mbar_wait_cluster(bar(bars->empty[stage]), phase ^ 1u, abort_flag, args.status,
                                MOSS_STATUS_TIMEOUT_LOAD)) {
@@ -326,17 +335,17 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (lane == 0) {
           const uint32_t dst = base + stage * kStageBytes;
-          const int ry = kColumns ? b * args.rp + s * kStep : b * args.rp + n0;
+          const int ry = kColumns ? s * kStep : n0;
           const int rz = kColumns ? n0 / 64 : s * 2;
           if constexpr (kCtas == 2) {
             if (leader) mbar_arrive_expect_tx(bar(bars->full[stage]), kCtas * kStageBytes);
             const uint32_t fb = mapa_shared(bar(bars->full[stage]), 0);
-            tma_load_3d_pair(dst, &tm_left, fb, 0, m0, s * 2);
-            tma_load_3d_pair(dst + kLeftBytes, &tm_right, fb, 0, ry, rz);
+            tma_load_4d_pair(dst, &tm_left, fb, 0, m0, s * 2, b);
+            tma_load_4d_pair(dst + kLeftBytes, &tm_right, fb, 0, ry, rz, b);
           } else {
             mbar_arrive_expect_tx(bar(bars->full[stage]), kStageBytes);
-            tma_load_3d(dst, &tm_left, bar(bars->full[stage]), 0, m0, s * 2);
-            tma_load_3d(dst + kLeftBytes, &tm_right, bar(bars->full[stage]), 0, ry, rz);
+            tma_load_4d(dst, &tm_left, bar(bars->full[stage]), 0, m0, s * 2, b);
+            tma_load_4d(dst + kLeftBytes, &tm_right, bar(bars->full[stage]), 0, ry, rz, b);
           }
           used |= 1u << stage;
           last_phase = (last_phase & ~(1u << stage)) | (phase << stage);
@@ -432,7 +441,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int q = warp & 3;
     const int half = (warp - kEpiWarp0) >> 2;
     const uint32_t lane_addr = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(half * (kN / 2));
-    const int cols = kMode == kUpdate ? args.cp : args.rp;
+    const int cols = kMode == kUpdate ? args.cp : args.sp;
     int it = 0;
     for (int u = first_unit; u < num_units; u += unit_step, ++it) {
       int b, m, n;
@@ -464,12 +473,14 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
         const int j = j0 + c * 32;
-        if (i < args.rp && j < cols) {  // otherwise past this matrix: the next one's rows, or nothing
+        // the update's last rows leave by the whole warp
+        if ((kMode == kUpdate ? i - lane : i) < args.r && j < cols) {
           float v[32];
 #pragma unroll
           for (int e = 0; e < 32; ++e) v[e] = __uint_as_float(r[e]);
           finish32<kMode>(args, b, i, j, kN == 64 ? m != n >> 1 : m != n, added[c & 1], v);
         }
+        if constexpr (kMode == kUpdate) __syncwarp();  // lanes past the last row left early
         if (c + 2 < kGroups) fetch32<kMode>(args, b, i, j + 64, added[c & 1]);
       }
     }
@@ -534,8 +545,8 @@ int launch_typed(const CUtensorMap& tl, const CUtensorMap& tr, Args a, cudaStrea
     }
   });
   MOSS_CUDA_TRY(attr_err);
-  a.tiles_m = (a.rp + kHalf * kCtas - 1) / (kHalf * kCtas);
-  a.tiles_n = ((kMode == kUpdate ? a.cp : a.rp) + kN - 1) / kN;
+  a.tiles_m = (a.r + kHalf * kCtas - 1) / (kHalf * kCtas);
+  a.tiles_n = ((kMode == kUpdate ? a.cp : a.sp) + kN - 1) / kN;
   a.tiles = kMode == kUpdate ? a.tiles_m * a.tiles_n : a.tiles_m * (a.tiles_m + 1) / 2 * (kN == 64 ? 2 : 1);
   const int64_t units = static_cast<int64_t>(a.tiles) * a.batch;
   if (units > INT32_MAX) return fail(MOSS_ERR_INVALID_ARGUMENT, "too many matrices to orthogonalize in one call");
@@ -554,10 +565,10 @@ int tile_columns(Mode mode, const Args& a) {
     const int64_t tiles = mode == kUpdate ? tm * tn : tm * (tm + 1) / 2 * (tn / tm);
     return (tiles * a.batch + slots - 1) / slots;
   };
-  const int64_t cols = mode == kUpdate ? a.cp : a.rp;
-  const int64_t pair = rounds((a.rp + 255) / 256, (cols + 255) / 256, std::max<int64_t>(1, sms / 2)) * 20;
-  const int64_t wide = rounds(a.rp / 128, cols / 128, sms) * 13;
-  const int64_t narrow = rounds(a.rp / 128, cols / 64, sms) * 9;
+  const int64_t tm = (a.r + 127) / 128, tn = mode == kUpdate ? a.cp / 128 : tm;
+  const int64_t pair = rounds((tm + 1) / 2, (tn + 1) / 2, std::max<int64_t>(1, sms / 2)) * 20;
+  const int64_t wide = rounds(tm, tn, sms) * 13;
+  const int64_t narrow = rounds(tm, 2 * tn, sms) * 9;
   if (pair <= wide && pair <= narrow) return 256;
   return wide <= narrow ? 128 : 64;
 }
@@ -574,18 +585,19 @@ int launch_mode(int columns, const CUtensorMap& tl, const CUtensorMap& tr, const
 int launch_gemm(Mode mode, const __half* left, const __half* right, const Args& a, cudaStream_t stream) {
   const int columns = tile_columns(mode, a);
   const uint32_t held = columns == 64 ? 64 : 128;  // columns of the right operand in one CTA
-  // [batch * rp][cols] viewed as {64, rows, cols / 64}: a box is rows of 64-wide columns
+  // [batch][r][cols] viewed as {64, r, cols / 64, batch}: a box is rows of 64-wide columns, and what it holds past
+  // the matrix's last row or column is zero, whatever the next matrix holds
   auto map = [&](CUtensorMap* m, const __half* p, int cols, uint32_t rows, uint32_t wide) {
     memset(m, 0, sizeof(*m));
-    const uint64_t dims[3] = {64, static_cast<uint64_t>(a.batch) * a.rp, static_cast<uint64_t>(cols / 64)};
-    const uint64_t strides[2] = {static_cast<uint64_t>(cols) * 2, 128};
-    const uint32_t box[3] = {64, rows, wide};
-    return gemm::make_map_nd(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, p, 3, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+    const uint64_t dims[4] = {64, static_cast<uint64_t>(a.r), static_cast<uint64_t>(cols / 64), static_cast<uint64_t>(a.batch)};
+    const uint64_t strides[3] = {static_cast<uint64_t>(cols) * 2, 128, static_cast<uint64_t>(a.r) * cols * 2};
+    const uint32_t box[4] = {64, rows, wide, 1};
+    return gemm::make_map_nd(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, p, 4, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
   };
   CUtensorMap tl, tr;
   const bool by_columns = mode == kUpdate;
-  if (!map(&tl, left, mode == kGram ? a.cp : a.rp, 128, 2) ||
-      !map(&tr, right, mode == kSquare ? a.rp : a.cp, by_columns ? 128 : held, by_columns ? held / 64 : 2))
+  if (!map(&tl, left, mode == kGram ? a.cp : a.sp, 128, 2) ||
+      !map(&tr, right, mode == kSquare ? a.sp : a.cp, by_columns ? 128 : held, by_columns ? held / 64 : 2))
     return fail(MOSS_ERR_CUDA, "the driver refused a tensor map of the orthogonalised update");
   switch (mode) {
     case kGram:

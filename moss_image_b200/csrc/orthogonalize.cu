@@ -109,11 +109,11 @@ __device__ __forceinline__ void split8(const float (&v)[8], float scale, uint4& 
   lo = make_uint4(l[0], l[1], l[2], l[3]);
 }
 
-// hi + lo = G * unit / max(|G|, eps), padded with zeros to [rp][cp]. A CTA: kNormRows rows of 512 columns.
+// hi + lo = G * unit / max(|G|, eps), its columns padded with zeros to cp. A CTA: kNormRows rows of 512 columns.
 constexpr int kNormRows = 16;
 template <int kKind>
-__global__ void __launch_bounds__(kThreads) normalize_kernel(const void* __restrict__ g, int r, int c, int rp, int cp,
-                                                             bool wide, const double* __restrict__ parts, int num_parts,
+__global__ void __launch_bounds__(kThreads) normalize_kernel(const void* __restrict__ g, int r, int c, int cp, bool wide,
+                                                             const double* __restrict__ parts, int num_parts,
                                                              float eps, float unit, __half* __restrict__ hi,
                                                              __half* __restrict__ lo) {
   pdl_wait();
@@ -135,7 +135,8 @@ __global__ void __launch_bounds__(kThreads) normalize_kernel(const void* __restr
   for (int k = 0; k < kNormRows / 4; ++k) {
     uint4 h, l;
     split8(v[k], scale, h, l);
-    const int64_t at = (b * rp + i0 + 4 * k) * cp + j;
+    if (i0 + 4 * k >= r) continue;
+    const int64_t at = (b * r + i0 + 4 * k) * cp + j;
     *reinterpret_cast<uint4*>(hi + at) = h;
     *reinterpret_cast<uint4*>(lo + at) = l;
   }
@@ -143,8 +144,8 @@ __global__ void __launch_bounds__(kThreads) normalize_kernel(const void* __restr
 
 // The same for a tall G [c][r]: 64 x 64 tiles turned through shared memory, so that both sides move whole rows.
 template <int kKind>
-__global__ void __launch_bounds__(kThreads) normalize_tall_kernel(const void* __restrict__ g, int r, int c, int rp, int cp,
-                                                                  bool wide, const double* __restrict__ parts,
+__global__ void __launch_bounds__(kThreads) normalize_tall_kernel(const void* __restrict__ g, int r, int c, int cp, bool wide,
+                                                                  const double* __restrict__ parts,
                                                                   int num_parts, float eps, float unit,
                                                                   __half* __restrict__ hi, __half* __restrict__ lo) {
   __shared__ float tile[64][65];
@@ -166,12 +167,13 @@ __global__ void __launch_bounds__(kThreads) normalize_tall_kernel(const void* __
   __syncthreads();
 #pragma unroll
   for (int k = w; k < 64; k += kThreads / 8) {
+    if (i0 + k >= r) continue;
     float v[8];
 #pragma unroll
     for (int q = 0; q < 8; ++q) v[q] = tile[k][e + q];
     uint4 h, l;
     split8(v, scale, h, l);
-    const int64_t at = (b * rp + i0 + k) * cp + j0 + e;
+    const int64_t at = (b * r + i0 + k) * cp + j0 + e;
     *reinterpret_cast<uint4*>(hi + at) = h;
     *reinterpret_cast<uint4*>(lo + at) = l;
   }
@@ -179,7 +181,7 @@ __global__ void __launch_bounds__(kThreads) normalize_tall_kernel(const void* __
 
 // Norms and the padded, scaled operands.
 template <int kKind>
-static int launch_normalize(const void* g, int64_t batch, int r, int c, int rp, int cp, bool tall, float eps, float unit,
+static int launch_normalize(const void* g, int64_t batch, int r, int c, int cp, bool tall, float eps, float unit,
                             double* parts, int num_parts, __half* hi, __half* lo, cudaStream_t stream) {
   const int64_t size = static_cast<int64_t>(r) * c;
   const bool aligned = reinterpret_cast<uintptr_t>(g) % 16 == 0;
@@ -188,14 +190,14 @@ static int launch_normalize(const void* g, int64_t batch, int r, int c, int rp, 
   MOSS_CUDA_TRY(cudaGetLastError());
   const bool wide = aligned && (tall ? r : c) % 8 == 0;
   if (tall)
-    return launch_dependent("normalize_tall_kernel", normalize_tall_kernel<kKind>, dim3(cp / 64, rp / 64, z), dim3(kThreads),
-                            0, stream, g, r, c, rp, cp, wide, parts, num_parts, eps, unit, hi, lo);
-  return launch_dependent("normalize_kernel", normalize_kernel<kKind>, dim3((cp + 511) / 512, rp / kNormRows, z),
-                          dim3(kThreads), 0, stream, g, r, c, rp, cp, wide, parts, num_parts, eps, unit, hi, lo);
+    return launch_dependent("normalize_tall_kernel", normalize_tall_kernel<kKind>, dim3(cp / 64, (r + 63) / 64, z), dim3(kThreads),
+                            0, stream, g, r, c, cp, wide, parts, num_parts, eps, unit, hi, lo);
+  return launch_dependent("normalize_kernel", normalize_kernel<kKind>, dim3((cp + 511) / 512, (r + kNormRows - 1) / kNormRows, z),
+                          dim3(kThreads), 0, stream, g, r, c, cp, wide, parts, num_parts, eps, unit, hi, lo);
 }
 
 struct Layout {
-  int r, c, rp, cp, side, chunks;
+  int r, c, sp, cp, side, chunks;
   bool tall, small;
   size_t x[2], low[2], a, b, parts, partial, q, factors, total;
 };
@@ -220,9 +222,9 @@ static Layout layout_of(int64_t batch, int64_t rows, int64_t cols) {
     l.q = take(square);
     l.factors = take(static_cast<size_t>(batch) * 8);
   } else {
-    l.rp = (l.r + 127) / 128 * 128;
+    l.sp = (l.r + 63) / 64 * 64;
     l.cp = (l.c + 127) / 128 * 128;
-    const size_t wide = static_cast<size_t>(batch) * l.rp * l.cp * 2, square = static_cast<size_t>(batch) * l.rp * l.rp * 2;
+    const size_t wide = static_cast<size_t>(batch) * l.r * l.cp * 2, square = static_cast<size_t>(batch) * l.r * l.sp * 2;
     for (int i = 0; i < 2; ++i) {
       l.x[i] = take(wide);
       l.low[i] = take(wide);
@@ -334,11 +336,11 @@ static int run(const void* g, int dtype, int64_t batch, int64_t rows, int64_t co
   __half* ga = reinterpret_cast<__half*>(ws + l.a);
   __half* gb = reinterpret_cast<__half*>(ws + l.b);
   if (dtype == kBF16)
-    rc = launch_normalize<kBF16>(g, batch, l.r, l.c, l.rp, l.cp, l.tall, eps, unit, parts, num_parts, x[0], low[0], stream);
+    rc = launch_normalize<kBF16>(g, batch, l.r, l.c, l.cp, l.tall, eps, unit, parts, num_parts, x[0], low[0], stream);
   else if (dtype == kF16)
-    rc = launch_normalize<kF16>(g, batch, l.r, l.c, l.rp, l.cp, l.tall, eps, unit, parts, num_parts, x[0], low[0], stream);
+    rc = launch_normalize<kF16>(g, batch, l.r, l.c, l.cp, l.tall, eps, unit, parts, num_parts, x[0], low[0], stream);
   else
-    rc = launch_normalize<kF32>(g, batch, l.r, l.c, l.rp, l.cp, l.tall, eps, unit, parts, num_parts, x[0], low[0], stream);
+    rc = launch_normalize<kF32>(g, batch, l.r, l.c, l.cp, l.tall, eps, unit, parts, num_parts, x[0], low[0], stream);
   if (rc != MOSS_OK) return rc;
   const int with_low = std::max(1, steps - 2);  // steps whose a X term reads lo
   for (int i = 0; i < steps; ++i) {
@@ -346,7 +348,7 @@ static int run(const void* g, int dtype, int64_t batch, int64_t rows, int64_t co
     Args a{};
     a.r = l.r;
     a.c = l.c;
-    a.rp = l.rp;
+    a.sp = l.sp;
     a.cp = l.cp;
     a.batch = static_cast<int>(batch);
     a.tall = l.tall;
