@@ -52,7 +52,8 @@ def rotary_frequencies(dim: int, *, theta: float = 10000.0, scaling: str | None 
         def index_of(beta: float) -> float:
             return (dim // 2) * math.log(original_length / (beta * 2.0 * math.pi)) / math.log(theta)
 
-        low, high = max(math.floor(index_of(beta_fast)), 0), min(math.ceil(index_of(beta_slow)), dim // 2 - 1)
+        # (the end may lie past the last pair: every pair then turns often enough to keep a part of its frequency)
+        low, high = max(math.floor(index_of(beta_fast)), 0), math.ceil(index_of(beta_slow))
         index = torch.arange(dim // 2, dtype=torch.float64, device=device)
         blend = ((index - low) / max(high - low, 1e-3)).clamp(0.0, 1.0)
         return frequencies * (1.0 - blend) + frequencies / factor * blend

@@ -76,3 +76,20 @@ def test_cpu_tensors_are_refused():
     q = torch.zeros(1, 2, 1, 4)
     with pytest.raises(RuntimeError, match="CUDA"):
         apply_rotary(q, q, torch.zeros(2, 2), torch.zeros(2, 2))
+
+
+@pytest.mark.parametrize("theta,length", [(1e4, 131072), (256.0, 4096), (500.0, 32768), (1e4, 2048), (1e6, 40)])
+def test_yarn_divides_wholly_only_pairs_that_turn_too_rarely(theta, length):
+    """Pair by pair: the divisor follows the pair's index between the ends of the ramp, which lie where
+    the turns pass the two betas, past the last pair too."""
+    factor, half = 8.0, 64
+    plain = rotary_frequencies(2 * half, theta=theta)
+    ratio = plain / rotary_frequencies(2 * half, theta=theta, scaling="yarn", factor=factor, original_length=length)
+    turns = length * plain / (2 * math.pi)
+    assert bool((ratio[turns > 1.001] < factor * (1 - 1e-9)).all())
+    low, high = (half * math.log(length / (beta * 2 * math.pi)) / math.log(theta) for beta in (32.0, 1.0))
+    low = max(math.floor(low), 0)
+    high = math.ceil(high)
+    for pair in range(half):
+        part = min(max((pair - low) / max(high - low, 1e-3), 0.0), 1.0)
+        assert math.isclose(float(1.0 / ratio[pair]), (1.0 - part) + part / factor, rel_tol=1e-9)
