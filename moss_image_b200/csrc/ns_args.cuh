@@ -39,10 +39,12 @@ struct Small {
   int r, c, tall, steps;
   int wide, out_wide;  // 4-value reads of G's rows, 8-value writes of the result's are aligned and whole
   float coefficients[3 * kMaxSteps];
-  float eps;
+  float eps_fraction;  // eps = fraction 2^exponent
+  int eps_exponent;
   __nv_bfloat16* out;
   int chunks;      // column ranges per matrix of the Gram kernel
-  float* partial;  // [batch][chunks][side * side]
+  float* partial;  // [batch][chunks][side * side], each times 4^-exponent
+  int* exponents;  // [batch][chunks]
   __half* q;       // [batch][hi, lo][side * side], scaled by a power of two
   float* factors;  // [batch][2]: X's scale in the product with Q, and the product's own
 };

@@ -90,9 +90,11 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return r;
 }
 __device__ __forceinline__ float pow2(int p) { return __uint_as_float(static_cast<uint32_t>(p + 127) << 23); }
-// p with v in [2^(p + 10), 2^(p + 11)): v 2^-p is about 1024. Kept where 2^p and 2^-p are normal.
+// p with v in [2^(p + 10), 2^(p + 11)): v 2^-p is about 1024. At most 117, and not below -127, where 2^-p is still
+// normal: what is smaller, f32's subnormals included, is then below 2 and on a grid of 2^-22, which float16 holds.
+constexpr int kLeastScale = -127;
 __device__ __forceinline__ int scale_of(float v) {
-  return min(110, max(-110, static_cast<int>((__float_as_uint(v) >> 23) & 0xffu) - 127 - 10));
+  return min(117, max(kLeastScale, static_cast<int>((__float_as_uint(v) >> 23) & 0xffu) - 127 - 10));
 }
 __device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
   const __half2 h = __floats2half2_rn(a, b);
@@ -208,7 +210,8 @@ __device__ __forceinline__ uint32_t block_columns(uint32_t tile, int pitch, int 
 
 // Partial X X^T over this CTA's column range: hi hi^T + hi lo^T + (hi lo^T)^T. A warp holds one block of at
 // most 32 x 32 of both products, over every kSplits-th 16 columns. X is scaled by the largest value met so
-// far; when a tile brings a larger one, the sums are scaled down with it (powers of two, exact).
+// far; when a tile brings a larger one, the sums are scaled down with it (powers of two, exact). They leave
+// scaled, with their exponent beside them: the squares of f32's values have twice its range.
 template <int kSide, int kKind>
 __global__ void __launch_bounds__(kThreads, 2) small_gram_kernel(const Small s) {
   constexpr int kC = kCols<kSide>, kP = kPitch<kSide>;
@@ -230,7 +233,7 @@ __global__ void __launch_bounds__(kThreads, 2) small_gram_kernel(const Small s) 
   __half* lo = tiles + kTileHalves<kSide>;
   const uint32_t hi_addr = smem_u32(hi), lo_addr = smem_u32(lo);
   float hh[kMT][kNT][4] = {}, hl[kMT][kNT][4] = {};
-  int p = -110;  // X is held times 2^-p
+  int p = kLeastScale;  // X is held times 2^-p
   Tile<kSide, kKind> next;
   if (first < last) next.fetch(s, b, first * kC);
   for (int range = first; range < last; ++range) {
@@ -302,7 +305,7 @@ __global__ void __launch_bounds__(kThreads, 2) small_gram_kernel(const Small s) 
   }
   __syncthreads();
   float* out = s.partial + (b * s.chunks + blockIdx.x) * kSide * kSide;
-  const float up = pow2(p);
+  if (threadIdx.x == 0) s.exponents[b * s.chunks + blockIdx.x] = p;
   for (int e = threadIdx.x; e < kSide * kSide; e += kThreads) {
     const int row = e / kSide, col = e % kSide;
     float same = 0.0f, across = 0.0f;
@@ -312,7 +315,7 @@ __global__ void __launch_bounds__(kThreads, 2) small_gram_kernel(const Small s) 
       same += part[row][col];
       across += part[kSide + row][col] + part[kSide + col][row];
     }
-    out[e] = (same + across) * up * up;
+    out[e] = same + across;
   }
   pdl_trigger();
 }
@@ -356,15 +359,23 @@ __global__ void __launch_bounds__(kIterateThreads<kSide>) small_iterate_kernel(c
   pdl_wait();
   pdl_trigger();
   const float* partial = s.partial + b * s.chunks * kSide * kSide;
+  // X, R and the norm are held in units of 2^xp of the matrix's largest value from here on. The exponents come with
+  // the sums: a pass over them before would be one more wait for L2.
+  const int* exponents = s.exponents + b * s.chunks;
+  int xp = kLeastScale;
   for (int e = threadIdx.x * 4; e < kSide * kSide; e += kIterateThreads<kSide> * 4) {
     float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    xp = kLeastScale;
 #pragma unroll 4
     for (int k = 0; k < s.chunks; ++k) {
       const float4 w = *reinterpret_cast<const float4*>(partial + static_cast<int64_t>(k) * kSide * kSide + e);
-      v.x += w.x;
-      v.y += w.y;
-      v.z += w.z;
-      v.w += w.w;
+      const int p = exponents[k], top = max(xp, p);
+      const float mine = pow2(max(-126, 2 * (xp - top))), its = pow2(max(-126, 2 * (p - top)));  // one of them is 1
+      v.x = fmaf(w.x, its, v.x * mine);
+      v.y = fmaf(w.y, its, v.y * mine);
+      v.z = fmaf(w.z, its, v.z * mine);
+      v.w = fmaf(w.w, its, v.w * mine);
+      xp = top;
     }
     *reinterpret_cast<float4*>(&R[e / kSide][e % kSide]) = v;
   }
@@ -372,7 +383,10 @@ __global__ void __launch_bounds__(kIterateThreads<kSide>) small_iterate_kernel(c
   float trace = 0.0f;
   for (int i = 0; i < s.r; ++i) trace += R[i][i];
   const float norm = sqrtf(trace);
-  const float inv = 1.0f / (norm < s.eps ? s.eps : norm);  // NaN stays NaN: every entry then is
+  // eps in the same units; what passes f32's range (a tiny matrix against an eps above 1) is left for the result
+  const int eps_exp = s.eps_exponent - xp;
+  const float eps = s.eps_fraction * pow2(min(126, max(-126, eps_exp)));
+  const float inv = 1.0f / (norm < eps ? eps : norm);  // NaN stays NaN: every entry then is
   __syncthreads();
   float z[4][4];
   auto put = [&](Row* to, bool transposed) {
@@ -423,7 +437,7 @@ __global__ void __launch_bounds__(kIterateThreads<kSide>) small_iterate_kernel(c
     }
   }
   __syncthreads();
-  // Q as hi + lo, times 2^-qp, and what the product has to be multiplied by. |x| <= |X|, so X is held times 2^-xp.
+  // Q as hi + lo, times 2^-qp, and what the product with X, times 2^-xp, has to be multiplied by.
   __shared__ float warp_max[kIterateThreads<kSide> / 32];
   float amax = 0.0f;
   for (int e = threadIdx.x; e < kSide * kSide; e += kIterateThreads<kSide>)
@@ -434,7 +448,7 @@ __global__ void __launch_bounds__(kIterateThreads<kSide>) small_iterate_kernel(c
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < kIterateThreads<kSide> / 32; ++w) amax = max_nan(amax, warp_max[w]);
-  const int qp = scale_of(amax), xp = scale_of(norm);
+  const int qp = max(-126, scale_of(amax));  // its own power of two is normal as well
   const float down = pow2(-qp);
   __half* hi = s.q + b * 2 * kSide * kSide;
   __half* lo = hi + kSide * kSide;
@@ -445,9 +459,8 @@ __global__ void __launch_bounds__(kIterateThreads<kSide>) small_iterate_kernel(c
     *reinterpret_cast<uint32_t*>(lo + e) = l;
   }
   if (threadIdx.x == 0) {
-    // 1 / |X| is divided between the two powers of two: each of the three may be far from 1, their product is not
     s.factors[2 * b] = pow2(-xp);
-    s.factors[2 * b + 1] = (inv * pow2(xp)) * pow2(qp);
+    s.factors[2 * b + 1] = inv * pow2(qp) * (norm < eps ? pow2(-min(126, max(0, eps_exp - 126))) : 1.0f);
   }
 }
 

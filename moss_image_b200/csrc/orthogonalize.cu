@@ -199,7 +199,7 @@ static int launch_normalize(const void* g, int64_t batch, int r, int c, int cp, 
 struct Layout {
   int r, c, sp, cp, side, chunks;
   bool tall, small;
-  size_t x[2], low[2], a, b, parts, partial, q, factors, total;
+  size_t x[2], low[2], a, b, parts, partial, exponents, q, factors, total;
 };
 
 static Layout layout_of(int64_t batch, int64_t rows, int64_t cols) {
@@ -219,6 +219,7 @@ static Layout layout_of(int64_t batch, int64_t rows, int64_t cols) {
     l.chunks = small_chunks(batch, l.r, l.c, sm_count());
     const size_t square = static_cast<size_t>(l.side) * l.side * 4 * batch;
     l.partial = take(square * l.chunks);
+    l.exponents = take(static_cast<size_t>(batch) * l.chunks * 4);
     l.q = take(square);
     l.factors = take(static_cast<size_t>(batch) * 8);
   } else {
@@ -312,10 +313,11 @@ static int run(const void* g, int dtype, int64_t batch, int64_t rows, int64_t co
     s.wide = inner % 4 == 0 && reinterpret_cast<uintptr_t>(g) % 16 == 0;
     s.out_wide = inner % 8 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0;
     std::memcpy(s.coefficients, coefficients, sizeof(float) * 3 * steps);
-    s.eps = eps;
+    s.eps_fraction = std::frexp(eps, &s.eps_exponent);
     s.out = out;
     s.chunks = l.chunks;
     s.partial = reinterpret_cast<float*>(ws + l.partial);
+    s.exponents = reinterpret_cast<int*>(ws + l.exponents);
     s.q = reinterpret_cast<__half*>(ws + l.q);
     s.factors = reinterpret_cast<float*>(ws + l.factors);
     rc = launch_small(s, stream);

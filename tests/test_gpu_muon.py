@@ -198,3 +198,29 @@ def test_results_of_any_width_and_alignment_stay_in_their_place(cuda_device, sha
     assert orthogonalize(update, out=out) is out
     assert torch.equal(out, orthogonalize(update)) and _off(out, _exact(update)) < WITHIN
     assert (room[:16 + offset] == 7.0).all() and (room[16 + offset + update.numel():] == 7.0).all()
+
+
+@pytest.mark.parametrize("scale", [1e-42, 1e-36, 1e-28, 1e-25, 1e-23, 1e-20, 1e25, 3e37])
+@pytest.mark.parametrize("shape", [(2, 12, 60), (2, 60, 12), (2, 32, 1100), (2, 1100, 32), (2, 61, 300), (2, 300, 64)])
+def test_small_sides_at_the_ends_of_the_range(cuda_device, shape, scale):
+    """Squares of these values leave float32; the values and the result do not."""
+    update = _updates("rows", shape, cuda_device, seed=12)
+    update[1] = update[0] / update[0].abs().amax() * scale
+    clean = orthogonalize(update[0])
+    for dtype in (torch.float32, torch.bfloat16):
+        for eps in (1e-7, 1e-30):
+            given = update.to(dtype)
+            want = _exact(given, eps=eps)
+            got = orthogonalize(given, eps=eps)
+            if float(want[1].abs().amax()) < 3e38:  # (below eps, a step only multiplies: tiny over a tiny eps may overflow)
+                # (1e-42 is zero in bfloat16)
+                assert float((got[1].double() - want[1]).norm()) <= (2.0 ** -8 + 1e-4) * float(want[1].norm())
+    assert _off(orthogonalize(update)[0], clean.double()) < 2.0 ** -8
+
+
+def test_small_sides_with_tiny_and_huge_columns(cuda_device):
+    update = _updates("plain", (16, 6000), cuda_device, seed=13)
+    update[:, :2500] *= 1e-30
+    update[:, 2500:] *= 1e30
+    got, want = orthogonalize(update), _exact(update)
+    assert _off(got[:, 2500:], want[:, 2500:]) < WITHIN
