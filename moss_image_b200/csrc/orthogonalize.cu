@@ -84,21 +84,31 @@ __global__ void __launch_bounds__(kThreads) sum_squares_kernel(const void* __res
   pdl_trigger();
 }
 
-// unit / max(|G|, eps) from the parts, the same in every warp.
-__device__ __forceinline__ float scale_of(const double* parts, int num_parts, float eps, float unit) {
+// unit / max(|G|, eps) from the parts, the same in every warp: as the product of a power of two and a factor near unit,
+// since the norm of float32 values, or what divides by it, may be past float32.
+struct Scale {
+  float power, factor;
+};
+__device__ __forceinline__ Scale scale_of(const double* parts, int num_parts, float eps, float unit) {
   double sum = 0.0;
   for (int p = threadIdx.x & 31; p < num_parts; p += 32) sum += parts[p];
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-  const float norm = static_cast<float>(sqrt(sum));
-  return unit / (norm < eps ? eps : norm);  // NaN stays NaN
+  const double norm = sqrt(sum);
+  const double divisor = norm < eps ? eps : norm;  // NaN stays NaN
+  const int exponent = static_cast<int>((__double2hiint(divisor) >> 20) & 0x7ff) - 1023;
+  const int p = min(126, max(-126, exponent));
+  // an infinity in G makes the norm one: the matrix is NaN
+  const float rest = exponent > 1000 ? __int_as_float(0x7fffffff)
+                                     : static_cast<float>(divisor * __hiloint2double((1023 - p) << 20, 0));
+  return {__uint_as_float(static_cast<uint32_t>(127 - p) << 23), unit / rest};
 }
 
-__device__ __forceinline__ void split8(const float (&v)[8], float scale, uint4& hi, uint4& lo) {
+__device__ __forceinline__ void split8(const float (&v)[8], Scale scale, uint4& hi, uint4& lo) {
   uint32_t h[4], l[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const float a = v[2 * i] * scale, b = v[2 * i + 1] * scale;
+    const float a = v[2 * i] * scale.power * scale.factor, b = v[2 * i + 1] * scale.power * scale.factor;
     const __half2 p = __floats2half2_rn(a, b);
     const float2 back = __half22float2(p);
     const __half2 q = __floats2half2_rn(a - back.x, b - back.y);
@@ -118,7 +128,7 @@ __global__ void __launch_bounds__(kThreads) normalize_kernel(const void* __restr
                                                              __half* __restrict__ lo) {
   pdl_wait();
   const int64_t b = blockIdx.z;
-  const float scale = scale_of(parts + b * num_parts, num_parts, eps, unit);
+  const Scale scale = scale_of(parts + b * num_parts, num_parts, eps, unit);
   const int j = blockIdx.x * 512 + (threadIdx.x & 63) * 8;
   const int i0 = blockIdx.y * kNormRows + (threadIdx.x >> 6);
   pdl_trigger();
@@ -151,7 +161,7 @@ __global__ void __launch_bounds__(kThreads) normalize_tall_kernel(const void* __
   __shared__ float tile[64][65];
   pdl_wait();
   const int64_t b = blockIdx.z;
-  const float scale = scale_of(parts + b * num_parts, num_parts, eps, unit);
+  const Scale scale = scale_of(parts + b * num_parts, num_parts, eps, unit);
   pdl_trigger();
   const int i0 = blockIdx.y * 64, j0 = blockIdx.x * 64;
   const int e = (threadIdx.x & 7) * 8, w = threadIdx.x >> 3;

@@ -224,3 +224,13 @@ def test_small_sides_with_tiny_and_huge_columns(cuda_device):
     update[:, 2500:] *= 1e30
     got, want = orthogonalize(update), _exact(update)
     assert _off(got[:, 2500:], want[:, 2500:]) < WITHIN
+
+
+@pytest.mark.parametrize("shape", [(2, 150, 210), (2, 210, 150)])
+@pytest.mark.parametrize("scale,eps", [(1e37, 1e-7), (1e-40, 1e-42)])
+def test_large_sides_at_the_ends_of_the_range(cuda_device, shape, scale, eps):
+    """Finite values whose norm, or its reciprocal in the iteration's units, leaves float32."""
+    update = _updates("plain", shape, cuda_device, seed=14)
+    update[1] = update[0] / update[0].abs().amax() * 4.0 * scale
+    got, want = orthogonalize(update, eps=eps), _exact(update, eps=eps)
+    assert _off(got[1], want[1]) < 2.0 ** -8 and _off(got[0], want[0]) < WITHIN
