@@ -19,6 +19,7 @@ struct Args {
   int r, c, sp, cp, batch;
   int tiles_m, tiles_n, tiles;  // per matrix (tiles: those computed)
   float alpha, beta;
+  const float* shifts;   // [batch]: X is held times 1 / shift. kGram: alpha times its square; last kUpdate: both times it
   const __half* add_hi;  // kSquare: A; kUpdate: X
   const __half* add_lo;  // kUpdate: X's low parts, or null
   __half* out_hi;        // A, B or X'

@@ -182,8 +182,8 @@ __device__ __forceinline__ void store_turned(const Args& a, __nv_bfloat16* out, 
 
 // 32 consecutive accumulators of one row through the mode's epilogue. i, j: row and first column.
 template <Mode kMode>
-__device__ __forceinline__ void finish32(const Args& a, int b, int i, int j, bool mirror, const Added& added,
-                                         float (&v)[32]) {
+__device__ __forceinline__ void finish32(const Args& a, float alpha, float beta, int b, int i, int j, bool mirror,
+                                         const Added& added, float (&v)[32]) {
   if constexpr (kMode == kUpdate) {
     const int64_t at = (static_cast<int64_t>(b) * a.r + i) * a.cp + j;
     float x[32];
@@ -195,7 +195,7 @@ __device__ __forceinline__ void finish32(const Args& a, int b, int i, int j, boo
       for (int e = 0; e < 32; ++e) x[e] += lo[e];
     }
 #pragma unroll
-    for (int e = 0; e < 32; ++e) v[e] = fmaf(a.beta, x[e], a.alpha * v[e]);
+    for (int e = 0; e < 32; ++e) v[e] = fmaf(beta, x[e], alpha * v[e]);
     if (a.result != nullptr) {
       __nv_bfloat16* out = a.result + static_cast<int64_t>(b) * a.r * a.c;
       if (a.tall) {  // lanes hold consecutive rows: 64 contiguous bytes per column
@@ -236,10 +236,10 @@ __device__ __forceinline__ void finish32(const Args& a, int b, int i, int j, boo
       float x[32];
       widen32(added.hi, x);
 #pragma unroll
-      for (int e = 0; e < 32; ++e) v[e] = fmaf(a.beta, x[e], a.alpha * v[e]);
+      for (int e = 0; e < 32; ++e) v[e] = fmaf(beta, x[e], alpha * v[e]);
     } else {
 #pragma unroll
-      for (int e = 0; e < 32; ++e) v[e] *= a.alpha;
+      for (int e = 0; e < 32; ++e) v[e] *= alpha;
     }
     store32(a.out_hi + at, v);
     if (mirror) {
@@ -448,6 +448,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       locate<kMode, kN>(args, u, b, m, n);
       const int i = m * kTileM + static_cast<int>(rank) * kHalf + q * 32 + lane;
       const int j0 = n * kN + half * (kN / 2);
+      float alpha = args.alpha, beta = args.beta;
+      if (kMode == kGram || (kMode == kUpdate && args.result != nullptr)) {
+        const float shift = __ldg(args.shifts + b);
+        alpha *= shift;
+        if (kMode == kGram) alpha *= shift;
+        beta *= shift;
+      }
       Added added[2];
       fetch32<kMode>(args, b, i, j0, added[0]);
       if constexpr (kGroups > 1) fetch32<kMode>(args, b, i, j0 + 32, added[1]);
@@ -478,7 +485,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           float v[32];
 #pragma unroll
           for (int e = 0; e < 32; ++e) v[e] = __uint_as_float(r[e]);
-          finish32<kMode>(args, b, i, j, kN == 64 ? m != n >> 1 : m != n, added[c & 1], v);
+          finish32<kMode>(args, alpha, beta, b, i, j, kN == 64 ? m != n >> 1 : m != n, added[c & 1], v);
         }
         if constexpr (kMode == kUpdate) __syncwarp();  // lanes past the last row left early
         if (c + 2 < kGroups) fetch32<kMode>(args, b, i, j + 64, added[c & 1]);

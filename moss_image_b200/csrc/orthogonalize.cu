@@ -85,23 +85,28 @@ __global__ void __launch_bounds__(kThreads) sum_squares_kernel(const void* __res
 }
 
 // unit / max(|G|, eps) from the parts, the same in every warp: as the product of a power of two and a factor near unit,
-// since the norm of float32 values, or what divides by it, may be past float32.
+// since the norm of float32 values, or what divides by it, may be past float32. A matrix whose norm is so far below eps
+// that the steps only multiply it (by `growth` at most) is held larger by 1 / shift, or float16 would lose it.
 struct Scale {
-  float power, factor;
+  float power, factor, shift;
 };
-__device__ __forceinline__ Scale scale_of(const double* parts, int num_parts, float eps, float unit) {
+__device__ __forceinline__ Scale scale_of(const double* parts, int num_parts, float eps, float unit, double growth) {
   double sum = 0.0;
   for (int p = threadIdx.x & 31; p < num_parts; p += 32) sum += parts[p];
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
   const double norm = sqrt(sum);
-  const double divisor = norm < eps ? eps : norm;  // NaN stays NaN
-  const int exponent = static_cast<int>((__double2hiint(divisor) >> 20) & 0x7ff) - 1023;
+  auto exponent_of = [](double v) { return static_cast<int>((__double2hiint(v) >> 20) & 0x7ff) - 1023; };
+  auto power_of = [](int e) { return __uint_as_float(static_cast<uint32_t>(127 + e) << 23); };
+  const int held = norm < eps ? min(126, max(0, exponent_of(eps) - exponent_of(norm * growth) - 1)) : 0;
+  const float shift = power_of(-held);
+  const double divisor = (norm < eps ? eps : norm) * shift;  // NaN stays NaN
+  const int exponent = exponent_of(divisor);
   const int p = min(126, max(-126, exponent));
   // an infinity in G makes the norm one: the matrix is NaN
   const float rest = exponent > 1000 ? __int_as_float(0x7fffffff)
                                      : static_cast<float>(divisor * __hiloint2double((1023 - p) << 20, 0));
-  return {__uint_as_float(static_cast<uint32_t>(127 - p) << 23), unit / rest};
+  return {power_of(-p), unit / rest, shift};
 }
 
 __device__ __forceinline__ void split8(const float (&v)[8], Scale scale, uint4& hi, uint4& lo) {
@@ -124,11 +129,13 @@ constexpr int kNormRows = 16;
 template <int kKind>
 __global__ void __launch_bounds__(kThreads) normalize_kernel(const void* __restrict__ g, int r, int c, int cp, bool wide,
                                                              const double* __restrict__ parts, int num_parts,
-                                                             float eps, float unit, __half* __restrict__ hi,
-                                                             __half* __restrict__ lo) {
+                                                             float eps, float unit, double growth,
+                                                             __half* __restrict__ hi, __half* __restrict__ lo,
+                                                             float* __restrict__ shifts) {
   pdl_wait();
   const int64_t b = blockIdx.z;
-  const Scale scale = scale_of(parts + b * num_parts, num_parts, eps, unit);
+  const Scale scale = scale_of(parts + b * num_parts, num_parts, eps, unit, growth);
+  if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) shifts[b] = scale.shift;
   const int j = blockIdx.x * 512 + (threadIdx.x & 63) * 8;
   const int i0 = blockIdx.y * kNormRows + (threadIdx.x >> 6);
   pdl_trigger();
@@ -156,12 +163,14 @@ __global__ void __launch_bounds__(kThreads) normalize_kernel(const void* __restr
 template <int kKind>
 __global__ void __launch_bounds__(kThreads) normalize_tall_kernel(const void* __restrict__ g, int r, int c, int cp, bool wide,
                                                                   const double* __restrict__ parts,
-                                                                  int num_parts, float eps, float unit,
-                                                                  __half* __restrict__ hi, __half* __restrict__ lo) {
+                                                                  int num_parts, float eps, float unit, double growth,
+                                                                  __half* __restrict__ hi, __half* __restrict__ lo,
+                                                                  float* __restrict__ shifts) {
   __shared__ float tile[64][65];
   pdl_wait();
   const int64_t b = blockIdx.z;
-  const Scale scale = scale_of(parts + b * num_parts, num_parts, eps, unit);
+  const Scale scale = scale_of(parts + b * num_parts, num_parts, eps, unit, growth);
+  if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) shifts[b] = scale.shift;
   pdl_trigger();
   const int i0 = blockIdx.y * 64, j0 = blockIdx.x * 64;
   const int e = (threadIdx.x & 7) * 8, w = threadIdx.x >> 3;
@@ -192,7 +201,8 @@ __global__ void __launch_bounds__(kThreads) normalize_tall_kernel(const void* __
 // Norms and the padded, scaled operands.
 template <int kKind>
 static int launch_normalize(const void* g, int64_t batch, int r, int c, int cp, bool tall, float eps, float unit,
-                            double* parts, int num_parts, __half* hi, __half* lo, cudaStream_t stream) {
+                            double growth, double* parts, int num_parts, __half* hi, __half* lo, float* shifts,
+                            cudaStream_t stream) {
   const int64_t size = static_cast<int64_t>(r) * c;
   const bool aligned = reinterpret_cast<uintptr_t>(g) % 16 == 0;
   const unsigned z = static_cast<unsigned>(batch);
@@ -201,15 +211,15 @@ static int launch_normalize(const void* g, int64_t batch, int r, int c, int cp, 
   const bool wide = aligned && (tall ? r : c) % 8 == 0;
   if (tall)
     return launch_dependent("normalize_tall_kernel", normalize_tall_kernel<kKind>, dim3(cp / 64, (r + 63) / 64, z), dim3(kThreads),
-                            0, stream, g, r, c, cp, wide, parts, num_parts, eps, unit, hi, lo);
+                            0, stream, g, r, c, cp, wide, parts, num_parts, eps, unit, growth, hi, lo, shifts);
   return launch_dependent("normalize_kernel", normalize_kernel<kKind>, dim3((cp + 511) / 512, (r + kNormRows - 1) / kNormRows, z),
-                          dim3(kThreads), 0, stream, g, r, c, cp, wide, parts, num_parts, eps, unit, hi, lo);
+                          dim3(kThreads), 0, stream, g, r, c, cp, wide, parts, num_parts, eps, unit, growth, hi, lo, shifts);
 }
 
 struct Layout {
   int r, c, sp, cp, side, chunks;
   bool tall, small;
-  size_t x[2], low[2], a, b, parts, partial, exponents, q, factors, total;
+  size_t x[2], low[2], a, b, parts, shifts, partial, exponents, q, factors, total;
 };
 
 static Layout layout_of(int64_t batch, int64_t rows, int64_t cols) {
@@ -243,6 +253,7 @@ static Layout layout_of(int64_t batch, int64_t rows, int64_t cols) {
     l.a = take(square);
     l.b = take(square);
     l.parts = take(static_cast<size_t>(batch) * kNormParts * 8);
+    l.shifts = take(static_cast<size_t>(batch) * 4);
   }
   l.total = at;
   return l;
@@ -339,7 +350,10 @@ static int run(const void* g, int dtype, int64_t batch, int64_t rows, int64_t co
   // powers of two: X in units of 1 / unit (entries near 1), A and B in units of 1 / gain (below 2^14)
   const float unit = std::exp2(std::round(0.5 * std::log2(static_cast<double>(l.c))));
   const float gain = std::exp2(std::floor(14.0 - std::log2(most)));
+  double growth = 1.0, product = 1.0;  // of what is too small for the steps' squares to matter
+  for (int i = 0; i < steps; ++i) growth = std::max(growth, product *= std::fabs(static_cast<double>(coefficients[3 * i])));
   double* parts = reinterpret_cast<double*>(ws + l.parts);
+  float* shifts = reinterpret_cast<float*>(ws + l.shifts);
   const int64_t size = rows * cols;
   const int num_parts = static_cast<int>(std::max<int64_t>(
       1, std::min<int64_t>({(size + kPartValues - 1) / kPartValues, kNormParts, 8LL * sm_count() / batch + 1})));
@@ -348,11 +362,14 @@ static int run(const void* g, int dtype, int64_t batch, int64_t rows, int64_t co
   __half* ga = reinterpret_cast<__half*>(ws + l.a);
   __half* gb = reinterpret_cast<__half*>(ws + l.b);
   if (dtype == kBF16)
-    rc = launch_normalize<kBF16>(g, batch, l.r, l.c, l.cp, l.tall, eps, unit, parts, num_parts, x[0], low[0], stream);
+    rc = launch_normalize<kBF16>(g, batch, l.r, l.c, l.cp, l.tall, eps, unit, growth, parts, num_parts, x[0], low[0], shifts,
+                                 stream);
   else if (dtype == kF16)
-    rc = launch_normalize<kF16>(g, batch, l.r, l.c, l.cp, l.tall, eps, unit, parts, num_parts, x[0], low[0], stream);
+    rc = launch_normalize<kF16>(g, batch, l.r, l.c, l.cp, l.tall, eps, unit, growth, parts, num_parts, x[0], low[0], shifts,
+                                 stream);
   else
-    rc = launch_normalize<kF32>(g, batch, l.r, l.c, l.cp, l.tall, eps, unit, parts, num_parts, x[0], low[0], stream);
+    rc = launch_normalize<kF32>(g, batch, l.r, l.c, l.cp, l.tall, eps, unit, growth, parts, num_parts, x[0], low[0], shifts,
+                                 stream);
   if (rc != MOSS_OK) return rc;
   const int with_low = std::max(1, steps - 2);  // steps whose a X term reads lo
   for (int i = 0; i < steps; ++i) {
@@ -364,6 +381,7 @@ static int run(const void* g, int dtype, int64_t batch, int64_t rows, int64_t co
     a.cp = l.cp;
     a.batch = static_cast<int>(batch);
     a.tall = l.tall;
+    a.shifts = shifts;
     a.status = StatusSink{status, status_mirror_for_current_device()};
     const __half* xi = x[i & 1];
     a.alpha = gain / (unit * unit);

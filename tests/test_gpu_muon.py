@@ -234,3 +234,15 @@ def test_large_sides_at_the_ends_of_the_range(cuda_device, shape, scale, eps):
     update[1] = update[0] / update[0].abs().amax() * 4.0 * scale
     got, want = orthogonalize(update, eps=eps), _exact(update, eps=eps)
     assert _off(got[1], want[1]) < 2.0 ** -8 and _off(got[0], want[0]) < WITHIN
+
+
+@pytest.mark.parametrize("shape", [(3, 150, 210), (3, 210, 150), (3, 513, 300)])
+@pytest.mark.parametrize("scale", [1e-40, 1e-30, 1e-20, 1e-15, 1e-12])
+def test_large_sides_far_below_eps(cuda_device, shape, scale):
+    """G / eps is then far below float16's range next to matrices that are not, and so is the result."""
+    update = _updates("rows", shape, cuda_device, seed=19)
+    update[1] = update[0] / update[0].abs().amax() * scale
+    got, want = orthogonalize(update), _exact(update)
+    for i, one in enumerate(want):
+        assert _off(got[i], one) < WITHIN, (i, scale)
+    assert torch.equal(got[0], orthogonalize(update[:1])[0])
