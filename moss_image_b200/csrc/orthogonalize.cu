@@ -8,10 +8,10 @@
 // cost no more on the tensor cores than bfloat16's 8, and its range is met by powers of two, X times
 // about sqrt(c) (entries near 1) and A, B times `gain`. X itself is held as two float16 numbers,
 // hi + lo: products read hi, the a X term reads both, so that hi's rounding enters only through
-// (b A + c A A), which is small in the directions that still have to grow. The last two steps
-// grow nothing and drop lo. Against float64 the result is within 1.4 times its own rounding to bfloat16,
-// momentum with a few directions 80 times stronger than the rest included; bfloat16 operands are
-// 5 to 100 times further off. Tested in tests/test_gpu_muon.py.
+// (b A + c A A), which is small in the directions that still have to grow. lo is dropped for the last steps, two at
+// most, whose product of growths (kLateGrowth) leaves hi's rounding below bfloat16's. With the usual coefficients the
+// result is within 1.4 times its own rounding to bfloat16 of float64's, momentum with a few directions 80 times
+// stronger than the rest included; bfloat16 operands are 5 to 100 times further off. Tested in tests/test_gpu_muon.py.
 #include <algorithm>
 #include <cmath>
 #include <cstring>
@@ -259,11 +259,22 @@ static Layout layout_of(int64_t batch, int64_t rows, int64_t cols) {
   return l;
 }
 
-// Largest |s (a + b s^2 + c s^4)| over [0, top], and largest |b l + c l^2| over l = s^2 of the same range.
-static void bounds_of(const float* k, double top, double* value, double* square) {
+// A step p changes a rounding error of X by at most the largest slope |p'| over the singular values. Steps without lo:
+// their slopes' product is at most this, which the last two with the usual coefficients reach (4.9 each at the upper end of
+// the range; 3.4 at 0).
+constexpr double kLateGrowth = 25.0;
+
+// Over s in [0, top]: largest |p(s)| = |s (a + b s^2 + c s^4)|, largest |p'(s)|, and largest |b s^2 + c s^4|.
+static void bounds_of(const float* k, double top, double* value, double* slope, double* square) {
   const double a = k[0], b = k[1], c = k[2];
   auto p = [&](double s) { return std::fabs(s * (a + s * s * (b + c * s * s))); };
   auto m = [&](double l) { return std::fabs(l * (b + c * l)); };
+  auto d = [&](double l) { return std::fabs(a + l * (3.0 * b + 5.0 * c * l)); };  // l = s^2
+  *slope = std::max(d(0.0), d(top * top));
+  if (c != 0.0) {
+    const double l = -3.0 * b / (10.0 * c);
+    if (l > 0.0 && l < top * top) *slope = std::max(*slope, d(l));
+  }
   *value = p(top);
   const double disc = 9.0 * b * b - 20.0 * a * c;  // p' = a + 3 b l + 5 c l^2, l = s^2
   if (c != 0.0 && disc >= 0.0) {
@@ -300,13 +311,13 @@ static int run(const void* g, int dtype, int64_t batch, int64_t rows, int64_t co
     return fail(MOSS_ERR_INVALID_ARGUMENT, "orthogonalize takes 1 to %d steps with three coefficients each", kMaxSteps);
   if (!(eps > 0.0f) || !std::isfinite(eps)) return fail(MOSS_ERR_INVALID_ARGUMENT, "eps must be positive and finite");
   // singular values start in [0, 1]: where each step can take them bounds X, A and B
-  double top = 1.001, most = 1.0, widest = 1.0;
+  double top = 1.001, most = 1.0, widest = 1.0, slopes[kMaxSteps];
   for (int i = 0; i < steps; ++i) {
     const float* k = coefficients + 3 * i;
     if (!std::isfinite(k[0]) || !std::isfinite(k[1]) || !std::isfinite(k[2]))
       return fail(MOSS_ERR_INVALID_ARGUMENT, "the coefficients must be finite");
     double value, square;
-    bounds_of(k, top, &value, &square);
+    bounds_of(k, top, &value, &slopes[i], &square);
     most = std::max({most, top * top, square});
     widest = std::max(widest, top);
     top = 1.02 * value;
@@ -371,7 +382,8 @@ static int run(const void* g, int dtype, int64_t batch, int64_t rows, int64_t co
     rc = launch_normalize<kF32>(g, batch, l.r, l.c, l.cp, l.tall, eps, unit, growth, parts, num_parts, x[0], low[0], shifts,
                                  stream);
   if (rc != MOSS_OK) return rc;
-  const int with_low = std::max(1, steps - 2);  // steps whose a X term reads lo
+  int with_low = steps;  // steps whose a X term reads lo
+  for (double late = 1.0; with_low > std::max(1, steps - 2) && (late *= slopes[with_low - 1]) <= kLateGrowth;) --with_low;
   for (int i = 0; i < steps; ++i) {
     const float* k = coefficients + 3 * i;
     Args a{};

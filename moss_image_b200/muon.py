@@ -11,8 +11,8 @@ around it. CUDA tensors only: there is no CPU path.
 
 The result is bfloat16 whatever the input's type: it is a direction, and its own rounding is the
 largest error in it. The iteration runs on float16 operands with float32 sums (float32 throughout
-when the shorter side is at most 64), which keeps the error against float64 within 1.5 times that
-rounding. An infinity or NaN in a matrix gives a NaN matrix; a zero matrix gives zeros.
+when the shorter side is at most 64), which with the usual coefficients keeps the error against float64
+within 1.5 times that rounding. An infinity or NaN in a matrix gives a NaN matrix; a zero matrix gives zeros.
 """
 
 from __future__ import annotations

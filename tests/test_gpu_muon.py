@@ -246,3 +246,11 @@ def test_large_sides_far_below_eps(cuda_device, shape, scale):
     for i, one in enumerate(want):
         assert _off(got[i], one) < WITHIN, (i, scale)
     assert torch.equal(got[0], orthogonalize(update[:1])[0])
+
+
+@pytest.mark.parametrize("shape", [(256, 400), (400, 256), (2, 130, 700)])
+def test_late_steps_that_grow_small_values_keep_their_precision(cuda_device, shape):
+    """Later steps that multiply small singular values by 5 each, against the usual 3.4."""
+    update = _updates("strong", shape, cuda_device, seed=18)
+    growing = ((3.0, -3.0, 1.0), (5.0, -5.0, 1.0), (5.0, -5.0, 1.0))
+    assert _off(orthogonalize(update, 3, growing), _exact(update, 3, growing)) < WITHIN
