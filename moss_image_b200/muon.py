@@ -94,6 +94,10 @@ class Muon(torch.optim.Optimizer):
     ``s = 0.2 sqrt(max(rows, cols))``, which gives the update the root mean square that AdamW's usually
     has, so that its learning rates carry over. Matrices only: norms, biases and embeddings
     belong to another optimiser. Parameters of one shape and dtype are orthogonalised in one call.
+
+    The state is float32 whatever the parameters' type. For 16-bit parameters it also holds what their last
+    rounding left out (``remainder``): decay and update are applied to the sum of the two, so that steps far
+    below half a rounding step of a weight add up. A weight changed from outside keeps its new value.
     """
 
     def __init__(self, params: Iterable, lr: float = 1e-3, *, momentum: float = 0.95, nesterov: bool = True,
@@ -127,17 +131,41 @@ class Muon(torch.optim.Optimizer):
 
     def _step_shape(self, group: dict, shape: torch.Size, params: list[torch.Tensor]) -> None:
         momentum, grads = group["momentum"], [p.grad for p in params]
-        buffers = []
+        wide = params[0].dtype == torch.float32
+        buffers, remainders = [], []
         for p in params:
             state = self.state[p]
             if "momentum_buffer" not in state:
-                state["momentum_buffer"] = torch.zeros_like(p)
+                state["momentum_buffer"] = torch.zeros_like(p, dtype=torch.float32)
+            if not wide and "remainder" not in state:
+                state["remainder"] = torch.zeros_like(p, dtype=torch.float32)
             buffers.append(state["momentum_buffer"])
+            if not wide:
+                remainders.append(state["remainder"])
         torch._foreach_mul_(buffers, momentum)
         torch._foreach_add_(buffers, grads)
-        updates = torch._foreach_add(grads, buffers, alpha=momentum) if group["nesterov"] else buffers
+        if group["nesterov"]:
+            updates = torch._foreach_add(grads if wide else [g.float() for g in grads], buffers, alpha=momentum)
+        else:
+            updates = buffers
         directions = orthogonalize(torch.stack(updates), group["steps"], group["coefficients"], group["eps"])
-        if group["weight_decay"]:
-            torch._foreach_mul_(params, 1.0 - group["lr"] * group["weight_decay"])
         rate = group["lr"] * 0.2 * math.sqrt(max(shape))
-        torch._foreach_add_(params, list(directions.unbind(0)), alpha=-rate)
+        if wide:
+            exact = params
+        else:  # a weight that its remainder no longer rounds to was changed from outside
+            exact = [torch.where(e.to(p.dtype) == p, e, p.float())
+                     for e, p in zip(torch._foreach_add(remainders, params), params)]
+        if group["weight_decay"]:
+            torch._foreach_mul_(exact, 1.0 - group["lr"] * group["weight_decay"])
+        torch._foreach_add_(exact, list(directions.unbind(0)), alpha=-rate)
+        if not wide:
+            torch._foreach_copy_(params, exact)
+            torch._foreach_copy_(remainders, torch._foreach_sub(exact, params))
+
+    def load_state_dict(self, state_dict: dict) -> None:
+        super().load_state_dict(state_dict)
+        # the base class casts state to the parameter's type: the float32 state is taken as it was saved
+        saved = [index for group in state_dict["param_groups"] for index in group["params"]]
+        for index, p in zip(saved, (p for group in self.param_groups for p in group["params"])):
+            for name, value in state_dict["state"].get(index, {}).items():
+                self.state[p][name] = value.to(device=p.device, dtype=torch.float32, copy=True)

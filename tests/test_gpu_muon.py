@@ -254,3 +254,76 @@ def test_late_steps_that_grow_small_values_keep_their_precision(cuda_device, sha
     update = _updates("strong", shape, cuda_device, seed=18)
     growing = ((3.0, -3.0, 1.0), (5.0, -5.0, 1.0), (5.0, -5.0, 1.0))
     assert _off(orthogonalize(update, 3, growing), _exact(update, 3, growing)) < WITHIN
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("shape", [(24, 100), (150, 130)])
+def test_many_small_steps_of_16_bit_parameters_are_kept(cuda_device, shape, dtype):
+    """Steps and decay far below half a rounding step of the weights, against float64."""
+    gen = torch.Generator(device=cuda_device).manual_seed(15)
+    lr, decay, steps = 1e-4, 0.1, 120
+    p = torch.nn.Parameter((0.02 * torch.randn(*shape, generator=gen, device=cuda_device)).to(dtype))
+    w, m = p.detach().double(), torch.zeros(shape, dtype=torch.float64, device=cuda_device)
+    start = w.clone()
+    base = torch.randn(*shape, generator=gen, device=cuda_device)
+    optimizer = Muon([p], lr=lr, weight_decay=decay)
+    rate = lr * 0.2 * max(shape) ** 0.5
+    moved = 0.0
+    for _ in range(steps):
+        p.grad = (base + 0.3 * torch.randn(*shape, generator=gen, device=cuda_device)).to(dtype)
+        m.mul_(0.95).add_(p.grad.double())
+        direction = _exact(p.grad.double() + 0.95 * m)
+        w.mul_(1 - lr * decay).sub_(rate * direction)
+        moved += rate * float(direction.norm())
+        optimizer.step()
+    # the weights' own rounding (half a step of the type), each direction's, and float32 sums
+    room = 2.0 ** (-9 if dtype == torch.bfloat16 else -12) * float(w.norm()) * 1.01 + WITHIN * moved + steps * 2.0 ** -23 * float(w.norm())
+    assert float((p.detach().double() - w).norm()) < room < 0.2 * float((w - start).norm())
+
+
+def test_decay_alone_reaches_16_bit_parameters(cuda_device):
+    p = torch.nn.Parameter(torch.full((16, 32), 0.02, dtype=torch.bfloat16, device=cuda_device))
+    start = float(p.detach()[0, 0])
+    optimizer = Muon([p], lr=1e-3, weight_decay=0.1)
+    p.grad = torch.zeros_like(p)
+    for _ in range(200):
+        optimizer.step()
+    want = start * (1 - 1e-4) ** 200
+    assert bool(((p.detach().double() - want).abs() <= 2.0 ** -9 * want * 1.001).all())
+
+
+def test_state_of_16_bit_parameters_survives_a_checkpoint(cuda_device):
+    gen = torch.Generator(device=cuda_device).manual_seed(16)
+    params = [torch.nn.Parameter(torch.randn(20, 40, generator=gen, device=cuda_device).bfloat16()) for _ in range(2)]
+    optimizer = Muon(params, lr=1e-4)
+
+    def step(optimizer, params, seed):
+        gen = torch.Generator(device=cuda_device).manual_seed(seed)
+        for p in params:
+            p.grad = torch.randn(p.shape, generator=gen, device=cuda_device).to(p.dtype)
+        optimizer.step()
+
+    for seed in range(3):
+        step(optimizer, params, seed)
+    copies = [torch.nn.Parameter(p.detach().clone()) for p in params]
+    resumed = Muon(copies, lr=1e-4)
+    resumed.load_state_dict(optimizer.state_dict())
+    for seed in range(3, 12):
+        step(optimizer, params, seed)
+        step(resumed, copies, seed)
+    for p, q in zip(params, copies):
+        assert torch.equal(p, q)
+        for name, value in optimizer.state[p].items():
+            assert value.dtype == torch.float32 and torch.equal(value, resumed.state[q][name])
+
+
+def test_a_16_bit_weight_changed_from_outside_keeps_its_new_value(cuda_device):
+    p = torch.nn.Parameter(torch.full((16, 32), 0.02, dtype=torch.bfloat16, device=cuda_device))
+    optimizer = Muon([p], lr=1e-3, weight_decay=0.1)
+    p.grad = torch.zeros_like(p)
+    optimizer.step()  # leaves a remainder of 2e-6
+    changed = torch.linspace(0.0, 1e-4, 16 * 32, device=cuda_device).view(16, 32).bfloat16()
+    p.data.copy_(changed)
+    optimizer.param_groups[0]["lr"] = 0.0
+    optimizer.step()
+    assert torch.equal(p.detach(), changed)
