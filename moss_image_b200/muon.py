@@ -27,6 +27,11 @@ import torch
 from . import _lib
 from .quant_kernels import poll_device_status, status_buffer
 
+# What one call of a step may hold besides the parameters and their state (sums, directions, workspace). Matrices that fill
+# the GPU gain nothing from a larger batch: four of 3072 x 3072 take as long a matrix as forty.
+STEP_BYTES = 1 << 30
+_MOST_MATRICES = 65535  # in one call
+
 # Steep at zero: small singular values grow 3.4-fold a step, and all end within about 0.7 to 1.2.
 COEFFICIENTS = (3.4445, -4.7750, 2.0315)
 
@@ -86,6 +91,13 @@ def orthogonalize(update: torch.Tensor, steps: int = 5,
     return out
 
 
+def _matrices_at_once(rows: int, cols: int) -> int:
+    # two sums in float32, the direction in bfloat16
+    one = 10 * rows * cols + _workspace_bytes(1, rows, cols)
+    side = -(-min(rows, cols) // 128) * 128
+    return max(1, min(STEP_BYTES // max(one, 1), _MOST_MATRICES, (2**31 - 1) // max(side, 1)))
+
+
 class Muon(torch.optim.Optimizer):
     """Momentum, orthogonalised, as the update of each trained matrix.
 
@@ -93,7 +105,8 @@ class Muon(torch.optim.Optimizer):
     ``orthogonalize(m)``; then ``w <- (1 - lr weight_decay) w - lr s direction`` with
     ``s = 0.2 sqrt(max(rows, cols))``, which gives the update the root mean square that AdamW's usually
     has, so that its learning rates carry over. Matrices only: norms, biases and embeddings
-    belong to another optimiser. Parameters of one shape and dtype are orthogonalised in one call.
+    belong to another optimiser. Parameters of one shape and dtype are orthogonalised together, as many at
+    a time as ``STEP_BYTES`` of memory allow.
 
     The state is float32 whatever the parameters' type. For 16-bit parameters it also holds what their last
     rounding left out (``remainder``): decay and update are applied to the sum of the two, so that steps far
@@ -126,7 +139,9 @@ class Muon(torch.optim.Optimizer):
                 if p.grad is not None:
                     shapes.setdefault((p.shape, p.dtype, p.device), []).append(p)
             for (shape, _, _), params in shapes.items():
-                self._step_shape(group, shape, params)
+                most = _matrices_at_once(*shape)
+                for first in range(0, len(params), most):
+                    self._step_shape(group, shape, params[first:first + most])
         return loss
 
     def _step_shape(self, group: dict, shape: torch.Size, params: list[torch.Tensor]) -> None:
@@ -142,25 +157,37 @@ class Muon(torch.optim.Optimizer):
             buffers.append(state["momentum_buffer"])
             if not wide:
                 remainders.append(state["remainder"])
-        torch._foreach_mul_(buffers, momentum)
-        torch._foreach_add_(buffers, grads)
-        if group["nesterov"]:
-            updates = torch._foreach_add(grads if wide else [g.float() for g in grads], buffers, alpha=momentum)
-        else:
-            updates = buffers
-        directions = orthogonalize(torch.stack(updates), group["steps"], group["coefficients"], group["eps"])
-        rate = group["lr"] * 0.2 * math.sqrt(max(shape))
         if wide:
-            exact = params
-        else:  # a weight that its remainder no longer rounds to was changed from outside
-            exact = [torch.where(e.to(p.dtype) == p, e, p.float())
-                     for e, p in zip(torch._foreach_add(remainders, params), params)]
-        if group["weight_decay"]:
-            torch._foreach_mul_(exact, 1.0 - group["lr"] * group["weight_decay"])
-        torch._foreach_add_(exact, list(directions.unbind(0)), alpha=-rate)
-        if not wide:
-            torch._foreach_copy_(params, exact)
-            torch._foreach_copy_(remainders, torch._foreach_sub(exact, params))
+            torch._foreach_mul_(buffers, momentum)
+            torch._foreach_add_(buffers, grads)
+            updates = torch.stack(torch._foreach_add(grads, buffers, alpha=momentum) if group["nesterov"] else buffers)
+        else:
+            updates = torch.empty(len(params), *shape, device=params[0].device)
+            for grad, buffer, update in zip(grads, buffers, updates):
+                torch.add(grad, buffer, alpha=momentum, out=buffer)
+                if group["nesterov"]:
+                    torch.add(grad, buffer, alpha=momentum, out=update)
+                else:
+                    update.copy_(buffer)
+        directions = orthogonalize(updates, group["steps"], group["coefficients"], group["eps"])
+        del updates
+        rate = group["lr"] * 0.2 * math.sqrt(max(shape))
+        keep = 1.0 - group["lr"] * group["weight_decay"]
+        if wide:
+            if group["weight_decay"]:
+                torch._foreach_mul_(params, keep)
+            torch._foreach_add_(params, list(directions.unbind(0)), alpha=-rate)
+            return
+        for p, remainder, direction in zip(params, remainders, directions):
+            held = p.float()
+            exact = remainder + held
+            # a weight that its remainder no longer rounds to was changed from outside
+            exact = torch.where(exact.to(p.dtype) == p, exact, held)
+            if group["weight_decay"]:
+                exact.mul_(keep)
+            exact.add_(direction, alpha=-rate)
+            p.copy_(exact)
+            torch.sub(exact, p, out=remainder)
 
     def load_state_dict(self, state_dict: dict) -> None:
         super().load_state_dict(state_dict)

@@ -327,3 +327,38 @@ def test_a_16_bit_weight_changed_from_outside_keeps_its_new_value(cuda_device):
     optimizer.param_groups[0]["lr"] = 0.0
     optimizer.step()
     assert torch.equal(p.detach(), changed)
+
+
+def test_a_step_in_parts_is_the_step_at_once(cuda_device, monkeypatch):
+    from moss_image_b200 import muon
+
+    def run(limit):
+        if limit is not None:
+            monkeypatch.setattr(muon, "STEP_BYTES", limit)
+        gen = torch.Generator(device=cuda_device).manual_seed(17)
+        params = [torch.nn.Parameter(torch.randn(*s, generator=gen, device=cuda_device))
+                  for s in [(200, 130)] * 5 + [(20, 300)] * 3 + [(1, 1)]]
+        optimizer = Muon(params, lr=0.02, weight_decay=0.1)
+        for _ in range(2):
+            for p in params:
+                p.grad = torch.randn(p.shape, generator=gen, device=cuda_device)
+            optimizer.step()
+        return params
+
+    at_once, one_by_one = run(None), run(1)
+    for a, b in zip(at_once, one_by_one):
+        # the order of a matrix's sums may follow the size of its batch: one rounding of a direction to bfloat16
+        assert float((a - b).detach().norm()) <= 2 * 0.004 * (a.shape[0] * a.shape[1]) ** 0.5 * 2.0 ** -8
+
+
+def test_a_step_holds_a_bounded_share_of_memory(cuda_device):
+    params = [torch.nn.Parameter(torch.zeros(2048, 2048, dtype=torch.bfloat16, device=cuda_device)) for _ in range(60)]
+    for p in params:
+        p.grad = torch.ones_like(p)
+    optimizer = Muon(params)
+    optimizer.step()  # the state exists after it
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated(cuda_device)
+    torch.cuda.reset_peak_memory_stats(cuda_device)
+    optimizer.step()
+    assert torch.cuda.max_memory_allocated(cuda_device) - before < 2 << 30
