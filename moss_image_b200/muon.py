@@ -44,13 +44,30 @@ def _workspace_bytes(batch: int, rows: int, cols: int) -> int:
     return size.value
 
 
-@lru_cache(maxsize=64)
 def _coefficient_array(coefficients: tuple, steps: int) -> ctypes.Array:
     if coefficients and not isinstance(coefficients[0], tuple):
         coefficients = (coefficients,) * steps
     if len(coefficients) != steps or any(len(step) != 3 for step in coefficients):
         raise ValueError("orthogonalize: coefficients must be (a, b, c), or one such triple for each step.")
     return (ctypes.c_float * (3 * steps))(*(float(value) for step in coefficients for value in step))
+
+
+@lru_cache(maxsize=64)
+def _checked_steps(coefficients: tuple, steps: int, eps: float) -> ctypes.Array:
+    if not 1 <= steps <= 16:
+        raise ValueError("orthogonalize: steps must be between 1 and 16.")
+    if not (eps > 0.0 and math.isfinite(eps)):
+        raise ValueError("orthogonalize: eps must be positive and finite.")
+    values = _coefficient_array(coefficients, steps)
+    # of no matrices: the library looks at the steps and returns
+    _lib.check(_lib.library().moss_orthogonalize(None, _lib.DTYPE_CODES[torch.float32], 0, 0, 0, steps, values, eps, None,
+                                                 None, 0, None, None), "moss_orthogonalize")
+    return values
+
+
+def _step_values(steps: int, coefficients: Sequence, eps: float) -> ctypes.Array:
+    """The coefficients of each step, once all that does not depend on the matrices is checked."""
+    return _checked_steps(tuple(tuple(c) if isinstance(c, (tuple, list)) else c for c in coefficients), steps, float(eps))
 
 
 def orthogonalize(update: torch.Tensor, steps: int = 5,
@@ -65,11 +82,7 @@ def orthogonalize(update: torch.Tensor, steps: int = 5,
         raise RuntimeError("orthogonalize runs on CUDA tensors only (there is no CPU path).")
     if update.ndim < 2 or update.dtype not in _lib.DTYPE_CODES:
         raise ValueError("orthogonalize: the update must be a float16, bfloat16 or float32 [..., rows, cols] tensor.")
-    if not 1 <= steps <= 16:
-        raise ValueError("orthogonalize: steps must be between 1 and 16.")
-    if not (eps > 0.0 and math.isfinite(eps)):
-        raise ValueError("orthogonalize: eps must be positive and finite.")
-    values = _coefficient_array(tuple(tuple(c) if isinstance(c, (tuple, list)) else c for c in coefficients), steps)
+    values = _step_values(steps, coefficients, eps)
     device = update.device
     status = status_buffer(device)
     poll_device_status(device)
@@ -89,6 +102,12 @@ def orthogonalize(update: torch.Tensor, steps: int = 5,
         _lib.ptr(workspace), size, status.data_ptr(), _lib.stream_handle(device)), "moss_orthogonalize")
     _lib.count_launch("orthogonalize")
     return out
+
+
+def _check_options(group: dict) -> None:
+    if group["lr"] < 0.0 or group["weight_decay"] < 0.0 or not 0.0 <= group["momentum"] < 1.0:
+        raise ValueError("Muon: lr and weight_decay must not be negative, and momentum must be in [0, 1).")
+    _step_values(group["steps"], group["coefficients"], group["eps"])
 
 
 def _matrices_at_once(rows: int, cols: int) -> int:
@@ -116,16 +135,15 @@ class Muon(torch.optim.Optimizer):
     def __init__(self, params: Iterable, lr: float = 1e-3, *, momentum: float = 0.95, nesterov: bool = True,
                  weight_decay: float = 0.0, steps: int = 5, coefficients: Sequence[float] = COEFFICIENTS,
                  eps: float = 1e-7) -> None:
-        if lr < 0.0 or weight_decay < 0.0 or not 0.0 <= momentum < 1.0:
-            raise ValueError("Muon: lr and weight_decay must not be negative, and momentum must be in [0, 1).")
         super().__init__(params, dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay,
                                       steps=steps, coefficients=tuple(coefficients), eps=eps))
 
     def add_param_group(self, param_group: dict) -> None:
+        _check_options({**self.defaults, **param_group})
         super().add_param_group(param_group)
-        if any(p.ndim != 2 for p in self.param_groups[-1]["params"]):
+        if any(p.ndim != 2 or p.dtype not in _lib.DTYPE_CODES for p in self.param_groups[-1]["params"]):
             self.param_groups.pop()
-            raise ValueError("Muon updates matrices only (2 dimensions).")
+            raise ValueError("Muon updates matrices only (2 dimensions), of float16, bfloat16 or float32.")
 
     @torch.no_grad()
     def step(self, closure=None):
@@ -133,15 +151,20 @@ class Muon(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        parts = []  # all that can be refused is, before a parameter or its state changes
         for group in self.param_groups:
+            _check_options(group)
             shapes: dict[tuple, list[torch.Tensor]] = {}
             for p in group["params"]:
                 if p.grad is not None:
                     shapes.setdefault((p.shape, p.dtype, p.device), []).append(p)
-            for (shape, _, _), params in shapes.items():
+            for (shape, _, device), params in shapes.items():
+                if device.type != "cuda":
+                    raise RuntimeError("Muon runs on CUDA tensors only (there is no CPU path).")
                 most = _matrices_at_once(*shape)
-                for first in range(0, len(params), most):
-                    self._step_shape(group, shape, params[first:first + most])
+                parts.extend((group, shape, params[first:first + most]) for first in range(0, len(params), most))
+        for part in parts:
+            self._step_shape(*part)
         return loss
 
     def _step_shape(self, group: dict, shape: torch.Size, params: list[torch.Tensor]) -> None:

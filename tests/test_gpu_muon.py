@@ -362,3 +362,20 @@ def test_a_step_holds_a_bounded_share_of_memory(cuda_device):
     torch.cuda.reset_peak_memory_stats(cuda_device)
     optimizer.step()
     assert torch.cuda.max_memory_allocated(cuda_device) - before < 2 << 30
+
+
+def test_a_refused_step_leaves_the_momentum(cuda_device):
+    p = torch.nn.Parameter(torch.ones(8, 8, device=cuda_device))
+    optimizer = Muon([p])
+    p.grad = torch.ones_like(p)
+    optimizer.step()
+    held = {name: value.clone() for name, value in optimizer.state[p].items()}
+    weight = p.detach().clone()
+    for bad in (dict(steps=0), dict(eps=0.0), dict(coefficients=(40.0, 0.0, 0.0))):
+        good = {name: optimizer.param_groups[0][name] for name in bad}
+        optimizer.param_groups[0].update(bad)
+        with pytest.raises(ValueError):
+            optimizer.step()
+        optimizer.param_groups[0].update(good)
+        assert torch.equal(p.detach(), weight)
+        assert all(torch.equal(value, optimizer.state[p][name]) for name, value in held.items())
