@@ -55,6 +55,22 @@ def lay_out_fp8_codes(codes: torch.Tensor) -> torch.Tensor:
     return held
 
 
+def _padded_codes(codes: torch.Tensor) -> torch.Tensor:
+    """The codes as whole padded rows, ``[out, ceil(in / 16) * 16]`` without gaps, so that any dense copy of them keeps the
+    kernels' row pitch. The same memory where it is laid out like that already."""
+    codes = lay_out_fp8_codes(codes)
+    rows, columns = codes.shape
+    pitch = -(-columns // 16) * 16
+    if rows == 0 or columns == 0:
+        return codes.new_empty(rows, pitch)
+    room = codes.untyped_storage().nbytes() - codes.storage_offset()
+    if codes.stride(0) == pitch and room >= rows * pitch:
+        return codes.as_strided((rows, pitch), (pitch, 1))
+    held = _pitched_codes(rows, pitch, codes.device)
+    held[:, :columns].view(torch.uint8).copy_(codes.view(torch.uint8))
+    return held
+
+
 def quantize_fp8_weight(weight: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """e4m3 codes ``[out, in]`` and float32 scales ``[ceil(out / 128), ceil(in / 128)]`` of a CUDA weight.
 
@@ -218,8 +234,10 @@ class FrozenFp8Linear(nn.Module):
     """Block-scaled fp8 linear with gradients only to its input.
 
     Same life as :class:`~moss_image_b200.quantization.FrozenInt8Linear`: built from a frozen
-    ``nn.Linear`` on CUDA or from stored codes, usable as the base of a ``LoRALinear``. Buffers
-    ``weight_fp8`` (e4m3 ``[out, in]``), ``weight_scale`` (float32 per block) and ``bias``.
+    ``nn.Linear`` on CUDA or from stored codes, usable as the base of a ``LoRALinear``. State:
+    ``weight_fp8`` (e4m3 ``[out, in]``), ``weight_scale`` (float32 per block) and ``bias``. The module
+    holds the codes with rows padded to 16 bytes (the buffer ``padded_codes``), so that copies of its
+    buffers, as block swapping makes them, are laid out as the kernels read them.
     """
 
     fuses_lora = False  # the adapter's update has its own product
@@ -252,7 +270,7 @@ class FrozenFp8Linear(nn.Module):
 
     def _set_codes(self, codes: torch.Tensor, scale: torch.Tensor, bias: torch.Tensor | None, dtype: torch.dtype) -> None:
         self.out_features, self.in_features = codes.shape
-        self.register_buffer("weight_fp8", codes)
+        self.register_buffer("padded_codes", _padded_codes(codes), persistent=False)  # saved as weight_fp8
         self.register_buffer("weight_scale", scale)
         self.register_buffer("_dtype_anchor", torch.empty(0, device=codes.device, dtype=dtype), persistent=False)
         self.register_buffer("bias", bias)
@@ -262,6 +280,12 @@ class FrozenFp8Linear(nn.Module):
         return self._dtype_anchor.dtype
 
     @property
+    def weight_fp8(self) -> torch.Tensor:
+        """The codes ``[out, in]``: a view of the padded rows."""
+        codes = self.padded_codes
+        return codes if codes.shape[1] == self.in_features else codes[:, :self.in_features]
+
+    @property
     def weight(self) -> torch.Tensor:
         """A transient decoded copy, for inspection (the module itself never makes one)."""
         spread = self.weight_scale.repeat_interleave(BLOCK, 0)[: self.out_features]
@@ -269,19 +293,37 @@ class FrozenFp8Linear(nn.Module):
         return (self.weight_fp8.float() * spread).to(self.compute_dtype)
 
     def _apply(self, fn, recurse=True):
-        # Codes keep their type and their row pitch and scales stay float32 when model.to(dtype=...) casts.
-        codes, scale = self.weight_fp8, self.weight_scale
-        self.weight_fp8 = codes.new_empty(0, dtype=torch.uint8)
-        result = super()._apply(fn, recurse=recurse)
-        device = self._dtype_anchor.device
-        self.weight_scale = scale.to(device=device, dtype=torch.float32)
-        self.weight_fp8 = codes if codes.device == device else lay_out_fp8_codes(codes.to(device))
+        # Codes keep their type and scales stay float32 when model.to(dtype=...) casts.
+        codes, scale = self.padded_codes, self.weight_scale
+        self.padded_codes = codes.view(torch.uint8)
+        try:
+            result = super()._apply(fn, recurse=recurse)
+        finally:
+            self.padded_codes = self.padded_codes.view(torch.float8_e4m3fn)
+        self.weight_scale = scale.to(device=self._dtype_anchor.device, dtype=torch.float32)
         return result
 
-    def _load_from_state_dict(self, state_dict, prefix, *args, **kwargs):
-        # a stored copy is dense: copied into the pitched rows
-        super()._load_from_state_dict(state_dict, prefix, *args, **kwargs)
-        self.weight_fp8 = lay_out_fp8_codes(self.weight_fp8)
+    def _save_to_state_dict(self, destination, prefix, keep_vars):
+        destination[prefix + "weight_fp8"] = self.weight_fp8 if keep_vars else self.weight_fp8.detach()
+        super()._save_to_state_dict(destination, prefix, keep_vars)
+
+    def _load_from_state_dict(self, state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys,
+                              error_msgs):
+        super()._load_from_state_dict(state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs)
+        key = prefix + "weight_fp8"
+        if key in unexpected_keys:  # it is no buffer of that name
+            unexpected_keys.remove(key)
+        codes = state_dict.get(key)
+        if codes is None:
+            if strict:
+                missing_keys.append(key)
+        elif tuple(codes.shape) != (self.out_features, self.in_features):
+            error_msgs.append(f"size mismatch for {key}: {tuple(codes.shape)} in the checkpoint, "
+                              f"{(self.out_features, self.in_features)} in the module.")
+        elif local_metadata.get("assign_to_params_buffers", False):
+            self.padded_codes = _padded_codes(codes.to(torch.float8_e4m3fn))
+        else:
+            self.weight_fp8.view(torch.uint8).copy_(codes.to(torch.float8_e4m3fn).view(torch.uint8))
 
     def forward(self, tokens: torch.Tensor) -> torch.Tensor:
         return fp8_linear(tokens, self.weight_fp8, self.weight_scale, self.bias,

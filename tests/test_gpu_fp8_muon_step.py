@@ -2,6 +2,7 @@
 
 from __future__ import annotations
 
+import copy
 import importlib.util
 from pathlib import Path
 
@@ -90,3 +91,55 @@ def test_frozen_format_is_checked(cuda_device):
     with pytest.raises(ValueError, match="int8 or fp8"):
         build_lora_model(1, device=cuda_device, dim=64, heads=1, mlp_dim=64, frozen="fp4")
     assert SyntheticBlock(64, 1, 128).heads == 1
+
+
+@pytest.mark.parametrize("mode", ["sync", "async"])
+def test_swapped_fp8_blocks_of_any_width(cuda_device, mode):
+    """Input widths that are no multiple of 16 (codes with padded rows), on the CPU or in a pinned master."""
+    resident, swapped = (build_lora_model(3, device=cuda_device, dim=104, heads=2, mlp_dim=200, rank=4, seed=7,
+                                          frozen="fp8").train() for _ in range(2))
+    for model in (resident, swapped):
+        gen = torch.Generator(device=cuda_device).manual_seed(8)
+        for layer in model.layers:
+            for name in ("q", "k", "v", "o"):
+                layer.proj[name].lora_B.data.normal_(0.0, 0.03, generator=gen)
+    place_model(resident, cuda_device, 0)
+    place_model(swapped, cuda_device, 2, block_swap_mode=mode)
+    tokens = torch.randn(2, 24, 104, device=cuda_device, dtype=torch.bfloat16)
+    t = torch.tensor([0.3, 0.6], device=cuda_device)
+    rotary = rotary_table(torch.arange(24, device=cuda_device), rotary_frequencies(52, device=cuda_device))
+    outputs = [model(tokens, t, rotary=rotary) for model in (resident, swapped)]
+    assert torch.equal(*outputs)
+    for output in outputs:
+        output.float().square().mean().backward()
+    for a, b in zip(resident.parameters(), swapped.parameters()):
+        assert (a.grad is None) == (b.grad is None)
+        if a.grad is not None:
+            assert torch.equal(a.grad, b.grad.to(a.grad.device))
+    if swapped.block_swap_manager is not None:
+        swapped.block_swap_manager.close()
+
+
+def test_fp8_codes_keep_their_rows_through_moves_and_checkpoints(cuda_device):
+    torch.manual_seed(9)
+    linear = torch.nn.Linear(100, 70, device=cuda_device, dtype=torch.bfloat16).requires_grad_(False)
+    module = FrozenFp8Linear(linear)
+    x = torch.randn(5, 100, device=cuda_device, dtype=torch.bfloat16)
+    want = module(x)
+    assert module.weight_fp8.shape == (70, 100)
+    state = {name: value.detach().cpu().contiguous() for name, value in module.state_dict().items()}
+    assert list(state) == ["weight_fp8", "weight_scale", "bias"] and state["weight_fp8"].shape == (70, 100)
+    other = FrozenFp8Linear(torch.nn.Linear(100, 70, device=cuda_device, dtype=torch.bfloat16).requires_grad_(False))
+    for assign in (False, True):
+        on_device = {name: value.to(cuda_device) for name, value in state.items()}
+        assert not any(other.load_state_dict(on_device if assign else state, assign=assign))
+        assert torch.equal(other(x), want)
+    with pytest.raises(RuntimeError, match="weight_fp8"):
+        other.load_state_dict({name: value for name, value in state.items() if name != "weight_fp8"})
+    with pytest.raises(RuntimeError, match="weight_fp8"):
+        other.load_state_dict({**state, "weight_fp8": state["weight_fp8"][:, :96]})
+    assert torch.equal(other.cpu().to(cuda_device)(x), want)
+    assert torch.equal(copy.deepcopy(other)(x), want)
+    again = FrozenFp8Linear.from_codes(state["weight_fp8"].to(cuda_device), state["weight_scale"].to(cuda_device),
+                                       state["bias"].to(cuda_device))
+    assert torch.equal(again(x), want)
