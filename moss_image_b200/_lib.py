@@ -13,6 +13,7 @@ import threading
 from pathlib import Path
 
 import torch
+from torch.autograd import forward_ad
 
 LIB_PATH = Path(__file__).resolve().parent / "libmoss_w8.so"
 
@@ -191,6 +192,14 @@ def dtype_code(dtype: torch.dtype) -> int:
         return DTYPE_CODES[dtype]
     except KeyError:
         raise TypeError(f"int8 kernels do not support {dtype}.") from None
+
+
+def refuse_forward_mode(what: str, *tensors: torch.Tensor) -> None:
+    """Raise for inputs with a tangent, which a call that bypasses autograd would drop (they do not require grad)."""
+    if getattr(forward_ad, "_current_level", 0) < 0:  # outside dual_level()
+        return
+    if any(forward_ad.unpack_dual(tensor).tangent is not None for tensor in tensors):
+        raise NotImplementedError(f"{what} has no forward-mode derivative.")
 
 
 def ptr(tensor: torch.Tensor | None) -> int | None:

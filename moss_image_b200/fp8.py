@@ -218,6 +218,7 @@ class _Fp8Linear(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, gradient):
         weight, scale = ctx.saved_tensors
+        _lib.refuse_forward_mode("fp8_linear", gradient)
         _poll_after_backward(gradient.device)
         return fp8_linear_backward(gradient, weight, scale, ctx.input_dtype), None, None, None, None
 
@@ -225,6 +226,7 @@ class _Fp8Linear(torch.autograd.Function):
 def fp8_linear(tokens: torch.Tensor, weight: torch.Tensor, scale: torch.Tensor, bias: torch.Tensor | None = None,
                output_dtype: torch.dtype | None = None) -> torch.Tensor:
     """:func:`fp8_linear_forward`, differentiable in ``tokens`` (weight, scales and bias are frozen)."""
+    _lib.refuse_forward_mode("fp8_linear", tokens)
     if torch.is_grad_enabled() and tokens.requires_grad:
         return _Fp8Linear.apply(tokens, weight, scale, bias, output_dtype)
     return fp8_linear_forward(tokens, weight, scale, bias, output_dtype)

@@ -82,6 +82,7 @@ def orthogonalize(update: torch.Tensor, steps: int = 5,
         raise RuntimeError("orthogonalize runs on CUDA tensors only (there is no CPU path).")
     if update.ndim < 2 or update.dtype not in _lib.DTYPE_CODES:
         raise ValueError("orthogonalize: the update must be a float16, bfloat16 or float32 [..., rows, cols] tensor.")
+    _lib.refuse_forward_mode("orthogonalize", update)
     values = _step_values(steps, coefficients, eps)
     device = update.device
     status = status_buffer(device)

@@ -119,6 +119,7 @@ class _Rotary(torch.autograd.Function):
     @staticmethod
     def backward(ctx, q_grad, k_grad):
         cos, sin, positions = ctx.saved_tensors
+        _lib.refuse_forward_mode("apply_rotary", q_grad, k_grad)
         # a linear map: its gradient is the opposite turn, and so on for the gradient's
         turn = _Rotary.apply if torch.is_grad_enabled() else _launch
         q_grad, k_grad = turn(q_grad, k_grad, cos, sin, positions, ctx.interleaved, not ctx.inverse)
@@ -127,7 +128,7 @@ class _Rotary(torch.autograd.Function):
 
 def apply_rotary(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, *, interleaved: bool = True,
                  positions: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
-    """Queries and keys turned by their positions; differentiable in ``q`` and ``k``.
+    """Queries and keys turned by their positions; differentiable in ``q`` and ``k`` (reverse mode, to any order).
 
     ``q``: ``[batch, tokens, q_heads, head_dim]``, ``k``: the same with its own head count (any strides with
     a dense last dimension; views of a fused projection are read in place), or both packed as
@@ -160,6 +161,7 @@ def apply_rotary(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor, sin: torch
         if tuple(positions.shape) not in ((tokens,), tuple(q_shape[:-2])):
             raise ValueError("apply_rotary: positions must be [tokens] or [batch, tokens].")
         positions = positions.contiguous()
+    _lib.refuse_forward_mode("apply_rotary", q, k, cos, sin)
     cos, sin = cos.contiguous(), sin.contiguous()
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad):
         return _Rotary.apply(q, k, cos, sin, positions, interleaved, False)

@@ -284,3 +284,19 @@ def test_tile_outputs_of_any_width_and_alignment_stay_in_their_place(cuda_device
         assert run(out) is out
         _check(out, _quantized_rows(rows), *want)
         assert (room[:16 + offset] == 7.0).all() and (room[16 + offset + m * width:] == 7.0).all()
+
+
+def test_forward_mode_is_refused(cuda_device):
+    from torch.autograd import forward_ad
+
+    x, codes, scale, bias, _ = _problem(4, 96, 80, torch.float32, cuda_device)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        with pytest.raises(NotImplementedError):
+            fp8.fp8_linear(dual, codes, scale, bias)
+        with torch.no_grad(), pytest.raises(NotImplementedError):
+            fp8.fp8_linear(dual, codes, scale, bias)
+        assert torch.equal(fp8.fp8_linear(x, codes, scale, bias), fp8.fp8_linear_forward(x, codes, scale, bias))
+        tracked, y = x.clone().requires_grad_(), fp8.fp8_linear_forward(x, codes, scale)
+        with pytest.raises(NotImplementedError):
+            torch.autograd.grad(fp8.fp8_linear(tracked, codes, scale), tracked, forward_ad.make_dual(y, y))

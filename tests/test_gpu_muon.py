@@ -379,3 +379,13 @@ def test_a_refused_step_leaves_the_momentum(cuda_device):
         optimizer.param_groups[0].update(good)
         assert torch.equal(p.detach(), weight)
         assert all(torch.equal(value, optimizer.state[p][name]) for name, value in held.items())
+
+
+def test_forward_mode_is_refused(cuda_device):
+    from torch.autograd import forward_ad
+
+    update = torch.randn(8, 12, device=cuda_device)
+    with forward_ad.dual_level():
+        with pytest.raises(NotImplementedError):
+            orthogonalize(forward_ad.make_dual(update, torch.ones_like(update)))
+        assert torch.equal(orthogonalize(update), orthogonalize(update))

@@ -166,3 +166,23 @@ def test_offsets_past_32_bits(cuda_device):
     out, small = apply_rotary(q, q[:, :, :1], cos, sin, interleaved=False)
     _check(out[:, -3:], _turn(tail, cos[-3:], sin[-3:], False), tail)
     assert torch.equal(small[:, -3:], out[:, -3:, :1]) and not out[:, : tokens // 2].any()
+
+
+def test_forward_mode_is_refused(cuda_device):
+    from torch.autograd import forward_ad
+
+    q = torch.randn(1, 4, 2, 8, device=cuda_device)
+    cos, sin = _table(4, 4, cuda_device)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(q, torch.ones_like(q))
+        tables = [forward_ad.make_dual(t, torch.ones_like(t)) for t in (cos, sin)]
+        for arguments in ((dual, q, cos, sin), (q, dual, cos, sin), (q, q, tables[0], sin), (q, q, cos, tables[1]),
+                          (dual, q.clone().requires_grad_(), cos, sin)):
+            with pytest.raises(NotImplementedError):
+                apply_rotary(*arguments)
+            with torch.no_grad(), pytest.raises(NotImplementedError):
+                apply_rotary(*arguments)
+        assert torch.equal(apply_rotary(q, q, cos, sin)[0], apply_rotary(q, q, cos, sin)[1])
+        tracked = q.clone().requires_grad_()
+        with pytest.raises(NotImplementedError):
+            torch.autograd.grad(apply_rotary(tracked, q, cos, sin)[0], tracked, dual)
