@@ -70,13 +70,24 @@ def _step_values(steps: int, coefficients: Sequence, eps: float) -> ctypes.Array
     return _checked_steps(tuple(tuple(c) if isinstance(c, (tuple, list)) else c for c in coefficients), steps, float(eps))
 
 
+class _WithoutGradient(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, update, arguments):
+        return _orthogonalize(update, *arguments)
+
+    @staticmethod
+    def backward(ctx, gradient):
+        raise NotImplementedError("orthogonalize has no gradient: detach the update.")
+
+
 def orthogonalize(update: torch.Tensor, steps: int = 5,
                   coefficients: Sequence[float] | Sequence[Sequence[float]] = COEFFICIENTS, eps: float = 1e-7, *,
                   out: torch.Tensor | None = None) -> torch.Tensor:
     """The orthogonalised update of ``[rows, cols]`` or each of ``[..., rows, cols]``, in bfloat16.
 
     ``update``: float16, bfloat16 or float32 on CUDA. ``coefficients``: one ``(a, b, c)`` for all ``steps``
-    (1 to 16), or one for each. ``eps``: the least norm a matrix is divided by.
+    (1 to 16), or one for each. ``eps``: the least norm a matrix is divided by. Not differentiable: a backward
+    pass that reaches an update that requires grad raises.
     """
     if not update.is_cuda:
         raise RuntimeError("orthogonalize runs on CUDA tensors only (there is no CPU path).")
@@ -84,6 +95,15 @@ def orthogonalize(update: torch.Tensor, steps: int = 5,
         raise ValueError("orthogonalize: the update must be a float16, bfloat16 or float32 [..., rows, cols] tensor.")
     _lib.refuse_forward_mode("orthogonalize", update)
     values = _step_values(steps, coefficients, eps)
+    if torch.is_grad_enabled() and update.requires_grad:
+        if out is not None:
+            raise RuntimeError("orthogonalize: an update that requires grad cannot be written to an output buffer.")
+        return _WithoutGradient.apply(update, (values, eps, None))
+    return _orthogonalize(update, values, eps, out)
+
+
+def _orthogonalize(update: torch.Tensor, values: ctypes.Array, eps: float, out: torch.Tensor | None) -> torch.Tensor:
+    steps = len(values) // 3
     device = update.device
     status = status_buffer(device)
     poll_device_status(device)

@@ -389,3 +389,16 @@ def test_forward_mode_is_refused(cuda_device):
         with pytest.raises(NotImplementedError):
             orthogonalize(forward_ad.make_dual(update, torch.ones_like(update)))
         assert torch.equal(orthogonalize(update), orthogonalize(update))
+
+
+def test_a_gradient_is_refused_and_the_values_stay(cuda_device):
+    update = torch.randn(8, 12, device=cuda_device)
+    tracked = update.clone().requires_grad_()
+    direction = orthogonalize(tracked)
+    assert torch.equal(direction.detach(), orthogonalize(update))
+    with pytest.raises(NotImplementedError):
+        (direction.float().sum() + tracked.sum()).backward()
+    with torch.no_grad():
+        assert not orthogonalize(tracked).requires_grad
+    with pytest.raises(RuntimeError):
+        orthogonalize(tracked, out=torch.empty(8, 12, dtype=torch.bfloat16, device=cuda_device))
