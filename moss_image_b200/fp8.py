@@ -263,11 +263,11 @@ class FrozenFp8Linear(nn.Module):
             raise ValueError("fp8 scales must be float32 [ceil(out / 128), ceil(in / 128)].")
         if scale.device != codes.device or (bias is not None and bias.device != codes.device):
             raise ValueError("codes, scales and bias must be on one device.")
-        if bias is not None and tuple(bias.shape) != (codes.shape[0],):
-            raise ValueError("bias must be [out].")
+        if bias is not None and (tuple(bias.shape) != (codes.shape[0],) or bias.dtype not in _FLOATS):
+            raise ValueError("bias must be [out], of float16, bfloat16 or float32.")
         module = cls.__new__(cls)
         nn.Module.__init__(module)
-        module._set_codes(codes, scale.contiguous(), bias, dtype)
+        module._set_codes(codes, scale.contiguous(), None if bias is None else bias.contiguous(), dtype)
         return module
 
     def _set_codes(self, codes: torch.Tensor, scale: torch.Tensor, bias: torch.Tensor | None, dtype: torch.dtype) -> None:
