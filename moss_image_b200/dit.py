@@ -165,13 +165,15 @@ class SyntheticDiT(nn.Module):
             tokens = self._run_layers(tokens, cond, frozenset(skip_layers), rotary=rotary)
             return self.final_norm(tokens)
 
-    def forward_packed(self, samples: list[torch.Tensor], timestep: torch.Tensor) -> list[torch.Tensor]:
+    def forward_packed(self, samples: list[torch.Tensor], timestep: torch.Tensor,
+                       rotary: tuple[torch.Tensor, torch.Tensor] | None = None) -> list[torch.Tensor]:
         """One traversal over a heterogeneous batch: ``samples[i]`` is ``[tokens_i, dim]``.
 
         Mirrors ``forward_packed`` (training/model.py:502-626): the samples are concatenated
         into one ``[1, total, dim]`` stream with cumulative boundaries, every linear runs once
         over all tokens, attention is isolated per sample, and each sample keeps its own
-        timestep conditioning. Returns the per-sample outputs.
+        timestep conditioning. ``rotary``: the (cos, sin) tables of the stream, one row per token, the
+        samples' one after another. Returns the per-sample outputs.
         """
         if not samples:
             raise ValueError("forward_packed requires at least one sample.")
@@ -179,6 +181,8 @@ class SyntheticDiT(nn.Module):
         if any(sample.ndim != 2 or sample.shape[0] == 0 or sample.device != device for sample in samples):
             raise ValueError("Each packed sample must be a non-empty [tokens, dim] tensor on one device.")
         lengths = [sample.shape[0] for sample in samples]
+        if rotary is not None and any(table.shape[0] != sum(lengths) for table in rotary):
+            raise ValueError("The rotary tables of a packed stream have one row for each of its tokens.")
         times = torch.as_tensor(timestep, device=device).reshape(-1).expand(len(samples))
         cu_seqlens = cumulative_lengths(lengths, device)
         cu_seqlens.moss_lengths = tuple(lengths)  # known on the host: no device read per block
@@ -186,7 +190,7 @@ class SyntheticDiT(nn.Module):
         tokens = torch.cat(samples, 0).unsqueeze(0)
         with activation_cpu_offload(self, self.activation_offload, device):
             cond = self.time_embedding(times).to(tokens.dtype)
-            tokens = self._run_layers(tokens, cond, frozenset(), cu_seqlens)
+            tokens = self._run_layers(tokens, cond, frozenset(), cu_seqlens, rotary)
             return list(self.final_norm(tokens)[0].split(lengths, 0))
 
     def _run_layers(self, tokens: torch.Tensor, cond: torch.Tensor, skipped: frozenset[int],
@@ -302,17 +306,19 @@ def build_lora_model(depth: int, *, device: torch.device, dim: int = 3072, heads
 
 
 def packed_flow_matching_loss(model: SyntheticDiT, latents: list[torch.Tensor], text: list[torch.Tensor],
-                              t: torch.Tensor, noise: list[torch.Tensor]) -> torch.Tensor:
+                              t: torch.Tensor, noise: list[torch.Tensor],
+                              rotary: tuple[torch.Tensor, torch.Tensor] | None = None) -> torch.Tensor:
     """The flow-matching loss of a heterogeneous batch in one packed traversal.
 
-    ``latents[i]``/``noise[i]``: ``[image_tokens_i, dim]``; ``text[i]``: ``[text_tokens_i, dim]``.
+    ``latents[i]``/``noise[i]``: ``[image_tokens_i, dim]``; ``text[i]``: ``[text_tokens_i, dim]``; ``rotary``: tables
+    with a row for each token of the stream (each sample's image tokens, then its text tokens).
     Each sample's loss is its mean over its image tokens; the batch loss is their mean.
     """
     samples = []
     for latent, context, noise_i, sigma in zip(latents, text, noise, t):
         sigma = sigma.to(latent.dtype)
         samples.append(torch.cat(((1 - sigma) * latent + sigma * noise_i, context), 0))
-    outputs = model.forward_packed(samples, t)
+    outputs = model.forward_packed(samples, t, rotary)
     losses = [F.mse_loss(out[: latent.shape[0]].float(), (noise_i - latent).float())
               for out, latent, noise_i in zip(outputs, latents, noise)]
     return torch.stack(losses).mean()

@@ -143,3 +143,39 @@ def test_fp8_codes_keep_their_rows_through_moves_and_checkpoints(cuda_device):
     again = FrozenFp8Linear.from_codes(state["weight_fp8"].to(cuda_device), state["weight_scale"].to(cuda_device),
                                        state["bias"].to(cuda_device))
     assert torch.equal(again(x), want)
+
+
+@pytest.mark.parametrize("frozen", ["int8", "fp8"])
+def test_positions_in_a_packed_batch(cuda_device, frozen):
+    from moss_image_b200.dit import packed_flow_matching_loss
+
+    model = build_lora_model(2, device=cuda_device, dim=256, heads=4, mlp_dim=512, rank=8, seed=3, frozen=frozen).eval()
+    lengths = (37, 5, 64)
+    gen = torch.Generator(device=cuda_device).manual_seed(4)
+    samples = [torch.randn(n, 256, generator=gen, device=cuda_device).bfloat16() for n in lengths]
+    t = torch.tensor([0.1, 0.5, 0.9], device=cuda_device)
+    frequencies = rotary_frequencies(64, device=cuda_device)
+    places = [torch.arange(n, device=cuda_device) for n in lengths]
+    rotary = rotary_table(torch.cat(places), frequencies)
+    with torch.no_grad():
+        packed = model.forward_packed(samples, t, rotary=rotary)
+        for i, (sample, own) in enumerate(zip(samples, places)):
+            alone = model(sample[None], t[i:i + 1], rotary=rotary_table(own, frequencies))[0]
+            # the same arithmetic through other kernels: bfloat16 roundings of two blocks
+            assert float((packed[i].float() - alone.float()).norm() / alone.float().norm()) < 2e-2
+        still = model.forward_packed(samples, t, rotary=(torch.ones_like(rotary[0]), torch.zeros_like(rotary[1])))
+        plain = model.forward_packed(samples, t)
+        assert all(torch.equal(a, b) for a, b in zip(still, plain))
+        assert not torch.equal(packed[0], plain[0])
+        moved = rotary_table(torch.cat([places[0], places[1], 7 * places[2]]), frequencies)
+        other = model.forward_packed(samples, t, rotary=moved)
+        assert torch.equal(other[0], packed[0]) and torch.equal(other[1], packed[1]) and not torch.equal(other[2], packed[2])
+    for wrong in ((rotary[0][:-1], rotary[1][:-1]), rotary_table(torch.arange(200, device=cuda_device), frequencies)):
+        with pytest.raises(ValueError, match="packed"):
+            model.forward_packed(samples, t, rotary=wrong)
+    model.train()
+    latents, text = [s[:-2] for s in samples], [s[-2:] for s in samples]
+    noise = [torch.randn(*x.shape, generator=gen, device=cuda_device).bfloat16() for x in latents]
+    loss = packed_flow_matching_loss(model, latents, text, t, noise, rotary=rotary)
+    loss.backward()
+    assert loss.isfinite() and not torch.equal(loss, packed_flow_matching_loss(model, latents, text, t, noise))
