@@ -161,6 +161,8 @@ def apply_rotary(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor, sin: torch
         if tuple(positions.shape) not in ((tokens,), tuple(q_shape[:-2])):
             raise ValueError("apply_rotary: positions must be [tokens] or [batch, tokens].")
         positions = positions.contiguous()
+    if torch.is_grad_enabled() and (cos.requires_grad or sin.requires_grad):
+        raise ValueError("apply_rotary: the tables get no gradient: detach them.")
     _lib.refuse_forward_mode("apply_rotary", q, k, cos, sin)
     cos, sin = cos.contiguous(), sin.contiguous()
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad):

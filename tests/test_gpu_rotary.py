@@ -186,3 +186,14 @@ def test_forward_mode_is_refused(cuda_device):
         tracked = q.clone().requires_grad_()
         with pytest.raises(NotImplementedError):
             torch.autograd.grad(apply_rotary(tracked, q, cos, sin)[0], tracked, dual)
+
+
+def test_tables_that_ask_for_a_gradient_are_refused(cuda_device):
+    q = torch.randn(1, 4, 2, 8, device=cuda_device)
+    cos, sin = _table(4, 4, cuda_device)
+    learned = cos.clone().requires_grad_()
+    for arguments in ((q, q, learned, sin), (q, q, cos, learned), (q.clone().requires_grad_(), q, learned, sin)):
+        with pytest.raises(ValueError, match="gradient"):
+            apply_rotary(*arguments)
+    with torch.no_grad():
+        assert torch.equal(apply_rotary(q, q, learned, sin)[0], apply_rotary(q, q, cos, sin)[0])
