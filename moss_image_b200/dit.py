@@ -207,8 +207,10 @@ class SyntheticDiT(nn.Module):
         manager = getattr(self, "block_swap_manager", None)
         streamed = [index for index in range(boundary, len(self.layers)) if index not in skipped]
         position = {index: slot for slot, index in enumerate(streamed)}
-        for table in rotary or ():
-            setattr(table, KEEP_RESIDENT, True)  # the same table in every block
+        if rotary is not None:  # the same dense table in every block, marked on tensors of the model's own
+            rotary = tuple(table.contiguous().view_as(table) for table in rotary)
+            for table in rotary:
+                setattr(table, KEEP_RESIDENT, True)
         for index, layer in enumerate(self.layers):
             if index in skipped:
                 continue

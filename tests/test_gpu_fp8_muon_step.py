@@ -179,3 +179,23 @@ def test_positions_in_a_packed_batch(cuda_device, frozen):
     loss = packed_flow_matching_loss(model, latents, text, t, noise, rotary=rotary)
     loss.backward()
     assert loss.isfinite() and not torch.equal(loss, packed_flow_matching_loss(model, latents, text, t, noise))
+
+
+def test_the_callers_tables_are_not_marked_and_strided_ones_stay_resident(cuda_device):
+    from moss_image_b200.activation_offload import KEEP_RESIDENT, offload_ring
+
+    model = build_lora_model(2, device=cuda_device, dim=256, heads=4, mlp_dim=512, rank=8, seed=3, frozen="fp8").train()
+    model.gradient_checkpointing = False
+    model.activation_offload = True
+    tokens = torch.randn(1, 40, 256, device=cuda_device, dtype=torch.bfloat16)
+    t = torch.tensor([0.4], device=cuda_device)
+    dense = rotary_table(torch.arange(40, device=cuda_device), rotary_frequencies(64, device=cuda_device))
+    strided = tuple(table.t().contiguous().t() for table in dense)
+    ring = offload_ring(cuda_device)
+    sent = []
+    for tables in (dense, strided):
+        before = ring.stats()["d2h_bytes"]
+        model(tokens, t, rotary=tables).float().square().mean().backward()
+        sent.append(ring.stats()["d2h_bytes"] - before)
+        assert not any(hasattr(table, KEEP_RESIDENT) for table in tables)
+    assert sent[0] == sent[1] > 0
