@@ -7,6 +7,7 @@
 #include <atomic>
 #include <cstdarg>
 #include <cstdio>
+#include <mutex>
 #include <string>
 
 #include "../../include/moss_w8.h"
@@ -54,6 +55,32 @@ inline int device_sm_count() {
   if (device < 64) known[device].store(n, std::memory_order_relaxed);
   return n;
 }
+
+// What a kernel needs set up once on each device (function attributes belong to a device): `run` returns its error, and may
+// leave a number in `value` that later calls read. One static object per kernel.
+class DeviceSetup {
+ public:
+  static constexpr int kDevices = 64;
+  template <typename F>
+  int operator()(const char* what, int* value, const F& run) {
+    int device = 0;
+    const cudaError_t e = cudaGetDevice(&device);
+    if (e != cudaSuccess) return check_cuda(e, "cudaGetDevice");
+    if (device < 0 || device >= kDevices) return fail(MOSS_ERR_UNSUPPORTED, "device %d is past the first %d", device, kDevices);
+    Slot& slot = slots_[device];
+    std::call_once(slot.once, [&] { slot.error = run(&slot.value); });
+    if (value != nullptr) *value = slot.value;
+    return check_cuda(slot.error, what);
+  }
+
+ private:
+  struct Slot {
+    std::once_flag once;
+    cudaError_t error = cudaSuccess;
+    int value = 0;
+  };
+  Slot slots_[kDevices];
+};
 
 // Makes the current device's context current on this thread, as a kernel launch would. A thread
 // that has made no CUDA call yet (an autograd worker's first backward) has none, and the

@@ -17,7 +17,6 @@
 // f32x2 multiply-adds 25% (register moves), with a scale load waited for in the loop 15%.
 #include <algorithm>
 #include <cstring>
-#include <mutex>
 
 #include "dequant.cuh"
 #include "fp8_args.cuh"
@@ -504,9 +503,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 template <bool kDX, int kCtas, bool kF32Out>
 int launch_typed(const CUtensorMap& ta, const CUtensorMap& tw, const CUtensorMap& to, const Args& a, cudaStream_t stream) {
   auto kern = fp8_gemm_kernel<kDX, kCtas, kF32Out>;
-  static std::once_flag once;
-  static cudaError_t attr_err = cudaSuccess;
-  static int max_groups = 0;
+  static DeviceSetup setup;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = kCtas;
@@ -519,20 +516,21 @@ int launch_typed(const CUtensorMap& ta, const CUtensorMap& tw, const CUtensorMap
   cfg.dynamicSmemBytes = kSmemBytes;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  std::call_once(once, [&] {
-    attr_err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
-    if (attr_err != cudaSuccess) return;
-    max_groups = sm_count() / kCtas;
-    if (kCtas > 1) {
-      cfg.gridDim = dim3(kCtas * max_groups);
+  int max_groups = 0;
+  const int rc = setup("fp8_gemm_kernel", &max_groups, [&](int* groups) {
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+    *groups = sm_count() / kCtas;
+    if (e == cudaSuccess && kCtas > 1) {
+      cfg.gridDim = dim3(kCtas * *groups);
       int clusters = 0;
       if (cudaOccupancyMaxActiveClusters(&clusters, kern, &cfg) == cudaSuccess && clusters > 0)
-        max_groups = clusters;
+        *groups = clusters;
       else
         cudaGetLastError();
     }
+    return e;
   });
-  MOSS_CUDA_TRY(attr_err);
+  if (rc != MOSS_OK) return rc;
   const int64_t units = static_cast<int64_t>(a.tiles_m) * a.tiles_n * a.splits;
   cfg.gridDim = dim3(static_cast<unsigned>(kCtas * std::max<int64_t>(1, std::min<int64_t>(units, max_groups))));
   cfg.stream = stream;

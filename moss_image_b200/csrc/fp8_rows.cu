@@ -12,7 +12,6 @@
 // that holds the weight tiles of the same columns. Every column tile does that again, but for so few
 // rows it is less than a launch (2 rows x 3072 -> 18432: 16.4 us a call instead of 18.5).
 #include <algorithm>
-#include <mutex>
 
 #include "fp8_args.cuh"
 #include "fp8_codes.cuh"
@@ -337,12 +336,11 @@ __global__ void __launch_bounds__(Ring<kTN>::kThreads, 2)
 template <bool kDX, int kTN>
 int launch_typed(const CUtensorMap& ta, const CUtensorMap& tw, const Args& a, cudaStream_t stream) {
   auto kern = fp8_rows_kernel<kDX, kTN>;
-  static std::once_flag once;
-  static cudaError_t attr_err = cudaSuccess;
-  std::call_once(once, [&] {
-    attr_err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Ring<kTN>::kSmemBytes);
+  static DeviceSetup setup;
+  const int rc = setup("fp8_rows_kernel", nullptr, [&](int*) {
+    return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Ring<kTN>::kSmemBytes);
   });
-  MOSS_CUDA_TRY(attr_err);
+  if (rc != MOSS_OK) return rc;
   if (Ring<kTN>::kQuantises) {  // the call's first kernel
     kern<<<static_cast<unsigned>(a.tiles_m * a.tiles_n * a.splits), Ring<kTN>::kThreads, Ring<kTN>::kSmemBytes, stream>>>(
         ta, tw, a);

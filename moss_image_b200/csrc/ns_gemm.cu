@@ -14,7 +14,6 @@
 // latency, 5 us a product: 1.3 us from the launch to the first tile, the steps, the epilogue.
 #include <algorithm>
 #include <cstring>
-#include <mutex>
 
 #include "dequant.cuh"
 #include "ns_args.cuh"
@@ -523,9 +522,7 @@ template <Mode kMode, int kCtas, int kN>
 int launch_typed(const CUtensorMap& tl, const CUtensorMap& tr, Args a, cudaStream_t stream) {
   constexpr uint32_t kSmemBytes = Shape<kCtas, kN>::kSmemBytes;
   auto kern = ns_gemm_kernel<kMode, kCtas, kN>;
-  static std::once_flag once;
-  static cudaError_t attr_err = cudaSuccess;
-  static int max_groups = 0;
+  static DeviceSetup setup;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = kCtas;
@@ -538,20 +535,21 @@ int launch_typed(const CUtensorMap& tl, const CUtensorMap& tr, Args a, cudaStrea
   cfg.dynamicSmemBytes = kSmemBytes;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  std::call_once(once, [&] {
-    attr_err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
-    if (attr_err != cudaSuccess) return;
-    max_groups = sm_count() / kCtas;
-    if (kCtas > 1) {
-      cfg.gridDim = dim3(kCtas * max_groups);
+  int max_groups = 0;
+  const int rc = setup("ns_gemm_kernel", &max_groups, [&](int* groups) {
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+    *groups = sm_count() / kCtas;
+    if (e == cudaSuccess && kCtas > 1) {
+      cfg.gridDim = dim3(kCtas * *groups);
       int clusters = 0;
       if (cudaOccupancyMaxActiveClusters(&clusters, kern, &cfg) == cudaSuccess && clusters > 0)
-        max_groups = clusters;
+        *groups = clusters;
       else
         cudaGetLastError();
     }
+    return e;
   });
-  MOSS_CUDA_TRY(attr_err);
+  if (rc != MOSS_OK) return rc;
   a.tiles_m = (a.r + kHalf * kCtas - 1) / (kHalf * kCtas);
   a.tiles_n = ((kMode == kUpdate ? a.cp : a.sp) + kN - 1) / kN;
   a.tiles = kMode == kUpdate ? a.tiles_m * a.tiles_n : a.tiles_m * (a.tiles_m + 1) / 2 * (kN == 64 ? 2 : 1);

@@ -13,7 +13,6 @@
 // 53 us, of which the first takes 19 (57 MB), the second 11 and the third 20; all three are bound by latency,
 // at two CTAs a multiprocessor with one tile in registers while another is worked on.
 #include <algorithm>
-#include <mutex>
 
 #include "ns_args.cuh"
 
@@ -566,18 +565,18 @@ template <int kSide, int kKind>
 int launch_typed(const Small& s, cudaStream_t stream) {
   constexpr int kIterateBytes = 4 * kSide * (kSide + 4) * 4;
   constexpr int kApplyBytes = 2 * (2 * kTileHalves<kSide> + 2 * kSide * (kSide + 8));
-  static std::once_flag once;
-  static cudaError_t attr_err = cudaSuccess;
-  std::call_once(once, [] {
-    attr_err = cudaFuncSetAttribute(small_iterate_kernel<kSide>, cudaFuncAttributeMaxDynamicSharedMemorySize, kIterateBytes);
-    if (attr_err == cudaSuccess)
-      attr_err = cudaFuncSetAttribute(small_apply_kernel<kSide, kKind>, cudaFuncAttributeMaxDynamicSharedMemorySize, kApplyBytes);
+  static DeviceSetup setup;
+  int rc = setup("small_iterate_kernel", nullptr, [](int*) {
+    const cudaError_t e =
+        cudaFuncSetAttribute(small_iterate_kernel<kSide>, cudaFuncAttributeMaxDynamicSharedMemorySize, kIterateBytes);
+    if (e != cudaSuccess) return e;
+    return cudaFuncSetAttribute(small_apply_kernel<kSide, kKind>, cudaFuncAttributeMaxDynamicSharedMemorySize, kApplyBytes);
   });
-  MOSS_CUDA_TRY(attr_err);
+  if (rc != MOSS_OK) return rc;
   const unsigned batch = static_cast<unsigned>(s.batch);
   small_gram_kernel<kSide, kKind><<<dim3(s.chunks, batch), kThreads, 0, stream>>>(s);
   MOSS_CUDA_TRY(cudaGetLastError());
-  const int rc = launch_dependent("small_iterate_kernel", small_iterate_kernel<kSide>, dim3(batch),
+  rc = launch_dependent("small_iterate_kernel", small_iterate_kernel<kSide>, dim3(batch),
                                   dim3(kIterateThreads<kSide>), kIterateBytes, stream, s);
   if (rc != MOSS_OK) return rc;
   const int tiles = (s.c + kCols<kSide> - 1) / kCols<kSide>;
