@@ -210,6 +210,10 @@ def ptr(tensor: torch.Tensor | None) -> int | None:
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
+# The library works on the thread's current device: a call whose tensors are on another runs under torch.cuda.device.
+current_device_index = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
 def stream_handle(device: torch.device) -> int:
     if _raw_stream is None or device.index is None:
         return torch.cuda.current_stream(device).cuda_stream

@@ -80,6 +80,9 @@ def quantize_fp8_weight(weight: torch.Tensor) -> tuple[torch.Tensor, torch.Tenso
         raise ValueError("fp8 weights are quantized from a float [out, in] matrix.")
     if not weight.is_cuda:
         raise RuntimeError("fp8 linears run on CUDA tensors only (there is no CPU path).")
+    if weight.get_device() != _lib.current_device_index():
+        with torch.cuda.device(weight.device):
+            return quantize_fp8_weight(weight)
     weight = weight.contiguous()
     rows, columns = weight.shape
     codes = _pitched_codes(rows, columns, weight.device)
@@ -101,6 +104,9 @@ def quantize_fp8_rows(tokens: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]
         raise ValueError("fp8 rows are quantized from a float [rows, k] matrix.")
     if not tokens.is_cuda:
         raise RuntimeError("fp8 linears run on CUDA tensors only (there is no CPU path).")
+    if tokens.get_device() != _lib.current_device_index():
+        with torch.cuda.device(tokens.device):
+            return quantize_fp8_rows(tokens)
     tokens = tokens.contiguous()
     rows, columns = tokens.shape
     codes = torch.empty(rows, _blocks(columns) * BLOCK, dtype=torch.uint8, device=tokens.device)
@@ -113,15 +119,16 @@ def quantize_fp8_rows(tokens: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]
 
 
 @lru_cache(maxsize=1024)
-def _workspace_bytes(m: int, n_out: int, k_red: int) -> int:
+def _workspace_bytes(device: int, m: int, n_out: int, k_red: int) -> int:
     size = ctypes.c_size_t()
-    _lib.check(_lib.library().moss_fp8_linear_workspace_bytes(m, n_out, k_red, ctypes.byref(size)),
-               "moss_fp8_linear_workspace_bytes")
+    with torch.cuda.device(device):  # the plan counts its multiprocessors
+        _lib.check(_lib.library().moss_fp8_linear_workspace_bytes(m, n_out, k_red, ctypes.byref(size)),
+                   "moss_fp8_linear_workspace_bytes")
     return size.value
 
 
-def _check(tokens: torch.Tensor, weight: torch.Tensor, scale: torch.Tensor, side: int, what: str) -> None:
-    """``side``: the weight dimension that the input's last one has to match."""
+def _check(tokens: torch.Tensor, weight: torch.Tensor, k: int, scale: torch.Tensor, side: int, what: str) -> None:
+    """``k``: columns of the weight, whose rows may be padded; ``side``: its dimension that the input's last one has to match."""
     if not tokens.is_cuda:
         raise RuntimeError(f"{what} runs on CUDA tensors only (there is no CPU path).")
     if tokens.dtype not in _FLOATS:
@@ -131,11 +138,11 @@ def _check(tokens: torch.Tensor, weight: torch.Tensor, scale: torch.Tensor, side
         raise ValueError(f"{what}: the weight and its scales must be on the input's device.")
     if weight.dtype != torch.float8_e4m3fn or weight.ndim != 2 or scale.dtype != torch.float32:
         raise ValueError(f"{what}: the weight must be float8_e4m3fn [out, in] with float32 scales.")
-    n, k = shape = weight.shape
+    n = weight.shape[0]
     if scale.shape != (-(-n // BLOCK), -(-k // BLOCK)) or not scale.is_contiguous():
         raise ValueError(f"{what}: the scales must be a contiguous [ceil(out / 128), ceil(in / 128)] tensor.")
-    if tokens.ndim < 1 or tokens.shape[-1] != shape[side]:
-        raise ValueError(f"{what}: the input's last dimension must be {shape[side]}.")
+    if tokens.ndim < 1 or tokens.shape[-1] != (k if side else n):
+        raise ValueError(f"{what}: the input's last dimension must be {k if side else n}.")
     pitch, step = weight.stride()
     if n and k and (step != 1 or pitch % 16 or pitch < k or weight.data_ptr() % 16):
         raise ValueError(f"{what}: the weight's rows must be 16-byte aligned (lay_out_fp8_codes).")
@@ -160,9 +167,18 @@ def fp8_linear_forward(tokens: torch.Tensor, weight: torch.Tensor, scale: torch.
                        bias: torch.Tensor | None = None, output_dtype: torch.dtype | None = None, *,
                        out: torch.Tensor | None = None) -> torch.Tensor:
     """``Y = q(X) dec(W)^T (+ bias)`` for ``[..., in]`` tokens; ``output_dtype`` defaults to the tokens' own."""
+    return _forward(tokens, weight, None, scale, bias, output_dtype, out)
+
+
+def _forward(tokens: torch.Tensor, weight: torch.Tensor, columns: int | None, scale: torch.Tensor, bias: torch.Tensor | None,
+             output_dtype: torch.dtype | None, out: torch.Tensor | None) -> torch.Tensor:
     what = "fp8_linear_forward"
-    _check(tokens, weight, scale, 1, what)
-    n, k = weight.shape
+    n, k = weight.shape if weight.ndim == 2 else (0, 0)
+    k = k if columns is None else columns
+    _check(tokens, weight, k, scale, 1, what)
+    if tokens.get_device() != _lib.current_device_index():
+        with torch.cuda.device(tokens.device):
+            return _forward(tokens, weight, columns, scale, bias, output_dtype, out)
     if bias is not None and (bias.device != tokens.device or tuple(bias.shape) != (n,) or bias.dtype not in _FLOATS
                              or not bias.is_contiguous()):
         raise ValueError(f"{what}: the bias must be a contiguous float [out] tensor on the input's device.")
@@ -172,7 +188,7 @@ def fp8_linear_forward(tokens: torch.Tensor, weight: torch.Tensor, scale: torch.
     tokens = tokens.contiguous()
     output = _output(tokens, n, output_dtype or tokens.dtype, out, what)
     rows = _rows(tokens)
-    size = _workspace_bytes(rows, n, k)
+    size = _workspace_bytes(device.index, rows, n, k)
     workspace = torch.empty(size, dtype=torch.uint8, device=device) if size else None
     _lib.check(_lib.library().moss_fp8_linear_fwd(
         tokens.data_ptr(), _lib.DTYPE_CODES[tokens.dtype], rows, k, weight.data_ptr(), weight.stride(0),
@@ -186,16 +202,25 @@ def fp8_linear_forward(tokens: torch.Tensor, weight: torch.Tensor, scale: torch.
 def fp8_linear_backward(gradient: torch.Tensor, weight: torch.Tensor, scale: torch.Tensor,
                         output_dtype: torch.dtype | None = None, *, out: torch.Tensor | None = None) -> torch.Tensor:
     """``dX = q(dY) dec(W)`` for ``[..., out]`` gradients, from the same ``[out, in]`` codes."""
+    return _backward(gradient, weight, None, scale, output_dtype, out)
+
+
+def _backward(gradient: torch.Tensor, weight: torch.Tensor, columns: int | None, scale: torch.Tensor,
+              output_dtype: torch.dtype | None, out: torch.Tensor | None) -> torch.Tensor:
     what = "fp8_linear_backward"
-    _check(gradient, weight, scale, 0, what)
-    n, k = weight.shape
+    n, k = weight.shape if weight.ndim == 2 else (0, 0)
+    k = k if columns is None else columns
+    _check(gradient, weight, k, scale, 0, what)
+    if gradient.get_device() != _lib.current_device_index():
+        with torch.cuda.device(gradient.device):
+            return _backward(gradient, weight, columns, scale, output_dtype, out)
     device = gradient.device
     status = status_buffer(device)
     poll_device_status(device)
     gradient = gradient.contiguous()
     output = _output(gradient, k, output_dtype or gradient.dtype, out, what)
     rows = _rows(gradient)
-    size = _workspace_bytes(rows, k, n)
+    size = _workspace_bytes(device.index, rows, k, n)
     workspace = torch.empty(size, dtype=torch.uint8, device=device) if size else None
     _lib.check(_lib.library().moss_fp8_linear_dx(
         gradient.data_ptr(), _lib.DTYPE_CODES[gradient.dtype], rows, n, weight.data_ptr(), weight.stride(0),
@@ -209,10 +234,10 @@ class _Fp8Linear(torch.autograd.Function):
     """Saves only the weight's codes and scales, as the int8 linear does (training/quantization.py:29-45)."""
 
     @staticmethod
-    def forward(ctx, tokens, weight, scale, bias, output_dtype):
+    def forward(ctx, tokens, weight, columns, scale, bias, output_dtype):
         ctx.save_for_backward(weight, scale)
-        ctx.input_dtype = tokens.dtype
-        return fp8_linear_forward(tokens, weight, scale, bias, output_dtype)
+        ctx.input_dtype, ctx.columns = tokens.dtype, columns
+        return _forward(tokens, weight, columns, scale, bias, output_dtype, None)
 
     @staticmethod
     @once_differentiable
@@ -220,16 +245,21 @@ class _Fp8Linear(torch.autograd.Function):
         weight, scale = ctx.saved_tensors
         _lib.refuse_forward_mode("fp8_linear", gradient)
         _poll_after_backward(gradient.device)
-        return fp8_linear_backward(gradient, weight, scale, ctx.input_dtype), None, None, None, None
+        return _backward(gradient, weight, ctx.columns, scale, ctx.input_dtype, None), None, None, None, None, None
 
 
 def fp8_linear(tokens: torch.Tensor, weight: torch.Tensor, scale: torch.Tensor, bias: torch.Tensor | None = None,
                output_dtype: torch.dtype | None = None) -> torch.Tensor:
     """:func:`fp8_linear_forward`, differentiable in ``tokens`` (weight, scales and bias are frozen)."""
+    return _linear(tokens, weight, None, scale, bias, output_dtype)
+
+
+def _linear(tokens: torch.Tensor, weight: torch.Tensor, columns: int | None, scale: torch.Tensor, bias: torch.Tensor | None,
+            output_dtype: torch.dtype | None) -> torch.Tensor:
     _lib.refuse_forward_mode("fp8_linear", tokens)
     if torch.is_grad_enabled() and tokens.requires_grad:
-        return _Fp8Linear.apply(tokens, weight, scale, bias, output_dtype)
-    return fp8_linear_forward(tokens, weight, scale, bias, output_dtype)
+        return _Fp8Linear.apply(tokens, weight, columns, scale, bias, output_dtype)
+    return _forward(tokens, weight, columns, scale, bias, output_dtype, None)
 
 
 class FrozenFp8Linear(nn.Module):
@@ -328,8 +358,8 @@ class FrozenFp8Linear(nn.Module):
             self.weight_fp8.view(torch.uint8).copy_(codes.to(torch.float8_e4m3fn).view(torch.uint8))
 
     def forward(self, tokens: torch.Tensor) -> torch.Tensor:
-        return fp8_linear(tokens, self.weight_fp8, self.weight_scale, self.bias,
-                          autocast_compute_dtype(tokens, self.compute_dtype))
+        return _linear(tokens, self.padded_codes, self.in_features, self.weight_scale, self.bias,
+                       autocast_compute_dtype(tokens, self.compute_dtype))
 
     def extra_repr(self) -> str:
         return f"in_features={self.in_features}, out_features={self.out_features}, bias={self.bias is not None}"

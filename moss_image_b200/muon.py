@@ -37,10 +37,11 @@ COEFFICIENTS = (3.4445, -4.7750, 2.0315)
 
 
 @lru_cache(maxsize=1024)
-def _workspace_bytes(batch: int, rows: int, cols: int) -> int:
+def _workspace_bytes(device: int, batch: int, rows: int, cols: int) -> int:
     size = ctypes.c_size_t()
-    _lib.check(_lib.library().moss_orthogonalize_workspace_bytes(batch, rows, cols, ctypes.byref(size)),
-               "moss_orthogonalize_workspace_bytes")
+    with torch.cuda.device(device):  # the plan counts its multiprocessors
+        _lib.check(_lib.library().moss_orthogonalize_workspace_bytes(batch, rows, cols, ctypes.byref(size)),
+                   "moss_orthogonalize_workspace_bytes")
     return size.value
 
 
@@ -67,13 +68,15 @@ def _checked_steps(coefficients: tuple, steps: int, eps: float) -> ctypes.Array:
 
 def _step_values(steps: int, coefficients: Sequence, eps: float) -> ctypes.Array:
     """The coefficients of each step, once all that does not depend on the matrices is checked."""
-    return _checked_steps(tuple(tuple(c) if isinstance(c, (tuple, list)) else c for c in coefficients), steps, float(eps))
+    if coefficients is not COEFFICIENTS:
+        coefficients = tuple(tuple(c) if isinstance(c, (tuple, list)) else c for c in coefficients)
+    return _checked_steps(coefficients, steps, float(eps))
 
 
 class _WithoutGradient(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, update, arguments):
-        return _orthogonalize(update, *arguments)
+    def forward(ctx, update, *options):
+        return orthogonalize(update, *options)
 
     @staticmethod
     def backward(ctx, gradient):
@@ -98,13 +101,11 @@ def orthogonalize(update: torch.Tensor, steps: int = 5,
     if torch.is_grad_enabled() and update.requires_grad:
         if out is not None:
             raise RuntimeError("orthogonalize: an update that requires grad cannot be written to an output buffer.")
-        return _WithoutGradient.apply(update, (values, eps, None))
-    return _orthogonalize(update, values, eps, out)
-
-
-def _orthogonalize(update: torch.Tensor, values: ctypes.Array, eps: float, out: torch.Tensor | None) -> torch.Tensor:
-    steps = len(values) // 3
+        return _WithoutGradient.apply(update, steps, coefficients, eps)
     device = update.device
+    if device.index != _lib.current_device_index():
+        with torch.cuda.device(device):
+            return orthogonalize(update, steps, coefficients, eps, out=out)
     status = status_buffer(device)
     poll_device_status(device)
     update = update.detach().contiguous()
@@ -116,7 +117,7 @@ def _orthogonalize(update: torch.Tensor, values: ctypes.Array, eps: float, out: 
     batch = 1
     for length in update.shape[:-2]:
         batch *= length
-    size = _workspace_bytes(batch, rows, cols)
+    size = _workspace_bytes(device.index, batch, rows, cols)
     workspace = torch.empty(size, dtype=torch.uint8, device=device) if size else None
     _lib.check(_lib.library().moss_orthogonalize(
         update.data_ptr(), _lib.DTYPE_CODES[update.dtype], batch, rows, cols, steps, values, float(eps), out.data_ptr(),
@@ -131,9 +132,9 @@ def _check_options(group: dict) -> None:
     _step_values(group["steps"], group["coefficients"], group["eps"])
 
 
-def _matrices_at_once(rows: int, cols: int) -> int:
+def _matrices_at_once(device: int, rows: int, cols: int) -> int:
     # two sums in float32, the direction in bfloat16
-    one = 10 * rows * cols + _workspace_bytes(1, rows, cols)
+    one = 10 * rows * cols + _workspace_bytes(device, 1, rows, cols)
     side = -(-min(rows, cols) // 128) * 128
     return max(1, min(STEP_BYTES // max(one, 1), _MOST_MATRICES, (2**31 - 1) // max(side, 1)))
 
@@ -182,7 +183,7 @@ class Muon(torch.optim.Optimizer):
             for (shape, _, device), params in shapes.items():
                 if device.type != "cuda":
                     raise RuntimeError("Muon runs on CUDA tensors only (there is no CPU path).")
-                most = _matrices_at_once(*shape)
+                most = _matrices_at_once(device.index, *shape)
                 parts.extend((group, shape, params[first:first + most]) for first in range(0, len(params), most))
         for part in parts:
             self._step_shape(*part)

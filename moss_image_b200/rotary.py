@@ -93,6 +93,10 @@ def _heads_view(name: str, tensor: torch.Tensor) -> torch.Tensor:
 
 def _launch(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, positions: torch.Tensor | None,
             interleaved: bool, inverse: bool) -> tuple[torch.Tensor, torch.Tensor]:
+    device = q.device
+    if device.index != _lib.current_device_index():
+        with torch.cuda.device(device):
+            return _launch(q, k, cos, sin, positions, interleaved, inverse)
     q4, k4 = _heads_view("q", q), _heads_view("k", k)
     batch, tokens, q_heads, head_dim = q4.shape
     q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
@@ -103,7 +107,7 @@ def _launch(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor, sin: torch.Tens
         _lib.dtype_code(q.dtype), batch, tokens, head_dim, cos.data_ptr(), sin.data_ptr(), cos.shape[0],
         2 * cos.shape[1], None if positions is None else positions.data_ptr(),
         tokens if positions is not None and positions.ndim == 2 else 0, int(interleaved), int(inverse),
-        q_out.data_ptr(), k_out.data_ptr(), _lib.stream_handle(q.device))
+        q_out.data_ptr(), k_out.data_ptr(), _lib.stream_handle(device))
     _lib.check(rc, "moss_rotary")
     _lib.count_launch("rotary")
     return q_out, k_out

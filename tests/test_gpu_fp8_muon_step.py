@@ -199,3 +199,47 @@ def test_the_callers_tables_are_not_marked_and_strided_ones_stay_resident(cuda_d
         sent.append(ring.stats()["d2h_bytes"] - before)
         assert not any(hasattr(table, KEEP_RESIDENT) for table in tables)
     assert sent[0] == sent[1] > 0
+
+
+def test_calls_run_on_their_tensors_device_whatever_the_current_one(cuda_device, monkeypatch):
+    """Every entry point of these operators switches to the device of its tensors where another is current."""
+    from moss_image_b200 import _lib
+    from moss_image_b200.fp8 import fp8_linear_backward, fp8_linear_forward, quantize_fp8_rows, quantize_fp8_weight
+    from moss_image_b200.muon import orthogonalize
+    from moss_image_b200.rotary import apply_rotary
+
+    x = torch.randn(4, 128, device=cuda_device)
+    cos = torch.zeros(4, 4, device=cuda_device)
+
+    def everything():
+        codes, scale = quantize_fp8_weight(x)
+        quantize_fp8_rows(x)
+        y = fp8_linear_forward(x, codes, scale)
+        fp8_linear_backward(y, codes, scale)
+        orthogonalize(x)
+        apply_rotary(x.view(1, 4, 4, 32), x.view(1, 4, 4, 32), cos, cos)
+
+    everything()
+    entered = []
+    index = cuda_device.index or 0
+    current = [index]
+
+    class Guard:
+        def __init__(self, device):
+            self.device = device
+
+        def __enter__(self):
+            entered.append(self.device)
+            current[0] = index
+
+        def __exit__(self, *error):
+            current[0] = index + 1
+            return False
+
+    monkeypatch.setattr(torch.cuda, "device", Guard)
+    everything()
+    assert not entered  # the right device is current: no switch
+    monkeypatch.setattr(_lib, "current_device_index", lambda: current[0])
+    current[0] = index + 1
+    everything()
+    assert len(entered) == 6 and all(torch.device(device) == cuda_device for device in entered)
