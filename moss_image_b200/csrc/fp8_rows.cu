@@ -187,18 +187,19 @@ __global__ void __launch_bounds__(Ring<kTN>::kThreads, 2)
       tma_load_2d(base + stage * R::kStageBytes, &tm_w, bar(bars->full[stage]), kDX ? f0 : kb * kBlock,
                   kDX ? kb * kBlock : f0);
     };
-    if (lane == 0)
-      for (int i = 0; i < early; ++i) load_weight(i, kb0 + i);
-    pdl_wait();
     int stage = 0;
     uint32_t phase = 0, used = 0, last_phase = 0;
+    if (lane == 0) {
+      for (int i = 0; i < early; ++i) load_weight(i, kb0 + i);
+      used = (1u << early) - 1u;  // waited for below, even if the loop is left at once
+    }
+    pdl_wait();
     for (int kb = kb0; kb < kb1; ++kb) {
       if (!mbar_wait(bar(bars->empty[stage]), phase ^ 1u, abort_flag, args.status, MOSS_STATUS_TIMEOUT_LOAD)) break;
       if (lane == 0) {
         if (kb - kb0 >= early) load_weight(stage, kb);
         if constexpr (!R::kQuantises)
           tma_load_2d(base + stage * R::kStageBytes + kWBytes, &tm_a, bar(bars->full[stage]), kb * kBlock, m0);
-        used |= 1u << stage;
         last_phase = (last_phase & ~(1u << stage)) | (phase << stage);
       }
       __syncwarp();
