@@ -364,6 +364,45 @@ __device__ __forceinline__ float load_as_float(const void* p, int kind, int64_t 
   return __half2float(static_cast<const __half*>(p)[i]);
 }
 
+// 8 consecutive values from `at`, by 16-byte loads where `wide` says that they are aligned and whole; zero from `count` on.
+template <int kKind>
+__device__ __forceinline__ void load8(const void* x, int64_t at, int64_t count, bool wide, float (&v)[8]) {
+  if (wide) {
+    if constexpr (kKind == kF32) {
+      const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(x) + at);
+      const float4 a = __ldg(p), b = __ldg(p + 1);
+      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+      v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    } else {
+      const uint4 a = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(x) + at));
+      const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (kKind == kBF16) {
+          v[2 * i] = __uint_as_float(w[i] << 16);
+          v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        } else {
+          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+          v[2 * i] = f.x;
+          v[2 * i + 1] = f.y;
+        }
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = i < count ? load_as_float(x, kKind, at + i) : 0.0f;
+  }
+}
+
+// fmaxf drops NaN; a range that holds one has to show it.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+// 2^p for p in [-126, 127].
+__device__ __forceinline__ float pow2(int p) { return __uint_as_float(static_cast<uint32_t>(p + 127) << 23); }
+
 // Round an f32 to the given 16/32-bit float kind and back (round-to-nearest-even).
 __device__ __forceinline__ float round_to_kind(float x, int kind) {
   if (kind == kBF16) return __bfloat162float(__float2bfloat16_rn(x));

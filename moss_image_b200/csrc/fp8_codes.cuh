@@ -13,50 +13,11 @@ struct Raw {  // 8 values
   uint32_t w[kKind == kF32 ? 8 : 4];
 };
 
-// 8 consecutive values of a row from column c0, zero past k.
-template <int kKind>
-__device__ __forceinline__ void load8(const void* x, int64_t row, int64_t k, int64_t c0, bool wide, float (&v)[8]) {
-  const int64_t at = row * k + c0;
-  if (wide && c0 + 8 <= k) {
-    if constexpr (kKind == kF32) {
-      const float4 a = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(x) + at));
-      const float4 b = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(x) + at) + 1);
-      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-      v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-    } else {
-      const uint4 a = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(x) + at));
-      const uint32_t p[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if constexpr (kKind == kBF16) {
-          v[2 * i] = __uint_as_float(p[i] << 16);
-          v[2 * i + 1] = __uint_as_float(p[i] & 0xffff0000u);
-        } else {
-          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&p[i]));
-          v[2 * i] = f.x;
-          v[2 * i + 1] = f.y;
-        }
-      }
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = c0 + i < k ? load_as_float(x, kKind, at + i) : 0.0f;
-  }
-}
-
-// fmaxf drops NaN; a block that holds one has to show it.
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
-
 // Exponent p of the row scale: the least with amax <= 448 * 2^p = 1.75 * 2^(p + 8).
 __device__ __forceinline__ int scale_exponent(float amax) {
   const uint32_t bits = __float_as_uint(amax);
   return static_cast<int>(bits >> 23) - 127 - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
 }
-__device__ __forceinline__ float pow2(int p) { return __uint_as_float(static_cast<uint32_t>(p + 127) << 23); }
 
 __device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d) {
   const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);

@@ -64,7 +64,8 @@ __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const void* __r
       float v[8];
       float amax = kAmaxFloor;
       if (row < m && first + i < kb) {
-        load8<kKind>(x, row, k, static_cast<int64_t>(first + i) * kBlock + sub * 8, false, v);
+        const int64_t c0 = static_cast<int64_t>(first + i) * kBlock + sub * 8;
+        load8<kKind>(x, row * k + c0, k - c0, false, v);
 #pragma unroll
         for (int j = 0; j < 8; ++j) amax = max_nan(amax, fabsf(v[j]));
       }
@@ -109,7 +110,7 @@ __global__ void __launch_bounds__(kThreads) quantize_weight_kernel(const void* _
   for (int i = 0; i < kSweeps; ++i) {
     const int64_t row = row0 + i * kRowsPerCta;
     if (row < n) {
-      load8<kKind>(w, row, k, c0, wide, v[i]);
+      load8<kKind>(w, row * k + c0, k - c0, wide && c0 + 8 <= k, v[i]);
     } else {
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[i][j] = 0.0f;

@@ -76,7 +76,7 @@ inline EncodeTiledFn encode_fn() {
   return fn;
 }
 
-// Tiled tensor map of `rank` (2 or 3) dimensions: dims/box innermost first, strides in bytes
+// Tiled tensor map of `rank` (2 to 4) dimensions: dims/box innermost first, strides in bytes
 // for dimensions 1.. . Returns false (no map) when TMA cannot describe the view.
 inline bool make_map_nd(CUtensorMap* map, CUtensorMapDataType dt, int esize, const void* ptr, int rank,
                         const uint64_t* dims, const uint64_t* strides, const uint32_t* box, CUtensorMapSwizzle swz) {

@@ -82,13 +82,6 @@ __device__ __forceinline__ float4 to_float4(const Raw4<kKind>& r) {
   }
 }
 
-// fmaxf drops NaN; a tile that holds one has to show it.
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ float pow2(int p) { return __uint_as_float(static_cast<uint32_t>(p + 127) << 23); }
 // p with v in [2^(p + 10), 2^(p + 11)): v 2^-p is about 1024. At most 117, and not below -127, where 2^-p is still
 // normal: what is smaller, f32's subnormals included, is then below 2 and on a grid of 2^-22, which float16 holds.
 constexpr int kLeastScale = -127;

@@ -27,36 +27,6 @@ constexpr int kThreads = 256;
 constexpr int kNormParts = 512;       // at most, per matrix
 constexpr int kPartValues = 16384;    // values per part where there are fewer
 
-// 8 consecutive values, by 16-byte loads where `wide` says that every matrix allows them.
-template <int kKind>
-__device__ __forceinline__ void load8(const void* g, int64_t at, int count, bool wide, float (&v)[8]) {
-  if (wide) {
-    if constexpr (kKind == kF32) {
-      const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(g) + at);
-      const float4 a = __ldg(p), b = __ldg(p + 1);
-      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-      v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-    } else {
-      const uint4 a = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(g) + at));
-      const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if constexpr (kKind == kBF16) {
-          v[2 * i] = __uint_as_float(w[i] << 16);
-          v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-        } else {
-          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-          v[2 * i] = f.x;
-          v[2 * i + 1] = f.y;
-        }
-      }
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = i < count ? load_as_float(g, kKind, at + i) : 0.0f;
-  }
-}
-
 // Sums of squares over equal ranges of a matrix, in f64 (neither overflow nor a loss in long sums).
 template <int kKind>
 __global__ void __launch_bounds__(kThreads) sum_squares_kernel(const void* __restrict__ g, int64_t size, bool wide,
@@ -68,7 +38,7 @@ __global__ void __launch_bounds__(kThreads) sum_squares_kernel(const void* __res
 #pragma unroll 4
   for (int64_t i = first + threadIdx.x; i < last; i += kThreads) {
     float v[8];
-    load8<kKind>(g, base + i * 8, static_cast<int>(min(static_cast<int64_t>(8), size - i * 8)), wide, v);
+    load8<kKind>(g, base + i * 8, size - i * 8, wide, v);
 #pragma unroll
     for (int j = 0; j < 8; ++j) sum += static_cast<double>(v[j]) * v[j];
   }
@@ -97,16 +67,15 @@ __device__ __forceinline__ Scale scale_of(const double* parts, int num_parts, fl
   for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
   const double norm = sqrt(sum);
   auto exponent_of = [](double v) { return static_cast<int>((__double2hiint(v) >> 20) & 0x7ff) - 1023; };
-  auto power_of = [](int e) { return __uint_as_float(static_cast<uint32_t>(127 + e) << 23); };
   const int held = norm < eps ? min(126, max(0, exponent_of(eps) - exponent_of(norm * growth) - 1)) : 0;
-  const float shift = power_of(-held);
+  const float shift = pow2(-held);
   const double divisor = (norm < eps ? eps : norm) * shift;  // NaN stays NaN
   const int exponent = exponent_of(divisor);
   const int p = min(126, max(-126, exponent));
   // an infinity in G makes the norm one: the matrix is NaN
   const float rest = exponent > 1000 ? __int_as_float(0x7fffffff)
                                      : static_cast<float>(divisor * __hiloint2double((1023 - p) << 20, 0));
-  return {power_of(-p), unit / rest, shift};
+  return {pow2(-p), unit / rest, shift};
 }
 
 __device__ __forceinline__ void split8(const float (&v)[8], Scale scale, uint4& hi, uint4& lo) {
