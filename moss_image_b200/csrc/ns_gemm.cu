@@ -140,8 +140,8 @@ __device__ __forceinline__ void store32(__half* p, const float (&v)[32]) {
 }
 
 // A warp's 32 x 32 block of the result, lane by lane a row, written by columns: rows of any alignment, 64 bytes of
-// one at a time (stores of each lane along its own row meet 32 sectors each: 149 x 176 x 2546 took 1890 us,
-// 1310 without). Turned by shuffles: shared memory for it would be taken from the L1
+// one at a time (stores of each lane along its own row meet 32 sectors each: with them 149 x 176 x 2546 took
+// 1.4 times as long). Turned by shuffles: shared memory for it would be taken from the L1
 // cache, and the products that read and write much were 10% slower.
 __device__ __forceinline__ void store_turned(const Args& a, __nv_bfloat16* out, int i0, int j, const float (&v)[32]) {
   const int lane = threadIdx.x & 31;

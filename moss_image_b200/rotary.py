@@ -104,7 +104,7 @@ def _launch(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor, sin: torch.Tens
     qs, ks = q4.stride(), k4.stride()
     rc = _lib.library().moss_rotary(
         q4.data_ptr(), qs[0], qs[1], qs[2], q_heads, k4.data_ptr(), ks[0], ks[1], ks[2], k4.shape[2],
-        _lib.dtype_code(q.dtype), batch, tokens, head_dim, cos.data_ptr(), sin.data_ptr(), cos.shape[0],
+        _lib.DTYPE_CODES[q.dtype], batch, tokens, head_dim, cos.data_ptr(), sin.data_ptr(), cos.shape[0],
         2 * cos.shape[1], None if positions is None else positions.data_ptr(),
         tokens if positions is not None and positions.ndim == 2 else 0, int(interleaved), int(inverse),
         q_out.data_ptr(), k_out.data_ptr(), _lib.stream_handle(device))
@@ -139,7 +139,7 @@ def apply_rotary(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor, sin: torch
     ``[tokens, heads, head_dim]``; float16, bfloat16 or float32. ``cos``/``sin``: float32 ``[rows, R / 2]`` with
     ``R <= head_dim``; values past ``R`` are copied. Token ``t`` takes row ``t``, or row
     ``positions[t]`` / ``positions[batch, t]`` (int64) of a longer table. The tensors stay on the device
-    unread, so a position outside the table is not an error here: its token comes out NaN.
+    unread, so a position outside the table is not an error here: its token's turned values come out NaN.
     """
     if not q.is_cuda:
         raise RuntimeError("apply_rotary runs on CUDA tensors only (there is no CPU path).")
@@ -165,10 +165,11 @@ def apply_rotary(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor, sin: torch
         if tuple(positions.shape) not in ((tokens,), tuple(q_shape[:-2])):
             raise ValueError("apply_rotary: positions must be [tokens] or [batch, tokens].")
         positions = positions.contiguous()
-    if torch.is_grad_enabled() and (cos.requires_grad or sin.requires_grad):
+    tracking = torch.is_grad_enabled()
+    if tracking and (cos.requires_grad or sin.requires_grad):
         raise ValueError("apply_rotary: the tables get no gradient: detach them.")
     _lib.refuse_forward_mode("apply_rotary", q, k, cos, sin)
     cos, sin = cos.contiguous(), sin.contiguous()
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad):
+    if tracking and (q.requires_grad or k.requires_grad):
         return _Rotary.apply(q, k, cos, sin, positions, interleaved, False)
     return _launch(q, k, cos, sin, positions, interleaved, False)
