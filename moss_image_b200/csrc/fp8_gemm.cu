@@ -12,7 +12,8 @@
 //
 // What bounds it: the MMAs of a 256 x 256 x 128 block take 715 cycles here (512 by the pipe's rate), and the
 // epilogue keeps pace with them; the staging of a finished tile is the rest. 9216 x 3072 -> 12288: 310 us
-// or 2.25 PFLOP/s (the MMAs alone 233 us; cuBLAS with one scale per tensor 245). What each part of the
+// or 2.25 PFLOP/s in short runs (the MMAs alone 233 us; cuBLAS with one scale per tensor 245; a call in a long loop, the
+// rows quantised first and the clock under the power cap, 385). What each part of the
 // epilogue is there for: with 16 warps of 64 sums it lost 7%, with direct row stores 20%, with packed
 // f32x2 multiply-adds 25% (register moves), with a scale load waited for in the loop 15%.
 #include <algorithm>

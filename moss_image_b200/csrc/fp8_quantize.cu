@@ -95,7 +95,8 @@ int launch_quantize_rows(const void* x, int dtype, int64_t m, int64_t k, uint8_t
   return launch_rows_of<kF32>(x, m, k, codes, scale, row_pitch, stream);
 }
 
-// One CTA per 128 x 128 weight block: 16 rows at a time, 8 sweeps held in registers.
+// One CTA per 128 x 128 weight block: 16 rows at a time, 8 sweeps held in registers. Once per weight: 12288 x 3072 bf16
+// 76 us (1.5 TB/s; a true division for every value).
 template <int kKind>
 __global__ void __launch_bounds__(kThreads) quantize_weight_kernel(const void* __restrict__ w, int64_t n, int64_t k,
                                                                    bool wide, uint8_t* __restrict__ codes, int64_t ld,

@@ -10,7 +10,7 @@
 // tiles would be three quarters empty here, and these kernels are bound by HBM and latency.)
 //
 // Three launches: partial R over column ranges, the iteration (one CTA per matrix), Q X. 144 x 32 x 3072 f32:
-// 53 us, of which the first takes 19 (57 MB), the second 11 and the third 20; all three are bound by latency,
+// 54 us, of which the first takes 19 (57 MB), the second 11 and the third 20; all three are bound by latency,
 // at two CTAs a multiprocessor with one tile in registers while another is worked on.
 #include <algorithm>
 
