@@ -272,6 +272,22 @@ MOSS_API int moss_rmsnorm_bwd(const void* dy, const void* x, int x_dtype, int64_
                      const void* weight, int w_dtype, const float* rstd, void* dx, moss_stream_t stream);
 
 /*
+ * Layer norm over the last dimension (1 to 16384 values): y = (x - mean) * rstd * weight + bias, statistics and
+ * arithmetic in f32, one rounding to y's dtype = promote(x, weight). weight and bias are [dim] of one dtype, either
+ * may be null. stats (optional in the forward): f32 [rows][2], each row's mean and rstd.
+ * The backward gives dx and, where dw or db is not null, the sums over rows of dy * n and of dy in the gain's
+ * dtype (zeros for no rows); dx may be null. `gain` says whether the forward had a weight or a bias (it
+ * decides dy's dtype). The sums need moss_layernorm_bwd_workspace_bytes(rows, dim) bytes, 16-byte aligned.
+ * Results do not depend on timing.
+ */
+MOSS_API int moss_layernorm_fwd(const void* x, int x_dtype, int64_t rows, int64_t dim, const void* weight,
+                       const void* bias, int g_dtype, float eps, void* y, float* stats, moss_stream_t stream);
+MOSS_API int moss_layernorm_bwd_workspace_bytes(int64_t rows, int64_t dim, size_t* bytes);
+MOSS_API int moss_layernorm_bwd(const void* dy, const void* x, int x_dtype, int64_t rows, int64_t dim,
+                       const void* weight, int g_dtype, const float* stats, int gain, void* dx, void* dw, void* db,
+                       void* workspace, size_t workspace_bytes, moss_stream_t stream);
+
+/*
  * Block-scaled fp8 (e4m3) frozen linear: the 8-bit floating-point sibling of the int8 linear
  * (training/quantization.py:68-131). Weight codes [n, k] with a row pitch ld (a multiple of 16 bytes, 16-byte
  * aligned) and one f32 scale per 128 x 128 block, [ceil(n / 128), ceil(k / 128)]. Activations and gradients are
