@@ -288,6 +288,25 @@ MOSS_API int moss_layernorm_bwd(const void* dy, const void* x, int x_dtype, int6
                        void* workspace, size_t workspace_bytes, moss_stream_t stream);
 
 /*
+ * Activations as 8-bit codes: int8 codes in [-127, 127] and one power of two for each block of 32 columns of a row, the
+ * least 2^p with max|x| <= 127 * 2^p, p in [-126, 9] for f16 and [-126, 121] otherwise; codes x / 2^p rounded to
+ * nearest even. exponents[rows][ceil(cols / 32)] holds p + 127, or 255 for a block with an infinity or NaN
+ * (it decodes to NaN). A decoded value is within max|x| / 127 of x, and exact in x's dtype. Codes are [rows, cols] with a
+ * pitch ld (a multiple of 16 bytes, 16-byte aligned; the encoder writes the least one, and zeros up to it).
+ *   gradient: dw[n, cols] = dy[rows, n]^T decode(codes), dy f16 or bf16, f32 sums in a fixed order, one rounding.
+ * `workspace`: at least moss_coded_gradient_workspace_bytes(rows, n, cols) bytes, 256-byte aligned, free for reuse
+ * once the stream has passed the call.
+ */
+MOSS_API int moss_codes_encode(const void* x, int dtype, int64_t rows, int64_t cols, int8_t* codes, int64_t ld,
+                      uint8_t* exponents, moss_stream_t stream);
+MOSS_API int moss_codes_decode(const int8_t* codes, int64_t ld, const uint8_t* exponents, int64_t rows, int64_t cols,
+                      void* out, int dtype, moss_stream_t stream);
+MOSS_API int moss_coded_gradient_workspace_bytes(int64_t rows, int64_t n, int64_t cols, size_t* bytes);
+MOSS_API int moss_coded_gradient(const void* dy, int dtype, int64_t rows, int64_t n, const int8_t* codes, int64_t ld,
+                        const uint8_t* exponents, int64_t cols, void* dw, int dw_dtype, void* workspace,
+                        size_t workspace_bytes, int* status, moss_stream_t stream);
+
+/*
  * Block-scaled fp8 (e4m3) frozen linear: the 8-bit floating-point sibling of the int8 linear
  * (training/quantization.py:68-131). Weight codes [n, k] with a row pitch ld (a multiple of 16 bytes, 16-byte
  * aligned) and one f32 scale per 128 x 128 block, [ceil(n / 128), ceil(k / 128)]. Activations and gradients are

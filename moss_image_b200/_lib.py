@@ -73,6 +73,11 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "moss_layernorm_bwd_workspace_bytes": (_i32, [_i64, _i64, ctypes.POINTER(_sz)]),
     "moss_layernorm_bwd": (
         _i32, [_vp, _vp, _i32, _i64, _i64, _vp, _i32, _vp, _i32, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "moss_codes_encode": (_i32, [_vp, _i32, _i64, _i64, _vp, _i64, _vp, _vp]),
+    "moss_codes_decode": (_i32, [_vp, _i64, _vp, _i64, _i64, _vp, _i32, _vp]),
+    "moss_coded_gradient_workspace_bytes": (_i32, [_i64, _i64, _i64, ctypes.POINTER(_sz)]),
+    "moss_coded_gradient": (
+        _i32, [_vp, _i32, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _i32, _vp, _sz, _vp, _vp]),
     "moss_fp8_linear_workspace_bytes": (_i32, [_i64, _i64, _i64, ctypes.POINTER(_sz)]),
     "moss_fp8_linear_fwd": (
         _i32, [_vp, _i32, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _i32, _vp, _i32, _vp, _sz, _vp, _vp]),

@@ -1,0 +1,48 @@
+// Shared declarations of the coded activations (activation_codes.cu, codes_gemm.cu, codes_rows.cu).
+//
+// A row of values is held as int8 codes with one power of two for each block of 32 columns:
+//   x ~ code * 2^p,  p the least with max|x| <= 127 * 2^p, within [-126, cap] (cap: 9 for f16, else 121)
+// The exponent byte is p + 127. A block with an infinity or NaN has the byte 255 and zero codes: its scale
+// reads as an infinity, and 0 * inf as NaN. A code has 7 bits and a sign and the scale is a power of two, so a
+// decoded value is exact in f16, bf16 and f32: what a product reads is what the codes stand for.
+#pragma once
+
+#include "common.cuh"
+#include "dequant.cuh"
+#include "errors.cuh"
+#include "gemm_args.cuh"
+
+namespace moss {
+namespace codes {
+
+constexpr int kBlock = 32;
+constexpr int kCodeMax = 127;
+
+// The weight gradient dW[n, k] = sum over rows m of dY[m, n] * X[m, k].
+struct Args {
+  int M, N, K;              // rows, features of dY, columns of X
+  const void* dy;           // few features: [M, N] dense
+  const int8_t* codes;      // few features: [M, K] with pitch ld
+  int64_t ld;
+  const uint8_t* exponents; // [M][ceil(K / 32)]
+  void* out;                // [N, K] dense
+  int out_kind;
+  float* partial;           // splits > 1: f32 [split][part_rows][part_cols]
+  int64_t part_rows, part_cols;
+  int splits, per_split;    // per_split: reduction steps (GEMM) or rows (few features) of a split
+  int tiles_m, tiles_n, group_m;
+  StatusSink status;
+};
+
+constexpr int kFewFeatures = 32;   // features that codes_rows.cu takes
+constexpr int kRowsColumns = 128;  // columns of X that one of its CTAs takes
+constexpr int kRowsMost = 1024;    // rows of one split (its dY rows stay in shared memory)
+constexpr int kStep = 128;         // reduction rows per stage of the GEMM
+
+int launch_decode(const int8_t* codes, int64_t ld, const uint8_t* exponents, int64_t rows, int64_t cols, void* out,
+                  int64_t out_ld, int kind, cudaStream_t stream);
+int launch_gemm(bool pair, int kind, const CUtensorMap& ty, const CUtensorMap& tx, const Args& a, cudaStream_t stream);
+int launch_rows(int kind, const Args& a, cudaStream_t stream);
+
+}  // namespace codes
+}  // namespace moss

@@ -1,0 +1,231 @@
+// Weight gradients of few features (an adapter's first factor) from coded activations:
+//   dW[n, k] = sum over rows m of dY[m, n] * code[m, k] * 2^p[m, k / 32],  n <= 32
+//
+// Bound by the codes, which cross HBM once: a CTA takes 128 columns and a run of rows, whose few values of dY it
+// keeps in shared memory. Its eight warps share the rows, 16 at a time: a lane loads 16 codes of each of four
+// rows (the next ones are on their way meanwhile), pairs them by rows, scales the pairs exactly and feeds them to
+// warp-level MMAs as they lie, column j of every lane forming one 8-column operand, against dY read transposed
+// from shared memory. The tensor work is small; the MMAs spare the CUDA cores the multiply-adds. The warps'
+// sums are added in warp order, the splits' in split order.
+#include <algorithm>
+
+#include "codes_args.cuh"
+
+namespace moss {
+namespace codes {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kWarps = kThreads / 32;
+constexpr int kPitch = 40;  // 16-bit values between rows of dY: eight rows of 16 bytes meet different banks
+constexpr int kSumPitch = kRowsColumns + 8;  // a feature's sums: [16 operands][8 columns], eight features in different banks
+constexpr uint32_t kSumBytes = kFewFeatures * kSumPitch * 4;
+
+__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr));
+}
+template <int K>
+__device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (K == kBF16)
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// The scales of two rows as one pair of 16-bit values. f16 has no 2^p below -24 although code * 2^p may be a value
+// of it: there the scale is two factors, the second of which is 1 for p >= -14.
+struct Scales {
+  uint32_t first, second;
+};
+template <int K>
+__device__ __forceinline__ Scales scales_of(uint32_t e0, uint32_t e1) {
+  Scales s;
+  if constexpr (K == kBF16) {
+    s.first = (e0 << 7) | (e1 << 23);
+    s.second = 0;
+  } else {
+    auto half_pow2 = [](int p) {  // p in [-24, 15]; 16 reads as an infinity
+      return p >= -14 ? static_cast<uint32_t>(p + 15) << 10 : 1u << (p + 24);
+    };
+    const int p0 = static_cast<int>(e0) - 127, p1 = static_cast<int>(e1) - 127;
+    // a block of zero codes may have any small power: what matters is that it is finite
+    s.first = half_pow2(max(-14, min(16, p0))) | (half_pow2(max(-14, min(16, p1))) << 16);
+    s.second = half_pow2(max(-24, min(0, p0 + 14))) | (half_pow2(max(-24, min(0, p1 + 14))) << 16);
+  }
+  return s;
+}
+
+// Codes c and c + 1 of two rows (words w0 and w1) as scaled pairs (row 0, row 1), for columns 2 h and 2 h + 1 of the word.
+template <int K>
+__device__ __forceinline__ void pairs_of(uint32_t w0, uint32_t w1, Scales s, uint32_t (&out)[4]) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const uint32_t both = prmt(w0, w1, h == 0 ? 0x5140u : 0x7362u);
+    if constexpr (K == kBF16) {
+      const __nv_bfloat162 f = *reinterpret_cast<const __nv_bfloat162*>(&s.first);
+      gemm::dequant_word_bf16(both, f, out[2 * h], out[2 * h + 1]);
+    } else {
+      const __half2 f = *reinterpret_cast<const __half2*>(&s.first), g = *reinterpret_cast<const __half2*>(&s.second);
+      gemm::dequant_word_f16(both, f, out[2 * h], out[2 * h + 1]);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        __half2 v = *reinterpret_cast<__half2*>(&out[2 * h + i]);
+        v = __hmul2(v, g);
+        out[2 * h + i] = *reinterpret_cast<uint32_t*>(&v);
+      }
+    }
+  }
+}
+
+// kTiles: 16-feature tiles of dW's rows.
+template <int K, int kTiles>
+__global__ void __launch_bounds__(kThreads, 1) codes_rows_kernel(const Args a) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  float* const sums = reinterpret_cast<float*>(smem);                  // [32][kSumPitch]
+  uint16_t* const dy = reinterpret_cast<uint16_t*>(smem + kSumBytes);  // [rows of the split, whole 16s][kPitch]
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int g = lane >> 2, t = lane & 3;
+  const int split = blockIdx.y, row0 = split * a.per_split;
+  const int rows = min(a.per_split, a.M - row0);
+  const int col = blockIdx.x * kRowsColumns + g * 16;  // this lane's 16 columns
+  const bool wanted = col < a.K;                       // (rows are padded to whole 16s)
+  const int64_t blocks = (a.K + kBlock - 1) / kBlock;
+  struct Held {
+    uint4 codes[4];
+    uint32_t exponent[4];
+  };
+  // rows 2 t, 2 t + 1, 2 t + 8 and 2 t + 9 of the 16 at `at`
+  auto fetch = [&](int at, Held& h) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = at + 2 * t + (i & 1) + (i >> 1) * 8;
+      h.codes[i] = make_uint4(0, 0, 0, 0);
+      h.exponent[i] = 127;
+      if (wanted && r < rows) {
+        const int64_t row = row0 + r;
+        const void* p = a.codes + row * a.ld + col;
+        asm volatile("ld.global.nc.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(h.codes[i].x), "=r"(h.codes[i].y), "=r"(h.codes[i].z), "=r"(h.codes[i].w)
+                     : "l"(p));
+        h.exponent[i] = __ldg(a.exponents + row * blocks + col / kBlock);
+      }
+    }
+  };
+  Held next;
+  fetch(warp * 16, next);
+  // dY's rows, zero past the last row and feature
+  const uint16_t* from = static_cast<const uint16_t*>(a.dy) + static_cast<int64_t>(row0) * a.N;
+  const int whole = (rows + 15) / 16 * 16;
+  if (a.N % 8 == 0 && (reinterpret_cast<uintptr_t>(from) & 15) == 0) {
+    for (int i = threadIdx.x; i < whole * 4; i += kThreads) {
+      const int r = i >> 2, c = (i & 3) * 8;
+      uint4 v = make_uint4(0, 0, 0, 0);
+      if (r < rows && c < a.N) v = __ldg(reinterpret_cast<const uint4*>(from + static_cast<int64_t>(r) * a.N + c));
+      *reinterpret_cast<uint4*>(dy + r * kPitch + c) = v;
+    }
+  } else {
+    for (int i = threadIdx.x; i < whole * kFewFeatures; i += kThreads) {
+      const int r = i / kFewFeatures, c = i % kFewFeatures;
+      dy[r * kPitch + c] = r < rows && c < a.N ? __ldg(from + static_cast<int64_t>(r) * a.N + c) : uint16_t{0};
+    }
+  }
+  __syncthreads();
+
+  float acc[kTiles][16][4];
+#pragma unroll
+  for (int i = 0; i < kTiles; ++i) {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[i][j][e] = 0.0f;
+    }
+  }
+  // 8 x 8 matrices of dY by rows m, transposed on the way: (n 0-7, m 0-7), (n 8-15, m 0-7), (n 0-7, m 8-15), (n 8-15, m 8-15)
+  const uint32_t dy_lane = smem_u32(dy) + (((lane >> 4) * 8 + (lane & 7)) * kPitch + ((lane >> 3) & 1) * 8) * 2;
+  for (int at = warp * 16; at < rows; at += kWarps * 16) {
+    const Held held = next;
+    fetch(at + kWarps * 16, next);
+    uint32_t left[kTiles][4];
+#pragma unroll
+    for (int i = 0; i < kTiles; ++i) ldmatrix_x4_trans(dy_lane + (at * kPitch + i * 16) * 2, left[i]);
+    const Scales s0 = scales_of<K>(held.exponent[0], held.exponent[1]);
+    const Scales s1 = scales_of<K>(held.exponent[2], held.exponent[3]);
+    const uint32_t w[4][4] = {{held.codes[0].x, held.codes[0].y, held.codes[0].z, held.codes[0].w},
+                              {held.codes[1].x, held.codes[1].y, held.codes[1].z, held.codes[1].w},
+                              {held.codes[2].x, held.codes[2].y, held.codes[2].z, held.codes[2].w},
+                              {held.codes[3].x, held.codes[3].y, held.codes[3].z, held.codes[3].w}};
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      uint32_t b0[4], b1[4];
+      pairs_of<K>(w[0][q], w[1][q], s0, b0);
+      pairs_of<K>(w[2][q], w[3][q], s1, b1);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+#pragma unroll
+        for (int i = 0; i < kTiles; ++i) mma_16816<K>(acc[i][4 * q + j], left[i], b0[j], b1[j]);
+      }
+    }
+  }
+
+  // acc[i][j]: features i * 16 + g and + 8, operand columns 2 t and 2 t + 1, which are columns (2 t) * 16 + j and + 16
+  for (int v = 0; v < kWarps; ++v) {
+    __syncthreads();
+    if (warp != v) continue;
+#pragma unroll
+    for (int i = 0; i < kTiles; ++i) {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float2* to = reinterpret_cast<float2*>(sums + (i * 16 + g + h * 8) * kSumPitch + j * 8 + 2 * t);
+          const float2 had = v > 0 ? *to : make_float2(0.0f, 0.0f);
+          *to = make_float2(acc[i][j][2 * h] + had.x, acc[i][j][2 * h + 1] + had.y);
+        }
+      }
+    }
+  }
+  __syncthreads();
+  const int cols = min(kRowsColumns, a.K - static_cast<int>(blockIdx.x) * kRowsColumns);
+  for (int i = threadIdx.x; i < a.N * kRowsColumns; i += kThreads) {
+    const int n = i / kRowsColumns, c = i % kRowsColumns;
+    if (c >= cols) continue;
+    const float v = sums[n * kSumPitch + c % 16 * 8 + c / 16];
+    if (a.splits > 1)
+      a.partial[(split * a.part_rows + n) * a.part_cols + blockIdx.x * kRowsColumns + c] = v;
+    else
+      store_from_float(a.out, a.out_kind, static_cast<int64_t>(n) * a.K + blockIdx.x * kRowsColumns + c, v);
+  }
+}
+
+template <int K, int kTiles>
+int launch_typed(const Args& a, cudaStream_t stream) {
+  auto kern = codes_rows_kernel<K, kTiles>;
+  static DeviceSetup setup;
+  constexpr int kMost = kSumBytes + kRowsMost * kPitch * 2;
+  const int rc = setup("codes_rows_kernel", nullptr, [&](int*) {
+    return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost);
+  });
+  if (rc != MOSS_OK) return rc;
+  const size_t smem = kSumBytes + static_cast<size_t>(a.per_split) * kPitch * 2;
+  kern<<<dim3(static_cast<unsigned>(a.tiles_n), static_cast<unsigned>(a.splits)), kThreads, smem, stream>>>(a);
+  return check_cuda(cudaGetLastError(), "codes_rows_kernel");
+}
+
+}  // namespace
+
+int launch_rows(int kind, const Args& a, cudaStream_t stream) {
+  if (a.splits > 65535) return fail(MOSS_ERR_INVALID_ARGUMENT, "too many rows of coded activations");
+  if (kind == kBF16) return a.N <= 16 ? launch_typed<kBF16, 1>(a, stream) : launch_typed<kBF16, 2>(a, stream);
+  return a.N <= 16 ? launch_typed<kF16, 1>(a, stream) : launch_typed<kF16, 2>(a, stream);
+}
+
+}  // namespace codes
+}  // namespace moss

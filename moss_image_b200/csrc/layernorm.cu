@@ -150,6 +150,18 @@ __device__ __forceinline__ void team_sum(float (&v)[N], float (*red)[kThreads / 
 
 // The gain (or offset) as f32 in shared memory, for all rows of the CTA (in registers it makes the kernels spill).
 __device__ __forceinline__ void stage_gain(float* to, const void* p, int kind, int dim, float absent) {
+  if (p != nullptr && kind != kF32 && dim % 8 == 0 && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
+    for (int i = threadIdx.x * 8; i < dim; i += kThreads * 8) {
+      float v[8];
+      if (kind == kBF16)
+        load8<kBF16>(p, i, 8, true, v);
+      else
+        load8<kF16>(p, i, 8, true, v);
+      *reinterpret_cast<float4*>(to + i) = make_float4(v[0], v[1], v[2], v[3]);
+      *reinterpret_cast<float4*>(to + i + 4) = make_float4(v[4], v[5], v[6], v[7]);
+    }
+    return;
+  }
   for (int i = threadIdx.x; i < dim; i += kThreads) to[i] = p == nullptr ? absent : load_as_float(p, kind, i);
 }
 template <int V>
@@ -175,7 +187,9 @@ __global__ void __launch_bounds__(kThreads) layernorm_fwd_kernel(const Args a) {
   const int thread = threadIdx.x % T;
   const int64_t step = static_cast<int64_t>(gridDim.x) * (kThreads / T);
   const float inv_dim = 1.0f / static_cast<float>(a.dim);
-  int64_t row = static_cast<int64_t>(blockIdx.x) * (kThreads / T) + threadIdx.x / T;
+  // few rows are spread over the CTAs first
+  int64_t row = T < 32 ? static_cast<int64_t>(blockIdx.x) * (kThreads / T) + threadIdx.x / T
+                       : blockIdx.x + static_cast<int64_t>(threadIdx.x / T) * gridDim.x;
   // a warp's teams take their shuffles together: rows past the end are computed on zeros and not stored
   const int64_t last = T < 32 ? (a.rows + 32 / T - 1) / (32 / T) * (32 / T) : a.rows;
   Raw<KX, V> next[C];
@@ -239,18 +253,95 @@ __global__ void __launch_bounds__(kThreads) layernorm_fwd_kernel(const Args a) {
   }
 }
 
-// kGain: the sums for dw and db are wanted (64 registers a thread, and a reduction at the end).
+// A thread's own values of a row that is on its way, in shared memory: pieces of at most 16 bytes, a piece of the
+// CTA's threads side by side. Written and read by the same thread, so no barrier is needed.
+template <int K, int V, int C>
+struct Staged {
+  static constexpr int kBytes = Raw<K, V>::kBytes;
+  static constexpr int kPiece = kBytes < 4 ? 4 : kBytes < 16 ? kBytes : 16;
+  static constexpr int kPieces = kBytes <= 16 ? 1 : kBytes / 16;
+  static constexpr uint32_t kRow = static_cast<uint32_t>(C) * kPieces * kThreads * kPiece;  // of all threads
+  __device__ __forceinline__ static uint32_t at(int i, int piece) {
+    return static_cast<uint32_t>(((i * kPieces + piece) * kThreads + threadIdx.x) * kPiece);
+  }
+  __device__ __forceinline__ static void copy(uint8_t* stage, int i, const void* p, int64_t from) {
+    const char* src = static_cast<const char*>(p) + from * (K == kF32 ? 4 : 2);
+#pragma unroll
+    for (int c = 0; c < kPieces; ++c) {
+      if constexpr (kBytes >= 16) {
+        cp_async16(smem_u32(stage + at(i, c)), src + 16 * c);
+      } else if constexpr (kBytes >= 4) {
+        asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(smem_u32(stage + at(i, 0))), "l"(src), "n"(kBytes) : "memory");
+      } else {  // two bytes: too few for an asynchronous copy
+        *reinterpret_cast<uint16_t*>(stage + at(i, 0)) = __ldg(reinterpret_cast<const uint16_t*>(src));
+      }
+    }
+  }
+  __device__ __forceinline__ static void read(const uint8_t* stage, int i, float (&f)[V]) {
+    Raw<K, V> r;
+    if constexpr (kBytes >= 16) {
+#pragma unroll
+      for (int c = 0; c < kPieces; ++c) {
+        const uint4 u = *reinterpret_cast<const uint4*>(stage + at(i, c));
+        r.w[4 * c] = u.x;
+        r.w[4 * c + 1] = u.y;
+        r.w[4 * c + 2] = u.z;
+        r.w[4 * c + 3] = u.w;
+      }
+    } else if constexpr (kBytes == 8) {
+      const uint2 u = *reinterpret_cast<const uint2*>(stage + at(i, 0));
+      r.w[0] = u.x;
+      r.w[1] = u.y;
+    } else if constexpr (kBytes == 4) {
+      r.w[0] = *reinterpret_cast<const uint32_t*>(stage + at(i, 0));
+    } else {
+      r.w[0] = *reinterpret_cast<const uint16_t*>(stage + at(i, 0));
+    }
+    widen<K, V>(r, f);
+  }
+};
+template <int KX, int KY, int V, int C>
+constexpr uint32_t stage_bytes() { return Staged<KX, V, C>::kRow + Staged<KY, V, C>::kRow; }
+
+// kGain: the sums for dw and db are wanted (up to 64 registers a thread, and a reduction at the end). The rows that a
+// team takes next are on their way, `stages` at a time (without them a team waits for every row: 9216 x 3072
+// took 60 us, 1.5 times as long).
 template <int KX, int KY, int T, int V, int C, bool kGain>
-__global__ void __launch_bounds__(kThreads) layernorm_bwd_kernel(const Args a) {
-  extern __shared__ __align__(16) float gain[];         // w, padded to 4 values
-  float* const joined = gain + (a.dim + 3) / 4 * 4;     // [2][dim], where a CTA has several teams
+__global__ void __launch_bounds__(kThreads) layernorm_bwd_kernel(const Args a, int stages) {
+  extern __shared__ __align__(16) float gain[];  // w, padded to 4 values; then the stages, and [2][dim] joined sums in their place
+  uint8_t* const ring = reinterpret_cast<uint8_t*>(gain + (a.dim + 3) / 4 * 4);
+  float* const joined = reinterpret_cast<float*>(ring);
   __shared__ float red[2][kThreads / 32][2];
+  using SX = Staged<KX, V, C>;
+  using SY = Staged<KY, V, C>;
+  constexpr uint32_t kStage = stage_bytes<KX, KY, V, C>();
   int slot = 0;
   const int thread = threadIdx.x % T;
   const int team = threadIdx.x / T;
   const int64_t step = static_cast<int64_t>(gridDim.x) * (kThreads / T);
   const float inv_dim = 1.0f / static_cast<float>(a.dim);
   const int64_t last = T < 32 ? (a.rows + 32 / T - 1) / (32 / T) * (32 / T) : a.rows;
+  const int64_t first = T < 32 ? static_cast<int64_t>(blockIdx.x) * (kThreads / T) + team : blockIdx.x + static_cast<int64_t>(team) * gridDim.x;
+  auto fetch = [&](int64_t row, int stage) {
+    if (row < a.rows) {
+      uint8_t* to = ring + stage * kStage;
+#pragma unroll
+      for (int i = 0; i < C; ++i) {
+        const int at = (thread + i * T) * V;
+        if (at >= a.dim) continue;
+        SX::copy(to, i, a.x, row * a.dim + at);
+        SY::copy(to + SX::kRow, i, a.dy, row * a.dim + at);
+      }
+    }
+    cp_async_commit();
+  };
+  // two groups are always under way, so that the wait's count is the same for any number of stages
+  for (int k = 0; k < 2; ++k) {
+    if (k < stages - 1)
+      fetch(first + k * step, k);
+    else
+      cp_async_commit();
+  }
   stage_gain(gain, a.w, a.g_kind, a.dim, 1.0f);
   __syncthreads();
   float dw[C][V], db[C][V];
@@ -259,27 +350,28 @@ __global__ void __launch_bounds__(kThreads) layernorm_bwd_kernel(const Args a) {
 #pragma unroll
     for (int j = 0; j < V; ++j) dw[i][j] = db[i][j] = 0.0f;
   }
-  for (int64_t row = static_cast<int64_t>(blockIdx.x) * (kThreads / T) + team; row < last; row += step) {
+  int stage = 0;
+  for (int64_t row = first; row < last; row += step) {
     const bool live = row < a.rows;
     const float2 stats = live ? __ldg(a.stats + row) : make_float2(0.0f, 0.0f);
-    Raw<KX, V> hx[C];
-    Raw<KY, V> hd[C];
-#pragma unroll
-    for (int i = 0; i < C; ++i) {
-      const int at = (thread + i * T) * V;
-      if (live && at < a.dim) {
-        hx[i] = load<KX, V>(a.x, row * a.dim + at);
-        hd[i] = load<KY, V>(a.dy, row * a.dim + at);
-      }
-    }
+    const int ahead = stage == 0 ? stages - 1 : stage - 1;  // the slot that the row before has left
+    fetch(row + (stages - 1) * step, ahead);
+    if (stages == 3)
+      cp_async_wait<2>();
+    else if (stages == 2)
+      cp_async_wait<1>();
+    else
+      cp_async_wait<0>();
+    const uint8_t* held = ring + stage * kStage;
+    if (++stage == stages) stage = 0;
     float sums[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int i = 0; i < C; ++i) {
       const int at = (thread + i * T) * V;
       if (!live || at >= a.dim) continue;
       float x[V], d[V], w[V];
-      widen<KX, V>(hx[i], x);
-      widen<KY, V>(hd[i], d);
+      SX::read(held, i, x);
+      SY::read(held + SX::kRow, i, d);
       gain_at<V>(gain, at, w);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
@@ -293,16 +385,15 @@ __global__ void __launch_bounds__(kThreads) layernorm_bwd_kernel(const Args a) {
       }
     }
     team_sum<T, 2>(sums, red, slot);
-    if (!live) continue;
+    if (!live || a.out == nullptr) continue;
     const float s0 = sums[0] * inv_dim, s1 = sums[1] * inv_dim;
-    if (a.out == nullptr) continue;
 #pragma unroll
     for (int i = 0; i < C; ++i) {
       const int at = (thread + i * T) * V;
       if (at >= a.dim) continue;
       float x[V], d[V], w[V];
-      widen<KX, V>(hx[i], x);
-      widen<KY, V>(hd[i], d);
+      SX::read(held, i, x);
+      SY::read(held + SX::kRow, i, d);
       gain_at<V>(gain, at, w);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
@@ -312,6 +403,8 @@ __global__ void __launch_bounds__(kThreads) layernorm_bwd_kernel(const Args a) {
       store<KX, V>(a.out, row * a.dim + at, x);
     }
   }
+  cp_async_wait<0>();
+  __syncthreads();
   if constexpr (kGain) {
     float* mine = a.partial + static_cast<int64_t>(blockIdx.x) * 2 * a.dim;
     if constexpr (T == kThreads) {
@@ -390,20 +483,21 @@ int team_of(int64_t dim, int v) {
   return dim <= 32 * held ? 32 : dim <= 128 * held ? 128 : 512;
 }
 
-// CTAs: each multiprocessor's resident ones (one of the backward pass: its partial sums are then few), no more than rows ask for.
+// CTAs: each multiprocessor's resident ones (one of the backward pass: its partial sums are then few), no more than
+// there are rows (teams of several rows a warp: than fill them).
 int ctas_of(int64_t rows, int team, int per_sm) {
-  const int64_t asked = ceil_div(rows, kThreads / team);
+  const int64_t asked = team < 32 ? ceil_div(rows, kThreads / team) : rows;
   return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(asked, static_cast<int64_t>(per_sm) * device_sm_count())));
 }
 
-template <int T, typename F>
-int launch_kernel(const char* what, F* kern, int ctas, size_t smem, const Args& a, cudaStream_t stream) {
-  if constexpr (T == kThreads) {  // wide rows: more shared memory than a kernel has unasked
-    const cudaError_t e = smem > 40 * 1024 ? cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem))
-                                           : cudaSuccess;
+template <typename F, typename... More>
+int launch_kernel(const char* what, F* kern, int ctas, size_t smem, const Args& a, cudaStream_t stream, More... more) {
+  // past what a kernel has unasked (with room for its fixed arrays)
+  if (smem > 40 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
     if (e != cudaSuccess) return check_cuda(e, what);
   }
-  kern<<<ctas, kThreads, smem, stream>>>(a);
+  kern<<<ctas, kThreads, smem, stream>>>(a, more...);
   return check_cuda(cudaGetLastError(), what);
 }
 
@@ -411,11 +505,16 @@ template <int KX, int KY, int T, int V, int C>
 int launch(bool backward, const Args& a, cudaStream_t stream) {
   const size_t gain = static_cast<size_t>(a.dim + 3) / 4 * 4 * sizeof(float);
   if (!backward)
-    return launch_kernel<T>("layernorm_fwd_kernel", layernorm_fwd_kernel<KX, KY, T, V, C>, ctas_of(a.rows, T, 2), 2 * gain, a, stream);
-  if (a.partial == nullptr)
-    return launch_kernel<T>("layernorm_bwd_kernel", layernorm_bwd_kernel<KX, KY, T, V, C, false>, ctas_of(a.rows, T, 2), gain, a, stream);
-  const size_t joined = T == kThreads ? 0 : 2 * sizeof(float) * a.dim;
-  return launch_kernel<T>("layernorm_bwd_kernel", layernorm_bwd_kernel<KX, KY, T, V, C, true>, ctas_of(a.rows, T, 1), gain + joined, a, stream);
+    return launch_kernel("layernorm_fwd_kernel", layernorm_fwd_kernel<KX, KY, T, V, C>, ctas_of(a.rows, T, 2), 2 * gain, a, stream);
+  // the stages that fit one CTA a multiprocessor: three, two (f32 rows), or one (f32 rows past 8192 values)
+  constexpr size_t kStage = stage_bytes<KX, KY, V, C>(), kRoom = 226 * 1024;
+  const int stages = static_cast<int>(std::max<size_t>(1, std::min<size_t>(3, (kRoom - gain) / kStage)));
+  const size_t joined = a.partial == nullptr || T == kThreads ? 0 : 2 * sizeof(float) * a.dim;
+  const size_t smem = gain + std::max(stages * kStage, joined);
+  auto run = [&](auto kern) {
+    return launch_kernel("layernorm_bwd_kernel", kern, ctas_of(a.rows, T, 1), smem, a, stream, stages);
+  };
+  return a.partial == nullptr ? run(layernorm_bwd_kernel<KX, KY, T, V, C, false>) : run(layernorm_bwd_kernel<KX, KY, T, V, C, true>);
 }
 
 template <int KX, int KY>
@@ -446,7 +545,7 @@ int launch_typed(bool backward, int x_kind, int y_kind, const Args& a, cudaStrea
 // The type of y: torch's promotion of x and the gain.
 int result_kind(int x, int g, bool gain) { return !gain || x == g ? x : kF32; }
 
-// Rows of partial sums that a backward pass may write: those of its narrowest vectors' teams are at most as many.
+// Rows of partial sums that a backward pass may write: narrow vectors' teams are as large or larger, so as many or more.
 int most_parts(int64_t rows, int64_t dim) { return ctas_of(rows, team_of(dim, 1), 1); }
 
 int check(int64_t rows, int64_t dim, int x_dtype, int g_dtype, bool gain) {

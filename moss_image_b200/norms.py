@@ -139,11 +139,18 @@ class _LayerNorm(torch.autograd.Function):
         return out
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, grad):
-        tokens, weight, bias, stats = ctx.saved_tensors
-        _lib.refuse_forward_mode("layer_norm", grad)
-        return (*_layer_norm_backward(grad, tokens, weight, bias, stats, ctx.needs_input_grad), None)
+        # (the guard against second derivatives costs microseconds, and is needed where a graph is recorded)
+        return _layer_norm_gradients_once(ctx, grad) if torch.is_grad_enabled() else _layer_norm_gradients(ctx, grad)
+
+
+def _layer_norm_gradients(ctx, grad):
+    tokens, weight, bias, stats = ctx.saved_tensors
+    _lib.refuse_forward_mode("layer_norm", grad)
+    return (*_layer_norm_backward(grad, tokens, weight, bias, stats, ctx.needs_input_grad), None)
+
+
+_layer_norm_gradients_once = once_differentiable(_layer_norm_gradients)
 
 
 def layer_norm(tokens: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None,
