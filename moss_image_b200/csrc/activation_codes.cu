@@ -103,20 +103,22 @@ __global__ void __launch_bounds__(kThreads) encode_wide_kernel(const void* __res
 // A warp takes kEach blocks at a time, a lane a column; codes from the row's end to its pitch are zero.
 constexpr int kEach = 4;
 template <int K>
-__global__ void __launch_bounds__(kThreads) encode_lane_kernel(const void* __restrict__ x, int64_t units, int64_t cols,
+__global__ void __launch_bounds__(kThreads) encode_lane_kernel(const void* __restrict__ x, uint32_t units, int64_t cols,
                                                                uint32_t blocks, int cap, int8_t* codes, int64_t ld,
                                                                uint8_t* exponents) {
   const int lane = threadIdx.x & 31;
-  const int64_t first = (static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5)) * kEach;
+  const uint32_t first = (blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5)) * kEach;
   float v[kEach];
 #pragma unroll
   for (int e = 0; e < kEach; ++e) {
-    const int64_t unit = first + e, row = unit / blocks, c = (unit - row * blocks) * kBlock + lane;
+    const uint32_t unit = first + e, at = unit / blocks;
+    const int64_t row = at, c = (unit - at * blocks) * kBlock + lane;
     v[e] = unit < units && c < cols ? load_as_float(x, K, row * cols + c) : 0.0f;
   }
 #pragma unroll
   for (int e = 0; e < kEach; ++e) {
-    const int64_t unit = first + e, row = unit / blocks, c = (unit - row * blocks) * kBlock + lane;
+    const uint32_t unit = first + e, at = unit / blocks;
+    const int64_t row = at, c = (unit - at * blocks) * kBlock + lane;
     if (unit >= units) break;
     float amax = fabsf(v[e]);
 #pragma unroll
@@ -171,19 +173,21 @@ __global__ void __launch_bounds__(kThreads) decode_wide_kernel(const int8_t* __r
 
 template <int K>
 __global__ void __launch_bounds__(kThreads) decode_lane_kernel(const int8_t* __restrict__ codes, int64_t ld,
-                                                               const uint8_t* __restrict__ exponents, int64_t units,
+                                                               const uint8_t* __restrict__ exponents, uint32_t units,
                                                                int64_t cols, uint32_t blocks, void* out, int64_t out_ld) {
   const int lane = threadIdx.x & 31;
-  const int64_t first = (static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5)) * kEach;
+  const uint32_t first = (blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5)) * kEach;
   float v[kEach];
 #pragma unroll
   for (int e = 0; e < kEach; ++e) {
-    const int64_t unit = first + e, row = unit / blocks, c = (unit - row * blocks) * kBlock + lane;
+    const uint32_t unit = first + e, at = unit / blocks;
+    const int64_t row = at, c = (unit - at * blocks) * kBlock + lane;
     v[e] = unit < units && c < cols ? static_cast<float>(codes[row * ld + c]) * scale_of(__ldg(exponents + unit)) : 0.0f;
   }
 #pragma unroll
   for (int e = 0; e < kEach; ++e) {
-    const int64_t unit = first + e, row = unit / blocks, c = (unit - row * blocks) * kBlock + lane;
+    const uint32_t unit = first + e, at = unit / blocks;
+    const int64_t row = at, c = (unit - at * blocks) * kBlock + lane;
     if (unit < units && c < cols) store_from_float(out, K, row * out_ld + c, v[e]);
   }
 }
@@ -215,7 +219,8 @@ bool aligned(const void* p, uintptr_t to) { return reinterpret_cast<uintptr_t>(p
 
 int check_rows(int64_t rows, int64_t cols) {
   if (rows < 0 || cols < 0) return fail(MOSS_ERR_INVALID_ARGUMENT, "negative shape of coded activations");
-  if (cols > INT32_MAX - 256 || (cols > 0 && rows > (int64_t{1} << 36) / cols))
+  // (blocks and halves of blocks are counted in 32 bits)
+  if (cols > INT32_MAX - 256 || (cols > 0 && rows > ((int64_t{1} << 32) - 4096) / ceil_div(cols, 16)))
     return fail(MOSS_ERR_INVALID_ARGUMENT, "coded activations of %lld x %lld values are too large",
                 static_cast<long long>(rows), static_cast<long long>(cols));
   return MOSS_OK;
@@ -242,9 +247,8 @@ int encode(const void* x, int kind, int64_t rows, int64_t cols, int8_t* codes, i
       encode_wide_kernel<kF32><<<grid, kThreads, 0, stream>>>(x, units, chunks, cap, codes, exponents);
   } else {
     const uint32_t blocks = static_cast<uint32_t>(ceil_div(cols, kBlock));
-    const int64_t units = rows * blocks;
-    const int64_t grid = ceil_div(units, kThreads / 32 * kEach);
-    if (grid > INT32_MAX) return fail(MOSS_ERR_INVALID_ARGUMENT, "too many blocks of coded activations");
+    const uint32_t units = static_cast<uint32_t>(rows * blocks);
+    const int64_t grid = ceil_div(rows * blocks, kThreads / 32 * kEach);
     if (kind == kF16)
       encode_lane_kernel<kF16><<<static_cast<unsigned>(grid), kThreads, 0, stream>>>(x, units, cols, blocks, cap, codes, ld, exponents);
     else if (kind == kBF16)
@@ -265,9 +269,8 @@ int decode_typed(const int8_t* codes, int64_t ld, const uint8_t* exponents, int6
   } else {
     const uint32_t blocks = static_cast<uint32_t>(ceil_div(cols, kBlock));
     const int64_t grid = ceil_div(rows * blocks, kThreads / 32 * kEach);
-    if (grid > INT32_MAX) return fail(MOSS_ERR_INVALID_ARGUMENT, "too many blocks of coded activations");
-    decode_lane_kernel<K><<<static_cast<unsigned>(grid), kThreads, 0, stream>>>(codes, ld, exponents, rows * blocks, cols,
-                                                                                blocks, out, out_ld);
+    decode_lane_kernel<K><<<static_cast<unsigned>(grid), kThreads, 0, stream>>>(codes, ld, exponents, static_cast<uint32_t>(rows * blocks),
+                                                                                cols, blocks, out, out_ld);
   }
   return check_cuda(cudaGetLastError(), "decode kernel");
 }

@@ -36,7 +36,7 @@ struct Args {
 
 constexpr int kFewFeatures = 32;   // features that codes_rows.cu takes
 constexpr int kRowsColumns = 128;  // columns of X that one of its CTAs takes
-constexpr int kRowsMost = 1024;    // rows of one split (its dY rows stay in shared memory)
+constexpr int kRowsMost = 2048;    // rows of one split (its dY rows stay in shared memory)
 constexpr int kStep = 128;         // reduction rows per stage of the GEMM
 
 int launch_decode(const int8_t* codes, int64_t ld, const uint8_t* exponents, int64_t rows, int64_t cols, void* out,

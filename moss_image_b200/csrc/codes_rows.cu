@@ -2,10 +2,10 @@
 //   dW[n, k] = sum over rows m of dY[m, n] * code[m, k] * 2^p[m, k / 32],  n <= 32
 //
 // Bound by the codes, which cross HBM once: a CTA takes 128 columns and a run of rows, whose few values of dY it
-// keeps in shared memory. Its eight warps share the rows, 16 at a time: a lane loads 16 codes of each of four
-// rows (the next ones are on their way meanwhile), pairs them by rows, scales the pairs exactly and feeds them to
-// warp-level MMAs as they lie, column j of every lane forming one 8-column operand, against dY read transposed
-// from shared memory. The tensor work is small; the MMAs spare the CUDA cores the multiply-adds. The warps'
+// keeps in shared memory. Two times eight warps share the columns and the rows, 16 at a time: a lane loads 8 codes of
+// each of four rows (the next two sixteens are on their way meanwhile), pairs them by rows, scales the pairs exactly
+// and feeds them to warp-level MMAs as they lie, column j of every lane forming one 8-column operand, against dY
+// read transposed from shared memory. The tensor work is small; the MMAs spare the CUDA cores the multiply-adds. The warps'
 // sums are added in warp order, the splits' in split order.
 #include <algorithm>
 
@@ -15,8 +15,10 @@ namespace moss {
 namespace codes {
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kWarps = kThreads / 32;
+constexpr int kThreads = 512;
+constexpr int kRowWarps = 8;               // warps that share the rows of 64 columns
+constexpr int kEach = kRowsColumns / 2 / 8;  // columns of one lane
+static_assert(kThreads == 2 * kRowWarps * 32 && kEach == 8, "two column halves, eight codes a load");
 constexpr int kPitch = 40;  // 16-bit values between rows of dY: eight rows of 16 bytes meet different banks
 constexpr int kSumPitch = kRowsColumns + 8;  // a feature's sums: [16 operands][8 columns], eight features in different banks
 constexpr uint32_t kSumBytes = kFewFeatures * kSumPitch * 4;
@@ -93,34 +95,36 @@ __global__ void __launch_bounds__(kThreads, 1) codes_rows_kernel(const Args a) {
   uint16_t* const dy = reinterpret_cast<uint16_t*>(smem + kSumBytes);  // [rows of the split, whole 16s][kPitch]
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, t = lane & 3;
+  const int row_warp = warp & (kRowWarps - 1), half = warp / kRowWarps;
   const int split = blockIdx.y, row0 = split * a.per_split;
   const int rows = min(a.per_split, a.M - row0);
-  const int col = blockIdx.x * kRowsColumns + g * 16;  // this lane's 16 columns
-  const bool wanted = col < a.K;                       // (rows are padded to whole 16s)
+  const int col = blockIdx.x * kRowsColumns + (half * 8 + g) * kEach;  // this lane's columns
+  const bool wanted = col < a.K;                                       // (rows are padded to whole 16s)
   const int64_t blocks = (a.K + kBlock - 1) / kBlock;
   struct Held {
-    uint4 codes[4];
+    uint2 codes[4];
     uint32_t exponent[4];
   };
   // rows 2 t, 2 t + 1, 2 t + 8 and 2 t + 9 of the 16 at `at`
+  const int8_t* const code_from = a.codes + static_cast<int64_t>(row0) * a.ld + col;
+  const uint8_t* const exponent_from = a.exponents + row0 * blocks + col / kBlock;
   auto fetch = [&](int at, Held& h) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int r = at + 2 * t + (i & 1) + (i >> 1) * 8;
-      h.codes[i] = make_uint4(0, 0, 0, 0);
+      h.codes[i] = make_uint2(0, 0);
       h.exponent[i] = 127;
       if (wanted && r < rows) {
-        const int64_t row = row0 + r;
-        const void* p = a.codes + row * a.ld + col;
-        asm volatile("ld.global.nc.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];"
-                     : "=r"(h.codes[i].x), "=r"(h.codes[i].y), "=r"(h.codes[i].z), "=r"(h.codes[i].w)
-                     : "l"(p));
-        h.exponent[i] = __ldg(a.exponents + row * blocks + col / kBlock);
+        asm volatile("ld.global.nc.L1::no_allocate.v2.b32 {%0, %1}, [%2];"
+                     : "=r"(h.codes[i].x), "=r"(h.codes[i].y)
+                     : "l"(code_from + r * a.ld));
+        h.exponent[i] = __ldg(exponent_from + r * blocks);
       }
     }
   };
-  Held next;
-  fetch(warp * 16, next);
+  Held next[2];
+  fetch(row_warp * 16, next[0]);
+  fetch((row_warp + kRowWarps) * 16, next[1]);
   // dY's rows, zero past the last row and feature
   const uint16_t* from = static_cast<const uint16_t*>(a.dy) + static_cast<int64_t>(row0) * a.N;
   const int whole = (rows + 15) / 16 * 16;
@@ -139,53 +143,53 @@ __global__ void __launch_bounds__(kThreads, 1) codes_rows_kernel(const Args a) {
   }
   __syncthreads();
 
-  float acc[kTiles][16][4];
+  float acc[kTiles][kEach][4];
 #pragma unroll
   for (int i = 0; i < kTiles; ++i) {
 #pragma unroll
-    for (int j = 0; j < 16; ++j) {
+    for (int j = 0; j < kEach; ++j) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) acc[i][j][e] = 0.0f;
     }
   }
   // 8 x 8 matrices of dY by rows m, transposed on the way: (n 0-7, m 0-7), (n 8-15, m 0-7), (n 0-7, m 8-15), (n 8-15, m 8-15)
   const uint32_t dy_lane = smem_u32(dy) + (((lane >> 4) * 8 + (lane & 7)) * kPitch + ((lane >> 3) & 1) * 8) * 2;
-  for (int at = warp * 16; at < rows; at += kWarps * 16) {
-    const Held held = next;
-    fetch(at + kWarps * 16, next);
+  auto take = [&](int at, Held& slot) {
+    const Held held = slot;
+    fetch(at + 2 * kRowWarps * 16, slot);
     uint32_t left[kTiles][4];
 #pragma unroll
     for (int i = 0; i < kTiles; ++i) ldmatrix_x4_trans(dy_lane + (at * kPitch + i * 16) * 2, left[i]);
     const Scales s0 = scales_of<K>(held.exponent[0], held.exponent[1]);
     const Scales s1 = scales_of<K>(held.exponent[2], held.exponent[3]);
-    const uint32_t w[4][4] = {{held.codes[0].x, held.codes[0].y, held.codes[0].z, held.codes[0].w},
-                              {held.codes[1].x, held.codes[1].y, held.codes[1].z, held.codes[1].w},
-                              {held.codes[2].x, held.codes[2].y, held.codes[2].z, held.codes[2].w},
-                              {held.codes[3].x, held.codes[3].y, held.codes[3].z, held.codes[3].w}};
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
+    for (int q = 0; q < 2; ++q) {
       uint32_t b0[4], b1[4];
-      pairs_of<K>(w[0][q], w[1][q], s0, b0);
-      pairs_of<K>(w[2][q], w[3][q], s1, b1);
+      pairs_of<K>(q == 0 ? held.codes[0].x : held.codes[0].y, q == 0 ? held.codes[1].x : held.codes[1].y, s0, b0);
+      pairs_of<K>(q == 0 ? held.codes[2].x : held.codes[2].y, q == 0 ? held.codes[3].x : held.codes[3].y, s1, b1);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
 #pragma unroll
         for (int i = 0; i < kTiles; ++i) mma_16816<K>(acc[i][4 * q + j], left[i], b0[j], b1[j]);
       }
     }
+  };
+  for (int at = row_warp * 16; at < rows; at += 2 * kRowWarps * 16) {
+    take(at, next[0]);
+    if (at + kRowWarps * 16 < rows) take(at + kRowWarps * 16, next[1]);
   }
 
-  // acc[i][j]: features i * 16 + g and + 8, operand columns 2 t and 2 t + 1, which are columns (2 t) * 16 + j and + 16
-  for (int v = 0; v < kWarps; ++v) {
+  // acc[i][j]: features i * 16 + g and + 8, operand columns 2 t and 2 t + 1, which are columns (2 t) * 8 + j and + 8 of the half
+  for (int v = 0; v < kRowWarps; ++v) {
     __syncthreads();
-    if (warp != v) continue;
+    if (row_warp != v) continue;
 #pragma unroll
     for (int i = 0; i < kTiles; ++i) {
 #pragma unroll
-      for (int j = 0; j < 16; ++j) {
+      for (int j = 0; j < kEach; ++j) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          float2* to = reinterpret_cast<float2*>(sums + (i * 16 + g + h * 8) * kSumPitch + j * 8 + 2 * t);
+          float2* to = reinterpret_cast<float2*>(sums + (i * 16 + g + h * 8) * kSumPitch + (half * kEach + j) * 8 + 2 * t);
           const float2 had = v > 0 ? *to : make_float2(0.0f, 0.0f);
           *to = make_float2(acc[i][j][2 * h] + had.x, acc[i][j][2 * h + 1] + had.y);
         }
@@ -197,7 +201,7 @@ __global__ void __launch_bounds__(kThreads, 1) codes_rows_kernel(const Args a) {
   for (int i = threadIdx.x; i < a.N * kRowsColumns; i += kThreads) {
     const int n = i / kRowsColumns, c = i % kRowsColumns;
     if (c >= cols) continue;
-    const float v = sums[n * kSumPitch + c % 16 * 8 + c / 16];
+    const float v = sums[n * kSumPitch + (c / 64 * kEach + c % kEach) * 8 + c % 64 / kEach];
     if (a.splits > 1)
       a.partial[(split * a.part_rows + n) * a.part_cols + blockIdx.x * kRowsColumns + c] = v;
     else
