@@ -288,6 +288,36 @@ MOSS_API int moss_layernorm_bwd(const void* dy, const void* x, int x_dtype, int6
                        void* workspace, size_t workspace_bytes, moss_stream_t stream);
 
 /*
+ * Attention to another sequence: out = softmax(scale Q K^T) V by heads, f16 or bf16, head_dim a multiple of 8 up to 128,
+ * query head h with key head h / (q_heads / k_heads). Batch entries of q_tokens and k_tokens rows (strides in values of
+ * batch, token and head; heads dense, rows on 16 bytes), or, with both offsets (device, int64 [batch + 1], from 0), packed
+ * rows of `batch` sequences: q_tokens and k_tokens are then the streams' lengths, batch strides are not read, and rows
+ * behind the last sequence give zeros. mask (batch entries only, may be null): bytes [batch][mask_ld], non-zero where a key may
+ * be looked at; what lies in other keys is never read into a result. A query without keys gives zeros. scale > 0.
+ * out: dense [rows][q_heads][head_dim]. lse (may be null): f32 [q_heads][rows], log2 of each row's sum of 2^logit, an
+ * infinity for a query without keys; the backward pass reads it.
+ * `workspace`: at least moss_cross_attention_workspace_bytes(..) bytes, 256-byte aligned, free for reuse once
+ * the stream has passed the call. Results do not depend on timing.
+ */
+MOSS_API int moss_cross_attention_workspace_bytes(int64_t batch, int64_t q_tokens, int64_t k_tokens, int64_t q_heads,
+                       int64_t k_heads, int64_t head_dim, int packed, int backward, size_t* bytes);
+MOSS_API int moss_cross_attention_fwd(const void* q, int64_t q_batch, int64_t q_token, int64_t q_head, const void* k,
+                       int64_t k_batch, int64_t k_token, int64_t k_head, const void* v, int64_t v_batch, int64_t v_token,
+                       int64_t v_head, int dtype, int64_t batch, int64_t q_tokens, int64_t k_tokens, int64_t q_heads,
+                       int64_t k_heads, int64_t head_dim, const int64_t* q_offsets, const int64_t* k_offsets,
+                       const uint8_t* mask, int64_t mask_ld, float scale, void* out, float* lse, void* workspace,
+                       size_t workspace_bytes, int* status, moss_stream_t stream);
+/* The gradients, dense, of the same arguments with the forward's out and lse; grad and out dense, on 16 bytes. dk and dv may
+ * both be null (dq is always computed: what the others need comes from its pass). */
+MOSS_API int moss_cross_attention_bwd(const void* grad, const void* q, int64_t q_batch, int64_t q_token, int64_t q_head,
+                       const void* k, int64_t k_batch, int64_t k_token, int64_t k_head, const void* v, int64_t v_batch,
+                       int64_t v_token, int64_t v_head, int dtype, int64_t batch, int64_t q_tokens, int64_t k_tokens,
+                       int64_t q_heads, int64_t k_heads, int64_t head_dim, const int64_t* q_offsets,
+                       const int64_t* k_offsets, const uint8_t* mask, int64_t mask_ld, float scale, const void* out,
+                       const float* lse, void* dq, void* dk, void* dv, void* workspace, size_t workspace_bytes, int* status,
+                       moss_stream_t stream);
+
+/*
  * Activations as 8-bit codes: int8 codes in [-127, 127] and one power of two for each block of 32 columns of a row, the
  * least 2^p with max|x| <= 127 * 2^p, p in [-126, 9] for f16 and [-126, 121] otherwise; codes x / 2^p rounded to
  * nearest even. exponents[rows][ceil(cols / 32)] holds p + 127, or 255 for a block with an infinity or NaN

@@ -78,6 +78,12 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "moss_coded_gradient_workspace_bytes": (_i32, [_i64, _i64, _i64, ctypes.POINTER(_sz)]),
     "moss_coded_gradient": (
         _i32, [_vp, _i32, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _i32, _vp, _sz, _vp, _vp]),
+    "moss_cross_attention_workspace_bytes": (_i32, [_i64] * 6 + [_i32, _i32, ctypes.POINTER(_sz)]),
+    "moss_cross_attention_fwd": (
+        _i32, [_vp, _i64, _i64, _i64] * 3 + [_i32] + [_i64] * 6 + [_vp, _vp, _vp, _i64, _f32, _vp, _vp, _vp, _sz, _vp, _vp]),
+    "moss_cross_attention_bwd": (
+        _i32, [_vp] + [_vp, _i64, _i64, _i64] * 3 + [_i32] + [_i64] * 6
+        + [_vp, _vp, _vp, _i64, _f32, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp, _vp]),
     "moss_fp8_linear_workspace_bytes": (_i32, [_i64, _i64, _i64, ctypes.POINTER(_sz)]),
     "moss_fp8_linear_fwd": (
         _i32, [_vp, _i32, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _i32, _vp, _i32, _vp, _sz, _vp, _vp]),

@@ -1,0 +1,307 @@
+// Shared declarations of the attention to another sequence (cross_forward.cu, cross_backward.cu, cross_attention.cu).
+//
+// For each sequence s and query head h, with key head h / group and the keys that are allowed:
+//   S = Q K^T,  P = softmax(scale S),  O = P V            (a query without keys: zeros)
+//   delta = rowsum(O dO),  dS = P (dO V^T - delta),  dQ = scale dS K,  dK = scale dS^T Q,  dV = P^T dO
+// Exponentials are taken in base 2: P = 2^(S scale log2(e) - L), with L the row's log2 of its sum (kept for the backward
+// pass; an infinity for a row without keys, which makes its P zero).
+//
+// Sequences are batch entries of one length, or runs of packed rows between device-side boundaries; rows behind the
+// last boundary belong to one more sequence that has nothing to look at (and nobody who looks at it). What the boundaries
+// hold is clamped to the tensors.
+#pragma once
+
+#include "common.cuh"
+#include "dequant.cuh"
+#include "errors.cuh"
+#include "gemm_args.cuh"
+
+namespace moss {
+namespace cross {
+
+constexpr int kTile = 128;  // queries, and keys, of one tile
+
+struct Args {
+  int batch, q_heads, k_heads, group, head_dim;
+  int tq, tk;                // rows of each batch entry, or of the whole packed stream
+  const int64_t* q_offsets;  // [batch + 1], packed; null for batch entries
+  const int64_t* k_offsets;
+  const uint8_t* mask;       // [batch][mask_ld] or null: non-zero where a key may be looked at
+  int64_t mask_ld;
+  float scale, scale_log2;
+  // results, dense [rows][heads][head_dim]; rows of a batch entry b start at b * tq (b * tk)
+  void* out;
+  float* lse;                // [q_heads][batch * tq or packed rows]
+  int64_t q_rows, k_rows;    // all rows
+  // splits > 1: f32 partials of each split, joined by a second kernel
+  float* partial;            // [split][q_rows][q_heads][head_dim] (forward, dq); [2][split][k_rows][k_heads][head_dim] (dk, dv)
+  float* partial_lse;        // [split][q_heads][q_rows]
+  int splits;
+  int tiles;                 // tiles (or pairs of tiles) of all sequences, at most
+  // backward
+  const void* o;             // dense
+  const void* grad;          // dense
+  float* delta;              // [q_heads][q_rows]
+  void* dk;
+  void* dv;
+  StatusSink status;
+};
+
+struct Sequence {
+  int q0, qn, k0, kn;  // rows in the tensor map's token dimension
+  int entry;           // and the map's batch coordinate
+  int64_t q_row, k_row;  // the first rows among all
+};
+
+__device__ __forceinline__ int clamped(const int64_t* offsets, int i, int total) {
+  return i == 0 ? 0 : static_cast<int>(max(int64_t{0}, min(static_cast<int64_t>(total), __ldg(offsets + i))));
+}
+
+__device__ __forceinline__ Sequence sequence_of(const Args& a, int s) {
+  Sequence r;
+  if (a.q_offsets == nullptr) {
+    r.q0 = r.k0 = 0;
+    r.qn = a.tq;
+    r.kn = a.tk;
+    r.entry = s;
+    r.q_row = static_cast<int64_t>(s) * a.tq;
+    r.k_row = static_cast<int64_t>(s) * a.tk;
+  } else {
+    r.entry = 0;
+    r.q0 = clamped(a.q_offsets, s, a.tq);
+    r.k0 = clamped(a.k_offsets, s, a.tk);
+    // rows behind the last sequence: queries without keys, and keys without queries
+    r.qn = (s < a.batch ? clamped(a.q_offsets, s + 1, a.tq) : a.tq) - r.q0;
+    r.kn = (s < a.batch ? clamped(a.k_offsets, s + 1, a.tk) : a.tk) - r.k0;
+    r.qn = max(r.qn, 0);
+    r.kn = max(r.kn, 0);
+    r.q_row = r.q0;
+    r.k_row = r.k0;
+  }
+  return r;
+}
+
+// Tile t (of `rows` rows) of all sequences: whose it is, and which. By a whole warp. False past the last one.
+template <bool kOfKeys>
+__device__ __forceinline__ bool find_tile(const Args& a, int rows, int t, int& seq, int& tile) {
+  if (a.q_offsets == nullptr) {
+    const int each = ((kOfKeys ? a.tk : a.tq) + rows - 1) / rows;
+    seq = t / each;
+    tile = t - seq * each;
+    return seq < a.batch;
+  }
+  const int lane = threadIdx.x & 31;
+  const int64_t* offsets = kOfKeys ? a.k_offsets : a.q_offsets;
+  const int total = kOfKeys ? a.tk : a.tq;
+  int before = 0;
+  for (int s0 = 0; s0 <= a.batch; s0 += 32) {
+    const int s = s0 + lane;
+    int n = 0;
+    if (s <= a.batch) {
+      const int end = s < a.batch ? clamped(offsets, s + 1, total) : total;
+      n = (max(end - clamped(offsets, s, total), 0) + rows - 1) / rows;
+    }
+    int upto = n;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, upto, d);
+      if (lane >= d) upto += v;
+    }
+    const uint32_t past = __ballot_sync(0xffffffffu, before + upto > t);
+    if (past != 0) {
+      const int first = __ffs(past) - 1;
+      seq = s0 + first;
+      tile = t - before - __shfl_sync(0xffffffffu, upto - n, first);
+      return true;
+    }
+    before += __shfl_sync(0xffffffffu, upto, 31);
+  }
+  return false;
+}
+
+// Which of the 128 keys from `key` on exist and are allowed, as four words. By a whole warp.
+struct KeyBits {
+  uint32_t w[4];
+  __device__ __forceinline__ bool all() const { return (w[0] & w[1] & w[2] & w[3]) == 0xffffffffu; }
+};
+__device__ __forceinline__ KeyBits key_bits(const Args& a, const Sequence& s, int key) {
+  KeyBits b;
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int k = key + i * 32 + lane;
+    bool ok = k < s.kn;
+    if (ok && a.mask != nullptr) ok = __ldg(a.mask + s.entry * a.mask_ld + k) != 0;
+    b.w[i] = __ballot_sync(0xffffffffu, ok);
+  }
+  return b;
+}
+
+// Bounded wait of a whole warp, which leaves it together with one answer.
+__device__ __forceinline__ bool wait_together(uint32_t bar, uint32_t parity, volatile int* abort_flag, StatusSink status,
+                                              int code) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, status, code)) != 0;
+}
+
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int c2,
+                                            int c3) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+      : "memory");
+}
+// 128 rows of a head as boxes of 64 values (what lies past the head's values reads as zero).
+template <int kD>
+__device__ __forceinline__ void load_tile(uint32_t dst, const CUtensorMap* map, uint32_t bar, int row, int head, int entry) {
+#pragma unroll
+  for (int c = 0; c < kD / 64; ++c) tma_load_4d(dst + c * 16384, map, bar, c * 64, row, head, entry);
+}
+
+// D[tmem] (+)= A[tmem, 16-bit pairs along the columns] * B[smem desc].
+__device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
+                                            uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// 128 x 128 products over a tile's values: A and B by rows (both reduced along the head).
+template <int kD>
+__device__ __forceinline__ void mma_over_head(uint32_t d, uint64_t a_desc, uint64_t b_desc, uint32_t idesc) {
+#pragma unroll
+  for (int kk = 0; kk < kD / 16; ++kk) {
+    const uint64_t at = ((kk >> 2) * 16384 + (kk & 3) * 32) >> 4;
+    umma_f16(d, a_desc + at, b_desc + at, idesc, kk > 0 ? 1u : 0u);
+  }
+}
+// 128 x kD products over a tile's 128 rows: A in TMEM, B by columns.
+__device__ __forceinline__ void mma_over_rows(uint32_t d, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, bool accumulate) {
+#pragma unroll
+  for (int kk = 0; kk < kTile / 16; ++kk)
+    umma_f16_ts(d, a_tmem + kk * 8, b_desc + kk * (2048 >> 4), idesc, accumulate || kk > 0 ? 1u : 0u);
+}
+__device__ __forceinline__ uint64_t by_rows_desc(uint32_t tile) { return umma_desc_sw128(tile, 16, 1024); }
+__device__ __forceinline__ uint64_t by_columns_desc(uint32_t tile) { return umma_desc_sw128(tile, 16384, 1024); }
+
+// tcgen05.wait::ld that also orders the use of the loaded registers behind it.
+__device__ __forceinline__ void wait_ld_of(uint32_t (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                 "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]),
+                 "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]),
+                 "+r"(r[30]), "+r"(r[31])
+               :
+               : "memory");
+}
+
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// A warp zeroes the rows of a 128-row tile whose bit is not set (what lies there may be anything, and 0 * NaN is NaN), a row
+// a lane, then makes that visible to the tensor cores.
+template <int kD>
+__device__ __forceinline__ void scrub_rows(uint32_t tile, const KeyBits& keep) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if ((keep.w[i] >> lane) & 1u) continue;
+    const uint32_t row = tile + (i * 32 + lane) * 128;
+#pragma unroll
+    for (int c = 0; c < kD / 8; ++c)  // (in an order of its own in each lane: neighbouring rows meet the same banks)
+      gemm::sts128(row + (c >> 3) * 16384 + (((c + lane) & 7) << 4), make_uint4(0, 0, 0, 0));
+  }
+  fence_proxy_async_smem();
+  __syncwarp();
+}
+
+// Which key tiles have a key that may be looked at, a bit for each tile of each entry, so that the others are passed over.
+// Masks of more tiles go without (every tile is then taken).
+constexpr int kMaxTileBits = 256;
+__device__ __forceinline__ bool has_tile_bits(const Args& a, int key_tiles) {
+  return a.mask != nullptr && static_cast<int64_t>(a.batch) * key_tiles <= kMaxTileBits;
+}
+// By the whole CTA, with a barrier behind it; `bits` is zero before.
+__device__ __forceinline__ void find_tile_bits(const Args& a, int key_tiles, uint32_t* bits) {
+  const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  const int total = a.batch * key_tiles;
+  for (int i = threadIdx.x >> 5; i < total; i += warps) {
+    const int entry = i / key_tiles, key = (i - entry * key_tiles) * kTile;
+    bool any = false;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int k = key + j * 32 + lane;
+      if (k < a.tk) any = any || __ldg(a.mask + entry * a.mask_ld + k) != 0;
+    }
+    if (__any_sync(0xffffffffu, any) && lane == 0) atomicOr(bits + (i >> 5), 1u << (i & 31));
+  }
+}
+struct TileBits {
+  const uint32_t* bits;  // null: every tile
+  int key_tiles;
+  __device__ __forceinline__ bool has(int entry, int tile) const {
+    const int i = entry * key_tiles + tile;
+    return bits == nullptr || ((bits[i >> 5] >> (i & 31)) & 1u) != 0;
+  }
+  // the first tile from t on that is taken, or end
+  __device__ __forceinline__ int next(int entry, int t, int end) const {
+    while (t < end && !has(entry, t)) ++t;
+    return t;
+  }
+};
+
+// Whether key tile `tile` holds the only key that the sequence's queries look at. P is then 1 whatever the logit is, and the
+// gradient of the logit nothing (the difference dP - delta would leave its rounding). By a whole warp. A key alone in a mask
+// of too many tiles for TileBits is not found out.
+__device__ __forceinline__ bool only_key(const Args& a, const TileBits& taken, const Sequence& s, int tile) {
+  if (s.kn == 1 || a.mask == nullptr) return s.kn == 1;
+  const int tiles = (s.kn + kTile - 1) / kTile;
+  if (taken.bits == nullptr && tiles > 1) return false;
+  if (taken.next(s.entry, 0, tiles) != tile || taken.next(s.entry, tile + 1, tiles) < tiles) return false;
+  const KeyBits b = key_bits(a, s, tile * kTile);
+  return __popc(b.w[0]) + __popc(b.w[1]) + __popc(b.w[2]) + __popc(b.w[3]) == 1;
+}
+
+// 32 consecutive values of a row, the first `count` of them (a multiple of 8).
+template <int kKind>
+__device__ __forceinline__ void store_row32(uint16_t* to, bool wide, int count, const float (&v)[32]) {
+  uint32_t w[16];
+#pragma unroll
+  for (int j = 0; j < 16; ++j) w[j] = gemm::pack2_kind<kKind>(v[2 * j], v[2 * j + 1]);
+  if (wide && count >= 32) {  // 32-byte aligned
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      uint32_t o[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) o[j] = w[8 * h + j];
+      gemm::stg256(to + 16 * h, o);
+    }
+    return;
+  }
+#pragma unroll
+  for (int h = 0; h < 4; ++h)
+    if (8 * h < count) *reinterpret_cast<uint4*>(to + 8 * h) = make_uint4(w[4 * h], w[4 * h + 1], w[4 * h + 2], w[4 * h + 3]);
+}
+__device__ __forceinline__ void store_row32_f32(float* to, int count, const float (&v)[32]) {
+#pragma unroll
+  for (int h = 0; h < 8; ++h)
+    if (4 * h < count) *reinterpret_cast<float4*>(to + 4 * h) = make_float4(v[4 * h], v[4 * h + 1], v[4 * h + 2], v[4 * h + 3]);
+}
+
+struct Maps {
+  CUtensorMap q, k, v, grad;
+};
+
+int launch_forward(int kind, const Maps& maps, const Args& a, cudaStream_t stream);
+int launch_dq(int kind, const Maps& maps, const Args& a, cudaStream_t stream);
+int launch_dkv(int kind, const Maps& maps, const Args& a, cudaStream_t stream);
+
+}  // namespace cross
+}  // namespace moss

@@ -1,0 +1,463 @@
+// Forward pass of the attention to another sequence, on the tensor cores (tcgen05.mma.kind::f16).
+//
+// A CTA takes two tiles of 128 queries of one head. For each tile of 128 keys: S = Q K^T into TMEM, a warpgroup for
+// each query tile reads its rows (a thread a row, so a row's maximum and sum need no shuffles), writes P back to TMEM as
+// 16-bit pairs over S, and O += P V takes P from there. While one tile's rows are exponentiated, the tensor cores
+// work for the other. O stays in TMEM; it is rescaled only where a row's maximum grows by more than 2^8 over the one
+// its exponentials are taken against (P up to 256 loses nothing: its sum is f32, and 16-bit rounding is relative).
+// The CTAs are persistent: the next pair's loads and first S run during the last tile's softmax.
+//
+// Warps: 0 loads by TMA, 1 issues the MMAs, 2 zeroes masked rows of V (0 * NaN is NaN), 4-7 and 8-11 the softmax.
+//
+// P is rounded to the inputs' 16-bit type (half a step of each term; the sum it is divided by is of the unrounded values).
+#include <algorithm>
+#include <cmath>
+#include <cstring>
+
+#include "cross_args.cuh"
+
+namespace moss {
+namespace cross {
+namespace {
+
+constexpr int kThreads = 384;
+constexpr int kMiscRegs = 56, kSoftmaxRegs = 224;
+static_assert(kMiscRegs + 2 * kSoftmaxRegs <= 3 * 168, "a larger split would wait forever");
+constexpr float kGrowth = 8.0f;
+
+template <int kD>
+struct Shape {
+  static constexpr uint32_t kTileBytes = kTile * kD * 2;
+  static constexpr int kStages = kD == 128 ? 5 : 8;  // tiles of K and V on their way
+  static constexpr uint32_t kDataBytes = (2 + kStages) * kTileBytes;
+  static constexpr uint32_t kSmemBytes = kDataBytes + 1024 + 512;
+  static_assert(kSmemBytes <= 227 * 1024, "tiles exceed the shared memory a CTA may use");
+};
+constexpr int kMaxStages = 8;
+
+struct Barriers {
+  uint64_t q_full[2], q_empty[2];
+  uint64_t full[kMaxStages], empty[kMaxStages];
+  uint64_t clean[kMaxStages];  // masked rows of the n-th V tile are zero (n modulo the stages)
+  uint64_t s_full[2];          // S is there (and the last product with P is done)
+  uint64_t p_ready[2];         // P is there, O may be added to
+  uint64_t o_full[2], o_free[2];
+  uint64_t drain;
+  uint32_t tile_bits[kMaxTileBits / 32];
+  uint32_t tmem_base;
+  int abort_flag;
+};
+static_assert(sizeof(Barriers) <= 512, "barrier block too large");
+
+// Work unit: a pair of query tiles of one head, and a run of its key tiles.
+struct Unit {
+  Sequence s;
+  int head, split, row, first, end;  // row: the pair's first within the sequence
+  __device__ __forceinline__ int tiles() const { return s.qn - row > kTile ? 2 : 1; }
+  __device__ __forceinline__ int next(const TileBits& taken, int t) const { return taken.next(s.entry, t + 1, end); }
+};
+__device__ __forceinline__ bool locate(const Args& a, const TileBits& taken, int u, Unit& unit) {
+  const int t = u % a.tiles, rest = u / a.tiles;
+  unit.split = rest % a.splits;
+  unit.head = rest / a.splits;
+  int seq, tile;
+  if (!find_tile<false>(a, 2 * kTile, t, seq, tile)) return false;
+  unit.s = sequence_of(a, seq);
+  if (seq >= a.batch) unit.s.kn = 0;
+  unit.row = tile * 2 * kTile;
+  const int keys = (unit.s.kn + kTile - 1) / kTile, each = (keys + a.splits - 1) / a.splits;
+  unit.end = min(keys, (unit.split + 1) * each);
+  unit.first = taken.next(unit.s.entry, min(keys, unit.split * each), unit.end);
+  return true;
+}
+
+// kMask: keys may be masked, or a tile may hold rows of the next sequence.
+template <int kKind, int kD, bool kMask>
+__global__ void __launch_bounds__(kThreads, 1)
+    cross_forward_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                         const __grid_constant__ CUtensorMap tm_v, const Args args) {
+  using S = Shape<kD>;
+  constexpr uint32_t kTileBytes = S::kTileBytes;
+  constexpr int kStages = S::kStages;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw_base = smem_u32(smem_raw);
+  const uint32_t base = (raw_base + 1023u) & ~1023u;
+  const uint32_t ring = base + 2 * kTileBytes;
+  Barriers* bars = reinterpret_cast<Barriers*>(smem_raw + (base - raw_base) + S::kDataBytes);
+  auto bar = [&](uint64_t& b) { return smem_u32(&b); };
+  volatile int* abort_flag = &bars->abort_flag;
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const int num_units = args.tiles * args.splits * args.q_heads;
+
+  if (threadIdx.x == 0) {
+    for (int x = 0; x < 2; ++x) {
+      mbar_init(bar(bars->q_full[x]), 1);
+      mbar_init(bar(bars->q_empty[x]), 1);
+      mbar_init(bar(bars->s_full[x]), 1);
+      mbar_init(bar(bars->p_ready[x]), kTile);
+      mbar_init(bar(bars->o_full[x]), 1);
+      mbar_init(bar(bars->o_free[x]), kTile);
+    }
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(bar(bars->full[s]), 1);
+      mbar_init(bar(bars->empty[s]), 1);
+      mbar_init(bar(bars->clean[s]), 1);
+    }
+    mbar_init(bar(bars->drain), 1);
+    bars->abort_flag = 0;
+    for (int i = 0; i < kMaxTileBits / 32; ++i) bars->tile_bits[i] = 0;
+    fence_mbar_init();
+  }
+  const int key_tiles = (args.tk + kTile - 1) / kTile;
+  const bool use_bits = kMask && has_tile_bits(args, key_tiles);
+  if (use_bits) {
+    __syncthreads();
+    find_tile_bits(args, key_tiles, bars->tile_bits);
+  }
+  if (warp == 1) {
+    tmem_alloc(smem_u32(&bars->tmem_base), 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const TileBits taken{use_bits ? bars->tile_bits : nullptr, key_tiles};
+  const uint32_t tmem = bars->tmem_base;  // S (and P) of the two tiles, then O of the two tiles
+
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kMiscRegs));
+    if (warp == 0) {
+      // ---------------------------------------------------------------- loads
+      uint32_t pos = 0, used = 0, last_phase = 0;
+      uint32_t q_uses[2] = {0, 0};
+      bool ok = true;
+      if (lane == 0) {
+        tma_prefetch_desc(&tm_q);
+        tma_prefetch_desc(&tm_k);
+        tma_prefetch_desc(&tm_v);
+      }
+      for (int u = blockIdx.x; u < num_units && ok; u += gridDim.x) {
+        Unit w;
+        if (!locate(args, taken, u, w) || w.first == w.end) continue;
+        const int k_head = w.head / args.group;
+        auto load_q = [&](int x) {
+          if (!wait_together(bar(bars->q_empty[x]), (q_uses[x] & 1u) ^ 1u, abort_flag, args.status, MOSS_STATUS_TIMEOUT_LOAD))
+            return false;
+          if (lane == 0) {
+            mbar_arrive_expect_tx(bar(bars->q_full[x]), kTileBytes);
+            load_tile<kD>(base + x * kTileBytes, &tm_q, bar(bars->q_full[x]), w.s.q0 + w.row + x * kTile, w.head, w.s.entry);
+          }
+          ++q_uses[x];
+          __syncwarp();
+          return true;
+        };
+        auto load_kv = [&](const CUtensorMap* map, int tile) {
+          const uint32_t stage = pos % kStages, phase = (pos / kStages) & 1u;
+          if (!wait_together(bar(bars->empty[stage]), phase ^ 1u, abort_flag, args.status, MOSS_STATUS_TIMEOUT_LOAD)) return false;
+          if (lane == 0) {
+            mbar_arrive_expect_tx(bar(bars->full[stage]), kTileBytes);
+            load_tile<kD>(ring + stage * kTileBytes, map, bar(bars->full[stage]), w.s.k0 + tile * kTile, k_head, w.s.entry);
+            used |= 1u << stage;
+            last_phase = (last_phase & ~(1u << stage)) | (phase << stage);
+          }
+          ++pos;
+          __syncwarp();
+          return true;
+        };
+        ok = load_q(0) && load_kv(&tm_k, w.first) && (w.tiles() == 1 || load_q(1)) && load_kv(&tm_v, w.first);
+        for (int t = w.next(taken, w.first); t < w.end && ok; t = w.next(taken, t)) ok = load_kv(&tm_k, t) && load_kv(&tm_v, t);
+      }
+      if (lane == 0) {  // the copies land before the CTA may leave
+        auto landed = [&](uint64_t& b, uint32_t parity) {
+          const long long start = clock64();
+          while (!mbar_try_wait(bar(b), parity)) {
+            if (clock64() - start > kWaitBudgetCycles) {
+              report_status(args.status, MOSS_STATUS_TIMEOUT_DRAIN);
+              break;
+            }
+          }
+        };
+        for (int s = 0; s < kStages; ++s)
+          if ((used >> s) & 1u) landed(bars->full[s], (last_phase >> s) & 1u);
+        for (int x = 0; x < 2; ++x)
+          if (q_uses[x] > 0) landed(bars->q_full[x], (q_uses[x] - 1) & 1u);
+      }
+    } else if (warp == 1) {
+      // ---------------------------------------------------------------- MMAs
+      constexpr uint32_t kFormat = kKind == kBF16 ? 1u : 0u;
+      constexpr uint32_t s_idesc = umma_idesc_f16(kFormat, false, kTile, kTile);
+      constexpr uint32_t o_idesc = umma_idesc_f16(kFormat, true, kTile, kD);
+      const uint64_t q_desc = by_rows_desc(base), k_desc = by_rows_desc(ring), v_desc = by_columns_desc(ring);
+      uint32_t pos = 0, q_uses[2] = {0, 0}, p_uses[2] = {0, 0}, o_uses[2] = {0, 0};
+      bool ok = true, issued = false;
+      auto wait = [&](uint64_t& b, uint32_t parity) {
+        return wait_together(bar(b), parity, abort_flag, args.status, MOSS_STATUS_TIMEOUT_MMA);
+      };
+      for (int u = blockIdx.x; u < num_units && ok; u += gridDim.x) {
+        Unit w;
+        if (!locate(args, taken, u, w) || w.first == w.end) continue;
+        const int tiles = w.tiles();
+        int following = w.next(taken, w.first);  // the key tile after the one at hand
+        // S of tile x against the key tile at ring position p
+        auto scores = [&](int x, uint32_t p, bool last) {
+          if (elect_one()) {
+            mma_over_head<kD>(tmem + x * kTile, q_desc + ((x * kTileBytes) >> 4),
+                              k_desc + (((p % kStages) * kTileBytes) >> 4), s_idesc);
+            umma_commit(bar(bars->s_full[x]));
+            if (last) umma_commit(bar(bars->q_empty[x]));
+          }
+          issued = true;
+          __syncwarp();
+        };
+        auto release = [&](uint32_t p) {
+          if (elect_one()) umma_commit(bar(bars->empty[p % kStages]));
+          __syncwarp();
+        };
+        ok = wait(bars->full[pos % kStages], (pos / kStages) & 1u);
+        for (int x = 0; x < tiles && ok; ++x) {
+          ok = wait(bars->q_full[x], q_uses[x]++ & 1u);
+          if (!ok) break;
+          tc_fence_after();
+          scores(x, pos, following >= w.end);
+        }
+        if (!ok) break;
+        release(pos);
+        bool begun = false;
+        while (ok) {
+          const bool more = following < w.end;
+          const int then = more ? w.next(taken, following) : w.end;
+          const uint32_t pv = pos + 1, pk = pos + 2;
+          const uint32_t nth = pos / 2;  // of the V tiles: what `clean` counts
+          ok = kMask ? wait(bars->clean[nth % kStages], (nth / kStages) & 1u) : wait(bars->full[pv % kStages], (pv / kStages) & 1u);
+          for (int x = 0; x < tiles && ok; ++x) {
+            if (!begun) ok = wait(bars->o_free[x], (o_uses[x]++ & 1u) ^ 1u);
+            ok = ok && wait(bars->p_ready[x], p_uses[x]++ & 1u);
+            if (!ok) break;
+            tc_fence_after();
+            if (elect_one()) {
+              mma_over_rows(tmem + 2 * kTile + x * kTile, tmem + x * kTile, v_desc + (((pv % kStages) * kTileBytes) >> 4),
+                            o_idesc, begun);
+              if (!more) umma_commit(bar(bars->o_full[x]));
+            }
+            __syncwarp();
+            if (more) {
+              if (x == 0) ok = wait(bars->full[pk % kStages], (pk / kStages) & 1u);
+              if (!ok) break;
+              tc_fence_after();
+              scores(x, pk, then >= w.end);
+            }
+          }
+          if (!ok) break;
+          release(pv);
+          pos += 2;
+          if (!more) break;
+          release(pk);
+          begun = true;
+          following = then;
+        }
+      }
+      if (lane == 0 && issued) {
+        umma_commit(bar(bars->drain));
+        const long long start = clock64();
+        while (!mbar_try_wait(bar(bars->drain), 0)) {
+          if (clock64() - start > kWaitBudgetCycles) {
+            report_status(args.status, MOSS_STATUS_TIMEOUT_DRAIN);
+            break;
+          }
+        }
+      }
+      __syncwarp();
+    } else if (kMask && warp == 2) {
+      // ---------------------------------------------------------------- masked rows of V
+      uint32_t pos = 0;
+      bool ok = true;
+      for (int u = blockIdx.x; u < num_units && ok; u += gridDim.x) {
+        Unit w;
+        if (!locate(args, taken, u, w) || w.first == w.end) continue;
+        for (int t = w.first; t < w.end; t = w.next(taken, t), pos += 2) {
+          const KeyBits keep = key_bits(args, w.s, t * kTile);
+          const uint32_t stage = (pos + 1) % kStages, phase = ((pos + 1) / kStages) & 1u;
+          ok = wait_together(bar(bars->full[stage]), phase, abort_flag, args.status, MOSS_STATUS_TIMEOUT_LOAD);
+          if (!ok) break;
+          if (!keep.all()) scrub_rows<kD>(ring + stage * kTileBytes, keep);
+          if (lane == 0) mbar_arrive(bar(bars->clean[(pos / 2) % kStages]));
+        }
+      }
+    }
+  } else {
+    // ---------------------------------------------------------------- softmax and output
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+    const int x = (warp - 4) >> 2;
+    const int row = (warp & 3) * 32 + lane;
+    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t s_tmem = tmem + x * kTile + lanes, o_tmem = tmem + 2 * kTile + x * kTile + lanes;
+    const bool wide = args.head_dim % 16 == 0 && (reinterpret_cast<uintptr_t>(args.out) & 31) == 0;
+    uint32_t s_uses = 0, o_uses = 0;
+    bool ok = true;
+    for (int u = blockIdx.x; u < num_units && ok; u += gridDim.x) {
+      Unit w;
+      if (!locate(args, taken, u, w) || x >= w.tiles()) continue;
+      const int at = w.row + x * kTile + row;  // within the sequence
+      const int64_t q_row = w.s.q_row + at;
+      const bool live = at < w.s.qn;
+      float top = -INFINITY, sum = 0.0f;  // the exponentials' reference, times scale_log2
+      for (int t = w.first; t < w.end; t = w.next(taken, t)) {
+        KeyBits keep;
+        const int keys = w.s.kn - t * kTile;
+        if constexpr (kMask) keep = key_bits(args, w.s, t * kTile);
+        ok = wait_together(bar(bars->s_full[x]), s_uses++ & 1u, abort_flag, args.status, MOSS_STATUS_TIMEOUT_EPILOGUE);
+        if (!ok) break;
+        tc_fence_after();
+        uint32_t r[4][32];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32(s_tmem + c * 32, r[c]);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) wait_ld_of(r[c]);
+        if constexpr (kMask) {
+          if (!keep.all()) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j)
+                if (((keep.w[c] >> j) & 1u) == 0) r[c][j] = 0xff800000u;
+            }
+          }
+        } else if (keys < kTile) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (c * 32 + j >= keys) r[c][j] = 0xff800000u;
+          }
+        }
+        float most[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int j = 0; j < 32; ++j) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) most[c] = fmaxf(most[c], __uint_as_float(r[c][j]));
+        }
+        // (the scale is positive, so the greatest product gives the greatest logit)
+        const float here = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])) * args.scale_log2;
+        const bool grows = here > top + kGrowth;  // (from -inf always, unless the tile is masked)
+        if (__any_sync(0xffffffffu, grows)) {
+          const float factor = grows ? exp2_approx(top - here) : 1.0f;
+          if (grows) top = here;
+          sum *= factor;
+          if (t > w.first) {
+#pragma unroll
+            for (int c = 0; c < kD / 32; ++c) {
+              uint32_t o[32];
+              tmem_ld_32x32b_x32(o_tmem + c * 32, o);
+              wait_ld_of(o);
+              uint32_t lo[16], hi[16];
+#pragma unroll
+              for (int j = 0; j < 16; ++j) {
+                lo[j] = __float_as_uint(__uint_as_float(o[j]) * factor);
+                hi[j] = __float_as_uint(__uint_as_float(o[16 + j]) * factor);
+              }
+              tmem_st_32x32b_x16(o_tmem + c * 32, lo);
+              tmem_st_32x32b_x16(o_tmem + c * 32 + 16, hi);
+            }
+          }
+        }
+        const float shift = top == -INFINITY ? 0.0f : top;
+        float add[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t p[16];
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            const float e0 = exp2_approx(fmaf(__uint_as_float(r[c][2 * j]), args.scale_log2, -shift));
+            const float e1 = exp2_approx(fmaf(__uint_as_float(r[c][2 * j + 1]), args.scale_log2, -shift));
+            add[j & 3] += e0 + e1;
+            p[j] = gemm::pack2_kind<kKind>(e0, e1);
+          }
+          tmem_st_32x32b_x16(s_tmem + c * 16, p);
+        }
+        sum += (add[0] + add[1]) + (add[2] + add[3]);
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(bar(bars->p_ready[x]));
+      }
+      if (!ok) break;
+      const bool any_keys = w.first < w.end;
+      if (any_keys) {
+        ok = wait_together(bar(bars->o_full[x]), o_uses++ & 1u, abort_flag, args.status, MOSS_STATUS_TIMEOUT_EPILOGUE);
+        if (!ok) break;
+        tc_fence_after();
+      }
+      const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
+      const int64_t at_out = (q_row * args.q_heads + w.head) * args.head_dim;
+#pragma unroll
+      for (int c = 0; c < kD / 32; ++c) {
+        uint32_t o[32];
+        float v[32];
+        __syncwarp();  // (lanes past the last row have nothing to store)
+        if (any_keys) {
+          tmem_ld_32x32b_x32(o_tmem + c * 32, o);
+          wait_ld_of(o);
+          if (c == kD / 32 - 1) {
+            tc_fence_before();
+            mbar_arrive(bar(bars->o_free[x]));
+          }
+        }
+        // (a row whose keys are all masked has zeros in O, and an empty one nothing)
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] = any_keys ? __uint_as_float(o[j]) * inverse : 0.0f;
+        const int count = args.head_dim - c * 32;
+        if (live && count > 0) {
+          if (args.splits > 1)
+            store_row32_f32(args.partial + w.split * args.q_rows * args.q_heads * args.head_dim + at_out + c * 32, count, v);
+          else
+            store_row32<kKind>(static_cast<uint16_t*>(args.out) + at_out + c * 32, wide, count, v);
+        }
+      }
+      if (live) {
+        const float l = sum == 0.0f ? -INFINITY : top + log2f(sum);
+        if (args.splits > 1)
+          args.partial_lse[(static_cast<int64_t>(w.split) * args.q_heads + w.head) * args.q_rows + q_row] = l;
+        else if (args.lse != nullptr)
+          args.lse[w.head * args.q_rows + q_row] = sum == 0.0f ? INFINITY : l;
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+template <int kKind, int kD, bool kMask>
+int launch_typed(const Maps& maps, const Args& a, cudaStream_t stream) {
+  auto kern = cross_forward_kernel<kKind, kD, kMask>;
+  static DeviceSetup setup;
+  const int rc = setup("cross_forward_kernel", nullptr, [&](int*) {
+    return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<kD>::kSmemBytes);
+  });
+  if (rc != MOSS_OK) return rc;
+  const int64_t units = static_cast<int64_t>(a.tiles) * a.splits * a.q_heads;
+  const unsigned grid = static_cast<unsigned>(std::min<int64_t>(units, device_sm_count()));
+  kern<<<grid, kThreads, Shape<kD>::kSmemBytes, stream>>>(maps.q, maps.k, maps.v, a);
+  return check_cuda(cudaGetLastError(), "cross_forward_kernel");
+}
+
+template <int kKind, int kD>
+int launch_mask(const Maps& maps, const Args& a, cudaStream_t stream) {
+  return a.mask != nullptr || a.q_offsets != nullptr ? launch_typed<kKind, kD, true>(maps, a, stream)
+                                                     : launch_typed<kKind, kD, false>(maps, a, stream);
+}
+
+}  // namespace
+
+int launch_forward(int kind, const Maps& maps, const Args& a, cudaStream_t stream) {
+  if (kind == kBF16)
+    return a.head_dim <= 64 ? launch_mask<kBF16, 64>(maps, a, stream) : launch_mask<kBF16, 128>(maps, a, stream);
+  return a.head_dim <= 64 ? launch_mask<kF16, 64>(maps, a, stream) : launch_mask<kF16, 128>(maps, a, stream);
+}
+
+}  // namespace cross
+}  // namespace moss
