@@ -25,6 +25,10 @@ constexpr int kThreads = 384;
 constexpr int kMiscRegs = 72, kMathRegs = 216;
 static_assert(kMiscRegs + 2 * kMathRegs <= 3 * 168, "a larger split would wait forever");
 constexpr int kHalf = kTile / 2;  // columns of one warpgroup
+// f16 has no normal values below 2^-14: there dV is summed from 2^14 P (at most 2^14) and scaled back at the end. dS has no
+// bound that would leave room for that: below 2^-14 it is rounded to multiples of 2^-24, as an f16 gradient itself is.
+template <int kKind>
+constexpr float kLift = kKind == kF16 ? 14.0f : 0.0f;
 
 template <int kD>
 struct Shape {
@@ -684,7 +688,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           const float ls[4] = {l.x, l.y, l.z, l.w};
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            v[j + e] = exp2_approx(fmaf(__uint_as_float(r[(j + e) >> 5][(j + e) & 31]), args.scale_log2, -ls[e]));
+            v[j + e] = exp2_approx(fmaf(__uint_as_float(r[(j + e) >> 5][(j + e) & 31]), args.scale_log2, kLift<kKind> - ls[e]));
         }
         if (!seen || rows < kHalf) {
 #pragma unroll
@@ -693,6 +697,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         __syncwarp();
         store64<kKind>(tmem + half * kHalf + lanes, v);
+        if constexpr (kKind == kF16) {
+#pragma unroll
+          for (int j = 0; j < 64; ++j) v[j] *= 1.0f / 16384.0f;
+        }
         tmem_wait_st();
         tc_fence_before();
         mbar_arrive(smem_u32(&bars->p_ready));
@@ -729,7 +737,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int64_t values = args.k_rows * args.k_heads * args.head_dim;
       const int64_t to = ((w.s.k_row + key) * args.k_heads + w.head) * args.head_dim;
       const uint32_t from = (half == 0 ? dv_tmem : dk_tmem) + lanes;
-      const float factor = half == 0 ? 1.0f : args.scale;
+      const float factor = half == 1 ? args.scale : kKind == kF16 ? 1.0f / 16384.0f : 1.0f;
 #pragma unroll
       for (int c = 0; c < kD / 32; ++c) {
         uint32_t o[32];

@@ -24,6 +24,9 @@ constexpr int kThreads = 384;
 constexpr int kMiscRegs = 56, kSoftmaxRegs = 224;
 static_assert(kMiscRegs + 2 * kSoftmaxRegs <= 3 * 168, "a larger split would wait forever");
 constexpr float kGrowth = 8.0f;
+// f16 has no normal values below 2^-14: there the exponentials are 2^7 larger (up to 2^15 with kGrowth), which their sum is too.
+template <int kKind>
+constexpr float kLift = kKind == kF16 ? 7.0f : 0.0f;
 
 template <int kD>
 struct Shape {
@@ -361,7 +364,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
         }
-        const float shift = top == -INFINITY ? 0.0f : top;
+        const float shift = top == -INFINITY ? 0.0f : top - kLift<kKind>;
         float add[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
@@ -414,7 +417,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       if (live) {
-        const float l = sum == 0.0f ? -INFINITY : top + log2f(sum);
+        const float l = sum == 0.0f ? -INFINITY : top - kLift<kKind> + log2f(sum);
         if (args.splits > 1)
           args.partial_lse[(static_cast<int64_t>(w.split) * args.q_heads + w.head) * args.q_rows + q_row] = l;
         else if (args.lse != nullptr)
