@@ -137,9 +137,43 @@ __device__ __forceinline__ KeyBits key_bits(const Args& a, const Sequence& s, in
   return b;
 }
 
+// Bounded wait that polls: a thread that try_wait suspends is woken some 500 cycles after the phase completes, several times
+// a tile on the way from the products to the softmax and back (4096 x 512 tokens, 2 x 24 x 128: 85 us with it).
+__device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(done)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return done != 0;
+}
+__device__ __forceinline__ bool mbar_poll(uint32_t bar, uint32_t parity, volatile int* abort_flag, StatusSink status, int code) {
+  if (mbar_test(bar, parity)) return true;
+  const long long start = clock64();
+  while (true) {
+#pragma unroll 1
+    for (int i = 0; i < 64; ++i)
+      if (mbar_test(bar, parity)) return true;
+    if (*abort_flag) return false;
+    if (clock64() - start > kWaitBudgetCycles) {
+      *abort_flag = 1;
+      report_status(status, code);
+      return false;
+    }
+  }
+}
+
 // Bounded wait of a whole warp, which leaves it together with one answer.
 __device__ __forceinline__ bool wait_together(uint32_t bar, uint32_t parity, volatile int* abort_flag, StatusSink status,
                                               int code) {
+  return __all_sync(0xffffffffu, mbar_poll(bar, parity, abort_flag, status, code)) != 0;
+}
+// The same for waits that are long and not on the way of a tile (loads far ahead): the warp is suspended meanwhile.
+__device__ __forceinline__ bool wait_suspended(uint32_t bar, uint32_t parity, volatile int* abort_flag, StatusSink status,
+                                               int code) {
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, status, code)) != 0;
 }
 
@@ -150,6 +184,12 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map
       " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
       "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
       : "memory");
+}
+__device__ __forceinline__ void tma_store_4d(const CUtensorMap* map, uint32_t src, int c0, int c1, int c2, int c3) {
+  asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.bulk_group [%0, {%2, %3, %4, %5}], [%1];" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(src), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+               : "memory");
 }
 // 128 rows of a head as boxes of 64 values (what lies past the head's values reads as zero).
 template <int kD>
@@ -296,7 +336,8 @@ __device__ __forceinline__ void store_row32_f32(float* to, int count, const floa
 }
 
 struct Maps {
-  CUtensorMap q, k, v, grad;
+  CUtensorMap q, k, v;
+  CUtensorMap grad;  // dense: dO, or O in the forward pass
 };
 
 int launch_forward(int kind, const Maps& maps, const Args& a, cudaStream_t stream);

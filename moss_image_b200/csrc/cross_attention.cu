@@ -225,9 +225,10 @@ int forward(const Problem& p, const void* q, Strides qs, const void* k, Strides 
   rc = bind_context();
   if (rc != MOSS_OK) return rc;
   Maps maps;
-  if (!make_map(&maps.q, dtype, q, p, p.tq, p.q_heads, qs) || !make_map(&maps.k, dtype, k, p, p.tk, p.k_heads, ks) ||
-      !make_map(&maps.v, dtype, v, p, p.tk, p.k_heads, vs))
-    return fail(MOSS_ERR_INVALID_ARGUMENT, "queries, keys and values need 16-byte aligned rows of one stride");
+  const Strides dense{p.tq * p.q_heads * p.head_dim, p.q_heads * p.head_dim, p.head_dim};
+  if (!make_map(&maps.grad, dtype, out, p, p.tq, p.q_heads, dense) || !make_map(&maps.q, dtype, q, p, p.tq, p.q_heads, qs) ||
+      !make_map(&maps.k, dtype, k, p, p.tk, p.k_heads, ks) || !make_map(&maps.v, dtype, v, p, p.tk, p.k_heads, vs))
+    return fail(MOSS_ERR_INVALID_ARGUMENT, "queries, keys, values and outputs need 16-byte aligned rows of one stride");
   rc = launch_forward(dtype, maps, a, stream);
   if (rc != MOSS_OK) return rc;
   if (a.splits > 1) {

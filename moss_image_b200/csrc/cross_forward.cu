@@ -7,7 +7,7 @@
 // its exponentials are taken against (P up to 256 loses nothing: its sum is f32, and 16-bit rounding is relative).
 // The CTAs are persistent: the next pair's loads and first S run during the last tile's softmax.
 //
-// Warps: 0 loads by TMA, 1 issues the MMAs, 2 zeroes masked rows of V (0 * NaN is NaN), 4-7 and 8-11 the softmax.
+// Warps: 0 loads by TMA, 1 issues the MMAs, 2 zeroes masked rows of V (0 * NaN is NaN), 3 stores, 4-7 and 8-11 the softmax.
 //
 // P is rounded to the inputs' 16-bit type (half a step of each term; the sum it is divided by is of the unrounded values).
 #include <algorithm>
@@ -21,7 +21,7 @@ namespace cross {
 namespace {
 
 constexpr int kThreads = 384;
-constexpr int kMiscRegs = 56, kSoftmaxRegs = 224;
+constexpr int kMiscRegs = 88, kSoftmaxRegs = 208;
 static_assert(kMiscRegs + 2 * kSoftmaxRegs <= 3 * 168, "a larger split would wait forever");
 constexpr float kGrowth = 8.0f;
 // f16 has no normal values below 2^-14: there the exponentials are 2^7 larger (up to 2^15 with kGrowth), which their sum is too.
@@ -31,20 +31,21 @@ constexpr float kLift = kKind == kF16 ? 7.0f : 0.0f;
 template <int kD>
 struct Shape {
   static constexpr uint32_t kTileBytes = kTile * kD * 2;
-  static constexpr int kStages = kD == 128 ? 5 : 8;  // tiles of K and V on their way
-  static constexpr uint32_t kDataBytes = (2 + kStages) * kTileBytes;
+  static constexpr int kStages = kD == 128 ? 3 : 8;  // tiles of K and V on their way
+  static constexpr uint32_t kDataBytes = (4 + kStages) * kTileBytes;
   static constexpr uint32_t kSmemBytes = kDataBytes + 1024 + 512;
   static_assert(kSmemBytes <= 227 * 1024, "tiles exceed the shared memory a CTA may use");
 };
 constexpr int kMaxStages = 8;
 
 struct Barriers {
-  uint64_t q_full[2], q_empty[2];
+  uint64_t q_full[4], q_empty[4];  // by pair (they take turns) and tile
   uint64_t full[kMaxStages], empty[kMaxStages];
   uint64_t clean[kMaxStages];  // masked rows of the n-th V tile are zero (n modulo the stages)
   uint64_t s_full[2];          // S is there (and the last product with P is done)
   uint64_t p_ready[2];         // P is there, O may be added to
   uint64_t o_full[2], o_free[2];
+  uint64_t out_full[2];        // the results are in shared memory
   uint64_t drain;
   uint32_t tile_bits[kMaxTileBits / 32];
   uint32_t tmem_base;
@@ -74,18 +75,26 @@ __device__ __forceinline__ bool locate(const Args& a, const TileBits& taken, int
   return true;
 }
 
+// A tile of a batch entry leaves through the shared memory of its queries, which nothing reads any more, by TMA (rows past
+// the entry are not written). Rows of a packed sequence's last tile, splits and queries without keys go by their threads.
+template <bool kMask>
+__device__ __forceinline__ bool leaves_by_tma(const Args& a, const Unit& w, int x) {
+  return a.splits == 1 && (!kMask || a.q_offsets == nullptr || w.s.qn - (w.row + x * kTile) >= kTile);
+}
+
 // kMask: keys may be masked, or a tile may hold rows of the next sequence.
 template <int kKind, int kD, bool kMask>
 __global__ void __launch_bounds__(kThreads, 1)
     cross_forward_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
-                         const __grid_constant__ CUtensorMap tm_v, const Args args) {
+                         const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_out,
+                         const Args args) {
   using S = Shape<kD>;
   constexpr uint32_t kTileBytes = S::kTileBytes;
   constexpr int kStages = S::kStages;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_base = smem_u32(smem_raw);
   const uint32_t base = (raw_base + 1023u) & ~1023u;
-  const uint32_t ring = base + 2 * kTileBytes;
+  const uint32_t ring = base + 4 * kTileBytes;
   Barriers* bars = reinterpret_cast<Barriers*>(smem_raw + (base - raw_base) + S::kDataBytes);
   auto bar = [&](uint64_t& b) { return smem_u32(&b); };
   volatile int* abort_flag = &bars->abort_flag;
@@ -94,13 +103,16 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int num_units = args.tiles * args.splits * args.q_heads;
 
   if (threadIdx.x == 0) {
-    for (int x = 0; x < 2; ++x) {
+    for (int x = 0; x < 4; ++x) {
       mbar_init(bar(bars->q_full[x]), 1);
       mbar_init(bar(bars->q_empty[x]), 1);
+    }
+    for (int x = 0; x < 2; ++x) {
       mbar_init(bar(bars->s_full[x]), 1);
-      mbar_init(bar(bars->p_ready[x]), kTile);
+      mbar_init(bar(bars->p_ready[x]), 4);
       mbar_init(bar(bars->o_full[x]), 1);
-      mbar_init(bar(bars->o_free[x]), kTile);
+      mbar_init(bar(bars->o_free[x]), 4);
+      mbar_init(bar(bars->out_full[x]), 4);
     }
     for (int s = 0; s < kStages; ++s) {
       mbar_init(bar(bars->full[s]), 1);
@@ -132,44 +144,58 @@ __global__ void __launch_bounds__(kThreads, 1)
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kMiscRegs));
     if (warp == 0) {
       // ---------------------------------------------------------------- loads
-      uint32_t pos = 0, used = 0, last_phase = 0;
-      uint32_t q_uses[2] = {0, 0};
+      // Queries are loaded a whole unit ahead (all CTAs ask for theirs at about the same time, and half a unit's work
+      // does not cover that), keys and values as the ring allows.
+      uint32_t pos = 0, q_uses[4] = {0, 0, 0, 0};
+      int u = blockIdx.x, ahead = u;
+      uint32_t asked = 0;  // units whose queries were asked for
       bool ok = true;
       if (lane == 0) {
         tma_prefetch_desc(&tm_q);
         tma_prefetch_desc(&tm_k);
         tma_prefetch_desc(&tm_v);
       }
-      for (int u = blockIdx.x; u < num_units && ok; u += gridDim.x) {
+      auto load_q = [&](const Unit& w, int x) {
+        const int slot = (asked & 1u) * 2 + x;
+        if (!wait_suspended(bar(bars->q_empty[slot]), (q_uses[slot] & 1u) ^ 1u, abort_flag, args.status, MOSS_STATUS_TIMEOUT_LOAD))
+          return false;
+        if (lane == 0) {
+          mbar_arrive_expect_tx(bar(bars->q_full[slot]), kTileBytes);
+          load_tile<kD>(base + slot * kTileBytes, &tm_q, bar(bars->q_full[slot]), w.s.q0 + w.row + x * kTile, w.head, w.s.entry);
+        }
+        ++q_uses[slot];
+        __syncwarp();
+        return true;
+      };
+      auto load_kv = [&](const CUtensorMap* map, const Unit& w, int tile) {
+        const uint32_t stage = pos % kStages, phase = (pos / kStages) & 1u;
+        if (!wait_suspended(bar(bars->empty[stage]), phase ^ 1u, abort_flag, args.status, MOSS_STATUS_TIMEOUT_LOAD)) return false;
+        if (lane == 0) {
+          mbar_arrive_expect_tx(bar(bars->full[stage]), kTileBytes);
+          load_tile<kD>(ring + stage * kTileBytes, map, bar(bars->full[stage]), w.s.k0 + tile * kTile, w.head / args.group, w.s.entry);
+        }
+        ++pos;
+        __syncwarp();
+        return true;
+      };
+      // the queries of the next unit that has keys
+      auto ask = [&]() {
+        for (; ahead < num_units; ahead += gridDim.x) {
+          Unit w;
+          if (!locate(args, taken, ahead, w) || w.first == w.end) continue;
+          if (!load_q(w, 0) || (w.tiles() > 1 && !load_q(w, 1))) return false;
+          ++asked;
+          ahead += gridDim.x;
+          break;
+        }
+        return true;
+      };
+      ok = ask();
+      for (; u < num_units && ok; u += gridDim.x) {
         Unit w;
         if (!locate(args, taken, u, w) || w.first == w.end) continue;
-        const int k_head = w.head / args.group;
-        auto load_q = [&](int x) {
-          if (!wait_together(bar(bars->q_empty[x]), (q_uses[x] & 1u) ^ 1u, abort_flag, args.status, MOSS_STATUS_TIMEOUT_LOAD))
-            return false;
-          if (lane == 0) {
-            mbar_arrive_expect_tx(bar(bars->q_full[x]), kTileBytes);
-            load_tile<kD>(base + x * kTileBytes, &tm_q, bar(bars->q_full[x]), w.s.q0 + w.row + x * kTile, w.head, w.s.entry);
-          }
-          ++q_uses[x];
-          __syncwarp();
-          return true;
-        };
-        auto load_kv = [&](const CUtensorMap* map, int tile) {
-          const uint32_t stage = pos % kStages, phase = (pos / kStages) & 1u;
-          if (!wait_together(bar(bars->empty[stage]), phase ^ 1u, abort_flag, args.status, MOSS_STATUS_TIMEOUT_LOAD)) return false;
-          if (lane == 0) {
-            mbar_arrive_expect_tx(bar(bars->full[stage]), kTileBytes);
-            load_tile<kD>(ring + stage * kTileBytes, map, bar(bars->full[stage]), w.s.k0 + tile * kTile, k_head, w.s.entry);
-            used |= 1u << stage;
-            last_phase = (last_phase & ~(1u << stage)) | (phase << stage);
-          }
-          ++pos;
-          __syncwarp();
-          return true;
-        };
-        ok = load_q(0) && load_kv(&tm_k, w.first) && (w.tiles() == 1 || load_q(1)) && load_kv(&tm_v, w.first);
-        for (int t = w.next(taken, w.first); t < w.end && ok; t = w.next(taken, t)) ok = load_kv(&tm_k, t) && load_kv(&tm_v, t);
+        ok = load_kv(&tm_k, w, w.first) && load_kv(&tm_v, w, w.first) && ask();
+        for (int t = w.next(taken, w.first); t < w.end && ok; t = w.next(taken, t)) ok = load_kv(&tm_k, w, t) && load_kv(&tm_v, w, t);
       }
       if (lane == 0) {  // the copies land before the CTA may leave
         auto landed = [&](uint64_t& b, uint32_t parity) {
@@ -181,9 +207,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
         };
-        for (int s = 0; s < kStages; ++s)
-          if ((used >> s) & 1u) landed(bars->full[s], (last_phase >> s) & 1u);
-        for (int x = 0; x < 2; ++x)
+        for (uint32_t p = pos > kStages ? pos - kStages : 0; p < pos; ++p) landed(bars->full[p % kStages], (p / kStages) & 1u);
+        for (int x = 0; x < 4; ++x)
           if (q_uses[x] > 0) landed(bars->q_full[x], (q_uses[x] - 1) & 1u);
       }
     } else if (warp == 1) {
@@ -192,73 +217,67 @@ __global__ void __launch_bounds__(kThreads, 1)
       constexpr uint32_t s_idesc = umma_idesc_f16(kFormat, false, kTile, kTile);
       constexpr uint32_t o_idesc = umma_idesc_f16(kFormat, true, kTile, kD);
       const uint64_t q_desc = by_rows_desc(base), k_desc = by_rows_desc(ring), v_desc = by_columns_desc(ring);
-      uint32_t pos = 0, q_uses[2] = {0, 0}, p_uses[2] = {0, 0}, o_uses[2] = {0, 0};
+      uint32_t pos = 0, units = 0, q_uses[4] = {0, 0, 0, 0}, p_uses[2] = {0, 0}, o_uses[2] = {0, 0};
       bool ok = true, issued = false;
-      auto wait = [&](uint64_t& b, uint32_t parity) {
-        return wait_together(bar(b), parity, abort_flag, args.status, MOSS_STATUS_TIMEOUT_MMA);
-      };
       for (int u = blockIdx.x; u < num_units && ok; u += gridDim.x) {
         Unit w;
         if (!locate(args, taken, u, w) || w.first == w.end) continue;
         const int tiles = w.tiles();
-        int following = w.next(taken, w.first);  // the key tile after the one at hand
-        // S of tile x against the key tile at ring position p
-        auto scores = [&](int x, uint32_t p, bool last) {
-          if (elect_one()) {
-            mma_over_head<kD>(tmem + x * kTile, q_desc + ((x * kTileBytes) >> 4),
+        int n = 0;
+        for (int t = w.first; t < w.end; t = w.next(taken, t)) ++n;
+        const uint32_t q_slot = (units & 1u) * 2;
+        issued = true;
+        // One thread waits and issues for the whole unit: with the warp's waits and elections between the products their issue
+        // took 4400 cycles a pair of tiles, and the products 2400.
+        if (elect_one()) {
+          auto wait = [&](uint64_t& b, uint32_t parity) {
+            ok = ok && mbar_poll(bar(b), parity & 1u, abort_flag, args.status, MOSS_STATUS_TIMEOUT_MMA);
+            tc_fence_after();
+            return ok;
+          };
+          // S of tile x against the key tile at ring position p
+          auto scores = [&](int x, uint32_t p) {
+            mma_over_head<kD>(tmem + x * kTile, q_desc + (((q_slot + x) * kTileBytes) >> 4),
                               k_desc + (((p % kStages) * kTileBytes) >> 4), s_idesc);
             umma_commit(bar(bars->s_full[x]));
-            if (last) umma_commit(bar(bars->q_empty[x]));
-          }
-          issued = true;
-          __syncwarp();
-        };
-        auto release = [&](uint32_t p) {
-          if (elect_one()) umma_commit(bar(bars->empty[p % kStages]));
-          __syncwarp();
-        };
-        ok = wait(bars->full[pos % kStages], (pos / kStages) & 1u);
-        for (int x = 0; x < tiles && ok; ++x) {
-          ok = wait(bars->q_full[x], q_uses[x]++ & 1u);
-          if (!ok) break;
-          tc_fence_after();
-          scores(x, pos, following >= w.end);
-        }
-        if (!ok) break;
-        release(pos);
-        bool begun = false;
-        while (ok) {
-          const bool more = following < w.end;
-          const int then = more ? w.next(taken, following) : w.end;
-          const uint32_t pv = pos + 1, pk = pos + 2;
-          const uint32_t nth = pos / 2;  // of the V tiles: what `clean` counts
-          ok = kMask ? wait(bars->clean[nth % kStages], (nth / kStages) & 1u) : wait(bars->full[pv % kStages], (pv / kStages) & 1u);
+          };
+          wait(bars->full[pos % kStages], pos / kStages);
           for (int x = 0; x < tiles && ok; ++x) {
-            if (!begun) ok = wait(bars->o_free[x], (o_uses[x]++ & 1u) ^ 1u);
-            ok = ok && wait(bars->p_ready[x], p_uses[x]++ & 1u);
-            if (!ok) break;
-            tc_fence_after();
-            if (elect_one()) {
-              mma_over_rows(tmem + 2 * kTile + x * kTile, tmem + x * kTile, v_desc + (((pv % kStages) * kTileBytes) >> 4),
-                            o_idesc, begun);
-              if (!more) umma_commit(bar(bars->o_full[x]));
-            }
-            __syncwarp();
-            if (more) {
-              if (x == 0) ok = wait(bars->full[pk % kStages], (pk / kStages) & 1u);
-              if (!ok) break;
-              tc_fence_after();
-              scores(x, pk, then >= w.end);
-            }
+            if (wait(bars->q_full[q_slot + x], q_uses[q_slot + x])) scores(x, pos);
           }
-          if (!ok) break;
-          release(pv);
-          pos += 2;
-          if (!more) break;
-          release(pk);
-          begun = true;
-          following = then;
+          if (ok) umma_commit(bar(bars->empty[pos % kStages]));
+          for (int i = 0; i < n && ok; ++i) {
+            const uint32_t pv = pos + 2 * i + 1, pk = pv + 1;
+            const bool more = i + 1 < n;
+            const uint32_t nth = pos / 2 + i;  // of the V tiles: what `clean` counts
+            if (kMask)
+              wait(bars->clean[nth % kStages], nth / kStages);
+            else
+              wait(bars->full[pv % kStages], pv / kStages);
+            if (more) wait(bars->full[pk % kStages], pk / kStages);
+            for (int x = 0; x < tiles && ok; ++x) {
+              if (i == 0) wait(bars->o_free[x], o_uses[x] ^ 1u);
+              if (!wait(bars->p_ready[x], p_uses[x] + i)) break;
+              mma_over_rows(tmem + 2 * kTile + x * kTile, tmem + x * kTile, v_desc + (((pv % kStages) * kTileBytes) >> 4),
+                            o_idesc, i > 0);
+              if (more)
+                scores(x, pk);
+              else
+                umma_commit(bar(bars->o_full[x]));
+            }
+            if (!ok) break;
+            umma_commit(bar(bars->empty[pv % kStages]));
+            if (more) umma_commit(bar(bars->empty[pk % kStages]));
+          }
         }
+        ok = __all_sync(0xffffffffu, ok) != 0;
+        for (int x = 0; x < tiles; ++x) {
+          ++q_uses[q_slot + x];
+          ++o_uses[x];
+          p_uses[x] += n;
+        }
+        ++units;
+        pos += 2 * n;
       }
       if (lane == 0 && issued) {
         umma_commit(bar(bars->drain));
@@ -287,6 +306,32 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (lane == 0) mbar_arrive(bar(bars->clean[(pos / 2) % kStages]));
         }
       }
+    } else if (warp == 3) {
+      // ---------------------------------------------------------------- stores (an own warp: their queue takes 1500 cycles a tile)
+      uint32_t units = 0, uses[2] = {0, 0};
+      bool ok = true;
+      for (int u = blockIdx.x; u < num_units && ok; u += gridDim.x) {
+        Unit w;
+        if (!locate(args, taken, u, w) || w.first == w.end) continue;
+        for (int x = 0; x < w.tiles() && ok; ++x) {
+          const uint32_t slot = (units & 1u) * 2 + x;
+          ok = wait_suspended(bar(bars->out_full[x]), uses[x]++ & 1u, abort_flag, args.status, MOSS_STATUS_TIMEOUT_EPILOGUE);
+          if (!ok) break;
+          if (lane == 0) {
+            if (leaves_by_tma<kMask>(args, w, x)) {
+#pragma unroll
+              for (int c = 0; c < kD / 64; ++c)
+                tma_store_4d(&tm_out, base + slot * kTileBytes + c * 16384, c * 64, w.s.q0 + w.row + x * kTile, w.head, w.s.entry);
+              bulk_commit();
+              bulk_wait_read();
+            }
+            mbar_arrive(bar(bars->q_empty[slot]));
+          }
+          __syncwarp();
+        }
+        ++units;
+      }
+      if (lane == 0) bulk_wait();
     }
   } else {
     // ---------------------------------------------------------------- softmax and output
@@ -296,11 +341,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t s_tmem = tmem + x * kTile + lanes, o_tmem = tmem + 2 * kTile + x * kTile + lanes;
     const bool wide = args.head_dim % 16 == 0 && (reinterpret_cast<uintptr_t>(args.out) & 31) == 0;
-    uint32_t s_uses = 0, o_uses = 0;
+    uint32_t s_uses = 0, o_uses = 0, units = 0;
     bool ok = true;
     for (int u = blockIdx.x; u < num_units && ok; u += gridDim.x) {
       Unit w;
-      if (!locate(args, taken, u, w) || x >= w.tiles()) continue;
+      if (!locate(args, taken, u, w)) continue;
+      const bool any_keys = w.first < w.end;
+      const uint32_t slot = (units & 1u) * 2 + x;
+      if (any_keys) ++units;
+      if (x >= w.tiles()) continue;
       const int at = w.row + x * kTile + row;  // within the sequence
       const int64_t q_row = w.s.q_row + at;
       const bool live = at < w.s.qn;
@@ -381,10 +430,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         sum += (add[0] + add[1]) + (add[2] + add[3]);
         tmem_wait_st();
         tc_fence_before();
-        mbar_arrive(bar(bars->p_ready[x]));
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(bars->p_ready[x]));
       }
       if (!ok) break;
-      const bool any_keys = w.first < w.end;
       if (any_keys) {
         ok = wait_together(bar(bars->o_full[x]), o_uses++ & 1u, abort_flag, args.status, MOSS_STATUS_TIMEOUT_EPILOGUE);
         if (!ok) break;
@@ -392,6 +441,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
       const int64_t at_out = (q_row * args.q_heads + w.head) * args.head_dim;
+      const bool by_tma = any_keys && leaves_by_tma<kMask>(args, w, x);
+      const uint32_t staged = base + slot * kTileBytes + row * 128;
 #pragma unroll
       for (int c = 0; c < kD / 32; ++c) {
         uint32_t o[32];
@@ -402,19 +453,31 @@ __global__ void __launch_bounds__(kThreads, 1)
           wait_ld_of(o);
           if (c == kD / 32 - 1) {
             tc_fence_before();
-            mbar_arrive(bar(bars->o_free[x]));
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(bars->o_free[x]));
           }
         }
         // (a row whose keys are all masked has zeros in O, and an empty one nothing)
 #pragma unroll
         for (int j = 0; j < 32; ++j) v[j] = any_keys ? __uint_as_float(o[j]) * inverse : 0.0f;
         const int count = args.head_dim - c * 32;
-        if (live && count > 0) {
+        if (by_tma) {
+#pragma unroll
+          for (int h = 0; h < 4; ++h)
+            gemm::sts128(staged + (c >> 1) * 16384 + ((((c & 1) * 4 + h) ^ (row & 7)) << 4),
+                         make_uint4(gemm::pack2_kind<kKind>(v[8 * h], v[8 * h + 1]), gemm::pack2_kind<kKind>(v[8 * h + 2], v[8 * h + 3]),
+                                    gemm::pack2_kind<kKind>(v[8 * h + 4], v[8 * h + 5]), gemm::pack2_kind<kKind>(v[8 * h + 6], v[8 * h + 7])));
+        } else if (live && count > 0) {
           if (args.splits > 1)
             store_row32_f32(args.partial + w.split * args.q_rows * args.q_heads * args.head_dim + at_out + c * 32, count, v);
           else
             store_row32<kKind>(static_cast<uint16_t*>(args.out) + at_out + c * 32, wide, count, v);
         }
+      }
+      if (any_keys) {
+        if (by_tma) fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(bars->out_full[x]));
       }
       if (live) {
         const float l = sum == 0.0f ? -INFINITY : top - kLift<kKind> + log2f(sum);
@@ -444,7 +507,7 @@ int launch_typed(const Maps& maps, const Args& a, cudaStream_t stream) {
   if (rc != MOSS_OK) return rc;
   const int64_t units = static_cast<int64_t>(a.tiles) * a.splits * a.q_heads;
   const unsigned grid = static_cast<unsigned>(std::min<int64_t>(units, device_sm_count()));
-  kern<<<grid, kThreads, Shape<kD>::kSmemBytes, stream>>>(maps.q, maps.k, maps.v, a);
+  kern<<<grid, kThreads, Shape<kD>::kSmemBytes, stream>>>(maps.q, maps.k, maps.v, maps.grad, a);
   return check_cuda(cudaGetLastError(), "cross_forward_kernel");
 }
 
