@@ -218,10 +218,10 @@ __device__ __forceinline__ void mma_over_head(uint32_t d, uint64_t a_desc, uint6
     umma_f16(d, a_desc + at, b_desc + at, idesc, kk > 0 ? 1u : 0u);
   }
 }
-// 128 x kD products over a tile's 128 rows: A in TMEM, B by columns.
-__device__ __forceinline__ void mma_over_rows(uint32_t d, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, bool accumulate) {
+// 128 x kD products over 64 of a tile's rows: A in TMEM, B by columns.
+__device__ __forceinline__ void mma_over_keys(uint32_t d, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, bool accumulate) {
 #pragma unroll
-  for (int kk = 0; kk < kTile / 16; ++kk)
+  for (int kk = 0; kk < kTile / 2 / 16; ++kk)
     umma_f16_ts(d, a_tmem + kk * 8, b_desc + kk * (2048 >> 4), idesc, accumulate || kk > 0 ? 1u : 0u);
 }
 __device__ __forceinline__ uint64_t by_rows_desc(uint32_t tile) { return umma_desc_sw128(tile, 16, 1024); }

@@ -7,7 +7,8 @@
 // its exponentials are taken against (P up to 256 loses nothing: its sum is f32, and 16-bit rounding is relative).
 // The CTAs are persistent: the next pair's loads and first S run during the last tile's softmax.
 //
-// Warps: 0 loads by TMA, 1 issues the MMAs, 2 zeroes masked rows of V (0 * NaN is NaN), 3 stores, 4-7 and 8-11 the softmax.
+// Warps: 0 loads by TMA, 1 and 3 issue the MMAs of a query tile each, 2 zeroes masked rows of V (0 * NaN is NaN) and stores,
+// 4-7 and 8-11 do the softmax.
 //
 // P is rounded to the inputs' 16-bit type (half a step of each term; the sum it is divided by is of the unrounded values).
 #include <algorithm>
@@ -23,6 +24,7 @@ namespace {
 constexpr int kThreads = 384;
 constexpr int kMiscRegs = 88, kSoftmaxRegs = 208;
 static_assert(kMiscRegs + 2 * kSoftmaxRegs <= 3 * 168, "a larger split would wait forever");
+constexpr int kHalf = kTile / 2;  // keys of one step
 constexpr float kGrowth = 8.0f;
 // f16 has no normal values below 2^-14: there the exponentials are 2^7 larger (up to 2^15 with kGrowth), which their sum is too.
 template <int kKind>
@@ -42,11 +44,12 @@ struct Barriers {
   uint64_t q_full[4], q_empty[4];  // by pair (they take turns) and tile
   uint64_t full[kMaxStages], empty[kMaxStages];
   uint64_t clean[kMaxStages];  // masked rows of the n-th V tile are zero (n modulo the stages)
-  uint64_t s_full[2];          // S is there (and the last product with P is done)
-  uint64_t p_ready[2];         // P is there, O may be added to
+  uint64_t s_full[2][2];       // by query tile and buffer: S is there
+  uint64_t p_ready[2][2];      // P is there, O may be added to
+  uint64_t pv_done[2];         // a product with P is done
   uint64_t o_full[2], o_free[2];
   uint64_t out_full[2];        // the results are in shared memory
-  uint64_t drain;
+  uint64_t drain[2];
   uint32_t tile_bits[kMaxTileBits / 32];
   uint32_t tmem_base;
   int abort_flag;
@@ -59,6 +62,8 @@ struct Unit {
   int head, split, row, first, end;  // row: the pair's first within the sequence
   __device__ __forceinline__ int tiles() const { return s.qn - row > kTile ? 2 : 1; }
   __device__ __forceinline__ int next(const TileBits& taken, int t) const { return taken.next(s.entry, t + 1, end); }
+  // the halves of key tile t that hold keys
+  __device__ __forceinline__ int halves(int t) const { return s.kn - t * kTile > kHalf ? 2 : 1; }
 };
 __device__ __forceinline__ bool locate(const Args& a, const TileBits& taken, int u, Unit& unit) {
   const int t = u % a.tiles, rest = u / a.tiles;
@@ -108,18 +113,21 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(bar(bars->q_empty[x]), 1);
     }
     for (int x = 0; x < 2; ++x) {
-      mbar_init(bar(bars->s_full[x]), 1);
-      mbar_init(bar(bars->p_ready[x]), 4);
+      for (int b = 0; b < 2; ++b) {
+        mbar_init(bar(bars->s_full[x][b]), 1);
+        mbar_init(bar(bars->p_ready[x][b]), 4);
+      }
+      mbar_init(bar(bars->pv_done[x]), 1);
       mbar_init(bar(bars->o_full[x]), 1);
       mbar_init(bar(bars->o_free[x]), 4);
       mbar_init(bar(bars->out_full[x]), 4);
     }
     for (int s = 0; s < kStages; ++s) {
       mbar_init(bar(bars->full[s]), 1);
-      mbar_init(bar(bars->empty[s]), 1);
+      mbar_init(bar(bars->empty[s]), 2);
       mbar_init(bar(bars->clean[s]), 1);
     }
-    mbar_init(bar(bars->drain), 1);
+    for (int x = 0; x < 2; ++x) mbar_init(bar(bars->drain[x]), 1);
     bars->abort_flag = 0;
     for (int i = 0; i < kMaxTileBits / 32; ++i) bars->tile_bits[i] = 0;
     fence_mbar_init();
@@ -138,7 +146,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   tc_fence_after();
   const TileBits taken{use_bits ? bars->tile_bits : nullptr, key_tiles};
-  const uint32_t tmem = bars->tmem_base;  // S (and P) of the two tiles, then O of the two tiles
+  // for each of the two query tiles: S (and P) of two halves of key tiles, then O
+  const uint32_t tmem = bars->tmem_base;
 
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kMiscRegs));
@@ -211,78 +220,87 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int x = 0; x < 4; ++x)
           if (q_uses[x] > 0) landed(bars->q_full[x], (q_uses[x] - 1) & 1u);
       }
-    } else if (warp == 1) {
-      // ---------------------------------------------------------------- MMAs
+    } else if (warp == 1 || warp == 3) {
+      // ---------------------------------------------------------------- MMAs, a warp for each query tile
+      // (One for both issued too slowly: each wait costs it 200 cycles, of the 1000 that the products of half a tile take.)
+      const int x = warp >> 1;
       constexpr uint32_t kFormat = kKind == kBF16 ? 1u : 0u;
-      constexpr uint32_t s_idesc = umma_idesc_f16(kFormat, false, kTile, kTile);
+      constexpr uint32_t s_idesc = umma_idesc_f16(kFormat, false, kTile, kHalf);
       constexpr uint32_t o_idesc = umma_idesc_f16(kFormat, true, kTile, kD);
       const uint64_t q_desc = by_rows_desc(base), k_desc = by_rows_desc(ring), v_desc = by_columns_desc(ring);
-      uint32_t pos = 0, units = 0, q_uses[4] = {0, 0, 0, 0}, p_uses[2] = {0, 0}, o_uses[2] = {0, 0};
+      const uint32_t s_tmem = tmem + x * 2 * kTile, o_tmem = s_tmem + kTile;
+      uint32_t pos = 0, units = 0, q_uses[2] = {0, 0}, steps = 0, o_uses = 0;
       bool ok = true, issued = false;
       for (int u = blockIdx.x; u < num_units && ok; u += gridDim.x) {
         Unit w;
         if (!locate(args, taken, u, w) || w.first == w.end) continue;
-        const int tiles = w.tiles();
-        int n = 0;
-        for (int t = w.first; t < w.end; t = w.next(taken, t)) ++n;
-        const uint32_t q_slot = (units & 1u) * 2;
-        issued = true;
-        // One thread waits and issues for the whole unit: with the warp's waits and elections between the products their issue
-        // took 4400 cycles a pair of tiles, and the products 2400.
+        int n = 0, m = 0;  // key tiles, and halves of them: only the last tile may have one
+        for (int t = w.first; t < w.end; t = w.next(taken, t)) {
+          ++n;
+          m += w.halves(t);
+        }
+        const uint32_t q_slot = (units & 1u) * 2 + x;
+        // one thread waits and issues for the whole unit
         if (elect_one()) {
           auto wait = [&](uint64_t& b, uint32_t parity) {
             ok = ok && mbar_poll(bar(b), parity & 1u, abort_flag, args.status, MOSS_STATUS_TIMEOUT_MMA);
-            tc_fence_after();
             return ok;
           };
-          // S of tile x against the key tile at ring position p
-          auto scores = [&](int x, uint32_t p) {
-            mma_over_head<kD>(tmem + x * kTile, q_desc + (((q_slot + x) * kTileBytes) >> 4),
-                              k_desc + (((p % kStages) * kTileBytes) >> 4), s_idesc);
-            umma_commit(bar(bars->s_full[x]));
-          };
-          wait(bars->full[pos % kStages], pos / kStages);
-          for (int x = 0; x < tiles && ok; ++x) {
-            if (wait(bars->q_full[q_slot + x], q_uses[q_slot + x])) scores(x, pos);
-          }
-          if (ok) umma_commit(bar(bars->empty[pos % kStages]));
-          for (int i = 0; i < n && ok; ++i) {
-            const uint32_t pv = pos + 2 * i + 1, pk = pv + 1;
-            const bool more = i + 1 < n;
-            const uint32_t nth = pos / 2 + i;  // of the V tiles: what `clean` counts
-            if (kMask)
-              wait(bars->clean[nth % kStages], nth / kStages);
-            else
-              wait(bars->full[pv % kStages], pv / kStages);
-            if (more) wait(bars->full[pk % kStages], pk / kStages);
-            for (int x = 0; x < tiles && ok; ++x) {
-              if (i == 0) wait(bars->o_free[x], o_uses[x] ^ 1u);
-              if (!wait(bars->p_ready[x], p_uses[x] + i)) break;
-              mma_over_rows(tmem + 2 * kTile + x * kTile, tmem + x * kTile, v_desc + (((pv % kStages) * kTileBytes) >> 4),
-                            o_idesc, i > 0);
-              if (more)
-                scores(x, pk);
-              else
-                umma_commit(bar(bars->o_full[x]));
+          auto there = [&](uint32_t p) { return wait(bars->full[p % kStages], p / kStages); };
+          auto release = [&](uint32_t p) { umma_commit(bar(bars->empty[p % kStages])); };
+          if (x >= w.tiles()) {  // the other warp's keys and values pass by
+            for (int i = 0; i < 2 * n && there(pos + i); ++i) mbar_arrive(bar(bars->empty[(pos + i) % kStages]));
+          } else {
+            // S against half j of the unit's key tiles
+            auto scores = [&](int j) {
+              const uint32_t g = steps + j, p = pos + (j & ~1);
+              tc_fence_after();
+              mma_over_head<kD>(s_tmem + (g & 1u) * kHalf, q_desc + ((q_slot * kTileBytes) >> 4),
+                                k_desc + (((p % kStages) * kTileBytes + (j & 1) * kHalf * 128) >> 4), s_idesc);
+              umma_commit(bar(bars->s_full[x][g & 1u]));
+            };
+            if (there(pos) && wait(bars->q_full[q_slot], q_uses[units & 1u])) {
+              scores(0);
+              if (m > 1) scores(1);
+              release(pos);
+              wait(bars->o_free[x], o_uses ^ 1u);
             }
-            if (!ok) break;
-            umma_commit(bar(bars->empty[pv % kStages]));
-            if (more) umma_commit(bar(bars->empty[pk % kStages]));
+            for (int j = 0; j < m && ok; ++j) {
+              const uint32_t pv = pos + (j & ~1) + 1;  // of V; the next tile's K is behind it
+              const uint32_t g = steps + j;
+              if ((j & 1) == 0) {
+                const uint32_t nth = pv / 2;  // of the V tiles: what `clean` counts
+                if (!(kMask ? wait(bars->clean[nth % kStages], nth / kStages) : there(pv))) break;
+              }
+              if (!wait(bars->p_ready[x][g & 1u], g >> 1)) break;
+              tc_fence_after();
+              mma_over_keys(o_tmem, s_tmem + (g & 1u) * kHalf, v_desc + (((pv % kStages) * kTileBytes + (j & 1) * kHalf * 128) >> 4),
+                            o_idesc, j > 0);
+              umma_commit(bar(j + 1 < m ? bars->pv_done[x] : bars->o_full[x]));
+              const bool last_half = (j & 1) == 1;
+              if (last_half || j + 1 == m) release(pv);
+              if (j + 2 < m) {
+                if (!last_half && !there(pv + 1)) break;
+                scores(j + 2);
+                if (last_half || j + 3 == m) release(pv + 1);
+              }
+            }
           }
         }
         ok = __all_sync(0xffffffffu, ok) != 0;
-        for (int x = 0; x < tiles; ++x) {
-          ++q_uses[q_slot + x];
-          ++o_uses[x];
-          p_uses[x] += n;
+        if (x < w.tiles()) {
+          issued = true;
+          ++q_uses[units & 1u];
+          ++o_uses;
+          steps += m;
         }
         ++units;
         pos += 2 * n;
       }
       if (lane == 0 && issued) {
-        umma_commit(bar(bars->drain));
+        umma_commit(bar(bars->drain[x]));
         const long long start = clock64();
-        while (!mbar_try_wait(bar(bars->drain), 0)) {
+        while (!mbar_try_wait(bar(bars->drain[x]), 0)) {
           if (clock64() - start > kWaitBudgetCycles) {
             report_status(args.status, MOSS_STATUS_TIMEOUT_DRAIN);
             break;
@@ -290,29 +308,24 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       __syncwarp();
-    } else if (kMask && warp == 2) {
-      // ---------------------------------------------------------------- masked rows of V
-      uint32_t pos = 0;
+    } else {
+      // ---------------------------------------------------------------- masked rows of V, and the stores (which a softmax warp
+      // would wait 1500 cycles a tile for)
+      uint32_t pos = 0, units = 0, uses[2] = {0, 0};
       bool ok = true;
       for (int u = blockIdx.x; u < num_units && ok; u += gridDim.x) {
         Unit w;
         if (!locate(args, taken, u, w) || w.first == w.end) continue;
-        for (int t = w.first; t < w.end; t = w.next(taken, t), pos += 2) {
-          const KeyBits keep = key_bits(args, w.s, t * kTile);
-          const uint32_t stage = (pos + 1) % kStages, phase = ((pos + 1) / kStages) & 1u;
-          ok = wait_together(bar(bars->full[stage]), phase, abort_flag, args.status, MOSS_STATUS_TIMEOUT_LOAD);
-          if (!ok) break;
-          if (!keep.all()) scrub_rows<kD>(ring + stage * kTileBytes, keep);
-          if (lane == 0) mbar_arrive(bar(bars->clean[(pos / 2) % kStages]));
+        if constexpr (kMask) {
+          for (int t = w.first; t < w.end; t = w.next(taken, t), pos += 2) {
+            const KeyBits keep = key_bits(args, w.s, t * kTile);
+            const uint32_t stage = (pos + 1) % kStages, phase = ((pos + 1) / kStages) & 1u;
+            ok = wait_together(bar(bars->full[stage]), phase, abort_flag, args.status, MOSS_STATUS_TIMEOUT_LOAD);
+            if (!ok) break;
+            if (!keep.all()) scrub_rows<kD>(ring + stage * kTileBytes, keep);
+            if (lane == 0) mbar_arrive(bar(bars->clean[(pos / 2) % kStages]));
+          }
         }
-      }
-    } else if (warp == 3) {
-      // ---------------------------------------------------------------- stores (an own warp: their queue takes 1500 cycles a tile)
-      uint32_t units = 0, uses[2] = {0, 0};
-      bool ok = true;
-      for (int u = blockIdx.x; u < num_units && ok; u += gridDim.x) {
-        Unit w;
-        if (!locate(args, taken, u, w) || w.first == w.end) continue;
         for (int x = 0; x < w.tiles() && ok; ++x) {
           const uint32_t slot = (units & 1u) * 2 + x;
           ok = wait_suspended(bar(bars->out_full[x]), uses[x]++ & 1u, abort_flag, args.status, MOSS_STATUS_TIMEOUT_EPILOGUE);
@@ -339,9 +352,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int x = (warp - 4) >> 2;
     const int row = (warp & 3) * 32 + lane;
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const uint32_t s_tmem = tmem + x * kTile + lanes, o_tmem = tmem + 2 * kTile + x * kTile + lanes;
+    const uint32_t tile_tmem = tmem + x * 2 * kTile + lanes, o_tmem = tile_tmem + kTile;
     const bool wide = args.head_dim % 16 == 0 && (reinterpret_cast<uintptr_t>(args.out) & 31) == 0;
-    uint32_t s_uses = 0, o_uses = 0, units = 0;
+    uint32_t step = 0, products = 0, o_uses = 0, units = 0;
     bool ok = true;
     for (int u = blockIdx.x; u < num_units && ok; u += gridDim.x) {
       Unit w;
@@ -354,86 +367,92 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int64_t q_row = w.s.q_row + at;
       const bool live = at < w.s.qn;
       float top = -INFINITY, sum = 0.0f;  // the exponentials' reference, times scale_log2
-      for (int t = w.first; t < w.end; t = w.next(taken, t)) {
+      bool begun = false;
+      for (int t = w.first; t < w.end && ok; t = w.next(taken, t)) {
         KeyBits keep;
-        const int keys = w.s.kn - t * kTile;
         if constexpr (kMask) keep = key_bits(args, w.s, t * kTile);
-        ok = wait_together(bar(bars->s_full[x]), s_uses++ & 1u, abort_flag, args.status, MOSS_STATUS_TIMEOUT_EPILOGUE);
-        if (!ok) break;
-        tc_fence_after();
-        uint32_t r[4][32];
+        const int halves = w.halves(t);
+#pragma unroll 1
+        for (int half = 0; half < halves; ++half, ++step) {
+          const int keys = w.s.kn - t * kTile - half * kHalf;
+          const uint32_t s_tmem = tile_tmem + (step & 1u) * kHalf;
+          ok = wait_together(bar(bars->s_full[x][step & 1u]), (step >> 1) & 1u, abort_flag, args.status, MOSS_STATUS_TIMEOUT_EPILOGUE);
+          if (!ok) break;
+          tc_fence_after();
+          uint32_t r[2][32];
+          tmem_ld_32x32b_x32(s_tmem, r[0]);
+          tmem_ld_32x32b_x32(s_tmem + 32, r[1]);
+          wait_ld_of(r[0]);
+          wait_ld_of(r[1]);
+          if constexpr (kMask) {
+            const uint32_t k0 = half == 0 ? keep.w[0] : keep.w[2], k1 = half == 0 ? keep.w[1] : keep.w[3];
+            if ((k0 & k1) != 0xffffffffu) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32(s_tmem + c * 32, r[c]);
-#pragma unroll
-        for (int c = 0; c < 4; ++c) wait_ld_of(r[c]);
-        if constexpr (kMask) {
-          if (!keep.all()) {
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-#pragma unroll
-              for (int j = 0; j < 32; ++j)
-                if (((keep.w[c] >> j) & 1u) == 0) r[c][j] = 0xff800000u;
-            }
-          }
-        } else if (keys < kTile) {
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-#pragma unroll
-            for (int j = 0; j < 32; ++j)
-              if (c * 32 + j >= keys) r[c][j] = 0xff800000u;
-          }
-        }
-        float most[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-        for (int j = 0; j < 32; ++j) {
-#pragma unroll
-          for (int c = 0; c < 4; ++c) most[c] = fmaxf(most[c], __uint_as_float(r[c][j]));
-        }
-        // (the scale is positive, so the greatest product gives the greatest logit)
-        const float here = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])) * args.scale_log2;
-        const bool grows = here > top + kGrowth;  // (from -inf always, unless the tile is masked)
-        if (__any_sync(0xffffffffu, grows)) {
-          const float factor = grows ? exp2_approx(top - here) : 1.0f;
-          if (grows) top = here;
-          sum *= factor;
-          if (t > w.first) {
-#pragma unroll
-            for (int c = 0; c < kD / 32; ++c) {
-              uint32_t o[32];
-              tmem_ld_32x32b_x32(o_tmem + c * 32, o);
-              wait_ld_of(o);
-              uint32_t lo[16], hi[16];
-#pragma unroll
-              for (int j = 0; j < 16; ++j) {
-                lo[j] = __float_as_uint(__uint_as_float(o[j]) * factor);
-                hi[j] = __float_as_uint(__uint_as_float(o[16 + j]) * factor);
+              for (int j = 0; j < 32; ++j) {
+                if (((k0 >> j) & 1u) == 0) r[0][j] = 0xff800000u;
+                if (((k1 >> j) & 1u) == 0) r[1][j] = 0xff800000u;
               }
-              tmem_st_32x32b_x16(o_tmem + c * 32, lo);
-              tmem_st_32x32b_x16(o_tmem + c * 32 + 16, hi);
+            }
+          } else if (keys < kHalf) {
+#pragma unroll
+            for (int j = 0; j < 64; ++j)
+              if (j >= keys) r[j >> 5][j & 31] = 0xff800000u;
+          }
+          float most[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int j = 0; j < 64; ++j) most[j & 3] = fmaxf(most[j & 3], __uint_as_float(r[j >> 5][j & 31]));
+          // (the scale is positive, so the greatest product gives the greatest logit)
+          const float here = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])) * args.scale_log2;
+          const bool grows = here > top + kGrowth;  // (from -inf always, unless all keys are masked)
+          if (__any_sync(0xffffffffu, grows)) {
+            const float factor = grows ? exp2_approx(top - here) : 1.0f;
+            if (grows) top = here;
+            sum *= factor;
+            if (begun) {  // the last product has to be done before its sums are touched
+              ok = wait_together(bar(bars->pv_done[x]), (products - 1) & 1u, abort_flag, args.status, MOSS_STATUS_TIMEOUT_EPILOGUE);
+              if (!ok) break;
+              tc_fence_after();
+#pragma unroll
+              for (int c = 0; c < kD / 32; ++c) {
+                uint32_t o[32];
+                tmem_ld_32x32b_x32(o_tmem + c * 32, o);
+                wait_ld_of(o);
+                uint32_t lo[16], hi[16];
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                  lo[j] = __float_as_uint(__uint_as_float(o[j]) * factor);
+                  hi[j] = __float_as_uint(__uint_as_float(o[16 + j]) * factor);
+                }
+                tmem_st_32x32b_x16(o_tmem + c * 32, lo);
+                tmem_st_32x32b_x16(o_tmem + c * 32 + 16, hi);
+              }
             }
           }
-        }
-        const float shift = top == -INFINITY ? 0.0f : top - kLift<kKind>;
-        float add[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+          const float shift = top == -INFINITY ? 0.0f : top - kLift<kKind>;
+          float add[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t p[16];
+          for (int c = 0; c < 2; ++c) {
+            uint32_t p[16];
 #pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            const float e0 = exp2_approx(fmaf(__uint_as_float(r[c][2 * j]), args.scale_log2, -shift));
-            const float e1 = exp2_approx(fmaf(__uint_as_float(r[c][2 * j + 1]), args.scale_log2, -shift));
-            add[j & 3] += e0 + e1;
-            p[j] = gemm::pack2_kind<kKind>(e0, e1);
+            for (int j = 0; j < 16; ++j) {
+              const float e0 = exp2_approx(fmaf(__uint_as_float(r[c][2 * j]), args.scale_log2, -shift));
+              const float e1 = exp2_approx(fmaf(__uint_as_float(r[c][2 * j + 1]), args.scale_log2, -shift));
+              add[j & 3] += e0 + e1;
+              p[j] = gemm::pack2_kind<kKind>(e0, e1);
+            }
+            tmem_st_32x32b_x16(s_tmem + c * 16, p);
           }
-          tmem_st_32x32b_x16(s_tmem + c * 16, p);
+          sum += (add[0] + add[1]) + (add[2] + add[3]);
+          tmem_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar(bars->p_ready[x][step & 1u]));
+          begun = true;
+          ++products;
         }
-        sum += (add[0] + add[1]) + (add[2] + add[3]);
-        tmem_wait_st();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar(bars->p_ready[x]));
       }
       if (!ok) break;
+      if (begun) --products;  // the unit's last product is told by o_full
       if (any_keys) {
         ok = wait_together(bar(bars->o_full[x]), o_uses++ & 1u, abort_flag, args.status, MOSS_STATUS_TIMEOUT_EPILOGUE);
         if (!ok) break;
