@@ -22,6 +22,7 @@ namespace cross {
 namespace {
 
 constexpr int kThreads = 384;
+constexpr int kMathWarps = 8;
 constexpr int kMiscRegs = 72, kMathRegs = 216;
 static_assert(kMiscRegs + 2 * kMathRegs <= 3 * 168, "a larger split would wait forever");
 constexpr int kHalf = kTile / 2;  // columns of one warpgroup
@@ -56,7 +57,7 @@ struct Barriers {
 };
 static_assert(sizeof(Barriers) <= 512, "barrier block too large");
 
-__device__ __forceinline__ void init_barriers(Barriers* bars, int stages, int stats) {
+__device__ __forceinline__ void init_barriers(Barriers* bars, int stages, int stats, int stat_writers) {
   auto init = [](uint64_t& b, uint32_t n) { mbar_init(smem_u32(&b), n); };
   init(bars->held_full, 1);
   init(bars->held_empty, 1);
@@ -66,15 +67,15 @@ __device__ __forceinline__ void init_barriers(Barriers* bars, int stages, int st
     init(bars->clean[s], 1);
   }
   for (int s = 0; s < stats; ++s) {
-    init(bars->stat_full[s], 1);
-    init(bars->stat_free[s], 2 * kTile);
+    init(bars->stat_full[s], stat_writers);
+    init(bars->stat_free[s], kMathWarps);
   }
   init(bars->s_full, 1);
   init(bars->dp_full, 1);
-  init(bars->p_ready, 2 * kTile);
-  init(bars->ds_ready, 2 * kTile);
+  init(bars->p_ready, kMathWarps);
+  init(bars->ds_ready, kMathWarps);
   init(bars->acc_full, 1);
-  init(bars->acc_free, 2 * kTile);
+  init(bars->acc_free, kMathWarps);
   init(bars->drain, 1);
   for (int i = 0; i < kMaxTileBits / 32; ++i) bars->tile_bits[i] = 0;
   bars->abort_flag = 0;
@@ -107,6 +108,14 @@ struct Cta {
   __device__ __forceinline__ bool wait(uint64_t& b, uint32_t parity, int code) const {
     return wait_together(smem_u32(&b), parity & 1u, abort_flag, status, code);
   }
+  // a wait of loads that run ahead
+  __device__ __forceinline__ bool wait_long(uint64_t& b, uint32_t parity) const {
+    return wait_suspended(smem_u32(&b), parity & 1u, abort_flag, status, MOSS_STATUS_TIMEOUT_LOAD);
+  }
+  // one thread's wait
+  __device__ __forceinline__ bool wait_alone(uint64_t& b, uint32_t parity) const {
+    return mbar_poll(smem_u32(&b), parity & 1u, abort_flag, status, MOSS_STATUS_TIMEOUT_MMA);
+  }
   __device__ __forceinline__ uint64_t& full(uint32_t pos) const { return bars->full[pos % S::kStages]; }
   __device__ __forceinline__ uint64_t& empty(uint32_t pos) const { return bars->empty[pos % S::kStages]; }
   __device__ __forceinline__ uint64_t& clean(uint32_t nth) const { return bars->clean[nth % S::kStages]; }
@@ -127,7 +136,7 @@ struct Cta {
     uint32_t pos = 0, held = 0;
   };
   __device__ __forceinline__ bool load_held(Loads& l, const CUtensorMap* first, const CUtensorMap* second, int row, int head, int entry) const {
-    if (!wait(bars->held_empty, l.held ^ 1u, MOSS_STATUS_TIMEOUT_LOAD)) return false;
+    if (!wait_long(bars->held_empty, l.held ^ 1u)) return false;
     if ((threadIdx.x & 31) == 0) {
       const uint32_t b = smem_u32(&bars->held_full);
       mbar_arrive_expect_tx(b, 2 * S::kTileBytes);
@@ -139,7 +148,7 @@ struct Cta {
     return true;
   }
   __device__ __forceinline__ bool load_next(Loads& l, const CUtensorMap* map, int row, int head, int entry) const {
-    if (!wait(empty(l.pos), round_of(l.pos) ^ 1u, MOSS_STATUS_TIMEOUT_LOAD)) return false;
+    if (!wait_long(empty(l.pos), round_of(l.pos) ^ 1u)) return false;
     if ((threadIdx.x & 31) == 0) {
       const uint32_t b = smem_u32(&full(l.pos));
       mbar_arrive_expect_tx(b, S::kTileBytes);
@@ -165,8 +174,8 @@ struct Cta {
 
 // Shared prologue: barriers, the mask's tiles, TMEM.
 template <int kD>
-__device__ __forceinline__ TileBits begin(const Cta<kD>& cta, const Args& args, bool masked) {
-  if (threadIdx.x == 0) init_barriers(cta.bars, Shape<kD>::kStages, Shape<kD>::kStats);
+__device__ __forceinline__ TileBits begin(const Cta<kD>& cta, const Args& args, bool masked, int stat_writers) {
+  if (threadIdx.x == 0) init_barriers(cta.bars, Shape<kD>::kStages, Shape<kD>::kStats, stat_writers);
   const int key_tiles = (args.tk + kTile - 1) / kTile;
   const bool use_bits = masked && has_tile_bits(args, key_tiles);
   if (use_bits) {
@@ -257,7 +266,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const Cta<kD> cta(smem_raw, args.status);
   if (cta.misplaced()) return;
   Barriers* const bars = cta.bars;
-  const TileBits taken = begin<kD>(cta, args, kMask);
+  const TileBits taken = begin<kD>(cta, args, kMask, kMathWarps);
   const uint32_t tmem = bars->tmem_base;  // S (and dS) of two key tiles, dP, dQ
   const uint32_t dp_tmem = tmem + 2 * kTile, dq_tmem = tmem + 3 * kTile;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -293,54 +302,52 @@ __global__ void __launch_bounds__(kThreads, 1)
       constexpr uint32_t d_idesc = umma_idesc_f16(kFormat, true, kTile, kD);
       uint32_t pos = 0, held = 0, steps = 0, accs = 0;
       bool issued = false;
-      auto wait = [&](uint64_t& b, uint32_t parity) { return cta.wait(b, parity, MOSS_STATUS_TIMEOUT_MMA); };
       for (int u = blockIdx.x; u < num_units && ok; u += gridDim.x) {
         QueryUnit w;
         if (!locate(args, taken, u, w) || w.first >= w.end) continue;
         int n = 0;
         for (int t = w.first; t < w.end; t = taken.next(w.s.entry, t + 1, w.end)) ++n;
-        // key tile i of the unit: K at ring position pos + 2 i, V behind it
-        auto scores = [&](int i) {
-          const uint32_t p = pos + 2 * i;
-          if (!(kMask ? wait(cta.clean(p / 2), (p / 2) / Shape<kD>::kStages) : wait(cta.full(p), cta.round_of(p)))) return false;
-          tc_fence_after();
-          if (elect_one()) mma_over_head<kD>(tmem + (i & 1) * kTile, by_rows_desc(cta.held(0)), by_rows_desc(cta.ring(p)), s_idesc);
-          issued = true;
-          __syncwarp();
-          return true;
-        };
-        auto grads = [&](int i) {
-          const uint32_t p = pos + 2 * i + 1;
-          if (!wait(cta.full(p), cta.round_of(p))) return false;
-          tc_fence_after();
-          if (elect_one()) {
+        if (elect_one()) {  // one thread waits and issues for the whole unit
+          // key tile i of the unit: K at ring position pos + 2 i, V behind it
+          auto scores = [&](int i) {
+            const uint32_t p = pos + 2 * i;
+            ok = ok && (kMask ? cta.wait_alone(cta.clean(p / 2), (p / 2) / Shape<kD>::kStages) : cta.wait_alone(cta.full(p), cta.round_of(p)));
+            if (!ok) return;
+            tc_fence_after();
+            mma_over_head<kD>(tmem + (i & 1) * kTile, by_rows_desc(cta.held(0)), by_rows_desc(cta.ring(p)), s_idesc);
+          };
+          auto grads = [&](int i) {
+            const uint32_t p = pos + 2 * i + 1;
+            ok = ok && cta.wait_alone(cta.full(p), cta.round_of(p));
+            if (!ok) return;
+            tc_fence_after();
             mma_over_head<kD>(dp_tmem, by_rows_desc(cta.held(1)), by_rows_desc(cta.ring(p)), s_idesc);
             umma_commit(smem_u32(&bars->dp_full));  // (S of this tile is done then too)
             umma_commit(smem_u32(&cta.empty(p)));
             if (i + 1 == n) umma_commit(smem_u32(&bars->held_empty));
-          }
-          __syncwarp();
-          return true;
-        };
-        ok = wait(bars->held_full, held++) && scores(0);
-        // S of the next tile goes first where its buffer is free, so that dP's arrival means both
-        ok = ok && grads(0) && (n == 1 || scores(1));
-        for (int i = 0; i < n && ok; ++i) {
-          ok = wait(bars->ds_ready, steps++);
-          if (!ok) break;
-          if (i + 1 < n) ok = grads(i + 1);
-          if (ok && i == 0) ok = wait(bars->acc_free, accs++ ^ 1u);
-          if (!ok) break;
-          tc_fence_after();
-          const uint32_t p = pos + 2 * i;
-          if (elect_one()) {
+          };
+          ok = cta.wait_alone(bars->held_full, held);
+          scores(0);
+          grads(0);
+          if (n > 1) scores(1);
+          for (int i = 0; i < n && ok; ++i) {
+            if (!(ok = cta.wait_alone(bars->ds_ready, steps + i))) break;
+            if (i + 1 < n) grads(i + 1);
+            if (i == 0) ok = ok && cta.wait_alone(bars->acc_free, accs ^ 1u);
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t p = pos + 2 * i;
             mma_over_halves(dq_tmem, tmem + (i & 1) * kTile, by_columns_desc(cta.ring(p)), d_idesc, i > 0);
             umma_commit(smem_u32(&cta.empty(p)));
             if (i + 1 == n) umma_commit(smem_u32(&bars->acc_full));
+            if (i + 2 < n) scores(i + 2);
           }
-          __syncwarp();
-          if (i + 2 < n) ok = scores(i + 2);
         }
+        ok = __all_sync(0xffffffffu, ok) != 0;
+        issued = true;
+        ++held;
+        ++accs;
+        steps += n;
         pos += 2 * n;
       }
       cta.drain(issued);
@@ -360,42 +367,6 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
       }
-    } else {
-      // ---------------------------------------------------------------- row sums, and delta = rowsum(O dO): four rows at a time
-      uint32_t nth = 0;
-      for (int u = blockIdx.x; u < num_units && ok; u += gridDim.x) {
-        QueryUnit w;
-        if (!locate(args, taken, u, w)) continue;
-        if (!cta.wait(bars->stat_free[nth % Shape<kD>::kStats], (nth / Shape<kD>::kStats) ^ 1u, MOSS_STATUS_TIMEOUT_LOAD)) break;
-        float* to = cta.stat(nth);
-        const int part = lane & 7;
-        const int count = args.head_dim - part * 16;
-#pragma unroll 2
-        for (int r = lane >> 3; r < kTile; r += 4) {
-          const int64_t row = w.s.q_row + w.row + r;
-          const bool live = w.row + r < w.s.qn;
-          float sum = 0.0f;
-          if (live && count > 0) {
-            const int64_t at = (row * args.q_heads + w.head) * args.head_dim + part * 16;
-            float o[16], g[16];
-            load_row16<kKind>(static_cast<const uint16_t*>(args.o) + at, count, o);
-            load_row16<kKind>(static_cast<const uint16_t*>(args.grad) + at, count, g);
-#pragma unroll
-            for (int j = 0; j < 16; ++j) sum = fmaf(o[j], g[j], sum);
-          }
-#pragma unroll
-          for (int d = 4; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-          if (part == 0) {
-            const int64_t at = w.head * args.q_rows + row;
-            to[r] = live ? __ldg(args.lse + at) : INFINITY;
-            to[kTile + r] = sum;
-            if (live && w.split == 0) args.delta[at] = sum;
-          }
-        }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&bars->stat_full[nth % Shape<kD>::kStats]));
-        ++nth;
-      }
     }
   } else {
     // ---------------------------------------------------------------- P and dS, and the output
@@ -408,11 +379,36 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int u = blockIdx.x; u < num_units && ok; u += gridDim.x) {
       QueryUnit w;
       if (!locate(args, taken, u, w)) continue;
-      ok = cta.wait(bars->stat_full[nth % Shape<kD>::kStats], nth / Shape<kD>::kStats, MOSS_STATUS_TIMEOUT_EPILOGUE);
+      // delta = rowsum(O dO): each warpgroup takes half of the head, and they meet in shared memory (in a slot that was last
+      // read two units ago, before the meeting of the unit between)
+      const int at = w.row + row;
+      const bool live = at < w.s.qn;
+      const int64_t q_row = w.s.q_row + at;
+      float lse = INFINITY, delta = 0.0f;
+      if (live) {
+        lse = __ldg(args.lse + w.head * args.q_rows + q_row);
+        const int64_t from = (q_row * args.q_heads + w.head) * args.head_dim + half * (kD / 2);
+        const uint16_t* o = static_cast<const uint16_t*>(args.o) + from;
+        const uint16_t* g = static_cast<const uint16_t*>(args.grad) + from;
+        const int count = args.head_dim - half * (kD / 2);
+#pragma unroll
+        for (int c = 0; c < kD / 32; ++c) {
+          float x[16], y[16];
+          load_row16<kKind>(o + c * 16, count - c * 16, x);
+          load_row16<kKind>(g + c * 16, count - c * 16, y);
+#pragma unroll
+          for (int j = 0; j < 16; ++j) delta = fmaf(x[j], y[j], delta);
+        }
+      }
+      float* const meet = cta.stats + (nth & 1u) * 2 * kTile;
+      meet[half * kTile + row] = delta;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&bars->stat_full[nth & 1u]));
+      ok = cta.wait(bars->stat_full[nth & 1u], nth >> 1, MOSS_STATUS_TIMEOUT_EPILOGUE);
       if (!ok) break;
-      const float lse = cta.stat(nth)[row], delta = cta.stat(nth)[kTile + row];
-      mbar_arrive(smem_u32(&bars->stat_free[nth % Shape<kD>::kStats]));
       ++nth;
+      delta = meet[row] + meet[kTile + row];
+      if (live && half == 0 && w.split == 0) args.delta[w.head * args.q_rows + q_row] = delta;
       const bool alone = w.first < w.end && only_key(args, taken, w.s, w.first);
       int i = 0;
       for (int t = w.first; t < w.end; t = taken.next(w.s.entry, t + 1, w.end), ++i) {
@@ -451,7 +447,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         store64<kKind>(s_tmem, v);
         tmem_wait_st();
         tc_fence_before();
-        mbar_arrive(smem_u32(&bars->ds_ready));
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&bars->ds_ready));
       }
       if (!ok) break;
       const bool any_keys = w.first < w.end;
@@ -460,8 +457,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!ok) break;
         tc_fence_after();
       }
-      const int at = w.row + row;
-      const int64_t to = ((w.s.q_row + at) * args.q_heads + w.head) * args.head_dim;
+      const int64_t to = (q_row * args.q_heads + w.head) * args.head_dim;
 #pragma unroll
       for (int c = 0; c < kD / 64; ++c) {  // this warpgroup's half of the head
         const int col = half * (kD / 2) + c * 32;
@@ -473,13 +469,14 @@ __global__ void __launch_bounds__(kThreads, 1)
           wait_ld_of(o);
           if (c == kD / 64 - 1) {
             tc_fence_before();
-            mbar_arrive(smem_u32(&bars->acc_free));
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&bars->acc_free));
           }
         }
 #pragma unroll
         for (int j = 0; j < 32; ++j) v[j] = any_keys ? __uint_as_float(o[j]) * args.scale : 0.0f;
         const int count = args.head_dim - col;
-        if (at < w.s.qn && count > 0) {
+        if (live && count > 0) {
           if (args.splits > 1)
             store_row32_f32(args.partial + w.split * args.q_rows * args.q_heads * args.head_dim + to + col, count, v);
           else
@@ -520,7 +517,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const Cta<kD> cta(smem_raw, args.status);
   if (cta.misplaced()) return;
   Barriers* const bars = cta.bars;
-  const TileBits taken = begin<kD>(cta, args, !kPacked);
+  const TileBits taken = begin<kD>(cta, args, !kPacked, 1);
   const uint32_t tmem = bars->tmem_base;  // S^T (and P^T), dP^T (and dS^T), dV, dK
   const uint32_t dp_tmem = tmem + kTile, dv_tmem = tmem + 2 * kTile, dk_tmem = tmem + 3 * kTile;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -555,52 +552,46 @@ __global__ void __launch_bounds__(kThreads, 1)
       constexpr uint32_t d_idesc = umma_idesc_f16(kFormat, true, kTile, kD);
       uint32_t pos = 0, held = 0, steps = 0, accs = 0;
       bool issued = false;
-      auto wait = [&](uint64_t& b, uint32_t parity) { return cta.wait(b, parity, MOSS_STATUS_TIMEOUT_MMA); };
-      auto there = [&](uint32_t p) {
-        return kPacked ? wait(cta.clean(p), cta.round_of(p)) : wait(cta.full(p), cta.round_of(p));
-      };
       for (int u = blockIdx.x; u < num_units && ok; u += gridDim.x) {
         KeyUnit w;
         if (!locate(args, taken, u, w) || w.first == w.end) continue;
         const int n = w.end - w.first;
-        // query tile i of the unit: Q at ring position pos + 2 i, dO behind it
-        auto product = [&](int i, int which) {  // 0: S^T = K Q^T, 1: dP^T = V dO^T
-          const uint32_t p = pos + 2 * i + which;
-          if (!there(p)) return false;
-          tc_fence_after();
-          if (elect_one()) {
+        if (elect_one()) {  // one thread waits and issues for the whole unit
+          // query tile i of the unit: Q at ring position pos + 2 i, dO behind it
+          auto product = [&](int i, int which) {  // 0: S^T = K Q^T, 1: dP^T = V dO^T
+            const uint32_t p = pos + 2 * i + which;
+            ok = ok && (kPacked ? cta.wait_alone(cta.clean(p), cta.round_of(p)) : cta.wait_alone(cta.full(p), cta.round_of(p)));
+            if (!ok) return;
+            tc_fence_after();
             mma_over_head<kD>(tmem + which * kTile, by_rows_desc(cta.held(which)), by_rows_desc(cta.ring(p)), s_idesc);
             umma_commit(which == 0 ? smem_u32(&bars->s_full) : smem_u32(&bars->dp_full));
             if (which == 1 && i + 1 == n) umma_commit(smem_u32(&bars->held_empty));
-          }
-          issued = true;
-          __syncwarp();
-          return true;
-        };
-        ok = wait(bars->held_full, held++) && product(0, 0) && product(0, 1);
-        for (int i = 0; i < n && ok; ++i, ++steps) {
-          const uint32_t p = pos + 2 * i;
-          ok = wait(bars->p_ready, steps);
-          if (ok && i == 0) ok = wait(bars->acc_free, accs++ ^ 1u);
-          if (!ok) break;
-          tc_fence_after();
-          if (elect_one()) {
+          };
+          ok = cta.wait_alone(bars->held_full, held);
+          product(0, 0);
+          product(0, 1);
+          for (int i = 0; i < n && ok; ++i) {
+            const uint32_t p = pos + 2 * i;
+            ok = cta.wait_alone(bars->p_ready, steps + i) && (i > 0 || cta.wait_alone(bars->acc_free, accs ^ 1u));
+            if (!ok) break;
+            tc_fence_after();
             mma_over_halves(dv_tmem, tmem, by_columns_desc(cta.ring(p + 1)), d_idesc, i > 0);
             umma_commit(smem_u32(&cta.empty(p + 1)));
-          }
-          __syncwarp();
-          if (i + 1 < n) ok = product(i + 1, 0);
-          ok = ok && wait(bars->ds_ready, steps);
-          if (!ok) break;
-          tc_fence_after();
-          if (elect_one()) {
+            if (i + 1 < n) product(i + 1, 0);
+            ok = ok && cta.wait_alone(bars->ds_ready, steps + i);
+            if (!ok) break;
+            tc_fence_after();
             mma_over_halves(dk_tmem, dp_tmem, by_columns_desc(cta.ring(p)), d_idesc, i > 0);
             umma_commit(smem_u32(&cta.empty(p)));
             if (i + 1 == n) umma_commit(smem_u32(&bars->acc_full));
+            if (i + 1 < n) product(i + 1, 1);
           }
-          __syncwarp();
-          if (i + 1 < n) ok = product(i + 1, 1);
         }
+        ok = __all_sync(0xffffffffu, ok) != 0;
+        issued = true;
+        ++held;
+        ++accs;
+        steps += n;
         pos += 2 * n;
       }
       cta.drain(issued);
@@ -703,7 +694,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         tmem_wait_st();
         tc_fence_before();
-        mbar_arrive(smem_u32(&bars->p_ready));
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&bars->p_ready));
         ok = cta.wait(bars->dp_full, steps, MOSS_STATUS_TIMEOUT_EPILOGUE);
         if (!ok) break;
         tc_fence_after();
@@ -721,11 +713,12 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (!seen || alone || j >= rows) v[j] = 0.0f;
         }
         __syncwarp();
-        mbar_arrive(smem_u32(&bars->stat_free[slot]));
+        if (lane == 0) mbar_arrive(smem_u32(&bars->stat_free[slot]));
         store64<kKind>(dp_tmem + half * kHalf + lanes, v);
         tmem_wait_st();
         tc_fence_before();
-        mbar_arrive(smem_u32(&bars->ds_ready));
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&bars->ds_ready));
       }
       if (!ok) break;
       const bool any = w.first < w.end;
@@ -748,7 +741,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           wait_ld_of(o);
           if (c == kD / 32 - 1) {
             tc_fence_before();
-            mbar_arrive(smem_u32(&bars->acc_free));
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&bars->acc_free));
           }
         }
 #pragma unroll
