@@ -124,8 +124,12 @@ struct KeyBits {
   uint32_t w[4];
   __device__ __forceinline__ bool all() const { return (w[0] & w[1] & w[2] & w[3]) == 0xffffffffu; }
 };
-__device__ __forceinline__ KeyBits key_bits(const Args& a, const Sequence& s, int key) {
+__device__ __forceinline__ KeyBits key_bits(const Args& a, const Sequence& s, int key, bool whole = false) {
   KeyBits b;
+  if (whole || (a.mask == nullptr && s.kn - key >= kTile)) {
+    b.w[0] = b.w[1] = b.w[2] = b.w[3] = 0xffffffffu;
+    return b;
+  }
   const int lane = threadIdx.x & 31;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -191,6 +195,15 @@ __device__ __forceinline__ void tma_store_4d(const CUtensorMap* map, uint32_t sr
                "r"(src), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
                : "memory");
 }
+// The same rows into the L2 cache only.
+template <int kD>
+__device__ __forceinline__ void prefetch_tile(const CUtensorMap* map, int row, int head, int entry) {
+#pragma unroll
+  for (int c = 0; c < kD / 64; ++c)
+    asm volatile("cp.async.bulk.prefetch.tensor.4d.L2.global [%0, {%1, %2, %3, %4}];" ::"l"(reinterpret_cast<uint64_t>(map)),
+                 "r"(c * 64), "r"(row), "r"(head), "r"(entry)
+                 : "memory");
+}
 // 128 rows of a head as boxes of 64 values (what lies past the head's values reads as zero).
 template <int kD>
 __device__ __forceinline__ void load_tile(uint32_t dst, const CUtensorMap* map, uint32_t bar, int row, int head, int entry) {
@@ -245,6 +258,63 @@ __device__ __forceinline__ float exp2_approx(float x) {
   return y;
 }
 
+// Pairs of f32 in one register pair: the CUDA cores take two of them an instruction.
+__device__ __forceinline__ uint64_t pair_of(float lo, float hi) {
+  uint64_t p;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(lo), "f"(hi));
+  return p;
+}
+__device__ __forceinline__ void split_pair(uint64_t p, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(p)); }
+__device__ __forceinline__ uint64_t fma_pair(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t mul_pair(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t add_pair(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+
+// 2^x of a pair on the CUDA cores, x in [-126, 127] (below it 2^-126, NaN and +inf NaN): 2^n p(f) with n the nearest whole
+// number and p the polynomial of degree 4 that is nearest to 2^f on [-1/2, 1/2] in relative error (Remez' exchange),
+// 2^-18.5 off at most. A multiprocessor's special-function units give 16 exponentials a cycle, which is what bounds the
+// softmax; a part of them is computed here meanwhile.
+__device__ __forceinline__ uint64_t exp2_pair(uint64_t x) {
+  float x0, x1;
+  split_pair(x, x0, x1);
+  x = pair_of(max_nan(x0, -126.0f), max_nan(x1, -126.0f));
+  const uint64_t t = add_pair(x, pair_of(12582912.0f, 12582912.0f));  // 1.5 * 2^23: the low bits are n
+  const uint64_t n = add_pair(t, pair_of(-12582912.0f, -12582912.0f));
+  const uint64_t f = fma_pair(n, pair_of(-1.0f, -1.0f), x);
+  uint64_t p = fma_pair(f, pair_of(0.009570102207362652f, 0.009570102207362652f), pair_of(0.05591785907745361f, 0.05591785907745361f));
+  p = fma_pair(f, p, pair_of(0.240247443318367f, 0.240247443318367f));
+  p = fma_pair(f, p, pair_of(0.6931217908859253f, 0.6931217908859253f));
+  p = fma_pair(f, p, pair_of(0.9999992847442627f, 0.9999992847442627f));
+  float p0, p1, t0, t1;
+  split_pair(p, p0, p1);
+  split_pair(t, t0, t1);
+  return pair_of(__uint_as_float((__float_as_uint(t0) << 23) + __float_as_uint(p0)),
+                 __uint_as_float((__float_as_uint(t1) << 23) + __float_as_uint(p1)));
+}
+// Of `i`-th pairs, those that are computed that way.
+__device__ __forceinline__ constexpr bool by_polynomial(int i) { return i % 3 == 2; }
+
+// 2^(s scale - shift) of the pair s; kAll: by the special-function unit in any case (it gives a masked value's zero).
+template <bool kAll>
+__device__ __forceinline__ uint64_t exponentials(int i, uint64_t s, uint64_t scale, uint64_t minus_shift) {
+  const uint64_t x = fma_pair(s, scale, minus_shift);
+  if (!kAll && by_polynomial(i)) return exp2_pair(x);
+  float x0, x1;
+  split_pair(x, x0, x1);
+  return pair_of(exp2_approx(x0), exp2_approx(x1));
+}
+
 // A warp zeroes the rows of a 128-row tile whose bit is not set (what lies there may be anything, and 0 * NaN is NaN), a row
 // a lane, then makes that visible to the tensor cores.
 template <int kD>
@@ -262,8 +332,8 @@ __device__ __forceinline__ void scrub_rows(uint32_t tile, const KeyBits& keep) {
   __syncwarp();
 }
 
-// Which key tiles have a key that may be looked at, a bit for each tile of each entry, so that the others are passed over.
-// Masks of more tiles go without (every tile is then taken).
+// Which key tiles have a key that may be looked at, a bit for each tile of each entry, so that the others are passed over; and
+// in a second row of bits which have no other (their masks are not read again). Masks of more tiles go without.
 constexpr int kMaxTileBits = 256;
 __device__ __forceinline__ bool has_tile_bits(const Args& a, int key_tiles) {
   return a.mask != nullptr && static_cast<int64_t>(a.batch) * key_tiles <= kMaxTileBits;
@@ -274,18 +344,28 @@ __device__ __forceinline__ void find_tile_bits(const Args& a, int key_tiles, uin
   const int total = a.batch * key_tiles;
   for (int i = threadIdx.x >> 5; i < total; i += warps) {
     const int entry = i / key_tiles, key = (i - entry * key_tiles) * kTile;
-    bool any = false;
+    bool any = false, all = true;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int k = key + j * 32 + lane;
-      if (k < a.tk) any = any || __ldg(a.mask + entry * a.mask_ld + k) != 0;
+      const bool seen = k < a.tk && __ldg(a.mask + entry * a.mask_ld + k) != 0;
+      any = any || seen;
+      all = all && seen;
     }
-    if (__any_sync(0xffffffffu, any) && lane == 0) atomicOr(bits + (i >> 5), 1u << (i & 31));
+    any = __any_sync(0xffffffffu, any);
+    all = __all_sync(0xffffffffu, all);
+    if (any && lane == 0) atomicOr(bits + (i >> 5), 1u << (i & 31));
+    if (all && lane == 0) atomicOr(bits + kMaxTileBits / 32 + (i >> 5), 1u << (i & 31));
   }
 }
 struct TileBits {
   const uint32_t* bits;  // null: every tile
   int key_tiles;
+  // whether all keys of a tile may be looked at (known only with bits)
+  __device__ __forceinline__ bool whole(int entry, int tile) const {
+    const int i = entry * key_tiles + tile;
+    return bits != nullptr && ((bits[kMaxTileBits / 32 + (i >> 5)] >> (i & 31)) & 1u) != 0;
+  }
   __device__ __forceinline__ bool has(int entry, int tile) const {
     const int i = entry * key_tiles + tile;
     return bits == nullptr || ((bits[i >> 5] >> (i & 31)) & 1u) != 0;
@@ -337,7 +417,7 @@ __device__ __forceinline__ void store_row32_f32(float* to, int count, const floa
 
 struct Maps {
   CUtensorMap q, k, v;
-  CUtensorMap grad;  // dense: dO, or O in the forward pass
+  CUtensorMap grad, o;  // dense (the forward pass has no grad)
 };
 
 int launch_forward(int kind, const Maps& maps, const Args& a, cudaStream_t stream);

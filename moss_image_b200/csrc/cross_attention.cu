@@ -226,7 +226,7 @@ int forward(const Problem& p, const void* q, Strides qs, const void* k, Strides 
   if (rc != MOSS_OK) return rc;
   Maps maps;
   const Strides dense{p.tq * p.q_heads * p.head_dim, p.q_heads * p.head_dim, p.head_dim};
-  if (!make_map(&maps.grad, dtype, out, p, p.tq, p.q_heads, dense) || !make_map(&maps.q, dtype, q, p, p.tq, p.q_heads, qs) ||
+  if (!make_map(&maps.o, dtype, out, p, p.tq, p.q_heads, dense) || !make_map(&maps.q, dtype, q, p, p.tq, p.q_heads, qs) ||
       !make_map(&maps.k, dtype, k, p, p.tk, p.k_heads, ks) || !make_map(&maps.v, dtype, v, p, p.tk, p.k_heads, vs))
     return fail(MOSS_ERR_INVALID_ARGUMENT, "queries, keys, values and outputs need 16-byte aligned rows of one stride");
   rc = launch_forward(dtype, maps, a, stream);
@@ -277,7 +277,7 @@ int backward(const Problem& p, const void* grad, const void* q, Strides qs, cons
   if (rc != MOSS_OK) return rc;
   Maps maps;
   const Strides dense{p.tq * p.q_heads * p.head_dim, p.q_heads * p.head_dim, p.head_dim};
-  if (reinterpret_cast<uintptr_t>(out) % 16 != 0 || !make_map(&maps.grad, dtype, grad, p, p.tq, p.q_heads, dense) ||
+  if (!make_map(&maps.o, dtype, out, p, p.tq, p.q_heads, dense) || !make_map(&maps.grad, dtype, grad, p, p.tq, p.q_heads, dense) ||
       !make_map(&maps.q, dtype, q, p, p.tq, p.q_heads, qs) || !make_map(&maps.k, dtype, k, p, p.tk, p.k_heads, ks) ||
       !make_map(&maps.v, dtype, v, p, p.tk, p.k_heads, vs))
     return fail(MOSS_ERR_INVALID_ARGUMENT, "queries, keys, values, outputs and gradients need 16-byte aligned rows of one stride");

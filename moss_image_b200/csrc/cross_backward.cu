@@ -45,13 +45,16 @@ constexpr int kMaxStages = 8;
 
 struct Barriers {
   uint64_t held_full, held_empty;                    // the tiles that stay: Q and dO, or K and V
-  uint64_t full[kMaxStages], empty[kMaxStages];      // the tiles that pass
+  uint64_t empty[kMaxStages];                        // the tiles that pass, by stage
+  // dkv: by stage; dq: K (and V) by number, modulo the stages (its masking warp waits for K alone, and a barrier by stage would go
+  // on to a V tile unseen)
+  uint64_t full[kMaxStages], v_full[kMaxStages];
   uint64_t clean[kMaxStages];                        // masked or foreign rows of the n-th tile that needs it are zero
   uint64_t stat_full[4], stat_free[4];
   uint64_t s_full, dp_full, p_ready, ds_ready;
   uint64_t acc_full, acc_free;
   uint64_t drain;
-  uint32_t tile_bits[kMaxTileBits / 32];
+  uint32_t tile_bits[2 * kMaxTileBits / 32];
   uint32_t tmem_base;
   int abort_flag;
 };
@@ -63,6 +66,7 @@ __device__ __forceinline__ void init_barriers(Barriers* bars, int stages, int st
   init(bars->held_empty, 1);
   for (int s = 0; s < stages; ++s) {
     init(bars->full[s], 1);
+    init(bars->v_full[s], 1);
     init(bars->empty[s], 1);
     init(bars->clean[s], 1);
   }
@@ -77,7 +81,7 @@ __device__ __forceinline__ void init_barriers(Barriers* bars, int stages, int st
   init(bars->acc_full, 1);
   init(bars->acc_free, kMathWarps);
   init(bars->drain, 1);
-  for (int i = 0; i < kMaxTileBits / 32; ++i) bars->tile_bits[i] = 0;
+  for (int i = 0; i < 2 * kMaxTileBits / 32; ++i) bars->tile_bits[i] = 0;
   bars->abort_flag = 0;
   fence_mbar_init();
 }
@@ -117,6 +121,7 @@ struct Cta {
     return mbar_poll(smem_u32(&b), parity & 1u, abort_flag, status, MOSS_STATUS_TIMEOUT_MMA);
   }
   __device__ __forceinline__ uint64_t& full(uint32_t pos) const { return bars->full[pos % S::kStages]; }
+  __device__ __forceinline__ uint64_t& v_full(uint32_t nth) const { return bars->v_full[nth % S::kStages]; }
   __device__ __forceinline__ uint64_t& empty(uint32_t pos) const { return bars->empty[pos % S::kStages]; }
   __device__ __forceinline__ uint64_t& clean(uint32_t nth) const { return bars->clean[nth % S::kStages]; }
   __device__ __forceinline__ static uint32_t round_of(uint32_t pos) { return pos / S::kStages; }
@@ -147,10 +152,10 @@ struct Cta {
     __syncwarp();
     return true;
   }
-  __device__ __forceinline__ bool load_next(Loads& l, const CUtensorMap* map, int row, int head, int entry) const {
+  __device__ __forceinline__ bool load_next(Loads& l, uint64_t& full, const CUtensorMap* map, int row, int head, int entry) const {
     if (!wait_long(empty(l.pos), round_of(l.pos) ^ 1u)) return false;
     if ((threadIdx.x & 31) == 0) {
-      const uint32_t b = smem_u32(&full(l.pos));
+      const uint32_t b = smem_u32(&full);
       mbar_arrive_expect_tx(b, S::kTileBytes);
       load_tile<kD>(ring(l.pos), map, b, row, head, entry);
     }
@@ -158,9 +163,13 @@ struct Cta {
     __syncwarp();
     return true;
   }
-  __device__ __forceinline__ void finish(const Loads& l) const {
+  __device__ __forceinline__ void finish(const Loads& l, bool by_number) const {
     if ((threadIdx.x & 31) != 0) return;
-    for (uint32_t p = l.pos > S::kStages ? l.pos - S::kStages : 0; p < l.pos; ++p) landed(full(p), round_of(p));
+    const uint32_t count = by_number ? l.pos / 2 : l.pos;
+    for (uint32_t p = count > S::kStages ? count - S::kStages : 0; p < count; ++p) {
+      landed(full(p), round_of(p));
+      if (by_number) landed(v_full(p), round_of(p));
+    }
     if (l.held > 0) landed(bars->held_full, l.held - 1);
   }
   __device__ __forceinline__ void drain(bool issued) const {
@@ -261,7 +270,8 @@ __device__ __forceinline__ void load_row16(const uint16_t* p, int count, float (
 template <int kKind, int kD, bool kMask>
 __global__ void __launch_bounds__(kThreads, 1)
     cross_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
-                    const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_grad, const Args args) {
+                    const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_grad,
+                    const __grid_constant__ CUtensorMap tm_o, const Args args) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   const Cta<kD> cta(smem_raw, args.status);
   if (cta.misplaced()) return;
@@ -289,12 +299,21 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!locate(args, taken, u, w) || w.first >= w.end) continue;
         const int k_head = w.head / args.group;
         ok = cta.load_held(l, &tm_q, &tm_grad, w.s.q0 + w.row, w.head, w.s.entry);
+        // all CTAs ask for their next tiles at about the same time: those are on their way to L2 a unit ahead
+        QueryUnit ahead;
+        if (ok && u + static_cast<int>(gridDim.x) < num_units && locate(args, taken, u + gridDim.x, ahead) && lane == 0) {
+          prefetch_tile<kD>(&tm_q, ahead.s.q0 + ahead.row, ahead.head, ahead.s.entry);
+          prefetch_tile<kD>(&tm_grad, ahead.s.q0 + ahead.row, ahead.head, ahead.s.entry);
+          prefetch_tile<kD>(&tm_o, ahead.s.q0 + ahead.row, ahead.head, ahead.s.entry);
+        }
+        __syncwarp();
         for (int t = w.first; t < w.end && ok; t = taken.next(w.s.entry, t + 1, w.end)) {
           const int row = w.s.k0 + t * kTile;
-          ok = cta.load_next(l, &tm_k, row, k_head, w.s.entry) && cta.load_next(l, &tm_v, row, k_head, w.s.entry);
+          ok = cta.load_next(l, cta.full(l.pos / 2), &tm_k, row, k_head, w.s.entry) &&
+               cta.load_next(l, cta.v_full(l.pos / 2), &tm_v, row, k_head, w.s.entry);
         }
       }
-      cta.finish(l);
+      cta.finish(l, true);
     } else if (warp == 1) {
       // ---------------------------------------------------------------- MMAs
       constexpr uint32_t kFormat = kKind == kBF16 ? 1u : 0u;
@@ -311,14 +330,14 @@ __global__ void __launch_bounds__(kThreads, 1)
           // key tile i of the unit: K at ring position pos + 2 i, V behind it
           auto scores = [&](int i) {
             const uint32_t p = pos + 2 * i;
-            ok = ok && (kMask ? cta.wait_alone(cta.clean(p / 2), (p / 2) / Shape<kD>::kStages) : cta.wait_alone(cta.full(p), cta.round_of(p)));
+            ok = ok && cta.wait_alone(kMask ? cta.clean(p / 2) : cta.full(p / 2), cta.round_of(p / 2));
             if (!ok) return;
             tc_fence_after();
             mma_over_head<kD>(tmem + (i & 1) * kTile, by_rows_desc(cta.held(0)), by_rows_desc(cta.ring(p)), s_idesc);
           };
           auto grads = [&](int i) {
             const uint32_t p = pos + 2 * i + 1;
-            ok = ok && cta.wait_alone(cta.full(p), cta.round_of(p));
+            ok = ok && cta.wait_alone(cta.v_full(p / 2), cta.round_of(p / 2));
             if (!ok) return;
             tc_fence_after();
             mma_over_head<kD>(dp_tmem, by_rows_desc(cta.held(1)), by_rows_desc(cta.ring(p)), s_idesc);
@@ -359,8 +378,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           QueryUnit w;
           if (!locate(args, taken, u, w) || w.first >= w.end) continue;
           for (int t = w.first; t < w.end; t = taken.next(w.s.entry, t + 1, w.end), pos += 2) {
-            const KeyBits keep = key_bits(args, w.s, t * kTile);
-            ok = cta.wait(cta.full(pos), cta.round_of(pos), MOSS_STATUS_TIMEOUT_LOAD);
+            const KeyBits keep = key_bits(args, w.s, t * kTile, taken.whole(w.s.entry, t));
+            ok = cta.wait(cta.full(pos / 2), cta.round_of(pos / 2), MOSS_STATUS_TIMEOUT_LOAD);
             if (!ok) break;
             if (!keep.all()) scrub_rows<kD>(cta.ring(pos), keep);
             if (lane == 0) mbar_arrive(smem_u32(&cta.clean(pos / 2)));
@@ -413,7 +432,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       int i = 0;
       for (int t = w.first; t < w.end; t = taken.next(w.s.entry, t + 1, w.end), ++i) {
         KeyBits keep;
-        if constexpr (kMask) keep = key_bits(args, w.s, t * kTile);
+        if constexpr (kMask) keep = key_bits(args, w.s, t * kTile, taken.whole(w.s.entry, t));
         const int keys = w.s.kn - t * kTile - half * kHalf;
         ok = cta.wait(bars->dp_full, steps++, MOSS_STATUS_TIMEOUT_EPILOGUE);
         if (!ok) break;
@@ -423,10 +442,15 @@ __global__ void __launch_bounds__(kThreads, 1)
         load64(s_tmem, s);
         load64(dp_tmem + half * kHalf + lanes, g);
         float v[64];
+        // (what the polynomial leaves of an exponential that should be zero, 2^-126, is nothing to a gradient; a row without keys
+        // has lse = inf, and its 2^-126 is masked)
+        const uint64_t scale2 = pair_of(args.scale_log2, args.scale_log2), minus_lse = pair_of(-lse, -lse), minus_delta = pair_of(-delta, -delta);
 #pragma unroll
-        for (int j = 0; j < 64; ++j) {
-          const float p = exp2_approx(fmaf(__uint_as_float(s[j >> 5][j & 31]), args.scale_log2, -lse));
-          v[j] = p * (__uint_as_float(g[j >> 5][j & 31]) - delta);
+        for (int j = 0; j < 64; j += 2) {
+          const uint64_t p = exponentials<false>(j / 2, pair_of(__uint_as_float(s[j >> 5][j & 31]), __uint_as_float(s[j >> 5][(j & 31) + 1])),
+                                                 scale2, minus_lse);
+          const uint64_t d = add_pair(pair_of(__uint_as_float(g[j >> 5][j & 31]), __uint_as_float(g[j >> 5][(j & 31) + 1])), minus_delta);
+          split_pair(mul_pair(p, d), v[j], v[j + 1]);
         }
         if constexpr (kMask) {
           if (!keep.all()) {
@@ -512,7 +536,8 @@ __device__ __forceinline__ bool locate(const Args& a, const TileBits& taken, int
 template <int kKind, int kD, bool kPacked>
 __global__ void __launch_bounds__(kThreads, 1)
     cross_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
-                     const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_grad, const Args args) {
+                     const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_grad,
+                     const __grid_constant__ CUtensorMap tm_o, const Args args) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   const Cta<kD> cta(smem_raw, args.status);
   if (cta.misplaced()) return;
@@ -541,10 +566,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         ok = cta.load_held(l, &tm_k, &tm_v, w.s.k0 + w.row, w.head, w.s.entry);
         for (int i = w.first; i < w.end && ok; ++i) {
           const int g = i / w.q_tiles, row = w.s.q0 + (i - g * w.q_tiles) * kTile, head = w.head * args.group + g;
-          ok = cta.load_next(l, &tm_q, row, head, w.s.entry) && cta.load_next(l, &tm_grad, row, head, w.s.entry);
+          ok = cta.load_next(l, cta.full(l.pos), &tm_q, row, head, w.s.entry) &&
+               cta.load_next(l, cta.full(l.pos), &tm_grad, row, head, w.s.entry);
         }
       }
-      cta.finish(l);
+      cta.finish(l, false);
     } else if (warp == 1) {
       // ---------------------------------------------------------------- MMAs
       constexpr uint32_t kFormat = kKind == kBF16 ? 1u : 0u;
@@ -630,8 +656,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int j = 0; j < 4; ++j) {
             const int r = j * 32 + lane;
             const bool live = row + r < w.s.qn;
-            l[j] = live ? __ldg(args.lse + at + r) : INFINITY;
-            d[j] = live ? __ldg(args.delta + at + r) : 0.0f;
+            l[j] = live ? kLift<kKind> - __ldg(args.lse + at + r) : -INFINITY;
+            d[j] = live ? -__ldg(args.delta + at + r) : 0.0f;
           }
           ok = cta.wait(bars->stat_free[nth % Shape<kD>::kStats], (nth / Shape<kD>::kStats) ^ 1u, MOSS_STATUS_TIMEOUT_LOAD);
           if (!ok) break;
@@ -655,6 +681,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     void* const result = half == 0 ? args.dv : args.dk;
     const bool wide = args.head_dim % 16 == 0 && (reinterpret_cast<uintptr_t>(result) & 31) == 0;
     uint32_t steps = 0, accs = 0;
+    const uint64_t scale2 = pair_of(args.scale_log2, args.scale_log2);
     for (int u = blockIdx.x; u < num_units && ok; u += gridDim.x) {
       KeyUnit w;
       if (!locate(args, taken, u, w)) continue;
@@ -674,12 +701,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         float v[64];
         load64(tmem + half * kHalf + lanes, r);
 #pragma unroll
-        for (int j = 0; j < 64; j += 4) {
+        for (int j = 0; j < 64; j += 4) {  // (the sums are kept negated, and lifted)
           const float4 l = *reinterpret_cast<const float4*>(lse + j);
-          const float ls[4] = {l.x, l.y, l.z, l.w};
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            v[j + e] = exp2_approx(fmaf(__uint_as_float(r[(j + e) >> 5][(j + e) & 31]), args.scale_log2, kLift<kKind> - ls[e]));
+          const uint64_t lo = exponentials<false>(j / 2, pair_of(__uint_as_float(r[j >> 5][j & 31]), __uint_as_float(r[j >> 5][(j & 31) + 1])),
+                                                  scale2, pair_of(l.x, l.y));
+          const uint64_t hi = exponentials<false>(j / 2 + 1, pair_of(__uint_as_float(r[j >> 5][(j & 31) + 2]), __uint_as_float(r[j >> 5][(j & 31) + 3])),
+                                                  scale2, pair_of(l.z, l.w));
+          split_pair(lo, v[j], v[j + 1]);
+          split_pair(hi, v[j + 2], v[j + 3]);
         }
         if (!seen || rows < kHalf) {
 #pragma unroll
@@ -702,10 +731,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         load64(dp_tmem + half * kHalf + lanes, r);
 #pragma unroll
         for (int j = 0; j < 64; j += 4) {
-          const float4 d = *reinterpret_cast<const float4*>(lse + kTile + j);
-          const float ds[4] = {d.x, d.y, d.z, d.w};
-#pragma unroll
-          for (int e = 0; e < 4; ++e) v[j + e] *= __uint_as_float(r[(j + e) >> 5][(j + e) & 31]) - ds[e];
+          const float4 d = *reinterpret_cast<const float4*>(lse + kTile + j);  // negated
+          const uint64_t lo = add_pair(pair_of(__uint_as_float(r[j >> 5][j & 31]), __uint_as_float(r[j >> 5][(j & 31) + 1])), pair_of(d.x, d.y));
+          const uint64_t hi = add_pair(pair_of(__uint_as_float(r[j >> 5][(j & 31) + 2]), __uint_as_float(r[j >> 5][(j & 31) + 3])), pair_of(d.z, d.w));
+          split_pair(mul_pair(pair_of(v[j], v[j + 1]), lo), v[j], v[j + 1]);
+          split_pair(mul_pair(pair_of(v[j + 2], v[j + 3]), hi), v[j + 2], v[j + 3]);
         }
         if (!seen || alone || rows < kHalf) {
 #pragma unroll
@@ -767,7 +797,7 @@ int launch(const char* what, F* kern, DeviceSetup& setup, int64_t units, const M
   });
   if (rc != MOSS_OK) return rc;
   const unsigned grid = static_cast<unsigned>(std::min<int64_t>(units, device_sm_count()));
-  kern<<<grid, kThreads, Shape<kD>::kSmemBytes, stream>>>(maps.q, maps.k, maps.v, maps.grad, a);
+  kern<<<grid, kThreads, Shape<kD>::kSmemBytes, stream>>>(maps.q, maps.k, maps.v, maps.grad, maps.o, a);
   return check_cuda(cudaGetLastError(), what);
 }
 

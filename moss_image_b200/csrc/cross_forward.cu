@@ -14,6 +14,7 @@
 #include <algorithm>
 #include <cmath>
 #include <cstring>
+#include <type_traits>
 
 #include "cross_args.cuh"
 
@@ -35,26 +36,29 @@ struct Shape {
   static constexpr uint32_t kTileBytes = kTile * kD * 2;
   static constexpr int kStages = kD == 128 ? 3 : 8;  // tiles of K and V on their way
   static constexpr uint32_t kDataBytes = (4 + kStages) * kTileBytes;
-  static constexpr uint32_t kSmemBytes = kDataBytes + 1024 + 512;
+  static constexpr uint32_t kSmemBytes = kDataBytes + 1024 + 768;
   static_assert(kSmemBytes <= 227 * 1024, "tiles exceed the shared memory a CTA may use");
 };
 constexpr int kMaxStages = 8;
 
 struct Barriers {
   uint64_t q_full[4], q_empty[4];  // by pair (they take turns) and tile
-  uint64_t full[kMaxStages], empty[kMaxStages];
-  uint64_t clean[kMaxStages];  // masked rows of the n-th V tile are zero (n modulo the stages)
+  uint64_t empty[kMaxStages];   // by stage
+  // by number, modulo the stages (who waits for one of them waits for each: a barrier by stage would go on to the other
+  // tensor's tile unseen)
+  uint64_t k_full[kMaxStages], v_full[kMaxStages];
+  uint64_t clean[kMaxStages];   // masked rows of a V tile are zero
   uint64_t s_full[2][2];       // by query tile and buffer: S is there
   uint64_t p_ready[2][2];      // P is there, O may be added to
   uint64_t pv_done[2];         // a product with P is done
   uint64_t o_full[2], o_free[2];
   uint64_t out_full[2];        // the results are in shared memory
   uint64_t drain[2];
-  uint32_t tile_bits[kMaxTileBits / 32];
+  uint32_t tile_bits[2 * kMaxTileBits / 32];
   uint32_t tmem_base;
   int abort_flag;
 };
-static_assert(sizeof(Barriers) <= 512, "barrier block too large");
+static_assert(sizeof(Barriers) <= 768, "barrier block too large");
 
 // Work unit: a pair of query tiles of one head, and a run of its key tiles.
 struct Unit {
@@ -123,13 +127,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(bar(bars->out_full[x]), 4);
     }
     for (int s = 0; s < kStages; ++s) {
-      mbar_init(bar(bars->full[s]), 1);
+      mbar_init(bar(bars->k_full[s]), 1);
+      mbar_init(bar(bars->v_full[s]), 1);
       mbar_init(bar(bars->empty[s]), 2);
       mbar_init(bar(bars->clean[s]), 1);
     }
     for (int x = 0; x < 2; ++x) mbar_init(bar(bars->drain[x]), 1);
     bars->abort_flag = 0;
-    for (int i = 0; i < kMaxTileBits / 32; ++i) bars->tile_bits[i] = 0;
+    for (int i = 0; i < 2 * kMaxTileBits / 32; ++i) bars->tile_bits[i] = 0;
     fence_mbar_init();
   }
   const int key_tiles = (args.tk + kTile - 1) / kTile;
@@ -180,8 +185,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t stage = pos % kStages, phase = (pos / kStages) & 1u;
         if (!wait_suspended(bar(bars->empty[stage]), phase ^ 1u, abort_flag, args.status, MOSS_STATUS_TIMEOUT_LOAD)) return false;
         if (lane == 0) {
-          mbar_arrive_expect_tx(bar(bars->full[stage]), kTileBytes);
-          load_tile<kD>(ring + stage * kTileBytes, map, bar(bars->full[stage]), w.s.k0 + tile * kTile, w.head / args.group, w.s.entry);
+          uint64_t& full = (pos & 1u) == 0 ? bars->k_full[pos / 2 % kStages] : bars->v_full[pos / 2 % kStages];
+          mbar_arrive_expect_tx(bar(full), kTileBytes);
+          load_tile<kD>(ring + stage * kTileBytes, map, bar(full), w.s.k0 + tile * kTile, w.head / args.group, w.s.entry);
         }
         ++pos;
         __syncwarp();
@@ -216,7 +222,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
         };
-        for (uint32_t p = pos > kStages ? pos - kStages : 0; p < pos; ++p) landed(bars->full[p % kStages], (p / kStages) & 1u);
+        for (uint32_t n = pos / 2 > kStages ? pos / 2 - kStages : 0; n < pos / 2; ++n) {
+          landed(bars->k_full[n % kStages], (n / kStages) & 1u);
+          landed(bars->v_full[n % kStages], (n / kStages) & 1u);
+        }
         for (int x = 0; x < 4; ++x)
           if (q_uses[x] > 0) landed(bars->q_full[x], (q_uses[x] - 1) & 1u);
       }
@@ -246,10 +255,12 @@ __global__ void __launch_bounds__(kThreads, 1)
             ok = ok && mbar_poll(bar(b), parity & 1u, abort_flag, args.status, MOSS_STATUS_TIMEOUT_MMA);
             return ok;
           };
-          auto there = [&](uint32_t p) { return wait(bars->full[p % kStages], p / kStages); };
+          auto k_there = [&](uint32_t p) { return wait(bars->k_full[p / 2 % kStages], p / 2 / kStages); };
+          auto v_there = [&](uint32_t p) { return wait(bars->v_full[p / 2 % kStages], p / 2 / kStages); };
           auto release = [&](uint32_t p) { umma_commit(bar(bars->empty[p % kStages])); };
           if (x >= w.tiles()) {  // the other warp's keys and values pass by
-            for (int i = 0; i < 2 * n && there(pos + i); ++i) mbar_arrive(bar(bars->empty[(pos + i) % kStages]));
+            for (int i = 0; i < 2 * n && ((i & 1) == 0 ? k_there(pos + i) : v_there(pos + i)); ++i)
+              mbar_arrive(bar(bars->empty[(pos + i) % kStages]));
           } else {
             // S against half j of the unit's key tiles
             auto scores = [&](int j) {
@@ -259,7 +270,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                                 k_desc + (((p % kStages) * kTileBytes + (j & 1) * kHalf * 128) >> 4), s_idesc);
               umma_commit(bar(bars->s_full[x][g & 1u]));
             };
-            if (there(pos) && wait(bars->q_full[q_slot], q_uses[units & 1u])) {
+            if (k_there(pos) && wait(bars->q_full[q_slot], q_uses[units & 1u])) {
               scores(0);
               if (m > 1) scores(1);
               release(pos);
@@ -270,7 +281,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               const uint32_t g = steps + j;
               if ((j & 1) == 0) {
                 const uint32_t nth = pv / 2;  // of the V tiles: what `clean` counts
-                if (!(kMask ? wait(bars->clean[nth % kStages], nth / kStages) : there(pv))) break;
+                if (!(kMask ? wait(bars->clean[nth % kStages], nth / kStages) : v_there(pv))) break;
               }
               if (!wait(bars->p_ready[x][g & 1u], g >> 1)) break;
               tc_fence_after();
@@ -280,7 +291,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               const bool last_half = (j & 1) == 1;
               if (last_half || j + 1 == m) release(pv);
               if (j + 2 < m) {
-                if (!last_half && !there(pv + 1)) break;
+                if (!last_half && !k_there(pv + 1)) break;
                 scores(j + 2);
                 if (last_half || j + 3 == m) release(pv + 1);
               }
@@ -318,9 +329,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!locate(args, taken, u, w) || w.first == w.end) continue;
         if constexpr (kMask) {
           for (int t = w.first; t < w.end; t = w.next(taken, t), pos += 2) {
-            const KeyBits keep = key_bits(args, w.s, t * kTile);
-            const uint32_t stage = (pos + 1) % kStages, phase = ((pos + 1) / kStages) & 1u;
-            ok = wait_together(bar(bars->full[stage]), phase, abort_flag, args.status, MOSS_STATUS_TIMEOUT_LOAD);
+            const KeyBits keep = key_bits(args, w.s, t * kTile, taken.whole(w.s.entry, t));
+            const uint32_t stage = (pos + 1) % kStages;
+            ok = wait_together(bar(bars->v_full[(pos / 2) % kStages]), (pos / 2 / kStages) & 1u, abort_flag, args.status, MOSS_STATUS_TIMEOUT_LOAD);
             if (!ok) break;
             if (!keep.all()) scrub_rows<kD>(ring + stage * kTileBytes, keep);
             if (lane == 0) mbar_arrive(bar(bars->clean[(pos / 2) % kStages]));
@@ -370,7 +381,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       bool begun = false;
       for (int t = w.first; t < w.end && ok; t = w.next(taken, t)) {
         KeyBits keep;
-        if constexpr (kMask) keep = key_bits(args, w.s, t * kTile);
+        if constexpr (kMask) keep = key_bits(args, w.s, t * kTile, taken.whole(w.s.entry, t));
         const int halves = w.halves(t);
 #pragma unroll 1
         for (int half = 0; half < halves; ++half, ++step) {
@@ -384,19 +395,24 @@ __global__ void __launch_bounds__(kThreads, 1)
           tmem_ld_32x32b_x32(s_tmem + 32, r[1]);
           wait_ld_of(r[0]);
           wait_ld_of(r[1]);
+          bool some_masked;
           if constexpr (kMask) {
             const uint32_t k0 = half == 0 ? keep.w[0] : keep.w[2], k1 = half == 0 ? keep.w[1] : keep.w[3];
-            if ((k0 & k1) != 0xffffffffu) {
+            some_masked = (k0 & k1) != 0xffffffffu;
+            if (some_masked) {
 #pragma unroll
               for (int j = 0; j < 32; ++j) {
                 if (((k0 >> j) & 1u) == 0) r[0][j] = 0xff800000u;
                 if (((k1 >> j) & 1u) == 0) r[1][j] = 0xff800000u;
               }
             }
-          } else if (keys < kHalf) {
+          } else {
+            some_masked = keys < kHalf;
+            if (some_masked) {
 #pragma unroll
-            for (int j = 0; j < 64; ++j)
-              if (j >= keys) r[j >> 5][j & 31] = 0xff800000u;
+              for (int j = 0; j < 64; ++j)
+                if (j >= keys) r[j >> 5][j & 31] = 0xff800000u;
+            }
           }
           float most[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
@@ -429,20 +445,31 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
           const float shift = top == -INFINITY ? 0.0f : top - kLift<kKind>;
-          float add[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+          const uint64_t scale2 = pair_of(args.scale_log2, args.scale_log2), minus_shift = pair_of(-shift, -shift);
+          uint64_t add[2] = {0, 0};
+          auto exponentiate = [&](auto all) {
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            uint32_t p[16];
+            for (int c = 0; c < 2; ++c) {
+              uint32_t p[16];
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {
-              const float e0 = exp2_approx(fmaf(__uint_as_float(r[c][2 * j]), args.scale_log2, -shift));
-              const float e1 = exp2_approx(fmaf(__uint_as_float(r[c][2 * j + 1]), args.scale_log2, -shift));
-              add[j & 3] += e0 + e1;
-              p[j] = gemm::pack2_kind<kKind>(e0, e1);
+              for (int j = 0; j < 16; ++j) {
+                const uint64_t e = exponentials<decltype(all)::value>(
+                    c * 16 + j, pair_of(__uint_as_float(r[c][2 * j]), __uint_as_float(r[c][2 * j + 1])), scale2, minus_shift);
+                add[j & 1] = add_pair(add[j & 1], e);
+                float e0, e1;
+                split_pair(e, e0, e1);
+                p[j] = gemm::pack2_kind<kKind>(e0, e1);
+              }
+              tmem_st_32x32b_x16(s_tmem + c * 16, p);
             }
-            tmem_st_32x32b_x16(s_tmem + c * 16, p);
-          }
-          sum += (add[0] + add[1]) + (add[2] + add[3]);
+          };
+          if (some_masked)
+            exponentiate(std::true_type{});
+          else
+            exponentiate(std::false_type{});
+          float add0, add1;
+          split_pair(add_pair(add[0], add[1]), add0, add1);
+          sum += add0 + add1;
           tmem_wait_st();
           tc_fence_before();
           __syncwarp();
@@ -526,7 +553,7 @@ int launch_typed(const Maps& maps, const Args& a, cudaStream_t stream) {
   if (rc != MOSS_OK) return rc;
   const int64_t units = static_cast<int64_t>(a.tiles) * a.splits * a.q_heads;
   const unsigned grid = static_cast<unsigned>(std::min<int64_t>(units, device_sm_count()));
-  kern<<<grid, kThreads, Shape<kD>::kSmemBytes, stream>>>(maps.q, maps.k, maps.v, maps.grad, a);
+  kern<<<grid, kThreads, Shape<kD>::kSmemBytes, stream>>>(maps.q, maps.k, maps.v, maps.o, a);
   return check_cuda(cudaGetLastError(), "cross_forward_kernel");
 }
 
