@@ -34,10 +34,11 @@ struct Args {
   float* lse;                // [q_heads][batch * tq or packed rows]
   int64_t q_rows, k_rows;    // all rows
   // splits > 1: f32 partials of each split, joined by a second kernel
-  float* partial;            // [split][q_rows][q_heads][head_dim] (forward, dq); [2][split][k_rows][k_heads][head_dim] (dk, dv)
+  float* partial;            // [split][q_rows][q_heads][head_dim] (forward, dq); [2][split][tail unit][128][head_dim] (dk, dv)
   float* partial_lse;        // [split][q_heads][q_rows]
   int splits;
   int tiles;                 // tiles (or pairs of tiles) of all sequences, at most
+  int whole, tail;           // dk, dv: units that are not split, and those that are (the last ones)
   // backward
   const void* o;             // dense
   const void* grad;          // dense

@@ -76,6 +76,38 @@ int join_sums(const float* partial, int splits, int64_t values, void* out, int k
   return check_cuda(cudaGetLastError(), "join_sums_kernel");
 }
 
+// The same for the split units of dk and dv, a CTA for each quarter of a unit and tensor.
+__global__ void __launch_bounds__(kThreads) join_tail_kernel(const Args a, int kind) {
+  const int of = a.whole + static_cast<int>(blockIdx.x), head = of / a.tiles;
+  int seq, tile;
+  if (!find_tile<true>(a, kTile, of - head * a.tiles, seq, tile)) return;
+  const Sequence s = sequence_of(a, seq);
+  const int rows = min(kTile, s.kn - tile * kTile), each = a.head_dim / 8;
+  const int64_t unit = static_cast<int64_t>(kTile) * a.head_dim, step = a.tail * unit;
+  const float* from = a.partial + static_cast<int64_t>(blockIdx.y) * a.splits * step + blockIdx.x * unit;
+  uint16_t* const to = static_cast<uint16_t*>(blockIdx.y == 0 ? a.dv : a.dk);
+  const int quarter = kTile / 4 * each;
+  for (int i = blockIdx.z * quarter + threadIdx.x; i < min(rows * each, static_cast<int>(blockIdx.z + 1) * quarter); i += kThreads) {
+    float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+    for (int p = 0; p < a.splits; ++p) {
+      float o[8];
+      load8<kF32>(from + p * step, i * 8, 8, true, o);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] += o[j];
+    }
+    uint4 w;
+    if (kind == kBF16)
+      w = make_uint4(gemm::pack2_kind<kBF16>(v[0], v[1]), gemm::pack2_kind<kBF16>(v[2], v[3]),
+                     gemm::pack2_kind<kBF16>(v[4], v[5]), gemm::pack2_kind<kBF16>(v[6], v[7]));
+    else
+      w = make_uint4(gemm::pack2_kind<kF16>(v[0], v[1]), gemm::pack2_kind<kF16>(v[2], v[3]),
+                     gemm::pack2_kind<kF16>(v[4], v[5]), gemm::pack2_kind<kF16>(v[6], v[7]));
+    const int row = i / each, c = i - row * each;
+    *reinterpret_cast<uint4*>(to + ((s.k_row + tile * kTile + row) * a.k_heads + head) * a.head_dim + c * 8) = w;
+  }
+}
+
 struct Problem {
   int64_t batch, tq, tk, q_heads, k_heads, head_dim;
   bool packed;
@@ -120,36 +152,48 @@ ForwardLayout forward_layout(const Problem& p, int splits) {
   return l;
 }
 
-// Splits of the queries that a key tile is summed over: those whose rounds over the multiprocessors are shortest, in steps of
-// a tile pair (1.2 us measured), with two more a unit for its start and end, and the partials' way through memory.
-int query_splits(const Problem& p) {
+// How dk and dv are shared out: whole units (a key tile of one head) in full rounds over the multiprocessors, and the last
+// ones split over their queries where that is shorter, in steps of a tile pair (1.2 us measured), with two more a unit for its
+// start and end, and the partial sums' way through memory. (192 units of 32 steps: 44 of them split in three.)
+struct KeyPlan {
+  int64_t whole = 0, tail = 0;
+  int splits = 1;
+};
+KeyPlan plan_keys(const Problem& p) {
   const int64_t sms = device_sm_count();
-  const int64_t units = std::max<int64_t>(1, p.k_heads * (p.packed ? ceil_div(p.tk, kTile) + p.batch / 2 : tiles_of(p, p.tk, kTile)));
+  const int64_t units = p.k_heads * tiles_of(p, p.tk, kTile);
+  // (of packed keys a tile for each sequence at most is not there)
+  const int64_t there = std::min(units, p.k_heads * (p.packed ? ceil_div(p.tk, kTile) + p.batch / 2 : units));
   const int64_t queries = p.packed ? ceil_div(p.tq, std::max<int64_t>(1, p.batch)) : p.tq;
   const int64_t steps = ceil_div(queries, kTile) * (p.q_heads / p.k_heads);
-  const double values = 2.0 * p.k_rows() * p.k_heads * p.head_dim;
-  int best = 1;
-  double least = 0.0;
-  for (int64_t s = 1; s <= std::min<int64_t>(16, std::max<int64_t>(1, steps / 2)); ++s) {
-    const double rounds = static_cast<double>(ceil_div(units * s, sms) * (ceil_div(steps, s) + 2));
+  KeyPlan plan;
+  const int64_t rest = there % sms;
+  double least = static_cast<double>(steps + 2);
+  for (int64_t s = 2; s <= std::min<int64_t>(16, steps / 2) && rest > 0; ++s) {
     // written and read once in f32, at 4 TB/s, and a launch
-    const double cost = rounds + (s == 1 ? 0.0 : values * s * 8.0 / 4e12 / 1.2e-6 + 3.0);
-    if (s == 1 || cost < least) {
-      best = static_cast<int>(s);
+    const double bytes = 16.0 * s * rest * kTile * p.head_dim;
+    const double cost = static_cast<double>(ceil_div(rest * s, sms) * (ceil_div(steps, s) + 2)) + bytes / 4e12 / 1.2e-6 + 3.0;
+    if (cost < least) {
+      plan.splits = static_cast<int>(s);
       least = cost;
     }
   }
-  return best;
+  // packed sequences differ in length, which only the device knows: more and smaller units even that out
+  if (p.packed) plan.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(ceil_div(4 * sms, std::max<int64_t>(1, there)), steps / 4)));
+  if (p.packed) plan.splits = std::min(plan.splits, 16);
+  plan.tail = plan.splits == 1 ? 0 : there < sms || p.packed ? units : rest;
+  plan.whole = units - plan.tail;
+  return plan;
 }
 
 struct BackwardLayout {
   size_t dq, dkv, total;  // after the deltas
 };
-BackwardLayout backward_layout(const Problem& p, int dq_splits, int dkv_splits) {
+BackwardLayout backward_layout(const Problem& p, int dq_splits, const KeyPlan& keys) {
   BackwardLayout l{};
   l.dq = up(static_cast<size_t>(p.q_heads) * p.q_rows() * 4);
   l.dkv = l.dq + (dq_splits > 1 ? up(static_cast<size_t>(dq_splits) * p.q_rows() * p.q_heads * p.head_dim * 4) : 0);
-  l.total = l.dkv + (dkv_splits > 1 ? up(static_cast<size_t>(dkv_splits) * 2 * p.k_rows() * p.k_heads * p.head_dim * 4) : 0);
+  l.total = l.dkv + up(static_cast<size_t>(keys.tail) * keys.splits * 2 * kTile * p.head_dim * 4);
   return l;
 }
 
@@ -259,8 +303,9 @@ int backward(const Problem& p, const void* grad, const void* q, Strides qs, cons
   }
   if (grad == nullptr || q == nullptr || k == nullptr || v == nullptr || out == nullptr || lse == nullptr)
     return fail(MOSS_ERR_INVALID_ARGUMENT, "null input pointer");
-  const int dq_splits = key_splits(p, kTile), dkv_splits = query_splits(p);
-  const BackwardLayout l = backward_layout(p, dq_splits, dkv_splits);
+  const int dq_splits = key_splits(p, kTile);
+  const KeyPlan keys = plan_keys(p);
+  const BackwardLayout l = backward_layout(p, dq_splits, keys);
   if (workspace == nullptr || workspace_bytes < l.total || reinterpret_cast<uintptr_t>(workspace) % 256 != 0)
     return fail(MOSS_ERR_INVALID_ARGUMENT, "the cross attention's gradients need %zu bytes of 256-byte aligned workspace", l.total);
   uint8_t* ws = static_cast<uint8_t*>(workspace);
@@ -287,13 +332,14 @@ int backward(const Problem& p, const void* grad, const void* q, Strides qs, cons
   a.dk = dk;
   a.dv = dv;
   a.partial = reinterpret_cast<float*>(ws + l.dkv);
-  a.splits = dkv_splits;
+  a.splits = keys.splits;
+  a.whole = static_cast<int>(keys.whole);
+  a.tail = static_cast<int>(keys.tail);
   a.tiles = static_cast<int>(tiles_of(p, p.tk, kTile));
   rc = launch_dkv(dtype, maps, a, stream);
-  if (rc == MOSS_OK && dkv_splits > 1) {
-    const int64_t values = static_cast<int64_t>(k_bytes / 2);
-    rc = join_sums(a.partial, dkv_splits, values, dv, dtype, stream);
-    if (rc == MOSS_OK) rc = join_sums(a.partial + dkv_splits * values, dkv_splits, values, dk, dtype, stream);
+  if (rc == MOSS_OK && a.tail > 0) {
+    join_tail_kernel<<<dim3(static_cast<unsigned>(a.tail), 2, 4), kThreads, 0, stream>>>(a, dtype);
+    rc = check_cuda(cudaGetLastError(), "join_tail_kernel");
   }
   return rc != MOSS_OK ? rc : clear_ok();
 }
@@ -313,7 +359,7 @@ extern "C" int moss_cross_attention_workspace_bytes(int64_t batch, int64_t q_tok
   const int rc = cross::check(p);
   if (rc != MOSS_OK) return rc;
   if (p.q_rows() == 0 || p.k_rows() == 0) return clear_ok();
-  *bytes = backward != 0 ? cross::backward_layout(p, cross::key_splits(p, cross::kTile), cross::query_splits(p)).total
+  *bytes = backward != 0 ? cross::backward_layout(p, cross::key_splits(p, cross::kTile), cross::plan_keys(p)).total
                          : cross::forward_layout(p, cross::key_splits(p, 2 * cross::kTile)).total;
   return clear_ok();
 }

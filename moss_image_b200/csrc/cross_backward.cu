@@ -515,19 +515,29 @@ __global__ void __launch_bounds__(kThreads, 1)
 // ---------------------------------------------------------------- dk and dv
 struct KeyUnit {
   Sequence s;
-  int head, split, row, first, end, q_tiles;  // head: of the keys; first to end: tiles of the group's heads, one head after another
+  int head, split, tail, row, first, end, q_tiles;  // head: of the keys; first to end: tiles of the group's heads, one head after another
 };
+// The units of the last round, which would leave multiprocessors idle, are split over their queries: tail says which one it is
+// (-1: a whole unit).
 __device__ __forceinline__ bool locate(const Args& a, const TileBits& taken, int u, KeyUnit& unit) {
-  const int t = u % a.tiles, rest = u / a.tiles;
-  unit.split = rest % a.splits;
-  unit.head = rest / a.splits;
+  int splits = 1, of = u;
+  unit.split = 0;
+  unit.tail = -1;
+  if (u >= a.whole) {
+    splits = a.splits;
+    unit.tail = (u - a.whole) / splits;
+    unit.split = u - a.whole - unit.tail * splits;
+    of = a.whole + unit.tail;
+  }
+  const int t = of % a.tiles;
+  unit.head = of / a.tiles;
   int seq, tile;
   if (!find_tile<true>(a, kTile, t, seq, tile)) return false;
   unit.s = sequence_of(a, seq);
   if (seq >= a.batch) unit.s.qn = 0;
   unit.row = tile * kTile;
   unit.q_tiles = (unit.s.qn + kTile - 1) / kTile;
-  const int all = taken.has(unit.s.entry, tile) ? unit.q_tiles * a.group : 0, each = (all + a.splits - 1) / a.splits;
+  const int all = taken.has(unit.s.entry, tile) ? unit.q_tiles * a.group : 0, each = (all + splits - 1) / splits;
   unit.first = min(all, unit.split * each);
   unit.end = min(all, unit.first + each);
   return true;
@@ -546,7 +556,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t tmem = bars->tmem_base;  // S^T (and P^T), dP^T (and dS^T), dV, dK
   const uint32_t dp_tmem = tmem + kTile, dv_tmem = tmem + 2 * kTile, dk_tmem = tmem + 3 * kTile;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int num_units = args.tiles * args.splits * args.k_heads;
+  const int num_units = args.whole + args.tail * args.splits;
   bool ok = true;
 
   if (warp < 4) {
@@ -757,7 +767,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!ok) break;
         tc_fence_after();
       }
-      const int64_t values = args.k_rows * args.k_heads * args.head_dim;
+      float* const part = args.partial + ((static_cast<int64_t>(half) * args.splits + w.split) * args.tail + w.tail) * kTile * args.head_dim;
       const int64_t to = ((w.s.k_row + key) * args.k_heads + w.head) * args.head_dim;
       const uint32_t from = (half == 0 ? dv_tmem : dk_tmem) + lanes;
       const float factor = half == 1 ? args.scale : kKind == kF16 ? 1.0f / 16384.0f : 1.0f;
@@ -779,8 +789,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int j = 0; j < 32; ++j) out[j] = any ? __uint_as_float(o[j]) * factor : 0.0f;
         const int count = args.head_dim - c * 32;
         if (key < w.s.kn && count > 0) {
-          if (args.splits > 1)
-            store_row32_f32(args.partial + (half * args.splits + w.split) * values + to + c * 32, count, out);
+          if (w.tail >= 0)
+            store_row32_f32(part + row * args.head_dim + c * 32, count, out);
           else
             store_row32<kKind>(static_cast<uint16_t*>(result) + to + c * 32, wide, count, out);
         }
@@ -811,7 +821,7 @@ template <int kKind, int kD, bool kPacked>
 int launch_dkv_typed(const Maps& maps, const Args& a, cudaStream_t stream) {
   static DeviceSetup setup;
   return launch<kD>("cross_dkv_kernel", cross_dkv_kernel<kKind, kD, kPacked>, setup,
-                    static_cast<int64_t>(a.tiles) * a.splits * a.k_heads, maps, a, stream);
+                    a.whole + static_cast<int64_t>(a.tail) * a.splits, maps, a, stream);
 }
 template <int kKind, int kD>
 int launch_shape(bool keys, const Maps& maps, const Args& a, cudaStream_t stream) {

@@ -18,22 +18,30 @@ Per-sample modulation and gates are applied by the native segment kernels on CUD
 code; the jagged, variable-length form for packed streams). Queries and keys may be turned by
 their positions (a table from :func:`~moss_image_b200.rotary.rotary_table`), and the frozen linears
 may be held in block-scaled fp8 instead of int8.
+
+A block may have a trained :class:`TextBranch`, in which its tokens look at a text encoder's states
+(:mod:`moss_image_b200.cross_attention`), and what training keeps of activations may be 8-bit codes
+(:mod:`moss_image_b200.activation_codes`): the inputs of checkpointed blocks (``coded_checkpoints`` of the
+stack) and of the trained projections (``coded_inputs`` of the blocks).
 """
 
 from __future__ import annotations
 
 import math
+from contextlib import nullcontext
 
 import torch
 from torch import nn
 from torch.nn import functional as F
 from torch.utils.checkpoint import checkpoint
 
+from .activation_codes import CodedActivation, coded_checkpoints, coded_linear, encode_activation
 from .activation_offload import KEEP_RESIDENT, activation_cpu_offload
+from .cross_attention import cross_attention, cross_attention_packed
 from .fp8 import quantize_frozen_linears_fp8
 from .lora import LoRALinear
 from .memory import offloaded_block
-from .norms import rms_norm
+from .norms import layer_norm, rms_norm
 from .packed import (
     CHECKPOINT_CHECK,
     batch_offsets,
@@ -66,6 +74,66 @@ class RMSNorm(nn.Module):
         return normalized.to(x.dtype) * self.weight
 
 
+class LayerNorm(nn.Module):
+    """Layer norm with a learned gain and offset; CUDA inputs run the native kernels."""
+
+    def __init__(self, dim: int, eps: float = 1e-6) -> None:
+        super().__init__()
+        self.eps = eps
+        self.weight = nn.Parameter(torch.ones(dim))
+        self.bias = nn.Parameter(torch.zeros(dim))
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        if x.is_cuda:
+            return layer_norm(x, self.weight, self.bias, self.eps)
+        return F.layer_norm(x.float(), x.shape[-1:], self.weight.float(), self.bias.float(), self.eps).to(x.dtype)
+
+
+def project(linear: nn.Module, tokens: torch.Tensor, coded: CodedActivation | None) -> torch.Tensor:
+    """``linear(tokens)``; a trained one keeps the tokens' codes for its gradient where they are given."""
+    if coded is not None and isinstance(linear, LoRALinear):
+        return linear(tokens, coded)
+    if coded is not None and isinstance(linear, nn.Linear) and linear.weight.requires_grad:
+        return coded_linear(tokens, linear.weight, linear.bias, coded=coded)
+    return linear(tokens)
+
+
+class TextBranch(nn.Module):
+    """``tokens + o(attention(q(norm(tokens)), k(context), v(context)))``: a trained residual branch in which image
+    tokens look at a text encoder's states. ``o`` starts at zero, so a new branch changes nothing."""
+
+    def __init__(self, dim: int, heads: int, text_dim: int, k_heads: int | None = None) -> None:
+        super().__init__()
+        self.head_dim = dim // heads
+        shared = (heads if k_heads is None else k_heads) * self.head_dim
+        self.norm = LayerNorm(dim)
+        self.q = nn.Linear(dim, dim, bias=False)
+        self.k = nn.Linear(text_dim, shared, bias=False)
+        self.v = nn.Linear(text_dim, shared, bias=False)
+        self.o = nn.Linear(dim, dim, bias=False)
+        nn.init.zeros_(self.o.weight)
+        self.coded_inputs = False
+
+    def forward(self, tokens: torch.Tensor, context: torch.Tensor, keys: torch.Tensor | None = None,
+                offsets: torch.Tensor | None = None) -> torch.Tensor:
+        """``tokens`` ``[B, T, dim]`` and ``context`` ``[B, S, text_dim]`` with an optional bool mask ``keys`` ``[B, S]``; or, with
+        the stream's boundaries ``offsets``, ``[1, total, dim]``, ``[1, states, text_dim]`` and the captions' boundaries ``keys``."""
+        coded = self.coded_inputs and torch.is_grad_enabled()
+
+        def heads(linear: nn.Linear, x: torch.Tensor, codes: CodedActivation | None) -> torch.Tensor:
+            return project(linear, x, codes).unflatten(-1, (-1, self.head_dim))
+
+        h = self.norm(tokens)
+        q = heads(self.q, h, encode_activation(h) if coded else None)
+        states = encode_activation(context) if coded else None  # one set of codes for both
+        k, v = heads(self.k, context, states), heads(self.v, context, states)
+        if offsets is None:
+            attended = cross_attention(q, k, v, key_mask=keys).flatten(2)
+        else:
+            attended = cross_attention_packed(q[0], k[0], v[0], offsets, keys).flatten(1)[None]
+        return tokens + project(self.o, attended, encode_activation(attended) if coded else None)
+
+
 class SyntheticBlock(nn.Module):
     """One joint attention + MLP block with its own adaLN modulation linear."""
 
@@ -81,12 +149,16 @@ class SyntheticBlock(nn.Module):
         self.mlp_up = nn.Linear(dim, mlp_dim, bias=True)
         self.mlp_down = nn.Linear(mlp_dim, dim, bias=True)
         self.adaln = nn.Linear(dim, 6 * dim, bias=True)
+        self.text: TextBranch | None = None
+        self.coded_inputs = False
 
     def forward(self, tokens: torch.Tensor, cond: torch.Tensor, cu_seqlens: torch.Tensor | None = None,
-                cos: torch.Tensor | None = None, sin: torch.Tensor | None = None) -> torch.Tensor:
+                cos: torch.Tensor | None = None, sin: torch.Tensor | None = None, context: torch.Tensor | None = None,
+                keys: torch.Tensor | None = None) -> torch.Tensor:
         """tokens: [B, T, dim] with cond [B, dim] (timestep embedding per sample), or a packed
         [1, total, dim] stream with cu_seqlens (int64 [S + 1]) and cond [S, dim]. With ``cos`` and
-        ``sin`` (float32 [T, half], one row per token) q and k are turned by their positions.
+        ``sin`` (float32 [T, half], one row per token) q and k are turned by their positions. ``context`` and ``keys``:
+        what the text branch looks at (:meth:`TextBranch.forward`), between the attention and the MLP.
 
         The conditioning follows training/model.py:288-312: ``norm(x) * (1 + scale) + shift``
         and ``x + branch * gate`` per sample, each op rounded in the activation dtype. On CUDA
@@ -114,9 +186,11 @@ class SyntheticBlock(nn.Module):
                 return x + branch * condition_for_tokens(gate, index)
 
         h = modulate(self.norm1(tokens), scale_a, shift_a)
-        q = self.q_norm(self.proj["q"](h).unflatten(-1, (self.heads, -1)))
-        k = self.k_norm(self.proj["k"](h).unflatten(-1, (self.heads, -1)))
-        v = self.proj["v"](h).unflatten(-1, (self.heads, -1))
+        keep_codes = self.coded_inputs and tokens.is_cuda and torch.is_grad_enabled()
+        coded = encode_activation(h) if keep_codes else None  # of q, k and v
+        q = self.q_norm(project(self.proj["q"], h, coded).unflatten(-1, (self.heads, -1)))
+        k = self.k_norm(project(self.proj["k"], h, coded).unflatten(-1, (self.heads, -1)))
+        v = project(self.proj["v"], h, coded).unflatten(-1, (self.heads, -1))
         if cos is not None:
             q, k = apply_rotary(q, k, cos, sin)
         if cu_seqlens is None:
@@ -124,7 +198,10 @@ class SyntheticBlock(nn.Module):
             attended = attended.transpose(1, 2).flatten(2)
         else:
             attended = varlen_attention(q[0], k[0], v[0], offsets, sequence_lengths(cu_seqlens)).flatten(1)[None]
-        tokens = gated(tokens, self.proj["o"](attended), gate_a)
+        coded = encode_activation(attended) if keep_codes else None
+        tokens = gated(tokens, project(self.proj["o"], attended, coded), gate_a)
+        if self.text is not None and context is not None:
+            tokens = self.text(tokens, context, keys, cu_seqlens)
         h = modulate(self.norm2(tokens), scale_f, shift_f)
         return gated(tokens, self.mlp_down(F.gelu(self.mlp_up(h), approximate="tanh")), gate_f)
 
@@ -156,24 +233,31 @@ class SyntheticDiT(nn.Module):
         self.final_norm = RMSNorm(dim)
         self.gradient_checkpointing = gradient_checkpointing
         self.activation_offload = False
+        self.coded_checkpoints = False
 
     def forward(self, tokens: torch.Tensor, timestep: torch.Tensor, skip_layers: tuple[int, ...] = (),
-                rotary: tuple[torch.Tensor, torch.Tensor] | None = None) -> torch.Tensor:
-        """``rotary``: the (cos, sin) tables of the tokens' positions, shared by all blocks."""
-        with activation_cpu_offload(self, self.activation_offload, tokens.device):
+                rotary: tuple[torch.Tensor, torch.Tensor] | None = None, context: torch.Tensor | None = None,
+                context_mask: torch.Tensor | None = None) -> torch.Tensor:
+        """``rotary``: the (cos, sin) tables of the tokens' positions, shared by all blocks. ``context`` ``[B, S, text_dim]``
+        and its bool mask ``[B, S]``: the states that the blocks' text branches look at."""
+        scope = activation_cpu_offload(self, self.activation_offload, tokens.device)
+        with scope:
             cond = self.time_embedding(timestep).to(tokens.dtype)
-            tokens = self._run_layers(tokens, cond, frozenset(skip_layers), rotary=rotary)
+            tokens = self._run_layers(tokens, cond, frozenset(skip_layers), rotary=rotary, context=context,
+                                      keys=context_mask, scope=scope)
             return self.final_norm(tokens)
 
     def forward_packed(self, samples: list[torch.Tensor], timestep: torch.Tensor,
-                       rotary: tuple[torch.Tensor, torch.Tensor] | None = None) -> list[torch.Tensor]:
+                       rotary: tuple[torch.Tensor, torch.Tensor] | None = None,
+                       context: list[torch.Tensor] | None = None) -> list[torch.Tensor]:
         """One traversal over a heterogeneous batch: ``samples[i]`` is ``[tokens_i, dim]``.
 
         Mirrors ``forward_packed`` (training/model.py:502-626): the samples are concatenated
         into one ``[1, total, dim]`` stream with cumulative boundaries, every linear runs once
         over all tokens, attention is isolated per sample, and each sample keeps its own
         timestep conditioning. ``rotary``: the (cos, sin) tables of the stream, one row per token, the
-        samples' one after another. Returns the per-sample outputs.
+        samples' one after another. ``context[i]``: ``[states_i, text_dim]`` of sample i (none for an empty
+        caption). Returns the per-sample outputs.
         """
         if not samples:
             raise ValueError("forward_packed requires at least one sample.")
@@ -188,14 +272,23 @@ class SyntheticDiT(nn.Module):
         cu_seqlens.moss_lengths = tuple(lengths)  # known on the host: no device read per block
         setattr(cu_seqlens, KEEP_RESIDENT, True)  # the same boundaries tensor in every recomputation
         tokens = torch.cat(samples, 0).unsqueeze(0)
-        with activation_cpu_offload(self, self.activation_offload, device):
+        states = keys = None
+        if context is not None:
+            if len(context) != len(samples):
+                raise ValueError("A packed batch has one context for each of its samples.")
+            states = torch.cat(context, 0).unsqueeze(0)
+            keys = cumulative_lengths([c.shape[0] for c in context], device)
+            setattr(keys, KEEP_RESIDENT, True)
+        scope = activation_cpu_offload(self, self.activation_offload, device)
+        with scope:
             cond = self.time_embedding(times).to(tokens.dtype)
-            tokens = self._run_layers(tokens, cond, frozenset(), cu_seqlens, rotary)
+            tokens = self._run_layers(tokens, cond, frozenset(), cu_seqlens, rotary, states, keys, scope)
             return list(self.final_norm(tokens)[0].split(lengths, 0))
 
     def _run_layers(self, tokens: torch.Tensor, cond: torch.Tensor, skipped: frozenset[int],
                     cu_seqlens: torch.Tensor | None = None,
-                    rotary: tuple[torch.Tensor, torch.Tensor] | None = None) -> torch.Tensor:
+                    rotary: tuple[torch.Tensor, torch.Tensor] | None = None, context: torch.Tensor | None = None,
+                    keys: torch.Tensor | None = None, scope: object = None) -> torch.Tensor:
         """Resident, synchronously swapped or streamed blocks, as ``place_model`` left them.
 
         Mirrors training/model.py:672-709: blocks at or past ``len(layers) - blocks_to_swap``
@@ -217,6 +310,8 @@ class SyntheticDiT(nn.Module):
             inputs = (tokens, cond) if cu_seqlens is None else (tokens, cond, cu_seqlens)
             if rotary is not None:
                 inputs = (tokens, cond, cu_seqlens, *rotary)
+            if context is not None:
+                inputs = (tokens, cond, cu_seqlens, *(rotary or (None, None)), context, keys)
             if manager is not None and index >= boundary:
                 at = position[index]
                 tokens = manager.block(
@@ -228,7 +323,8 @@ class SyntheticDiT(nn.Module):
             elif index >= boundary:
                 tokens = offloaded_block(layer, *inputs)
             elif self.gradient_checkpointing and self.training and torch.is_grad_enabled():
-                tokens = checkpoint(layer, *inputs, use_reentrant=False, determinism_check=CHECKPOINT_CHECK)
+                with coded_checkpoints(tokens, scope) if self.coded_checkpoints else nullcontext():
+                    tokens = checkpoint(layer, *inputs, use_reentrant=False, determinism_check=CHECKPOINT_CHECK)
             else:
                 tokens = layer(*inputs)
         return tokens
@@ -262,7 +358,7 @@ def _inject_block(layer: SyntheticBlock, rank: int, alpha: float, targets: tuple
 def build_lora_model(depth: int, *, device: torch.device, dim: int = 3072, heads: int = 24, mlp_dim: int = 12288,
                      rank: int = 32, alpha: float | None = None, seed: int = 0,
                      dtype: torch.dtype = torch.bfloat16, full_qkvo: bool = False,
-                     frozen: str = "int8") -> SyntheticDiT:
+                     frozen: str = "int8", text_dim: int | None = None, coded: bool = False) -> SyntheticDiT:
     """Random-init stack (weights ~ N(0, 0.02)), int8 base, LoRA on q/k/v/o.
 
     Mirrors the trainer's order (training/train.py:577-589): build, cast, inject LoRA,
@@ -273,7 +369,9 @@ def build_lora_model(depth: int, *, device: torch.device, dim: int = 3072, heads
     ``dtype`` masters, no adapters) and every other linear is frozen int8: the hybrid that
     ``quantize_frozen_linears`` allows at module level (training/quantization.py:156-157;
     the reference trainer itself only pairs int8 bases with LoRA, training/train.py:543-545).
-    ``frozen="fp8"`` holds the frozen linears as block-scaled fp8 (:mod:`moss_image_b200.fp8`).
+    ``frozen="fp8"`` holds the frozen linears as block-scaled fp8 (:mod:`moss_image_b200.fp8`). ``text_dim`` gives
+    every block a trained :class:`TextBranch` over states of that width. ``coded`` keeps block and projection
+    inputs as 8-bit codes (``coded_checkpoints``, ``coded_inputs``).
     """
     if frozen not in ("int8", "fp8"):
         raise ValueError("frozen linears are held as int8 or fp8.")
@@ -302,8 +400,15 @@ def build_lora_model(depth: int, *, device: torch.device, dim: int = 3072, heads
         else:
             _inject_block(block, rank, alpha, ("q", "k", "v", "o"), 0.01)
         quantize(block)
+        if text_dim is not None:
+            block.text = TextBranch(dim, heads, text_dim)
+            for linear in (block.text.q, block.text.k, block.text.v):
+                nn.init.normal_(linear.weight, 0.0, 0.02)
+            block.text.to(device=device, dtype=dtype).coded_inputs = coded
+        block.coded_inputs = coded
         layers.append(block)
     model.layers = nn.ModuleList(layers)
+    model.coded_checkpoints = coded
     return model
 
 
@@ -327,11 +432,12 @@ def packed_flow_matching_loss(model: SyntheticDiT, latents: list[torch.Tensor], 
 
 
 def flow_matching_loss(model: SyntheticDiT, latents: torch.Tensor, text: torch.Tensor, t: torch.Tensor,
-                       noise: torch.Tensor, rotary: tuple[torch.Tensor, torch.Tensor] | None = None) -> torch.Tensor:
-    """Rectified-flow velocity loss on the image tokens (text tokens are conditioning)."""
+                       noise: torch.Tensor, rotary: tuple[torch.Tensor, torch.Tensor] | None = None,
+                       context: torch.Tensor | None = None, context_mask: torch.Tensor | None = None) -> torch.Tensor:
+    """Rectified-flow velocity loss on the image tokens (text tokens are conditioning, and so is the text branches' ``context``)."""
     sigma = t.view(-1, 1, 1).to(latents.dtype)
     noisy = (1 - sigma) * latents + sigma * noise
     tokens = torch.cat((noisy, text), dim=1)
-    pred = model(tokens, t, rotary=rotary)[:, : latents.shape[1]]
+    pred = model(tokens, t, rotary=rotary, context=context, context_mask=context_mask)[:, : latents.shape[1]]
     target = noise - latents
     return F.mse_loss(pred.float(), target.float())

@@ -14,7 +14,8 @@ and the input gradient is likewise one launch,
     dx = dy dec(W) + (dy B) (scale * A)                  (rank-r block appended to N)
 
 with the two small rank-r products (``x A^T`` and ``dy B``) and the adapter weight
-gradients done as plain library GEMMs. The reference adds the update after rounding the
+gradients done as plain library GEMMs (``lora_A``'s by the native kernel from 8-bit codes, where the
+caller gives the input's codes to keep in its place). The reference adds the update after rounding the
 base output and the update separately (``result + update.to(result.dtype) * scale``); the
 fused form rounds once, which stays within the 5e-3 relative-Frobenius bar.
 
@@ -29,20 +30,22 @@ import torch
 from torch import nn
 from torch.nn import functional as F
 
+from .activation_codes import CodedActivation, coded_weight_gradient
 from .quant_kernels import autocast_compute_dtype, int8_linear_backward, int8_linear_forward, resolve_quantized_backend
 from .quantization import FrozenInt8Linear
 
 
 class _FusedLoRAInt8Linear(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, tokens, lora_a, lora_b, weight, scale, bias, weight_dtype, backend, lora_scale, compute_dtype):
+    def forward(ctx, tokens, lora_a, lora_b, weight, scale, bias, weight_dtype, backend, lora_scale, compute_dtype,
+                codes=None, exponents=None):
         resolve_quantized_backend(backend, tokens, weight, scale)
         x = tokens.to(compute_dtype)
         a = lora_a.to(compute_dtype)
         xa = F.linear(x, a)  # [.., r] plain library GEMM (rank r)
         y = int8_linear_forward(x, weight, scale, bias, compute_dtype, weight_dtype, lora_xa=xa, lora_b=lora_b,
                                 lora_scale=lora_scale)
-        ctx.save_for_backward(x, xa, lora_a, lora_b, weight, scale)
+        ctx.save_for_backward(x if codes is None else None, xa, lora_a, lora_b, weight, scale, codes, exponents)
         ctx.input_dtype = tokens.dtype
         ctx.input_shape = tokens.shape
         ctx.weight_dtype = weight_dtype
@@ -52,7 +55,7 @@ class _FusedLoRAInt8Linear(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, gradient):
-        x, xa, lora_a, lora_b, weight, scale = ctx.saved_tensors
+        x, xa, lora_a, lora_b, weight, scale, codes, exponents = ctx.saved_tensors
         cd = ctx.compute_dtype
         g = gradient.to(cd)
         g2 = g.reshape(-1, g.shape[-1])
@@ -65,13 +68,15 @@ class _FusedLoRAInt8Linear(torch.autograd.Function):
                                               lora_scale=ctx.lora_scale)
         grad_a = grad_b = None
         s = ctx.lora_scale
-        if ctx.needs_input_grad[1]:
+        if ctx.needs_input_grad[1] and codes is not None:
+            grad_a = coded_weight_gradient(dyb, codes, exponents, torch.float32).mul_(s).to(lora_a.dtype)
+        elif ctx.needs_input_grad[1]:
             x2 = x.reshape(-1, x.shape[-1])
             grad_a = (dyb.t() @ x2).to(lora_a.dtype).mul_(s)
         if ctx.needs_input_grad[2]:
             xa2 = xa.reshape(-1, xa.shape[-1])
             grad_b = (g2.t() @ xa2).to(lora_b.dtype).mul_(s)
-        return grad_input, grad_a, grad_b, None, None, None, None, None, None, None
+        return grad_input, grad_a, grad_b, None, None, None, None, None, None, None, None, None
 
 
 class LoRALinear(nn.Module):
@@ -114,7 +119,10 @@ class LoRALinear(nn.Module):
             compute_dtype = torch.get_autocast_dtype(tokens.device.type)
         return compute_dtype
 
-    def forward(self, tokens: torch.Tensor) -> torch.Tensor:
+    def forward(self, tokens: torch.Tensor, coded: CodedActivation | None = None) -> torch.Tensor:
+        """``coded``: codes of the tokens, which the fused form then keeps in their place for ``lora_A``'s gradient."""
+        if coded is not None and (coded.shape != tokens.shape or coded.codes.device != tokens.device):
+            raise ValueError("The codes are not those of these tokens (another shape or device).")
         adapter_dtype = self._adapter_dtype(tokens)
         base = self.base
         if (
@@ -127,6 +135,7 @@ class LoRALinear(nn.Module):
             return _FusedLoRAInt8Linear.apply(
                 tokens, self.lora_A, self.lora_B, base.weight_int8, base.weight_scale, base.bias,
                 base.compute_dtype, base.quantized_backend, float(self.scale), adapter_dtype,
+                *(() if coded is None else (coded.codes, coded.exponents)),
             )
         # Reference composition (training/lora.py:70-86).
         result = base(tokens)
