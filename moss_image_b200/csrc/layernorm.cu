@@ -207,8 +207,9 @@ __global__ void __launch_bounds__(kThreads) layernorm_fwd_kernel(const Args a) {
   }
   fetch(row);
   float* const offset = gain + (a.dim + 3) / 4 * 4;
-  stage_gain(gain, a.w, a.g_kind, a.dim, 1.0f);
-  stage_gain(offset, a.b, a.g_kind, a.dim, 0.0f);
+  const bool plain = a.w == nullptr && a.b == nullptr;
+  if (!plain) stage_gain(gain, a.w, a.g_kind, a.dim, 1.0f);
+  if (!plain) stage_gain(offset, a.b, a.g_kind, a.dim, 0.0f);
   __syncthreads();
   for (; row < last; row += step) {
     Raw<KX, V> held[C];
@@ -242,12 +243,18 @@ __global__ void __launch_bounds__(kThreads) layernorm_fwd_kernel(const Args a) {
     for (int i = 0; i < C; ++i) {
       const int at = (thread + i * T) * V;
       if (at >= a.dim) continue;
-      float f[V], w[V], b[V];
+      float f[V];
       widen<KX, V>(held[i], f);
-      gain_at<V>(gain, at, w);
-      gain_at<V>(offset, at, b);
+      if (plain) {
 #pragma unroll
-      for (int j = 0; j < V; ++j) f[j] = fmaf((f[j] - mean) * rstd, w[j], b[j]);
+        for (int j = 0; j < V; ++j) f[j] = (f[j] - mean) * rstd;
+      } else {
+        float w[V], b[V];
+        gain_at<V>(gain, at, w);
+        gain_at<V>(offset, at, b);
+#pragma unroll
+        for (int j = 0; j < V; ++j) f[j] = fmaf((f[j] - mean) * rstd, w[j], b[j]);
+      }
       store<KY, V>(a.out, row * a.dim + at, f);
     }
   }
