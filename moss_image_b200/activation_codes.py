@@ -209,6 +209,8 @@ def coded_linear(tokens: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor 
         raise ValueError("coded_linear: the weight must be [out, in] for [..., in] tokens.")
     if bias is not None and bias.shape != weight.shape[:1]:
         raise ValueError("coded_linear: the bias must be [out].")
+    if torch.is_autocast_enabled("cuda") and torch.get_autocast_dtype("cuda") != tokens.dtype:
+        raise ValueError("coded_linear: autocast runs in another dtype than the tokens and the weight have.")
     if coded is not None and (coded.shape != tokens.shape or coded.codes.device != tokens.device):
         raise ValueError("coded_linear: the codes are not those of these tokens (another shape or device).")
     _lib.refuse_forward_mode("coded_linear", *given)

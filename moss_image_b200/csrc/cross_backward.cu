@@ -4,8 +4,8 @@
 //   dq:  a tile of 128 queries of one head against its key tiles:  S, dP = dO V^T, then dQ += dS K
 //   dkv: a tile of 128 keys of one key head against the query tiles of its heads, everything turned:
 //        S^T = K Q^T, dP^T = V dO^T, then dV += P^T dO and dK += dS^T Q
-// Seven products for a tile pair where five would do with dQ added up across CTAs; the two more cost less than f32
-// additions of dQ to memory for every key tile (32 bytes a value and key tile against 16 tensor-core cycles).
+// Seven products for a tile pair where five would do with dQ added up across CTAs: a dQ value would be written and read in
+// f32 for every key tile, 900 MB for 2 x 24 heads of 128, 4096 x 512 tokens, 140 us against 40 for the two products more.
 // The dq kernel also takes delta = rowsum(O dO) on the way, which the other reads.
 //
 // In both, P and dS are written over S and dP in TMEM as 16-bit pairs and feed the next product from there; a thread has a

@@ -311,8 +311,7 @@ template <int KX, int KY, int V, int C>
 constexpr uint32_t stage_bytes() { return Staged<KX, V, C>::kRow + Staged<KY, V, C>::kRow; }
 
 // kGain: the sums for dw and db are wanted (up to 64 registers a thread, and a reduction at the end). The rows that a
-// team takes next are on their way, `stages` at a time (without them a team waits for every row: 9216 x 3072
-// took 60 us, 1.5 times as long).
+// team takes next are on their way, `stages` at a time (9216 x 3072 bf16: 47 us, 50 without).
 template <int KX, int KY, int T, int V, int C, bool kGain>
 __global__ void __launch_bounds__(kThreads) layernorm_bwd_kernel(const Args a, int stages) {
   extern __shared__ __align__(16) float gain[];  // w, padded to 4 values; then the stages, and [2][dim] joined sums in their place

@@ -14,6 +14,7 @@ from torch.utils.checkpoint import checkpoint
 
 from moss_image_b200.activation_codes import (CodedActivation, coded_checkpoints, coded_linear, coded_weight_gradient,
                                               decode_activation, encode_activation)
+from moss_image_b200.activation_offload import activation_cpu_offload
 
 pytestmark = pytest.mark.gpu
 
@@ -258,6 +259,22 @@ def test_coded_checkpoint_recomputes_from_the_decoded_input(cuda_device):
     assert all(torch.equal(a, b) for a, b in zip(got, expected))
 
 
+@pytest.mark.parametrize("width", [64, 50])
+def test_codes_leave_with_the_offload(cuda_device, width):
+    torch.manual_seed(1)
+    block = torch.nn.Linear(width, width).to("cuda", BF16)
+    leaf = torch.randn(7, width, device="cuda").to(BF16).requires_grad_()
+    dy = torch.randn(7, width, device="cuda").to(BF16)
+    grads = []
+    for offload in (False, True):
+        scope = activation_cpu_offload(block, offload, leaf.device)
+        x = leaf * 1.0
+        with scope, coded_checkpoints(x, scope):
+            y = checkpoint(block, x, use_reentrant=False)
+        grads.append(torch.autograd.grad(y, [leaf, *block.parameters()], dy))
+    assert all(torch.equal(a, b) for a, b in zip(*grads))
+
+
 def test_refusals(cuda_device):
     x = torch.randn(8, 64, device="cuda", dtype=BF16)
     coded = encode_activation(x)
@@ -277,6 +294,8 @@ def test_refusals(cuda_device):
         coded_linear(x, torch.randn(4, 64, device="cuda"))
     with pytest.raises(ValueError, match="not those"):
         coded_linear(x, torch.randn(4, 64, device="cuda", dtype=BF16), coded=encode_activation(x[:4]))
+    with torch.autocast("cuda", F16), pytest.raises(ValueError, match="autocast"):
+        coded_linear(x, torch.randn(4, 64, device="cuda", dtype=BF16))
     weight = torch.randn(4, 64, device="cuda", dtype=BF16, requires_grad=True)
     slope, = torch.autograd.grad(coded_linear(x.requires_grad_(), weight).float().square().sum(), weight, create_graph=True)
     with pytest.raises(RuntimeError):
