@@ -282,14 +282,15 @@ __device__ __forceinline__ uint64_t add_pair(uint64_t a, uint64_t b) {
   return d;
 }
 
-// 2^x of a pair on the CUDA cores, x in [-126, 127] (below it 2^-126, NaN and +inf NaN): 2^n p(f) with n the nearest whole
-// number and p the polynomial of degree 4 that is nearest to 2^f on [-1/2, 1/2] in relative error (Remez' exchange),
-// 2^-18.5 off at most. A multiprocessor's special-function units give 16 exponentials a cycle, which is what bounds the
-// softmax; a part of them is computed here meanwhile.
+// 2^x of a pair on the CUDA cores, x up to 127 (below -126.5 zero, -inf too; NaN and +inf give NaN): 2^n p(f) with n the
+// nearest whole number and p the polynomial of degree 4 that is nearest to 2^f on [-1/2, 1/2] in relative error (Remez'
+// exchange), 2^-18.5 off at most. A multiprocessor's special-function units give 16 exponentials a cycle, which is what bounds
+// the softmax; a part of them is computed here meanwhile. 2^n is a factor, not an addition to p's exponent bits: a sum of
+// bits would turn a NaN into a number. n = -127 has the bits of zero.
 __device__ __forceinline__ uint64_t exp2_pair(uint64_t x) {
   float x0, x1;
   split_pair(x, x0, x1);
-  x = pair_of(max_nan(x0, -126.0f), max_nan(x1, -126.0f));
+  x = pair_of(max_nan(x0, -127.0f), max_nan(x1, -127.0f));
   const uint64_t t = add_pair(x, pair_of(12582912.0f, 12582912.0f));  // 1.5 * 2^23: the low bits are n
   const uint64_t n = add_pair(t, pair_of(-12582912.0f, -12582912.0f));
   const uint64_t f = fma_pair(n, pair_of(-1.0f, -1.0f), x);
@@ -297,20 +298,18 @@ __device__ __forceinline__ uint64_t exp2_pair(uint64_t x) {
   p = fma_pair(f, p, pair_of(0.240247443318367f, 0.240247443318367f));
   p = fma_pair(f, p, pair_of(0.6931217908859253f, 0.6931217908859253f));
   p = fma_pair(f, p, pair_of(0.9999992847442627f, 0.9999992847442627f));
-  float p0, p1, t0, t1;
-  split_pair(p, p0, p1);
+  float t0, t1;
   split_pair(t, t0, t1);
-  return pair_of(__uint_as_float((__float_as_uint(t0) << 23) + __float_as_uint(p0)),
-                 __uint_as_float((__float_as_uint(t1) << 23) + __float_as_uint(p1)));
+  return mul_pair(p, pair_of(__uint_as_float((__float_as_uint(t0) << 23) + 0x3f800000u),
+                             __uint_as_float((__float_as_uint(t1) << 23) + 0x3f800000u)));
 }
 // Of `i`-th pairs, those that are computed that way.
 __device__ __forceinline__ constexpr bool by_polynomial(int i) { return i % 3 == 2; }
 
-// 2^(s scale - shift) of the pair s; kAll: by the special-function unit in any case (it gives a masked value's zero).
-template <bool kAll>
+// 2^(s scale - shift) of the i-th pair s of a row.
 __device__ __forceinline__ uint64_t exponentials(int i, uint64_t s, uint64_t scale, uint64_t minus_shift) {
   const uint64_t x = fma_pair(s, scale, minus_shift);
-  if (!kAll && by_polynomial(i)) return exp2_pair(x);
+  if (by_polynomial(i)) return exp2_pair(x);
   float x0, x1;
   split_pair(x, x0, x1);
   return pair_of(exp2_approx(x0), exp2_approx(x1));

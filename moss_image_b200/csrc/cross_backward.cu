@@ -445,12 +445,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         load64(s_tmem, s);
         load64(dp_tmem + half * kHalf + lanes, g);
         float v[64];
-        // (what the polynomial leaves of an exponential that should be zero, 2^-126, is nothing to a gradient; a row without keys
-        // has lse = inf, and its 2^-126 is masked)
+        // (a row without keys has lse = inf, which makes its exponentials zero)
         const uint64_t scale2 = pair_of(args.scale_log2, args.scale_log2), minus_lse = pair_of(-lse, -lse), minus_delta = pair_of(-delta, -delta);
 #pragma unroll
         for (int j = 0; j < 64; j += 2) {
-          const uint64_t p = exponentials<false>(j / 2, pair_of(__uint_as_float(s[j >> 5][j & 31]), __uint_as_float(s[j >> 5][(j & 31) + 1])),
+          const uint64_t p = exponentials(j / 2, pair_of(__uint_as_float(s[j >> 5][j & 31]), __uint_as_float(s[j >> 5][(j & 31) + 1])),
                                                  scale2, minus_lse);
           const uint64_t d = add_pair(pair_of(__uint_as_float(g[j >> 5][j & 31]), __uint_as_float(g[j >> 5][(j & 31) + 1])), minus_delta);
           split_pair(mul_pair(p, d), v[j], v[j + 1]);
@@ -716,9 +715,9 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int j = 0; j < 64; j += 4) {  // (the sums are kept negated, and lifted)
           const float4 l = *reinterpret_cast<const float4*>(lse + j);
-          const uint64_t lo = exponentials<false>(j / 2, pair_of(__uint_as_float(r[j >> 5][j & 31]), __uint_as_float(r[j >> 5][(j & 31) + 1])),
+          const uint64_t lo = exponentials(j / 2, pair_of(__uint_as_float(r[j >> 5][j & 31]), __uint_as_float(r[j >> 5][(j & 31) + 1])),
                                                   scale2, pair_of(l.x, l.y));
-          const uint64_t hi = exponentials<false>(j / 2 + 1, pair_of(__uint_as_float(r[j >> 5][(j & 31) + 2]), __uint_as_float(r[j >> 5][(j & 31) + 3])),
+          const uint64_t hi = exponentials(j / 2 + 1, pair_of(__uint_as_float(r[j >> 5][(j & 31) + 2]), __uint_as_float(r[j >> 5][(j & 31) + 3])),
                                                   scale2, pair_of(l.z, l.w));
           split_pair(lo, v[j], v[j + 1]);
           split_pair(hi, v[j + 2], v[j + 3]);

@@ -19,7 +19,6 @@
 #include <algorithm>
 #include <cmath>
 #include <cstring>
-#include <type_traits>
 
 #include "cross_args.cuh"
 
@@ -400,11 +399,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           tmem_ld_32x32b_x32(s_tmem + 32, r[1]);
           wait_ld_of(r[0]);
           wait_ld_of(r[1]);
-          bool some_masked;
           if constexpr (kMask) {
             const uint32_t k0 = half == 0 ? keep.w[0] : keep.w[2], k1 = half == 0 ? keep.w[1] : keep.w[3];
-            some_masked = (k0 & k1) != 0xffffffffu;
-            if (some_masked) {
+            if ((k0 & k1) != 0xffffffffu) {
 #pragma unroll
               for (int j = 0; j < 32; ++j) {
                 if (((k0 >> j) & 1u) == 0) r[0][j] = 0xff800000u;
@@ -412,8 +409,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               }
             }
           } else {
-            some_masked = keys < kHalf;
-            if (some_masked) {
+            if (keys < kHalf) {
 #pragma unroll
               for (int j = 0; j < 64; ++j)
                 if (j >= keys) r[j >> 5][j & 31] = 0xff800000u;
@@ -422,7 +418,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           float most[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
           for (int j = 0; j < 64; ++j) most[j & 3] = fmaxf(most[j & 3], __uint_as_float(r[j >> 5][j & 31]));
-          // (the scale is positive, so the greatest product gives the greatest logit)
+          // (the scale is positive, so the greatest product gives the greatest logit; fmaxf drops NaN, whose exponential is NaN against
+          // any reference)
           const float here = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])) * args.scale_log2;
           const bool grows = here > top + kGrowth;  // (from -inf always, unless all keys are masked)
           if (__any_sync(0xffffffffu, grows)) {
@@ -452,26 +449,20 @@ __global__ void __launch_bounds__(kThreads, 1)
           const float shift = top == -INFINITY ? 0.0f : top - kLift<kKind>;
           const uint64_t scale2 = pair_of(args.scale_log2, args.scale_log2), minus_shift = pair_of(-shift, -shift);
           uint64_t add[2] = {0, 0};
-          auto exponentiate = [&](auto all) {
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              uint32_t p[16];
+          for (int c = 0; c < 2; ++c) {
+            uint32_t p[16];
 #pragma unroll
-              for (int j = 0; j < 16; ++j) {
-                const uint64_t e = exponentials<decltype(all)::value>(
-                    c * 16 + j, pair_of(__uint_as_float(r[c][2 * j]), __uint_as_float(r[c][2 * j + 1])), scale2, minus_shift);
-                add[j & 1] = add_pair(add[j & 1], e);
-                float e0, e1;
-                split_pair(e, e0, e1);
-                p[j] = gemm::pack2_kind<kKind>(e0, e1);
-              }
-              tmem_st_32x32b_x16(s_tmem + c * 16, p);
+            for (int j = 0; j < 16; ++j) {
+              const uint64_t e = exponentials(c * 16 + j, pair_of(__uint_as_float(r[c][2 * j]), __uint_as_float(r[c][2 * j + 1])),
+                                              scale2, minus_shift);
+              add[j & 1] = add_pair(add[j & 1], e);
+              float e0, e1;
+              split_pair(e, e0, e1);
+              p[j] = gemm::pack2_kind<kKind>(e0, e1);
             }
-          };
-          if (some_masked)
-            exponentiate(std::true_type{});
-          else
-            exponentiate(std::false_type{});
+            tmem_st_32x32b_x16(s_tmem + c * 16, p);
+          }
           float add0, add1;
           split_pair(add_pair(add[0], add[1]), add0, add1);
           sum += add0 + add1;

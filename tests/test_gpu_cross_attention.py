@@ -388,3 +388,71 @@ def test_refusals(cuda_device):
     with torch.autograd.forward_ad.dual_level():
         with pytest.raises(NotImplementedError):
             cross_attention(torch.autograd.forward_ad.make_dual(q, q), k, v)
+
+
+# ------------------------------------------------------------------------------------------ NaN and infinities that are looked at
+def _run_with_nan(q, k, v, grad, **options):
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    o = cross_attention(*leaves, **options)
+    got = [o.detach(), *torch.autograd.grad(o, leaves, grad)]
+    check_device_status(q.device)
+    return got
+
+
+def _assert_non_finite_as_defined(q, k, v, grad, mask, poisoned, head):
+    """NaN where the formulas have it, in float64, and nowhere else; other heads as without the poison; what stays finite of the
+    poisoned one is within its bounds (there the poisoned key's weight is zero)."""
+    scale = q.shape[-1] ** -0.5
+    allowed = torch.ones(q.shape[0], k.shape[1], dtype=torch.bool, device="cuda") if mask is None else mask
+    got = _run_with_nan(q, k, v, grad, key_mask=mask)
+    with_poison = _exact(q, k, v, allowed[:, None, None], scale, grad)
+    calm, left = k.clone(), allowed.clone()
+    calm[:, poisoned, head] = 0.0
+    left[:, poisoned] = False
+    without = _exact(q, calm, v, left[:, None, None], scale, grad)
+    clean = _run(q, calm, v, grad, key_mask=mask)
+    for part in (*with_poison[2:], *without[2:]):
+        part[0][~allowed] = 0.0  # a key that may not be looked at has no gradient, whatever the others hold
+    for name, value, (exact, _), (near, slack), other in zip(("o", "dq", "dk", "dv"), got, with_poison, without, clean):
+        assert torch.equal(value.isnan(), exact.isnan()), name
+        good = ~exact.isnan()
+        good[:, :, [h for h in range(value.shape[2]) if h != head]] = False
+        bound = slack + HALF_STEP[value.dtype] * (near.abs() + slack) + _least(value.dtype)
+        assert ((value.double() - near).abs()[good] <= bound[good]).all(), name
+        rest = [h for h in range(value.shape[2]) if h != head]
+        assert torch.equal(value[:, :, rest], other[:, :, rest]), name
+
+
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_non_finite_keys_that_are_looked_at(cuda_device, dim, dtype, masked):
+    q, k, v, grad = _tensors(1, 130, 140, 2, 2, dim, dtype, 11)
+    mask = None
+    if masked:  # a key that may not be looked at in the poisoned half tile
+        mask = torch.ones(1, 140, dtype=torch.bool, device="cuda")
+        mask[:, 20] = False
+    for key in (*range(12), 63, 139):
+        for poison in (float("nan"), float("inf"), -float("inf")):
+            bad = k.clone()
+            bad[0, key, 0, 5] = poison  # logits of both signs where it is an infinity
+            _assert_non_finite_as_defined(q, bad, v, grad, mask, [key], 0)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("tq,tk", [(130, 140), (1, 1024)])  # whole, and with the keys split
+def test_two_nan_keys_are_not_a_row_without_keys(cuda_device, tq, tk, dtype):
+    q, k, v, grad = _tensors(1, tq, tk, 1, 1, 64, dtype, 12)
+    k[0, 4], k[0, 5] = float("nan"), float("nan")
+    assert all(t.isnan().all() for t in _run_with_nan(q, k, v, grad))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("tq,tk", [(130, 140), (1, 1024)])
+def test_logits_of_minus_infinity_weigh_nothing(cuda_device, tq, tk, dtype):
+    q, k, v, grad = _tensors(1, tq, tk, 1, 1, 64, dtype, 13)
+    q[..., 3] = q[..., 3].abs() + 0.125
+    k[..., 3] = -float("inf")
+    o, dq, dk, dv = _run_with_nan(q, k, v, grad)
+    assert not o.any() and not dk.any() and not dv.any()
+    assert dq[..., 3].isnan().all() and not dq[..., :3].any() and not dq[..., 4:].any()  # 0 * inf
