@@ -378,7 +378,7 @@ struct TileBits {
 };
 
 // Whether key tile `tile` holds the only key that the sequence's queries look at. P is then 1 whatever the logit is, and the
-// gradient of the logit nothing (the difference dP - delta would leave its rounding). By a whole warp. A key alone in a mask
+// gradient of the logit nothing times dP - delta, whose rounding would be left otherwise. By a whole warp. A key alone in a mask
 // of too many tiles for TileBits is not found out.
 __device__ __forceinline__ bool only_key(const Args& a, const TileBits& taken, const Sequence& s, int tile) {
   if (s.kn == 1 || a.mask == nullptr) return s.kn == 1;

@@ -466,9 +466,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int j = 0; j < 64; ++j)
             if (j >= keys) v[j] = 0.0f;
         }
-        if (alone) {
+        if (alone) {  // (NaN stays)
 #pragma unroll
-          for (int j = 0; j < 64; ++j) v[j] = 0.0f;
+          for (int j = 0; j < 64; ++j) v[j] *= 0.0f;
         }
         store64<kKind>(s_tmem, v);
         tmem_wait_st();
@@ -749,10 +749,14 @@ __global__ void __launch_bounds__(kThreads, 1)
           split_pair(mul_pair(pair_of(v[j], v[j + 1]), lo), v[j], v[j + 1]);
           split_pair(mul_pair(pair_of(v[j + 2], v[j + 3]), hi), v[j + 2], v[j + 3]);
         }
-        if (!seen || alone || rows < kHalf) {
+        if (!seen || rows < kHalf) {
 #pragma unroll
           for (int j = 0; j < 64; ++j)
-            if (!seen || alone || j >= rows) v[j] = 0.0f;
+            if (!seen || j >= rows) v[j] = 0.0f;
+        }
+        if (alone) {  // (NaN stays)
+#pragma unroll
+          for (int j = 0; j < 64; ++j) v[j] *= 0.0f;
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&bars->stat_free[slot]));

@@ -456,3 +456,24 @@ def test_logits_of_minus_infinity_weigh_nothing(cuda_device, tq, tk, dtype):
     o, dq, dk, dv = _run_with_nan(q, k, v, grad)
     assert not o.any() and not dk.any() and not dv.any()
     assert dq[..., 3].isnan().all() and not dq[..., :3].any() and not dq[..., 4:].any()  # 0 * inf
+
+
+@pytest.mark.parametrize("masked", [False, True])
+def test_one_key_keeps_nan_in_its_gradients(cuda_device, masked):
+    tensors = _tensors(1, 50, 300 if masked else 1, 1, 1, 64, BF16, 14)
+    at = 260 if masked else 0
+    mask = None
+    if masked:
+        mask = torch.zeros(1, 300, dtype=torch.bool, device="cuda")
+        mask[:, at] = True
+    for which, place in ((0, (0, 5)), (1, (0, at)), (2, (0, at, 0, 3)), (3, (0, 5))):  # in q, k, v and the gradient of o
+        bad = [t.clone() for t in tensors]
+        bad[which][place] = float("nan")
+        q, k, v, grad = bad
+        dq, dk = (t.isnan() for t in _run_with_nan(q, k, v, grad, key_mask=mask)[1:3])
+        rows = torch.zeros(1, 50, 1, 64, dtype=torch.bool, device="cuda")
+        rows[(0, 5) if which in (0, 3) else ...] = True  # whose logit's gradient is NaN
+        assert torch.equal(dq, rows)
+        assert dk[0, at].all()
+        if which != 0:  # (the sum dS^T Q has the NaN of Q whatever dS is)
+            assert dk.sum() == 64
