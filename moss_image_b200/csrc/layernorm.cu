@@ -496,13 +496,15 @@ int ctas_of(int64_t rows, int team, int per_sm) {
   return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(asked, static_cast<int64_t>(per_sm) * device_sm_count())));
 }
 
+// most: the dynamic shared memory that the kernel is allowed, once for each device. (Asked for by call, it would be the last
+// caller's: another thread's launch between a call's request and its launch could then be refused.)
 template <typename F, typename... More>
-int launch_kernel(const char* what, F* kern, int ctas, size_t smem, const Args& a, cudaStream_t stream, More... more) {
-  // past what a kernel has unasked (with room for its fixed arrays)
-  if (smem > 40 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-    if (e != cudaSuccess) return check_cuda(e, what);
-  }
+int launch_kernel(const char* what, F* kern, DeviceSetup& setup, size_t most, int ctas, size_t smem, const Args& a, cudaStream_t stream,
+                  More... more) {
+  const int rc = setup(what, nullptr, [&](int*) {
+    return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(most));
+  });
+  if (rc != MOSS_OK) return rc;
   kern<<<ctas, kThreads, smem, stream>>>(a, more...);
   return check_cuda(cudaGetLastError(), what);
 }
@@ -510,17 +512,22 @@ int launch_kernel(const char* what, F* kern, int ctas, size_t smem, const Args& 
 template <int KX, int KY, int T, int V, int C>
 int launch(bool backward, const Args& a, cudaStream_t stream) {
   const size_t gain = static_cast<size_t>(a.dim + 3) / 4 * 4 * sizeof(float);
-  if (!backward)
-    return launch_kernel("layernorm_fwd_kernel", layernorm_fwd_kernel<KX, KY, T, V, C>, ctas_of(a.rows, T, 2), 2 * gain, a, stream);
+  if (!backward) {
+    static DeviceSetup setup;
+    constexpr size_t kMost = 2 * sizeof(float) * ((std::min(T * V * C, kMaxDim) + 3) / 4 * 4);
+    return launch_kernel("layernorm_fwd_kernel", layernorm_fwd_kernel<KX, KY, T, V, C>, setup, kMost, ctas_of(a.rows, T, 2), 2 * gain, a, stream);
+  }
   // the stages that fit one CTA a multiprocessor: three, two (f32 rows), or one (f32 rows past 8192 values)
   constexpr size_t kStage = stage_bytes<KX, KY, V, C>(), kRoom = 226 * 1024;
   const int stages = static_cast<int>(std::max<size_t>(1, std::min<size_t>(3, (kRoom - gain) / kStage)));
   const size_t joined = a.partial == nullptr || T == kThreads ? 0 : 2 * sizeof(float) * a.dim;
   const size_t smem = gain + std::max(stages * kStage, joined);
-  auto run = [&](auto kern) {
-    return launch_kernel("layernorm_bwd_kernel", kern, ctas_of(a.rows, T, 1), smem, a, stream, stages);
+  auto run = [&](auto kern, DeviceSetup& setup) {
+    return launch_kernel("layernorm_bwd_kernel", kern, setup, kRoom, ctas_of(a.rows, T, 1), smem, a, stream, stages);
   };
-  return a.partial == nullptr ? run(layernorm_bwd_kernel<KX, KY, T, V, C, false>) : run(layernorm_bwd_kernel<KX, KY, T, V, C, true>);
+  static DeviceSetup without, with_gain;
+  return a.partial == nullptr ? run(layernorm_bwd_kernel<KX, KY, T, V, C, false>, without)
+                              : run(layernorm_bwd_kernel<KX, KY, T, V, C, true>, with_gain);
 }
 
 template <int KX, int KY>

@@ -8,9 +8,13 @@ one rounding to the result's type: half a step.
 
 from __future__ import annotations
 
+import ctypes
+import threading
+
 import pytest
 import torch
 
+from moss_image_b200 import _lib
 from moss_image_b200.norms import layer_norm
 
 pytestmark = pytest.mark.gpu
@@ -219,3 +223,45 @@ def test_refusals(cuda_device):
     with torch.autograd.forward_ad.dual_level():
         with pytest.raises(NotImplementedError):
             layer_norm(torch.autograd.forward_ad.make_dual(x, torch.ones_like(x)))
+
+
+@pytest.mark.parametrize("dims", [(6144, 12288), (1024, 3072)])
+def test_two_threads_at_once(cuda_device, dims):
+    """Widths that run the same kernels with different shared memory, from two threads on streams of their own."""
+    cases = []
+    for dim in dims:
+        x, weight, bias, grad = _inputs((8, dim), BF16, "same", dim)
+        y, (dx, dw, db) = _check(x, weight, bias, grad)
+        cases.append((x, weight, bias, grad, y.detach(), dx, dw, db))
+    torch.cuda.synchronize()
+    start, wrong = threading.Barrier(len(cases)), []
+
+    def run(x, weight, bias, grad, *expected):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                rows, dim = x.shape
+                got = [torch.empty_like(t) for t in expected]
+                stats = torch.empty(rows, 2, device="cuda")
+                size = ctypes.c_size_t()
+                lib, stream = _lib.library(), torch.cuda.current_stream().cuda_stream
+                _lib.check(lib.moss_layernorm_bwd_workspace_bytes(rows, dim, ctypes.byref(size)), "workspace")
+                workspace = torch.empty(size.value, dtype=torch.uint8, device="cuda")
+                forward = (x.data_ptr(), 1, rows, dim, weight.data_ptr(), bias.data_ptr(), 1, 1e-6, got[0].data_ptr(),
+                           stats.data_ptr(), stream)
+                backward = (grad.data_ptr(), x.data_ptr(), 1, rows, dim, weight.data_ptr(), 1, stats.data_ptr(), 1,
+                            *(t.data_ptr() for t in got[1:]), workspace.data_ptr(), size.value, stream)
+                start.wait()
+                for _ in range(20000):  # the entry points themselves, as close together as they come
+                    _lib.check(lib.moss_layernorm_fwd(*forward), "moss_layernorm_fwd")
+                    _lib.check(lib.moss_layernorm_bwd(*backward), "moss_layernorm_bwd")
+                torch.cuda.current_stream().synchronize()
+                assert all(torch.equal(a, b) for a, b in zip(got, expected))
+        except Exception as error:  # (the test's own thread tells it)
+            wrong.append(error)
+
+    threads = [threading.Thread(target=run, args=case) for case in cases]
+    for thread in threads:
+        thread.start()
+    for thread in threads:
+        thread.join()
+    assert not wrong, wrong[0]
