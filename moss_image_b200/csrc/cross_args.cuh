@@ -377,16 +377,17 @@ struct TileBits {
   }
 };
 
-// Whether key tile `tile` holds the only key that the sequence's queries look at. P is then 1 whatever the logit is, and the
-// gradient of the logit nothing times dP - delta, whose rounding would be left otherwise. By a whole warp. A key alone in a mask
-// of too many tiles for TileBits is not found out.
-__device__ __forceinline__ bool only_key(const Args& a, const TileBits& taken, const Sequence& s, int tile) {
+// Whether the sequence's queries look at one key alone. P is then 1 whatever the logit is, and the gradient of the logit nothing
+// times dP - delta, whose rounding would be left otherwise. By a whole warp; it ends at the second key it finds.
+__device__ __forceinline__ bool only_key(const Args& a, const TileBits& taken, const Sequence& s) {
   if (s.kn == 1 || a.mask == nullptr) return s.kn == 1;
   const int tiles = (s.kn + kTile - 1) / kTile;
-  if (taken.bits == nullptr && tiles > 1) return false;
-  if (taken.next(s.entry, 0, tiles) != tile || taken.next(s.entry, tile + 1, tiles) < tiles) return false;
-  const KeyBits b = key_bits(a, s, tile * kTile);
-  return __popc(b.w[0]) + __popc(b.w[1]) + __popc(b.w[2]) + __popc(b.w[3]) == 1;
+  int seen = 0;
+  for (int t = taken.next(s.entry, 0, tiles); t < tiles && seen < 2; t = taken.next(s.entry, t + 1, tiles)) {
+    const KeyBits b = key_bits(a, s, t * kTile, taken.whole(s.entry, t));
+    seen += __popc(b.w[0]) + __popc(b.w[1]) + __popc(b.w[2]) + __popc(b.w[3]);
+  }
+  return seen == 1;
 }
 
 // 32 consecutive values of a row, the first `count` of them (a multiple of 8).

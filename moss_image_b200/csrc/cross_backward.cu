@@ -431,7 +431,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       ++nth;
       delta = meet[row] + meet[kTile + row];
       if (live && half == 0 && w.split == 0) args.delta[w.head * args.q_rows + q_row] = delta;
-      const bool alone = w.first < w.end && only_key(args, taken, w.s, w.first);
+      const bool alone = w.first < w.end && only_key(args, taken, w.s);
       int i = 0;
       for (int t = w.first; t < w.end; t = taken.next(w.s.entry, t + 1, w.end), ++i) {
         KeyBits keep;
@@ -700,7 +700,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int key = w.row + row;
       bool seen = key < w.s.kn;
       if (seen && args.mask != nullptr) seen = __ldg(args.mask + w.s.entry * args.mask_ld + key) != 0;
-      const bool alone = w.first < w.end && only_key(args, taken, w.s, w.row / kTile);
+      const bool alone = w.first < w.end && only_key(args, taken, w.s);
       for (int i = w.first; i < w.end; ++i, ++steps) {
         const int rows = w.s.qn - i % w.q_tiles * kTile - half * kHalf;  // query columns of this thread that exist
         const uint32_t slot = steps % Shape<kD>::kStats;

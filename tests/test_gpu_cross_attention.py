@@ -477,3 +477,15 @@ def test_one_key_keeps_nan_in_its_gradients(cuda_device, masked):
         assert dk[0, at].all()
         if which != 0:  # (the sum dS^T Q has the NaN of Q whatever dS is)
             assert dk.sum() == 64
+
+
+@pytest.mark.parametrize("batch,tk", [(65, 400), (1, 33000)])  # masks of more than 256 tiles
+def test_one_key_in_masks_of_many_tiles(cuda_device, batch, tk):
+    q, k, v, grad = _tensors(batch, 3, tk, 1, 1, 64, BF16, 15)
+    mask = torch.zeros(batch, tk, dtype=torch.bool, device="cuda")
+    at = torch.arange(batch, device="cuda") * 61 % tk if batch > 1 else torch.tensor([tk - 200], device="cuda")
+    mask[torch.arange(batch, device="cuda"), at] = True
+    o, dq, dk, dv = _run(q, k, v, grad, key_mask=mask)
+    assert torch.equal(o, v[mask][:, None].expand_as(o)) and not dq.any() and not dk.any()
+    mask[-1, (int(at[-1]) + 150) % tk] = True  # a second key for one of them
+    _check(q, k, v, grad, mask=mask)
