@@ -43,6 +43,7 @@ struct Args {
   const void* o;             // dense
   const void* grad;          // dense
   float* delta;              // [q_heads][q_rows]
+  int* sizes;                // f16: [2][sequences][k_heads], exponents of the greatest |V|^2 and |dO|^2 (of a row's halves); else null
   void* dk;
   void* dv;
   StatusSink status;
@@ -51,6 +52,7 @@ struct Args {
 struct Sequence {
   int q0, qn, k0, kn;  // rows in the tensor map's token dimension
   int entry;           // and the map's batch coordinate
+  int index;
   int64_t q_row, k_row;  // the first rows among all
 };
 
@@ -60,6 +62,7 @@ __device__ __forceinline__ int clamped(const int64_t* offsets, int i, int total)
 
 __device__ __forceinline__ Sequence sequence_of(const Args& a, int s) {
   Sequence r;
+  r.index = s;
   if (a.q_offsets == nullptr) {
     r.q0 = r.k0 = 0;
     r.qn = a.tq;
@@ -414,6 +417,21 @@ __device__ __forceinline__ void store_row32_f32(float* to, int count, const floa
 #pragma unroll
   for (int h = 0; h < 8; ++h)
     if (4 * h < count) *reinterpret_cast<float4*>(to + 4 * h) = make_float4(v[4 * h], v[4 * h + 1], v[4 * h + 2], v[4 * h + 3]);
+}
+
+// f16 has no normal values below 2^-14, and dS = P (dP - delta) is often smaller: it is held times 2^e, e as large as its bound
+// allows. |dP| and |delta| are at most |dO| |V| (O is a mean of rows of V), so |dS| <= 2 |dO| |V|, with the greatest |V| of the
+// keys that the sequence looks at, and for dQ a row's |dO|, for dK the greatest of the sequence's rows. The biased exponents of
+// |V|^2 and of the greater half of |dO|^2 give log2 of 2 |dO| |V| within 2; the bound is placed at 2^14, so that a term keeps
+// its 11 bits down to 2^-26 of it. (Where V or dO is infinite, what e is does not matter.)
+__device__ __forceinline__ int lift_of(int v_exponent, int grad_exponent) {
+  const int log2_product = (v_exponent + grad_exponent - 251 + 1) >> 1;  // of |dO| |V|, rounded up
+  return max(-30, min(62, 13 - log2_product));
+}
+__device__ __forceinline__ int exponent_of(float square) { return static_cast<int>(__float_as_uint(square) >> 23); }  // not negative
+// Whether other CTAs came first or not, the greatest stays.
+__device__ __forceinline__ void raise_to(int* at, int value) {
+  if (value > *static_cast<volatile int*>(at)) atomicMax(at, value);
 }
 
 struct Maps {

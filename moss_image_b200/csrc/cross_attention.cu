@@ -108,6 +108,44 @@ __global__ void __launch_bounds__(kThreads) join_tail_kernel(const Args a, int k
   }
 }
 
+// Exponents of the greatest |V|^2 that each sequence's keys have, by key head: 16 lanes a row of a head.
+__global__ void __launch_bounds__(kThreads) value_sizes_kernel(const Args a, const uint16_t* __restrict__ v, int64_t v_batch,
+                                                               int64_t v_token, int64_t v_head) {
+  const int64_t at = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) / 16, row = at / a.k_heads;
+  const int head = static_cast<int>(at - row * a.k_heads), part = threadIdx.x & 15;
+  int seq = -1;
+  const uint16_t* from = v;
+  if (row < a.k_rows) {
+    if (a.k_offsets == nullptr) {
+      seq = static_cast<int>(row / a.tk);
+      const int64_t key = row - static_cast<int64_t>(seq) * a.tk;
+      if (a.mask != nullptr && __ldg(a.mask + seq * a.mask_ld + key) == 0) seq = -1;
+      from += seq * v_batch + key * v_token;
+    } else {
+      int low = 0, high = a.batch;  // the first boundary behind the row is that of `low`
+      while (low < high) {
+        const int mid = (low + high) / 2;
+        if (clamped(a.k_offsets, mid + 1, a.tk) > row)
+          high = mid;
+        else
+          low = mid + 1;
+      }
+      if (low < a.batch) seq = low;  // (nobody looks at rows behind the last sequence)
+      from += row * v_token;
+    }
+  }
+  float sum = 0.0f;
+  if (seq >= 0 && 8 * part < a.head_dim) {
+    float x[8];
+    load8<kF16>(from + head * v_head, 8 * part, 8, true, x);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) sum = fmaf(x[j], x[j], sum);
+  }
+#pragma unroll
+  for (int d = 8; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+  if (seq >= 0 && part == 0) raise_to(a.sizes + static_cast<int64_t>(seq) * a.k_heads + head, exponent_of(fabsf(sum)));
+}
+
 struct Problem {
   int64_t batch, tq, tk, q_heads, k_heads, head_dim;
   bool packed;
@@ -187,13 +225,15 @@ KeyPlan plan_keys(const Problem& p) {
 }
 
 struct BackwardLayout {
-  size_t dq, dkv, total;  // after the deltas
+  size_t dq, dkv, sizes, sizes_bytes, total;  // after the deltas
 };
 BackwardLayout backward_layout(const Problem& p, int dq_splits, const KeyPlan& keys) {
   BackwardLayout l{};
   l.dq = up(static_cast<size_t>(p.q_heads) * p.q_rows() * 4);
   l.dkv = l.dq + (dq_splits > 1 ? up(static_cast<size_t>(dq_splits) * p.q_rows() * p.q_heads * p.head_dim * 4) : 0);
-  l.total = l.dkv + up(static_cast<size_t>(keys.tail) * keys.splits * 2 * kTile * p.head_dim * 4);
+  l.sizes = l.dkv + up(static_cast<size_t>(keys.tail) * keys.splits * 2 * kTile * p.head_dim * 4);
+  l.sizes_bytes = 2 * static_cast<size_t>(p.batch + 1) * p.k_heads * sizeof(int);  // (rows behind the last sequence are one more)
+  l.total = l.sizes + up(l.sizes_bytes);
   return l;
 }
 
@@ -326,6 +366,14 @@ int backward(const Problem& p, const void* grad, const void* q, Strides qs, cons
       !make_map(&maps.q, dtype, q, p, p.tq, p.q_heads, qs) || !make_map(&maps.k, dtype, k, p, p.tk, p.k_heads, ks) ||
       !make_map(&maps.v, dtype, v, p, p.tk, p.k_heads, vs))
     return fail(MOSS_ERR_INVALID_ARGUMENT, "queries, keys, values, outputs and gradients need 16-byte aligned rows of one stride");
+  if (dtype == kF16) {
+    a.sizes = reinterpret_cast<int*>(ws + l.sizes);
+    MOSS_CUDA_TRY(cudaMemsetAsync(a.sizes, 0, l.sizes_bytes, stream));
+    const int64_t threads = p.k_rows() * p.k_heads * 16;
+    value_sizes_kernel<<<static_cast<unsigned>(ceil_div(threads, kThreads)), kThreads, 0, stream>>>(
+        a, static_cast<const uint16_t*>(v), vs.batch, vs.token, vs.head);
+    MOSS_CUDA_TRY(cudaGetLastError());
+  }
   rc = launch_dq(dtype, maps, a, stream);
   if (rc == MOSS_OK && dq_splits > 1) rc = join_sums(a.partial, dq_splits, static_cast<int64_t>(q_bytes / 2), dq, dtype, stream);
   if (rc != MOSS_OK || dk == nullptr) return rc != MOSS_OK ? rc : clear_ok();

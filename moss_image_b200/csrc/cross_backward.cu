@@ -9,8 +9,8 @@
 // The dq kernel also takes delta = rowsum(O dO) on the way, which the other reads.
 //
 // In both, P and dS are written over S and dP in TMEM as 16-bit pairs and feed the next product from there; a thread has a
-// row and half of the columns (two warpgroups). P and dS are rounded to the inputs' type, half a step of each term; sums
-// are f32. The next tile's S and dP run while a tile's elements are worked on.
+// row and half of the columns (two warpgroups). P and dS are rounded to the inputs' type, half a step of each term (f16: times
+// a power of two, see lift_of); sums are f32. The next tile's S and dP run while a tile's elements are worked on.
 #include <algorithm>
 #include <cmath>
 #include <cstring>
@@ -29,8 +29,7 @@ constexpr int kMathWarps = 8;
 constexpr int kMiscRegs = 72, kMathRegs = 216;
 static_assert(kMiscRegs + 2 * kMathRegs <= 3 * 168, "a larger split would wait forever");
 constexpr int kHalf = kTile / 2;  // columns of one warpgroup
-// f16 has no normal values below 2^-14: there dV is summed from 2^14 P (at most 2^14) and scaled back at the end. dS has no
-// bound that would leave room for that: below 2^-14 it is rounded to multiples of 2^-24, as an f16 gradient itself is.
+// f16 has no normal values below 2^-14: there dV is summed from 2^14 P (at most 2^14) and scaled back at the end.
 template <int kKind>
 constexpr float kLift = kKind == kF16 ? 14.0f : 0.0f;
 
@@ -41,7 +40,7 @@ struct Shape {
   static constexpr uint32_t kDataBytes = (2 + kStages) * kTileBytes;
   static constexpr int kStats = kD == 128 ? 2 : 4;  // row sums and deltas of so many tiles
   // (shared memory starts on 1024 bytes, which is checked: there is no room for padding)
-  static constexpr uint32_t kSmemBytes = kDataBytes + kStats * 2 * kTile * 4 + 512;
+  static constexpr uint32_t kSmemBytes = kDataBytes + kStats * 2 * kTile * 4 + 512 + 2 * 2 * kTile;
   static_assert(kSmemBytes <= 227 * 1024, "tiles exceed the shared memory a CTA may use");
 };
 constexpr int kMaxStages = 8;
@@ -96,12 +95,14 @@ struct Cta {
   uint32_t base;  // two tiles that stay, then the ring
   Barriers* bars;
   float* stats;   // [kStats][2][128]
+  uint8_t* sizes; // dq: [2][2][128], exponents of halves of |dO|^2
   volatile int* abort_flag;
   StatusSink status;
   __device__ __forceinline__ explicit Cta(uint8_t* raw, StatusSink sink) : status(sink) {
     base = smem_u32(raw);
     stats = reinterpret_cast<float*>(raw + S::kDataBytes);
     bars = reinterpret_cast<Barriers*>(raw + S::kDataBytes + S::kStats * 2 * kTile * 4);
+    sizes = reinterpret_cast<uint8_t*>(bars) + 512;
     abort_flag = &bars->abort_flag;
   }
   // The tiles' swizzle wants 1024-byte addresses.
@@ -406,7 +407,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int at = w.row + row;
       const bool live = at < w.s.qn;
       const int64_t q_row = w.s.q_row + at;
-      float lse = INFINITY, delta = 0.0f;
+      float lse = INFINITY, delta = 0.0f, square = 0.0f;
       if (live) {
         lse = __ldg(args.lse + w.head * args.q_rows + q_row);
         const int64_t from = (q_row * args.q_heads + w.head) * args.head_dim + half * (kD / 2);
@@ -420,10 +421,16 @@ __global__ void __launch_bounds__(kThreads, 1)
           load_row16<kKind>(g + c * 16, count - c * 16, y);
 #pragma unroll
           for (int j = 0; j < 16; ++j) delta = fmaf(x[j], y[j], delta);
+          if constexpr (kKind == kF16) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) square = fmaf(y[j], y[j], square);
+          }
         }
       }
       float* const meet = cta.stats + (nth & 1u) * 2 * kTile;
       meet[half * kTile + row] = delta;
+      uint8_t* const sizes = cta.sizes + (nth & 1u) * 2 * kTile;
+      if constexpr (kKind == kF16) sizes[half * kTile + row] = static_cast<uint8_t>(exponent_of(fabsf(square)));
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&bars->stat_full[nth & 1u]));
       ok = cta.wait(bars->stat_full[nth & 1u], nth >> 1, MOSS_STATUS_TIMEOUT_EPILOGUE);
@@ -431,7 +438,15 @@ __global__ void __launch_bounds__(kThreads, 1)
       ++nth;
       delta = meet[row] + meet[kTile + row];
       if (live && half == 0 && w.split == 0) args.delta[w.head * args.q_rows + q_row] = delta;
+      int lift = 0;
+      if constexpr (kKind == kF16) {
+        const int size = max(sizes[row], sizes[kTile + row]), at_sizes = w.s.index * args.k_heads + w.head / args.group;
+        lift = lift_of(args.sizes[at_sizes], size);
+        const int most = __reduce_max_sync(0xffffffffu, size);
+        if (half == 0 && w.split == 0 && lane == 0) raise_to(args.sizes + (args.batch + 1) * args.k_heads + at_sizes, most);
+      }
       const bool alone = w.first < w.end && only_key(args, taken, w.s);
+      const float raised = kKind == kF16 ? pow2(lift) : 1.0f;
       int i = 0;
       for (int t = w.first; t < w.end; t = taken.next(w.s.entry, t + 1, w.end), ++i) {
         KeyBits keep;
@@ -446,12 +461,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         load64(dp_tmem + half * kHalf + lanes, g);
         float v[64];
         // (a row without keys has lse = inf, which makes its exponentials zero)
-        const uint64_t scale2 = pair_of(args.scale_log2, args.scale_log2), minus_lse = pair_of(-lse, -lse), minus_delta = pair_of(-delta, -delta);
+        const uint64_t scale2 = pair_of(args.scale_log2, args.scale_log2), minus_lse = pair_of(-lse, -lse), raise2 = pair_of(raised, raised),
+                       minus_delta = pair_of(-delta * raised, -delta * raised);
 #pragma unroll
         for (int j = 0; j < 64; j += 2) {
           const uint64_t p = exponentials(j / 2, pair_of(__uint_as_float(s[j >> 5][j & 31]), __uint_as_float(s[j >> 5][(j & 31) + 1])),
                                                  scale2, minus_lse);
-          const uint64_t d = add_pair(pair_of(__uint_as_float(g[j >> 5][j & 31]), __uint_as_float(g[j >> 5][(j & 31) + 1])), minus_delta);
+          const uint64_t dp = pair_of(__uint_as_float(g[j >> 5][j & 31]), __uint_as_float(g[j >> 5][(j & 31) + 1]));
+          const uint64_t d = kKind == kF16 ? fma_pair(dp, raise2, minus_delta) : add_pair(dp, minus_delta);
           split_pair(mul_pair(p, d), v[j], v[j + 1]);
         }
         if constexpr (kMask) {
@@ -484,6 +501,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc_fence_after();
       }
       const int64_t to = (q_row * args.q_heads + w.head) * args.head_dim;
+      const float factor = kKind == kF16 ? args.scale * pow2(-lift) : args.scale;
 #pragma unroll
       for (int c = 0; c < kD / 64; ++c) {  // this warpgroup's half of the head
         const int col = half * (kD / 2) + c * 32;
@@ -500,7 +518,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
 #pragma unroll
-        for (int j = 0; j < 32; ++j) v[j] = any_keys ? __uint_as_float(o[j]) * args.scale : 0.0f;
+        for (int j = 0; j < 32; ++j) v[j] = any_keys ? __uint_as_float(o[j]) * factor : 0.0f;
         const int count = args.head_dim - col;
         if (live && count > 0) {
           if (args.splits > 1)
@@ -701,6 +719,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       bool seen = key < w.s.kn;
       if (seen && args.mask != nullptr) seen = __ldg(args.mask + w.s.entry * args.mask_ld + key) != 0;
       const bool alone = w.first < w.end && only_key(args, taken, w.s);
+      int lift = 0;
+      if constexpr (kKind == kF16) {
+        const int* const sizes = args.sizes + w.s.index * args.k_heads + w.head;
+        lift = lift_of(__ldg(sizes), __ldg(sizes + (args.batch + 1) * args.k_heads));
+      }
+      const float of_p = pow2(lift - static_cast<int>(kLift<kKind>));  // what P, which is lifted for dV, takes to be lifted for dS
       for (int i = w.first; i < w.end; ++i, ++steps) {
         const int rows = w.s.qn - i % w.q_tiles * kTile - half * kHalf;  // query columns of this thread that exist
         const uint32_t slot = steps % Shape<kD>::kStats;
@@ -731,7 +755,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         store64<kKind>(tmem + half * kHalf + lanes, v);
         if constexpr (kKind == kF16) {
 #pragma unroll
-          for (int j = 0; j < 64; ++j) v[j] *= 1.0f / 16384.0f;
+          for (int j = 0; j < 64; ++j) v[j] *= of_p;
         }
         tmem_wait_st();
         tc_fence_before();
@@ -776,7 +800,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       float* const part = args.partial + ((static_cast<int64_t>(half) * args.splits + w.split) * args.tail + w.tail) * kTile * args.head_dim;
       const int64_t to = ((w.s.k_row + key) * args.k_heads + w.head) * args.head_dim;
       const uint32_t from = (half == 0 ? dv_tmem : dk_tmem) + lanes;
-      const float factor = half == 1 ? args.scale : kKind == kF16 ? 1.0f / 16384.0f : 1.0f;
+      const float factor = half == 1 ? args.scale * pow2(-lift) : pow2(-static_cast<int>(kLift<kKind>));
 #pragma unroll
       for (int c = 0; c < kD / 32; ++c) {
         uint32_t o[32];
