@@ -321,9 +321,10 @@ MOSS_API int moss_cross_attention_bwd(const void* grad, const void* q, int64_t q
  * Activations as 8-bit codes: int8 codes in [-127, 127] and one power of two for each block of 32 columns of a row, the
  * least 2^p with max|x| <= 127 * 2^p, p in [-126, 9] for f16 and [-126, 121] otherwise; codes x / 2^p rounded to
  * nearest even. exponents[rows][ceil(cols / 32)] holds p + 127, or 255 for a block with an infinity or NaN
- * (it decodes to NaN). A decoded value is within max|x| / 127 of x, and exact in x's dtype. Codes are [rows, cols] with a
- * pitch ld (a multiple of 16 bytes, 16-byte aligned; the encoder writes the least one, and zeros up to it).
- *   gradient: dw[n, cols] = dy[rows, n]^T decode(codes), dy f16 or bf16, f32 sums in a fixed order, one rounding.
+ * (it decodes to NaN). A decoded value is within max|x| / 127 of x (2^-127 where p is -126), and exact in x's dtype. Codes are
+ * [rows, cols] with a pitch ld (a multiple of 16 bytes, 16-byte aligned; the encoder writes the least one, and zeros up to it).
+ *   gradient: dw[n, cols] = dy[rows, n]^T decode(codes), dy f16 or bf16, f32 sums in a fixed order, one rounding. Codes are
+ *   decoded to dy's dtype: f16 gradients want codes of f16 values (what f16 does not hold is rounded, or infinite).
  * `workspace`: at least moss_coded_gradient_workspace_bytes(rows, n, cols) bytes, 256-byte aligned, free for reuse
  * once the stream has passed the call.
  */

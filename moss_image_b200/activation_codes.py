@@ -3,8 +3,8 @@
 What the forward pass keeps for the backward one is half of a step's memory, and
 :mod:`moss_image_b200.activation_offload` moves it out whole. Here it is kept in half the bytes: int8
 codes with one power of two for each 32 values of a row (:func:`encode_activation`), 8.25 bits a value. A
-decoded value is within 1/127 of its block's largest magnitude and, since a code has seven bits and a
-sign, exact in the activation's own 16-bit type, so that what a product reads is what the codes stand for.
+decoded value is within 1/127 of its block's largest magnitude (or within 2^-127, in blocks below 2^-119) and, since a
+code has seven bits and a sign, exact in the activation's own type, so that what a product reads is what the codes stand for.
 
 * :func:`encode_activation` / :func:`decode_activation`: the codes on their own. A block with an infinity
   or NaN decodes to NaN.
@@ -120,6 +120,11 @@ def decode_activation(coded: CodedActivation, dtype: torch.dtype | None = None) 
     return out
 
 
+def _holds(dtype: torch.dtype, coded_dtype: torch.dtype) -> bool:
+    """Whether products in ``dtype`` can read codes of ``coded_dtype`` tokens as what they stand for."""
+    return dtype != torch.float16 or coded_dtype == torch.float16
+
+
 @lru_cache(maxsize=1024)
 def _workspace_bytes(device: int, rows: int, features: int, columns: int) -> int:
     size = ctypes.c_size_t()
@@ -130,10 +135,15 @@ def _workspace_bytes(device: int, rows: int, features: int, columns: int) -> int
 
 
 def coded_weight_gradient(gradient: torch.Tensor, codes: torch.Tensor, exponents: torch.Tensor,
-                          output_dtype: torch.dtype | None = None) -> torch.Tensor:
+                          output_dtype: torch.dtype | None = None, *,
+                          coded_dtype: torch.dtype | None = None) -> torch.Tensor:
     """``dW = dY^T decode(X)``: ``[features, columns]`` from ``[..., features]`` float16 or bfloat16 gradients and the
     codes of the ``[..., columns]`` input. Sums are float32, in a fixed order, rounded once to ``output_dtype``
-    (the gradient's own by default)."""
+    (the gradient's own by default).
+
+    ``coded_dtype``: what the codes were made from, the gradient's dtype where it is not given. The product reads decoded
+    values in the gradient's dtype: bfloat16 holds those of any codes, float16 those of float16 tokens only.
+    """
     what = "coded_weight_gradient"
     if not gradient.is_cuda:
         raise RuntimeError(f"{what} runs on CUDA tensors only (there is no CPU path).")
@@ -144,11 +154,13 @@ def coded_weight_gradient(gradient: torch.Tensor, codes: torch.Tensor, exponents
     dtype = gradient.dtype if output_dtype is None else output_dtype
     if dtype not in _FLOATS:
         raise ValueError(f"{what}: the output must be float16, bfloat16 or float32.")
+    if not _holds(gradient.dtype, gradient.dtype if coded_dtype is None else coded_dtype):
+        raise ValueError(f"{what}: float16 does not hold what codes of {coded_dtype} tokens stand for.")
     _lib.refuse_forward_mode(what, gradient)
     device = gradient.device
     if device.index != _lib.current_device_index():
         with torch.cuda.device(device):
-            return coded_weight_gradient(gradient, codes, exponents, output_dtype)
+            return coded_weight_gradient(gradient, codes, exponents, output_dtype, coded_dtype=coded_dtype)
     codes = _check_codes(codes, exponents, what)
     rows, columns = codes.shape
     features = gradient.shape[-1]
@@ -213,6 +225,8 @@ def coded_linear(tokens: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor 
         raise ValueError("coded_linear: autocast runs in another dtype than the tokens and the weight have.")
     if coded is not None and (coded.shape != tokens.shape or coded.codes.device != tokens.device):
         raise ValueError("coded_linear: the codes are not those of these tokens (another shape or device).")
+    if coded is not None and coded.dtype != tokens.dtype:
+        raise ValueError("coded_linear: the codes are those of tokens of another dtype.")
     _lib.refuse_forward_mode("coded_linear", *given)
     if not torch.is_grad_enabled() or not any(t.requires_grad for t in given):
         return F.linear(tokens, weight, bias)

@@ -4,7 +4,8 @@
 //   x ~ code * 2^p,  p the least with max|x| <= 127 * 2^p, within [-126, cap] (cap: 9 for f16, else 121)
 // The exponent byte is p + 127. A block with an infinity or NaN has the byte 255 and zero codes: its scale
 // reads as an infinity, and 0 * inf as NaN. A code has 7 bits and a sign and the scale is a power of two, so a
-// decoded value is exact in f16, bf16 and f32: what a product reads is what the codes stand for.
+// decoded value is exact in the type that was encoded, and in bf16 and f32 in any case: what a product reads is what the codes
+// stand for. f16 has no room for codes of the other types with large p (they read as infinities there) or small p (rounded).
 #pragma once
 
 #include "common.cuh"

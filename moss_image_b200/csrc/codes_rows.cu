@@ -43,8 +43,9 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4],
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// The scales of two rows as one pair of 16-bit values. f16 has no 2^p below -24 although code * 2^p may be a value
-// of it: there the scale is two factors, the second of which is 1 for p >= -14.
+// The scales of two rows as one pair of 16-bit values. f16 has no 2^p below -24 or above 15 although code * 2^p may be a value of
+// it (or zero): there the scale is two factors, the second of which is 1 for p in [-14, 15]. The scale of a block with an
+// infinity or NaN is an infinity.
 struct Scales {
   uint32_t first, second;
 };
@@ -58,10 +59,13 @@ __device__ __forceinline__ Scales scales_of(uint32_t e0, uint32_t e1) {
     auto half_pow2 = [](int p) {  // p in [-24, 15]; 16 reads as an infinity
       return p >= -14 ? static_cast<uint32_t>(p + 15) << 10 : 1u << (p + 24);
     };
-    const int p0 = static_cast<int>(e0) - 127, p1 = static_cast<int>(e1) - 127;
-    // a block of zero codes may have any small power: what matters is that it is finite
-    s.first = half_pow2(max(-14, min(16, p0))) | (half_pow2(max(-14, min(16, p1))) << 16);
-    s.second = half_pow2(max(-24, min(0, p0 + 14))) | (half_pow2(max(-24, min(0, p1 + 14))) << 16);
+    auto first = [&](uint32_t e) { return half_pow2(e == 255u ? 16 : max(-14, min(15, static_cast<int>(e) - 127))); };
+    auto second = [&](uint32_t e) {
+      const int p = static_cast<int>(e) - 127;
+      return half_pow2(p > 15 ? min(15, p - 15) : max(-24, min(0, p + 14)));
+    };
+    s.first = first(e0) | (first(e1) << 16);
+    s.second = second(e0) | (second(e1) << 16);
   }
   return s;
 }

@@ -123,6 +123,8 @@ class LoRALinear(nn.Module):
         """``coded``: codes of the tokens, which the fused form then keeps in their place for ``lora_A``'s gradient."""
         if coded is not None and (coded.shape != tokens.shape or coded.codes.device != tokens.device):
             raise ValueError("The codes are not those of these tokens (another shape or device).")
+        if coded is not None and coded.dtype != tokens.dtype:
+            raise ValueError("The codes are those of tokens of another dtype.")
         adapter_dtype = self._adapter_dtype(tokens)
         base = self.base
         if (
@@ -132,6 +134,8 @@ class LoRALinear(nn.Module):
             and adapter_dtype in (torch.float16, torch.bfloat16)
             and autocast_compute_dtype(tokens, base.compute_dtype) == adapter_dtype
         ):
+            if coded is not None and adapter_dtype == torch.float16 != coded.dtype:
+                coded = None  # float16 does not hold what they stand for: the tokens are kept
             return _FusedLoRAInt8Linear.apply(
                 tokens, self.lora_A, self.lora_B, base.weight_int8, base.weight_scale, base.bias,
                 base.compute_dtype, base.quantized_backend, float(self.scale), adapter_dtype,

@@ -15,6 +15,8 @@ from torch.utils.checkpoint import checkpoint
 from moss_image_b200.activation_codes import (CodedActivation, coded_checkpoints, coded_linear, coded_weight_gradient,
                                               decode_activation, encode_activation)
 from moss_image_b200.activation_offload import activation_cpu_offload
+from moss_image_b200.lora import LoRALinear
+from moss_image_b200.quantization import FrozenInt8Linear
 
 pytestmark = pytest.mark.gpu
 
@@ -300,3 +302,45 @@ def test_refusals(cuda_device):
     slope, = torch.autograd.grad(coded_linear(x.requires_grad_(), weight).float().square().sum(), weight, create_graph=True)
     with pytest.raises(RuntimeError):
         torch.autograd.grad(slope.float().sum(), weight)
+
+
+@pytest.mark.parametrize("features", [8, 40])
+def test_codes_past_float16(cuda_device, features):
+    """Codes of wider types under a float16 gradient: refused where the caller says so, else what float16 makes of their values."""
+    x = torch.zeros(48, 96, device="cuda")
+    x[3, 0], x[3, 5] = 127.0 * 2.0 ** 16, 2.0 ** 16  # past float16; the block's other values are zeros
+    x[4, 40], x[4, 41] = 127.0 * 2.0 ** 40, 1.0
+    x[5, 64:] = 60000.0  # a block of float16 values whose power of two is one
+    x[6, :32] = 2.0 ** -30
+    x[7, 70] = float("nan")
+    coded = encode_activation(x)
+    dy = torch.randn(48, features, device="cuda").to(F16)
+    with pytest.raises(ValueError, match="does not hold"):
+        coded_weight_gradient(dy, coded.codes, coded.exponents, coded_dtype=F32)
+    got = coded_weight_gradient(dy, coded.codes, coded.exponents, F32)
+    exact = dy.double().t() @ decode_activation(coded, F16).double()
+    assert torch.equal(got.isnan(), exact.isnan()) and torch.equal(got.isinf(), exact.isinf())
+    good = exact.isfinite()
+    assert ((got.double() - exact).abs()[good] <= 2.0 ** -20 * (dy.double().abs().t() @ x.abs().nan_to_num(0).double())[good]).all()
+    wide = coded_weight_gradient(dy.to(BF16), coded.codes, coded.exponents, F32, coded_dtype=F32)
+    assert torch.equal(wide.isfinite(), torch.arange(96, device="cuda").lt(64).expand_as(wide))
+
+
+def test_codes_of_another_dtype_are_refused(cuda_device):
+    x = torch.randn(8, 64, device="cuda", dtype=F16)
+    weight = torch.randn(4, 64, device="cuda", dtype=F16, requires_grad=True)
+    with pytest.raises(ValueError, match="another dtype"):
+        coded_linear(x, weight, coded=encode_activation(x.to(BF16)))
+    base = torch.nn.Linear(64, 32).to("cuda", F16).requires_grad_(False)
+    layer = LoRALinear(FrozenInt8Linear(base), 4, 8.0).to("cuda")
+    torch.nn.init.normal_(layer.lora_B, std=0.05)
+    with pytest.raises(ValueError, match="another dtype"):
+        layer(x, encode_activation(x.to(BF16)))
+    # float16 adapters of wider tokens keep the tokens
+    tokens = torch.randn(8, 64, device="cuda", dtype=BF16)
+    grads = []
+    for codes in (None, encode_activation(tokens)):
+        with torch.autocast("cuda", F16):
+            y = layer(tokens, codes)
+        grads.append(torch.autograd.grad(y.float().sum(), layer.lora_A)[0])
+    assert torch.equal(*grads)
