@@ -240,9 +240,8 @@ def coded_linear(tokens: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor 
 def coded_checkpoints(tokens: torch.Tensor, outer: ContextManager | None = None) -> ContextManager:
     """A scope for one ``checkpoint`` call (non-reentrant) of a block on ``tokens``: what it keeps of the tokens are codes.
 
-    Everything of the tokens' shape and dtype that autograd saves directly in the scope is coded; for a checkpointed
-    block that is its input, for a block that is not checkpointed it would be every such activation. The rest is kept as it
-    is. ``outer``: the saved-tensor hooks of the scope around it (``activation_cpu_offload``), which then
+    The tokens are coded where autograd saves them in the scope; everything else that it saves is kept as it is, other
+    tensors of their shape too. ``outer``: the saved-tensor hooks of the scope around it (``activation_cpu_offload``), which then
     receive the codes and everything else.
     """
     def same(value: torch.Tensor) -> torch.Tensor:
@@ -250,11 +249,12 @@ def coded_checkpoints(tokens: torch.Tensor, outer: ContextManager | None = None)
 
     hide: Callable = getattr(outer, "pack_hook", same)
     show: Callable = getattr(outer, "unpack_hook", same)
-    shape, dtype = tokens.shape, tokens.dtype
-    codable = tokens.is_cuda and dtype in _FLOATS and tokens.ndim >= 1
+    codable = tokens.is_cuda and tokens.dtype in _FLOATS and tokens.ndim >= 1
+    # (the caller holds the tokens while the scope is open: nothing else has their address)
+    which = (tokens.data_ptr(), tokens.shape, tokens.stride(), tokens.dtype)
 
     def pack(saved: torch.Tensor):
-        if not codable or saved.shape != shape or saved.dtype != dtype or not saved.is_cuda:
+        if not codable or not saved.is_cuda or (saved.data_ptr(), saved.shape, saved.stride(), saved.dtype) != which:
             return hide(saved), None, None
         codes, exponents, *meant = encode_activation(saved)
         return hide(codes), hide(exponents), meant

@@ -344,3 +344,22 @@ def test_codes_of_another_dtype_are_refused(cuda_device):
             y = layer(tokens, codes)
         grads.append(torch.autograd.grad(y.float().sum(), layer.lora_A)[0])
     assert torch.equal(*grads)
+
+
+def test_only_the_tokens_of_a_checkpoint_are_coded(cuda_device):
+    """Another input of the tokens' shape and dtype (a context) stays whole."""
+    torch.manual_seed(2)
+    weight = torch.randn(64, 64, device="cuda", dtype=BF16, requires_grad=True)
+
+    def block(x, context):
+        return (x @ weight) * context
+
+    leaf, context = (torch.randn(2, 50, 64, device="cuda").to(BF16) for _ in range(2))
+    x, other = leaf.requires_grad_() * 1.0, context.requires_grad_() * 1.0
+    dy = torch.randn(2, 50, 64, device="cuda").to(BF16)
+    with coded_checkpoints(x):
+        y = checkpoint(block, x, other, use_reentrant=False)
+    got = torch.autograd.grad(y, [leaf, context, weight], dy)
+    near = decode_activation(encode_activation(x)).requires_grad_()
+    expected = torch.autograd.grad(block(near, context), [near, context, weight], dy)
+    assert all(torch.equal(a, b) for a, b in zip(got, expected))
