@@ -312,18 +312,22 @@ class SyntheticDiT(nn.Module):
                 inputs = (tokens, cond, cu_seqlens, *rotary)
             if context is not None:
                 inputs = (tokens, cond, cu_seqlens, *(rotary or (None, None)), context, keys)
+            # every block that is checkpointed, wherever its parameters are
+            kept = coded_checkpoints(tokens, scope) if self.coded_checkpoints and torch.is_grad_enabled() else nullcontext()
             if manager is not None and index >= boundary:
                 at = position[index]
-                tokens = manager.block(
-                    index, *inputs,
-                    forward_prefetch=streamed[at + 1] if at + 1 < len(streamed) else None,
-                    backward_prefetch=streamed[at - 1] if at else None,
-                    checkpoint_block=torch.is_grad_enabled(),
-                )
+                with kept:
+                    tokens = manager.block(
+                        index, *inputs,
+                        forward_prefetch=streamed[at + 1] if at + 1 < len(streamed) else None,
+                        backward_prefetch=streamed[at - 1] if at else None,
+                        checkpoint_block=torch.is_grad_enabled(),
+                    )
             elif index >= boundary:
-                tokens = offloaded_block(layer, *inputs)
+                with kept:
+                    tokens = offloaded_block(layer, *inputs)
             elif self.gradient_checkpointing and self.training and torch.is_grad_enabled():
-                with coded_checkpoints(tokens, scope) if self.coded_checkpoints else nullcontext():
+                with kept:
                     tokens = checkpoint(layer, *inputs, use_reentrant=False, determinism_check=CHECKPOINT_CHECK)
             else:
                 tokens = layer(*inputs)

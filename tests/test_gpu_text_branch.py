@@ -10,9 +10,11 @@ import pytest
 import torch
 from torch.nn import functional as F
 
+from moss_image_b200 import _lib
 from moss_image_b200.activation_codes import coded_weight_gradient, decode_activation, encode_activation
 from moss_image_b200.dit import TextBranch, build_lora_model
 from moss_image_b200.lora import LoRALinear
+from moss_image_b200.memory import place_model
 from moss_image_b200.packed import cumulative_lengths
 from moss_image_b200.quantization import FrozenInt8Linear
 
@@ -188,3 +190,28 @@ def test_decoded_checkpoint_input(cuda_device):
         normed = model.final_norm(whole)
     inner = torch.autograd.grad(normed, whole, dy)[0]
     assert torch.equal(got, torch.autograd.grad(block, near, inner)[0])
+
+
+@pytest.mark.parametrize("mode,text_dim", [("sync", 96), ("async", None)])
+def test_swapped_and_streamed_blocks_keep_codes_too(cuda_device, mode, text_dim):
+    """The same gradients wherever a block's parameters are, its checkpointed input kept as codes, with a text branch in it."""
+    tokens = torch.randn(2, 40, 128, device="cuda").to(BF16)
+    options = {} if text_dim is None else {"context": torch.randn(2, 24, text_dim, device="cuda").to(BF16)}
+    t = torch.tensor([0.2, 0.7], device="cuda")
+    results = []
+    for blocks in (0, 2):
+        model = build_lora_model(2, device=cuda_device, dim=128, heads=2, mlp_dim=256, rank=4, seed=6, text_dim=text_dim).train()
+        for layer in model.layers:
+            for name in ("q", "k", "v", "o"):
+                torch.nn.init.constant_(layer.proj[name].lora_B, 0.01)
+            if text_dim is not None:
+                torch.nn.init.constant_(layer.text.o.weight, 0.02)
+        model.coded_checkpoints = True
+        place_model(model, cuda_device, blocks, block_swap_mode=mode)
+        before = _lib.launch_counts.get("codes", 0)
+        out, grads = _gradients(model, tokens, t, **options)
+        # an encode and a decode for each block whose input is looked at again
+        results.append((out, {name: grad.to(cuda_device) for name, grad in grads.items()}, _lib.launch_counts.get("codes", 0) - before))
+    resident, placed = results
+    assert resident[2] == placed[2] >= 4 and torch.equal(resident[0], placed[0]) and resident[1].keys() == placed[1].keys()
+    assert all(torch.equal(resident[1][name], placed[1][name]) for name in resident[1])
