@@ -44,6 +44,7 @@ from .memory import offloaded_block
 from .norms import layer_norm, rms_norm
 from .packed import (
     CHECKPOINT_CHECK,
+    VARLEN_LOOP_MAX_SEQUENCES,
     batch_offsets,
     condition_for_tokens,
     cumulative_lengths,
@@ -118,20 +119,18 @@ class TextBranch(nn.Module):
                 offsets: torch.Tensor | None = None) -> torch.Tensor:
         """``tokens`` ``[B, T, dim]`` and ``context`` ``[B, S, text_dim]`` with an optional bool mask ``keys`` ``[B, S]``; or, with
         the stream's boundaries ``offsets``, ``[1, total, dim]``, ``[1, states, text_dim]`` and the captions' boundaries ``keys``."""
-        coded = self.coded_inputs and torch.is_grad_enabled()
-
-        def heads(linear: nn.Linear, x: torch.Tensor, codes: CodedActivation | None) -> torch.Tensor:
-            return project(linear, x, codes).unflatten(-1, (-1, self.head_dim))
+        def heads(x: torch.Tensor) -> torch.Tensor:
+            return x.unflatten(-1, (-1, self.head_dim))
 
         h = self.norm(tokens)
-        q = heads(self.q, h, encode_activation(h) if coded else None)
-        states = encode_activation(context) if coded else None  # one set of codes for both
-        k, v = heads(self.k, context, states), heads(self.v, context, states)
+        coded = encode_activation(h) if self.coded_inputs and torch.is_grad_enabled() else None
+        # the rest of what is kept lives anyway: the context belongs to the caller, and the attention keeps its own output
+        q, k, v = heads(project(self.q, h, coded)), heads(self.k(context)), heads(self.v(context))
         if offsets is None:
             attended = cross_attention(q, k, v, key_mask=keys).flatten(2)
         else:
             attended = cross_attention_packed(q[0], k[0], v[0], offsets, keys).flatten(1)[None]
-        return tokens + project(self.o, attended, encode_activation(attended) if coded else None)
+        return tokens + self.o(attended)
 
 
 class SyntheticBlock(nn.Module):
@@ -194,11 +193,15 @@ class SyntheticBlock(nn.Module):
         if cos is not None:
             q, k = apply_rotary(q, k, cos, sin)
         if cu_seqlens is None:
-            attended = F.scaled_dot_product_attention(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2))
-            attended = attended.transpose(1, 2).flatten(2)
+            output = F.scaled_dot_product_attention(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2))
+            attended = output.transpose(1, 2).flatten(2)
+            copied = attended.data_ptr() != output.data_ptr()
+            del output
         else:
+            copied = len(sequence_lengths(cu_seqlens)) <= VARLEN_LOOP_MAX_SEQUENCES  # joined from one output for each
             attended = varlen_attention(q[0], k[0], v[0], offsets, sequence_lengths(cu_seqlens)).flatten(1)[None]
-        coded = encode_activation(attended) if keep_codes else None
+        # (the attention keeps its output for the backward pass: where this is a view of it, codes would come on top)
+        coded = encode_activation(attended) if keep_codes and copied else None
         tokens = gated(tokens, project(self.proj["o"], attended, coded), gate_a)
         if self.text is not None and context is not None:
             tokens = self.text(tokens, context, keys, cu_seqlens)

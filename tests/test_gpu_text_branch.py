@@ -215,3 +215,37 @@ def test_swapped_and_streamed_blocks_keep_codes_too(cuda_device, mode, text_dim)
     resident, placed = results
     assert resident[2] == placed[2] >= 4 and torch.equal(resident[0], placed[0]) and resident[1].keys() == placed[1].keys()
     assert all(torch.equal(resident[1][name], placed[1][name]) for name in resident[1])
+
+
+def _held(run) -> int:
+    """Bytes that a forward pass leaves in use, its result among them (as asked for: the allocator rounds by a megabyte)."""
+    run()  # (workspaces and lazily made buffers are there)
+    before = torch.cuda.memory_stats()["requested_bytes.all.current"]
+    kept = run()
+    after = torch.cuda.memory_stats()["requested_bytes.all.current"]
+    del kept
+    return after - before
+
+
+@pytest.mark.parametrize("packed", [False, True])
+def test_coded_inputs_hold_less(cuda_device, packed):
+    """What a branch and a block keep for the backward pass is less with codes, by about half of each input that is coded."""
+    tokens = torch.randn(1, 4096, 512, device="cuda").to(BF16).requires_grad_()
+    context = torch.randn(1, 3000, 256, device="cuda").to(BF16)
+    bounds = (cumulative_lengths([1000, 2000], tokens.device), cumulative_lengths([2000, 2096], tokens.device)) if packed else (None, None)
+    branch = _branch(3, dim=512, heads=8, text_dim=256)
+    branches = []
+    for coded in (False, True):
+        branch.coded_inputs = coded
+        branches.append(_held(lambda: branch(tokens, context, *bounds)))
+    saved = tokens.numel() * (2 - 33 / 32)
+    assert abs(branches[0] - branches[1] - saved) < 0.02 * saved
+    block = build_lora_model(1, device=cuda_device, dim=512, heads=8, mlp_dim=1024, rank=8, seed=7).train().layers[0]
+    cond = torch.randn(2 if packed else 1, 512, device="cuda").to(BF16)
+    blocks = []
+    for coded in (False, True):
+        block.coded_inputs = coded
+        with torch.autocast("cuda", BF16):
+            blocks.append(_held(lambda: block(tokens, cond, bounds[1])))
+    copies = 2 if packed else 1  # q, k and v's input; and o's, where the attention's outputs are joined to one
+    assert abs(blocks[0] - blocks[1] - copies * saved) < 0.02 * saved
