@@ -203,6 +203,13 @@ class _CodedLinear(torch.autograd.Function):
         return d_tokens, d_weight, d_bias, None, None
 
 
+def codes_serve(tokens: torch.Tensor, weight_dtype: torch.dtype) -> bool:
+    """Whether :func:`coded_linear` takes the tokens with a weight of this dtype, under the autocast that is on."""
+    if not tokens.is_cuda or tokens.dtype not in (torch.float16, torch.bfloat16) or weight_dtype != tokens.dtype:
+        return False
+    return not torch.is_autocast_enabled("cuda") or torch.get_autocast_dtype("cuda") == tokens.dtype
+
+
 def coded_linear(tokens: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, *,
                  coded: CodedActivation | None = None) -> torch.Tensor:
     """``F.linear(tokens, weight, bias)`` that keeps its input as codes for the weight's gradient.

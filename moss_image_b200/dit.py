@@ -35,7 +35,7 @@ from torch import nn
 from torch.nn import functional as F
 from torch.utils.checkpoint import checkpoint
 
-from .activation_codes import CodedActivation, coded_checkpoints, coded_linear, encode_activation
+from .activation_codes import CodedActivation, coded_checkpoints, coded_linear, codes_serve, encode_activation
 from .activation_offload import KEEP_RESIDENT, activation_cpu_offload
 from .cross_attention import cross_attention, cross_attention_packed
 from .fp8 import quantize_frozen_linears_fp8
@@ -90,13 +90,22 @@ class LayerNorm(nn.Module):
         return F.layer_norm(x.float(), x.shape[-1:], self.weight.float(), self.bias.float(), self.eps).to(x.dtype)
 
 
+def keeps_codes(linear: nn.Module, tokens: torch.Tensor) -> bool:
+    """Whether ``linear(tokens)`` would keep the tokens' codes in their place: a trained linear or adapter with 16-bit products."""
+    if not torch.is_grad_enabled():
+        return False
+    if isinstance(linear, LoRALinear):
+        return linear.keeps_codes(tokens)
+    return isinstance(linear, nn.Linear) and linear.weight.requires_grad and codes_serve(tokens, linear.weight.dtype)
+
+
 def project(linear: nn.Module, tokens: torch.Tensor, coded: CodedActivation | None) -> torch.Tensor:
-    """``linear(tokens)``; a trained one keeps the tokens' codes for its gradient where they are given."""
-    if coded is not None and isinstance(linear, LoRALinear):
+    """``linear(tokens)``; where it can, it keeps the tokens' codes for its gradient if they are given."""
+    if coded is None or not keeps_codes(linear, tokens):
+        return linear(tokens)
+    if isinstance(linear, LoRALinear):
         return linear(tokens, coded)
-    if coded is not None and isinstance(linear, nn.Linear) and linear.weight.requires_grad:
-        return coded_linear(tokens, linear.weight, linear.bias, coded=coded)
-    return linear(tokens)
+    return coded_linear(tokens, linear.weight, linear.bias, coded=coded)
 
 
 class TextBranch(nn.Module):
@@ -123,7 +132,7 @@ class TextBranch(nn.Module):
             return x.unflatten(-1, (-1, self.head_dim))
 
         h = self.norm(tokens)
-        coded = encode_activation(h) if self.coded_inputs and torch.is_grad_enabled() else None
+        coded = encode_activation(h) if self.coded_inputs and keeps_codes(self.q, h) else None
         # the rest of what is kept lives anyway: the context belongs to the caller, and the attention keeps its own output
         q, k, v = heads(project(self.q, h, coded)), heads(self.k(context)), heads(self.v(context))
         if offsets is None:
@@ -185,8 +194,9 @@ class SyntheticBlock(nn.Module):
                 return x + branch * condition_for_tokens(gate, index)
 
         h = modulate(self.norm1(tokens), scale_a, shift_a)
-        keep_codes = self.coded_inputs and tokens.is_cuda and torch.is_grad_enabled()
-        coded = encode_activation(h) if keep_codes else None  # of q, k and v
+        coded = None
+        if self.coded_inputs and any(keeps_codes(self.proj[name], h) for name in ("q", "k", "v")):
+            coded = encode_activation(h)  # one set for the three
         q = self.q_norm(project(self.proj["q"], h, coded).unflatten(-1, (self.heads, -1)))
         k = self.k_norm(project(self.proj["k"], h, coded).unflatten(-1, (self.heads, -1)))
         v = project(self.proj["v"], h, coded).unflatten(-1, (self.heads, -1))
@@ -201,7 +211,7 @@ class SyntheticBlock(nn.Module):
             copied = len(sequence_lengths(cu_seqlens)) <= VARLEN_LOOP_MAX_SEQUENCES  # joined from one output for each
             attended = varlen_attention(q[0], k[0], v[0], offsets, sequence_lengths(cu_seqlens)).flatten(1)[None]
         # (the attention keeps its output for the backward pass: where this is a view of it, codes would come on top)
-        coded = encode_activation(attended) if keep_codes and copied else None
+        coded = encode_activation(attended) if self.coded_inputs and copied and keeps_codes(self.proj["o"], attended) else None
         tokens = gated(tokens, project(self.proj["o"], attended, coded), gate_a)
         if self.text is not None and context is not None:
             tokens = self.text(tokens, context, keys, cu_seqlens)
@@ -377,8 +387,9 @@ def build_lora_model(depth: int, *, device: torch.device, dim: int = 3072, heads
     ``quantize_frozen_linears`` allows at module level (training/quantization.py:156-157;
     the reference trainer itself only pairs int8 bases with LoRA, training/train.py:543-545).
     ``frozen="fp8"`` holds the frozen linears as block-scaled fp8 (:mod:`moss_image_b200.fp8`). ``text_dim`` gives
-    every block a trained :class:`TextBranch` over states of that width. ``coded`` keeps block and projection
-    inputs as 8-bit codes (``coded_checkpoints``, ``coded_inputs``).
+    every block a trained :class:`TextBranch` over states of that width. ``coded`` keeps block inputs as 8-bit
+    codes (``coded_checkpoints``), and the inputs of trained projections and adapters whose products are 16-bit
+    (``coded_inputs``).
     """
     if frozen not in ("int8", "fp8"):
         raise ValueError("frozen linears are held as int8 or fp8.")

@@ -15,7 +15,7 @@ and the input gradient is likewise one launch,
 
 with the two small rank-r products (``x A^T`` and ``dy B``) and the adapter weight
 gradients done as plain library GEMMs (``lora_A``'s by the native kernel from 8-bit codes, where the
-caller gives the input's codes to keep in its place). The reference adds the update after rounding the
+caller gives the input's codes to keep in its place; so too where the adapter runs beside another base). The reference adds the update after rounding the
 base output and the update separately (``result + update.to(result.dtype) * scale``); the
 fused form rounds once, which stays within the 5e-3 relative-Frobenius bar.
 
@@ -30,7 +30,7 @@ import torch
 from torch import nn
 from torch.nn import functional as F
 
-from .activation_codes import CodedActivation, coded_weight_gradient
+from .activation_codes import CodedActivation, coded_linear, coded_weight_gradient, codes_serve
 from .quant_kernels import autocast_compute_dtype, int8_linear_backward, int8_linear_forward, resolve_quantized_backend
 from .quantization import FrozenInt8Linear
 
@@ -119,23 +119,37 @@ class LoRALinear(nn.Module):
             compute_dtype = torch.get_autocast_dtype(tokens.device.type)
         return compute_dtype
 
-    def forward(self, tokens: torch.Tensor, coded: CodedActivation | None = None) -> torch.Tensor:
-        """``coded``: codes of the tokens, which the fused form then keeps in their place for ``lora_A``'s gradient."""
-        if coded is not None and (coded.shape != tokens.shape or coded.codes.device != tokens.device):
-            raise ValueError("The codes are not those of these tokens (another shape or device).")
-        if coded is not None and coded.dtype != tokens.dtype:
-            raise ValueError("The codes are those of tokens of another dtype.")
-        adapter_dtype = self._adapter_dtype(tokens)
+    def _fuses(self, tokens: torch.Tensor, adapter_dtype: torch.dtype | None) -> bool:
         base = self.base
-        if (
+        return (
             isinstance(base, FrozenInt8Linear)
             and base.fuses_lora
             and tokens.device.type == "cuda"
             and adapter_dtype in (torch.float16, torch.bfloat16)
             and autocast_compute_dtype(tokens, base.compute_dtype) == adapter_dtype
-        ):
-            if coded is not None and adapter_dtype == torch.float16 != coded.dtype:
-                coded = None  # float16 does not hold what they stand for: the tokens are kept
+        )
+
+    def keeps_codes(self, tokens: torch.Tensor) -> bool:
+        """Whether a call now would keep codes of the tokens in their place. It does for a trained ``lora_A`` whose product is
+        16-bit: of any tokens in the fused bfloat16 form, of tokens of the product's own dtype otherwise."""
+        dtype = self._adapter_dtype(tokens)
+        if not (tokens.is_cuda and torch.is_grad_enabled() and self.lora_A.requires_grad):
+            return False
+        if self._fuses(tokens, dtype) and dtype == torch.bfloat16:
+            return tokens.dtype in (torch.float16, torch.bfloat16, torch.float32)
+        return tokens.dtype == dtype and codes_serve(tokens, dtype)
+
+    def forward(self, tokens: torch.Tensor, coded: CodedActivation | None = None) -> torch.Tensor:
+        """``coded``: codes of the tokens, kept in their place for ``lora_A``'s gradient where :meth:`keeps_codes` says so."""
+        if coded is not None and (coded.shape != tokens.shape or coded.codes.device != tokens.device):
+            raise ValueError("The codes are not those of these tokens (another shape or device).")
+        if coded is not None and coded.dtype != tokens.dtype:
+            raise ValueError("The codes are those of tokens of another dtype.")
+        if coded is not None and not self.keeps_codes(tokens):
+            coded = None
+        adapter_dtype = self._adapter_dtype(tokens)
+        base = self.base
+        if self._fuses(tokens, adapter_dtype):
             return _FusedLoRAInt8Linear.apply(
                 tokens, self.lora_A, self.lora_B, base.weight_int8, base.weight_scale, base.bias,
                 base.compute_dtype, base.quantized_backend, float(self.scale), adapter_dtype,
@@ -149,5 +163,9 @@ class LoRALinear(nn.Module):
         else:
             adapter_input = tokens.to(adapter_dtype)
             adapter_a, adapter_b = self.lora_A.to(adapter_dtype), self.lora_B.to(adapter_dtype)
-        update = F.linear(F.linear(adapter_input, adapter_a), adapter_b)
+        if coded is None:
+            low = F.linear(adapter_input, adapter_a)
+        else:
+            low = coded_linear(adapter_input, adapter_a, coded=coded)
+        update = F.linear(low, adapter_b)
         return result + update.to(result.dtype) * self.scale

@@ -13,6 +13,7 @@ from torch.nn import functional as F
 from moss_image_b200 import _lib
 from moss_image_b200.activation_codes import coded_weight_gradient, decode_activation, encode_activation
 from moss_image_b200.dit import TextBranch, build_lora_model
+from moss_image_b200.fp8 import FrozenFp8Linear
 from moss_image_b200.lora import LoRALinear
 from moss_image_b200.memory import place_model
 from moss_image_b200.packed import cumulative_lengths
@@ -249,3 +250,68 @@ def test_coded_inputs_hold_less(cuda_device, packed):
             blocks.append(_held(lambda: block(tokens, cond, bounds[1])))
     copies = 2 if packed else 1  # q, k and v's input; and o's, where the attention's outputs are joined to one
     assert abs(blocks[0] - blocks[1] - copies * saved) < 0.02 * saved
+
+
+def _kept(layer, x, codes):
+    """What a call keeps of its tokens, by dtype, with its gradients."""
+    kept = []
+
+    def note(t):
+        if t.numel() == x.numel():
+            kept.append(t.dtype)
+        return t
+
+    with torch.autograd.graph.saved_tensors_hooks(note, lambda t: t):
+        y = layer(x, codes)
+    return set(kept), torch.autograd.grad(y.float().square().sum(), [x, layer.lora_A, layer.lora_B])
+
+
+@pytest.mark.parametrize("base", ["int8", "fp8", "dense"])
+def test_adapters_on_any_base_keep_codes_where_they_say_so(cuda_device, base):
+    torch.manual_seed(8)
+    linear = torch.nn.Linear(256, 192).to("cuda", BF16).requires_grad_(False)
+    linear = {"int8": FrozenInt8Linear, "fp8": FrozenFp8Linear, "dense": lambda x: x}[base](linear)
+    layer = LoRALinear(linear, 8, 16.0).to("cuda")
+    layer.lora_A.data, layer.lora_B.data = layer.lora_A.data.float(), torch.randn(192, 8, device="cuda") * 0.05
+    x = torch.randn(90, 256, device="cuda").to(BF16).requires_grad_()
+    coded = encode_activation(x)
+    with torch.autocast("cuda", BF16):
+        assert layer.keeps_codes(x)
+        kept, grads = _kept(layer, x, coded)
+        whole_kept, whole = _kept(layer, x, None)
+    assert kept == {torch.int8} and whole_kept == {BF16}
+    assert torch.equal(grads[0], whole[0]) and torch.equal(grads[2], whole[2])
+    # a decoded input is within 1/127 of its block's largest value, a quarter of that in the 2-norm; the gradient is linear in it
+    assert 0 < (grads[1] - whole[1]).norm() <= 0.02 * whole[1].norm()
+    # float32 products: the tokens are kept, and the codes not used
+    assert not layer.keeps_codes(x)
+    kept, grads = _kept(layer, x, coded)
+    assert torch.int8 not in kept and torch.equal(grads[1], _kept(layer, x, None)[1][1])
+    layer.lora_A.requires_grad_(False)
+    with torch.autocast("cuda", BF16), torch.no_grad():
+        assert not layer.keeps_codes(x)
+
+
+@pytest.mark.parametrize("frozen,autocast,expected", [("int8", True, 2), ("fp8", True, 2), ("int8", False, 0), ("fp8", False, 0)])
+def test_blocks_encode_only_what_a_projection_keeps(cuda_device, frozen, autocast, expected):
+    model = build_lora_model(1, device=cuda_device, dim=256, heads=4, mlp_dim=512, rank=8, seed=9, frozen=frozen).train()
+    block = model.layers[0]
+    block.coded_inputs = True
+    bounds = cumulative_lengths([30, 50], torch.device("cuda"))
+    tokens, cond = torch.randn(1, 80, 256, device="cuda").to(BF16), torch.randn(2, 256, device="cuda").to(BF16)
+    before = _lib.launch_counts.get("codes", 0)
+    with torch.autocast("cuda", BF16, enabled=autocast):
+        block(tokens, cond, bounds)
+    assert _lib.launch_counts.get("codes", 0) - before == expected  # q, k and v's input, and o's
+
+
+def test_a_branch_with_float32_masters_runs_without_codes(cuda_device):
+    branch = _branch(5).float()
+    tokens, context = (torch.randn(2, n, c, device="cuda").to(BF16).requires_grad_() for n, c in ((40, 128), (30, 96)))
+    results = []
+    for coded in (False, True):
+        branch.coded_inputs = coded
+        with torch.autocast("cuda", BF16):
+            y = branch(tokens, context)
+        results.append([y, *torch.autograd.grad(y.float().square().sum(), [tokens, *branch.parameters()])])
+    assert all(torch.equal(a, b) for a, b in zip(*results))
