@@ -326,7 +326,8 @@ MOSS_API int moss_cross_attention_bwd(const void* grad, const void* q, int64_t q
  *   gradient: dw[n, cols] = dy[rows, n]^T decode(codes), dy f16 or bf16, f32 sums in a fixed order, one rounding. Codes are
  *   decoded to dy's dtype: f16 gradients want codes of f16 values (what f16 does not hold is rounded, or infinite).
  * `workspace`: at least moss_coded_gradient_workspace_bytes(rows, n, cols) bytes, 256-byte aligned, free for reuse
- * once the stream has passed the call.
+ * once the stream has passed the call. The last rows * n * 2 of them (rounded up to 256) are for a copy of dy where n > 32:
+ * a dy of 16-byte aligned rows (n a multiple of 8) needs that much less.
  */
 MOSS_API int moss_codes_encode(const void* x, int dtype, int64_t rows, int64_t cols, int8_t* codes, int64_t ld,
                       uint8_t* exponents, moss_stream_t stream);

@@ -33,6 +33,7 @@ from .quant_kernels import _poll_after_backward, poll_device_status, status_buff
 
 CODE_BLOCK = 32
 _FLOATS = (torch.float16, torch.bfloat16, torch.float32)
+_FEW_FEATURES = 32  # gradients that the kernels read in place whatever their alignment is
 
 
 class CodedActivation(NamedTuple):
@@ -171,6 +172,8 @@ def coded_weight_gradient(gradient: torch.Tensor, codes: torch.Tensor, exponents
     gradient = gradient.detach().contiguous()
     out = torch.empty(features, columns, dtype=dtype, device=device)
     size = _workspace_bytes(device.index, rows, features, columns)
+    if size and features > _FEW_FEATURES and features % 8 == 0 and gradient.data_ptr() % 16 == 0:
+        size -= -(-rows * features * 2 // 256) * 256  # read in place: no room for a copy
     workspace = torch.empty(size, dtype=torch.uint8, device=device) if size else None
     _lib.check(_lib.library().moss_coded_gradient(
         gradient.data_ptr(), _lib.DTYPE_CODES[gradient.dtype], rows, features, codes.data_ptr(), _pitch(codes),

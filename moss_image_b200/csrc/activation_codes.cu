@@ -315,24 +315,24 @@ Plan make_plan(int64_t m, int64_t n, int64_t k, int sms) {
   return p;
 }
 
-// Workspace: decoded rows, copied gradient rows, partials; each 256-byte aligned.
+// Workspace: decoded rows, partials, copied gradient rows; each 256-byte aligned. The last are needed for gradients that TMA
+// cannot read in place alone, so their room comes last.
 struct Layout {
   int64_t x_ld, y_ld, part_rows, part_cols;
-  size_t y, partial, total;
+  size_t partial, y, total;
 };
 Layout layout_of(int64_t m, int64_t n, int64_t k, const Plan& p) {
   Layout l{};
   auto up = [](size_t v) { return (v + 255) / 256 * 256; };
   l.x_ld = ceil_div(k, 16) * 16;
   l.y_ld = ceil_div(n, 8) * 8;
-  l.y = p.few ? 0 : up(static_cast<size_t>(m) * l.x_ld * 2);
-  // (an unaligned gradient of any width is copied too: room for it is always there)
-  l.partial = l.y + (p.few ? 0 : up(static_cast<size_t>(m) * l.y_ld * 2));
+  l.partial = p.few ? 0 : up(static_cast<size_t>(m) * l.x_ld * 2);
   if (p.splits > 1) {
     l.part_rows = p.few ? n : static_cast<int64_t>(p.tiles_m) * (p.pair ? 256 : 128);
     l.part_cols = p.few ? static_cast<int64_t>(p.tiles_n) * kRowsColumns : static_cast<int64_t>(p.tiles_n) * (p.pair ? 256 : 128);
   }
-  l.total = l.partial + (p.splits > 1 ? up(static_cast<size_t>(p.splits) * l.part_rows * l.part_cols * 4) : 0);
+  l.y = l.partial + (p.splits > 1 ? up(static_cast<size_t>(p.splits) * l.part_rows * l.part_cols * 4) : 0);
+  l.total = l.y + (p.few ? 0 : up(static_cast<size_t>(m) * l.y_ld * 2));
   return l;
 }
 
@@ -360,8 +360,10 @@ int gradient(const void* dy, int dtype, int64_t m, int64_t n, const int8_t* code
   if (rc != MOSS_OK) return rc;
   const Plan plan = make_plan(m, n, k, device_sm_count());
   const Layout l = layout_of(m, n, k, plan);
-  if (l.total > 0 && (workspace == nullptr || workspace_bytes < l.total || !aligned(workspace, 256)))
-    return fail(MOSS_ERR_INVALID_ARGUMENT, "the coded gradient needs %zu bytes of 256-byte aligned workspace", l.total);
+  const bool in_place = n % 8 == 0 && aligned(dy, 16);
+  const size_t needed = in_place ? l.y : l.total;
+  if (needed > 0 && (workspace == nullptr || workspace_bytes < needed || !aligned(workspace, 256)))
+    return fail(MOSS_ERR_INVALID_ARGUMENT, "the coded gradient needs %zu bytes of 256-byte aligned workspace", needed);
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   Args a{};
   a.M = static_cast<int>(m);
@@ -390,7 +392,7 @@ int gradient(const void* dy, int dtype, int64_t m, int64_t n, const int8_t* code
     rc = launch_decode(codes, ld, exponents, m, k, ws, l.x_ld, dtype, stream);
     if (rc != MOSS_OK) return rc;
     const void* rows = dy;
-    if (n % 8 != 0 || !aligned(dy, 16)) {
+    if (!in_place) {
       copy_rows_kernel<<<static_cast<unsigned>(std::min<int64_t>(m, 8LL * device_sm_count())), kThreads, 0, stream>>>(
           static_cast<const uint16_t*>(dy), m, n, reinterpret_cast<uint16_t*>(ws + l.y), l.y_ld);
       MOSS_CUDA_TRY(cudaGetLastError());

@@ -363,3 +363,22 @@ def test_only_the_tokens_of_a_checkpoint_are_coded(cuda_device):
     near = decode_activation(encode_activation(x)).requires_grad_()
     expected = torch.autograd.grad(block(near, context), [near, context, weight], dy)
     assert all(torch.equal(a, b) for a, b in zip(got, expected))
+
+
+@pytest.mark.parametrize("features,copied", [(64, False), (24, False), (60, True)])
+def test_room_for_a_copy_of_the_gradient_only_where_one_is_made(cuda_device, features, copied):
+    rows, columns = 40000, 64
+    coded = encode_activation(_tokens(rows, columns, BF16, 1, 0.5))
+    dy = _tokens(rows, features, BF16, 2, 0.5)
+    coded_weight_gradient(dy, coded.codes, coded.exponents)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_stats()["requested_bytes.all.current"]
+    coded_weight_gradient(dy, coded.codes, coded.exponents)
+    used = torch.cuda.memory_stats()["requested_bytes.all.peak"] - before
+    decoded = rows * columns * 2 if features > 32 else 0
+    partials = 4 * 160 * 128 * 128  # one tile of sums for each multiprocessor, at most
+    padded = rows * 64 * 2 if copied else 0
+    assert decoded + padded <= used <= decoded + padded + partials
+    nothing = encode_activation(torch.empty(40, 0, device="cuda", dtype=BF16))
+    assert coded_weight_gradient(dy[:40], nothing.codes, nothing.exponents).shape == (features, 0)
