@@ -56,7 +56,10 @@ struct Barriers {
   uint64_t p_ready[2][2];      // P is there, O may be added to
   uint64_t pv_done[2];         // a product with P is done
   uint64_t o_full[2], o_free[2];
-  uint64_t out_full[2];        // the results are in shared memory
+  // the results are in shared memory, by pair and tile as q_full: a pair's next results come after its next queries, and those after
+  // its stores. (By tile alone, one softmax warpgroup finished two units while the stores waited for the other, and the
+  // barrier went on unseen.)
+  uint64_t out_full[4];
   uint64_t drain[2];
   uint32_t tile_bits[2 * kMaxTileBits / 32];
   uint32_t tmem_base;
@@ -119,6 +122,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int x = 0; x < 4; ++x) {
       mbar_init(bar(bars->q_full[x]), 1);
       mbar_init(bar(bars->q_empty[x]), 1);
+      mbar_init(bar(bars->out_full[x]), 4);
     }
     for (int x = 0; x < 2; ++x) {
       for (int b = 0; b < 2; ++b) {
@@ -128,7 +132,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(bar(bars->pv_done[x]), 1);
       mbar_init(bar(bars->o_full[x]), 1);
       mbar_init(bar(bars->o_free[x]), 4);
-      mbar_init(bar(bars->out_full[x]), 4);
     }
     for (int s = 0; s < kStages; ++s) {
       mbar_init(bar(bars->k_full[s]), 1);
@@ -326,7 +329,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     } else {
       // ---------------------------------------------------------------- masked rows of V, and the stores (which a softmax warp
       // would wait 1500 cycles a tile for)
-      uint32_t pos = 0, units = 0, uses[2] = {0, 0};
+      uint32_t pos = 0, units = 0, uses[4] = {0, 0, 0, 0};
       bool ok = true;
       for (int u = blockIdx.x; u < num_units && ok; u += gridDim.x) {
         Unit w;
@@ -343,7 +346,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         for (int x = 0; x < w.tiles() && ok; ++x) {
           const uint32_t slot = (units & 1u) * 2 + x;
-          ok = wait_suspended(bar(bars->out_full[x]), uses[x]++ & 1u, abort_flag, args.status, MOSS_STATUS_TIMEOUT_EPILOGUE);
+          ok = wait_suspended(bar(bars->out_full[slot]), uses[slot]++ & 1u, abort_flag, args.status, MOSS_STATUS_TIMEOUT_EPILOGUE);
           if (!ok) break;
           if (lane == 0) {
             if (leaves_by_tma<kMask>(args, w, x)) {
@@ -519,7 +522,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (any_keys) {
         if (by_tma) fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive(bar(bars->out_full[x]));
+        if (lane == 0) mbar_arrive(bar(bars->out_full[slot]));
       }
       if (live) {
         const float l = sum == 0.0f ? -INFINITY : top - kLift<kKind> + log2f(sum);

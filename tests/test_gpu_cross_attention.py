@@ -489,3 +489,21 @@ def test_one_key_in_masks_of_many_tiles(cuda_device, batch, tk):
     assert torch.equal(o, v[mask][:, None].expand_as(o)) and not dq.any() and not dk.any()
     mask[-1, (int(at[-1]) + 150) % tk] = True  # a second key for one of them
     _check(q, k, v, grad, mask=mask)
+
+
+@pytest.mark.parametrize("dim,dtype", [(64, BF16), (128, F16)])
+@pytest.mark.parametrize("tk", [5, 100, 130])
+def test_many_units_of_few_keys(cuda_device, tk, dim, dtype):
+    """A multiprocessor's units follow one another within a microsecond or two, thousands of them in a row."""
+    q, k, v, grad = _tensors(1, 20000, tk, 48, 48, dim, dtype, 16)
+    rows = torch.randint(0, 20000, (40,), device="cuda")
+    mask = torch.rand(1, tk, device="cuda") < 0.5
+    for options in ({}, {"key_mask": mask}):
+        first = _run(q, k, v, grad, **options)
+        for _ in range(12):
+            with torch.no_grad():
+                assert torch.equal(cross_attention(q, k, v, **options), first[0])
+        check_device_status(q.device)
+        allowed = None if not options else mask[:, None, None]
+        _assert_near(("o", "dq"), [t[:, rows] for t in first[:2]],
+                     _exact(q[:, rows], k, v, allowed, dim ** -0.5, grad[:, rows])[:2])
