@@ -380,6 +380,12 @@ struct TileBits {
   }
 };
 
+// Whether all keys that the sequence's queries look at are in one tile.
+__device__ __forceinline__ bool one_tile(const TileBits& taken, const Sequence& s) {
+  const int tiles = (s.kn + kTile - 1) / kTile, first = taken.next(s.entry, 0, tiles);
+  return first < tiles && taken.next(s.entry, first + 1, tiles) == tiles;
+}
+
 // Whether the sequence's queries look at one key alone. P is then 1 whatever the logit is, and the gradient of the logit nothing
 // times dP - delta, whose rounding would be left otherwise. By a whole warp; it ends at the second key it finds.
 __device__ __forceinline__ bool only_key(const Args& a, const TileBits& taken, const Sequence& s) {

@@ -6,7 +6,9 @@
 //        S^T = K Q^T, dP^T = V dO^T, then dV += P^T dO and dK += dS^T Q
 // Seven products for a tile pair where five would do with dQ added up across CTAs: a dQ value would be written and read in
 // f32 for every key tile, 900 MB for 2 x 24 heads of 128, 4096 x 512 tokens, 140 us against 40 for the two products more.
-// The dq kernel also takes delta = rowsum(O dO) on the way, which the other reads.
+// The dq kernel also takes delta = rowsum(O dO) on the way, which the other reads. Where all of a sequence's keys are in one tile, it
+// is rowsum(P dP) instead, in f32: O's rounding is half of what dP - delta is off by there (8 keys: dQ 0.0031 off in the 2-norm,
+// bf16, and 0.0024 so), and less with more keys.
 //
 // In both, P and dS are written over S and dP in TMEM as 16-bit pairs and feed the next product from there; a thread has a
 // row and half of the columns (two warpgroups). P and dS are rounded to the inputs' type, half a step of each term (f16: times
@@ -427,17 +429,22 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
       }
-      float* const meet = cta.stats + (nth & 1u) * 2 * kTile;
-      meet[half * kTile + row] = delta;
-      uint8_t* const sizes = cta.sizes + (nth & 1u) * 2 * kTile;
-      if constexpr (kKind == kF16) sizes[half * kTile + row] = static_cast<uint8_t>(exponent_of(fabsf(square)));
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&bars->stat_full[nth & 1u]));
-      ok = cta.wait(bars->stat_full[nth & 1u], nth >> 1, MOSS_STATUS_TIMEOUT_EPILOGUE);
+      // the sum of both warpgroups' halves of a row's value
+      auto meet = [&](float value) {
+        float* const slot = cta.stats + (nth & 1u) * 2 * kTile;
+        slot[half * kTile + row] = value;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&bars->stat_full[nth & 1u]));
+        ok = cta.wait(bars->stat_full[nth & 1u], nth >> 1, MOSS_STATUS_TIMEOUT_EPILOGUE);
+        ++nth;
+        return slot[row] + slot[kTile + row];
+      };
+      const uint8_t* const sizes = cta.sizes + (nth & 1u) * 2 * kTile;
+      if constexpr (kKind == kF16) cta.sizes[(nth & 1u) * 2 * kTile + half * kTile + row] = static_cast<uint8_t>(exponent_of(fabsf(square)));
+      delta = meet(delta);
       if (!ok) break;
-      ++nth;
-      delta = meet[row] + meet[kTile + row];
-      if (live && half == 0 && w.split == 0) args.delta[w.head * args.q_rows + q_row] = delta;
+      const bool single = one_tile(taken, w.s);
+      if (live && half == 0 && w.split == 0 && !single) args.delta[w.head * args.q_rows + q_row] = delta;
       int lift = 0;
       if constexpr (kKind == kF16) {
         const int size = max(sizes[row], sizes[kTile + row]), at_sizes = w.s.index * args.k_heads + w.head / args.group;
@@ -456,13 +463,40 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!ok) break;
         tc_fence_after();
         const uint32_t s_tmem = tmem + (i & 1) * kTile + half * kHalf + lanes;
+        const uint64_t scale2 = pair_of(args.scale_log2, args.scale_log2), minus_lse = pair_of(-lse, -lse), raise2 = pair_of(raised, raised);
+        if (single) {  // all of the row's keys are here: delta = sum P dP in f32
+          uint64_t sum2 = 0;
+#pragma unroll 1
+          for (int c = 0; c < 2; ++c) {
+            const int count = keys - 32 * c;
+            const uint32_t k = kMask ? (half == 0 ? (c == 0 ? keep.w[0] : keep.w[1]) : c == 0 ? keep.w[2] : keep.w[3])
+                                     : count >= 32 ? 0xffffffffu : count <= 0 ? 0u : (1u << count) - 1u;
+            uint32_t x[32], y[32];
+            tmem_ld_32x32b_x32(s_tmem + 32 * c, x);
+            tmem_ld_32x32b_x32(dp_tmem + half * kHalf + lanes + 32 * c, y);
+            wait_ld_of(x);
+            wait_ld_of(y);
+#pragma unroll
+            for (int j = 0; j < 32; j += 2) {
+              float p0, p1;
+              split_pair(exponentials(j / 2, pair_of(__uint_as_float(x[j]), __uint_as_float(x[j + 1])), scale2, minus_lse), p0, p1);
+              const bool in0 = ((k >> j) & 1u) != 0, in1 = ((k >> j) & 2u) != 0;
+              sum2 = fma_pair(pair_of(in0 ? p0 : 0.0f, in1 ? p1 : 0.0f),
+                              pair_of(in0 ? __uint_as_float(y[j]) : 0.0f, in1 ? __uint_as_float(y[j + 1]) : 0.0f), sum2);
+            }
+          }
+          float sum0, sum1;
+          split_pair(sum2, sum0, sum1);
+          delta = meet(sum0 + sum1);
+          if (!ok) break;
+          if (live && half == 0) args.delta[w.head * args.q_rows + q_row] = delta;
+        }
         uint32_t s[2][32], g[2][32];
         load64(s_tmem, s);
         load64(dp_tmem + half * kHalf + lanes, g);
         float v[64];
         // (a row without keys has lse = inf, which makes its exponentials zero)
-        const uint64_t scale2 = pair_of(args.scale_log2, args.scale_log2), minus_lse = pair_of(-lse, -lse), raise2 = pair_of(raised, raised),
-                       minus_delta = pair_of(-delta * raised, -delta * raised);
+        const uint64_t minus_delta = pair_of(-delta * raised, -delta * raised);
 #pragma unroll
         for (int j = 0; j < 64; j += 2) {
           const uint64_t p = exponentials(j / 2, pair_of(__uint_as_float(s[j >> 5][j & 31]), __uint_as_float(s[j >> 5][(j & 31) + 1])),

@@ -507,3 +507,27 @@ def test_many_units_of_few_keys(cuda_device, tk, dim, dtype):
         allowed = None if not options else mask[:, None, None]
         _assert_near(("o", "dq"), [t[:, rows] for t in first[:2]],
                      _exact(q[:, rows], k, v, allowed, dim ** -0.5, grad[:, rows])[:2])
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("layout", ["dense", "masked", "packed"])
+@pytest.mark.parametrize("keys", [2, 4, 9, 30, 128])
+def test_gradients_of_short_captions_have_two_roundings(cuda_device, keys, layout, dtype):
+    """A value's rounding is off by h / sqrt(3) / m in the mean, m in [1, 2) its mantissa: 0.425 h over values of all sizes. dQ and dK
+    have that of dS and their own, 0.6 h, and a tenth of that for the sample; not that of O, which delta could be taken from."""
+    batch, tq, heads, dim = 3, 500, 4, 64
+    q, k, v, grad = _tensors(batch, tq, 140 if layout == "masked" else keys, heads, heads, dim, dtype, 18)
+    allowed = None
+    if layout == "packed":
+        offsets = [cumulative_lengths([n] * batch, q.device) for n in (tq, keys)]
+        got = [t.unflatten(0, (batch, -1)) for t in _run_packed(*(t.flatten(0, 1) for t in (q, k, v, grad)), *offsets)]
+    elif layout == "masked":
+        mask = torch.zeros(batch, 140, dtype=torch.bool, device="cuda")
+        mask[:, : 2 * keys : 2] = True
+        mask[:, 128:] = False
+        allowed = mask[:, None, None]
+        got = _run(q, k, v, grad, key_mask=mask)
+    else:
+        got = _run(q, k, v, grad)
+    for name, value, (exact, _) in zip(("dq", "dk"), got[1:], _exact(q, k, v, allowed, dim ** -0.5, grad)[1:]):
+        assert (value.double() - exact).norm() <= 0.66 * HALF_STEP[dtype] * exact.norm(), name
