@@ -387,9 +387,11 @@ __device__ __forceinline__ bool one_tile(const TileBits& taken, const Sequence& 
 }
 
 // Whether the sequence's queries look at one key alone. P is then 1 whatever the logit is, and the gradient of the logit nothing
-// times dP - delta, whose rounding would be left otherwise. By a whole warp; it ends at the second key it finds.
-__device__ __forceinline__ bool only_key(const Args& a, const TileBits& taken, const Sequence& s) {
+// times dP - delta, whose rounding would be left otherwise. By a whole warp; the mask is read again only where its tiles do not
+// tell, up to the second key.
+__device__ __forceinline__ bool only_key(const Args& a, const TileBits& taken, const Sequence& s, bool in_one_tile) {
   if (s.kn == 1 || a.mask == nullptr) return s.kn == 1;
+  if (taken.bits != nullptr && !in_one_tile) return false;
   const int tiles = (s.kn + kTile - 1) / kTile;
   int seen = 0;
   for (int t = taken.next(s.entry, 0, tiles); t < tiles && seen < 2; t = taken.next(s.entry, t + 1, tiles)) {

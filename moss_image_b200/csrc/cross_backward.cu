@@ -452,7 +452,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int most = __reduce_max_sync(0xffffffffu, size);
         if (half == 0 && w.split == 0 && lane == 0) raise_to(args.sizes + (args.batch + 1) * args.k_heads + at_sizes, most);
       }
-      const bool alone = w.first < w.end && only_key(args, taken, w.s);
+      const bool alone = w.first < w.end && only_key(args, taken, w.s, single);
       const float raised = kKind == kF16 ? pow2(lift) : 1.0f;
       int i = 0;
       for (int t = w.first; t < w.end; t = taken.next(w.s.entry, t + 1, w.end), ++i) {
@@ -752,7 +752,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int key = w.row + row;
       bool seen = key < w.s.kn;
       if (seen && args.mask != nullptr) seen = __ldg(args.mask + w.s.entry * args.mask_ld + key) != 0;
-      const bool alone = w.first < w.end && only_key(args, taken, w.s);
+      const bool alone = w.first < w.end && only_key(args, taken, w.s, one_tile(taken, w.s));
       int lift = 0;
       if constexpr (kKind == kF16) {
         const int* const sizes = args.sizes + w.s.index * args.k_heads + w.head;
