@@ -10,9 +10,11 @@ written, and the backward pass recomputes the probabilities from the row sums th
 * :func:`cross_attention_packed`: packed rows of several sequences (:mod:`moss_image_b200.packed`) with
   boundaries for the queries and for the keys, each sequence looking at its own keys.
 
-A query without keys (an empty caption, a mask that leaves nothing) gives zeros, and no gradient. What lies in
-masked places is never read into a result, infinities and NaN included. Gradients of shared key heads and all
-other sums are float32 in a fixed order (no atomics), rounded once.
+A query without keys (an empty caption, a mask that leaves nothing, logits of minus infinity) gives zeros, and no
+gradient. What lies in masked places is never read into a result, infinities and NaN included; NaN in a place that
+is looked at reaches all that depends on it. Gradients of shared key heads and all other sums are float32 in a fixed
+order, rounded once. Probabilities and the logits' gradients are rounded to the inputs' type before their products
+(float16: times a power of two that keeps them normal); logits are float32, whose own steps show past 2^20.
 
 CUDA tensors only: there is no CPU path.
 """

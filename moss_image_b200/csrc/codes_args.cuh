@@ -35,7 +35,10 @@ struct Args {
   StatusSink status;
 };
 
-constexpr int kFewFeatures = 32;   // features that codes_rows.cu takes
+// Features that codes_rows.cu takes: two operand tiles of 16, what its sums have registers for. 9216 x 3072, this kernel against the
+// GEMM behind a decode, us: 18 and 33 for 8 features, 18 and 29 for 16, 20 and 29 for 32; from there the GEMM alone, 33 for 40,
+// 30 for 48, 27 for 64.
+constexpr int kFewFeatures = 32;
 constexpr int kRowsColumns = 128;  // columns of X that one of its CTAs takes
 constexpr int kRowsMost = 2048;    // rows of one split (its dY rows stay in shared memory)
 constexpr int kStep = 128;         // reduction rows per stage of the GEMM

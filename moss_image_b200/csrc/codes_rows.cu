@@ -6,8 +6,9 @@
 // each of four rows (the next two sixteens are on their way meanwhile), pairs them by rows, scales the pairs exactly
 // and feeds them to warp-level MMAs as they lie, column j of every lane forming one 8-column operand, against dY
 // read transposed from shared memory. The tensor work is small; the MMAs spare the CUDA cores the multiply-adds. The warps'
-// sums are added in warp order, the splits' in split order. 9216 x 3072 -> 32: 20 us (the codes' way through HBM 4.4): what
-// is left is instructions, 310 for 1024 codes of a warp, and the run's start and end.
+// sums are added in warp order, the splits' in split order. 9216 x 3072 -> 32: 19 us (the codes' way through HBM 4.4): 8 of
+// them to issue 310 instructions for 1024 codes of a warp; the rest are two loads ahead of 16 warps, which do not cover their
+// latency, and the eight rounds of sums at the end.
 #include <algorithm>
 
 #include "codes_args.cuh"

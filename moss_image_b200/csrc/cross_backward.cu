@@ -19,8 +19,8 @@
 
 #include "cross_args.cuh"
 
-// Bound by latency: 2 x 24 heads of 128, 4096 x (308 and 512) tokens, bf16: dq 148 us, of which the start and end of its units take
-// 40% (3.5 key tiles a unit), dkv 110 us (4,700 cycles a tile pair for 2,048 of products); all products of both 61 us
+// Bound by latency: 2 x 24 heads of 128, 4096 x (308 and 512) tokens, bf16: dq 155 us, of which the start and end of its units take
+// 40% (3.5 key tiles a unit), dkv 119 us (5,000 cycles a tile pair for 2,048 of products); all products of both 61 us
 // at the GPU's rate.
 namespace moss {
 namespace cross {

@@ -4,9 +4,11 @@
 //   dx = rstd * (dn - sum(dn) / dim - n * sum(dn * n) / dim)  with dn = dy * w
 //   dw = sum over rows of dy * n,   db = sum over rows of dy
 // Everything between a load and a store is f32; the variance is summed from the centred values, so a mean
-// far from zero costs no digits.
+// far from zero costs it no digits (the mean has its own rounding, which is a part of the centred values).
 //
-// Bound by HBM: x and y (forward), x, dy and dx (backward) cross it once, because a row stays in the registers of
+// Bound by HBM where no gain is read (32768 x 3072 f32: 144 us, 0.85 of the copy rate), with one by shared memory as well, which
+// it is read from as f32 (9216 x 3072 bf16: 32 us forward, 48 backward, 7 for the join). x and y (forward), x, dy and dx
+// (backward) cross HBM once, because a row stays in the registers of
 // its team of 8, 32, 128 or 512 threads from the load to the store. A thread owns the same columns in every row, so
 // the gain and the offset are read once for each thread, and the weight gradients are summed in registers
 // over all of a team's rows, then over the CTA's teams through shared memory; one row of f32 partials for

@@ -22,7 +22,8 @@ may be held in block-scaled fp8 instead of int8.
 A block may have a trained :class:`TextBranch`, in which its tokens look at a text encoder's states
 (:mod:`moss_image_b200.cross_attention`), and what training keeps of activations may be 8-bit codes
 (:mod:`moss_image_b200.activation_codes`): the inputs of checkpointed blocks (``coded_checkpoints`` of the
-stack) and of the trained projections (``coded_inputs`` of the blocks).
+stack), swapped and streamed ones among them, and of the trained projections with 16-bit products (``coded_inputs`` of the
+blocks), where nothing else keeps them anyway.
 """
 
 from __future__ import annotations
