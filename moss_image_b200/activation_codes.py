@@ -135,6 +135,16 @@ def _workspace_bytes(device: int, rows: int, features: int, columns: int) -> int
     return size.value
 
 
+class _WithoutGradient(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, gradient, codes, exponents, output_dtype, coded_dtype):
+        return coded_weight_gradient(gradient, codes, exponents, output_dtype, coded_dtype=coded_dtype)
+
+    @staticmethod
+    def backward(ctx, gradient):
+        raise NotImplementedError("coded_weight_gradient has no gradient (no second derivatives).")
+
+
 def coded_weight_gradient(gradient: torch.Tensor, codes: torch.Tensor, exponents: torch.Tensor,
                           output_dtype: torch.dtype | None = None, *,
                           coded_dtype: torch.dtype | None = None) -> torch.Tensor:
@@ -143,7 +153,8 @@ def coded_weight_gradient(gradient: torch.Tensor, codes: torch.Tensor, exponents
     (the gradient's own by default).
 
     ``coded_dtype``: what the codes were made from, the gradient's dtype where it is not given. The product reads decoded
-    values in the gradient's dtype: bfloat16 holds those of any codes, float16 those of float16 tokens only.
+    values in the gradient's dtype: bfloat16 holds those of any codes, float16 those of float16 tokens only. Not
+    differentiable: a backward pass that reaches a result whose gradient input requires grad raises.
     """
     what = "coded_weight_gradient"
     if not gradient.is_cuda:
@@ -158,6 +169,8 @@ def coded_weight_gradient(gradient: torch.Tensor, codes: torch.Tensor, exponents
     if not _holds(gradient.dtype, gradient.dtype if coded_dtype is None else coded_dtype):
         raise ValueError(f"{what}: float16 does not hold what codes of {coded_dtype} tokens stand for.")
     _lib.refuse_forward_mode(what, gradient)
+    if torch.is_grad_enabled() and gradient.requires_grad:
+        return _WithoutGradient.apply(gradient, codes, exponents, output_dtype, coded_dtype)
     device = gradient.device
     if device.index != _lib.current_device_index():
         with torch.cuda.device(device):

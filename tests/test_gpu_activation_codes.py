@@ -382,3 +382,22 @@ def test_room_for_a_copy_of_the_gradient_only_where_one_is_made(cuda_device, fea
     assert decoded + padded <= used <= decoded + padded + partials
     nothing = encode_activation(torch.empty(40, 0, device="cuda", dtype=BF16))
     assert coded_weight_gradient(dy[:40], nothing.codes, nothing.exponents).shape == (features, 0)
+
+
+def test_second_derivatives_are_refused(cuda_device):
+    coded = encode_activation(torch.randn(40, 64, device="cuda", dtype=BF16))
+    dy = torch.randn(40, 48, device="cuda", dtype=BF16, requires_grad=True)
+    got = coded_weight_gradient(dy * 1.0, coded.codes, coded.exponents, F32)
+    assert torch.equal(got, coded_weight_gradient(dy.detach(), coded.codes, coded.exponents, F32))
+    with pytest.raises(NotImplementedError, match="no gradient"):
+        got.sum().backward()
+    # an adapter on codes, whose own backward pass records its steps
+    base = torch.nn.Linear(64, 32).to("cuda", BF16).requires_grad_(False)
+    layer = LoRALinear(FrozenInt8Linear(base), 4, 8.0).to("cuda")
+    torch.nn.init.normal_(layer.lora_B, std=0.05)
+    x = torch.randn(8, 64, device="cuda", dtype=BF16)
+    with torch.autocast("cuda", BF16):
+        y = layer(x, encode_activation(x))
+    slope, = torch.autograd.grad(y.float().square().sum(), layer.lora_A, create_graph=True)
+    with pytest.raises(NotImplementedError, match="no gradient"):
+        torch.autograd.grad(slope.square().sum(), layer.lora_B)
