@@ -215,7 +215,8 @@ class _CodedLinear(torch.autograd.Function):
             _poll_after_backward(gradient.device)
             d_weight = coded_weight_gradient(gradient, codes, exponents, weight.dtype)
         if ctx.needs_input_grad[2]:
-            d_bias = gradient.reshape(-1, gradient.shape[-1]).sum(0, dtype=torch.float32).to(ctx.bias_dtype)
+            rows = math.prod(gradient.shape[:-1])  # (a row of no features tells no number of rows)
+            d_bias = gradient.reshape(rows, gradient.shape[-1]).sum(0, dtype=torch.float32).to(ctx.bias_dtype)
         return d_tokens, d_weight, d_bias, None, None
 
 

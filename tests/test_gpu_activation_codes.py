@@ -401,3 +401,14 @@ def test_second_derivatives_are_refused(cuda_device):
     slope, = torch.autograd.grad(y.float().square().sum(), layer.lora_A, create_graph=True)
     with pytest.raises(NotImplementedError, match="no gradient"):
         torch.autograd.grad(slope.square().sum(), layer.lora_B)
+
+
+@pytest.mark.parametrize("rows,features,columns", [((2, 5), 0, 32), ((0,), 24, 32), ((3,), 24, 0), ((), 24, 32)])
+def test_coded_linear_of_nothing(cuda_device, rows, features, columns):
+    x = torch.randn(*rows, columns, device="cuda").to(BF16).requires_grad_()
+    weight, bias = (torch.randn(*shape, device="cuda").to(BF16).requires_grad_() for shape in ((features, columns), (features,)))
+    y, plain = coded_linear(x, weight, bias), torch.nn.functional.linear(x, weight, bias)
+    dy = torch.randn_like(plain)
+    got, whole = (torch.autograd.grad(t, [x, weight, bias], dy) for t in (y, plain))
+    assert torch.equal(y, plain) and all(a.shape == b.shape for a, b in zip(got, whole))
+    assert torch.equal(got[0], whole[0]) and torch.equal(got[2], whole[2])
